@@ -183,13 +183,17 @@ Call begin_call() {
     call.wait = g_thread.wait;
 
     g_thread.kernels.clear();
+    // The id of a stream cannot be asked for while it is captured into a graph; that of the capture stands for it then, so
+    // each graph has status words of its own.
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(call.stream, &capture) != cudaSuccess) (void)cudaGetLastError();
-    call.capturing = capture != cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
-    MOPS_CUDA_OK(cudaStreamGetId(call.stream, &id));
+    if (cudaStreamGetCaptureInfo(call.stream, &capture, &id) != cudaSuccess) (void)cudaGetLastError();
+    call.capturing = capture != cudaStreamCaptureStatusNone;
+    if (call.capturing) id |= 1ull << 63;
+    else MOPS_CUDA_OK(cudaStreamGetId(call.stream, &id));
     const auto key = std::make_pair(call.device, id);
     if (g_thread.last == nullptr || key != g_thread.last_key) {
+        const RelaxedCapture relaxed; // (a first call allocates)
         g_thread.last = &state_of(key, call.capturing);
         g_thread.last_key = key;
     }
