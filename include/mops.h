@@ -228,6 +228,66 @@ MOPS_EXPORT int mops_b200_cuda_sort_index(mops_tensor_1d_i32_t sorted,
                                           mops_tensor_1d_i32_t permutation,
                                           mops_tensor_1d_i32_t indices, int64_t n_rows);
 
+/* ---- Block operators (no counterpart in the reference): what stands before and behind the sparse
+ * operations in a model. The rows of a table for every atom or token, a matrix for each group of rows
+ * (species, experts), and the residual connection with its gate and norms.
+ *
+ * Arrays are views with a type and strides (counted in values), of f32, f64, f16 or bf16; all
+ * floating-point arrays of a call have one type. Inputs may have rows that lie apart (any stride but
+ * the last, which is 1); outputs are contiguous. Sums are held in 32 bits (f64: 64) and rounded
+ * once. A gradient output with data == NULL is skipped. Same status convention, stream and completion rules as the
+ * mops_cuda_* entry points. */
+enum {
+    MOPS_B200_F32 = 0,
+    MOPS_B200_F64 = 1,
+    MOPS_B200_F16 = 2,
+    MOPS_B200_BF16 = 3,
+    MOPS_B200_I32 = 4
+};
+typedef struct mops_b200_array_t {
+    void* data;
+    int32_t type;       /* MOPS_B200_* */
+    int32_t dimensions; /* 1 to 3 */
+    int64_t shape[3];
+    int64_t stride[3];
+} mops_b200_array_t;
+
+/* output[t,:] = scale * W[indices[t],:]. An index outside of W gives a row of zeros, and an error. */
+MOPS_EXPORT int mops_b200_cuda_embedding_lookup(mops_b200_array_t output, mops_b200_array_t W,
+                                                mops_b200_array_t indices, double scale);
+/* grad_W[v,:] = scale * sum of grad_output[t,:] over the t with indices[t] == v, taken in the order of t in pieces
+ * that depend on the sizes alone (the same call gives the same bits); zeros for rows without any, and for
+ * row padding_index (-1: none). */
+MOPS_EXPORT int mops_b200_cuda_embedding_lookup_vjp(mops_b200_array_t grad_W, mops_b200_array_t grad_output,
+                                                    mops_b200_array_t indices, double scale, int64_t padding_index);
+
+/* output[r,:] = A[r,:] W[g,:,:] for the rows offsets[g] <= r < offsets[g+1] of group g; zeros for rows
+ * of no group. offsets: int32, one more than groups, ascending, in device memory. The last two
+ * dimensions of W may be stored either way round. */
+MOPS_EXPORT int mops_b200_cuda_grouped_matrix_product(mops_b200_array_t output, mops_b200_array_t A,
+                                                      mops_b200_array_t W, mops_b200_array_t offsets);
+/* grad_A[r,:] = grad_output[r,:] W[g]^T, grad_W[g] = A[rows of g]^T grad_output[rows of g] (zeros for
+ * a group without rows). The last two dimensions of grad_W may be stored either way round. */
+MOPS_EXPORT int mops_b200_cuda_grouped_matrix_product_vjp(mops_b200_array_t grad_A, mops_b200_array_t grad_W,
+                                                          mops_b200_array_t grad_output, mops_b200_array_t A,
+                                                          mops_b200_array_t W, mops_b200_array_t offsets);
+
+/* stream = residual + scale * weight_branch * sigmoid(gate) * branch / rms(branch),
+ * normed = weight_output * stream / rms(stream), where rms(v) = sqrt(mean(v^2) + epsilon) over a row.
+ * gate: as the residual, or one column (a gate for each row), or an array of 0 dimensions (no gate). normed is
+ * computed from the stream before it is rounded. */
+MOPS_EXPORT int mops_b200_cuda_gated_residual_norm(mops_b200_array_t stream, mops_b200_array_t normed,
+                                                   mops_b200_array_t residual, mops_b200_array_t branch,
+                                                   mops_b200_array_t gate, mops_b200_array_t scale,
+                                                   mops_b200_array_t weight_branch,
+                                                   mops_b200_array_t weight_output, double epsilon);
+MOPS_EXPORT int mops_b200_cuda_gated_residual_norm_vjp(
+    mops_b200_array_t grad_residual, mops_b200_array_t grad_branch, mops_b200_array_t grad_gate,
+    mops_b200_array_t grad_scale, mops_b200_array_t grad_weight_branch, mops_b200_array_t grad_weight_output,
+    mops_b200_array_t grad_stream, mops_b200_array_t grad_normed, mops_b200_array_t residual,
+    mops_b200_array_t branch, mops_b200_array_t gate, mops_b200_array_t scale, mops_b200_array_t weight_branch,
+    mops_b200_array_t weight_output, double epsilon);
+
 /* Names (with template arguments) of the main kernels the calling thread's last mops_cuda_*
  * call dispatched to, "; "-separated; valid until that thread's next call. For tools that
  * pair a timing with the profile of the same kernel instantiation. */

@@ -17,6 +17,11 @@ Accepted arrays
     in, kernels and copies out are queued on three CUDA streams and overlap across calls;
     results are valid when the block ends.
 
+Beside the five operations stand the operators of the block around them, with gradients:
+``embedding_lookup`` (a row of a table for every atom or token), ``grouped_matrix_product`` (a matrix for
+each group of rows) and ``gated_residual_norm`` (the residual connection with its gate and norms). They
+also take float16 and bfloat16.
+
 Differences from the reference front end: no CuPy dispatch (CuPy is replaced by torch CUDA
 tensors); OPSAW and SASAW run on the GPU instead of raising "CUDA implementation does not
 exist yet".
@@ -30,7 +35,9 @@ from . import _lib
 from ._lib import MopsError  # noqa: F401
 
 __all__ = [f"{op}{lvl}" for op in _lib.OPERATIONS for lvl in _lib.LEVELS] + [
-    "MopsError", "HostQueue", "Plan", "sort_indices"]
+    "MopsError", "HostQueue", "Plan", "sort_indices"] + [
+    f"{op}{lvl}" for op in ("embedding_lookup", "grouped_matrix_product", "gated_residual_norm")
+    for lvl in ("", "_vjp")]
 
 
 def _torch():
@@ -259,7 +266,8 @@ class HostQueue:
 class _Arena:
     """Moves one call's arrays to the device and its results back to where the inputs live."""
 
-    def __init__(self, first):
+    def __init__(self, first, half=False):
+        """``half``: whether the operation takes float16 and bfloat16."""
         torch = _torch()
         if not torch.cuda.is_available():
             raise MopsError("no CUDA device available: this build of mops runs on the GPU only "
@@ -278,14 +286,12 @@ class _Arena:
         else:
             self.device = first.device
             self.host = False
-        if isinstance(first, np.ndarray):
-            self.dtype = {np.dtype("float32"): torch.float32,
-                          np.dtype("float64"): torch.float64}.get(first.dtype)
-        else:
-            self.dtype = first.dtype if first.dtype in (torch.float32, torch.float64) else None
+        taken = (torch.float32, torch.float64) + ((torch.float16, torch.bfloat16) if half else ())
+        self.dtype = {_dtype_name(torch.empty(0, dtype=t)): t for t in taken}.get(_dtype_name(first))
         if self.dtype is None:
-            raise TypeError("Unsupported dtype detected. Only float32 and float64 are supported")
-        self.suffix = "f32" if self.dtype == torch.float32 else "f64"
+            raise TypeError("Unsupported dtype detected. Only float32" + (
+                ", float64, float16 and bfloat16" if half else " and float64") + " are supported")
+        self.suffix = "f64" if self.dtype == torch.float64 else "f32"
 
     def floats(self, x):
         t = self.torch.from_numpy(np.ascontiguousarray(x)) if isinstance(x, np.ndarray) else x
@@ -296,6 +302,14 @@ class _Arena:
             self.ready.append(ready)
             return dev
         return t.to(self.device, non_blocking=True).contiguous()
+
+    def rows(self, x):
+        """As ``floats``, but a CUDA tensor whose rows lie apart stays where it is."""
+        t = x if not isinstance(x, np.ndarray) else None
+        if t is not None and t.is_cuda and t.device == self.device and t.dtype == self.dtype and \
+                t.stride(-1) == 1 and not t.is_neg():
+            return t
+        return self.floats(x)
 
     def ints(self, x):
         t = self.torch.from_numpy(np.ascontiguousarray(x)) if isinstance(x, np.ndarray) else x
@@ -338,13 +352,22 @@ class _Arena:
 
     def run(self, name, tensors):
         """tensors: list of torch tensors, or ``(None, ndim)`` for a skipped gradient."""
-        torch = self.torch
         structs = []
         for t in tensors:
             if isinstance(t, tuple):
                 structs.append(_lib.null_struct(t[1]))
             else:
                 structs.append(_lib.make_struct(t.data_ptr(), t.shape))
+        self._call(f"mops_cuda_{name}_{self.suffix}", structs)
+
+    def run_arrays(self, name, *args):
+        """A block operator; args: torch tensors, None for what is skipped, and C scalars."""
+        self._call(f"mops_b200_cuda_{name}", [
+            _lib.Array() if x is None else x if not isinstance(x, self.torch.Tensor) else
+            _lib.make_array(x.data_ptr(), _dtype_name(x), x.shape, x.stride()) for x in args])
+
+    def _call(self, symbol, structs):
+        torch = self.torch
         lib = _lib.library()
         if self.queue is not None:
             q = self.queue
@@ -355,7 +378,7 @@ class _Arena:
                 lib.mops_b200_set_stream(q.compute.cuda_stream)
                 lib.mops_b200_set_wait(0)
                 try:
-                    _lib.call(f"mops_cuda_{name}_{self.suffix}", structs)
+                    _lib.call(symbol, structs)
                 finally:
                     lib.mops_b200_set_stream(previous)
                     lib.mops_b200_set_wait(waited)
@@ -366,7 +389,7 @@ class _Arena:
             previous = lib.mops_b200_get_stream()
             lib.mops_b200_set_stream(torch.cuda.current_stream().cuda_stream)
             try:
-                _lib.call(f"mops_cuda_{name}_{self.suffix}", structs)
+                _lib.call(symbol, structs)
             finally:
                 lib.mops_b200_set_stream(previous)
 
@@ -649,3 +672,104 @@ def sparse_accumulation_scatter_add_with_weights_vjp_vjp(grad_grad_A, grad_grad_
                _opt(m, grad_grad_B, 2), (None, 2), g_, A_, B_, C_, W_, m.ints(indices_A),
                m.ints(indices_W_1), m.ints(indices_W_2), m.ints(indices_output_1),
                m.ints(indices_output_2)])
+
+
+# ------------------------------------------------------------------- operators of the block
+def _check_real(value, operation, name):
+    if not isinstance(value, (int, float, np.integer, np.floating)) or isinstance(value, bool):
+        raise TypeError(f"`{name}` must be a number in {operation}, got {type(value)}")
+
+
+def embedding_lookup(W, indices, scale=1.0):
+    """``output[t,:] = scale * W[indices[t],:]``."""
+    op = "embedding_lookup"
+    _check(W, 2, "f", op, "W"); _check(indices, 1, "i", op, "indices")
+    _check_real(scale, op, "scale")
+    m = _Arena(W, half=True)
+    W_, i_ = m.rows(W), m.ints(indices)
+    out = m.empty((i_.shape[0], W_.shape[1]))
+    m.run_arrays(op, out, W_, i_, ctypes.c_double(scale))
+    return m.back(out)
+
+
+def embedding_lookup_vjp(grad_output, indices, n_rows, scale=1.0, padding_index=-1):
+    """The gradient of ``W`` (``n_rows`` rows): sums over equal indices, the same bits in every call; zeros
+    for rows that are not asked for, and for ``padding_index``."""
+    op = "embedding_lookup_vjp"
+    _check(grad_output, 2, "f", op, "grad_output"); _check(indices, 1, "i", op, "indices")
+    _check_scalar(n_rows, op, "n_rows"); _check_scalar(padding_index, op, "padding_index")
+    _check_real(scale, op, "scale")
+    m = _Arena(grad_output, half=True)
+    g_, i_ = m.rows(grad_output), m.ints(indices)
+    grad_W = m.empty((n_rows, g_.shape[1]))
+    m.run_arrays(op, grad_W, g_, i_, ctypes.c_double(scale), ctypes.c_int64(padding_index))
+    return m.back(grad_W)
+
+
+def _grouped_common(op, A, W, offsets):
+    _check(A, 2, "f", op, "A"); _check(W, 3, "f", op, "W"); _check(offsets, 1, "i", op, "offsets")
+
+
+def grouped_matrix_product(A, W, offsets):
+    """``output[r,:] = A[r,:] @ W[g]`` for the rows ``offsets[g] <= r < offsets[g+1]`` of group g; zeros for
+    rows of no group."""
+    op = "grouped_matrix_product"
+    _grouped_common(op, A, W, offsets)
+    m = _Arena(A, half=True)
+    A_, W_, o_ = m.rows(A), m.rows(W), m.ints(offsets)
+    out = m.empty((A_.shape[0], W_.shape[2]))
+    m.run_arrays(op, out, A_, W_, o_)
+    return m.back(out)
+
+
+def grouped_matrix_product_vjp(grad_output, A, W, offsets, compute_grad_A=True, compute_grad_W=True):
+    op = "grouped_matrix_product_vjp"
+    _check(grad_output, 2, "f", op, "grad_output")
+    _grouped_common(op, A, W, offsets)
+    m = _Arena(A, half=True)
+    g_, A_, W_, o_ = m.rows(grad_output), m.rows(A), m.rows(W), m.ints(offsets)
+    gA = m.empty(A_.shape) if compute_grad_A else None
+    gW = m.empty(W_.shape) if compute_grad_W else None
+    m.run_arrays(op, gA, gW, g_, A_, W_, o_)
+    return m.back(gA), m.back(gW)
+
+
+def _residual_inputs(m, residual, branch, gate, scale, weight_branch, weight_output):
+    return (m.rows(residual), m.rows(branch), None if gate is None else m.rows(gate), m.floats(scale),
+            m.floats(weight_branch), m.floats(weight_output))
+
+
+def _residual_check(op, residual, branch, gate, scale, weight_branch, weight_output, epsilon):
+    _check(residual, 2, "f", op, "residual"); _check(branch, 2, "f", op, "branch")
+    if gate is not None:
+        _check(gate, 2, "f", op, "gate")
+    _check(scale, 1, "f", op, "scale"); _check(weight_branch, 1, "f", op, "weight_branch")
+    _check(weight_output, 1, "f", op, "weight_output")
+    _check_real(epsilon, op, "epsilon")
+
+
+def gated_residual_norm(residual, branch, gate, scale, weight_branch, weight_output, epsilon=1e-6):
+    """The residual connection around a block with the norm behind the block and that in front of the next one:
+    returns ``stream = residual + scale * weight_branch * sigmoid(gate) * branch / rms(branch)`` and
+    ``normed = weight_output * stream / rms(stream)``, with ``rms(v) = sqrt(mean(v**2) + epsilon)`` over a
+    row. ``gate`` has the shape of ``residual``, or one column, or is None."""
+    op = "gated_residual_norm"
+    _residual_check(op, residual, branch, gate, scale, weight_branch, weight_output, epsilon)
+    m = _Arena(residual, half=True)
+    inputs = _residual_inputs(m, residual, branch, gate, scale, weight_branch, weight_output)
+    stream, normed = m.empty(inputs[0].shape), m.empty(inputs[0].shape)
+    m.run_arrays(op, stream, normed, *inputs, ctypes.c_double(epsilon))
+    return m.back(stream), m.back(normed)
+
+
+def gated_residual_norm_vjp(grad_stream, grad_normed, residual, branch, gate, scale, weight_branch,
+                            weight_output, epsilon=1e-6):
+    """Gradients of (residual, branch, gate, scale, weight_branch, weight_output); None without a gate."""
+    op = "gated_residual_norm_vjp"
+    _check(grad_stream, 2, "f", op, "grad_stream"); _check(grad_normed, 2, "f", op, "grad_normed")
+    _residual_check(op, residual, branch, gate, scale, weight_branch, weight_output, epsilon)
+    m = _Arena(residual, half=True)
+    inputs = _residual_inputs(m, residual, branch, gate, scale, weight_branch, weight_output)
+    gradients = [None if x is None else m.empty(x.shape) for x in inputs]
+    m.run_arrays(op, *gradients, m.rows(grad_stream), m.rows(grad_normed), *inputs, ctypes.c_double(epsilon))
+    return tuple(m.back(x) for x in gradients)

@@ -32,7 +32,10 @@ EXTENSION_SYMBOLS = ("mops_b200_set_stream", "mops_b200_get_stream", "mops_b200_
                      "mops_b200_get_wait", "mops_b200_version", "mops_b200_last_kernels",
                      "mops_b200_plan_create", "mops_b200_plan_destroy", "mops_b200_plan_bind",
                      "mops_b200_plan_bound", "mops_b200_plan_tables", "mops_b200_cuda_sort_index",
-                     "mops_b200_cuda_sparse_accumulation_scatter_add_with_weights_noalloc_f64")
+                     "mops_b200_cuda_sparse_accumulation_scatter_add_with_weights_noalloc_f64",
+                     "mops_b200_cuda_embedding_lookup", "mops_b200_cuda_embedding_lookup_vjp",
+                     "mops_b200_cuda_grouped_matrix_product", "mops_b200_cuda_grouped_matrix_product_vjp",
+                     "mops_b200_cuda_gated_residual_norm", "mops_b200_cuda_gated_residual_norm_vjp")
 
 
 class MopsError(Exception):
@@ -127,6 +130,23 @@ def null_struct(ndim):
     t = TENSOR[ndim]()
     t.data = None
     return t
+
+
+class Array(ctypes.Structure):
+    """A typed, strided view: ``mops_b200_array_t``."""
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int32), ("dimensions", ctypes.c_int32),
+                ("shape", ctypes.c_int64 * 3), ("stride", ctypes.c_int64 * 3)]
+
+
+ARRAY_TYPES = {"float32": 0, "float64": 1, "float16": 2, "bfloat16": 3, "int32": 4}
+
+
+def make_array(ptr, dtype, shape, stride):
+    """``dtype``: a key of ARRAY_TYPES; ``stride`` in values."""
+    a = Array(ptr, ARRAY_TYPES[dtype], len(shape))
+    for d, (n, s) in enumerate(zip(shape, stride)):
+        a.shape[d], a.stride[d] = n, s
+    return a
 
 
 def call(symbol, structs):

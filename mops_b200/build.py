@@ -29,7 +29,7 @@ NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-ccbin", HOST_CXX, "-Xco
                      "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr"]
 
 KERNEL_SOURCES = ["runtime.cu", "hpe.cu", "hpe_tmem.cu", "sap.cu", "sap_tmem.cu", "opsa.cu", "opsa_gathered.cu",
-                  "sasaw.cu", "sasaw_rows.cu", "sort.cu", "capi.cu", "host_stubs.cpp"]
+                  "embedding.cu", "grouped.cu", "residual_norm.cu", "sasaw.cu", "sasaw_rows.cu", "sort.cu", "capi.cu", "host_stubs.cpp"]
 
 
 def _newer(target, deps):
@@ -93,18 +93,27 @@ def build_torch(force=False):
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     jobs, libs = [], []
-    for name, source, more in (("libmops_torch.so", "torch_ops.cpp", []),
-                               ("_calls.so", "python_calls.cpp", ["-ltorch_python"])):
-        src, lib = os.path.join(CSRC, source), os.path.join(LIB, name)
+    links = []
+    for name, sources, more in (("libmops_torch.so", ["torch_ops.cpp", "torch_block_ops.cpp"], []),
+                                ("_calls.so", ["python_calls.cpp"], ["-ltorch_python"])):
+        lib, objs = os.path.join(LIB, name), []
         libs.append(lib)
-        if force or _newer(lib, [src, core] + _headers()):
-            jobs.append([HOST_CXX, "-O2", "-std=c++17", "-fPIC", "-shared",
-                         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", CSRC, "-I", INCLUDE] + inc +
-                        [src, "-o", lib, "-L", LIB, "-lmops", "-L", torch_lib, "-ltorch",
-                         "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda"] + more +
-                        ["-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
-    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        for source in sources:
+            src = os.path.join(CSRC, source)
+            obj = os.path.join(OBJ, os.path.splitext(source)[0] + ".o")
+            objs.append(obj)
+            if force or _newer(obj, [src] + _headers()):
+                jobs.append([HOST_CXX, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                             "-I", CSRC, "-I", INCLUDE] + inc + ["-c", src, "-o", obj])
+        links.append((lib, objs, [HOST_CXX, "-shared"] + objs +
+                      ["-o", lib, "-L", LIB, "-lmops", "-L", torch_lib, "-ltorch", "-ltorch_cpu", "-lc10",
+                       "-ltorch_cuda", "-lc10_cuda"] + more +
+                      ["-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]))
+    with cf.ThreadPoolExecutor(max_workers=3) as ex:
         list(ex.map(_run, jobs))
+    for lib, objs, cmd in links:
+        if force or _newer(lib, objs + [core]):
+            _run(cmd)
     return libs[0]
 
 

@@ -7,6 +7,7 @@
 #include <string>
 
 #include "../../include/mops.h"
+#include "block_ops.hpp"
 #include "mops.hpp"
 #include "runtime.hpp"
 
@@ -164,6 +165,30 @@ extern "C" int mops_b200_cuda_sort_index(mops_tensor_1d_i32_t sorted,
                                          mops_tensor_1d_i32_t indices, int64_t n_rows) {
     return guarded([&] { mops_b200::sort_index(cpp(sorted), cpp(permutation), cpp(indices), n_rows); });
 }
+
+#define BLOCK_ENTRY(name, DECLARED, ...)                                                          \
+    extern "C" int mops_b200_cuda_##name DECLARED {                                                \
+        return guarded([&] { mops_b200::name(__VA_ARGS__); });                                     \
+    }
+using Array = mops_b200_array_t;
+BLOCK_ENTRY(embedding_lookup, (Array output, Array W, Array indices, double scale), output, W, indices, scale)
+BLOCK_ENTRY(embedding_lookup_vjp,
+            (Array grad_W, Array grad_output, Array indices, double scale, int64_t padding_index), grad_W,
+            grad_output, indices, scale, padding_index)
+BLOCK_ENTRY(grouped_matrix_product, (Array output, Array A, Array W, Array offsets), output, A, W, offsets)
+BLOCK_ENTRY(grouped_matrix_product_vjp,
+            (Array grad_A, Array grad_W, Array grad_output, Array A, Array W, Array offsets), grad_A, grad_W,
+            grad_output, A, W, offsets)
+BLOCK_ENTRY(gated_residual_norm,
+            (Array stream, Array normed, Array residual, Array branch, Array gate, Array scale,
+             Array weight_branch, Array weight_output, double epsilon),
+            stream, normed, residual, branch, gate, scale, weight_branch, weight_output, epsilon)
+BLOCK_ENTRY(gated_residual_norm_vjp,
+            (Array grad_residual, Array grad_branch, Array grad_gate, Array grad_scale, Array grad_weight_branch,
+             Array grad_weight_output, Array grad_stream, Array grad_normed, Array residual, Array branch, Array gate,
+             Array scale, Array weight_branch, Array weight_output, double epsilon),
+            grad_residual, grad_branch, grad_gate, grad_scale, grad_weight_branch, grad_weight_output, grad_stream,
+            grad_normed, residual, branch, gate, scale, weight_branch, weight_output, epsilon)
 
 extern "C" int mops_b200_plan_create(mops_b200_plan_t** plan) {
     return guarded([&] {

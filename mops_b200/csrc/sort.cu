@@ -13,6 +13,7 @@
 
 #include "checks.hpp"
 #include "device.cuh"
+#include "sort.hpp"
 
 namespace mops_b200 {
 namespace {
@@ -35,7 +36,8 @@ __device__ __forceinline__ int sort_digit(int32_t key, int shift) { return (key 
 // also checks the range of the values.
 __global__ void __launch_bounds__(kSortThreads)
 radix_histogram(const int32_t* __restrict__ keys, int64_t n, int shift, int64_t n_rows,
-                bool check_range, int32_t* __restrict__ hist, Status st) {
+                bool check_range, int32_t replacement, int32_t dropped, int32_t* __restrict__ hist,
+                Status st) {
     __shared__ int32_t h[256];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     h[tid] = 0;
@@ -47,7 +49,9 @@ radix_histogram(const int32_t* __restrict__ keys, int64_t n, int shift, int64_t 
             int32_t key = __ldg(keys + pos);
             if (check_range && (key < 0 || key >= n_rows)) {
                 report_bad_index(st, 0);
-                key = 0;
+                key = replacement;
+            } else if (check_range && key == dropped) {
+                key = replacement;
             }
             atomicAdd(&h[sort_digit(key, shift)], 1);
         }
@@ -91,8 +95,8 @@ radix_scan_rows(int32_t* __restrict__ hist, int64_t blocks, int32_t* __restrict_
 __global__ void __launch_bounds__(kSortThreads)
 radix_scatter(const int32_t* __restrict__ keys_in, const int32_t* __restrict__ vals_in,
               int32_t* __restrict__ keys_out, int32_t* __restrict__ vals_out, int64_t n, int shift,
-              int64_t n_rows, bool clamp, const int32_t* __restrict__ scanned,
-              const int32_t* __restrict__ totals) {
+              int64_t n_rows, bool clamp, int32_t replacement, int32_t dropped,
+              const int32_t* __restrict__ scanned, const int32_t* __restrict__ totals) {
     __shared__ int32_t next[kSortWarps][256]; // per warp: where its next key of each digit goes
     __shared__ int32_t digit_base[256];       // keys with a smaller digit, over all tiles
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -117,7 +121,8 @@ radix_scatter(const int32_t* __restrict__ keys_in, const int32_t* __restrict__ v
         const int64_t pos = sort_position(tile0, warp, r, lane);
         const bool in = pos < n;
         key[r] = in ? __ldg(keys_in + pos) : 0;
-        if (clamp && (key[r] < 0 || key[r] >= n_rows)) key[r] = 0; // reported by the histogram pass
+        // (those out of range were reported by the histogram pass)
+        if (clamp && (key[r] < 0 || key[r] >= n_rows || key[r] == dropped)) key[r] = replacement;
         val[r] = in ? (vals_in != nullptr ? __ldg(vals_in + pos) : static_cast<int32_t>(pos)) : 0;
         const int d = in ? sort_digit(key[r], shift) : 256 + lane; // out-of-range lanes match nobody
         const unsigned peers = __match_any_sync(kFullMask, d);
@@ -160,19 +165,10 @@ const char* const kSortIndexNames[] = {"indices"};
 
 } // namespace
 
-void sort_index(mops::Tensor<int32_t, 1> sorted, mops::Tensor<int32_t, 1> permutation,
-                mops::Tensor<int32_t, 1> indices, int64_t n_rows) {
-    const std::string op = "cuda_sort_index";
-    same_size(indices, "indices", 0, sorted, "sorted", 0, op);
-    same_size(indices, "indices", 0, permutation, "permutation", 0, op);
-    fits_int32(indices.shape[0], "indices.shape[0]", op);
-    if (n_rows < 0 || n_rows > INT32_MAX)
-        throw std::runtime_error("n_rows does not fit the int32 index type in " + op);
-    const int64_t n = static_cast<int64_t>(indices.shape[0]);
-    if (n == 0) return;
-    Call call = begin_call();
+void sort_keys(const Call& call, int32_t* sorted, int32_t* permutation, const int32_t* indices, int64_t n,
+               int64_t n_rows, int32_t replacement, int32_t dropped) {
     int bits = 1;
-    while ((int64_t(1) << bits) < n_rows) bits++;
+    while ((int64_t(1) << bits) < std::max<int64_t>(n_rows, int64_t(replacement) + 1)) bits++;
     const int passes = (bits + 7) / 8;
     const int64_t blocks = ceil_div(n, kSortTile);
     const size_t hist_bytes = static_cast<size_t>(256) * blocks * sizeof(int32_t);
@@ -186,23 +182,38 @@ void sort_index(mops::Tensor<int32_t, 1> sorted, mops::Tensor<int32_t, 1> permut
     int32_t* tmp_keys[2] = {reinterpret_cast<int32_t*>(bufs), reinterpret_cast<int32_t*>(bufs + buf_bytes)};
     int32_t* tmp_vals[2] = {reinterpret_cast<int32_t*>(bufs + 2 * buf_bytes),
                             reinterpret_cast<int32_t*>(bufs + 3 * buf_bytes)};
-    const int32_t* keys_in = indices.data;
+    const int32_t* keys_in = indices;
     const int32_t* vals_in = nullptr;
     for (int pass = 0; pass < passes; pass++) {
         const bool last = pass == passes - 1;
-        int32_t* keys_out = last ? sorted.data : tmp_keys[pass & 1];
-        int32_t* vals_out = last ? permutation.data : tmp_vals[pass & 1];
+        int32_t* keys_out = last ? sorted : tmp_keys[pass & 1];
+        int32_t* vals_out = last ? permutation : tmp_vals[pass & 1];
         radix_histogram<<<static_cast<unsigned>(blocks), kSortThreads, 0, call.stream>>>(
-            keys_in, n, 8 * pass, n_rows, pass == 0, hist, call.status);
+            keys_in, n, 8 * pass, n_rows, pass == 0, replacement, dropped, hist, call.status);
         radix_scan_rows<<<256, 1024, 0, call.stream>>>(hist, blocks, totals);
         radix_scatter<<<static_cast<unsigned>(blocks), kSortThreads, 0, call.stream>>>(
-            keys_in, vals_in, keys_out, vals_out, n, 8 * pass, n_rows, pass == 0, hist, totals);
+            keys_in, vals_in, keys_out, vals_out, n, 8 * pass, n_rows, pass == 0, replacement, dropped, hist,
+            totals);
         MOPS_CUDA_OK(cudaGetLastError());
         keys_in = keys_out;
         vals_in = vals_out;
     }
     note_kernel_f("radix sort, %d passes", passes);
     scratch_free(call, scratch);
+}
+
+void sort_index(mops::Tensor<int32_t, 1> sorted, mops::Tensor<int32_t, 1> permutation,
+                mops::Tensor<int32_t, 1> indices, int64_t n_rows) {
+    const std::string op = "cuda_sort_index";
+    same_size(indices, "indices", 0, sorted, "sorted", 0, op);
+    same_size(indices, "indices", 0, permutation, "permutation", 0, op);
+    fits_int32(indices.shape[0], "indices.shape[0]", op);
+    if (n_rows < 0 || n_rows > INT32_MAX)
+        throw std::runtime_error("n_rows does not fit the int32 index type in " + op);
+    const int64_t n = static_cast<int64_t>(indices.shape[0]);
+    if (n == 0) return;
+    Call call = begin_call();
+    sort_keys(call, sorted.data, permutation.data, indices.data, n, n_rows, 0, -1);
     end_call(call, op.c_str(), kSortIndexNames, 1);
 }
 

@@ -4,6 +4,17 @@ Mirrors python/mops-torch/src/mops/torch/__init__.py of the reference: importing
 loads the operator library, after which the five operations are available both as
 ``torch.ops.mops.<name>`` and as attributes of this module, differentiable through autograd
 and usable from TorchScript. CUDA tensors only.
+
+So are the operators of the block around them (no counterpart in the reference), for float32, float64,
+float16 and bfloat16:
+
+* ``embedding_lookup(W, indices, scale=1.0, padding_index=-1)``: ``scale * W[indices]``; the gradient of
+  ``W`` leaves out ``padding_index``.
+* ``grouped_matrix_product(A, W, offsets)``: ``A[r] @ W[g]`` for the rows ``offsets[g] <= r < offsets[g+1]``.
+  ``W`` may be a transposed view (``weights.transpose(1, 2)``): nothing is copied.
+* ``gated_residual_norm(residual, branch, gate, scale, weight_branch, weight_output, epsilon=1e-6)``:
+  ``stream = residual + scale * weight_branch * sigmoid(gate) * branch / rms(branch)`` and
+  ``weight_output * stream / rms(stream)``.
 """
 import os
 
@@ -23,6 +34,9 @@ outer_product_scatter_add_with_weights = torch.ops.mops.outer_product_scatter_ad
 sparse_accumulation_scatter_add_with_weights = (
     torch.ops.mops.sparse_accumulation_scatter_add_with_weights
 )
+embedding_lookup = torch.ops.mops.embedding_lookup
+grouped_matrix_product = torch.ops.mops.grouped_matrix_product
+gated_residual_norm = torch.ops.mops.gated_residual_norm
 
 __all__ = [
     "homogeneous_polynomial_evaluation",
@@ -30,4 +44,7 @@ __all__ = [
     "outer_product_scatter_add",
     "outer_product_scatter_add_with_weights",
     "sparse_accumulation_scatter_add_with_weights",
+    "embedding_lookup",
+    "grouped_matrix_product",
+    "gated_residual_norm",
 ]
