@@ -1,20 +1,13 @@
-// Tiles of rows that belong to one group, for kernels over arrays whose rows are sorted by group.
+// Pieces of work on arrays whose rows are sorted by group, found on the device.
 //
-// The offsets of the groups are in device memory, so the host does not know how many tiles there are. It launches for the
-// most there can be (one partial tile for each group on top of the full ones), and each tile looks up which group it is
-// in, a warp at a time: 32 groups per step, whose tiles a prefix sum over the lanes counts.
+// The offsets of the groups are in device memory, so the host does not know how many tiles of rows there are. Each worker (a
+// warp) counts through the groups, 32 per step with a prefix sum over the lanes, to the piece that it is to do.
 #ifndef MOPS_B200_GROUP_TILES_CUH
 #define MOPS_B200_GROUP_TILES_CUH
 
 #include "device.cuh"
 
 namespace mops_b200 {
-
-// Rows [row, row + rows) of `group`; group == -1: rows of no group. rows == 0: there is no such tile.
-struct GroupTile {
-    int64_t group, row;
-    int rows;
-};
 
 // Where group g's rows lie, kept inside of [0, rows) whatever the offsets say. g == -1: the rows in front of the
 // first group; g == groups: those behind the last one.
@@ -25,60 +18,69 @@ __device__ __forceinline__ void group_bounds(const int32_t* __restrict__ offsets
     hi = max(lo, hi);
 }
 
-inline int64_t most_tiles(int64_t rows, int64_t groups, int tile_rows) {
-    return rows / tile_rows + std::min(rows, groups + 2);
-}
+// The rows [lo, hi) of a group and which of its pieces is meant; found == false: there is no such piece.
+struct GroupPiece {
+    bool found;
+    int64_t group, lo, hi, within;
+};
 
-// Walks the tiles of all groups in order. All lanes of a warp call it together and get the same answers; `want` must
-// not decrease from call to call.
-struct TileWalk {
+// Walks the pieces of groups first .. last in order, where pieces(rows of the group) says how many a group has. All
+// lanes of a warp call it together and get the same answers; `want` must not decrease from call to call.
+template <typename Pieces> struct GroupWalk {
     const int32_t* offsets;
-    int64_t groups, rows;
-    int tile_rows;
-    int64_t base = -1, before = 0; // first group of the step at hand, tiles in front of it
-    int64_t mine = -1;             // tiles of group base + lane (-1: not read yet)
+    int64_t groups, rows, last;
+    Pieces pieces;
+    int64_t base, before = 0;  // first group of the step at hand, pieces in front of it
+    int64_t up_to = 0;         // pieces of groups base .. base + lane
+    bool counted = false;
 
-    __device__ TileWalk(const int32_t* offsets, int64_t groups, int64_t rows, int tile_rows)
-        : offsets(offsets), groups(groups), rows(rows), tile_rows(tile_rows) {}
+    __device__ GroupWalk(const int32_t* offsets, int64_t groups, int64_t rows, int64_t first, int64_t last, Pieces pieces)
+        : offsets(offsets), groups(groups), rows(rows), last(last), pieces(pieces), base(first) {}
 
-    __device__ GroupTile find(int64_t want, int lane) {
-        while (base <= groups) {
-            if (mine < 0) {
-                mine = 0;
-                if (base + lane <= groups) {
+    __device__ GroupPiece find(int64_t want, int lane) {
+        while (base <= last) {
+            if (!counted) {
+                up_to = 0;
+                if (base + lane <= last) {
                     int64_t lo, hi;
                     group_bounds(offsets, groups, rows, base + lane, lo, hi);
-                    mine = ceil_div_device(hi - lo, tile_rows);
+                    up_to = pieces(hi - lo);
                 }
-            }
-            int64_t up_to = mine; // tiles of groups base .. base + lane
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int64_t v = __shfl_up_sync(kFullMask, up_to, d);
-                if (lane >= d) up_to += v;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int64_t v = __shfl_up_sync(kFullMask, up_to, d);
+                    if (lane >= d) up_to += v;
+                }
+                counted = true;
             }
             const unsigned reached = __ballot_sync(kFullMask, before + up_to > want);
             if (reached) {
                 const int at = __ffs(reached) - 1;
-                const int64_t within = want - before - __shfl_sync(kFullMask, up_to - mine, at);
-                GroupTile t;
-                t.group = base + at;
-                int64_t lo, hi;
-                group_bounds(offsets, groups, rows, t.group, lo, hi);
-                t.row = lo + within * tile_rows;
-                t.rows = static_cast<int>(min(hi - t.row, int64_t(tile_rows)));
-                if (t.group >= groups) t.group = -1;
-                return t;
+                const int64_t in_front = __shfl_sync(kFullMask, up_to, at > 0 ? at - 1 : 0);
+                GroupPiece p;
+                p.found = true;
+                p.group = base + at;
+                p.within = want - before - (at > 0 ? in_front : 0);
+                group_bounds(offsets, groups, rows, p.group, p.lo, p.hi);
+                return p;
             }
             before += __shfl_sync(kFullMask, up_to, 31);
             base += 32;
-            mine = -1;
+            counted = false;
         }
-        return GroupTile{-1, 0, 0};
+        return GroupPiece{false, 0, 0, 0, 0};
     }
-
-    __device__ static int64_t ceil_div_device(int64_t a, int64_t b) { return (a + b - 1) / b; }
 };
+
+// Tiles of `tile_rows` rows by `columns` tiles.
+struct RowTiles {
+    int tile_rows;
+    int64_t columns;
+    __device__ int64_t operator()(int64_t rows) const { return (rows + tile_rows - 1) / tile_rows * columns; }
+};
+inline int64_t most_row_tiles(int64_t rows, int64_t groups, int tile_rows) {
+    return rows / tile_rows + std::min(rows, groups + 2);
+}
 
 // Reports offsets that are not ascending within [0, rows] (index array 0); any block may do it.
 __device__ __forceinline__ void check_offsets(const int32_t* __restrict__ offsets, int64_t groups, int64_t rows,

@@ -9,6 +9,7 @@
 #include "arrays.hpp"
 #include "block_ops.hpp"
 #include "group_tiles.cuh"
+#include "grouped_mma.hpp"
 
 namespace mops_b200 {
 namespace {
@@ -57,16 +58,19 @@ grouped_rows_plain(T* __restrict__ out, const T* __restrict__ X, int64_t stride,
              int64_t depth, int64_t columns, Status st) {
     __shared__ Sum<T> a[kSlice][kTile + kPad], b[kSlice][kTile + kPad];
     if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(offsets, groups, rows, st);
-    TileWalk walk(offsets, groups, rows, kTile);
-    const GroupTile tile = walk.find(blockIdx.x, threadIdx.x & 31);
-    if (tile.rows == 0) return;
+    GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{kTile, 1});
+    const GroupPiece piece = walk.find(blockIdx.x, threadIdx.x & 31);
+    if (!piece.found) return;
+    const bool in_group = piece.group >= 0 && piece.group < groups;
+    const int64_t row0 = piece.lo + piece.within * kTile;
+    const int64_t here = min(piece.hi - row0, int64_t(kTile));
     for (int64_t j0 = static_cast<int64_t>(blockIdx.y) * kTile; j0 < columns; j0 += static_cast<int64_t>(gridDim.y) * kTile) {
         Sum<T> c[4][4] = {};
-        if (tile.group >= 0) {
-            const T* x = X + tile.row * stride;
-            const T* m = M + tile.group * group_stride + j0 * column_stride;
+        if (in_group) {
+            const T* x = X + row0 * stride;
+            const T* m = M + piece.group * group_stride + j0 * column_stride;
             for (int64_t d0 = 0; d0 < depth; d0 += kSlice) {
-                load_slice<T>(a, x + d0, 1, stride, depth - d0, tile.rows);
+                load_slice<T>(a, x + d0, 1, stride, depth - d0, here);
                 load_slice<T>(b, m + d0 * depth_stride, depth_stride, column_stride, depth - d0, columns - j0);
                 __syncthreads();
                 multiply_slices(c, a, b);
@@ -78,8 +82,8 @@ grouped_rows_plain(T* __restrict__ out, const T* __restrict__ X, int64_t stride,
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (i0 + i < tile.rows && j0 + jt + j < columns)
-                    out[(tile.row + i0 + i) * columns + j0 + jt + j] = narrow<T>(c[i][j]);
+                if (i0 + i < here && j0 + jt + j < columns)
+                    out[(row0 + i0 + i) * columns + j0 + jt + j] = narrow<T>(c[i][j]);
     }
 }
 
@@ -115,19 +119,11 @@ grouped_outer_plain(T* __restrict__ out, const T* __restrict__ X, int64_t x_stri
 
 const char* const kIndexNames[] = {"offsets"};
 
-// out = X (rows x depth) times, for each group, M (depth x columns; strides of its own).
-struct RowsProblem {
-    Array out, X, M;
-    int64_t depth_stride, column_stride; // of M
-    const int32_t* offsets;
-    int64_t groups, rows, depth, columns;
-};
-
 void multiply_rows(const Call& call, const RowsProblem& p, const std::string& op) {
-    if (p.rows == 0 || p.columns == 0) return;
+    if (p.rows == 0 || p.columns == 0 || multiply_rows_mma(call, p, op)) return;
     for_type(p.X.type, [&](auto zero) {
         using T = decltype(zero);
-        const int64_t tiles = most_tiles(p.rows, p.groups, kTile);
+        const int64_t tiles = most_row_tiles(p.rows, p.groups, kTile);
         fits_int32(static_cast<size_t>(tiles), "the number of tiles", op);
         const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>(ceil_div(p.columns, kTile), 65535)));
         grouped_rows_plain<T><<<grid, kThreads, 0, call.stream>>>(
@@ -138,11 +134,11 @@ void multiply_rows(const Call& call, const RowsProblem& p, const std::string& op
     MOPS_CUDA_OK(cudaGetLastError());
 }
 
-// out[g] = X[rows of g]^T Y[rows of g], contiguous.
-void multiply_outer(const Call& call, const Array& out, const Array& X, const Array& Y, const int32_t* offsets, int64_t groups,
-                    const std::string& op) {
-    const int64_t rows = X.shape[0], height = X.shape[1], columns = Y.shape[1];
-    if (groups == 0 || height == 0 || columns == 0) return;
+void multiply_outer(const Call& call, const OuterProblem& p, const std::string& op) {
+    const Array &out = p.out, &X = p.X, &Y = p.Y;
+    const int32_t* offsets = p.offsets;
+    const int64_t groups = p.groups, rows = X.shape[0], height = X.shape[1], columns = Y.shape[1];
+    if (groups == 0 || height == 0 || columns == 0 || multiply_outer_mma(call, p, op)) return;
     fits_int32(static_cast<size_t>(groups), "the number of groups", op);
     for_type(X.type, [&](auto zero) {
         using T = decltype(zero);
@@ -222,8 +218,8 @@ void grouped_matrix_product_vjp(Array grad_A, Array grad_W, Array grad_output, A
                       {grad_A, grad_output, W, W.stride[2], W.stride[1], starts, W.shape[0], A.shape[0], W.shape[2], A.shape[1]},
                       op);
     if (need_W) {
-        if (turned) multiply_outer(call, grad_W, grad_output, A, starts, W.shape[0], op);
-        else multiply_outer(call, grad_W, A, grad_output, starts, W.shape[0], op);
+        if (turned) multiply_outer(call, {grad_W, grad_output, A, starts, W.shape[0]}, op);
+        else multiply_outer(call, {grad_W, A, grad_output, starts, W.shape[0]}, op);
     }
     end_call(call, op.c_str(), kIndexNames, 1);
 }

@@ -1,0 +1,573 @@
+// grouped_matrix_product on tensor cores, for f16 and bf16.
+//
+// One block per SM works off tiles of 128 rows by kColumns columns. One warp has the copy engine fetch boxes of both operands into a ring
+// of stages of 64 values of depth, one thread of another issues the products (tcgen05.mma, accumulators in tensor
+// memory), and four warps move finished accumulators through shared memory to the output while the next tile is under way in
+// the other half of tensor memory.
+//
+// Rows: a tile begins where its group's rows do, wherever that is; of a tile that reaches past the end of its group the rows
+// behind it are computed and not stored. Outer products: the depth is the group's rows, and of the last stage of a
+// group the rows behind its end are cleared in shared memory before they are multiplied.
+#include "group_tiles.cuh"
+#include "grouped_mma.hpp"
+#include "tensor_map.hpp"
+#include "umma.cuh"
+
+namespace mops_b200 {
+
+namespace {
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        MOPS_CUDA_OK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &found));
+        if (entry == nullptr) throw std::runtime_error("the driver has no cuTensorMapEncodeTiled");
+        return reinterpret_cast<EncodeTiled>(entry);
+    }();
+    return f;
+}
+} // namespace
+
+CUtensorMap tensor_map_64(int32_t type, const void* data, int64_t inner, int64_t outer, int64_t slices,
+                          int64_t outer_stride, int64_t slice_stride, int box) {
+    CUtensorMap map;
+    // strides of dimensions of size 1 mean nothing, but have to look well
+    if (outer == 1) outer_stride = ceil_div(inner, 8) * 8;
+    if (slices == 1) slice_stride = outer * outer_stride;
+    const cuuint64_t size[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(slices)};
+    const cuuint64_t stride[2] = {static_cast<cuuint64_t>(outer_stride) * 2, static_cast<cuuint64_t>(slice_stride) * 2};
+    const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
+    const CUresult r = encode_tiled()(&map, type == MOPS_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                      3, const_cast<void*>(data), size, stride, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        throw std::runtime_error("CUDA error: cuTensorMapEncodeTiled returned " + std::to_string(static_cast<int>(r)));
+    return map;
+}
+
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kThreads = 192;   // the copying warp, the multiplying warp, four that store
+constexpr int kStoreWarps = 4;
+constexpr int kStaging = 32 * kBoxRow; // bytes: 32 rows of 64 values, of one warp
+constexpr int kBand = 16;       // tiles of rows that are taken in turn for a tile of columns, so that both stay in L2
+
+// What a block keeps in shared memory.
+template <int kColumns> struct Layout {
+    static constexpr int kStages = kColumns == 256 ? 4 : kColumns == 128 ? 6 : 8;
+    static constexpr int kA = kTileRows * kBoxRow, kB = kColumns * kBoxRow; // bytes of a stage
+    static constexpr int kStage = kA + kB;
+    static constexpr int kStagingAt = kStages * kStage;
+    static constexpr int kBarriersAt = kStagingAt + kStoreWarps * 2 * kStaging;
+    static constexpr int kBytes = kBarriersAt + 256 + 1024; // (boxes begin on multiples of 1024 bytes)
+    static constexpr unsigned kTmem = 2 * kColumns;         // columns of tensor memory: two accumulators
+};
+
+struct Barriers {
+    uint64_t full[8], empty[8], done[2], free[2];
+    uint32_t tmem;
+    int gave_up;
+};
+
+// Output tiles of a block of `rows` x `columns` tiles, kBand tiles of rows at a time.
+__device__ __forceinline__ void banded(int64_t at, int64_t rows, int64_t columns, int64_t& row, int64_t& column) {
+    const int64_t band = at / (kBand * columns);
+    const int64_t high = min(int64_t(kBand), rows - band * kBand);
+    const int64_t r = at - band * kBand * columns;
+    column = r / high;
+    row = band * kBand + (r - column * high);
+}
+
+// The parts that both kernels share: setting up and leaving, and the turn that each side takes at the ring of stages and
+// at the two accumulators. A wait that runs out is reported, and everybody leaves.
+template <int kColumns> struct Block {
+    using L = Layout<kColumns>;
+    unsigned char* smem;
+    Barriers* b;
+    uint32_t base; // shared-memory address of the stages
+    Status st;
+
+    __device__ Block(unsigned char* raw, const Status& st) : st(st) {
+        smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+        b = reinterpret_cast<Barriers*>(smem + L::kBarriersAt);
+        base = smem_address(smem);
+    }
+    __device__ void begin(int warp) {
+        if (warp == 1) tmem_alloc(&b->tmem, L::kTmem);
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < L::kStages; s++) mbarrier_init(&b->full[s], 1), mbarrier_init(&b->empty[s], 1);
+            for (int a = 0; a < 2; a++) mbarrier_init(&b->done[a], 1), mbarrier_init(&b->free[a], kStoreWarps);
+            b->gave_up = 0;
+            mbarrier_init_fence();
+        }
+        tmem_fence_before_sync();
+        __syncthreads();
+        tmem_fence_after_sync();
+    }
+    __device__ void end(int warp) {
+        tmem_fence_before_sync();
+        __syncthreads();
+        tmem_fence_after_sync();
+        if (warp == 1) tmem_free(b->tmem, L::kTmem);
+    }
+    __device__ bool wait(uint64_t* bar, unsigned parity) {
+        if (*static_cast<volatile int*>(&b->gave_up) == 0 && mbarrier_wait(bar, parity)) return true;
+        if (atomicExch(&b->gave_up, 1) == 0) report_stalled(st);
+        return false;
+    }
+    __device__ uint32_t stage(int64_t i) const { return base + static_cast<uint32_t>(i % L::kStages) * L::kStage; }
+    // The copying thread, before it fills stage i; before it leaves, for the copies that nobody waited for.
+    __device__ bool wait_empty(int64_t i) {
+        return i < L::kStages || wait(&b->empty[i % L::kStages], static_cast<unsigned>(i / L::kStages - 1) & 1);
+    }
+    __device__ void drain(int64_t issued) {
+        if (*static_cast<volatile int*>(&b->gave_up) == 0) return;
+        for (int64_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; i++)
+            (void)mbarrier_wait(&b->full[i % L::kStages], static_cast<unsigned>(i / L::kStages) & 1);
+    }
+    __device__ bool wait_full(int64_t i) { return wait(&b->full[i % L::kStages], static_cast<unsigned>(i / L::kStages) & 1); }
+    __device__ bool wait_free(int64_t tile) { return tile < 2 || wait(&b->free[tile & 1], static_cast<unsigned>(tile / 2 - 1) & 1); }
+    __device__ bool wait_done(int64_t tile) { return wait(&b->done[tile & 1], static_cast<unsigned>(tile / 2) & 1); }
+    __device__ uint32_t accumulator(int64_t tile) const { return b->tmem + static_cast<uint32_t>(tile & 1) * kColumns; }
+};
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// Writes the 64 columns that follow `column` of a warp's 32 rows of an accumulator: a whole band by the copy engine, of a band that the group's
+// end cuts (`here` rows) each lane its row.
+template <bool BF16>
+__device__ __forceinline__ void store_columns(uint32_t accumulator, uint32_t staging, int64_t& sent, const CUtensorMap& map,
+                                              uint16_t* __restrict__ out, int64_t row, int slice, int column, int64_t columns, int here,
+                                              int lane) {
+    uint32_t r[2][32];
+    tmem_load(accumulator, r[0]);
+    tmem_load(accumulator + 32, r[1]);
+    tmem_wait_load();
+    tmem_pin(r[0]);
+    tmem_pin(r[1]);
+    uint4 v[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+        const uint32_t* w = &r[c / 4][c % 4 * 8];
+        v[c] = make_uint4(pack2<BF16>(w[0], w[1]), pack2<BF16>(w[2], w[3]), pack2<BF16>(w[4], w[5]), pack2<BF16>(w[6], w[7]));
+    }
+    if (here == 32) {
+        const uint32_t to = staging + static_cast<uint32_t>(sent & 1) * kStaging;
+        if (lane == 0) boxes_left<1>();
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 8; c++) smem_store16(to + lane * kBoxRow + ((c ^ (lane & 7)) << 4), v[c]);
+        async_proxy_fence();
+        __syncwarp();
+        if (lane == 0) box_out(map, column, static_cast<int>(row), slice, to);
+        sent++;
+    } else if (lane < here) {
+        uint4* to = reinterpret_cast<uint4*>(out + (row + lane) * columns + column);
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (column + c * 8 < columns) to[c] = v[c]; // (columns are a multiple of 8 here)
+    }
+}
+
+// ---------------------------------------------------------------------------------- rows
+// out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
+template <bool BF16, bool M_MN, int kColumns>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m,
+                 const __grid_constant__ CUtensorMap map_out, uint16_t* __restrict__ out, const int32_t* __restrict__ offsets,
+                 int64_t groups, int64_t rows, int depth, int columns, Status st) {
+    extern __shared__ unsigned char raw[];
+    using L = Layout<kColumns>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Block<kColumns> block(raw, st);
+    block.begin(warp);
+    if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
+
+    const int64_t column_tiles = (columns + kColumns - 1) / kColumns;
+    const int steps = (depth + kBoxDepth - 1) / kBoxDepth;
+    GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{kTileRows, column_tiles});
+    int64_t step = 0, tile = 0; // so far
+    int64_t sent = 0;           // boxes that this warp has stored
+    for (int64_t want = blockIdx.x;; want += gridDim.x) {
+        const GroupPiece piece = walk.find(want, lane);
+        if (!piece.found) break;
+        int64_t tile_row, tile_column;
+        banded(piece.within, (piece.hi - piece.lo + kTileRows - 1) / kTileRows, column_tiles, tile_row, tile_column);
+        const int64_t row = piece.lo + tile_row * kTileRows;
+        const int column = static_cast<int>(tile_column) * kColumns;
+        const bool in_group = piece.group >= 0 && piece.group < groups;
+        bool ok = true;
+        if (warp == 0) {
+            if (lane == 0 && in_group) {
+                for (int s = 0; s < steps && ok; s++, step++) {
+                    ok = block.wait_empty(step);
+                    if (!ok) break;
+                    uint64_t* full = &block.b->full[step % L::kStages];
+                    const uint32_t a = block.stage(step), b = a + L::kA;
+                    mbarrier_arrive_expect(full, L::kStage);
+                    box_in(a, map_x, s * kBoxDepth, static_cast<int>(row), 0, full);
+                    if constexpr (M_MN) {
+#pragma unroll
+                        for (int j = 0; j < kColumns / 64; j++)
+                            box_in(b + j * kBoxBytes, map_m, column + j * 64, s * kBoxDepth, static_cast<int>(piece.group), full);
+                    } else {
+                        box_in(b, map_m, s * kBoxDepth, column, static_cast<int>(piece.group), full);
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0 && in_group) {
+                constexpr uint32_t instruction = instruction_descriptor(BF16, false, M_MN, kColumns);
+                ok = block.wait_free(tile);
+                tmem_fence_after_sync();
+                for (int s = 0; s < steps && ok; s++, step++) {
+                    ok = block.wait_full(step);
+                    if (!ok) break;
+                    tmem_fence_after_sync();
+                    const uint64_t a = operand_descriptor(block.stage(step), kBoxBytes);
+                    const uint64_t b = operand_descriptor(block.stage(step) + L::kA, kBoxBytes);
+#pragma unroll
+                    for (int k = 0; k < kBoxDepth / 16; k++)
+                        umma(block.accumulator(tile), a + k * kDepthStep<false>, b + k * kDepthStep<M_MN>, instruction, s + k > 0);
+                    umma_arrive(&block.b->empty[step % L::kStages]);
+                }
+                if (ok) umma_arrive(&block.b->done[tile & 1]);
+                tile++;
+            }
+        } else {
+            const int quadrant = warp & 3;
+            const int64_t band = row + quadrant * 32;
+            const int here = static_cast<int>(min(max(piece.hi - band, int64_t(0)), int64_t(32)));
+            const int wide = min(columns - column, kColumns);
+            if (in_group) {
+                ok = block.wait_done(tile);
+                if (ok) {
+                    tmem_fence_after_sync();
+                    const uint32_t from = tmem_quadrant(block.accumulator(tile), quadrant);
+                    const uint32_t staging = block.base + L::kStagingAt + quadrant * 2 * kStaging;
+                    if (here > 0)
+                        for (int c = 0; c < wide; c += 64)
+                            store_columns<BF16>(from + c, staging, sent, map_out, out, band, 0, column + c, columns, here, lane);
+                    tmem_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbarrier_arrive(&block.b->free[tile & 1]);
+                }
+                tile++;
+            } else if (lane < here) { // rows of no group
+                uint4* to = reinterpret_cast<uint4*>(out + (band + lane) * columns + column);
+                for (int c = 0; c < wide / 8; c++) to[c] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (!__shfl_sync(kFullMask, ok, 0)) break;
+    }
+    if (warp == 0 && lane == 0) block.drain(step);
+    if (warp >= 2 && lane == 0) boxes_left<0>();
+    __syncwarp();
+    block.end(warp);
+}
+
+// ------------------------------------------------------------------------- outer products
+// A group's rows are cut into segments of `segment` rows; the pieces of work are (segment, tile of the output). A group of more than one segment
+// leaves its tiles in `parts`, in f32, one after the other, and grouped_outer_join adds them up.
+struct OuterPieces {
+    int64_t segment, tiles;
+    __device__ int64_t operator()(int64_t rows) const { return max((rows + segment - 1) / segment, int64_t(1)) * tiles; }
+};
+struct OuterParts { // of those, the ones that are left in parts
+    int64_t segment, tiles;
+    __device__ int64_t operator()(int64_t rows) const { return rows > segment ? (rows + segment - 1) / segment * tiles : 0; }
+};
+struct OuterJoins {
+    int64_t segment, tiles;
+    __device__ int64_t operator()(int64_t rows) const { return rows > segment ? tiles : 0; }
+};
+
+// How many parts the groups in front of `group` leave (a warp together).
+__device__ __forceinline__ int64_t parts_before(const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int64_t group,
+                                                OuterParts parts, int lane) {
+    int64_t n = 0;
+    for (int64_t g = lane; g < group; g += 32) {
+        int64_t lo, hi;
+        group_bounds(offsets, groups, rows, g, lo, hi);
+        n += parts(hi - lo);
+    }
+    return warp_sum(n);
+}
+
+// out[g] = X[rows of g]^T Y[rows of g].
+template <bool BF16, int kColumns>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                  const __grid_constant__ CUtensorMap map_out, float* __restrict__ parts, int64_t most_parts,
+                  const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment,
+                  Status st) {
+    extern __shared__ unsigned char raw[];
+    using L = Layout<kColumns>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Block<kColumns> block(raw, st);
+    block.begin(warp);
+    if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
+
+    const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
+    const int64_t tiles = row_tiles * column_tiles;
+    GroupWalk<OuterPieces> walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles});
+    int64_t step = 0, tile = 0, sent = 0;
+    for (int64_t want = blockIdx.x;; want += gridDim.x) {
+        const GroupPiece piece = walk.find(want, lane);
+        if (!piece.found) break;
+        const int64_t part = piece.within / tiles;
+        int64_t tile_row, tile_column;
+        banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
+        const int row = static_cast<int>(tile_row) * kTileRows, column = static_cast<int>(tile_column) * kColumns;
+        const int64_t lo = piece.lo + part * segment, hi = min(lo + segment, piece.hi);
+        const int steps = static_cast<int>((hi - lo + kBoxDepth - 1) / kBoxDepth);
+        bool ok = true;
+        if (warp == 0) {
+            if (lane == 0) {
+                for (int s = 0; s < steps && ok; s++, step++) {
+                    ok = block.wait_empty(step);
+                    if (!ok) break;
+                    uint64_t* full = &block.b->full[step % L::kStages];
+                    const uint32_t a = block.stage(step), b = a + L::kA;
+                    const int at = static_cast<int>(lo) + s * kBoxDepth;
+                    mbarrier_arrive_expect(full, L::kStage);
+#pragma unroll
+                    for (int i = 0; i < kTileRows / 64; i++) box_in(a + i * kBoxBytes, map_x, row + i * 64, at, 0, full);
+#pragma unroll
+                    for (int j = 0; j < kColumns / 64; j++) box_in(b + j * kBoxBytes, map_y, column + j * 64, at, 0, full);
+                }
+            }
+        } else if (warp == 1) {
+            if (steps > 0) {
+                constexpr uint32_t instruction = instruction_descriptor(BF16, true, true, kColumns);
+                if (lane == 0) ok = block.wait_free(tile);
+                ok = __shfl_sync(kFullMask, ok, 0);
+                tmem_fence_after_sync();
+                for (int s = 0; s < steps && ok; s++, step++) {
+                    const int64_t left = hi - lo - int64_t(s) * kBoxDepth;
+                    if (lane == 0 || left < kBoxDepth) ok = block.wait_full(step);
+                    ok = __all_sync(kFullMask, ok);
+                    if (!ok) break;
+                    if (left < kBoxDepth) { // the rows behind are of another group
+                        const uint32_t from = static_cast<uint32_t>(left) * kBoxRow;
+                        for (uint32_t box = 0; box < L::kStage; box += kBoxBytes)
+                            for (uint32_t at = from + lane * 16; at < kBoxBytes; at += 32 * 16)
+                                smem_store16(block.stage(step) + box + at, make_uint4(0, 0, 0, 0));
+                        async_proxy_fence();
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+                        tmem_fence_after_sync();
+                        const uint64_t a = operand_descriptor(block.stage(step), kBoxBytes);
+                        const uint64_t b = operand_descriptor(block.stage(step) + L::kA, kBoxBytes);
+#pragma unroll
+                        for (int k = 0; k < kBoxDepth / 16; k++)
+                            umma(block.accumulator(tile), a + k * kDepthStep<true>, b + k * kDepthStep<true>, instruction, s + k > 0);
+                        umma_arrive(&block.b->empty[step % L::kStages]);
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0 && ok) umma_arrive(&block.b->done[tile & 1]);
+                tile++;
+            }
+        } else {
+            const int quadrant = warp & 3;
+            const int band = row + quadrant * 32, wide = min(columns - column, kColumns);
+            if (steps > 0) ok = block.wait_done(tile);
+            if (ok) {
+                const uint32_t from = tmem_quadrant(block.accumulator(tile), quadrant);
+                const uint32_t staging = block.base + L::kStagingAt + quadrant * 2 * kStaging;
+                tmem_fence_after_sync();
+                if (piece.hi - piece.lo > segment) {
+                    const int64_t slot = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
+                    float* to = parts + (slot * kTileRows + quadrant * 32 + lane) * kColumns;
+                    // (there are more parts than there is room for only where offsets descend, which is reported)
+                    for (int c = 0; c < wide && slot < most_parts; c += 32) {
+                        uint32_t r[32];
+                        tmem_load(from + c, r);
+                        tmem_wait_load();
+                        tmem_pin(r);
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            *reinterpret_cast<uint4*>(to + c + 4 * i) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                    }
+                } else if (band < height) {
+                    for (int c = 0; c < wide; c += 64) {
+                        if (steps > 0) {
+                            store_columns<BF16>(from + c, staging, sent, map_out, nullptr, band, static_cast<int>(piece.group), column + c,
+                                                columns, 32, lane);
+                        } else { // a group without rows
+                            const uint32_t to = staging + static_cast<uint32_t>(sent & 1) * kStaging;
+                            if (lane == 0) boxes_left<1>();
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 8; i++) smem_store16(to + lane * kBoxRow + i * 16, make_uint4(0, 0, 0, 0));
+                            async_proxy_fence();
+                            __syncwarp();
+                            if (lane == 0) box_out(map_out, column + c, band, static_cast<int>(piece.group), to);
+                            sent++;
+                        }
+                    }
+                }
+                if (steps > 0) {
+                    tmem_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbarrier_arrive(&block.b->free[tile & 1]);
+                    tile++;
+                }
+            }
+        }
+        if (!__shfl_sync(kFullMask, ok, 0)) break;
+    }
+    if (warp == 0 && lane == 0) block.drain(step);
+    if (warp >= 2 && lane == 0) boxes_left<0>();
+    __syncwarp();
+    block.end(warp);
+}
+
+// Adds up the parts of a tile, in the order of the rows.
+template <typename T, int kColumns>
+__global__ void __launch_bounds__(256)
+grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t most_parts,
+                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment) {
+    const int lane = threadIdx.x & 31;
+    const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
+    const int64_t tiles = row_tiles * column_tiles;
+    GroupWalk<OuterJoins> walk(offsets, groups, rows, 0, groups - 1, OuterJoins{segment, tiles});
+    const GroupPiece piece = walk.find(blockIdx.x, lane);
+    if (!piece.found) return;
+    int64_t tile_row, tile_column;
+    banded(piece.within, row_tiles, column_tiles, tile_row, tile_column);
+    const int row = static_cast<int>(tile_row) * kTileRows, column = static_cast<int>(tile_column) * kColumns;
+    const int64_t n = (piece.hi - piece.lo + segment - 1) / segment;
+    const int64_t first = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
+    if (first + (n - 1) * tiles >= most_parts) return;
+    constexpr int kSplit = 8; // blocks to a tile
+    constexpr int kValues = kTileRows * kColumns / kSplit;
+    for (int at = blockIdx.y * kValues + threadIdx.x * 4; at < (blockIdx.y + 1) * kValues; at += 256 * 4) {
+        const int i = at / kColumns, j = at % kColumns;
+        if (row + i >= height || column + j >= columns) continue;
+        float4 sum = make_float4(0, 0, 0, 0);
+        const float* from = parts + (first * kTileRows + i) * kColumns + j;
+        for (int64_t s = 0; s < n; s++) {
+            const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kTileRows * kColumns);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        T* to = out + (piece.group * height + row + i) * columns + column + j;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (column + j + k < columns) to[k] = narrow<T>(v[k]);
+    }
+}
+
+// Whether the copy engine can fetch an array of 16-bit values by its rows.
+bool boxable(const void* data, int64_t outer, int64_t outer_stride, int64_t inner, int64_t slices, int64_t slice_stride) {
+    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (outer == 1 || (outer_stride % 8 == 0 && outer_stride >= inner)) &&
+           (slices == 1 || (slice_stride % 8 == 0 && slice_stride > 0));
+}
+
+} // namespace
+
+bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string& op) {
+    if (p.X.type != MOPS_B200_F16 && p.X.type != MOPS_B200_BF16) return false;
+    const bool mn = p.column_stride == 1;
+    const int64_t stride = mn ? p.depth_stride : p.column_stride; // of M
+    if (p.depth == 0 || p.groups == 0 || p.columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0 ||
+        !boxable(p.X.data, p.rows, p.X.stride[0], p.depth, 1, 0) ||
+        !boxable(p.M.data, mn ? p.depth : p.columns, stride, mn ? p.columns : p.depth, p.groups, p.M.stride[0]))
+        return false;
+    const int sms = sm_count(call.device);
+    auto launch = [&](auto type, auto major, auto width) {
+        constexpr bool BF16 = decltype(type)::value, M_MN = decltype(major)::value;
+        constexpr int kColumns = decltype(width)::value;
+        using L = Layout<kColumns>;
+        const CUtensorMap x = tensor_map_64(p.X.type, p.X.data, p.depth, p.rows, 1, p.X.stride[0], 0, kTileRows);
+        const CUtensorMap m = M_MN ? tensor_map_64(p.X.type, p.M.data, p.columns, p.depth, p.groups, stride, p.M.stride[0], 64)
+                                   : tensor_map_64(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
+        const CUtensorMap out = tensor_map_64(p.X.type, p.out.data, p.columns, p.rows, 1, p.columns, 0, 32);
+        const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
+        auto kernel = grouped_rows_mma<BF16, M_MN, kColumns>;
+        allow_dynamic_smem(kernel, call.device, L::kBytes);
+        kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kThreads, L::kBytes, call.stream>>>(
+            x, m, out, static_cast<uint16_t*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth),
+            static_cast<int>(p.columns), call.status);
+        note_kernel_f("grouped_rows_mma<%s,%s,%d>", BF16 ? "bf16" : "f16", M_MN ? "columns" : "depth", kColumns);
+    };
+    auto by_width = [&](auto type, auto major) {
+        // The wider the tile, the fewer times X is fetched; the narrower, the more blocks share the work.
+        const int64_t row_tiles = most_row_tiles(p.rows, p.groups, kTileRows);
+        if (p.columns > 128 && row_tiles * ceil_div(p.columns, 256) >= sms) launch(type, major, std::integral_constant<int, 256>());
+        else if (p.columns > 64 && row_tiles * ceil_div(p.columns, 128) >= sms / 2) launch(type, major, std::integral_constant<int, 128>());
+        else launch(type, major, std::integral_constant<int, 64>());
+    };
+    auto by_major = [&](auto type) {
+        if (mn) by_width(type, std::true_type());
+        else by_width(type, std::false_type());
+    };
+    if (p.X.type == MOPS_B200_BF16) by_major(std::true_type());
+    else by_major(std::false_type());
+    MOPS_CUDA_OK(cudaGetLastError());
+    return true;
+}
+
+bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::string& op) {
+    if (p.X.type != MOPS_B200_F16 && p.X.type != MOPS_B200_BF16) return false;
+    const int64_t rows = p.X.shape[0], height = p.X.shape[1], columns = p.Y.shape[1];
+    if (rows == 0 || columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0 ||
+        !boxable(p.X.data, rows, p.X.stride[0], height, 1, 0) || !boxable(p.Y.data, rows, p.Y.stride[0], columns, 1, 0))
+        return false;
+    const int sms = sm_count(call.device);
+    auto launch = [&](auto type, auto width) {
+        constexpr bool BF16 = decltype(type)::value;
+        constexpr int kColumns = decltype(width)::value;
+        using L = Layout<kColumns>;
+        using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+        const CUtensorMap x = tensor_map_64(p.X.type, p.X.data, height, rows, 1, p.X.stride[0], 0, 64);
+        const CUtensorMap y = tensor_map_64(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, 64);
+        const CUtensorMap out = tensor_map_64(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
+        const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
+        // Segments such that, were all rows in one group, there would be some four pieces of work for each SM; so no block has much more
+        // than its share, and few tiles are left in parts where there are many groups.
+        const int64_t segment = std::max<int64_t>(ceil_div(rows * tiles, int64_t(sms) * 4 * 64) * 64, 256);
+        const int64_t most_parts = tiles * (rows / segment * 2);
+        float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
+                                      : nullptr;
+        auto kernel = grouped_outer_mma<BF16, kColumns>;
+        allow_dynamic_smem(kernel, call.device, L::kBytes);
+        const int64_t pieces = tiles * (rows / segment + p.groups);
+        kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
+            x, y, out, parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment, call.status);
+        if (rows > segment) {
+            const int64_t joins = tiles * std::min<int64_t>(p.groups, rows / segment);
+            fits_int32(static_cast<size_t>(joins), "the number of tiles", op);
+            grouped_outer_join<T, kColumns><<<dim3(static_cast<unsigned>(joins), 8), 256, 0, call.stream>>>(
+                static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment);
+            scratch_free(call, parts);
+        }
+        note_kernel_f("grouped_outer_mma<%s,%d>", BF16 ? "bf16" : "f16", kColumns);
+    };
+    auto by_width = [&](auto type) {
+        if (columns > 128) launch(type, std::integral_constant<int, 256>());
+        else if (columns > 64) launch(type, std::integral_constant<int, 128>());
+        else launch(type, std::integral_constant<int, 64>());
+    };
+    if (p.X.type == MOPS_B200_BF16) by_width(std::true_type());
+    else by_width(std::false_type());
+    MOPS_CUDA_OK(cudaGetLastError());
+    return true;
+}
+
+} // namespace mops_b200

@@ -1,0 +1,29 @@
+// grouped_matrix_product on tensor cores (grouped_mma.cu): the problems, and launches that say whether they took one on.
+#ifndef MOPS_B200_GROUPED_MMA_HPP
+#define MOPS_B200_GROUPED_MMA_HPP
+
+#include "arrays.hpp"
+
+namespace mops_b200 {
+
+// out = X (rows x depth) times, for each group, M (value (d, j) at d * depth_stride + j * column_stride, one of them 1).
+struct RowsProblem {
+    Array out, X, M;
+    int64_t depth_stride, column_stride;
+    const int32_t* offsets;
+    int64_t groups, rows, depth, columns;
+};
+
+// out[g] = X[rows of g]^T Y[rows of g]; out is contiguous.
+struct OuterProblem {
+    Array out, X, Y;
+    const int32_t* offsets;
+    int64_t groups;
+};
+
+bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string& op);
+bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::string& op);
+
+} // namespace mops_b200
+
+#endif

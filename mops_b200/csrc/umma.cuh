@@ -1,0 +1,81 @@
+// Tensor-core products with operands in shared memory and accumulators in tensor memory (tcgen05.mma), and the tiled copies
+// (cp.async.bulk.tensor) that feed them. One thread issues each of them.
+//
+// Operand tiles are boxes of rows of 128 bytes (64 values of 16 bits), swizzled: the 16-byte chunk c of row r lies at chunk
+// c ^ (r mod 8). Where the rows run along the depth of the product (K-major) a box holds `rows` rows or columns of the operand; where
+// they run across it (MN-major) a box holds 64 of them, 64 deep, and boxes of further ones follow.
+#ifndef MOPS_B200_UMMA_CUH
+#define MOPS_B200_UMMA_CUH
+
+#include <cuda.h>
+
+#include "tmem.cuh"
+
+namespace mops_b200 {
+
+constexpr int kBoxRow = 128;               // bytes
+constexpr int kBoxDepth = 64;              // values in a row, and the depth of a stage
+constexpr int kBoxBytes = 64 * kBoxRow;    // of a box of 64 rows
+
+// The shared-memory descriptor of an operand: version 1, 128-byte swizzle. `across`: bytes between boxes of 64 rows or columns (MN-major;
+// K-major operands ignore it). Groups of eight rows are 1024 bytes apart in both.
+__device__ __forceinline__ uint64_t operand_descriptor(uint32_t address, uint32_t across) {
+    return static_cast<uint64_t>((address & 0x3ffff) >> 4) | static_cast<uint64_t>(across >> 4) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+// What one step of 16 values in depth adds to a descriptor.
+template <bool MN> constexpr uint64_t kDepthStep = MN ? 2048 >> 4 : 32 >> 4;
+
+// f32 accumulators of 128 x n; both operands bf16 (or both f16).
+__host__ __device__ constexpr uint32_t instruction_descriptor(bool bf16, bool a_mn, bool b_mn, int n) {
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
+           static_cast<uint32_t>(n / 8) << 17 | static_cast<uint32_t>(128 / 16) << 24;
+}
+
+__device__ __forceinline__ void umma(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(accumulator),
+                 "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate))
+                 : "memory");
+}
+// Arrives on `bar` when the products issued so far by this thread are done.
+__device__ __forceinline__ void umma_arrive(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_address(bar))
+                 : "memory");
+}
+
+__device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_address(bar)) : "memory");
+}
+
+// Makes this thread's writes to shared memory visible to the copy engine and the tensor cores.
+__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+// Box at (inner, outer, slice) of an array, completion counted on `bar`.
+__device__ __forceinline__ void box_in(uint32_t smem, const CUtensorMap& map, int inner, int outer, int slice, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::
+                     "r"(smem),
+                 "l"(&map), "r"(inner), "r"(outer), "r"(slice), "r"(smem_address(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void box_out(const CUtensorMap& map, int inner, int outer, int slice, uint32_t smem) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(&map),
+                 "r"(inner), "r"(outer), "r"(slice), "r"(smem)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+// Until all but the last N boxes that this thread sent out have left shared memory.
+template <int N> __device__ __forceinline__ void boxes_left() {
+    asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void map_prefetch(const CUtensorMap& map) {
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
+}
+
+__device__ __forceinline__ void smem_store16(uint32_t address, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+} // namespace mops_b200
+
+#endif
