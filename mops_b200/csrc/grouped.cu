@@ -120,7 +120,9 @@ grouped_outer_plain(T* __restrict__ out, const T* __restrict__ X, int64_t x_stri
 const char* const kIndexNames[] = {"offsets"};
 
 void multiply_rows(const Call& call, const RowsProblem& p, const std::string& op) {
-    if (p.rows == 0 || p.columns == 0 || multiply_rows_mma(call, p, op)) return;
+    if (p.rows == 0 || p.columns == 0 || multiply_rows_mma(call, p, op) ||
+        multiply_rows_split(call, p, op))
+        return;
     for_type(p.X.type, [&](auto zero) {
         using T = decltype(zero);
         const int64_t tiles = most_row_tiles(p.rows, p.groups, kTile);
@@ -138,7 +140,9 @@ void multiply_outer(const Call& call, const OuterProblem& p, const std::string& 
     const Array &out = p.out, &X = p.X, &Y = p.Y;
     const int32_t* offsets = p.offsets;
     const int64_t groups = p.groups, rows = X.shape[0], height = X.shape[1], columns = Y.shape[1];
-    if (groups == 0 || height == 0 || columns == 0 || multiply_outer_mma(call, p, op)) return;
+    if (groups == 0 || height == 0 || columns == 0 || multiply_outer_mma(call, p, op) ||
+        multiply_outer_split(call, p, op))
+        return;
     fits_int32(static_cast<size_t>(groups), "the number of groups", op);
     for_type(X.type, [&](auto zero) {
         using T = decltype(zero);

@@ -8,10 +8,9 @@
 // Rows: a tile begins where its group's rows do, wherever that is; of a tile that reaches past the end of its group the rows
 // behind it are computed and not stored. Outer products: the depth is the group's rows, and of the last stage of a
 // group the rows behind its end are cleared in shared memory before they are multiplied.
-#include "group_tiles.cuh"
+#include "grouped_block.cuh"
 #include "grouped_mma.hpp"
 #include "tensor_map.hpp"
-#include "umma.cuh"
 
 namespace mops_b200 {
 
@@ -50,11 +49,9 @@ CUtensorMap tensor_map_64(int32_t type, const void* data, int64_t inner, int64_t
 
 namespace {
 
-constexpr int kTileRows = 128;
 constexpr int kThreads = 192;   // the copying warp, the multiplying warp, four that store
 constexpr int kStoreWarps = 4;
 constexpr int kStaging = 32 * kBoxRow; // bytes: 32 rows of 64 values, of one warp
-constexpr int kBand = 16;       // tiles of rows that are taken in turn for a tile of columns, so that both stay in L2
 
 // What a block keeps in shared memory.
 template <int kColumns> struct Layout {
@@ -65,74 +62,7 @@ template <int kColumns> struct Layout {
     static constexpr int kBarriersAt = kStagingAt + kStoreWarps * 2 * kStaging;
     static constexpr int kBytes = kBarriersAt + 256 + 1024; // (boxes begin on multiples of 1024 bytes)
     static constexpr unsigned kTmem = 2 * kColumns;         // columns of tensor memory: two accumulators
-};
-
-struct Barriers {
-    uint64_t full[8], empty[8], done[2], free[2];
-    uint32_t tmem;
-    int gave_up;
-};
-
-// Output tiles of a block of `rows` x `columns` tiles, kBand tiles of rows at a time.
-__device__ __forceinline__ void banded(int64_t at, int64_t rows, int64_t columns, int64_t& row, int64_t& column) {
-    const int64_t band = at / (kBand * columns);
-    const int64_t high = min(int64_t(kBand), rows - band * kBand);
-    const int64_t r = at - band * kBand * columns;
-    column = r / high;
-    row = band * kBand + (r - column * high);
-}
-
-// The parts that both kernels share: setting up and leaving, and the turn that each side takes at the ring of stages and
-// at the two accumulators. A wait that runs out is reported, and everybody leaves.
-template <int kColumns> struct Block {
-    using L = Layout<kColumns>;
-    unsigned char* smem;
-    Barriers* b;
-    uint32_t base; // shared-memory address of the stages
-    Status st;
-
-    __device__ Block(unsigned char* raw, const Status& st) : st(st) {
-        smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-        b = reinterpret_cast<Barriers*>(smem + L::kBarriersAt);
-        base = smem_address(smem);
-    }
-    __device__ void begin(int warp) {
-        if (warp == 1) tmem_alloc(&b->tmem, L::kTmem);
-        if (threadIdx.x == 0) {
-            for (int s = 0; s < L::kStages; s++) mbarrier_init(&b->full[s], 1), mbarrier_init(&b->empty[s], 1);
-            for (int a = 0; a < 2; a++) mbarrier_init(&b->done[a], 1), mbarrier_init(&b->free[a], kStoreWarps);
-            b->gave_up = 0;
-            mbarrier_init_fence();
-        }
-        tmem_fence_before_sync();
-        __syncthreads();
-        tmem_fence_after_sync();
-    }
-    __device__ void end(int warp) {
-        tmem_fence_before_sync();
-        __syncthreads();
-        tmem_fence_after_sync();
-        if (warp == 1) tmem_free(b->tmem, L::kTmem);
-    }
-    __device__ bool wait(uint64_t* bar, unsigned parity) {
-        if (*static_cast<volatile int*>(&b->gave_up) == 0 && mbarrier_wait(bar, parity)) return true;
-        if (atomicExch(&b->gave_up, 1) == 0) report_stalled(st);
-        return false;
-    }
-    __device__ uint32_t stage(int64_t i) const { return base + static_cast<uint32_t>(i % L::kStages) * L::kStage; }
-    // The copying thread, before it fills stage i; before it leaves, for the copies that nobody waited for.
-    __device__ bool wait_empty(int64_t i) {
-        return i < L::kStages || wait(&b->empty[i % L::kStages], static_cast<unsigned>(i / L::kStages - 1) & 1);
-    }
-    __device__ void drain(int64_t issued) {
-        if (*static_cast<volatile int*>(&b->gave_up) == 0) return;
-        for (int64_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; i++)
-            (void)mbarrier_wait(&b->full[i % L::kStages], static_cast<unsigned>(i / L::kStages) & 1);
-    }
-    __device__ bool wait_full(int64_t i) { return wait(&b->full[i % L::kStages], static_cast<unsigned>(i / L::kStages) & 1); }
-    __device__ bool wait_free(int64_t tile) { return tile < 2 || wait(&b->free[tile & 1], static_cast<unsigned>(tile / 2 - 1) & 1); }
-    __device__ bool wait_done(int64_t tile) { return wait(&b->done[tile & 1], static_cast<unsigned>(tile / 2) & 1); }
-    __device__ uint32_t accumulator(int64_t tile) const { return b->tmem + static_cast<uint32_t>(tile & 1) * kColumns; }
+    static constexpr unsigned kFillers = 1, kStorers = kStoreWarps;
 };
 
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
@@ -191,7 +121,7 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     extern __shared__ unsigned char raw[];
     using L = Layout<kColumns>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Block<kColumns> block(raw, st);
+    Block<L> block(raw, st);
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
@@ -279,33 +209,6 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 }
 
 // ------------------------------------------------------------------------- outer products
-// A group's rows are cut into segments of `segment` rows; the pieces of work are (segment, tile of the output). A group of more than one segment
-// leaves its tiles in `parts`, in f32, one after the other, and grouped_outer_join adds them up.
-struct OuterPieces {
-    int64_t segment, tiles;
-    __device__ int64_t operator()(int64_t rows) const { return max((rows + segment - 1) / segment, int64_t(1)) * tiles; }
-};
-struct OuterParts { // of those, the ones that are left in parts
-    int64_t segment, tiles;
-    __device__ int64_t operator()(int64_t rows) const { return rows > segment ? (rows + segment - 1) / segment * tiles : 0; }
-};
-struct OuterJoins {
-    int64_t segment, tiles;
-    __device__ int64_t operator()(int64_t rows) const { return rows > segment ? tiles : 0; }
-};
-
-// How many parts the groups in front of `group` leave (a warp together).
-__device__ __forceinline__ int64_t parts_before(const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int64_t group,
-                                                OuterParts parts, int lane) {
-    int64_t n = 0;
-    for (int64_t g = lane; g < group; g += 32) {
-        int64_t lo, hi;
-        group_bounds(offsets, groups, rows, g, lo, hi);
-        n += parts(hi - lo);
-    }
-    return warp_sum(n);
-}
-
 // out[g] = X[rows of g]^T Y[rows of g].
 template <bool BF16, int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -316,7 +219,7 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     extern __shared__ unsigned char raw[];
     using L = Layout<kColumns>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Block<kColumns> block(raw, st);
+    Block<L> block(raw, st);
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
@@ -437,42 +340,6 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     block.end(warp);
 }
 
-// Adds up the parts of a tile, in the order of the rows.
-template <typename T, int kColumns>
-__global__ void __launch_bounds__(256)
-grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t most_parts,
-                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment) {
-    const int lane = threadIdx.x & 31;
-    const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
-    const int64_t tiles = row_tiles * column_tiles;
-    GroupWalk<OuterJoins> walk(offsets, groups, rows, 0, groups - 1, OuterJoins{segment, tiles});
-    const GroupPiece piece = walk.find(blockIdx.x, lane);
-    if (!piece.found) return;
-    int64_t tile_row, tile_column;
-    banded(piece.within, row_tiles, column_tiles, tile_row, tile_column);
-    const int row = static_cast<int>(tile_row) * kTileRows, column = static_cast<int>(tile_column) * kColumns;
-    const int64_t n = (piece.hi - piece.lo + segment - 1) / segment;
-    const int64_t first = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
-    if (first + (n - 1) * tiles >= most_parts) return;
-    constexpr int kSplit = 8; // blocks to a tile
-    constexpr int kValues = kTileRows * kColumns / kSplit;
-    for (int at = blockIdx.y * kValues + threadIdx.x * 4; at < (blockIdx.y + 1) * kValues; at += 256 * 4) {
-        const int i = at / kColumns, j = at % kColumns;
-        if (row + i >= height || column + j >= columns) continue;
-        float4 sum = make_float4(0, 0, 0, 0);
-        const float* from = parts + (first * kTileRows + i) * kColumns + j;
-        for (int64_t s = 0; s < n; s++) {
-            const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kTileRows * kColumns);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-        }
-        T* to = out + (piece.group * height + row + i) * columns + column + j;
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (column + j + k < columns) to[k] = narrow<T>(v[k]);
-    }
-}
-
 // Whether the copy engine can fetch an array of 16-bit values by its rows.
 bool boxable(const void* data, int64_t outer, int64_t outer_stride, int64_t inner, int64_t slices, int64_t slice_stride) {
     return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (outer == 1 || (outer_stride % 8 == 0 && outer_stride >= inner)) &&
@@ -539,10 +406,7 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         const CUtensorMap y = tensor_map_64(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, 64);
         const CUtensorMap out = tensor_map_64(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
         const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
-        // Segments such that, were all rows in one group, there would be some four pieces of work for each SM; so no block has much more
-        // than its share, and few tiles are left in parts where there are many groups.
-        const int64_t segment = std::max<int64_t>(ceil_div(rows * tiles, int64_t(sms) * 4 * 64) * 64, 256);
-        const int64_t most_parts = tiles * (rows / segment * 2);
+        const int64_t segment = outer_segment(rows, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
         float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
                                       : nullptr;
         auto kernel = grouped_outer_mma<BF16, kColumns>;
@@ -551,10 +415,7 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
             x, y, out, parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment, call.status);
         if (rows > segment) {
-            const int64_t joins = tiles * std::min<int64_t>(p.groups, rows / segment);
-            fits_int32(static_cast<size_t>(joins), "the number of tiles", op);
-            grouped_outer_join<T, kColumns><<<dim3(static_cast<unsigned>(joins), 8), 256, 0, call.stream>>>(
-                static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment);
+            join_outer<T, kColumns>(call, p, parts, most_parts, tiles, segment, op);
             scratch_free(call, parts);
         }
         note_kernel_f("grouped_outer_mma<%s,%d>", BF16 ? "bf16" : "f16", kColumns);

@@ -23,6 +23,9 @@ struct OuterProblem {
 
 bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string& op);
 bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::string& op);
+// The same for f32 and for arrays that the copy engine cannot fetch (grouped_split.cu).
+bool multiply_rows_split(const Call& call, const RowsProblem& p, const std::string& op);
+bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::string& op);
 
 } // namespace mops_b200
 
