@@ -4,12 +4,14 @@
 //   grad_A[r,:] = grad_output[r,:] W[g,:,:]^T
 //   grad_W[g]   = A[rows of g]^T grad_output[rows of g]
 //
-// The products here run on the ordinary arithmetic units: a block computes a tile of 64 x 64 values, 4 x 4 of them per thread in
-// registers, from slices of 16 that both operands leave in shared memory.
+// The products of 16 and 32 bits run on the tensor cores (grouped_mma.cu, grouped_split.cu). Those of f64 are computed here, by the ordinary
+// arithmetic units, which are as fast as the tensor cores for f64: a block computes a tile of 64 x 64 values, 4 x 4 of them per
+// thread in registers, from slices of 16 that both operands leave in shared memory. So are the zeros of empty sums.
 #include "arrays.hpp"
 #include "block_ops.hpp"
 #include "group_tiles.cuh"
 #include "grouped_mma.hpp"
+#include "pack.hpp"
 
 namespace mops_b200 {
 namespace {
@@ -179,6 +181,11 @@ void check_matrices(const Array& W, const char* name, const std::string& op) {
         throw std::runtime_error(std::string(name) + " must have a stride of 1 in one of its last two dimensions in " + op);
 }
 
+// Whether there are products to compute that the tensor cores take on (the other problems go to the kernels of this file).
+bool on_tensor_cores(const Array& A, const Array& W) {
+    return A.type != MOPS_B200_F64 && A.shape[0] > 0 && A.shape[1] > 0 && W.shape[0] > 0 && W.shape[2] > 0;
+}
+
 } // namespace
 
 void grouped_matrix_product(Array output, Array A, Array W, Array offsets) {
@@ -188,10 +195,17 @@ void grouped_matrix_product(Array output, Array A, Array W, Array offsets) {
     check_output(output, "output", op);
     if (output.shape[0] == 0 || output.shape[1] == 0) return;
     Call call = begin_call();
+    Packing packing(call);
+    if (on_tensor_cores(A, W)) {
+        packing.add(A);
+        packing.add(W);
+        packing.run();
+    }
     multiply_rows(call,
                   {output, A, W, W.stride[1], W.stride[2], static_cast<const int32_t*>(offsets.data), W.shape[0], A.shape[0],
                    A.shape[1], W.shape[2]},
                   op);
+    packing.release();
     end_call(call, op.c_str(), kIndexNames, 1);
 }
 
@@ -216,6 +230,13 @@ void grouped_matrix_product_vjp(Array grad_A, Array grad_W, Array grad_output, A
     }
     if (!need_A && !need_W) return;
     Call call = begin_call();
+    Packing packing(call);
+    if (on_tensor_cores(A, W)) {
+        packing.add(grad_output);
+        if (need_A) packing.add(W);
+        if (need_W) packing.add(A);
+        packing.run();
+    }
     const int32_t* starts = static_cast<const int32_t*>(offsets.data);
     if (need_A)
         multiply_rows(call,
@@ -225,6 +246,7 @@ void grouped_matrix_product_vjp(Array grad_A, Array grad_W, Array grad_output, A
         if (turned) multiply_outer(call, {grad_W, grad_output, A, starts, W.shape[0]}, op);
         else multiply_outer(call, {grad_W, A, grad_output, starts, W.shape[0]}, op);
     }
+    packing.release();
     end_call(call, op.c_str(), kIndexNames, 1);
 }
 

@@ -14,10 +14,21 @@ namespace mops_b200 {
 constexpr int kTileRows = 128;
 constexpr int kBand = 16; // tiles of rows that are taken in turn for a tile of columns, so that both stay in L2
 
-struct Barriers {
-    uint64_t full[8], empty[8], done[2], free[2];
-    uint32_t tmem;
-    int gave_up;
+// Whose turn it is in a ring of N places: a place and the parity of the round.
+template <int N> struct Turn {
+    int at = 0;
+    unsigned round = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) at = 0, round ^= 1;
+    }
+};
+
+// Between those who fill the places of a ring and those who empty them.
+template <int N> struct Ring {
+    uint64_t full[N], empty[N];
+    __device__ void begin(unsigned fillers, unsigned emptiers) {
+        for (int i = 0; i < N; i++) mbarrier_init(&full[i], fillers), mbarrier_init(&empty[i], emptiers);
+    }
 };
 
 // Output tiles of a block of `rows` x `columns` tiles, kBand tiles of rows at a time.
@@ -29,26 +40,24 @@ __device__ __forceinline__ void banded(int64_t at, int64_t rows, int64_t columns
     row = band * kBand + (r - column * high);
 }
 
-// What the kernels share: setting up and leaving, and the turn that each side takes at the ring of stages and at the two accumulators. A
-// wait that runs out is reported, and everybody leaves. L says how shared and tensor memory are laid out, how many arrivals fill
-// a stage and how many free an accumulator.
+// What the kernels share: setting up, waiting and leaving. A wait that runs out is reported, and everybody leaves. L says how shared memory is
+// laid out, how many columns of tensor memory there are, and what the rings are (L::Rings, with begin(), `tmem` and `gave_up`).
 template <typename L> struct Block {
     unsigned char* smem;
-    Barriers* b;
+    typename L::Rings* rings;
     uint32_t base; // shared-memory address of the stages
     Status st;
 
     __device__ Block(unsigned char* raw, const Status& st) : st(st) {
         smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-        b = reinterpret_cast<Barriers*>(smem + L::kBarriersAt);
+        rings = reinterpret_cast<typename L::Rings*>(smem + L::kRingsAt);
         base = smem_address(smem);
     }
     __device__ void begin(int warp) {
-        if (warp == 1) tmem_alloc(&b->tmem, L::kTmem);
+        if (warp == 1) tmem_alloc(&rings->tmem, L::kTmem);
         if (threadIdx.x == 0) {
-            for (int s = 0; s < L::kStages; s++) mbarrier_init(&b->full[s], L::kFillers), mbarrier_init(&b->empty[s], 1);
-            for (int a = 0; a < 2; a++) mbarrier_init(&b->done[a], 1), mbarrier_init(&b->free[a], L::kStorers);
-            b->gave_up = 0;
+            rings->begin();
+            rings->gave_up = 0;
             mbarrier_init_fence();
         }
         tmem_fence_before_sync();
@@ -59,27 +68,32 @@ template <typename L> struct Block {
         tmem_fence_before_sync();
         __syncthreads();
         tmem_fence_after_sync();
-        if (warp == 1) tmem_free(b->tmem, L::kTmem);
+        if (warp == 1) tmem_free(rings->tmem, L::kTmem);
     }
-    __device__ bool wait(uint64_t* bar, unsigned parity) {
-        if (*static_cast<volatile int*>(&b->gave_up) == 0 && mbarrier_wait(bar, parity)) return true;
-        if (atomicExch(&b->gave_up, 1) == 0) report_stalled(st);
+    __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity) {
+        if (mbarrier_try_wait(bar, parity)) return true;
+        if (*static_cast<volatile int*>(&rings->gave_up) == 0 && mbarrier_wait(bar, parity)) return true;
+        if (atomicExch(&rings->gave_up, 1) == 0) report_stalled(st);
         return false;
     }
-    __device__ uint32_t stage(int64_t i) const { return base + static_cast<uint32_t>(i % L::kStages) * L::kStage; }
-    // The copying thread, before it fills stage i; before it leaves, for the copies that nobody waited for.
-    __device__ bool wait_empty(int64_t i) {
-        return i < L::kStages || wait(&b->empty[i % L::kStages], static_cast<unsigned>(i / L::kStages - 1) & 1);
+    template <int N> __device__ __forceinline__ bool wait_full(Ring<N>& ring, const Turn<N>& turn) {
+        return wait(&ring.full[turn.at], turn.round);
     }
-    __device__ void drain(int64_t issued) {
-        if (*static_cast<volatile int*>(&b->gave_up) == 0) return;
-        for (int64_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; i++)
-            (void)mbarrier_wait(&b->full[i % L::kStages], static_cast<unsigned>(i / L::kStages) & 1);
+    template <int N> __device__ __forceinline__ bool wait_empty(Ring<N>& ring, const Turn<N>& turn) { // (a fresh one is empty)
+        return wait(&ring.empty[turn.at], turn.round ^ 1);
     }
-    __device__ bool wait_full(int64_t i) { return wait(&b->full[i % L::kStages], static_cast<unsigned>(i / L::kStages) & 1); }
-    __device__ bool wait_free(int64_t tile) { return tile < 2 || wait(&b->free[tile & 1], static_cast<unsigned>(tile / 2 - 1) & 1); }
-    __device__ bool wait_done(int64_t tile) { return wait(&b->done[tile & 1], static_cast<unsigned>(tile / 2) & 1); }
-    __device__ uint32_t accumulator(int64_t tile) const { return b->tmem + static_cast<uint32_t>(tile & 1) * (L::kTmem / 2); }
+    // The copying thread, before it leaves when somebody gave up: the copies that may be under way, at most one for each place. A place
+    // that has none is full or waits in vain.
+    template <int N> __device__ void drain(Ring<N>& ring, Turn<N> turn, int64_t issued) {
+        if (*static_cast<volatile int*>(&rings->gave_up) == 0) return;
+        for (int i = 0; i < N && i < issued; i++) {
+            // the place before this turn, filled in its round
+            turn.at = turn.at == 0 ? N - 1 : turn.at - 1;
+            if (turn.at == N - 1) turn.round ^= 1;
+            (void)mbarrier_wait(&ring.full[turn.at], turn.round);
+        }
+    }
+    __device__ uint32_t accumulator(const Turn<2>& turn) const { return rings->tmem + static_cast<uint32_t>(turn.at) * (L::kTmem / 2); }
 };
 
 // A group's rows are cut into segments of `segment` rows; the pieces of work are (segment, tile of the output). A group of more than one segment
@@ -126,23 +140,29 @@ grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t
     const int64_t n = (piece.hi - piece.lo + segment - 1) / segment;
     const int64_t first = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
     if (first + (n - 1) * tiles >= most_parts) return;
-    constexpr int kSplit = 8; // blocks to a tile
-    constexpr int kValues = kTileRows * kColumns / kSplit;
-    for (int at = blockIdx.y * kValues + threadIdx.x * 4; at < (blockIdx.y + 1) * kValues; at += 256 * 4) {
-        const int i = at / kColumns, j = at % kColumns;
-        if (row + i >= height || column + j >= columns) continue;
-        float4 sum = make_float4(0, 0, 0, 0);
-        const float* from = parts + (first * kTileRows + i) * kColumns + j;
-        for (int64_t s = 0; s < n; s++) {
-            const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kTileRows * kColumns);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-        }
-        T* to = out + (piece.group * height + row + i) * columns + column + j;
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    // four values to a thread
+    const int at = (blockIdx.y * 256 + threadIdx.x) * 4, i = at / kColumns, j = at % kColumns;
+    if (row + i >= height || column + j >= columns) return;
+    const float* from = parts + (first * kTileRows + i) * kColumns + j;
+    float4 sum = make_float4(0, 0, 0, 0);
+    int64_t s = 0;
+    constexpr int kInFlight = 8;
+    for (; s + kInFlight <= n; s += kInFlight) {
+        float4 v[kInFlight];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (column + j + k < columns) to[k] = narrow<T>(v[k]);
+        for (int k = 0; k < kInFlight; k++) v[k] = *reinterpret_cast<const float4*>(from + (s + k) * tiles * kTileRows * kColumns);
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
     }
+    for (; s < n; s++) {
+        const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kTileRows * kColumns);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    T* to = out + (piece.group * height + row + i) * columns + column + j;
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (column + j + k < columns) to[k] = narrow<T>(v[k]);
 }
 
 // Segments such that, were all rows in one group, there would be some four pieces of work for each SM; so no block has much more than its share,
@@ -158,7 +178,7 @@ void join_outer(const Call& call, const OuterProblem& p, const float* parts, int
                 const std::string& op) {
     const int64_t rows = p.X.shape[0], joins = tiles * std::min<int64_t>(p.groups, rows / segment);
     fits_int32(static_cast<size_t>(joins), "the number of tiles", op);
-    grouped_outer_join<T, kColumns><<<dim3(static_cast<unsigned>(joins), 8), 256, 0, call.stream>>>(
+    grouped_outer_join<T, kColumns><<<dim3(static_cast<unsigned>(joins), kTileRows * kColumns / 1024), 256, 0, call.stream>>>(
         static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(p.X.shape[1]),
         static_cast<int>(p.Y.shape[1]), segment);
     MOPS_CUDA_OK(cudaGetLastError());

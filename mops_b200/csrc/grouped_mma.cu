@@ -15,39 +15,6 @@
 namespace mops_b200 {
 
 namespace {
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-    static const EncodeTiled f = [] {
-        void* entry = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        MOPS_CUDA_OK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &found));
-        if (entry == nullptr) throw std::runtime_error("the driver has no cuTensorMapEncodeTiled");
-        return reinterpret_cast<EncodeTiled>(entry);
-    }();
-    return f;
-}
-} // namespace
-
-CUtensorMap tensor_map_64(int32_t type, const void* data, int64_t inner, int64_t outer, int64_t slices,
-                          int64_t outer_stride, int64_t slice_stride, int box) {
-    CUtensorMap map;
-    // strides of dimensions of size 1 mean nothing, but have to look well
-    if (outer == 1) outer_stride = ceil_div(inner, 8) * 8;
-    if (slices == 1) slice_stride = outer * outer_stride;
-    const cuuint64_t size[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(slices)};
-    const cuuint64_t stride[2] = {static_cast<cuuint64_t>(outer_stride) * 2, static_cast<cuuint64_t>(slice_stride) * 2};
-    const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
-    const CUresult r = encode_tiled()(&map, type == MOPS_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                                      3, const_cast<void*>(data), size, stride, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        throw std::runtime_error("CUDA error: cuTensorMapEncodeTiled returned " + std::to_string(static_cast<int>(r)));
-    return map;
-}
-
-namespace {
 
 constexpr int kThreads = 192;   // the copying warp, the multiplying warp, four that store
 constexpr int kStoreWarps = 4;
@@ -59,10 +26,20 @@ template <int kColumns> struct Layout {
     static constexpr int kA = kTileRows * kBoxRow, kB = kColumns * kBoxRow; // bytes of a stage
     static constexpr int kStage = kA + kB;
     static constexpr int kStagingAt = kStages * kStage;
-    static constexpr int kBarriersAt = kStagingAt + kStoreWarps * 2 * kStaging;
-    static constexpr int kBytes = kBarriersAt + 256 + 1024; // (boxes begin on multiples of 1024 bytes)
-    static constexpr unsigned kTmem = 2 * kColumns;         // columns of tensor memory: two accumulators
-    static constexpr unsigned kFillers = 1, kStorers = kStoreWarps;
+    static constexpr int kRingsAt = kStagingAt + kStoreWarps * 2 * kStaging;
+    static constexpr int kBytes = kRingsAt + 256 + 1024; // (boxes begin on multiples of 1024 bytes)
+    static constexpr unsigned kTmem = 2 * kColumns;      // columns of tensor memory: two accumulators
+    struct Rings {
+        Ring<kStages> stages;
+        Ring<2> accumulators;
+        uint32_t tmem;
+        int gave_up;
+        __device__ void begin() {
+            stages.begin(1, 1);
+            accumulators.begin(1, kStoreWarps);
+        }
+    };
+    static_assert(sizeof(Rings) <= 256, "room for the rings");
 };
 
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
@@ -75,11 +52,11 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint
     }
 }
 
-// Writes the 64 columns that follow `column` of a warp's 32 rows of an accumulator: a whole band by the copy engine, of a band that the group's
-// end cuts (`here` rows) each lane its row.
+// Writes the 64 columns that follow `column` of a warp's 32 rows of an accumulator, `here` of which are the group's: all of them by the copy engine,
+// fewer each lane its row. Where rows of the output begin anywhere (loose), a row after the other, value by value. out: the first row of the band.
 template <bool BF16>
 __device__ __forceinline__ void store_columns(uint32_t accumulator, uint32_t staging, int64_t& sent, const CUtensorMap& map,
-                                              uint16_t* __restrict__ out, int64_t row, int slice, int column, int64_t columns, int here,
+                                              uint16_t* __restrict__ out, int row, int slice, int column, int columns, int here, bool loose,
                                               int lane) {
     uint32_t r[2][32];
     tmem_load(accumulator, r[0]);
@@ -93,18 +70,31 @@ __device__ __forceinline__ void store_columns(uint32_t accumulator, uint32_t sta
         const uint32_t* w = &r[c / 4][c % 4 * 8];
         v[c] = make_uint4(pack2<BF16>(w[0], w[1]), pack2<BF16>(w[2], w[3]), pack2<BF16>(w[4], w[5]), pack2<BF16>(w[6], w[7]));
     }
-    if (here == 32) {
+    if (loose || here == 32) {
         const uint32_t to = staging + static_cast<uint32_t>(sent & 1) * kStaging;
-        if (lane == 0) boxes_left<1>();
+        if (!loose && lane == 0) boxes_left<1>();
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < 8; c++) smem_store16(to + lane * kBoxRow + ((c ^ (lane & 7)) << 4), v[c]);
-        async_proxy_fence();
-        __syncwarp();
-        if (lane == 0) box_out(map, column, static_cast<int>(row), slice, to);
+        if (loose) {
+            __syncwarp();
+            const int wide = columns - column;
+            for (int i = 0; i < here; i++) {
+                uint16_t* p = out + static_cast<int64_t>(i) * columns + column;
+#pragma unroll
+                for (int h = 0; h < 64; h += 32) {
+                    const int c = h + lane;
+                    if (c < wide) p[c] = smem_load2(to + i * kBoxRow + ((c / 8 ^ (i & 7)) << 4) + c % 8 * 2);
+                }
+            }
+        } else {
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) box_out(map, column, row, slice, to);
+        }
         sent++;
     } else if (lane < here) {
-        uint4* to = reinterpret_cast<uint4*>(out + (row + lane) * columns + column);
+        uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(lane) * columns + column);
 #pragma unroll
         for (int c = 0; c < 8; c++)
             if (column + c * 8 < columns) to[c] = v[c]; // (columns are a multiple of 8 here)
@@ -117,7 +107,7 @@ template <bool BF16, bool M_MN, int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m,
                  const __grid_constant__ CUtensorMap map_out, uint16_t* __restrict__ out, const int32_t* __restrict__ offsets,
-                 int64_t groups, int64_t rows, int depth, int columns, Status st) {
+                 int64_t groups, int64_t rows, int depth, int columns, bool loose, Status st) {
     extern __shared__ unsigned char raw[];
     using L = Layout<kColumns>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -128,8 +118,10 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const int64_t column_tiles = (columns + kColumns - 1) / kColumns;
     const int steps = (depth + kBoxDepth - 1) / kBoxDepth;
     GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{kTileRows, column_tiles});
-    int64_t step = 0, tile = 0; // so far
-    int64_t sent = 0;           // boxes that this warp has stored
+    Turn<L::kStages> stage;
+    Turn<2> tile;     // accumulator
+    int64_t sent = 0; // boxes that this warp has fetched or stored
+    auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
     for (int64_t want = blockIdx.x;; want += gridDim.x) {
         const GroupPiece piece = walk.find(want, lane);
         if (!piece.found) break;
@@ -141,11 +133,11 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         bool ok = true;
         if (warp == 0) {
             if (lane == 0 && in_group) {
-                for (int s = 0; s < steps && ok; s++, step++) {
-                    ok = block.wait_empty(step);
+                for (int s = 0; s < steps && ok; s++) {
+                    ok = block.wait_empty(block.rings->stages, stage);
                     if (!ok) break;
-                    uint64_t* full = &block.b->full[step % L::kStages];
-                    const uint32_t a = block.stage(step), b = a + L::kA;
+                    uint64_t* full = &block.rings->stages.full[stage.at];
+                    const uint32_t a = stage_at(), b = a + L::kA;
                     mbarrier_arrive_expect(full, L::kStage);
                     box_in(a, map_x, s * kBoxDepth, static_cast<int>(row), 0, full);
                     if constexpr (M_MN) {
@@ -155,26 +147,29 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     } else {
                         box_in(b, map_m, s * kBoxDepth, column, static_cast<int>(piece.group), full);
                     }
+                    stage.next();
+                    sent++;
                 }
             }
         } else if (warp == 1) {
             if (lane == 0 && in_group) {
                 constexpr uint32_t instruction = instruction_descriptor(BF16, false, M_MN, kColumns);
-                ok = block.wait_free(tile);
+                ok = block.wait_empty(block.rings->accumulators, tile);
                 tmem_fence_after_sync();
-                for (int s = 0; s < steps && ok; s++, step++) {
-                    ok = block.wait_full(step);
+                for (int s = 0; s < steps && ok; s++) {
+                    ok = block.wait_full(block.rings->stages, stage);
                     if (!ok) break;
                     tmem_fence_after_sync();
-                    const uint64_t a = operand_descriptor(block.stage(step), kBoxBytes);
-                    const uint64_t b = operand_descriptor(block.stage(step) + L::kA, kBoxBytes);
+                    const uint64_t a = operand_descriptor(stage_at(), kBoxBytes);
+                    const uint64_t b = operand_descriptor(stage_at() + L::kA, kBoxBytes);
 #pragma unroll
                     for (int k = 0; k < kBoxDepth / 16; k++)
                         umma(block.accumulator(tile), a + k * kDepthStep<false>, b + k * kDepthStep<M_MN>, instruction, s + k > 0);
-                    umma_arrive(&block.b->empty[step % L::kStages]);
+                    umma_arrive(&block.rings->stages.empty[stage.at]);
+                    stage.next();
                 }
-                if (ok) umma_arrive(&block.b->done[tile & 1]);
-                tile++;
+                if (ok) umma_arrive(&block.rings->accumulators.full[tile.at]);
+                tile.next();
             }
         } else {
             const int quadrant = warp & 3;
@@ -182,27 +177,28 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             const int here = static_cast<int>(min(max(piece.hi - band, int64_t(0)), int64_t(32)));
             const int wide = min(columns - column, kColumns);
             if (in_group) {
-                ok = block.wait_done(tile);
+                ok = block.wait_full(block.rings->accumulators, tile);
                 if (ok) {
                     tmem_fence_after_sync();
                     const uint32_t from = tmem_quadrant(block.accumulator(tile), quadrant);
                     const uint32_t staging = block.base + L::kStagingAt + quadrant * 2 * kStaging;
                     if (here > 0)
                         for (int c = 0; c < wide; c += 64)
-                            store_columns<BF16>(from + c, staging, sent, map_out, out, band, 0, column + c, columns, here, lane);
+                            store_columns<BF16>(from + c, staging, sent, map_out, out + band * columns, static_cast<int>(band), 0, column + c,
+                                                        columns, here, loose, lane);
                     tmem_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbarrier_arrive(&block.b->free[tile & 1]);
+                    if (lane == 0) mbarrier_arrive(&block.rings->accumulators.empty[tile.at]);
                 }
-                tile++;
-            } else if (lane < here) { // rows of no group
-                uint4* to = reinterpret_cast<uint4*>(out + (band + lane) * columns + column);
-                for (int c = 0; c < wide / 8; c++) to[c] = make_uint4(0, 0, 0, 0);
+                tile.next();
+            } else { // rows of no group
+                for (int i = 0; i < here; i++)
+                    for (int c = lane; c < wide; c += 32) out[(band + i) * columns + column + c] = 0;
             }
         }
         if (!__shfl_sync(kFullMask, ok, 0)) break;
     }
-    if (warp == 0 && lane == 0) block.drain(step);
+    if (warp == 0 && lane == 0) block.drain(block.rings->stages, stage, sent);
     if (warp >= 2 && lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
@@ -213,9 +209,9 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 template <bool BF16, int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
-                  const __grid_constant__ CUtensorMap map_out, float* __restrict__ parts, int64_t most_parts,
+                  const __grid_constant__ CUtensorMap map_out, uint16_t* __restrict__ out, float* __restrict__ parts, int64_t most_parts,
                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment,
-                  Status st) {
+                  bool loose, Status st) {
     extern __shared__ unsigned char raw[];
     using L = Layout<kColumns>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -226,7 +222,10 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
     const int64_t tiles = row_tiles * column_tiles;
     GroupWalk<OuterPieces> walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles});
-    int64_t step = 0, tile = 0, sent = 0;
+    Turn<L::kStages> stage;
+    Turn<2> tile;
+    int64_t sent = 0;
+    auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
     for (int64_t want = blockIdx.x;; want += gridDim.x) {
         const GroupPiece piece = walk.find(want, lane);
         if (!piece.found) break;
@@ -239,56 +238,59 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         bool ok = true;
         if (warp == 0) {
             if (lane == 0) {
-                for (int s = 0; s < steps && ok; s++, step++) {
-                    ok = block.wait_empty(step);
+                for (int s = 0; s < steps && ok; s++) {
+                    ok = block.wait_empty(block.rings->stages, stage);
                     if (!ok) break;
-                    uint64_t* full = &block.b->full[step % L::kStages];
-                    const uint32_t a = block.stage(step), b = a + L::kA;
+                    uint64_t* full = &block.rings->stages.full[stage.at];
+                    const uint32_t a = stage_at(), b = a + L::kA;
                     const int at = static_cast<int>(lo) + s * kBoxDepth;
                     mbarrier_arrive_expect(full, L::kStage);
 #pragma unroll
                     for (int i = 0; i < kTileRows / 64; i++) box_in(a + i * kBoxBytes, map_x, row + i * 64, at, 0, full);
 #pragma unroll
                     for (int j = 0; j < kColumns / 64; j++) box_in(b + j * kBoxBytes, map_y, column + j * 64, at, 0, full);
+                    stage.next();
+                    sent++;
                 }
             }
         } else if (warp == 1) {
             if (steps > 0) {
                 constexpr uint32_t instruction = instruction_descriptor(BF16, true, true, kColumns);
-                if (lane == 0) ok = block.wait_free(tile);
+                if (lane == 0) ok = block.wait_empty(block.rings->accumulators, tile);
                 ok = __shfl_sync(kFullMask, ok, 0);
                 tmem_fence_after_sync();
-                for (int s = 0; s < steps && ok; s++, step++) {
+                for (int s = 0; s < steps && ok; s++) {
                     const int64_t left = hi - lo - int64_t(s) * kBoxDepth;
-                    if (lane == 0 || left < kBoxDepth) ok = block.wait_full(step);
+                    if (lane == 0 || left < kBoxDepth) ok = block.wait_full(block.rings->stages, stage);
                     ok = __all_sync(kFullMask, ok);
                     if (!ok) break;
                     if (left < kBoxDepth) { // the rows behind are of another group
                         const uint32_t from = static_cast<uint32_t>(left) * kBoxRow;
                         for (uint32_t box = 0; box < L::kStage; box += kBoxBytes)
                             for (uint32_t at = from + lane * 16; at < kBoxBytes; at += 32 * 16)
-                                smem_store16(block.stage(step) + box + at, make_uint4(0, 0, 0, 0));
+                                smem_store16(stage_at() + box + at, make_uint4(0, 0, 0, 0));
                         async_proxy_fence();
                         __syncwarp();
                     }
                     if (lane == 0) {
                         tmem_fence_after_sync();
-                        const uint64_t a = operand_descriptor(block.stage(step), kBoxBytes);
-                        const uint64_t b = operand_descriptor(block.stage(step) + L::kA, kBoxBytes);
+                        const uint64_t a = operand_descriptor(stage_at(), kBoxBytes);
+                        const uint64_t b = operand_descriptor(stage_at() + L::kA, kBoxBytes);
 #pragma unroll
                         for (int k = 0; k < kBoxDepth / 16; k++)
                             umma(block.accumulator(tile), a + k * kDepthStep<true>, b + k * kDepthStep<true>, instruction, s + k > 0);
-                        umma_arrive(&block.b->empty[step % L::kStages]);
+                        umma_arrive(&block.rings->stages.empty[stage.at]);
                     }
+                    stage.next();
                     __syncwarp();
                 }
-                if (lane == 0 && ok) umma_arrive(&block.b->done[tile & 1]);
-                tile++;
+                if (lane == 0 && ok) umma_arrive(&block.rings->accumulators.full[tile.at]);
+                tile.next();
             }
         } else {
             const int quadrant = warp & 3;
             const int band = row + quadrant * 32, wide = min(columns - column, kColumns);
-            if (steps > 0) ok = block.wait_done(tile);
+            if (steps > 0) ok = block.wait_full(block.rings->accumulators, tile);
             if (ok) {
                 const uint32_t from = tmem_quadrant(block.accumulator(tile), quadrant);
                 const uint32_t staging = block.base + L::kStagingAt + quadrant * 2 * kStaging;
@@ -306,44 +308,33 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                         for (int i = 0; i < 8; i++)
                             *reinterpret_cast<uint4*>(to + c + 4 * i) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
                     }
-                } else if (band < height) {
-                    for (int c = 0; c < wide; c += 64) {
-                        if (steps > 0) {
-                            store_columns<BF16>(from + c, staging, sent, map_out, nullptr, band, static_cast<int>(piece.group), column + c,
-                                                columns, 32, lane);
-                        } else { // a group without rows
-                            const uint32_t to = staging + static_cast<uint32_t>(sent & 1) * kStaging;
-                            if (lane == 0) boxes_left<1>();
-                            __syncwarp();
-#pragma unroll
-                            for (int i = 0; i < 8; i++) smem_store16(to + lane * kBoxRow + i * 16, make_uint4(0, 0, 0, 0));
-                            async_proxy_fence();
-                            __syncwarp();
-                            if (lane == 0) box_out(map_out, column + c, band, static_cast<int>(piece.group), to);
-                            sent++;
-                        }
+                } else {
+                    const int here = min(height - band, 32);
+                    uint16_t* to = out + (piece.group * height + band) * static_cast<int64_t>(columns);
+                    if (here > 0 && steps > 0) {
+                        // (the copy engine leaves out what lies behind the output's last row)
+                        for (int c = 0; c < wide; c += 64)
+                            store_columns<BF16>(from + c, staging, sent, map_out, to, band, static_cast<int>(piece.group),
+                                                        column + c, columns, loose ? here : 32, loose, lane);
+                    } else { // a group without rows
+                        for (int i = 0; i < here; i++)
+                            for (int c = lane; c < wide; c += 32) to[static_cast<int64_t>(i) * columns + column + c] = 0;
                     }
                 }
                 if (steps > 0) {
                     tmem_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbarrier_arrive(&block.b->free[tile & 1]);
-                    tile++;
+                    if (lane == 0) mbarrier_arrive(&block.rings->accumulators.empty[tile.at]);
+                    tile.next();
                 }
             }
         }
         if (!__shfl_sync(kFullMask, ok, 0)) break;
     }
-    if (warp == 0 && lane == 0) block.drain(step);
+    if (warp == 0 && lane == 0) block.drain(block.rings->stages, stage, sent);
     if (warp >= 2 && lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
-}
-
-// Whether the copy engine can fetch an array of 16-bit values by its rows.
-bool boxable(const void* data, int64_t outer, int64_t outer_stride, int64_t inner, int64_t slices, int64_t slice_stride) {
-    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (outer == 1 || (outer_stride % 8 == 0 && outer_stride >= inner)) &&
-           (slices == 1 || (slice_stride % 8 == 0 && slice_stride > 0));
 }
 
 } // namespace
@@ -352,25 +343,23 @@ bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string
     if (p.X.type != MOPS_B200_F16 && p.X.type != MOPS_B200_BF16) return false;
     const bool mn = p.column_stride == 1;
     const int64_t stride = mn ? p.depth_stride : p.column_stride; // of M
-    if (p.depth == 0 || p.groups == 0 || p.columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0 ||
-        !boxable(p.X.data, p.rows, p.X.stride[0], p.depth, 1, 0) ||
-        !boxable(p.M.data, mn ? p.depth : p.columns, stride, mn ? p.columns : p.depth, p.groups, p.M.stride[0]))
-        return false;
+    if (p.depth == 0 || p.groups == 0) return false;
+    const bool loose = p.columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
     const int sms = sm_count(call.device);
     auto launch = [&](auto type, auto major, auto width) {
         constexpr bool BF16 = decltype(type)::value, M_MN = decltype(major)::value;
         constexpr int kColumns = decltype(width)::value;
         using L = Layout<kColumns>;
-        const CUtensorMap x = tensor_map_64(p.X.type, p.X.data, p.depth, p.rows, 1, p.X.stride[0], 0, kTileRows);
-        const CUtensorMap m = M_MN ? tensor_map_64(p.X.type, p.M.data, p.columns, p.depth, p.groups, stride, p.M.stride[0], 64)
-                                   : tensor_map_64(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
-        const CUtensorMap out = tensor_map_64(p.X.type, p.out.data, p.columns, p.rows, 1, p.columns, 0, 32);
+        const CUtensorMap x = tensor_map(p.X.type, p.X.data, p.depth, p.rows, 1, p.X.stride[0], 0, kTileRows);
+        const CUtensorMap m = M_MN ? tensor_map(p.X.type, p.M.data, p.columns, p.depth, p.groups, stride, p.M.stride[0], 64)
+                                   : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
+        const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, p.columns, p.rows, 1, p.columns, 0, 32);
         const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
         auto kernel = grouped_rows_mma<BF16, M_MN, kColumns>;
         allow_dynamic_smem(kernel, call.device, L::kBytes);
         kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kThreads, L::kBytes, call.stream>>>(
             x, m, out, static_cast<uint16_t*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth),
-            static_cast<int>(p.columns), call.status);
+            static_cast<int>(p.columns), loose, call.status);
         note_kernel_f("grouped_rows_mma<%s,%s,%d>", BF16 ? "bf16" : "f16", M_MN ? "columns" : "depth", kColumns);
     };
     auto by_width = [&](auto type, auto major) {
@@ -393,18 +382,17 @@ bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string
 bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::string& op) {
     if (p.X.type != MOPS_B200_F16 && p.X.type != MOPS_B200_BF16) return false;
     const int64_t rows = p.X.shape[0], height = p.X.shape[1], columns = p.Y.shape[1];
-    if (rows == 0 || columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0 ||
-        !boxable(p.X.data, rows, p.X.stride[0], height, 1, 0) || !boxable(p.Y.data, rows, p.Y.stride[0], columns, 1, 0))
-        return false;
+    if (rows == 0) return false;
+    const bool loose = columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
     const int sms = sm_count(call.device);
     auto launch = [&](auto type, auto width) {
         constexpr bool BF16 = decltype(type)::value;
         constexpr int kColumns = decltype(width)::value;
         using L = Layout<kColumns>;
         using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
-        const CUtensorMap x = tensor_map_64(p.X.type, p.X.data, height, rows, 1, p.X.stride[0], 0, 64);
-        const CUtensorMap y = tensor_map_64(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, 64);
-        const CUtensorMap out = tensor_map_64(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
+        const CUtensorMap x = tensor_map(p.X.type, p.X.data, height, rows, 1, p.X.stride[0], 0, 64);
+        const CUtensorMap y = tensor_map(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, 64);
+        const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
         const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
         const int64_t segment = outer_segment(rows, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
         float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
@@ -413,7 +401,8 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         allow_dynamic_smem(kernel, call.device, L::kBytes);
         const int64_t pieces = tiles * (rows / segment + p.groups);
         kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
-            x, y, out, parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment, call.status);
+            x, y, out, static_cast<uint16_t*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height),
+            static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {
             join_outer<T, kColumns>(call, p, parts, most_parts, tiles, segment, op);
             scratch_free(call, parts);

@@ -21,9 +21,10 @@ struct OuterProblem {
     int64_t groups;
 };
 
+// On arrays that the copy engine can fetch (pack.hpp); f16 and bf16 in grouped_mma.cu, f32 in grouped_split.cu. false: not taken on
+// (another type, or nothing to multiply).
 bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string& op);
 bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::string& op);
-// The same for f32 and for arrays that the copy engine cannot fetch (grouped_split.cu).
 bool multiply_rows_split(const Call& call, const RowsProblem& p, const std::string& op);
 bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::string& op);
 

@@ -1,248 +1,228 @@
-// grouped_matrix_product on tensor cores for operands that the copy engine cannot bring in as they are: f32, and f16 or bf16 whose rows
-// begin anywhere. Eight warps load the operands, turn them into what the tensor cores take and put that into the ring of
-// stages; the rest is as in grouped_mma.cu.
+// grouped_matrix_product on tensor cores, for f32.
 //
-// f32: a value is split into three bf16 parts of eight bits each, by cutting bits off, so that the parts add up to the value exactly:
-// x = x0 + x1 + x2. Of the nine products of parts the six of up to 2^-16 of the largest are computed, the small ones first (the three left out are about 2^-24 of the
-// result, as a rounding to f32 is). The tensor cores add to their f32 accumulators by cutting off what does not fit, an error of one sign
-// that grows with the number of additions; so an accumulator takes one stage (64 values of depth) and is then added, rounded, to sums in
+// A value is split into three bf16 parts of eight bits each, by cutting bits off, so that the parts add up to the value exactly: x = x0 + x1 +
+// x2. Of the nine products of parts the six of up to 2^-16 of the largest are computed, the small ones first; the three left out are about
+// 2^-24 of the result, as a rounding to f32 is. The tensor cores add to their f32 accumulators by cutting off what does not fit, an error of one sign that
+// grows with the number of additions; so an accumulator takes kRun stages (64 values of depth) and is then added, rounded, to sums in
 // registers. An infinite or NaN operand gives NaN.
+//
+// The copy engine fetches boxes of f32 into one ring of stages; eight warps split them into the parts of a second ring; one thread issues the
+// products; eight warps add up what the accumulators hold and store the tiles. Bounded by shared memory, which moves 13 bytes for each byte of operand: in,
+// out, three halves in, and six times half a byte into each of the products.
+#include <mutex>
+#include <set>
+
 #include "grouped_block.cuh"
 #include "grouped_mma.hpp"
+#include "tensor_map.hpp"
 
 namespace mops_b200 {
 namespace {
 
-constexpr int kFillWarps = 8, kStoreWarps = 8;
-constexpr int kThreads = (1 + kFillWarps + kStoreWarps) * 32;
-constexpr int kFillThreads = kFillWarps * 32;
-constexpr int kMultiplyWarp = kFillWarps;
+constexpr int kSplitWarps = 8, kStoreWarps = 8;
+constexpr int kMultiplyWarp = kSplitWarps + kStoreWarps, kCopyWarp = kMultiplyWarp + 1;
+constexpr int kThreads = (kMultiplyWarp + 4) * 32; // (registers are dealt out to four warps at a time)
+constexpr int kSplitThreads = kSplitWarps * 32;
+constexpr int kDepth = 32; // values of depth in a stage: a row of 128 bytes in f32
+constexpr int kRun = 2;    // stages that an accumulator takes
+constexpr int kParts = 3;
 
-template <int kColumns, int kParts> struct Layout {
-    static constexpr int kA = kTileRows * kBoxRow, kB = kColumns * kBoxRow; // bytes of one part of a stage
-    static constexpr int kStage = kParts * (kA + kB);
-    static constexpr int kStages = kParts == 3 ? 2 : kColumns == 128 ? 6 : 8;
-    static constexpr int kStagingAt = kStages * kStage;
-    static constexpr int kStaging = 32 * 33 * 4; // bytes: 32 x 32 sums of one warp, rows one word apart in banks
-    static constexpr int kBarriersAt = kStagingAt + kStoreWarps * kStaging;
-    static constexpr int kBytes = kBarriersAt + 256 + 1024;
+// Registers per thread: those who store hold a tile's sums, the others need few. What the parts take adds up to what the block is launched
+// with (check_registers).
+constexpr int kLaunchRegisters = 96, kSplitRegisters = 80, kStoreRegisters = 120, kMultiplyRegisters = 64;
+static_assert(kSplitWarps * kSplitRegisters + kStoreWarps * kStoreRegisters + 4 * kMultiplyRegisters <= kThreads / 32 * kLaunchRegisters,
+              "a block cannot have more registers than it is launched with");
+template <int kRegisters> __device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegisters));
+}
+template <int kRegisters> __device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegisters));
+}
+
+template <int kColumns> struct Layout {
+    static constexpr int kRawA = kTileRows * kDepth * 4, kRawB = kColumns * kDepth * 4; // bytes of a stage of f32
+    static constexpr int kA = kRawA / 2, kB = kRawB / 2;                                // of one part
+    static constexpr int kRaw = kRawA + kRawB, kStage = kParts * (kA + kB);
+    static constexpr int kRaws = kColumns == 128 ? 3 : 4, kStages = 2;
+    static constexpr int kStagesAt = kRaws * kRaw;
+    static constexpr int kStaging = 32 * 33 * 4; // bytes: 32 x 32 sums of a warp; rows begin one bank apart
+    static constexpr int kStagingAt = kStagesAt + kStages * kStage;
+    static constexpr int kRingsAt = kStagingAt + kStoreWarps * kStaging;
+    static constexpr int kBytes = kRingsAt + 256 + 1024;
     static constexpr unsigned kTmem = 2 * kColumns;
-    static constexpr unsigned kFillers = kFillWarps, kStorers = kStoreWarps;
+    struct Rings {
+        Ring<kRaws> raws;
+        Ring<kStages> stages;
+        Ring<2> accumulators;
+        int valid[kRaws]; // rows of depth that a raw stage has (MN-major); -1: there are no more
+        uint32_t tmem;
+        int gave_up;
+        __device__ void begin() {
+            raws.begin(1, kSplitWarps);
+            stages.begin(kSplitWarps, 1);
+            accumulators.begin(1, kStoreWarps);
+        }
+    };
+    static_assert(sizeof(Rings) <= 256, "room for the rings");
 };
 
-// ------------------------------------------------------------------ bringing operands in
-// A chunk is eight neighbouring values, 16 bytes of a row of a stage.
-template <typename T> struct Chunk {
-    static constexpr int kWords = 8 * sizeof(T) / 4;
-    uint32_t w[kWords];
-};
+// Operands of a stage. In f32: boxes of rows of 128 bytes, swizzled, K-major one of kRows rows, MN-major one for each 32 rows or columns, 32 rows of depth high.
+// In parts: K-major kRows rows of 64 bytes, MN-major boxes of 64 rows or columns, 32 rows of 128 bytes.
+template <bool MN, int kRows> struct Operand {
+    static constexpr int kChunks = kRows * kDepth / 8 / kSplitThreads; // of eight values, of a thread
+    static constexpr int kPart = kRows * kDepth * 2;
+    static constexpr int kBoxHeight = MN ? kDepth : kRows, kBoxes = MN ? kRows / 32 : 1;
+    static constexpr int kPartRow = MN ? 128 : 64;
+    static constexpr uint64_t kStep = (MN ? 16 * 128 : 32) >> 4; // 16 values of depth, in a descriptor
 
-// n values (at most eight; none if n <= 0) from p, zeros behind them. [begin, end): the bytes that the array reaches over. Loads are of
-// 16 bytes, at multiples of 16 and inside of the array; near its ends, value by value.
-template <typename T>
-__device__ __forceinline__ void load_chunk(Chunk<T>& c, const T* p, int n, const unsigned char* begin, const unsigned char* end) {
-    constexpr int kWords = Chunk<T>::kWords;
-    n = min(n, 8);
-#pragma unroll
-    for (int i = 0; i < kWords; i++) c.w[i] = 0;
-    if (n <= 0) return;
-    const unsigned char* at = reinterpret_cast<const unsigned char*>(p);
-    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
-    const unsigned char* from = at - shift;
-    const int vectors = (shift + n * static_cast<int>(sizeof(T)) + 15) / 16;
-    if (from >= begin && from + 16 * vectors <= end) {
-        uint32_t w[kWords + 4];
-#pragma unroll
-        for (int v = 0; v < kWords / 4 + 1; v++) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (v < vectors) u = __ldg(reinterpret_cast<const uint4*>(from) + v);
-            w[4 * v] = u.x, w[4 * v + 1] = u.y, w[4 * v + 2] = u.z, w[4 * v + 3] = u.w;
-        }
-        // shift the words down by 8, 4 and 2 bytes as needed
-        if (shift & 8) {
-#pragma unroll
-            for (int i = 0; i < kWords + 2; i++) w[i] = w[i + 2];
-        }
-        if (shift & 4) {
-#pragma unroll
-            for (int i = 0; i < kWords + 1; i++) w[i] = w[i + 1];
-        }
-        const int bits = (shift & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < kWords; i++) c.w[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], bits);
-        if (n < 8) {
-#pragma unroll
-            for (int i = 0; i < kWords; i++) {
-                if constexpr (sizeof(T) == 4) {
-                    if (i >= n) c.w[i] = 0;
-                } else {
-                    if (2 * i >= n) c.w[i] = 0;
-                    else if (2 * i + 1 >= n) c.w[i] &= 0xffff;
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (i >= n) break;
-            if constexpr (sizeof(T) == 4) c.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-            else c.w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p) + i)) << (16 * (i & 1));
-        }
-    }
-}
-
-// Puts a chunk into its place in each part of a stage.
-template <typename T>
-__device__ __forceinline__ void store_chunk(const Chunk<T>& c, uint32_t address, uint32_t part_bytes) {
-    if constexpr (sizeof(T) == 2) {
-        smem_store16(address, make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]));
-    } else {
-        uint32_t part[3][4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t x[2] = {c.w[2 * i], c.w[2 * i + 1]};
-#pragma unroll
-            for (int k = 0; k < 3; k++) {
-                part[k][i] = __byte_perm(x[0], x[1], 0x7632); // the upper halves
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    x[j] = __float_as_uint(__uint_as_float(x[j]) - __uint_as_float(x[j] & 0xffff0000u));
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 3; k++) smem_store16(address + k * part_bytes, make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]));
-    }
-}
-
-// One operand in memory. [begin, end): the bytes that it reaches over.
-template <typename T> struct Matrix {
-    const T* data;
-    int64_t stride, slice; // in values, between rows and between groups
-    const unsigned char *begin, *end;
-};
-
-// One operand of a stage: kRows rows of 64 values. K-major: the tile's rows, along the depth. MN-major: boxes of 64 rows, a row for
-// each value of depth.
-template <typename T, bool MN, int kRows> struct Source {
-    const T* p;        // the tile's first value of the stage
-    const Matrix<T>* m;
-    int across, depth; // how much of it there is from there
-    static constexpr int kChunks = kRows * 8 / kFillThreads; // of each thread
-
-    __device__ __forceinline__ void begin(const Matrix<T>& of, const T* first, int64_t size_across, int64_t size_depth) {
-        m = &of, p = first;
-        across = static_cast<int>(min(size_across, int64_t(kRows))), depth = static_cast<int>(size_depth);
-    }
-    __device__ __forceinline__ void advance() {
-        p += MN ? kBoxDepth * m->stride : kBoxDepth;
-        depth -= kBoxDepth;
-    }
-    __device__ __forceinline__ void load(Chunk<T>& c, int k) const {
-        const int task = k * kFillThreads + (threadIdx.x % kFillThreads), row = task / 8, value = task % 8 * 8;
+    // (Neighbouring lanes read from different banks: eight of them two rows of four chunks, or one row of two boxes.)
+    __device__ static __forceinline__ void load(uint4 (&v)[2], uint32_t raw, int k) {
+        const int task = k * kSplitThreads + (threadIdx.x % kSplitThreads);
         if constexpr (MN) {
-            const int d = row % 64, i = row / 64 * 64 + value;
-            load_chunk<T>(c, p + d * m->stride + i, d < depth ? across - i : 0, m->begin, m->end);
+            const int i = task % (kRows / 8), d = task / (kRows / 8), box = i / 4, odd = box & 1;
+            const uint32_t row = raw + box * (kDepth * 128) + d * 128;
+            const int first = 2 * (i % 4) + odd;
+            const uint4 a = smem_load16(row + ((first ^ (d & 7)) << 4)), b = smem_load16(row + ((first ^ 1 ^ (d & 7)) << 4));
+            v[0] = odd ? b : a;
+            v[1] = odd ? a : b;
         } else {
-            load_chunk<T>(c, p + row * m->stride + value, row < across ? depth - value : 0, m->begin, m->end);
+            const int c = task % 4, r = task / 4;
+#pragma unroll
+            for (int h = 0; h < 2; h++) v[h] = smem_load16(raw + r * 128 + (((2 * c + h) ^ (r & 7)) << 4));
         }
     }
-    __device__ static __forceinline__ void store(const Chunk<T>& c, int k, uint32_t to) {
-        const int task = k * kFillThreads + (threadIdx.x % kFillThreads), row = task / 8, chunk = task % 8;
-        store_chunk<T>(c, to + row * kBoxRow + ((chunk ^ (row & 7)) << 4), kRows * kBoxRow);
+    __device__ static __forceinline__ void store(const uint4 (&v)[2], uint32_t to, int k, int valid) {
+        const int task = k * kSplitThreads + (threadIdx.x % kSplitThreads);
+        uint32_t x[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+        if constexpr (MN) {
+            const int i = task % (kRows / 8), d = task / (kRows / 8);
+            to += i / 8 * (kDepth * 128) + d * 128 + ((i % 8 ^ (d & 7)) << 4);
+            if (d >= valid) { // a row of another group
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = 0;
+            }
+        } else {
+            const int c = task % 4, r = task / 4;
+            to += r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                w[j] = __byte_perm(x[2 * j], x[2 * j + 1], 0x7632); // the upper halves
+                if (p + 1 == kParts) continue;
+#pragma unroll
+                for (int h = 2 * j; h < 2 * j + 2; h++)
+                    x[h] = __float_as_uint(__uint_as_float(x[h]) - __uint_as_float(x[h] & 0xffff0000u));
+            }
+            smem_store16(to + p * kPart, make_uint4(w[0], w[1], w[2], w[3]));
+        }
     }
+    __device__ static __forceinline__ uint64_t descriptor(uint32_t at) { return operand_descriptor<kPartRow>(at, kDepth * 128); }
 };
 
-// ------------------------------------------------------------------ the work of a block
-// What both kernels do with a tile once they know where its operands lie.
-template <typename T, bool A_MN, bool B_MN, int kColumns> struct Tiles {
-    static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-    using L = Layout<kColumns, kParts>;
-    using A = Source<T, A_MN, kTileRows>;
-    using B = Source<T, B_MN, kColumns>;
-    static constexpr bool kBf16 = !std::is_same<T, __half>::value;
+// What the parts of a block do, of both kernels.
+template <bool A_MN, bool B_MN, int kColumns> struct Work {
+    using L = Layout<kColumns>;
+    using A = Operand<A_MN, kTileRows>;
+    using B = Operand<B_MN, kColumns>;
     static constexpr int kOwn = kColumns / 2; // columns of a storing warp
-    // stages that an accumulator takes before it is added to the sums in registers
-    static constexpr int kRun = kParts == 3 ? 1 : INT32_MAX;
 
     Block<L>& block;
-    int64_t step = 0, run = 0; // so far
+    Turn<L::kRaws> raw;
+    Turn<L::kStages> stage;
+    Turn<2> run;
+    int64_t fetched = 0;
 
-    // A filling warp, through all of the block's tiles: next() finds one, at(tile, a, b) says where its operands begin and returns its number of
-    // stages. The next stage's values are loaded into registers while this one's are put into place.
-    template <typename Next, typename At> __device__ __forceinline__ void fill(Next next, At at, int lane) {
-        Chunk<T> a[A::kChunks], b[B::kChunks];
-        A from_a;
-        B from_b;
-        auto t = next();
-        if (!t.found) return;
-        int steps = at(t, from_a, from_b), s = 0;
+    // The copying thread: a stage of both operands; boxes of A at (a_inner, a_outer), of B at (b_inner, b_outer, slice). valid < 0: no more will come.
+    __device__ __forceinline__ bool fetch(const CUtensorMap& map_a, const CUtensorMap& map_b, int a_inner, int a_outer, int b_inner,
+                                          int b_outer, int slice, int valid) {
+        if (!block.wait_empty(block.rings->raws, raw)) return false;
+        uint64_t* full = &block.rings->raws.full[raw.at];
+        *static_cast<volatile int*>(&block.rings->valid[raw.at]) = valid;
+        if (valid < 0) {
+            mbarrier_arrive(full);
+            return true;
+        }
+        const uint32_t a = block.base + static_cast<uint32_t>(raw.at) * L::kRaw, b = a + L::kRawA;
+        mbarrier_arrive_expect(full, L::kRaw);
 #pragma unroll
-        for (int k = 0; k < A::kChunks; k++) from_a.load(a[k], k);
+        for (int i = 0; i < A::kBoxes; i++) box_in(a + i * A::kBoxHeight * 128, map_a, a_inner + 32 * i, a_outer, 0, full);
 #pragma unroll
-        for (int k = 0; k < B::kChunks; k++) from_b.load(b[k], k);
-        for (bool more = true; more; step++) {
-            if (++s < steps) {
-                from_a.advance();
-                from_b.advance();
-            } else {
-                t = next();
-                more = t.found;
-                if (more) steps = at(t, from_a, from_b), s = 0;
-            }
+        for (int i = 0; i < B::kBoxes; i++) box_in(b + i * B::kBoxHeight * 128, map_b, b_inner + 32 * i, b_outer, slice, full);
+        raw.next();
+        fetched++;
+        return true;
+    }
+
+    // A splitting warp, until no more stages come.
+    __device__ __forceinline__ void split(int lane) {
+        for (;;) {
             bool ok = true;
-            if (lane == 0) ok = block.wait_empty(step);
+            if (lane == 0) ok = block.wait_full(block.rings->raws, raw);
             if (!__shfl_sync(kFullMask, ok, 0)) return;
-            const uint32_t to = block.stage(step);
+            if (lane != 0) ok = block.wait_full(block.rings->raws, raw); // (so that every lane has seen it)
+            const int valid = *static_cast<volatile int*>(&block.rings->valid[raw.at]);
+            if (valid < 0) return;
+            const uint32_t from = block.base + static_cast<uint32_t>(raw.at) * L::kRaw;
+            uint4 a[A::kChunks][2], b[B::kChunks][2];
 #pragma unroll
-            for (int k = 0; k < A::kChunks; k++) {
-                A::store(a[k], k, to);
-                if (more) from_a.load(a[k], k);
-            }
+            for (int k = 0; k < A::kChunks; k++) A::load(a[k], from, k);
 #pragma unroll
-            for (int k = 0; k < B::kChunks; k++) {
-                B::store(b[k], k, to + kParts * L::kA);
-                if (more) from_b.load(b[k], k);
+            for (int k = 0; k < B::kChunks; k++) B::load(b[k], from + L::kRawA, k);
+            __syncwarp();
+            if (lane == 0) {
+                mbarrier_arrive(&block.rings->raws.empty[raw.at]);
+                ok = block.wait_empty(block.rings->stages, stage);
             }
+            if (!__shfl_sync(kFullMask, ok, 0)) return;
+            raw.next();
+            const uint32_t to = block.base + L::kStagesAt + static_cast<uint32_t>(stage.at) * L::kStage;
+#pragma unroll
+            for (int k = 0; k < A::kChunks; k++) A::store(a[k], to, k, valid);
+#pragma unroll
+            for (int k = 0; k < B::kChunks; k++) B::store(b[k], to + kParts * L::kA, k, valid);
             async_proxy_fence();
             __syncwarp();
-            if (lane == 0) mbarrier_arrive(&block.b->full[step % L::kStages]);
+            if (lane == 0) mbarrier_arrive(&block.rings->stages.full[stage.at]);
+            stage.next();
         }
     }
 
-    // One thread.
+    // The multiplying thread: a tile.
     __device__ __forceinline__ bool multiply(int steps) {
-        constexpr uint32_t instruction = instruction_descriptor(kBf16, A_MN, B_MN, kColumns);
-        for (int s = 0; s < steps; s++, step++) {
-            if (s % kRun == 0) {
-                if (!block.wait_free(run)) return false;
-            }
-            if (!block.wait_full(step)) return false;
+        constexpr uint32_t instruction = instruction_descriptor(true, A_MN, B_MN, kColumns);
+        constexpr int part_a[6] = {0, 2, 1, 0, 1, 0}, part_b[6] = {2, 0, 1, 1, 0, 0}; // small products first
+        for (int s = 0; s < steps; s++) {
+            if (s % kRun == 0 && !block.wait_empty(block.rings->accumulators, run)) return false;
+            if (!block.wait_full(block.rings->stages, stage)) return false;
             tmem_fence_after_sync();
-            const uint64_t da = operand_descriptor(block.stage(step), kBoxBytes);
-            const uint64_t db = operand_descriptor(block.stage(step) + kParts * L::kA, kBoxBytes);
-            constexpr int kProducts = kParts == 3 ? 6 : 1;
-            constexpr int part_a[6] = {0, 2, 1, 0, 1, 0}, part_b[6] = {2, 0, 1, 1, 0, 0}; // small products first
-            bool add = s % kRun != 0;
+            const uint32_t at = block.base + L::kStagesAt + static_cast<uint32_t>(stage.at) * L::kStage;
+            const uint64_t a = A::descriptor(at), b = B::descriptor(at + kParts * L::kA);
+            const uint32_t accumulator = block.accumulator(run);
 #pragma unroll
-            for (int i = 0; i < kProducts; i++) {
-                const uint64_t pa = da + (kParts == 3 ? part_a[i] * (L::kA >> 4) : 0), pb = db + (kParts == 3 ? part_b[i] * (L::kB >> 4) : 0);
+            for (int i = 0; i < 6; i++)
 #pragma unroll
-                for (int k = 0; k < kBoxDepth / 16; k++, add = true)
-                    umma(block.accumulator(run), pa + k * kDepthStep<A_MN>, pb + k * kDepthStep<B_MN>, instruction, add);
+                for (int k = 0; k < kDepth / 16; k++)
+                    umma(accumulator, a + (part_a[i] * (L::kA >> 4) + k * A::kStep), b + (part_b[i] * (L::kB >> 4) + k * B::kStep), instruction,
+                         s % kRun + i + k > 0);
+            umma_arrive(&block.rings->stages.empty[stage.at]);
+            stage.next();
+            if ((s + 1) % kRun == 0 || s + 1 == steps) {
+                umma_arrive(&block.rings->accumulators.full[run.at]);
+                run.next();
             }
-            umma_arrive(&block.b->empty[step % L::kStages]);
-            if ((s + 1) % kRun == 0 || s + 1 == steps) umma_arrive(&block.b->done[run & 1]), run++;
         }
         return true;
     }
 
     // A storing warp: the tile's sums of its 32 rows and kOwn columns.
     __device__ __forceinline__ bool collect(float (&sum)[kOwn], int steps, int quadrant, int half, int lane) {
-        const int runs = kRun == 1 ? steps : steps > 0 ? 1 : 0;
 #pragma unroll
         for (int i = 0; i < kOwn; i++) sum[i] = 0;
-        for (int i = 0; i < runs; i++, run++) {
-            if (!block.wait_done(run)) return false;
+        for (int s = 0; s < steps; s += kRun) {
+            if (!block.wait_full(block.rings->accumulators, run)) return false;
             tmem_fence_after_sync();
             const uint32_t from = tmem_quadrant(block.accumulator(run), quadrant) + half * kOwn;
 #pragma unroll
@@ -256,14 +236,16 @@ template <typename T, bool A_MN, bool B_MN, int kColumns> struct Tiles {
             }
             tmem_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbarrier_arrive(&block.b->free[run & 1]);
+            if (lane == 0) mbarrier_arrive(&block.rings->accumulators.empty[run.at]);
+            run.next();
         }
         return true;
     }
 
-    // Writes them, 32 columns at a time through shared memory, a row after the other.
-    __device__ __forceinline__ void store(const float (&sum)[kOwn], int warp, T* out, int64_t stride, int64_t here, int64_t wide, int lane) {
+    // Writes them, 32 columns at a time through shared memory, a row after the other; rows of the output may begin anywhere.
+    __device__ __forceinline__ void store(const float (&sum)[kOwn], int warp, float* out, int64_t stride, int64_t here, int64_t wide, int lane) {
         float* staging = reinterpret_cast<float*>(block.smem + L::kStagingAt + warp * L::kStaging);
+        const int rows = static_cast<int>(min(here, int64_t(32)));
 #pragma unroll
         for (int c = 0; c < kOwn; c += 32) {
             if (c >= wide) break;
@@ -271,9 +253,8 @@ template <typename T, bool A_MN, bool B_MN, int kColumns> struct Tiles {
             for (int j = 0; j < 32; j++) staging[lane * 33 + j] = sum[c + j];
             __syncwarp();
             if (c + lane < wide) {
-                const int rows = static_cast<int>(min(here, int64_t(32)));
 #pragma unroll 8
-                for (int r = 0; r < rows; r++) out[r * stride + c + lane] = narrow<T>(staging[r * 33 + lane]);
+                for (int r = 0; r < rows; r++) out[r * stride + c + lane] = staging[r * 33 + lane];
             }
             __syncwarp();
         }
@@ -281,61 +262,74 @@ template <typename T, bool A_MN, bool B_MN, int kColumns> struct Tiles {
 };
 
 // ---------------------------------------------------------------------------------- rows
-template <typename T, bool M_MN, int kColumns>
+// out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
+template <bool M_MN, int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
-grouped_rows_split(T* __restrict__ out, const __grid_constant__ Matrix<T> x, const __grid_constant__ Matrix<T> m, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows,
-                   int64_t depth, int64_t columns, Status st) {
+grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m, float* __restrict__ out,
+                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int depth, int columns, Status st) {
     extern __shared__ unsigned char raw[];
-    using Work = Tiles<T, false, M_MN, kColumns>;
-    using L = typename Work::L;
+    using W = Work<false, M_MN, kColumns>;
+    using L = typename W::L;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
     const int64_t column_tiles = (columns + kColumns - 1) / kColumns;
-    const int steps = static_cast<int>((depth + kBoxDepth - 1) / kBoxDepth);
-    Work work{block};
+    const int steps = (depth + kDepth - 1) / kDepth;
+    W work{block};
     GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{kTileRows, column_tiles});
     struct Tile {
         bool found, in_group;
-        int64_t row, hi, group, column;
+        int64_t row, hi;
+        int group, column;
     };
-    int64_t want = static_cast<int64_t>(blockIdx.x) - gridDim.x;
-    auto next = [&](bool only_groups) { // the block's next tile
+    int64_t want = blockIdx.x;
+    auto next = [&] {
+        const GroupPiece piece = walk.find(want, lane);
+        want += gridDim.x;
         Tile t;
-        do {
-            want += gridDim.x;
-            const GroupPiece piece = walk.find(want, lane);
-            t.found = piece.found;
-            int64_t tile_row, tile_column;
-            banded(piece.within, max((piece.hi - piece.lo + kTileRows - 1) / kTileRows, int64_t(1)), column_tiles, tile_row, tile_column);
-            t.row = piece.lo + tile_row * kTileRows, t.hi = piece.hi, t.group = piece.group, t.column = tile_column * kColumns;
-            t.in_group = piece.group >= 0 && piece.group < groups;
-        } while (t.found && only_groups && !t.in_group);
+        t.found = piece.found;
+        if (!t.found) return t;
+        int64_t tile_row, tile_column;
+        banded(piece.within, (piece.hi - piece.lo + kTileRows - 1) / kTileRows, column_tiles, tile_row, tile_column);
+        t.row = piece.lo + tile_row * kTileRows, t.hi = piece.hi;
+        t.group = static_cast<int>(piece.group), t.column = static_cast<int>(tile_column) * kColumns;
+        t.in_group = piece.group >= 0 && piece.group < groups;
         return t;
     };
-    if (warp < kFillWarps) {
-        work.fill([&] { return next(true); },
-                  [&](const Tile& t, typename Work::A& a, typename Work::B& b) {
-                      a.begin(x, x.data + t.row * x.stride, t.hi - t.row, depth);
-                      b.begin(m, m.data + t.group * m.slice + t.column * (M_MN ? 1 : m.stride), columns - t.column, depth);
-                      return steps;
-                  },
-                  lane);
-    } else if (warp == kMultiplyWarp) {
-        for (Tile t = next(true); t.found; t = next(true)) {
-            bool ok = true;
-            if (lane == 0) ok = work.multiply(steps);
-            if (!__shfl_sync(kFullMask, ok, 0)) break;
+    if (warp < kSplitWarps) {
+        fewer_registers<kSplitRegisters>();
+        work.split(lane);
+    } else if (warp < kMultiplyWarp) {
+        more_registers<kStoreRegisters>();
+        const int quadrant = warp & 3, half = (warp - kSplitWarps) / 4;
+        for (Tile t = next(); t.found; t = next()) {
+            float sum[W::kOwn];
+            if (!work.collect(sum, t.in_group ? steps : 0, quadrant, half, lane)) break;
+            const int64_t row = t.row + quadrant * 32, column = t.column + half * W::kOwn;
+            work.store(sum, warp - kSplitWarps, out + row * columns + column, columns, t.hi - row, columns - column, lane);
         }
     } else {
-        const int quadrant = warp & 3, half = (warp - kMultiplyWarp - 1) / 4;
-        for (Tile t = next(false); t.found; t = next(false)) {
-            float sum[Work::kOwn];
-            if (!work.collect(sum, t.in_group ? steps : 0, quadrant, half, lane)) break;
-            const int64_t row = t.row + quadrant * 32, column = t.column + half * Work::kOwn;
-            work.store(sum, warp - kMultiplyWarp - 1, out + row * columns + column, columns, t.hi - row, columns - column, lane);
+        fewer_registers<kMultiplyRegisters>();
+        bool ok = true;
+        if (warp == kMultiplyWarp) {
+            for (Tile t = next(); t.found && ok; t = next()) {
+                if (lane == 0 && t.in_group) ok = work.multiply(steps);
+                ok = __shfl_sync(kFullMask, ok, 0);
+            }
+        } else if (warp == kCopyWarp) {
+            for (Tile t = next(); t.found && ok; t = next()) {
+                if (lane == 0 && t.in_group)
+                    for (int s = 0; s < steps && ok; s++)
+                        ok = work.fetch(map_x, map_m, s * kDepth, static_cast<int>(t.row), M_MN ? t.column : s * kDepth,
+                                        M_MN ? s * kDepth : t.column, t.group, kDepth);
+                ok = __shfl_sync(kFullMask, ok, 0);
+            }
+            if (lane == 0) {
+                if (ok) (void)work.fetch(map_x, map_m, 0, 0, 0, 0, 0, -1);
+                block.drain(block.rings->raws, work.raw, work.fetched);
+            }
         }
     }
     __syncwarp();
@@ -343,14 +337,15 @@ grouped_rows_split(T* __restrict__ out, const __grid_constant__ Matrix<T> x, con
 }
 
 // ------------------------------------------------------------------------- outer products
-template <typename T, int kColumns>
+// out[g] = X[rows of g]^T Y[rows of g].
+template <int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
-grouped_outer_split(T* __restrict__ out, const __grid_constant__ Matrix<T> x, const __grid_constant__ Matrix<T> y, float* __restrict__ parts, int64_t most_parts,
-                    const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int64_t height, int64_t columns, int64_t segment,
-                    Status st) {
+grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y, float* __restrict__ out,
+                    float* __restrict__ parts, int64_t most_parts, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height,
+                    int columns, int64_t segment, Status st) {
     extern __shared__ unsigned char raw[];
-    using Work = Tiles<T, true, true, kColumns>;
-    using L = typename Work::L;
+    using W = Work<true, true, kColumns>;
+    using L = typename W::L;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
@@ -358,60 +353,69 @@ grouped_outer_split(T* __restrict__ out, const __grid_constant__ Matrix<T> x, co
 
     const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
     const int64_t tiles = row_tiles * column_tiles;
-    Work work{block};
+    W work{block};
     GroupWalk<OuterPieces> walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles});
     struct Piece {
         bool found, part;
-        int64_t row, column, lo, hi, group, within;
-        int steps;
+        int row, column, lo, hi, steps;
+        int64_t group, within;
     };
-    int64_t want = static_cast<int64_t>(blockIdx.x) - gridDim.x;
-    auto next = [&](bool only_full) {
+    int64_t want = blockIdx.x;
+    auto next = [&] {
+        const GroupPiece piece = walk.find(want, lane);
+        want += gridDim.x;
         Piece t;
-        do {
-            want += gridDim.x;
-            const GroupPiece piece = walk.find(want, lane);
-            t.found = piece.found, t.group = piece.group, t.within = piece.within, t.part = piece.hi - piece.lo > segment;
-            const int64_t part = piece.within / tiles;
-            int64_t tile_row, tile_column;
-            banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
-            t.row = tile_row * kTileRows, t.column = tile_column * kColumns;
-            t.lo = piece.lo + part * segment, t.hi = min(t.lo + segment, piece.hi);
-            t.steps = static_cast<int>((t.hi - t.lo + kBoxDepth - 1) / kBoxDepth);
-        } while (t.found && only_full && t.steps == 0);
+        t.found = piece.found;
+        if (!t.found) return t;
+        t.group = piece.group, t.within = piece.within, t.part = piece.hi - piece.lo > segment;
+        const int64_t part = piece.within / tiles;
+        int64_t tile_row, tile_column;
+        banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
+        t.row = static_cast<int>(tile_row) * kTileRows, t.column = static_cast<int>(tile_column) * kColumns;
+        t.lo = static_cast<int>(piece.lo + part * segment), t.hi = static_cast<int>(min(t.lo + segment, piece.hi));
+        t.steps = (t.hi - t.lo + kDepth - 1) / kDepth;
         return t;
     };
-    if (warp < kFillWarps) {
-        work.fill([&] { return next(true); },
-                  [&](const Piece& t, typename Work::A& a, typename Work::B& b) {
-                      a.begin(x, x.data + t.lo * x.stride + t.row, height - t.row, t.hi - t.lo);
-                      b.begin(y, y.data + t.lo * y.stride + t.column, columns - t.column, t.hi - t.lo);
-                      return t.steps;
-                  },
-                  lane);
-    } else if (warp == kMultiplyWarp) {
-        for (Piece t = next(true); t.found; t = next(true)) {
-            bool ok = true;
-            if (lane == 0) ok = work.multiply(t.steps);
-            if (!__shfl_sync(kFullMask, ok, 0)) break;
-        }
-    } else {
-        const int quadrant = warp & 3, half = (warp - kMultiplyWarp - 1) / 4;
-        for (Piece t = next(false); t.found; t = next(false)) {
-            float sum[Work::kOwn];
+    if (warp < kSplitWarps) {
+        fewer_registers<kSplitRegisters>();
+        work.split(lane);
+    } else if (warp < kMultiplyWarp) {
+        more_registers<kStoreRegisters>();
+        const int quadrant = warp & 3, half = (warp - kSplitWarps) / 4;
+        for (Piece t = next(); t.found; t = next()) {
+            float sum[W::kOwn];
             if (!work.collect(sum, t.steps, quadrant, half, lane)) break;
             if (t.part) {
                 const int64_t slot = parts_before(offsets, groups, rows, t.group, OuterParts{segment, tiles}, lane) + t.within;
                 // (there are more parts than there is room for only where offsets descend, which is reported)
                 if (slot >= most_parts) continue;
-                float* to = parts + (slot * kTileRows + quadrant * 32 + lane) * kColumns + half * Work::kOwn;
+                float* to = parts + (slot * kTileRows + quadrant * 32 + lane) * kColumns + half * W::kOwn;
 #pragma unroll
-                for (int i = 0; i < Work::kOwn; i += 4)
+                for (int i = 0; i < W::kOwn; i += 4)
                     *reinterpret_cast<float4*>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
             } else {
-                const int64_t row = t.row + quadrant * 32, column = t.column + half * Work::kOwn;
-                work.store(sum, warp - kMultiplyWarp - 1, out + (t.group * height + row) * columns + column, columns, height - row, columns - column,
-                           lane);
+                const int64_t row = t.row + quadrant * 32, column = t.column + half * W::kOwn;
+                work.store(sum, warp - kSplitWarps, out + (t.group * height + row) * columns + column, columns, height - row, columns - column, lane);
+            }
+        }
+    } else {
+        fewer_registers<kMultiplyRegisters>();
+        bool ok = true;
+        if (warp == kMultiplyWarp) {
+            for (Piece t = next(); t.found && ok; t = next()) {
+                if (lane == 0) ok = work.multiply(t.steps);
+                ok = __shfl_sync(kFullMask, ok, 0);
+            }
+        } else if (warp == kCopyWarp) {
+            for (Piece t = next(); t.found && ok; t = next()) {
+                if (lane == 0)
+                    for (int s = 0; s < t.steps && ok; s++)
+                        ok = work.fetch(map_x, map_y, t.row, t.lo + s * kDepth, t.column, t.lo + s * kDepth, 0, min(t.hi - t.lo - s * kDepth, kDepth));
+                ok = __shfl_sync(kFullMask, ok, 0);
+            }
+            if (lane == 0) {
+                if (ok) (void)work.fetch(map_x, map_y, 0, 0, 0, 0, 0, -1);
+                block.drain(block.rings->raws, work.raw, work.fetched);
             }
         }
     }
@@ -419,80 +423,82 @@ grouped_outer_split(T* __restrict__ out, const __grid_constant__ Matrix<T> x, co
     block.end(warp);
 }
 
-template <typename T> Matrix<T> matrix(const Array& a, int64_t rows, int64_t stride, int64_t row_values, int64_t slices, int64_t slice) {
-    const unsigned char* begin = static_cast<const unsigned char*>(a.data);
-    return {static_cast<const T*>(a.data), stride, slice, begin,
-            begin + ((slices - 1) * slice + (rows - 1) * stride + row_values) * static_cast<int64_t>(sizeof(T))};
-}
-
-template <typename F> void for_split_type(int32_t type, F&& f) {
-    if (type == MOPS_B200_F32) f(float());
-    else if (type == MOPS_B200_F16) f(__half());
-    else f(__nv_bfloat16());
+// That the compiler gave the kernel the registers that its parts deal out among themselves (with fewer they would wait for good).
+void check_registers(const void* kernel, const std::string& op) {
+    static std::mutex mutex;
+    static std::set<const void*> good;
+    std::lock_guard<std::mutex> lock(mutex);
+    if (good.count(kernel)) return;
+    cudaFuncAttributes attributes;
+    MOPS_CUDA_OK(cudaFuncGetAttributes(&attributes, kernel));
+    if (attributes.numRegs != kLaunchRegisters)
+        throw std::runtime_error("internal error in operation " + op + ": a kernel was built with " +
+                                 std::to_string(attributes.numRegs) + " registers");
+    good.insert(kernel);
 }
 
 } // namespace
 
 bool multiply_rows_split(const Call& call, const RowsProblem& p, const std::string& op) {
-    if (p.X.type == MOPS_B200_F64 || p.depth == 0 || p.groups == 0) return false;
+    if (p.X.type != MOPS_B200_F32 || p.depth == 0 || p.groups == 0) return false;
     const bool mn = p.column_stride == 1;
     const int64_t stride = mn ? p.depth_stride : p.column_stride; // of M
     const int sms = sm_count(call.device);
-    for_split_type(p.X.type, [&](auto zero) {
-        using T = decltype(zero);
-        auto launch = [&](auto major, auto width) {
-            constexpr bool M_MN = decltype(major)::value;
-            constexpr int kColumns = decltype(width)::value;
-            using L = typename Tiles<T, false, M_MN, kColumns>::L;
-            const Matrix<T> x = matrix<T>(p.X, p.rows, p.X.stride[0], p.depth, 1, 0);
-            const Matrix<T> m = matrix<T>(p.M, mn ? p.depth : p.columns, stride, mn ? p.columns : p.depth, p.groups, p.M.stride[0]);
-            const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
-            auto kernel = grouped_rows_split<T, M_MN, kColumns>;
-            allow_dynamic_smem(kernel, call.device, L::kBytes);
-            kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kThreads, L::kBytes, call.stream>>>(
-                static_cast<T*>(p.out.data), x, m, p.offsets, p.groups, p.rows, p.depth, p.columns, call.status);
-            note_kernel_f("grouped_rows_split<%s,%s,%d>", array_type_name<T>(), M_MN ? "columns" : "depth", kColumns);
-        };
-        auto by_width = [&](auto major) {
-            if (p.columns > 64 && most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, 128) >= sms / 2)
-                launch(major, std::integral_constant<int, 128>());
-            else launch(major, std::integral_constant<int, 64>());
-        };
-        if (mn) by_width(std::true_type());
-        else by_width(std::false_type());
-    });
+    auto launch = [&](auto major, auto width) {
+        constexpr bool M_MN = decltype(major)::value;
+        constexpr int kColumns = decltype(width)::value;
+        using L = Layout<kColumns>;
+        const CUtensorMap x = tensor_map(p.X.type, p.X.data, p.depth, p.rows, 1, p.X.stride[0], 0, kTileRows);
+        const CUtensorMap m = M_MN ? tensor_map(p.X.type, p.M.data, p.columns, p.depth, p.groups, stride, p.M.stride[0], kDepth)
+                                   : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
+        const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
+        auto kernel = grouped_rows_split<M_MN, kColumns>;
+        allow_dynamic_smem(kernel, call.device, L::kBytes);
+        check_registers(reinterpret_cast<const void*>(kernel), op);
+        kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kThreads, L::kBytes, call.stream>>>(
+            x, m, static_cast<float*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns),
+            call.status);
+        note_kernel_f("grouped_rows_split<%s,%d>", M_MN ? "columns" : "depth", kColumns);
+    };
+    auto by_width = [&](auto major) {
+        if (p.columns > 64 && most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, 128) >= sms / 2)
+            launch(major, std::integral_constant<int, 128>());
+        else launch(major, std::integral_constant<int, 64>());
+    };
+    if (mn) by_width(std::true_type());
+    else by_width(std::false_type());
     MOPS_CUDA_OK(cudaGetLastError());
     return true;
 }
 
 bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::string& op) {
     const int64_t rows = p.X.shape[0], height = p.X.shape[1], columns = p.Y.shape[1];
-    if (p.X.type == MOPS_B200_F64 || rows == 0) return false;
+    if (p.X.type != MOPS_B200_F32 || rows == 0) return false;
     const int sms = sm_count(call.device);
-    for_split_type(p.X.type, [&](auto zero) {
-        using T = decltype(zero);
-        auto launch = [&](auto width) {
-            constexpr int kColumns = decltype(width)::value;
-            using L = typename Tiles<T, true, true, kColumns>::L;
-            const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
-            const int64_t segment = outer_segment(rows, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
-            float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
-                                          : nullptr;
-            auto kernel = grouped_outer_split<T, kColumns>;
-            allow_dynamic_smem(kernel, call.device, L::kBytes);
-            const int64_t pieces = tiles * (rows / segment + p.groups);
-            kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
-                static_cast<T*>(p.out.data), matrix<T>(p.X, rows, p.X.stride[0], height, 1, 0), matrix<T>(p.Y, rows, p.Y.stride[0], columns, 1, 0),
-                parts, most_parts, p.offsets, p.groups, rows, height, columns, segment, call.status);
-            if (rows > segment) {
-                join_outer<T, kColumns>(call, p, parts, most_parts, tiles, segment, op);
-                scratch_free(call, parts);
-            }
-            note_kernel_f("grouped_outer_split<%s,%d>", array_type_name<T>(), kColumns);
-        };
-        if (columns > 64) launch(std::integral_constant<int, 128>());
-        else launch(std::integral_constant<int, 64>());
-    });
+    auto launch = [&](auto width) {
+        constexpr int kColumns = decltype(width)::value;
+        using L = Layout<kColumns>;
+        const CUtensorMap x = tensor_map(p.X.type, p.X.data, height, rows, 1, p.X.stride[0], 0, kDepth);
+        const CUtensorMap y = tensor_map(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, kDepth);
+        const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
+        const int64_t segment = outer_segment(rows, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
+        float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
+                                      : nullptr;
+        auto kernel = grouped_outer_split<kColumns>;
+        allow_dynamic_smem(kernel, call.device, L::kBytes);
+        check_registers(reinterpret_cast<const void*>(kernel), op);
+        const int64_t pieces = tiles * (rows / segment + p.groups);
+        kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
+            x, y, static_cast<float*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns),
+            segment, call.status);
+        if (rows > segment) {
+            join_outer<float, kColumns>(call, p, parts, most_parts, tiles, segment, op);
+            scratch_free(call, parts);
+        }
+        note_kernel_f("grouped_outer_split<%d>", kColumns);
+    };
+    if (columns > 64) launch(std::integral_constant<int, 128>());
+    else launch(std::integral_constant<int, 64>());
     MOPS_CUDA_OK(cudaGetLastError());
     return true;
 }

@@ -17,11 +17,12 @@ constexpr int kBoxRow = 128;               // bytes
 constexpr int kBoxDepth = 64;              // values in a row, and the depth of a stage
 constexpr int kBoxBytes = 64 * kBoxRow;    // of a box of 64 rows
 
-// The shared-memory descriptor of an operand: version 1, 128-byte swizzle. `across`: bytes between boxes of 64 rows or columns (MN-major;
-// K-major operands ignore it). Groups of eight rows are 1024 bytes apart in both.
-__device__ __forceinline__ uint64_t operand_descriptor(uint32_t address, uint32_t across) {
+// The shared-memory descriptor of an operand: version 1, swizzle over 128 bytes (or 64, for rows of 32 values). `across`: bytes between boxes
+// of 64 rows or columns (MN-major; K-major operands ignore it). Groups of eight rows follow each other.
+template <int kRowBytes = kBoxRow> __device__ __forceinline__ uint64_t operand_descriptor(uint32_t address, uint32_t across) {
+    static_assert(kRowBytes == 128 || kRowBytes == 64, "swizzles");
     return static_cast<uint64_t>((address & 0x3ffff) >> 4) | static_cast<uint64_t>(across >> 4) << 16 |
-           static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+           static_cast<uint64_t>(8 * kRowBytes >> 4) << 32 | uint64_t(1) << 46 | uint64_t(kRowBytes == 128 ? 2 : 4) << 61;
 }
 // What one step of 16 values in depth adds to a descriptor.
 template <bool MN> constexpr uint64_t kDepthStep = MN ? 2048 >> 4 : 32 >> 4;
@@ -74,6 +75,17 @@ __device__ __forceinline__ void map_prefetch(const CUtensorMap& map) {
 
 __device__ __forceinline__ void smem_store16(uint32_t address, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ uint16_t smem_load2(uint32_t address) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 smem_load16(uint32_t address) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+    return v;
 }
 
 } // namespace mops_b200
