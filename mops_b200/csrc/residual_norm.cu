@@ -19,6 +19,8 @@
 
 #include "arrays.hpp"
 #include "block_ops.hpp"
+#include "bulk.cuh"
+#include "pairs.cuh"
 
 namespace mops_b200 {
 namespace {
@@ -33,6 +35,7 @@ enum Gate : int { kNoGate = 0, kRowGate = 1, kFullGate = 2 };
 template <typename S> __device__ __forceinline__ S sigmoid(S v) { return S(1) / (S(1) + exp(-v)); }
 template <> __device__ __forceinline__ float sigmoid<float>(float v) { return 1.0f / (1.0f + expf(-v)); }
 template <typename S> __device__ __forceinline__ S inverse_root(S v) { return S(1) / sqrt(v); }
+template <> __device__ __forceinline__ float inverse_root<float>(float v) { return rsqrtf(v); }
 
 // The sums of K values over the block, for every thread.
 template <int K, typename S> __device__ __forceinline__ void block_sums(S (&v)[K], S (*shared)[K]) {
@@ -157,215 +160,463 @@ residual_norm_vjp_plain(Gradients<T> g, Inputs<T> in) {
 // array. The next row's values are on their way while this one is worked on. Blocks stay for the whole call, so that scales and weights are read
 // once and the sums over rows stay in registers until the end.
 constexpr int kTeamThreads = 512; // at most
+// Values of a thread, in 16-byte packs or one by one: eight of them (f64: four), or twice as many for long rows.
+template <typename T> constexpr int kFewValues = sizeof(T) == 8 ? 4 : 8;
 
-// The sums of K values over the team, for every thread of it. `shared`: two of these are used in turn, so that one barrier does.
+// Sums over the team, of one value or of two, for every thread of it. The warps' sums go through shared memory, in two places that are used in
+// turn, so that one barrier does. Two values are added up together: half of the lanes for each.
 template <typename S> struct TeamSums {
-    S (*shared)[kTeamThreads / 32][2];
-    int warps, turn = 0;
-    template <int K> __device__ __forceinline__ void add_up(S (&v)[K]) {
-#pragma unroll
-        for (int k = 0; k < K; k++) v[k] = warp_sum(v[k]);
-        if (warps == 1) return;
-        S(*to)[2] = shared[turn];
-        turn ^= 1;
-        if ((threadIdx.x & 31) == 0)
-#pragma unroll
-            for (int k = 0; k < K; k++) to[threadIdx.x >> 5][k] = v[k];
+    static constexpr int kMost = kTeamThreads / 32; // warps
+    static_assert(kMost == 16, "half a warp adds up the warps' sums");
+    struct Place {
+        S of_warp[2 * kMost]; // of the first value, then of the second
+    };
+    Place* places;
+    bool one_warp;
+    int turn = 0;
+    __device__ TeamSums(Place (&shared)[2], int team) : places(shared), one_warp(team == 32) {
+        if (one_warp) return;
+        for (int i = threadIdx.x; i < 4 * kMost; i += blockDim.x) shared[i / (2 * kMost)].of_warp[i % (2 * kMost)] = 0; // (of warps that there are none of)
         __syncthreads();
+    }
+    __device__ __forceinline__ static S half_sum(S v) {
 #pragma unroll
-        for (int k = 0; k < K; k++) v[k] = 0;
-        for (int w = 0; w < warps; w++)
-#pragma unroll
-            for (int k = 0; k < K; k++) v[k] += to[w][k];
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+        return v;
+    }
+    __device__ __forceinline__ void add_up(S& a) {
+        a = warp_sum(a);
+        if (one_warp) return;
+        Place& place = places[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) place.of_warp[threadIdx.x >> 5] = a;
+        __syncthreads();
+        a = half_sum(place.of_warp[threadIdx.x & (kMost - 1)]);
+    }
+    __device__ __forceinline__ void add_up(S& a, S& b) {
+        const bool upper = threadIdx.x & 16;
+        S v = half_sum((upper ? b : a) + __shfl_xor_sync(kFullMask, upper ? a : b, 16));
+        if (!one_warp) {
+            Place& place = places[turn];
+            turn ^= 1;
+            if ((threadIdx.x & 15) == 0) place.of_warp[(upper ? kMost : 0) + (threadIdx.x >> 5)] = v;
+            __syncthreads();
+            v = half_sum(place.of_warp[threadIdx.x & 31]);
+        }
+        const S other = __shfl_xor_sync(kFullMask, v, 16);
+        a = upper ? other : v;
+        b = upper ? v : other;
     }
 };
 
-// A thread's values of a row.
-template <typename T, int N, int kPacks> struct Values {
-    Pack<T, N> p[kPacks];
-    __device__ __forceinline__ Sum<T> operator[](int i) const { return widen(p[i / N].v[i % N]); }
-    // `row` begins the row; packs behind the row's end are zeros
-    __device__ __forceinline__ void load(const T* __restrict__ row, int member, int team, int packs) {
+// A thread's values of a row, kPacks packs of N; where a pack lies behind the row's end, zeros (which stay in `p` from one row to the next).
+template <typename T, int N, int kPacks> struct alignas(16) Values {
+    static constexpr int kPairs = N * kPacks / 2;
+    T v[N * kPacks];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int k = 0; k < kPacks; k++) {
-            const int at = k * team + member;
-            if (at < packs) p[k] = *reinterpret_cast<const Pack<T, N>*>(row + static_cast<int64_t>(at) * N);
-            else
+        for (int i = 0; i < N * kPacks; i++) v[i] = narrow<T>(0);
+    }
+    // first: the thread's first pack of the row
+    __device__ __forceinline__ void load(const T* __restrict__ first, int member, int team, int packs) {
 #pragma unroll
-                for (int i = 0; i < N; i++) p[k].v[i] = narrow<T>(0);
+        for (int k = 0; k < kPacks; k++)
+            if (k * team + member < packs)
+                *reinterpret_cast<Pack<T, N>*>(&v[k * N]) = *reinterpret_cast<const Pack<T, N>*>(first + k * team * N);
+    }
+    __device__ __forceinline__ void store(T* __restrict__ first, int member, int team, int packs) const {
+#pragma unroll
+        for (int k = 0; k < kPacks; k++)
+            if (k * team + member < packs)
+                *reinterpret_cast<Pack<T, N>*>(first + k * team * N) = *reinterpret_cast<const Pack<T, N>*>(&v[k * N]);
+    }
+    __device__ __forceinline__ Pair<Sum<T>> operator[](int i) const { return widen2(&v[2 * i]); }
+    __device__ __forceinline__ void set(int i, Pair<Sum<T>> value) { narrow2(&v[2 * i], value); }
+};
+
+// sigmoid(v). In f32 and f64 with the functions of the mathematical library; of 16-bit gates, whose results are rounded to as many bits, by
+// the approximate instructions (2^v within 2 units of the 22nd bit, 1 / v within 1 of the 23rd).
+template <typename T> __device__ __forceinline__ Pair<Sum<T>> gates(Pair<Sum<T>> v) {
+    if constexpr (sizeof(T) == 2) {
+        Pair<float> e = v * -1.44269504f;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+        e = e + both(1.0f);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+        return e;
+    } else {
+        return {sigmoid<Sum<T>>(v.x), sigmoid<Sum<T>>(v.y)};
+    }
+}
+
+// A thread's own weights: scale * weight_branch, where registers are short in shared memory, and weight_output.
+template <typename T, int N, int kPacks, bool kShared> struct Weights {
+    using S = Sum<T>;
+    using V = Values<T, N, kPacks>;
+    Pair<S> own[kShared ? 1 : V::kPairs];
+    const Pair<S>* place; // the thread's pairs are `threads` apart
+    int threads;
+    V p;
+    // room: of the block's threads, 2 kPairs values each
+    __device__ __forceinline__ void load(const Inputs<T>& in, int member, int team, int packs, S* room) {
+        V s, w;
+        s.clear(), w.clear(), p.clear();
+        s.load(in.scale + member * N, member, team, packs);
+        w.load(in.weight_branch + member * N, member, team, packs);
+        p.load(in.weight_output + member * N, member, team, packs);
+        Pair<S>* to = reinterpret_cast<Pair<S>*>(room) + threadIdx.x;
+        threads = blockDim.x;
+        place = to;
+#pragma unroll
+        for (int i = 0; i < V::kPairs; i++) {
+            if constexpr (kShared) to[i * threads] = s[i] * w[i];
+            else own[i] = s[i] * w[i];
         }
     }
-};
-template <int N, int kPacks, typename T>
-__device__ __forceinline__ void store_values(T* __restrict__ row, const Sum<T> (&v)[N * kPacks], int member, int team, int packs) {
-#pragma unroll
-    for (int k = 0; k < kPacks; k++) {
-        const int at = k * team + member;
-        Pack<T, N> p;
-#pragma unroll
-        for (int i = 0; i < N; i++) p.v[i] = narrow<T>(v[k * N + i]);
-        if (at < packs) *reinterpret_cast<Pack<T, N>*>(row + static_cast<int64_t>(at) * N) = p;
+    __device__ __forceinline__ Pair<S> sw(int i) const {
+        if constexpr (kShared) return place[i * threads];
+        else return own[i];
     }
-}
+};
 
-// The gate of 16-bit values needs fewer bits than that of f32.
-template <typename T> __device__ __forceinline__ Sum<T> gate_value(Sum<T> v) {
-    if constexpr (sizeof(T) == 2) return __fdividef(1.0f, 1.0f + __expf(-v));
-    else return sigmoid<Sum<T>>(v);
-}
+// A row forward, in two steps, with what is held in between.
+template <typename T, int GATE, int N, int kPacks> struct RowForward {
+    using S = Sum<T>;
+    using V = Values<T, N, kPacks>;
+    Pair<S> y[V::kPairs];
+    S per_column, epsilon;
+    __device__ RowForward(const Inputs<T>& in) : per_column(S(1) / static_cast<S>(in.columns)), epsilon(static_cast<S>(in.epsilon)) {}
+
+    __device__ __forceinline__ S inverse_rms(const V& b, TeamSums<S>& sums) const {
+        Pair<S> square = both(S(0));
+#pragma unroll
+        for (int i = 0; i < V::kPairs; i++) square = fma2(b[i], b[i], square);
+        S sum = total(square);
+        sums.add_up(sum);
+        return inverse_root<S>(sum * per_column + epsilon);
+    }
+    template <typename W> // returns the sum of squares of the thread's values
+    __device__ __forceinline__ S stream(V& out, const W& weights, const V& x, const V& b, const V& g, T gate, S q) {
+        const Pair<S> z_row = GATE == kRowGate ? gates<T>(both(widen(gate))) : both(S(1));
+        Pair<S> square = both(S(0));
+#pragma unroll
+        for (int i = 0; i < V::kPairs; i++) {
+            const Pair<S> z = GATE == kFullGate ? gates<T>(g[i]) : z_row;
+            y[i] = fma2(weights.sw(i) * z, b[i] * q, x[i]);
+            square = fma2(y[i], y[i], square);
+            out.set(i, y[i]);
+        }
+        return total(square);
+    }
+    __device__ __forceinline__ void normed(V& out, const V& p, S sum_of_squares) const {
+        const S r = inverse_root<S>(sum_of_squares * per_column + epsilon);
+#pragma unroll
+        for (int i = 0; i < V::kPairs; i++) out.set(i, p[i] * (y[i] * r));
+    }
+};
 
 template <typename T, int GATE, int N, int kPacks>
 __global__ void __launch_bounds__(kTeamThreads)
 residual_norm_rows(T* __restrict__ stream, T* __restrict__ normed, const __grid_constant__ Inputs<T> in, int team) {
     using S = Sum<T>;
-    constexpr int kValues = N * kPacks;
     using V = Values<T, N, kPacks>;
-    __shared__ S shared[2][kTeamThreads / 32][2];
+    __shared__ typename TeamSums<S>::Place shared[2];
     const int member = threadIdx.x % team, teams = blockDim.x / team, packs = static_cast<int>(in.columns / N);
-    const S epsilon = static_cast<S>(in.epsilon), C = static_cast<S>(in.columns);
-    TeamSums<S> sums{shared, team / 32};
-    V s, w, p;
-    s.load(in.scale, member, team, packs);
-    w.load(in.weight_branch, member, team, packs);
-    p.load(in.weight_output, member, team, packs);
+    TeamSums<S> sums(shared, team);
+    Weights<T, N, kPacks, false> weights;
+    weights.load(in, member, team, packs, nullptr);
+    RowForward<T, GATE, N, kPacks> work(in);
     const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
     int64_t row = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team;
-    V next_x, next_b, next_g;
+    V next_x, next_b, next_g, out;
     T next_gate{};
+    next_x.clear(), next_b.clear(), next_g.clear();
     auto fetch = [&](int64_t r) {
         if (r >= in.rows) return;
-        next_b.load(in.branch + r * in.branch_stride, member, team, packs);
-        next_x.load(in.residual + r * in.residual_stride, member, team, packs);
-        if constexpr (GATE == kFullGate) next_g.load(in.gate + r * in.gate_stride, member, team, packs);
+        next_b.load(in.branch + r * in.branch_stride + member * N, member, team, packs);
+        next_x.load(in.residual + r * in.residual_stride + member * N, member, team, packs);
+        if constexpr (GATE == kFullGate) next_g.load(in.gate + r * in.gate_stride + member * N, member, team, packs);
         if constexpr (GATE == kRowGate) next_gate = in.gate[r * in.gate_stride];
     };
     fetch(row);
-    for (; row < in.rows; row += step) { // (all teams of a block of several are warps, which do not wait for one another)
+    for (; row < in.rows; row += step) { // (teams of a block of several are warps, which do not wait for one another)
         const V x = next_x, b = next_b, g = next_g;
         const T gate = next_gate;
         fetch(row + step);
-        S sum[1] = {0};
-#pragma unroll
-        for (int i = 0; i < kValues; i++) sum[0] += b[i] * b[i];
+        const S q = work.inverse_rms(b, sums);
+        S sum = work.stream(out, weights, x, b, g, gate, q);
+        const int64_t at = row * in.columns + member * N;
+        out.store(stream + at, member, team, packs);
         sums.add_up(sum);
-        const S q = inverse_root<S>(sum[0] / C + epsilon);
-        const S z_row = GATE == kRowGate ? gate_value<T>(widen(gate)) : S(1);
-        S y[kValues];
-        sum[0] = 0;
-#pragma unroll
-        for (int i = 0; i < kValues; i++) {
-            const S z = GATE == kFullGate ? gate_value<T>(g[i]) : z_row;
-            y[i] = x[i] + s[i] * w[i] * z * (b[i] * q);
-            sum[0] += y[i] * y[i];
-        }
-        store_values<N, kPacks>(stream + row * in.columns, y, member, team, packs);
-        sums.add_up(sum);
-        const S r = inverse_root<S>(sum[0] / C + epsilon);
-#pragma unroll
-        for (int i = 0; i < kValues; i++) y[i] = p[i] * y[i] * r;
-        store_values<N, kPacks>(normed + row * in.columns, y, member, team, packs);
+        work.normed(out, weights.p, sum);
+        out.store(normed + at, member, team, packs);
     }
 }
 
+// Rows that a block shares and whose packs are whole: the rows of the inputs come into shared memory by bulk copies, kRing rows ahead, which
+// leaves registers for two blocks on an SM: while one waits at a barrier the other works.
+template <typename T, int kInputs, int kRing> struct RowRing {
+    unsigned char* places;
+    uint64_t* full;
+    int row_bytes, at = 0;
+    unsigned round = 0;
+
+    __device__ RowRing(unsigned char* places, uint64_t (&full)[kRing], int64_t columns)
+        : places(places), full(full), row_bytes(static_cast<int>(columns * sizeof(T))) {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < kRing; i++) mbarrier_init(&full[i], 1);
+            mbarrier_init_fence();
+        }
+    }
+    // one thread; rows: where each input's row begins
+    __device__ __forceinline__ void fetch(int place, const T* const (&rows)[kInputs]) {
+        unsigned char* to = places + place * kInputs * row_bytes;
+        mbarrier_arrive_expect(&full[place], static_cast<unsigned>(kInputs * row_bytes));
+#pragma unroll
+        for (int i = 0; i < kInputs; i++) bulk_copy_in(to + i * row_bytes, rows[i], row_bytes, &full[place]);
+    }
+    __device__ __forceinline__ bool wait() { return mbarrier_wait(&full[at], round); }
+    __device__ __forceinline__ const T* row() const { return reinterpret_cast<const T*>(places + at * kInputs * row_bytes); }
+    __device__ __forceinline__ void next() {
+        if (++at == kRing) at = 0, round ^= 1;
+    }
+};
+constexpr int kForwardRing = 3, kBackwardRing = 2;
+
+template <typename T, int GATE, int kPacks>
+__global__ void __launch_bounds__(kTeamThreads, kPacks * kPack<T> > kFewValues<T> ? 1 : 2)
+residual_norm_staged(T* __restrict__ stream, T* __restrict__ normed, const __grid_constant__ Inputs<T> in, Status st) {
+    using S = Sum<T>;
+    constexpr int N = kPack<T>, kInputs = GATE == kFullGate ? 3 : 2;
+    using V = Values<T, N, kPacks>;
+    extern __shared__ __align__(128) unsigned char stages[];
+    __shared__ typename TeamSums<S>::Place shared[2];
+    __shared__ uint64_t full[kForwardRing];
+    const int member = threadIdx.x, team = blockDim.x, packs = static_cast<int>(in.columns / N), columns = static_cast<int>(in.columns);
+    RowRing<T, kInputs, kForwardRing> ring(stages, full, in.columns);
+    TeamSums<S> sums(shared, team); // (ends with a barrier: a team of one warp does not come here)
+    const int64_t step = gridDim.x;
+    auto fetch = [&](int64_t r, int place) {
+        if (threadIdx.x != 0 || r >= in.rows) return;
+        const T* b = in.branch + r * in.branch_stride;
+        const T* x = in.residual + r * in.residual_stride;
+        if constexpr (GATE == kFullGate) ring.fetch(place, {b, x, in.gate + r * in.gate_stride});
+        else ring.fetch(place, {b, x});
+    };
+    int64_t row = blockIdx.x;
+    for (int i = 0; i < kForwardRing; i++) fetch(row + i * step, i);
+    Weights<T, N, kPacks, false> weights;
+    weights.load(in, member, team, packs, nullptr);
+    RowForward<T, GATE, N, kPacks> work(in);
+    for (; row < in.rows; row += step, ring.next()) {
+        const T gate = GATE == kRowGate ? in.gate[row * in.gate_stride] : T{};
+        if (!ring.wait()) {
+            report_stalled(st);
+            return;
+        }
+        const T* first = ring.row() + member * N;
+        V x, b, g, out;
+        x.clear(), b.clear(), g.clear();
+        b.load(first, member, team, packs);
+        const S q = work.inverse_rms(b, sums);
+        x.load(first + columns, member, team, packs);
+        if constexpr (GATE == kFullGate) g.load(first + 2 * columns, member, team, packs);
+        S sum = work.stream(out, weights, x, b, g, gate, q);
+        const int64_t at = row * in.columns + member * N;
+        out.store(stream + at, member, team, packs);
+        sums.add_up(sum); // (and everybody is done with the row's place)
+        fetch(row + kForwardRing * step, ring.at);
+        work.normed(out, weights.p, sum);
+        out.store(normed + at, member, team, packs);
+    }
+}
+
+// The backward pass of a row, in steps, with what is held from one to the next.
+template <typename T, int GATE, int N, int kPacks, bool kShared> struct RowBackward {
+    using S = Sum<T>;
+    using V = Values<T, N, kPacks>;
+    static constexpr int kPairs = V::kPairs;
+    const Weights<T, N, kPacks, kShared>& weights;
+    S per_column, epsilon;
+    Pair<S> z[kPairs], y[kPairs];                 // y: the stream; z: in the end what of its gradient goes to n
+    Pair<S> of_branch[kPairs], of_output[kPairs]; // sums over rows
+
+    __device__ RowBackward(const Weights<T, N, kPacks, kShared>& weights, const Inputs<T>& in)
+        : weights(weights), per_column(S(1) / static_cast<S>(in.columns)), epsilon(static_cast<S>(in.epsilon)) {
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) of_branch[i] = of_output[i] = both(S(0));
+    }
+    __device__ __forceinline__ S inverse_rms(const V& b, TeamSums<S>& sums) const {
+        Pair<S> square = both(S(0));
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) square = fma2(b[i], b[i], square);
+        S sum = total(square);
+        sums.add_up(sum);
+        return inverse_root<S>(sum * per_column + epsilon);
+    }
+    // sums of squares of the stream, and of its products with the gradient of its norm
+    __device__ __forceinline__ void forward(const V& x, const V& b, const V& g, T gate, const V& gh, S q, S& squares, S& products) {
+        const Pair<S> z_row = GATE == kRowGate ? gates<T>(both(widen(gate))) : both(S(1));
+        Pair<S> square = both(S(0)), along = both(S(0));
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) {
+            z[i] = GATE == kFullGate ? gates<T>(g[i]) : z_row;
+            y[i] = fma2(weights.sw(i) * z[i], b[i] * q, x[i]);
+            square = fma2(y[i], y[i], square);
+            along = fma2(weights.p[i] * gh[i], y[i], along);
+        }
+        squares = total(square), products = total(along);
+    }
+    // The gradients of the stream and of full gates, and sums over the row of what those of the branch and of the row's gate need.
+    __device__ __forceinline__ void backward(V& out_stream, V& out_gate, const V& b, const V& gs, const V& gh, S q, S squares, S products,
+                                             S& of_n, S& of_gate) {
+        const S r = inverse_root<S>(squares * per_column + epsilon), back = -products * r * r * r * per_column;
+        Pair<S> sum_n = both(S(0)), sum_gate = both(S(0));
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) {
+            const Pair<S> n = b[i] * q, h = gh[i] * r;
+            of_output[i] = fma2(h, y[i], of_output[i]);
+            const Pair<S> ds = fma2(weights.p[i], h, fma2(y[i], both(back), gs[i]));
+            out_stream.set(i, ds);
+            of_branch[i] = fma2(ds * z[i], n, of_branch[i]);
+            const Pair<S> dn = ds * weights.sw(i) * z[i], all = dn * n;
+            sum_n = sum_n + all;
+            if constexpr (GATE != kNoGate) {
+                const Pair<S> to_gate = fma2(all, z[i] * S(-1), all);
+                if constexpr (GATE == kFullGate) out_gate.set(i, to_gate);
+                else sum_gate = sum_gate + to_gate;
+            }
+            z[i] = dn;
+        }
+        of_n = total(sum_n), of_gate = total(sum_gate);
+    }
+    __device__ __forceinline__ void branch(V& out, const V& b, S q, S of_n) const {
+        const S lost = -q * of_n * per_column;
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) out.set(i, fma2(b[i], both(lost), z[i]) * q);
+    }
+    // the sums over the rows of this thread; `add`: on top of what is there
+    __device__ __forceinline__ void leave(S* own, const Inputs<T>& in, int member, int team, int packs, bool add) const {
+#pragma unroll
+        for (int i = 0; i < 2 * kPairs; i++) {
+            const int pack = i / N * team + member;
+            if (pack >= packs) continue;
+            const int64_t c = static_cast<int64_t>(pack) * N + i % N;
+            own[c] = (add ? own[c] : S(0)) + (i & 1 ? of_branch[i / 2].y : of_branch[i / 2].x);
+            own[in.columns + c] = (add ? own[in.columns + c] : S(0)) + (i & 1 ? of_output[i / 2].y : of_output[i / 2].x);
+        }
+    }
+};
+
 template <typename T, int GATE, int N, int kPacks>
-__global__ void __launch_bounds__(kTeamThreads)
+__global__ void __launch_bounds__(kTeamThreads, 1)
 residual_norm_vjp_rows(const __grid_constant__ Gradients<T> grad, const __grid_constant__ Inputs<T> in, int team) {
     using S = Sum<T>;
-    constexpr int kValues = N * kPacks;
     using V = Values<T, N, kPacks>;
-    __shared__ S shared[2][kTeamThreads / 32][2];
+    __shared__ typename TeamSums<S>::Place shared[2];
     const int member = threadIdx.x % team, teams = blockDim.x / team, packs = static_cast<int>(in.columns / N);
-    const S epsilon = static_cast<S>(in.epsilon), C = static_cast<S>(in.columns);
-    TeamSums<S> sums{shared, team / 32};
-    V s, w, p;
-    s.load(in.scale, member, team, packs);
-    w.load(in.weight_branch, member, team, packs);
-    p.load(in.weight_output, member, team, packs);
-    S of_branch[kValues], of_output[kValues]; // sums over the team's rows
-#pragma unroll
-    for (int i = 0; i < kValues; i++) of_branch[i] = of_output[i] = 0;
+    TeamSums<S> sums(shared, team);
+    Weights<T, N, kPacks, false> weights;
+    weights.load(in, member, team, packs, nullptr);
+    RowBackward<T, GATE, N, kPacks, false> work(weights, in);
     const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team;
-    V next_x, next_b, next_g, next_gs, next_gh;
-    T next_gate{};
-    auto fetch = [&](int64_t r) {
-        if (r >= in.rows) return;
-        next_b.load(in.branch + r * in.branch_stride, member, team, packs);
-        next_x.load(in.residual + r * in.residual_stride, member, team, packs);
-        if constexpr (GATE == kFullGate) next_g.load(in.gate + r * in.gate_stride, member, team, packs);
-        if constexpr (GATE == kRowGate) next_gate = in.gate[r * in.gate_stride];
-        next_gh.load(grad.normed + r * grad.normed_stride, member, team, packs);
-        next_gs.load(grad.stream + r * grad.stream_stride, member, team, packs);
-    };
-    fetch(row);
-    for (; row < in.rows; row += step) {
-        const V x = next_x, b = next_b, g = next_g, gs = next_gs, gh = next_gh;
-        const T gate = next_gate;
-        fetch(row + step);
-        S sum[2] = {0, 0};
-        S one[1] = {0};
-#pragma unroll
-        for (int i = 0; i < kValues; i++) one[0] += b[i] * b[i];
-        sums.add_up(one);
-        const S q = inverse_root<S>(one[0] / C + epsilon);
-        const S z_row = GATE == kRowGate ? gate_value<T>(widen(gate)) : S(1);
-        S z[kValues], y[kValues];
-#pragma unroll
-        for (int i = 0; i < kValues; i++) {
-            z[i] = GATE == kFullGate ? gate_value<T>(g[i]) : z_row;
-            y[i] = x[i] + s[i] * w[i] * z[i] * (b[i] * q);
-            sum[0] += y[i] * y[i];
-            sum[1] += p[i] * gh[i] * y[i];
-        }
-        sums.add_up(sum);
-        const S r = inverse_root<S>(sum[0] / C + epsilon), back = sum[1] * r * r * r / C;
-        sum[0] = sum[1] = 0;
-#pragma unroll
-        for (int i = 0; i < kValues; i++) {
-            const S zn = z[i] * (b[i] * q);
-            of_output[i] += gh[i] * y[i] * r;
-            y[i] = gs[i] + r * (p[i] * gh[i]) - y[i] * back; // from here on the stream's gradient
-            of_branch[i] += y[i] * zn;
-            const S full = y[i] * s[i] * w[i] * zn;
-            sum[0] += full;
-            if constexpr (GATE == kRowGate) sum[1] += full * (1 - z[i]);
-        }
-        if (grad.residual != nullptr) store_values<N, kPacks>(grad.residual + row * in.columns, y, member, team, packs);
-        if constexpr (GATE == kFullGate)
-            if (grad.gate != nullptr) {
-                S v[kValues];
-#pragma unroll
-                for (int i = 0; i < kValues; i++) v[i] = y[i] * s[i] * w[i] * z[i] * (b[i] * q) * (1 - z[i]);
-                store_values<N, kPacks>(grad.gate + row * in.columns, v, member, team, packs);
-            }
-        if constexpr (GATE == kRowGate) {
-            sums.add_up(sum);
-            if (grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(sum[1]);
-        } else {
-            one[0] = sum[0];
-            sums.add_up(one);
-            sum[0] = one[0];
-        }
-        const S mean = sum[0] / C;
-#pragma unroll
-        for (int i = 0; i < kValues; i++) y[i] = q * (y[i] * s[i] * w[i] * z[i] - b[i] * q * mean);
-        if (grad.branch != nullptr) store_values<N, kPacks>(grad.branch + row * in.columns, y, member, team, packs);
+    V x, b, g, gs, gh, out, out_gate;
+    x.clear(), b.clear(), g.clear(), gs.clear(), gh.clear();
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team; row < in.rows; row += step) {
+        b.load(in.branch + row * in.branch_stride + member * N, member, team, packs);
+        x.load(in.residual + row * in.residual_stride + member * N, member, team, packs);
+        gh.load(grad.normed + row * grad.normed_stride + member * N, member, team, packs);
+        if constexpr (GATE == kFullGate) g.load(in.gate + row * in.gate_stride + member * N, member, team, packs);
+        const T gate = GATE == kRowGate ? in.gate[row * in.gate_stride] : T{};
+        gs.load(grad.stream + row * grad.stream_stride + member * N, member, team, packs);
+        const S q = work.inverse_rms(b, sums);
+        S squares, products, of_n, of_gate;
+        work.forward(x, b, g, gate, gh, q, squares, products);
+        sums.add_up(squares, products);
+        work.backward(out, out_gate, b, gs, gh, q, squares, products, of_n, of_gate);
+        const int64_t at = row * in.columns + member * N;
+        if (grad.residual != nullptr) out.store(grad.residual + at, member, team, packs);
+        if (GATE == kFullGate && grad.gate != nullptr) out_gate.store(grad.gate + at, member, team, packs);
+        if constexpr (GATE == kRowGate) sums.add_up(of_n, of_gate);
+        else sums.add_up(of_n);
+        if (GATE == kRowGate && grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(of_gate);
+        work.branch(out, b, q, of_n);
+        if (grad.branch != nullptr) out.store(grad.branch + at, member, team, packs);
     }
-    if (grad.columns == nullptr) return;
     // the teams of a block add to its sums one after the other
     S* own = grad.columns + static_cast<int64_t>(blockIdx.x) * 2 * in.columns;
     for (int t = 0; t < teams; t++) {
         if (t > 0) __syncthreads();
-        if (static_cast<int>(threadIdx.x) / team != t) continue;
-#pragma unroll
-        for (int i = 0; i < kValues; i++) {
-            const int pack = i / N * team + member;
-            if (pack >= packs) continue;
-            const int64_t c = static_cast<int64_t>(pack) * N + i % N;
-            own[c] = (t > 0 ? own[c] : S(0)) + of_branch[i];
-            own[in.columns + c] = (t > 0 ? own[in.columns + c] : S(0)) + of_output[i];
-        }
+        if (static_cast<int>(threadIdx.x) / team == t) work.leave(own, in, member, team, packs, t > 0);
     }
+}
+
+template <typename T, int GATE, int kPacks>
+__global__ void __launch_bounds__(kTeamThreads, kPacks * kPack<T> > kFewValues<T> ? 1 : 2)
+residual_norm_vjp_staged(const __grid_constant__ Gradients<T> grad, const __grid_constant__ Inputs<T> in, Status st) {
+    using S = Sum<T>;
+    constexpr int N = kPack<T>, kInputs = GATE == kFullGate ? 5 : 4;
+    using V = Values<T, N, kPacks>;
+    extern __shared__ __align__(128) unsigned char stages[];
+    __shared__ typename TeamSums<S>::Place shared[2];
+    __shared__ uint64_t full[kBackwardRing];
+    const int member = threadIdx.x, team = blockDim.x, packs = static_cast<int>(in.columns / N), columns = static_cast<int>(in.columns);
+    RowRing<T, kInputs, kBackwardRing> ring(stages, full, in.columns);
+    TeamSums<S> sums(shared, team); // (ends with a barrier: a team of one warp does not come here)
+    const int64_t step = gridDim.x;
+    auto fetch = [&](int64_t r, int place) {
+        if (threadIdx.x != 0 || r >= in.rows) return;
+        const T *b = in.branch + r * in.branch_stride, *x = in.residual + r * in.residual_stride;
+        const T *gh = grad.normed + r * grad.normed_stride, *gs = grad.stream + r * grad.stream_stride;
+        if constexpr (GATE == kFullGate) ring.fetch(place, {b, x, gh, gs, in.gate + r * in.gate_stride});
+        else ring.fetch(place, {b, x, gh, gs});
+    };
+    int64_t row = blockIdx.x;
+    for (int i = 0; i < kBackwardRing; i++) fetch(row + i * step, i);
+    Weights<T, N, kPacks, true> weights;
+    weights.load(in, member, team, packs, reinterpret_cast<S*>(stages + kBackwardRing * kInputs * ring.row_bytes));
+    RowBackward<T, GATE, N, kPacks, true> work(weights, in);
+    for (; row < in.rows; row += step, ring.next()) {
+        const T gate = GATE == kRowGate ? in.gate[row * in.gate_stride] : T{};
+        if (!ring.wait()) {
+            report_stalled(st);
+            return;
+        }
+        const T* first = ring.row() + member * N;
+        V b, out;
+        b.clear();
+        b.load(first, member, team, packs);
+        const S q = work.inverse_rms(b, sums);
+        S squares, products, of_n, of_gate;
+        {
+            V x, g, gh;
+            x.clear(), g.clear(), gh.clear();
+            x.load(first + columns, member, team, packs);
+            gh.load(first + 2 * columns, member, team, packs);
+            if constexpr (GATE == kFullGate) g.load(first + 4 * columns, member, team, packs);
+            work.forward(x, b, g, gate, gh, q, squares, products);
+        }
+        sums.add_up(squares, products);
+        const int64_t at = row * in.columns + member * N;
+        {
+            V gs, gh, out_gate;
+            gs.clear(), gh.clear();
+            gh.load(first + 2 * columns, member, team, packs);
+            gs.load(first + 3 * columns, member, team, packs);
+            work.backward(out, out_gate, b, gs, gh, q, squares, products, of_n, of_gate);
+            if (grad.residual != nullptr) out.store(grad.residual + at, member, team, packs);
+            if (GATE == kFullGate && grad.gate != nullptr) out_gate.store(grad.gate + at, member, team, packs);
+        }
+        if constexpr (GATE == kRowGate) sums.add_up(of_n, of_gate);
+        else sums.add_up(of_n);
+        // (everybody is done with the row's place)
+        fetch(row + kBackwardRing * step, ring.at);
+        if (GATE == kRowGate && grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(of_gate);
+        work.branch(out, b, q, of_n);
+        if (grad.branch != nullptr) out.store(grad.branch + at, member, team, packs);
+    }
+    work.leave(grad.columns + static_cast<int64_t>(blockIdx.x) * 2 * in.columns, in, member, team, packs, false);
 }
 
 // The sums over rows from those of the blocks: 32 warps add up a range of blocks each, for 32 columns, then those.
@@ -413,9 +664,6 @@ inline Teams teams_of(int64_t columns, int values) {
     const int team = static_cast<int>(ceil_div(needed, 32) * 32);
     return {team, team};
 }
-// Values of a thread, in 16-byte packs or one by one: eight of them (f64: four), or twice as many for long rows.
-template <typename T> constexpr int kFewValues = sizeof(T) == 8 ? 4 : 8;
-
 // Checks the inputs; returns which gate there is.
 Gate check_inputs(Array& residual, Array& branch, Array& gate, Array& scale, Array& weight_branch, Array& weight_output,
                   double epsilon, const std::string& op) {
@@ -453,6 +701,9 @@ Inputs<T> inputs_of(const Array& residual, const Array& branch, const Array& gat
     return {data(residual), data(branch), data(gate), data(scale), data(weight_branch), data(weight_output),
             residual.stride[0], branch.stride[0], gate.stride[0], residual.shape[0], residual.shape[1], epsilon};
 }
+
+// Whether a block may have so much dynamic shared memory beside its own.
+bool fits_block(const Call& call, size_t bytes) { return bytes + 4096 <= static_cast<size_t>(max_optin_smem(call.device)); }
 
 bool all_aligned(std::initializer_list<const Array*> arrays) {
     for (const Array* a : arrays)
@@ -499,6 +750,17 @@ void gated_residual_norm(Array stream, Array normed, Array residual, Array branc
                 constexpr int N = decltype(width)::value, kPacks = decltype(count)::value / N;
                 const Teams t = teams_of(in.columns, N * kPacks);
                 if (t.threads == 0) return false;
+                if constexpr (N > 1) {
+                    const size_t stages = static_cast<size_t>(kForwardRing) * (GATE == kFullGate ? 3 : 2) * in.columns * sizeof(T);
+                    if (t.team > 32 && fits_block(call, stages)) {
+                        auto kernel = residual_norm_staged<T, GATE, kPacks>;
+                        const int resident = resident_blocks(kernel, call.device, t.threads, stages) * sm_count(call.device);
+                        kernel<<<static_cast<unsigned>(t.blocks(in.rows, resident)), t.threads, stages, call.stream>>>(
+                            static_cast<T*>(stream.data), static_cast<T*>(normed.data), in, call.status);
+                        note_kernel_f("residual_norm_staged<%s,%d,%d>", array_type_name<T>(), GATE, kPacks);
+                        return true;
+                    }
+                }
                 auto kernel = residual_norm_rows<T, GATE, N, kPacks>;
                 const int resident = resident_blocks(kernel, call.device, t.threads, 0) * sm_count(call.device);
                 kernel<<<static_cast<unsigned>(t.blocks(in.rows, resident)), t.threads, 0, call.stream>>>(
@@ -571,6 +833,18 @@ void gated_residual_norm_vjp(Array grad_residual, Array grad_branch, Array grad_
                 constexpr int N = decltype(width)::value, kPacks = decltype(count)::value / N;
                 const Teams t = teams_of(columns, N * kPacks);
                 if (t.threads == 0) return false;
+                if constexpr (N > 1) {
+                    const size_t stages = static_cast<size_t>(kBackwardRing) * (GATE == kFullGate ? 5 : 4) * columns * sizeof(T) +
+                                          static_cast<size_t>(t.threads) * N * kPacks * sizeof(Sum<T>);
+                    if (t.team > 32 && fits_block(call, stages)) {
+                        auto kernel = residual_norm_vjp_staged<T, GATE, kPacks>;
+                        const int resident = resident_blocks(kernel, call.device, t.threads, stages) * sm_count(call.device);
+                        const Gradients<T> grad = room(t.blocks(rows, resident));
+                        kernel<<<static_cast<unsigned>(blocks), t.threads, stages, call.stream>>>(grad, in, call.status);
+                        note_kernel_f("residual_norm_vjp_staged<%s,%d,%d>", array_type_name<T>(), GATE, kPacks);
+                        return true;
+                    }
+                }
                 auto kernel = residual_norm_vjp_rows<T, GATE, N, kPacks>;
                 const int resident = resident_blocks(kernel, call.device, t.threads, 0) * sm_count(call.device);
                 const Gradients<T> grad = room(t.blocks(rows, resident));

@@ -445,7 +445,7 @@ std::map<std::tuple<const void*, int, int, size_t>, int> g_kernel_blocks;
 } // namespace
 
 void allow_dynamic_smem(const void* kernel, int device, size_t smem) {
-    if (smem <= 48 * 1024) return; // allowed as it is
+    if (smem <= 44 * 1024) return; // allowed as it is, beside what the kernel declares itself (48 KB together)
     std::lock_guard<std::mutex> lock(g_kernel_mutex);
     size_t& allowed = g_kernel_smem[{kernel, device}];
     if (smem <= allowed) return;
