@@ -70,133 +70,150 @@ embedding_rows(T* __restrict__ output, const T* __restrict__ W, int64_t stride, 
 }
 
 // ------------------------------------------------------------------------------ gradient
-// The sorted tokens are cut into chunks. A warp takes a chunk and a slab of 32 N columns and adds up the rows of grad_output, token
-// by token. A run of equal tokens that lies inside a chunk goes to its row of grad_W at once; of one
-// that a chunk's end cuts, each chunk leaves a partial sum (place 0: the run had begun before the chunk;
-// place 1: it begins in it and goes on after it), and embedding_join adds those up.
-constexpr int kRowsInFlight = 8; // loads of a warp under way
+// Few tokens: one block sorts them, in shared memory, while the others clear the rows of grad_W that no token asks for, which takes
+// longer. Digits of eight bits, lowest first, every pass stable: a warp's keys in order, warps in order.
+constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderItems = 16;
+constexpr int kFewTokens = kOrderThreads * kOrderItems;
+struct OrderMemory {
+    int32_t keys[kFewTokens];
+    uint16_t values[kFewTokens];
+    uint16_t counts[kOrderWarps][256]; // then: where a warp's next key with this digit goes
+    int32_t of_warp[8];
+};
+constexpr int kFlags = sizeof(OrderMemory); // rows that a block looks at together, a byte each
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kThreads)
-embedding_sums(T* __restrict__ grad_W, const T* __restrict__ grad_output, int64_t stride,
-               const int32_t* __restrict__ sorted, const int32_t* __restrict__ permutation, int64_t tokens, int64_t rows,
-               int64_t columns, int chunk, int64_t chunks, int64_t slabs, Sum<T> scale, Sum<T>* __restrict__ partial) {
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    if (unit >= chunks * slabs) return;
-    const int64_t c = unit / slabs;
-    const int64_t column = ((unit - c * slabs) * 32 + lane) * N;
-    const bool mine = column < columns;
-    const int64_t lo = c * chunk, hi = min(lo + chunk, tokens);
-    int32_t before = lo > 0 ? __ldg(sorted + lo - 1) : -1; // the key in front of the next entry
-    bool begun_before = true;                               // the run at hand began before the chunk
-    Sum<T> sum[N];
+__device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ sorted, int32_t* __restrict__ permutation,
+                                         const int32_t* __restrict__ indices, int tokens, int32_t rows, int32_t dropped, int passes, const Status& st) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rounds = (tokens + kOrderThreads - 1) / kOrderThreads, first = warp * rounds * 32 + lane;
+    int32_t key[kOrderItems];
+    uint32_t value[kOrderItems];
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < N; i++) sum[i] = 0;
-    for (int64_t base = lo; base < hi; base += 32) {
-        const int n = static_cast<int>(min(hi - base, int64_t(32)));
-        // the keys of 32 entries, and of the one behind them
-        const int32_t key = base + lane < tokens ? __ldg(sorted + base + lane) : -1;
-        const int32_t from = lane < n ? __ldg(permutation + base + lane) : 0;
-        const int32_t beyond = base + 32 < tokens ? __ldg(sorted + base + 32) : -1;
-        for (int j0 = 0; j0 < n; j0 += kRowsInFlight) {
-            Pack<T, N> value[kRowsInFlight];
+    for (int r = 0; r < kOrderItems; r++) {
+        const int at = first + r * 32;
+        value[r] = at;
+        if (r >= rounds || at >= tokens) continue;
+        key[r] = __ldg(indices + at);
+        const bool outside = static_cast<uint32_t>(key[r]) >= static_cast<uint32_t>(rows);
+        bad |= outside;
+        if (outside || key[r] == dropped) key[r] = rows;
+    }
+    if (bad) report_bad_index(st, 0);
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = 8 * pass;
+        for (int i = tid; i < kOrderWarps * 256 / 2; i += kOrderThreads) reinterpret_cast<uint32_t*>(m.counts)[i] = 0;
+        __syncthreads();
+        // each warp counts its digits
 #pragma unroll
-            for (int u = 0; u < kRowsInFlight; u++) {
-                const int64_t t = __shfl_sync(kFullMask, from, (j0 + u) & 31);
-                if (mine && j0 + u < n)
-                    value[u] = *reinterpret_cast<const Pack<T, N>*>(grad_output + t * stride + column);
+        for (int r = 0; r < kOrderItems; r++) {
+            if (r >= rounds) break;
+            const bool in = first + r * 32 < tokens;
+            const int digit = in ? key[r] >> shift & 255 : 256 + lane; // (lanes without a key match nobody)
+            const unsigned peers = __match_any_sync(kFullMask, digit);
+            if (in && (peers & ((1u << lane) - 1)) == 0) m.counts[warp][digit] += __popc(peers);
+            __syncwarp();
+        }
+        __syncthreads();
+        // where each warp's keys of a digit go: behind smaller digits, and behind earlier warps
+        int total = 0, up_to = 0;
+        if (tid < 256) {
+            for (int w = 0; w < kOrderWarps; w++) {
+                const int n = m.counts[w][tid];
+                m.counts[w][tid] = static_cast<uint16_t>(total);
+                total += n;
             }
+            up_to = total;
 #pragma unroll
-            for (int u = 0; u < kRowsInFlight; u++) {
-                const int j = j0 + u;
-                if (j >= n) break;
-                const int32_t k = __shfl_sync(kFullMask, key, j);
-                const int32_t next = j == 31 ? beyond : __shfl_sync(kFullMask, key, (j + 1) & 31);
-                if (k >= rows) return; // (sorted behind all others) tokens that give no gradient
-                if (k != before) {
-                    begun_before = false;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(kFullMask, up_to, d);
+                if (lane >= d) up_to += v;
+            }
+            if (lane == 31) m.of_warp[warp] = up_to;
+        }
+        __syncthreads();
+        if (tid < 256) {
+            int base = up_to - total;
+            for (int w = 0; w < warp; w++) base += m.of_warp[w];
+            for (int w = 0; w < kOrderWarps; w++) m.counts[w][tid] += static_cast<uint16_t>(base); // (at most 2^14)
+        }
+        __syncthreads();
+        const bool last = pass == passes - 1;
 #pragma unroll
-                    for (int i = 0; i < N; i++) sum[i] = 0;
-                }
-                before = k;
-                if (mine) {
+        for (int r = 0; r < kOrderItems; r++) {
+            if (r >= rounds) break;
+            const bool in = first + r * 32 < tokens;
+            const int digit = in ? key[r] >> shift & 255 : 256 + lane;
+            const unsigned peers = __match_any_sync(kFullMask, digit);
+            const int rank = __popc(peers & ((1u << lane) - 1));
+            int to = 0;
+            if (in) to = m.counts[warp][digit] + rank;
+            __syncwarp();
+            if (in && rank == 0) m.counts[warp][digit] += __popc(peers);
+            __syncwarp();
+            if (in && last) sorted[to] = key[r], permutation[to] = static_cast<int32_t>(value[r]);
+            if (in && !last) m.keys[to] = key[r], m.values[to] = static_cast<uint16_t>(value[r]);
+        }
+        if (last) return;
+        __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < N; i++) sum[i] += widen(value[u].v[i]);
-                }
-                const bool ends = next != k, cut = base + j == hi - 1 && !ends;
-                if (!ends && !cut) continue;
-                if (!mine) continue;
-                if (begun_before || cut) {
-                    Sum<T>* to = partial + (2 * c + (begun_before ? 0 : 1)) * columns + column;
+        for (int r = 0; r < kOrderItems; r++) {
+            const int at = first + r * 32;
+            if (r < rounds && at < tokens) key[r] = m.keys[at], value[r] = m.values[at];
+        }
+    }
+}
+
+// Clears the rows [lo, hi) that no token asks for. A block marks in shared memory which ones are, kFlags rows at a time.
+template <typename T, int N>
+__device__ __forceinline__ void clear_rows(unsigned char* flags, T* __restrict__ grad_W, const int32_t* __restrict__ indices, int tokens,
+                                           int64_t lo, int64_t hi, int32_t dropped, uint32_t packs, const Divider& by_packs) {
+    Pack<T, N> zero;
 #pragma unroll
-                    for (int i = 0; i < N; i++) to[i] = sum[i];
-                } else {
-                    Pack<T, N> out;
-#pragma unroll
-                    for (int i = 0; i < N; i++) out.v[i] = narrow<T>(sum[i] * scale);
-                    *reinterpret_cast<Pack<T, N>*>(grad_W + k * columns + column) = out;
-                }
+    for (int i = 0; i < N; i++) zero.v[i] = narrow<T>(0);
+    for (int64_t row0 = lo; row0 < hi; row0 += kFlags) {
+        const int here = static_cast<int>(min(hi - row0, int64_t(kFlags)));
+        __syncthreads();
+        for (int i = threadIdx.x; i < (here + 3) / 4; i += kOrderThreads) reinterpret_cast<uint32_t*>(flags)[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int t = threadIdx.x; t < tokens; t += kOrderThreads) {
+            const int32_t row = __ldg(indices + t);
+            if (row >= row0 && row < row0 + here && row != dropped) flags[row - row0] = 1;
+        }
+        __syncthreads();
+        // rows of whole multiples of a few thousand packs at a time, so that 32 bits do
+        const int group = max(1, static_cast<int>((1u << 30) / packs));
+        for (int r0 = 0; r0 < here; r0 += group) {
+            const uint32_t all = static_cast<uint32_t>(min(group, here - r0)) * packs;
+            for (uint32_t i = threadIdx.x; i < all; i += kOrderThreads) {
+                const uint32_t r = r0 + by_packs.divide(i), p = i - (r - r0) * packs;
+                if (!flags[r]) *reinterpret_cast<Pack<T, N>*>(grad_W + ((row0 + r) * packs + p) * N) = zero;
             }
         }
     }
 }
 
-// Adds up the partial sums of the run that begins in chunk blockIdx.x and goes on after it, if there is one: each warp
-// those of a range of chunks, then one after the other.
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads)
-embedding_join(T* __restrict__ grad_W, const int32_t* __restrict__ sorted, int64_t tokens, int64_t rows, int64_t columns,
-               int chunk, Sum<T> scale, const Sum<T>* __restrict__ partial) {
-    __shared__ Sum<T> joined[kWarps][32 * N];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = blockIdx.x, lo = c * chunk, last = lo + chunk - 1;
-    if (last + 1 >= tokens) return;
-    const int32_t k = __ldg(sorted + last);
-    if (k >= rows || __ldg(sorted + last + 1) != k) return;
-    if (lo > 0 && __ldg(sorted + lo - 1) == k) return;
-    const int64_t end = warp_lower_bound(sorted, last + 1, tokens, k + 1, lane); // (k < rows <= 2^31 - 1)
-    const int64_t n = (end - 1) / chunk - c + 1;                              // chunks of the run
-    const int64_t per = (n + kWarps - 1) / kWarps;
-    const int64_t from = min(warp * per, n), to = min(from + per, n);
-    for (int64_t slab = blockIdx.y; slab * 32 * N < columns; slab += gridDim.y) {
-        const int64_t column = (slab * 32 + lane) * N;
-        const bool mine = column < columns;
-        Sum<T> sum[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) sum[i] = 0;
-        if (mine) {
-#pragma unroll 8
-            for (int64_t i = from; i < to; i++) {
-                const Sum<T>* p = partial + (2 * (c + i) + (i == 0 ? 1 : 0)) * columns + column;
-#pragma unroll
-                for (int v = 0; v < N; v++) sum[v] += p[v];
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < N; v++) joined[warp][lane * N + v] = sum[v];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 32 * N; i += kThreads) {
-            const int64_t to_column = slab * 32 * N + i;
-            if (to_column >= columns) break;
-            Sum<T> all = 0;
-            for (int w = 0; w < kWarps; w++) all += joined[w][i];
-            grad_W[k * columns + to_column] = narrow<T>(all * scale);
-        }
-        __syncthreads();
+__global__ void __launch_bounds__(kOrderThreads, 1)
+embedding_order(T* __restrict__ grad_W, int32_t* __restrict__ sorted, int32_t* __restrict__ permutation, const int32_t* __restrict__ indices,
+                int tokens, int32_t rows, int32_t dropped, int passes, uint32_t packs, Divider by_packs, Status st) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    if (blockIdx.x == 0) {
+        sort_few(*reinterpret_cast<OrderMemory*>(memory), sorted, permutation, indices, tokens, rows, dropped, passes, st);
+    } else {
+        const int64_t blocks = gridDim.x - 1, b = blockIdx.x - 1;
+        clear_rows<T, N>(memory, grad_W, indices, tokens, rows * b / blocks, rows * (b + 1) / blocks, dropped, packs, by_packs);
     }
 }
 
-// Zeros for the rows that no token asks for: a block looks 64 rows up in the sorted tokens, a thread each, and clears those
+// Many tokens are sorted by kernels of their own (sort.cu). Then a block looks 64 rows up in the sorted tokens, a thread each, and clears those
 // that are not there.
 constexpr int kClearRows = 64;
-
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads)
-embedding_clear(T* __restrict__ grad_W, const int32_t* __restrict__ sorted, int64_t tokens, int64_t rows,
-                uint32_t packs, Divider by_packs) {
+__device__ __forceinline__ void clear_some_rows(int64_t row0, T* __restrict__ grad_W, const int32_t* __restrict__ sorted, int64_t tokens, int64_t rows,
+                                                uint32_t packs) {
     __shared__ bool empty[kClearRows];
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kClearRows;
     const int here = static_cast<int>(min(rows - row0, int64_t(kClearRows)));
     if (threadIdx.x < here) {
         const int32_t v = static_cast<int32_t>(row0 + threadIdx.x);
@@ -212,10 +229,149 @@ embedding_clear(T* __restrict__ grad_W, const int32_t* __restrict__ sorted, int6
     Pack<T, N> zero;
 #pragma unroll
     for (int i = 0; i < N; i++) zero.v[i] = narrow<T>(0);
-    for (int r = 0; r < here; r++) {
+    for (int r = threadIdx.x / 32; r < here; r += kWarps) {
         if (!empty[r]) continue;
-        for (uint32_t p = threadIdx.x; p < packs; p += kThreads)
+        for (uint32_t p = threadIdx.x % 32; p < packs; p += 32)
             *reinterpret_cast<Pack<T, N>*>(grad_W + ((row0 + r) * packs + p) * N) = zero;
+    }
+}
+
+// The sorted tokens are cut into chunks. A warp takes a chunk and a slab of 32 N columns and adds up the rows of grad_output, token
+// by token. A run of equal tokens that lies inside a chunk goes to its row of grad_W at once; of one
+// that a chunk's end cuts, each chunk leaves a partial sum (place 0: the run had begun before the chunk;
+// place 1: it begins in it and goes on after it), and embedding_join adds those up.
+// The first clear_blocks blocks clear rows instead.
+constexpr int kRowsInFlight = 8; // loads of a warp under way
+
+// (Partial sums are vectors of whole packs: slabs * 32 N columns.)
+template <typename S, int N> struct alignas(N * sizeof(S) < 16 ? N * sizeof(S) : 16) Sums {
+    S v[N];
+};
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads)
+embedding_sums(T* __restrict__ grad_W, const T* __restrict__ grad_output, int64_t stride,
+               const int32_t* __restrict__ sorted, const int32_t* __restrict__ permutation, int64_t tokens, int64_t rows,
+               int64_t columns, int chunk, int64_t chunks, int64_t slabs, Sum<T> scale, Sums<Sum<T>, N>* __restrict__ partial,
+               int64_t clear_blocks) {
+    if (blockIdx.x < clear_blocks) {
+        clear_some_rows<T, N>(blockIdx.x * int64_t(kClearRows), grad_W, sorted, tokens, rows, static_cast<uint32_t>(columns / N));
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (static_cast<int64_t>(blockIdx.x) - clear_blocks) * kWarps + (threadIdx.x >> 5);
+    if (unit >= chunks * slabs) return;
+    const int64_t c = unit / slabs, slab = unit - c * slabs;
+    const int64_t column = (slab * 32 + lane) * N;
+    const bool mine = column < columns;
+    const int64_t lo = c * chunk, hi = min(lo + chunk, tokens);
+    int32_t before = lo > 0 ? __ldg(sorted + lo - 1) : -1; // the key in front of the next entry
+    bool begun_before = true;                               // the run at hand began before the chunk
+    Sums<Sum<T>, N> sum;
+#pragma unroll
+    for (int i = 0; i < N; i++) sum.v[i] = 0;
+    for (int64_t base = lo; base < hi; base += 32) {
+        const int n = static_cast<int>(min(hi - base, int64_t(32)));
+        // the keys of 32 entries, and of the one behind them
+        const int32_t key = base + lane < tokens ? __ldg(sorted + base + lane) : -1;
+        const int32_t from = lane < n ? __ldg(permutation + base + lane) : 0;
+        const int32_t beyond = base + 32 < tokens ? __ldg(sorted + base + 32) : -1;
+        int32_t after = __shfl_down_sync(kFullMask, key, 1);
+        if (lane == 31) after = beyond;
+        // entries whose run ends with them, and those that give no gradient (sorted behind all others)
+        const unsigned ends = __ballot_sync(kFullMask, after != key), none = __ballot_sync(kFullMask, key >= rows);
+        for (int j0 = 0; j0 < n; j0 += kRowsInFlight) {
+            Pack<T, N> value[kRowsInFlight];
+#pragma unroll
+            for (int u = 0; u < kRowsInFlight; u++) {
+                const int64_t t = __shfl_sync(kFullMask, from, (j0 + u) & 31);
+                if (mine && j0 + u < n && !(none >> ((j0 + u) & 31) & 1))
+                    value[u] = *reinterpret_cast<const Pack<T, N>*>(grad_output + t * stride + column);
+            }
+#pragma unroll
+            for (int u = 0; u < kRowsInFlight; u++) {
+                const int j = j0 + u;
+                if (j >= n) break;
+                if (none >> j & 1) return;
+                const int32_t k = __shfl_sync(kFullMask, key, j);
+                if (k != before) {
+                    begun_before = false;
+#pragma unroll
+                    for (int i = 0; i < N; i++) sum.v[i] = 0;
+                }
+                before = k;
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) sum.v[i] += widen(value[u].v[i]);
+                }
+                const bool end = ends >> j & 1, cut = base + j == hi - 1 && !end;
+                if (!end && !cut) continue;
+                if (begun_before || cut) {
+                    partial[((2 * c + (begun_before ? 0 : 1)) * slabs + slab) * 32 + lane] = sum;
+                } else if (mine) {
+                    Pack<T, N> out;
+#pragma unroll
+                    for (int i = 0; i < N; i++) out.v[i] = narrow<T>(sum.v[i] * scale);
+                    *reinterpret_cast<Pack<T, N>*>(grad_W + k * columns + column) = out;
+                }
+            }
+        }
+    }
+}
+
+// Adds up the partial sums of the run that begins in chunk blockIdx.x and goes on after it, if there is one: each warp
+// those of a range of chunks, then one after the other.
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads)
+embedding_join(T* __restrict__ grad_W, const int32_t* __restrict__ sorted, int64_t tokens, int64_t rows, int64_t columns,
+               int chunk, int64_t slabs, Sum<T> scale, const Sums<Sum<T>, N>* __restrict__ partial) {
+    __shared__ Sums<Sum<T>, N> joined[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = blockIdx.x, lo = c * chunk, last = lo + chunk - 1;
+    if (last + 1 >= tokens) return;
+    const int32_t k = __ldg(sorted + last), next = __ldg(sorted + last + 1), before = lo > 0 ? __ldg(sorted + lo - 1) : -1;
+    if (k >= rows || next != k || before == k) return;
+    // its end: mostly in the next chunk
+    const int64_t near = min(last + 1 + 32, tokens);
+    const bool same = last + 1 + lane < near && __ldg(sorted + last + 1 + lane) == k;
+    const unsigned run = __ballot_sync(kFullMask, same);
+    const int64_t end = run == kFullMask ? warp_lower_bound(sorted, near, tokens, k + 1, lane) // (k < rows <= 2^31 - 1)
+                                         : last + 1 + __popc(run);
+    const int64_t n = (end - 1) / chunk - c + 1; // chunks of the run
+    const int64_t per = (n + kWarps - 1) / kWarps;
+    const int64_t from = min(warp * per, n), to = min(from + per, n);
+    for (int64_t slab = blockIdx.y; slab < slabs; slab += gridDim.y) {
+        Sums<Sum<T>, N> sum;
+#pragma unroll
+        for (int i = 0; i < N; i++) sum.v[i] = 0;
+        auto part = [&](int64_t i) { return partial[((2 * (c + i) + (i == 0 ? 1 : 0)) * slabs + slab) * 32 + lane]; };
+        int64_t i = from;
+        for (; i + 4 <= to; i += 4) {
+            Sums<Sum<T>, N> v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = part(i + u);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int x = 0; x < N; x++) sum.v[x] += v[u].v[x];
+        }
+        for (; i < to; i++) {
+            const Sums<Sum<T>, N> v = part(i);
+#pragma unroll
+            for (int x = 0; x < N; x++) sum.v[x] += v.v[x];
+        }
+        joined[warp][lane] = sum;
+        __syncthreads();
+        const int used = static_cast<int>(min((n + per - 1) / per, int64_t(kWarps)));
+        const Sum<T>* all = reinterpret_cast<const Sum<T>*>(joined);
+        for (int x = threadIdx.x; x < 32 * N; x += kThreads) {
+            const int64_t to_column = slab * 32 * N + x;
+            if (to_column >= columns) break;
+            Sum<T> total = 0;
+            for (int w = 0; w < used; w++) total += all[w * 32 * N + x];
+            grad_W[k * columns + to_column] = narrow<T>(total * scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -284,34 +440,44 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
     unsigned char* order = static_cast<unsigned char*>(scratch_alloc(call, 2 * index_room + 256));
     int32_t* sorted = reinterpret_cast<int32_t*>(order);
     int32_t* permutation = reinterpret_cast<int32_t*>(order + index_room);
-    // tokens outside of the table and those of the padding row sort behind all others
-    if (tokens > 0)
-        sort_keys(call, sorted, permutation, static_cast<const int32_t*>(indices.data), tokens, rows,
-                  static_cast<int32_t>(rows), static_cast<int32_t>(padding_index));
+    const int32_t* given = static_cast<const int32_t*>(indices.data);
     for_type(grad_W.type, [&](auto zero) {
         using T = decltype(zero);
         auto launch = [&](auto width) {
             constexpr int N = decltype(width)::value;
             const int64_t packs = columns / N, slabs = ceil_div(columns, 32 * N);
+            T* out = static_cast<T*>(grad_W.data);
+            // tokens outside of the table and those of the padding row sort behind all others
+            int64_t clear_blocks = ceil_div(rows, kClearRows);
+            if (tokens <= kFewTokens) {
+                int bits = 1;
+                while ((int64_t(1) << bits) < rows + 1) bits++;
+                auto kernel = embedding_order<T, N>;
+                allow_dynamic_smem(kernel, call.device, sizeof(OrderMemory));
+                const int64_t blocks = std::min<int64_t>(ceil_div(rows * packs, 4 * kOrderThreads), sm_count(call.device) - 1);
+                kernel<<<grid_of(1 + blocks, op), kOrderThreads, sizeof(OrderMemory), call.stream>>>(
+                    out, sorted, permutation, given, static_cast<int>(tokens), static_cast<int32_t>(rows), static_cast<int32_t>(padding_index),
+                    (bits + 7) / 8, static_cast<uint32_t>(packs), Divider(static_cast<uint32_t>(packs)), call.status);
+                note_kernel_f("embedding_order<%s,%d>", array_type_name<T>(), N);
+                clear_blocks = 0;
+                if (tokens == 0) return;
+            } else {
+                sort_keys(call, sorted, permutation, given, tokens, rows, static_cast<int32_t>(rows), static_cast<int32_t>(padding_index));
+            }
             // Chunks as long as they can be while there are some 30 warps for each SM.
             int chunk = 256;
             while (chunk > 32 && ceil_div(tokens, chunk) * slabs < int64_t(sm_count(call.device)) * 32) chunk /= 2;
             const int64_t chunks = ceil_div(tokens, chunk);
-            T* out = static_cast<T*>(grad_W.data);
-            embedding_clear<T, N><<<grid_of(ceil_div(rows, kClearRows), op), kThreads, 0, call.stream>>>(
-                out, sorted, tokens, rows, static_cast<uint32_t>(packs), Divider(static_cast<uint32_t>(packs)));
-            if (tokens > 0) {
-                Sum<T>* partial = static_cast<Sum<T>*>(
-                    scratch_alloc(call, static_cast<size_t>(2 * chunks * columns) * sizeof(Sum<T>)));
-                embedding_sums<T, N><<<grid_of(ceil_div(chunks * slabs, kWarps), op), kThreads, 0, call.stream>>>(
-                    out, static_cast<const T*>(grad_output.data), grad_output.stride[0], sorted, permutation, tokens, rows,
-                    columns, chunk, chunks, slabs, static_cast<Sum<T>>(scale), partial);
-                if (chunks > 1)
-                    embedding_join<T, N>
-                        <<<dim3(grid_of(chunks, op), static_cast<unsigned>(std::min<int64_t>(slabs, 65535))), kThreads, 0,
-                           call.stream>>>(out, sorted, tokens, rows, columns, chunk, static_cast<Sum<T>>(scale), partial);
-                scratch_free(call, partial);
-            }
+            using P = Sums<Sum<T>, N>;
+            P* partial = static_cast<P*>(scratch_alloc(call, static_cast<size_t>(2 * chunks * slabs * 32) * sizeof(P)));
+            embedding_sums<T, N><<<grid_of(clear_blocks + ceil_div(chunks * slabs, kWarps), op), kThreads, 0, call.stream>>>(
+                out, static_cast<const T*>(grad_output.data), grad_output.stride[0], sorted, permutation, tokens, rows,
+                columns, chunk, chunks, slabs, static_cast<Sum<T>>(scale), partial, clear_blocks);
+            if (chunks > 1)
+                embedding_join<T, N>
+                    <<<dim3(grid_of(chunks, op), static_cast<unsigned>(std::min<int64_t>(slabs, 65535))), kThreads, 0, call.stream>>>(
+                        out, sorted, tokens, rows, columns, chunk, slabs, static_cast<Sum<T>>(scale), partial);
+            scratch_free(call, partial);
             note_kernel_f("embedding_sums<%s,%d>", array_type_name<T>(), N);
         };
         if (aligned16(grad_W) && aligned16(grad_output)) launch(std::integral_constant<int, kPack<T>>());
