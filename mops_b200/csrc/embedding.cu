@@ -77,29 +77,43 @@ constexpr int kFewTokens = kOrderThreads * kOrderItems;
 struct OrderMemory {
     int32_t keys[kFewTokens];
     uint16_t values[kFewTokens];
-    uint16_t counts[kOrderWarps][256]; // then: where a warp's next key with this digit goes
-    int32_t of_warp[8];
+    uint16_t counts[kOrderWarps][256]; // then: how many of a digit earlier warps have
+    int32_t of_warp[8], first[256];       // of each digit
 };
 constexpr int kFlags = sizeof(OrderMemory); // rows that a block looks at together, a byte each
+
+// The lanes whose digit is the caller's (of those that have one), by a ballot for each bit: a few instructions each, where __match_any_sync
+// takes hundreds of clocks with all warps of an SM at it.
+__device__ __forceinline__ unsigned lanes_with(int digit, bool in) {
+    unsigned peers = __ballot_sync(kFullMask, in);
+#pragma unroll
+    for (int bit = 0; bit < 8; bit++) {
+        const unsigned set = __ballot_sync(kFullMask, digit >> bit & 1);
+        peers &= digit >> bit & 1 ? set : ~set;
+    }
+    return peers;
+}
 
 __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ sorted, int32_t* __restrict__ permutation,
                                          const int32_t* __restrict__ indices, int tokens, int32_t rows, int32_t dropped, int passes, const Status& st) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rounds = (tokens + kOrderThreads - 1) / kOrderThreads, first = warp * rounds * 32 + lane;
     int32_t key[kOrderItems];
-    uint32_t value[kOrderItems];
-    bool bad = false;
+    uint32_t value[kOrderItems]; // where the key was; above that, the place among the warp's keys of its digit
 #pragma unroll
     for (int r = 0; r < kOrderItems; r++) {
         const int at = first + r * 32;
         value[r] = at;
-        if (r >= rounds || at >= tokens) continue;
-        key[r] = __ldg(indices + at);
+        key[r] = r < rounds && at < tokens ? __ldg(indices + at) : 0;
+    }
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < kOrderItems; r++) {
         const bool outside = static_cast<uint32_t>(key[r]) >= static_cast<uint32_t>(rows);
         bad |= outside;
         if (outside || key[r] == dropped) key[r] = rows;
     }
-    if (bad) report_bad_index(st, 0);
+    if (bad && rows > 0) report_bad_index(st, 0);
     for (int pass = 0; pass < passes; pass++) {
         const int shift = 8 * pass;
         for (int i = tid; i < kOrderWarps * 256 / 2; i += kOrderThreads) reinterpret_cast<uint32_t*>(m.counts)[i] = 0;
@@ -109,9 +123,12 @@ __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ s
         for (int r = 0; r < kOrderItems; r++) {
             if (r >= rounds) break;
             const bool in = first + r * 32 < tokens;
-            const int digit = in ? key[r] >> shift & 255 : 256 + lane; // (lanes without a key match nobody)
-            const unsigned peers = __match_any_sync(kFullMask, digit);
-            if (in && (peers & ((1u << lane) - 1)) == 0) m.counts[warp][digit] += __popc(peers);
+            const int digit = key[r] >> shift & 255;
+            const unsigned peers = lanes_with(digit, in);
+            const int rank = __popc(peers & ((1u << lane) - 1));
+            if (in) value[r] |= static_cast<uint32_t>(m.counts[warp][digit] + rank) << 16;
+            __syncwarp();
+            if (in && rank == 0) m.counts[warp][digit] += __popc(peers);
             __syncwarp();
         }
         __syncthreads();
@@ -135,33 +152,26 @@ __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ s
         if (tid < 256) {
             int base = up_to - total;
             for (int w = 0; w < warp; w++) base += m.of_warp[w];
-            for (int w = 0; w < kOrderWarps; w++) m.counts[w][tid] += static_cast<uint16_t>(base); // (at most 2^14)
+            m.first[tid] = base;
         }
         __syncthreads();
-        const bool last = pass == passes - 1;
 #pragma unroll
         for (int r = 0; r < kOrderItems; r++) {
-            if (r >= rounds) break;
-            const bool in = first + r * 32 < tokens;
-            const int digit = in ? key[r] >> shift & 255 : 256 + lane;
-            const unsigned peers = __match_any_sync(kFullMask, digit);
-            const int rank = __popc(peers & ((1u << lane) - 1));
-            int to = 0;
-            if (in) to = m.counts[warp][digit] + rank;
-            __syncwarp();
-            if (in && rank == 0) m.counts[warp][digit] += __popc(peers);
-            __syncwarp();
-            if (in && last) sorted[to] = key[r], permutation[to] = static_cast<int32_t>(value[r]);
-            if (in && !last) m.keys[to] = key[r], m.values[to] = static_cast<uint16_t>(value[r]);
+            if (r >= rounds || first + r * 32 >= tokens) break;
+            const int digit = key[r] >> shift & 255;
+            const int to = m.first[digit] + m.counts[warp][digit] + (value[r] >> 16);
+            m.keys[to] = key[r];
+            m.values[to] = static_cast<uint16_t>(value[r]);
         }
-        if (last) return;
         __syncthreads();
+        if (pass == passes - 1) break;
 #pragma unroll
         for (int r = 0; r < kOrderItems; r++) {
             const int at = first + r * 32;
             if (r < rounds && at < tokens) key[r] = m.keys[at], value[r] = m.values[at];
         }
     }
+    for (int i = tid; i < tokens; i += kOrderThreads) sorted[i] = m.keys[i], permutation[i] = m.values[i];
 }
 
 // Clears the rows [lo, hi) that no token asks for. A block marks in shared memory which ones are, kFlags rows at a time.
@@ -241,15 +251,30 @@ __device__ __forceinline__ void clear_some_rows(int64_t row0, T* __restrict__ gr
 // that a chunk's end cuts, each chunk leaves a partial sum (place 0: the run had begun before the chunk;
 // place 1: it begins in it and goes on after it), and embedding_join adds those up.
 // The first clear_blocks blocks clear rows instead.
-constexpr int kRowsInFlight = 8; // loads of a warp under way
+constexpr int kRowsInFlight = 16; // loads of a warp under way
 
 // (Partial sums are vectors of whole packs: slabs * 32 N columns.)
 template <typename S, int N> struct alignas(N * sizeof(S) < 16 ? N * sizeof(S) : 16) Sums {
     S v[N];
 };
 
+// Keeps loaded packs as they are up to here.
+template <typename T, int N, int M> __device__ __forceinline__ void keep_packed(Pack<T, N> (&v)[M]) {
+    if constexpr (N * sizeof(T) == 16) {
+#pragma unroll
+        for (int u = 0; u < M; u++) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v[u]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) asm volatile("" : "+r"(w[i]));
+        }
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int u = 0; u < M; u++) asm volatile("" : "+h"(*reinterpret_cast<uint16_t*>(&v[u])));
+    }
+}
+
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 embedding_sums(T* __restrict__ grad_W, const T* __restrict__ grad_output, int64_t stride,
                const int32_t* __restrict__ sorted, const int32_t* __restrict__ permutation, int64_t tokens, int64_t rows,
                int64_t columns, int chunk, int64_t chunks, int64_t slabs, Sum<T> scale, Sums<Sum<T>, N>* __restrict__ partial,
@@ -264,58 +289,73 @@ embedding_sums(T* __restrict__ grad_W, const T* __restrict__ grad_output, int64_
     const int64_t c = unit / slabs, slab = unit - c * slabs;
     const int64_t column = (slab * 32 + lane) * N;
     const bool mine = column < columns;
+    const T* from_column = grad_output + (mine ? column : 0);
     const int64_t lo = c * chunk, hi = min(lo + chunk, tokens);
-    int32_t before = lo > 0 ? __ldg(sorted + lo - 1) : -1; // the key in front of the next entry
-    bool begun_before = true;                               // the run at hand began before the chunk
+    bool begun_before = true; // the run at hand began before the chunk
     Sums<Sum<T>, N> sum;
 #pragma unroll
     for (int i = 0; i < N; i++) sum.v[i] = 0;
     for (int64_t base = lo; base < hi; base += 32) {
         const int n = static_cast<int>(min(hi - base, int64_t(32)));
-        // the keys of 32 entries, and of the one behind them
+        // the keys of 32 entries, of the one in front of them and of the one behind them
         const int32_t key = base + lane < tokens ? __ldg(sorted + base + lane) : -1;
         const int32_t from = lane < n ? __ldg(permutation + base + lane) : 0;
-        const int32_t beyond = base + 32 < tokens ? __ldg(sorted + base + 32) : -1;
-        int32_t after = __shfl_down_sync(kFullMask, key, 1);
-        if (lane == 31) after = beyond;
-        // entries whose run ends with them, and those that give no gradient (sorted behind all others)
-        const unsigned ends = __ballot_sync(kFullMask, after != key), none = __ballot_sync(kFullMask, key >= rows);
-        for (int j0 = 0; j0 < n; j0 += kRowsInFlight) {
+        int32_t before = __shfl_up_sync(kFullMask, key, 1), after = __shfl_down_sync(kFullMask, key, 1);
+        if (lane == 0) before = base > 0 ? __ldg(sorted + base - 1) : -1;
+        if (lane == 31) after = base + 32 < tokens ? __ldg(sorted + base + 32) : -1;
+        // entries that begin a run and that end one, and those that give no gradient (sorted behind all others)
+        const unsigned begins = __ballot_sync(kFullMask, before != key), ends = __ballot_sync(kFullMask, after != key);
+        const int valid = __popc(__ballot_sync(kFullMask, lane < n && key < rows));
+        const int64_t offset = from * stride; // (of lane's entry)
+        const uint32_t offset_lo = static_cast<uint32_t>(offset), offset_hi = static_cast<uint32_t>(offset >> 32);
+        auto leave = [&](int j) { // the run ends with entry j, or the chunk does
+            if (begun_before || !(ends >> j & 1)) {
+                partial[((2 * c + (begun_before ? 0 : 1)) * slabs + slab) * 32 + lane] = sum;
+                return;
+            }
+            const int64_t k = __shfl_sync(kFullMask, key, j);
+            Pack<T, N> out;
+#pragma unroll
+            for (int i = 0; i < N; i++) out.v[i] = narrow<T>(sum.v[i] * scale);
+            if (mine) *reinterpret_cast<Pack<T, N>*>(grad_W + k * columns + column) = out;
+        };
+        auto restart = [&] {
+            begun_before = false;
+#pragma unroll
+            for (int i = 0; i < N; i++) sum.v[i] = 0;
+        };
+        for (int j0 = 0; j0 < valid; j0 += kRowsInFlight) {
             Pack<T, N> value[kRowsInFlight];
 #pragma unroll
-            for (int u = 0; u < kRowsInFlight; u++) {
-                const int64_t t = __shfl_sync(kFullMask, from, (j0 + u) & 31);
-                if (mine && j0 + u < n && !(none >> ((j0 + u) & 31) & 1))
-                    value[u] = *reinterpret_cast<const Pack<T, N>*>(grad_output + t * stride + column);
+            for (int u = 0; u < kRowsInFlight; u++) { // (the last entry again where there are no more, and the first column)
+                const int j = min(j0 + u, valid - 1);
+                const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(__shfl_sync(kFullMask, offset_hi, j)) << 32 |
+                                                        __shfl_sync(kFullMask, offset_lo, j));
+                value[u] = *reinterpret_cast<const Pack<T, N>*>(from_column + at);
+            }
+            keep_packed(value); // (else each load is waited for, to be widened, before the next)
+            const unsigned group = (1u << kRowsInFlight) - 1;
+            if (j0 + kRowsInFlight <= valid && !((begins >> j0 >> 1 | ends >> j0) & group >> 1)) { // one run
+                if (begins >> j0 & 1) restart();
+#pragma unroll
+                for (int u = 0; u < kRowsInFlight; u++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) sum.v[i] += widen(value[u].v[i]);
+                const int j = j0 + kRowsInFlight - 1;
+                if (ends >> j & 1 || base + j == hi - 1) leave(j);
+                continue;
             }
 #pragma unroll
             for (int u = 0; u < kRowsInFlight; u++) {
                 const int j = j0 + u;
-                if (j >= n) break;
-                if (none >> j & 1) return;
-                const int32_t k = __shfl_sync(kFullMask, key, j);
-                if (k != before) {
-                    begun_before = false;
+                if (j >= valid) break;
+                if (begins >> j & 1) restart();
 #pragma unroll
-                    for (int i = 0; i < N; i++) sum.v[i] = 0;
-                }
-                before = k;
-                if (mine) {
-#pragma unroll
-                    for (int i = 0; i < N; i++) sum.v[i] += widen(value[u].v[i]);
-                }
-                const bool end = ends >> j & 1, cut = base + j == hi - 1 && !end;
-                if (!end && !cut) continue;
-                if (begun_before || cut) {
-                    partial[((2 * c + (begun_before ? 0 : 1)) * slabs + slab) * 32 + lane] = sum;
-                } else if (mine) {
-                    Pack<T, N> out;
-#pragma unroll
-                    for (int i = 0; i < N; i++) out.v[i] = narrow<T>(sum.v[i] * scale);
-                    *reinterpret_cast<Pack<T, N>*>(grad_W + k * columns + column) = out;
-                }
+                for (int i = 0; i < N; i++) sum.v[i] += widen(value[u].v[i]);
+                if (ends >> j & 1 || base + j == hi - 1) leave(j);
             }
         }
+        if (valid < n) return;
     }
 }
 
@@ -466,7 +506,7 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
             }
             // Chunks as long as they can be while there are some 30 warps for each SM.
             int chunk = 256;
-            while (chunk > 32 && ceil_div(tokens, chunk) * slabs < int64_t(sm_count(call.device)) * 32) chunk /= 2;
+            while (chunk > kRowsInFlight && ceil_div(tokens, chunk) * slabs < int64_t(sm_count(call.device)) * 32) chunk /= 2;
             const int64_t chunks = ceil_div(tokens, chunk);
             using P = Sums<Sum<T>, N>;
             P* partial = static_cast<P*>(scratch_alloc(call, static_cast<size_t>(2 * chunks * slabs * 32) * sizeof(P)));
