@@ -251,7 +251,7 @@ __device__ __forceinline__ void clear_some_rows(int64_t row0, T* __restrict__ gr
 // that a chunk's end cuts, each chunk leaves a partial sum (place 0: the run had begun before the chunk;
 // place 1: it begins in it and goes on after it), and embedding_join adds those up.
 // The first clear_blocks blocks clear rows instead.
-constexpr int kRowsInFlight = 16; // loads of a warp under way
+constexpr int kRowsInFlight = 8; // loads of a warp under way
 
 // (Partial sums are vectors of whole packs: slabs * 32 N columns.)
 template <typename S, int N> struct alignas(N * sizeof(S) < 16 ? N * sizeof(S) : 16) Sums {
@@ -274,7 +274,7 @@ template <typename T, int N, int M> __device__ __forceinline__ void keep_packed(
 }
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 4)
 embedding_sums(T* __restrict__ grad_W, const T* __restrict__ grad_output, int64_t stride,
                const int32_t* __restrict__ sorted, const int32_t* __restrict__ permutation, int64_t tokens, int64_t rows,
                int64_t columns, int chunk, int64_t chunks, int64_t slabs, Sum<T> scale, Sums<Sum<T>, N>* __restrict__ partial,
@@ -386,12 +386,13 @@ embedding_join(T* __restrict__ grad_W, const int32_t* __restrict__ sorted, int64
         for (int i = 0; i < N; i++) sum.v[i] = 0;
         auto part = [&](int64_t i) { return partial[((2 * (c + i) + (i == 0 ? 1 : 0)) * slabs + slab) * 32 + lane]; };
         int64_t i = from;
-        for (; i + 4 <= to; i += 4) {
-            Sums<Sum<T>, N> v[4];
+        constexpr int kAtOnce = 32 / N < 8 ? 32 / N : 8;
+        for (; i + kAtOnce <= to; i += kAtOnce) {
+            Sums<Sum<T>, N> v[kAtOnce];
 #pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = part(i + u);
+            for (int u = 0; u < kAtOnce; u++) v[u] = part(i + u);
 #pragma unroll
-            for (int u = 0; u < 4; u++)
+            for (int u = 0; u < kAtOnce; u++)
 #pragma unroll
                 for (int x = 0; x < N; x++) sum.v[x] += v[u].v[x];
         }
@@ -506,7 +507,7 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
             }
             // Chunks as long as they can be while there are some 30 warps for each SM.
             int chunk = 256;
-            while (chunk > kRowsInFlight && ceil_div(tokens, chunk) * slabs < int64_t(sm_count(call.device)) * 32) chunk /= 2;
+            while (chunk > 16 && ceil_div(tokens, chunk) * slabs < int64_t(sm_count(call.device)) * 32) chunk /= 2;
             const int64_t chunks = ceil_div(tokens, chunk);
             using P = Sums<Sum<T>, N>;
             P* partial = static_cast<P*>(scratch_alloc(call, static_cast<size_t>(2 * chunks * slabs * 32) * sizeof(P)));
