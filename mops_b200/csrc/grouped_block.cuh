@@ -21,6 +21,11 @@ template <int N> struct Turn {
     __device__ __forceinline__ void next() {
         if (++at == N) at = 0, round ^= 1;
     }
+    __device__ __forceinline__ void skip(int n) {
+        at += n;
+        round ^= static_cast<unsigned>(at / N) & 1;
+        at %= N;
+    }
 };
 
 // Between those who fill the places of a ring and those who empty them.
@@ -41,7 +46,8 @@ __device__ __forceinline__ void banded(int64_t at, int64_t rows, int64_t columns
 }
 
 // What the kernels share: setting up, waiting and leaving. A wait that runs out is reported, and everybody leaves. L says how shared memory is
-// laid out, how many columns of tensor memory there are, and what the rings are (L::Rings, with begin(), `tmem` and `gave_up`).
+// laid out, how many columns of tensor memory there are, what the rings are (L::Rings, with begin(), `tmem` and `gave_up`), and whether two blocks
+// work as a pair (L::kPair).
 template <typename L> struct Block {
     unsigned char* smem;
     typename L::Rings* rings;
@@ -54,25 +60,40 @@ template <typename L> struct Block {
         base = smem_address(smem);
     }
     __device__ void begin(int warp) {
-        if (warp == 1) tmem_alloc(&rings->tmem, L::kTmem);
+        if (warp == 1) {
+            if constexpr (L::kPair) pair_tmem_alloc(&rings->tmem, L::kTmem);
+            else tmem_alloc(&rings->tmem, L::kTmem);
+        }
         if (threadIdx.x == 0) {
             rings->begin();
             rings->gave_up = 0;
             mbarrier_init_fence();
         }
+        sync();
+    }
+    __device__ void sync() {
         tmem_fence_before_sync();
         __syncthreads();
+        if constexpr (L::kPair) pair_sync(); // (neither block leaves while the other may reach into its memory)
         tmem_fence_after_sync();
     }
     __device__ void end(int warp) {
-        tmem_fence_before_sync();
-        __syncthreads();
-        tmem_fence_after_sync();
-        if (warp == 1) tmem_free(rings->tmem, L::kTmem);
+        sync();
+        if (warp == 1) {
+            if constexpr (L::kPair) pair_tmem_free(rings->tmem, L::kTmem);
+            else tmem_free(rings->tmem, L::kTmem);
+        }
     }
-    __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity) {
-        if (mbarrier_try_wait(bar, parity)) return true;
-        if (*static_cast<volatile int*>(&rings->gave_up) == 0 && mbarrier_wait(bar, parity)) return true;
+    template <bool kOfPair> __device__ __forceinline__ static bool passed(uint64_t* bar, unsigned parity) {
+        if constexpr (kOfPair) return mbarrier_try_wait_pair(bar, parity);
+        else return mbarrier_try_wait(bar, parity);
+    }
+    // For about a second, as mbarrier_wait. kOfPair: for what threads of the other block have written, too.
+    template <bool kOfPair = false> __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity) {
+        if (passed<kOfPair>(bar, parity)) return true;
+        const long long start = clock64();
+        while (*static_cast<volatile int*>(&rings->gave_up) == 0 && clock64() - start < 2000000000LL)
+            if (passed<kOfPair>(bar, parity)) return true;
         if (atomicExch(&rings->gave_up, 1) == 0) report_stalled(st);
         return false;
     }
@@ -124,38 +145,38 @@ __device__ __forceinline__ int64_t parts_before(const int32_t* __restrict__ offs
 }
 
 // Adds up the parts of a tile, in the order of the rows.
-template <typename T, int kColumns>
+template <typename T, int kRows, int kColumns>
 static __global__ void __launch_bounds__(256)
 grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t most_parts,
                    const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment) {
     const int lane = threadIdx.x & 31;
-    const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
+    const int64_t row_tiles = (height + kRows - 1) / kRows, column_tiles = (columns + kColumns - 1) / kColumns;
     const int64_t tiles = row_tiles * column_tiles;
     GroupWalk<OuterJoins> walk(offsets, groups, rows, 0, groups - 1, OuterJoins{segment, tiles});
     const GroupPiece piece = walk.find(blockIdx.x, lane);
     if (!piece.found) return;
     int64_t tile_row, tile_column;
     banded(piece.within, row_tiles, column_tiles, tile_row, tile_column);
-    const int row = static_cast<int>(tile_row) * kTileRows, column = static_cast<int>(tile_column) * kColumns;
+    const int row = static_cast<int>(tile_row) * kRows, column = static_cast<int>(tile_column) * kColumns;
     const int64_t n = (piece.hi - piece.lo + segment - 1) / segment;
     const int64_t first = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
     if (first + (n - 1) * tiles >= most_parts) return;
     // four values to a thread
     const int at = (blockIdx.y * 256 + threadIdx.x) * 4, i = at / kColumns, j = at % kColumns;
     if (row + i >= height || column + j >= columns) return;
-    const float* from = parts + (first * kTileRows + i) * kColumns + j;
+    const float* from = parts + (first * kRows + i) * kColumns + j;
     float4 sum = make_float4(0, 0, 0, 0);
     int64_t s = 0;
     constexpr int kInFlight = 8;
     for (; s + kInFlight <= n; s += kInFlight) {
         float4 v[kInFlight];
 #pragma unroll
-        for (int k = 0; k < kInFlight; k++) v[k] = *reinterpret_cast<const float4*>(from + (s + k) * tiles * kTileRows * kColumns);
+        for (int k = 0; k < kInFlight; k++) v[k] = *reinterpret_cast<const float4*>(from + (s + k) * tiles * kRows * kColumns);
 #pragma unroll
         for (int k = 0; k < kInFlight; k++) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
     }
     for (; s < n; s++) {
-        const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kTileRows * kColumns);
+        const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kRows * kColumns);
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
     T* to = out + (piece.group * height + row + i) * columns + column + j;
@@ -173,12 +194,12 @@ inline int64_t outer_segment(int64_t rows, int64_t tiles, int sms) {
 // Room for the parts: a group of r > segment rows leaves at most 2 r / segment of each tile.
 inline int64_t most_outer_parts(int64_t rows, int64_t tiles, int64_t segment) { return tiles * (rows / segment * 2); }
 
-template <typename T, int kColumns>
+template <typename T, int kRows, int kColumns>
 void join_outer(const Call& call, const OuterProblem& p, const float* parts, int64_t most_parts, int64_t tiles, int64_t segment,
                 const std::string& op) {
     const int64_t rows = p.X.shape[0], joins = tiles * std::min<int64_t>(p.groups, rows / segment);
     fits_int32(static_cast<size_t>(joins), "the number of tiles", op);
-    grouped_outer_join<T, kColumns><<<dim3(static_cast<unsigned>(joins), kTileRows * kColumns / 1024), 256, 0, call.stream>>>(
+    grouped_outer_join<T, kRows, kColumns><<<dim3(static_cast<unsigned>(joins), kRows * kColumns / 1024), 256, 0, call.stream>>>(
         static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(p.X.shape[1]),
         static_cast<int>(p.Y.shape[1]), segment);
     MOPS_CUDA_OK(cudaGetLastError());

@@ -5,9 +5,16 @@
 // memory), and four warps move finished accumulators through shared memory to the output while the next tile is under way in
 // the other half of tensor memory.
 //
+// Pairs: shared memory bounds such a block: of a stage of 128 x 256 it takes 48 KB in and gives 48 KB to the tensor cores in 512 clocks,
+// 192 bytes a clock, and it moves some 140. Two blocks that multiply together (cta_group::2), 256 rows by 256 columns, take half of the columns' operand
+// each: 128 bytes a clock. Where there are enough rows to a group, pairs do the work.
+//
 // Rows: a tile begins where its group's rows do, wherever that is; of a tile that reaches past the end of its group the rows
-// behind it are computed and not stored. Outer products: the depth is the group's rows, and of the last stage of a
-// group the rows behind its end are cleared in shared memory before they are multiplied.
+// behind it are computed and not stored. Outer products: the depth is the group's rows, and in the last stage of a
+// group the rows behind its end are cleared in shared memory, by a warp that does nothing else, before they are multiplied.
+#include <map>
+#include <mutex>
+
 #include "grouped_block.cuh"
 #include "grouped_mma.hpp"
 #include "tensor_map.hpp"
@@ -16,14 +23,18 @@ namespace mops_b200 {
 
 namespace {
 
-constexpr int kThreads = 192;   // the copying warp, the multiplying warp, four that store
+constexpr int kThreads = 224;   // the copying warp, the multiplying warp, four that store, the one that clears
+constexpr int kClearWarp = 6;
 constexpr int kStoreWarps = 4;
 constexpr int kStaging = 32 * kBoxRow; // bytes: 32 rows of 64 values, of one warp
 
 // What a block keeps in shared memory.
-template <int kColumns> struct Layout {
-    static constexpr int kStages = kColumns == 256 ? 4 : kColumns == 128 ? 6 : 8;
-    static constexpr int kA = kTileRows * kBoxRow, kB = kColumns * kBoxRow; // bytes of a stage
+template <int kColumns, bool kPaired> struct Layout {
+    static constexpr bool kPair = kPaired;
+    static constexpr int kOwnColumns = kPair ? kColumns / 2 : kColumns; // that a block fetches
+    static constexpr int kRows = kPair ? 2 * kTileRows : kTileRows;     // of a tile
+    static constexpr int kStages = kOwnColumns == 256 ? 4 : kOwnColumns == 128 ? 6 : 8;
+    static constexpr int kA = kTileRows * kBoxRow, kB = kOwnColumns * kBoxRow; // bytes of a stage
     static constexpr int kStage = kA + kB;
     static constexpr int kStagingAt = kStages * kStage;
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * 2 * kStaging;
@@ -32,11 +43,13 @@ template <int kColumns> struct Layout {
     struct Rings {
         Ring<kStages> stages;
         Ring<2> accumulators;
+        uint64_t to_clear[kStages]; // the copies of stages that are cleared in part before they count as full
         uint32_t tmem;
         int gave_up;
         __device__ void begin() {
-            stages.begin(1, 1);
-            accumulators.begin(1, kStoreWarps);
+            stages.begin(kPair ? 2 : 1, 1);
+            accumulators.begin(1, kPair ? 2 * kStoreWarps : kStoreWarps);
+            for (int i = 0; i < kStages; i++) mbarrier_init(&to_clear[i], 1);
         }
     };
     static_assert(sizeof(Rings) <= 256, "room for the rings");
@@ -101,15 +114,42 @@ __device__ __forceinline__ void store_columns(uint32_t accumulator, uint32_t sta
     }
 }
 
+// What a pair and a block by itself do differently.
+template <typename L> struct Hand {
+    // A stage's barrier, on which both blocks of a pair count, is that of the first; so are those that say that accumulators are free.
+    __device__ static __forceinline__ void expect(uint64_t* full) {
+        if constexpr (L::kPair) pair_arrive_expect(first_of_pair(full), L::kStage);
+        else mbarrier_arrive_expect(full, L::kStage);
+    }
+    __device__ static __forceinline__ void fetch(uint32_t to, const CUtensorMap& map, int inner, int outer, int slice, uint64_t* full) {
+        if constexpr (L::kPair) pair_box_in(to, map, inner, outer, slice, first_of_pair(full));
+        else box_in(to, map, inner, outer, slice, full);
+    }
+    __device__ static __forceinline__ void arrive(uint64_t* bar) {
+        if constexpr (L::kPair) pair_arrive(first_of_pair(bar));
+        else mbarrier_arrive(bar);
+    }
+    __device__ static __forceinline__ void multiply(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
+        if constexpr (L::kPair) pair_umma(accumulator, a, b, instruction, add);
+        else umma(accumulator, a, b, instruction, add);
+    }
+    __device__ static __forceinline__ void multiplied(uint64_t* bar) { // to be told to both
+        if constexpr (L::kPair) pair_umma_arrive(bar);
+        else umma_arrive(bar);
+    }
+};
+
 // ---------------------------------------------------------------------------------- rows
 // out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
-template <bool BF16, bool M_MN, int kColumns>
+template <bool BF16, bool M_MN, int kColumns, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m,
                  const __grid_constant__ CUtensorMap map_out, uint16_t* __restrict__ out, const int32_t* __restrict__ offsets,
                  int64_t groups, int64_t rows, int depth, int columns, bool loose, Status st) {
     extern __shared__ unsigned char raw[];
-    using L = Layout<kColumns>;
+    using L = Layout<kColumns, kPair>;
+    using H = Hand<L>;
+    const int rank = kPair ? static_cast<int>(pair_rank()) : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
@@ -117,17 +157,17 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 
     const int64_t column_tiles = (columns + kColumns - 1) / kColumns;
     const int steps = (depth + kBoxDepth - 1) / kBoxDepth;
-    GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{kTileRows, column_tiles});
+    GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{L::kRows, column_tiles});
     Turn<L::kStages> stage;
     Turn<2> tile;     // accumulator
     int64_t sent = 0; // boxes that this warp has fetched or stored
     auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
-    for (int64_t want = blockIdx.x;; want += gridDim.x) {
+    if (warp != kClearWarp) for (int64_t want = blockIdx.x / (kPair ? 2 : 1);; want += gridDim.x / (kPair ? 2 : 1)) {
         const GroupPiece piece = walk.find(want, lane);
         if (!piece.found) break;
         int64_t tile_row, tile_column;
-        banded(piece.within, (piece.hi - piece.lo + kTileRows - 1) / kTileRows, column_tiles, tile_row, tile_column);
-        const int64_t row = piece.lo + tile_row * kTileRows;
+        banded(piece.within, (piece.hi - piece.lo + L::kRows - 1) / L::kRows, column_tiles, tile_row, tile_column);
+        const int64_t row = piece.lo + tile_row * L::kRows + rank * kTileRows; // of this block's half
         const int column = static_cast<int>(tile_column) * kColumns;
         const bool in_group = piece.group >= 0 && piece.group < groups;
         bool ok = true;
@@ -138,22 +178,23 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     if (!ok) break;
                     uint64_t* full = &block.rings->stages.full[stage.at];
                     const uint32_t a = stage_at(), b = a + L::kA;
-                    mbarrier_arrive_expect(full, L::kStage);
-                    box_in(a, map_x, s * kBoxDepth, static_cast<int>(row), 0, full);
+                    const int own_column = column + rank * L::kOwnColumns;
+                    H::expect(full);
+                    H::fetch(a, map_x, s * kBoxDepth, static_cast<int>(min(row, rows)), 0, full);
                     if constexpr (M_MN) {
 #pragma unroll
-                        for (int j = 0; j < kColumns / 64; j++)
-                            box_in(b + j * kBoxBytes, map_m, column + j * 64, s * kBoxDepth, static_cast<int>(piece.group), full);
+                        for (int j = 0; j < L::kOwnColumns / 64; j++)
+                            H::fetch(b + j * kBoxBytes, map_m, own_column + j * 64, s * kBoxDepth, static_cast<int>(piece.group), full);
                     } else {
-                        box_in(b, map_m, s * kBoxDepth, column, static_cast<int>(piece.group), full);
+                        H::fetch(b, map_m, s * kBoxDepth, own_column, static_cast<int>(piece.group), full);
                     }
                     stage.next();
                     sent++;
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0 && in_group) {
-                constexpr uint32_t instruction = instruction_descriptor(BF16, false, M_MN, kColumns);
+            if (lane == 0 && in_group && rank == 0) {
+                constexpr uint32_t instruction = instruction_descriptor(BF16, false, M_MN, kColumns, L::kRows);
                 ok = block.wait_empty(block.rings->accumulators, tile);
                 tmem_fence_after_sync();
                 for (int s = 0; s < steps && ok; s++) {
@@ -164,14 +205,14 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     const uint64_t b = operand_descriptor(stage_at() + L::kA, kBoxBytes);
 #pragma unroll
                     for (int k = 0; k < kBoxDepth / 16; k++)
-                        umma(block.accumulator(tile), a + k * kDepthStep<false>, b + k * kDepthStep<M_MN>, instruction, s + k > 0);
-                    umma_arrive(&block.rings->stages.empty[stage.at]);
+                        H::multiply(block.accumulator(tile), a + k * kDepthStep<false>, b + k * kDepthStep<M_MN>, instruction, s + k > 0);
+                    H::multiplied(&block.rings->stages.empty[stage.at]);
                     stage.next();
                 }
-                if (ok) umma_arrive(&block.rings->accumulators.full[tile.at]);
+                if (ok) H::multiplied(&block.rings->accumulators.full[tile.at]);
                 tile.next();
             }
-        } else {
+        } else if (warp < kClearWarp) {
             const int quadrant = warp & 3;
             const int64_t band = row + quadrant * 32;
             const int here = static_cast<int>(min(max(piece.hi - band, int64_t(0)), int64_t(32)));
@@ -188,7 +229,7 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                                                         columns, here, loose, lane);
                     tmem_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbarrier_arrive(&block.rings->accumulators.empty[tile.at]);
+                    if (lane == 0) H::arrive(&block.rings->accumulators.empty[tile.at]);
                 }
                 tile.next();
             } else { // rows of no group
@@ -199,40 +240,43 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         if (!__shfl_sync(kFullMask, ok, 0)) break;
     }
     if (warp == 0 && lane == 0) block.drain(block.rings->stages, stage, sent);
-    if (warp >= 2 && lane == 0) boxes_left<0>();
+    if (warp >= 2 && warp < kClearWarp && lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
 }
 
 // ------------------------------------------------------------------------- outer products
 // out[g] = X[rows of g]^T Y[rows of g].
-template <bool BF16, int kColumns>
+template <bool BF16, int kColumns, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                   const __grid_constant__ CUtensorMap map_out, uint16_t* __restrict__ out, float* __restrict__ parts, int64_t most_parts,
                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment,
                   bool loose, Status st) {
     extern __shared__ unsigned char raw[];
-    using L = Layout<kColumns>;
+    using L = Layout<kColumns, kPair>;
+    using H = Hand<L>;
+    const int rank = kPair ? static_cast<int>(pair_rank()) : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
-    const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
+    const int64_t row_tiles = (height + L::kRows - 1) / L::kRows, column_tiles = (columns + kColumns - 1) / kColumns;
     const int64_t tiles = row_tiles * column_tiles;
     GroupWalk<OuterPieces> walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles});
     Turn<L::kStages> stage;
     Turn<2> tile;
     int64_t sent = 0;
+    unsigned cleared = 0; // a bit for each place of the ring: the round of its to_clear
     auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
-    for (int64_t want = blockIdx.x;; want += gridDim.x) {
+    for (int64_t want = blockIdx.x / (kPair ? 2 : 1);; want += gridDim.x / (kPair ? 2 : 1)) {
         const GroupPiece piece = walk.find(want, lane);
         if (!piece.found) break;
         const int64_t part = piece.within / tiles;
         int64_t tile_row, tile_column;
         banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
-        const int row = static_cast<int>(tile_row) * kTileRows, column = static_cast<int>(tile_column) * kColumns;
+        const int row = static_cast<int>(tile_row) * L::kRows + rank * kTileRows, column = static_cast<int>(tile_column) * kColumns;
         const int64_t lo = piece.lo + part * segment, hi = min(lo + segment, piece.hi);
         const int steps = static_cast<int>((hi - lo + kBoxDepth - 1) / kBoxDepth);
         bool ok = true;
@@ -244,48 +288,69 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     uint64_t* full = &block.rings->stages.full[stage.at];
                     const uint32_t a = stage_at(), b = a + L::kA;
                     const int at = static_cast<int>(lo) + s * kBoxDepth;
-                    mbarrier_arrive_expect(full, L::kStage);
+                    const int own_column = column + rank * L::kOwnColumns;
+                    if (hi - lo - int64_t(s) * kBoxDepth >= kBoxDepth) {
+                        H::expect(full);
 #pragma unroll
-                    for (int i = 0; i < kTileRows / 64; i++) box_in(a + i * kBoxBytes, map_x, row + i * 64, at, 0, full);
+                        for (int i = 0; i < kTileRows / 64; i++) H::fetch(a + i * kBoxBytes, map_x, row + i * 64, at, 0, full);
 #pragma unroll
-                    for (int j = 0; j < kColumns / 64; j++) box_in(b + j * kBoxBytes, map_y, column + j * 64, at, 0, full);
+                        for (int j = 0; j < L::kOwnColumns / 64; j++) H::fetch(b + j * kBoxBytes, map_y, own_column + j * 64, at, 0, full);
+                    } else { // to the clearing warp first
+                        uint64_t* copied = &block.rings->to_clear[stage.at];
+                        mbarrier_arrive_expect(copied, L::kStage);
+#pragma unroll
+                        for (int i = 0; i < kTileRows / 64; i++) box_in(a + i * kBoxBytes, map_x, row + i * 64, at, 0, copied);
+#pragma unroll
+                        for (int j = 0; j < L::kOwnColumns / 64; j++) box_in(b + j * kBoxBytes, map_y, own_column + j * 64, at, 0, copied);
+                    }
                     stage.next();
                     sent++;
                 }
             }
         } else if (warp == 1) {
-            if (steps > 0) {
-                constexpr uint32_t instruction = instruction_descriptor(BF16, true, true, kColumns);
-                if (lane == 0) ok = block.wait_empty(block.rings->accumulators, tile);
-                ok = __shfl_sync(kFullMask, ok, 0);
+            if (lane == 0 && rank == 0 && steps > 0) {
+                constexpr uint32_t instruction = instruction_descriptor(BF16, true, true, kColumns, L::kRows);
+                ok = block.wait_empty(block.rings->accumulators, tile);
                 tmem_fence_after_sync();
                 for (int s = 0; s < steps && ok; s++) {
                     const int64_t left = hi - lo - int64_t(s) * kBoxDepth;
-                    if (lane == 0 || left < kBoxDepth) ok = block.wait_full(block.rings->stages, stage);
-                    ok = __all_sync(kFullMask, ok);
+                    if (kPair && left < kBoxDepth) ok = block.template wait<true>(&block.rings->stages.full[stage.at], stage.round); // cleared by both
+                    else ok = block.wait_full(block.rings->stages, stage);
                     if (!ok) break;
-                    if (left < kBoxDepth) { // the rows behind are of another group
-                        const uint32_t from = static_cast<uint32_t>(left) * kBoxRow;
-                        for (uint32_t box = 0; box < L::kStage; box += kBoxBytes)
-                            for (uint32_t at = from + lane * 16; at < kBoxBytes; at += 32 * 16)
-                                smem_store16(stage_at() + box + at, make_uint4(0, 0, 0, 0));
-                        async_proxy_fence();
-                        __syncwarp();
-                    }
-                    if (lane == 0) {
-                        tmem_fence_after_sync();
-                        const uint64_t a = operand_descriptor(stage_at(), kBoxBytes);
-                        const uint64_t b = operand_descriptor(stage_at() + L::kA, kBoxBytes);
+                    tmem_fence_after_sync();
+                    const uint64_t a = operand_descriptor(stage_at(), kBoxBytes);
+                    const uint64_t b = operand_descriptor(stage_at() + L::kA, kBoxBytes);
 #pragma unroll
-                        for (int k = 0; k < kBoxDepth / 16; k++)
-                            umma(block.accumulator(tile), a + k * kDepthStep<true>, b + k * kDepthStep<true>, instruction, s + k > 0);
-                        umma_arrive(&block.rings->stages.empty[stage.at]);
-                    }
+                    for (int k = 0; k < kBoxDepth / 16; k++)
+                        if (k * 16 < left)
+                            H::multiply(block.accumulator(tile), a + k * kDepthStep<true>, b + k * kDepthStep<true>, instruction, s + k > 0);
+                    H::multiplied(&block.rings->stages.empty[stage.at]);
                     stage.next();
-                    __syncwarp();
                 }
-                if (lane == 0 && ok) umma_arrive(&block.rings->accumulators.full[tile.at]);
+                if (ok) H::multiplied(&block.rings->accumulators.full[tile.at]);
                 tile.next();
+            }
+        } else if (warp == kClearWarp) {
+            const int left = static_cast<int>((hi - lo) % kBoxDepth); // rows of the last stage
+            if (left > 0) {
+                stage.skip(steps - 1);
+                if (lane == 0) ok = block.wait(&block.rings->to_clear[stage.at], cleared >> stage.at & 1);
+                ok = __shfl_sync(kFullMask, ok, 0);
+                if (ok) ok = block.wait(&block.rings->to_clear[stage.at], cleared >> stage.at & 1); // (so that every lane has seen it)
+                ok = __all_sync(kFullMask, ok);
+                cleared ^= 1u << stage.at;
+                if (ok) { // the rows behind are of another group; 16 of them are multiplied at a time
+                    const uint32_t from = static_cast<uint32_t>(left) * kBoxRow, to = static_cast<uint32_t>(left + 15) / 16 * 16 * kBoxRow;
+                    for (uint32_t box = 0; box < L::kStage; box += kBoxBytes)
+                        for (uint32_t at = from + lane * 16; at < to; at += 32 * 16)
+                            smem_store16(stage_at() + box + at, make_uint4(0, 0, 0, 0));
+                    async_proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) H::arrive(&block.rings->stages.full[stage.at]);
+                }
+                stage.next();
+            } else {
+                stage.skip(steps);
             }
         } else {
             const int quadrant = warp & 3;
@@ -297,7 +362,7 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 tmem_fence_after_sync();
                 if (piece.hi - piece.lo > segment) {
                     const int64_t slot = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
-                    float* to = parts + (slot * kTileRows + quadrant * 32 + lane) * kColumns;
+                    float* to = parts + (slot * L::kRows + rank * kTileRows + quadrant * 32 + lane) * kColumns;
                     // (there are more parts than there is room for only where offsets descend, which is reported)
                     for (int c = 0; c < wide && slot < most_parts; c += 32) {
                         uint32_t r[32];
@@ -324,7 +389,7 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 if (steps > 0) {
                     tmem_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbarrier_arrive(&block.rings->accumulators.empty[tile.at]);
+                    if (lane == 0) H::arrive(&block.rings->accumulators.empty[tile.at]);
                     tile.next();
                 }
             }
@@ -332,9 +397,44 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         if (!__shfl_sync(kFullMask, ok, 0)) break;
     }
     if (warp == 0 && lane == 0) block.drain(block.rings->stages, stage, sent);
-    if (warp >= 2 && lane == 0) boxes_left<0>();
+    if (warp >= 2 && warp < kClearWarp && lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
+}
+
+// How many pairs of blocks can run at the same time: where an odd SM is left over in its part of the chip, fewer than half the SMs (asked once).
+int resident_pairs(const void* kernel, int device, const cudaLaunchConfig_t& config) {
+    static std::mutex mutex;
+    static std::map<std::pair<const void*, int>, int> known;
+    std::lock_guard<std::mutex> lock(mutex);
+    int& pairs = known[{kernel, device}];
+    if (pairs == 0) {
+        MOPS_CUDA_OK(cudaOccupancyMaxActiveClusters(&pairs, kernel, &config));
+        if (pairs < 1) pairs = 1;
+    }
+    return pairs;
+}
+
+// Launches as many blocks, or pairs of them, as there are pieces of work, or as fit the GPU at once.
+template <typename L, typename... P, typename... A>
+void launch_blocks(const Call& call, void (*kernel)(P...), int64_t pieces, const A&... arguments) {
+    allow_dynamic_smem(kernel, call.device, L::kBytes);
+    if constexpr (!L::kPair) {
+        kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sm_count(call.device))), kThreads, L::kBytes, call.stream>>>(arguments...);
+    } else {
+        cudaLaunchConfig_t config{};
+        cudaLaunchAttribute cluster{};
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = 2, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+        config.attrs = &cluster;
+        config.numAttrs = 1;
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = L::kBytes;
+        config.stream = call.stream;
+        config.gridDim = dim3(2);
+        config.gridDim = dim3(2 * static_cast<unsigned>(std::min<int64_t>(pieces, resident_pairs(reinterpret_cast<const void*>(kernel), call.device, config))));
+        MOPS_CUDA_OK(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
+    }
 }
 
 } // namespace
@@ -346,28 +446,35 @@ bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string
     if (p.depth == 0 || p.groups == 0) return false;
     const bool loose = p.columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
     const int sms = sm_count(call.device);
-    auto launch = [&](auto type, auto major, auto width) {
-        constexpr bool BF16 = decltype(type)::value, M_MN = decltype(major)::value;
+    auto launch = [&](auto type, auto major, auto width, auto paired) {
+        constexpr bool BF16 = decltype(type)::value, M_MN = decltype(major)::value, kPair = decltype(paired)::value;
         constexpr int kColumns = decltype(width)::value;
-        using L = Layout<kColumns>;
+        using L = Layout<kColumns, kPair>;
         const CUtensorMap x = tensor_map(p.X.type, p.X.data, p.depth, p.rows, 1, p.X.stride[0], 0, kTileRows);
         const CUtensorMap m = M_MN ? tensor_map(p.X.type, p.M.data, p.columns, p.depth, p.groups, stride, p.M.stride[0], 64)
-                                   : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
+                                   : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], L::kOwnColumns);
         const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, p.columns, p.rows, 1, p.columns, 0, 32);
-        const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
-        auto kernel = grouped_rows_mma<BF16, M_MN, kColumns>;
-        allow_dynamic_smem(kernel, call.device, L::kBytes);
-        kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kThreads, L::kBytes, call.stream>>>(
-            x, m, out, static_cast<uint16_t*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth),
-            static_cast<int>(p.columns), loose, call.status);
-        note_kernel_f("grouped_rows_mma<%s,%s,%d>", BF16 ? "bf16" : "f16", M_MN ? "columns" : "depth", kColumns);
+        const int64_t tiles = most_row_tiles(p.rows, p.groups, L::kRows) * ceil_div(p.columns, kColumns);
+        launch_blocks<L>(call, grouped_rows_mma<BF16, M_MN, kColumns, kPair>, tiles, x, m, out, static_cast<uint16_t*>(p.out.data), p.offsets,
+                         p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns), loose, call.status);
+        note_kernel_f("grouped_rows_mma<%s,%s,%d,%s>", BF16 ? "bf16" : "f16", M_MN ? "columns" : "depth", kColumns, kPair ? "pair" : "block");
     };
     auto by_width = [&](auto type, auto major) {
+        using std::integral_constant;
         // The wider the tile, the fewer times X is fetched; the narrower, the more blocks share the work.
         const int64_t row_tiles = most_row_tiles(p.rows, p.groups, kTileRows);
-        if (p.columns > 128 && row_tiles * ceil_div(p.columns, 256) >= sms) launch(type, major, std::integral_constant<int, 256>());
-        else if (p.columns > 64 && row_tiles * ceil_div(p.columns, 128) >= sms / 2) launch(type, major, std::integral_constant<int, 128>());
-        else launch(type, major, std::integral_constant<int, 64>());
+        // Half of a tile for each group is rows that are not there, on average; a pair computes its tiles in some 0.8 of the time
+        // that two blocks take for theirs.
+        const int64_t of_blocks = ceil_div((2 * p.rows / kTileRows + p.groups) * ceil_div(p.columns, 256), 2 * sms);
+        const int64_t of_pairs = ceil_div((p.rows / kTileRows + p.groups) * ceil_div(p.columns, 256), sms);
+        if (p.columns > 128 && row_tiles * ceil_div(p.columns, 256) >= sms) {
+            if (4 * of_pairs <= 5 * of_blocks - 1) launch(type, major, integral_constant<int, 256>(), std::true_type());
+            else launch(type, major, integral_constant<int, 256>(), std::false_type());
+        } else if (p.columns > 64 && row_tiles * ceil_div(p.columns, 128) >= sms / 2) {
+            launch(type, major, integral_constant<int, 128>(), std::false_type());
+        } else {
+            launch(type, major, integral_constant<int, 64>(), std::false_type());
+        }
     };
     auto by_major = [&](auto type) {
         if (mn) by_width(type, std::true_type());
@@ -385,34 +492,33 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
     if (rows == 0) return false;
     const bool loose = columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
     const int sms = sm_count(call.device);
-    auto launch = [&](auto type, auto width) {
-        constexpr bool BF16 = decltype(type)::value;
+    auto launch = [&](auto type, auto width, auto paired) {
+        constexpr bool BF16 = decltype(type)::value, kPair = decltype(paired)::value;
         constexpr int kColumns = decltype(width)::value;
-        using L = Layout<kColumns>;
+        using L = Layout<kColumns, kPair>;
         using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
         const CUtensorMap x = tensor_map(p.X.type, p.X.data, height, rows, 1, p.X.stride[0], 0, 64);
         const CUtensorMap y = tensor_map(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, 64);
         const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
-        const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
-        const int64_t segment = outer_segment(rows, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
-        float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
+        const int64_t tiles = ceil_div(height, L::kRows) * ceil_div(columns, kColumns);
+        const int64_t segment = outer_segment(rows, tiles, kPair ? sms / 2 : sms), most_parts = most_outer_parts(rows, tiles, segment);
+        float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * L::kRows * kColumns * sizeof(float)))
                                       : nullptr;
-        auto kernel = grouped_outer_mma<BF16, kColumns>;
-        allow_dynamic_smem(kernel, call.device, L::kBytes);
-        const int64_t pieces = tiles * (rows / segment + p.groups);
-        kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
-            x, y, out, static_cast<uint16_t*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height),
-            static_cast<int>(columns), segment, loose, call.status);
+        launch_blocks<L>(call, grouped_outer_mma<BF16, kColumns, kPair>, tiles * (rows / segment + p.groups), x, y, out,
+                         static_cast<uint16_t*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height),
+                         static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {
-            join_outer<T, kColumns>(call, p, parts, most_parts, tiles, segment, op);
+            join_outer<T, L::kRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);
             scratch_free(call, parts);
         }
-        note_kernel_f("grouped_outer_mma<%s,%d>", BF16 ? "bf16" : "f16", kColumns);
+        note_kernel_f("grouped_outer_mma<%s,%d,%s>", BF16 ? "bf16" : "f16", kColumns, kPair ? "pair" : "block");
     };
     auto by_width = [&](auto type) {
-        if (columns > 128) launch(type, std::integral_constant<int, 256>());
-        else if (columns > 64) launch(type, std::integral_constant<int, 128>());
-        else launch(type, std::integral_constant<int, 64>());
+        using std::integral_constant;
+        if (columns > 128 && height > kTileRows) launch(type, integral_constant<int, 256>(), std::true_type());
+        else if (columns > 128) launch(type, integral_constant<int, 256>(), std::false_type());
+        else if (columns > 64) launch(type, integral_constant<int, 128>(), std::false_type());
+        else launch(type, integral_constant<int, 64>(), std::false_type());
     };
     if (p.X.type == MOPS_B200_BF16) by_width(std::true_type());
     else by_width(std::false_type());

@@ -50,6 +50,7 @@ template <int kColumns> struct Layout {
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * kStaging;
     static constexpr int kBytes = kRingsAt + 256 + 1024;
     static constexpr unsigned kTmem = 2 * kColumns;
+    static constexpr bool kPair = false;
     struct Rings {
         Ring<kRaws> raws;
         Ring<kStages> stages;
@@ -492,7 +493,7 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
             x, y, static_cast<float*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns),
             segment, call.status);
         if (rows > segment) {
-            join_outer<float, kColumns>(call, p, parts, most_parts, tiles, segment, op);
+            join_outer<float, kTileRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);
             scratch_free(call, parts);
         }
         note_kernel_f("grouped_outer_split<%d>", kColumns);

@@ -27,10 +27,10 @@ template <int kRowBytes = kBoxRow> __device__ __forceinline__ uint64_t operand_d
 // What one step of 16 values in depth adds to a descriptor.
 template <bool MN> constexpr uint64_t kDepthStep = MN ? 2048 >> 4 : 32 >> 4;
 
-// f32 accumulators of 128 x n; both operands bf16 (or both f16).
-__host__ __device__ constexpr uint32_t instruction_descriptor(bool bf16, bool a_mn, bool b_mn, int n) {
+// f32 accumulators of m x n (m: 128, or 256 over a pair of SMs); both operands bf16 (or both f16).
+__host__ __device__ constexpr uint32_t instruction_descriptor(bool bf16, bool a_mn, bool b_mn, int n, int m = 128) {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
-           static_cast<uint32_t>(n / 8) << 17 | static_cast<uint32_t>(128 / 16) << 24;
+           static_cast<uint32_t>(n / 8) << 17 | static_cast<uint32_t>(m / 16) << 24;
 }
 
 __device__ __forceinline__ void umma(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
@@ -86,6 +86,69 @@ __device__ __forceinline__ uint4 smem_load16(uint32_t address) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
     return v;
+}
+
+// ---- pairs of blocks (clusters of two), whose SMs multiply together: each has half of the rows of the accumulator in its tensor memory, and half of
+// either operand in its shared memory, at the same addresses. The first block of the pair issues the products.
+__device__ __forceinline__ unsigned pair_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+// Both blocks, all threads.
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// The address of the first block's copy of something in shared memory.
+__device__ __forceinline__ uint32_t first_of_pair(const void* p) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(a) : "r"(smem_address(p)));
+    return a;
+}
+__device__ __forceinline__ void pair_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_arrive_expect(uint32_t bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Sees what the other block wrote before it arrived, too (which costs hundreds of clocks: not for barriers that only copies and products are
+// counted on).
+__device__ __forceinline__ bool mbarrier_try_wait_pair(uint64_t* bar, unsigned parity) {
+    unsigned done;
+    asm volatile("{\n .reg .pred p;\n"
+                 " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                 " selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(smem_address(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+// Into this block's shared memory, completion counted on a barrier of either block.
+__device__ __forceinline__ void pair_box_in(uint32_t smem, const CUtensorMap& map, int inner, int outer, int slice, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];\n" ::
+                     "r"(smem),
+                 "l"(&map), "r"(inner), "r"(outer), "r"(slice), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_umma(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(accumulator),
+                 "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate))
+                 : "memory");
+}
+// Arrives on the barrier at this address of both blocks.
+__device__ __forceinline__ void pair_umma_arrive(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(smem_address(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* smem_address_out, unsigned columns) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_address(smem_address_out)), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_free(uint32_t address, unsigned columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(address), "r"(columns) : "memory");
 }
 
 } // namespace mops_b200

@@ -271,7 +271,8 @@ def check_grouped(A, W, offsets, grad):
 @pytest.mark.parametrize("rows,K,N", [
     ([1], 1, 1), ([1], 64, 64), ([3, 0, 5], 7, 9), ([0, 0, 4, 0], 16, 24), ([64, 64], 64, 128), ([63, 65, 1], 72, 136),
     ([128, 129, 127], 128, 256), ([200, 0, 1, 300], 264, 40), ([1] * 40, 32, 48), ([17, 700], 96, 520), ([2000], 8, 16),
-    ([5, 1, 250], 509, 131), ([33, 31], 1030, 30), ([0, 0], 16, 16), ([1000, 1], 130, 258), ([7] * 70, 16, 16)])
+    ([5, 1, 250], 509, 131), ([33, 31], 1030, 30), ([0, 0], 16, 16), ([1000, 1], 130, 258), ([7] * 70, 16, 16),
+    ([3000, 0, 129, 2500], 136, 1000), ([1111, 4000], 600, 770), ([300, 5000], 1000, 264)])
 def test_grouped_matches_64_bits(dtype, rows, K, N):
     R = sum(rows)
     check_grouped(normal((R, K), dtype, 1), normal((len(rows), K, N), dtype, 2, K ** -0.5), offsets_of(rows),
