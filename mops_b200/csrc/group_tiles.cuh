@@ -25,19 +25,21 @@ struct GroupPiece {
 };
 
 // Walks the pieces of groups first .. last in order, where pieces(rows of the group) says how many a group has. All
-// lanes of a warp call it together and get the same answers; `want` must not decrease from call to call.
+// lanes of a warp call it together and get the same answers. It goes on from where the last call found its piece (and begins anew where a
+// piece in front of that is asked for).
 template <typename Pieces> struct GroupWalk {
     const int32_t* offsets;
-    int64_t groups, rows, last;
+    int64_t groups, rows, first, last;
     Pieces pieces;
     int64_t base, before = 0;  // first group of the step at hand, pieces in front of it
     int64_t up_to = 0;         // pieces of groups base .. base + lane
     bool counted = false;
 
     __device__ GroupWalk(const int32_t* offsets, int64_t groups, int64_t rows, int64_t first, int64_t last, Pieces pieces)
-        : offsets(offsets), groups(groups), rows(rows), last(last), pieces(pieces), base(first) {}
+        : offsets(offsets), groups(groups), rows(rows), first(first), last(last), pieces(pieces), base(first) {}
 
     __device__ GroupPiece find(int64_t want, int lane) {
+        if (want < before) base = first, before = 0, counted = false;
         while (base <= last) {
             if (!counted) {
                 up_to = 0;

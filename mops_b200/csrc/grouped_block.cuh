@@ -161,35 +161,39 @@ grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t
     const int64_t n = (piece.hi - piece.lo + segment - 1) / segment;
     const int64_t first = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
     if (first + (n - 1) * tiles >= most_parts) return;
-    // four values to a thread
-    const int at = (blockIdx.y * 256 + threadIdx.x) * 4, i = at / kColumns, j = at % kColumns;
-    if (row + i >= height || column + j >= columns) return;
-    const float* from = parts + (first * kRows + i) * kColumns + j;
-    float4 sum = make_float4(0, 0, 0, 0);
-    int64_t s = 0;
-    constexpr int kInFlight = 8;
-    for (; s + kInFlight <= n; s += kInFlight) {
-        float4 v[kInFlight];
+    constexpr int kBlocks = kRows * kColumns / 8192; // to a tile: 32 values to a thread, four at a time
+    for (int at = (blockIdx.y * 256 + threadIdx.x) * 4; at < kRows * kColumns; at += kBlocks * 1024) {
+        const int i = at / kColumns, j = at % kColumns;
+        if (row + i >= height || column + j >= columns) continue;
+        const float* from = parts + (first * kRows + i) * kColumns + j;
+        float4 sum = make_float4(0, 0, 0, 0);
+        int64_t s = 0;
+        constexpr int kInFlight = 8;
+        for (; s + kInFlight <= n; s += kInFlight) {
+            float4 v[kInFlight];
 #pragma unroll
-        for (int k = 0; k < kInFlight; k++) v[k] = *reinterpret_cast<const float4*>(from + (s + k) * tiles * kRows * kColumns);
+            for (int k = 0; k < kInFlight; k++) v[k] = *reinterpret_cast<const float4*>(from + (s + k) * tiles * kRows * kColumns);
 #pragma unroll
-        for (int k = 0; k < kInFlight; k++) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+            for (int k = 0; k < kInFlight; k++) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+        }
+        for (; s < n; s++) {
+            const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kRows * kColumns);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        T* to = out + (piece.group * height + row + i) * columns + column + j;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (column + j + k < columns) to[k] = narrow<T>(v[k]);
     }
-    for (; s < n; s++) {
-        const float4 v = *reinterpret_cast<const float4*>(from + s * tiles * kRows * kColumns);
-        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-    }
-    T* to = out + (piece.group * height + row + i) * columns + column + j;
-    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (column + j + k < columns) to[k] = narrow<T>(v[k]);
 }
 
-// Segments such that, were all rows in one group, there would be some four pieces of work for each SM; so no block has much more than its share,
-// and few tiles are left in parts where there are many groups.
-inline int64_t outer_segment(int64_t rows, int64_t tiles, int sms) {
-    return std::max<int64_t>(ceil_div(rows * tiles, int64_t(sms) * 4 * kBoxDepth) * kBoxDepth, 256);
+// How many rows a segment has. Where a group has tiles for all `workers` (blocks, or pairs), its rows are not cut: what parts cost to write and to join is
+// that of some 800 rows of a tile. Where it has fewer, segments are such that, were all rows in one group, there would be three pieces for
+// each worker; so nobody has much more than its share, and few tiles are left in parts where there are many groups.
+inline int64_t outer_segment(int64_t rows, int64_t tiles, int workers) {
+    if (tiles >= workers) return std::max<int64_t>(rows, 1);
+    return std::max<int64_t>(ceil_div(rows * tiles, int64_t(workers) * 3 * kBoxDepth) * kBoxDepth, 256);
 }
 // Room for the parts: a group of r > segment rows leaves at most 2 r / segment of each tile.
 inline int64_t most_outer_parts(int64_t rows, int64_t tiles, int64_t segment) { return tiles * (rows / segment * 2); }
@@ -199,7 +203,7 @@ void join_outer(const Call& call, const OuterProblem& p, const float* parts, int
                 const std::string& op) {
     const int64_t rows = p.X.shape[0], joins = tiles * std::min<int64_t>(p.groups, rows / segment);
     fits_int32(static_cast<size_t>(joins), "the number of tiles", op);
-    grouped_outer_join<T, kRows, kColumns><<<dim3(static_cast<unsigned>(joins), kRows * kColumns / 1024), 256, 0, call.stream>>>(
+    grouped_outer_join<T, kRows, kColumns><<<dim3(static_cast<unsigned>(joins), kRows * kColumns / 8192), 256, 0, call.stream>>>(
         static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(p.X.shape[1]),
         static_cast<int>(p.Y.shape[1]), segment);
     MOPS_CUDA_OK(cudaGetLastError());

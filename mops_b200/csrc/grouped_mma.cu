@@ -1,6 +1,6 @@
 // grouped_matrix_product on tensor cores, for f16 and bf16.
 //
-// One block per SM works off tiles of 128 rows by kColumns columns. One warp has the copy engine fetch boxes of both operands into a ring
+// A block has an SM to itself and works off tiles of 128 rows by kColumns columns. One warp has the copy engine fetch boxes of both operands into a ring
 // of stages of 64 values of depth, one thread of another issues the products (tcgen05.mma, accumulators in tensor
 // memory), and four warps move finished accumulators through shared memory to the output while the next tile is under way in
 // the other half of tensor memory.
@@ -10,11 +10,8 @@
 // each: 128 bytes a clock. Where there are enough rows to a group, pairs do the work.
 //
 // Rows: a tile begins where its group's rows do, wherever that is; of a tile that reaches past the end of its group the rows
-// behind it are computed and not stored. Outer products: the depth is the group's rows, and in the last stage of a
-// group the rows behind its end are cleared in shared memory, by a warp that does nothing else, before they are multiplied.
-#include <map>
-#include <mutex>
-
+// behind it are computed and not stored. Outer products: the depth is the group's rows; of those that do not fill a stage the ones behind the group's
+// end are cleared in shared memory, by a warp that does nothing else, before they are multiplied.
 #include "grouped_block.cuh"
 #include "grouped_mma.hpp"
 #include "tensor_map.hpp"
@@ -23,8 +20,8 @@ namespace mops_b200 {
 
 namespace {
 
-constexpr int kThreads = 224;   // the copying warp, the multiplying warp, four that store, the one that clears
-constexpr int kClearWarp = 6;
+constexpr int kThreads = 256;   // the copying warp, the multiplying warp, four that store, the one that clears, the one that gets work
+constexpr int kClearWarp = 6, kWorkWarp = 7;
 constexpr int kStoreWarps = 4;
 constexpr int kStaging = 32 * kBoxRow; // bytes: 32 rows of 64 values, of one warp
 
@@ -38,21 +35,25 @@ template <int kColumns, bool kPaired> struct Layout {
     static constexpr int kStage = kA + kB;
     static constexpr int kStagingAt = kStages * kStage;
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * 2 * kStaging;
-    static constexpr int kBytes = kRingsAt + 256 + 1024; // (boxes begin on multiples of 1024 bytes)
+    static constexpr int kPieces = 2;                    // known ahead
+    static constexpr int kBytes = kRingsAt + 512 + 1024; // (boxes begin on multiples of 1024 bytes)
     static constexpr unsigned kTmem = 2 * kColumns;      // columns of tensor memory: two accumulators
     struct Rings {
         Ring<kStages> stages;
         Ring<2> accumulators;
         uint64_t to_clear[kStages]; // the copies of stages that are cleared in part before they count as full
+        Ring<kPieces> pieces;
+        uint4 answers[kPieces];     // whose work is taken over
         uint32_t tmem;
         int gave_up;
         __device__ void begin() {
             stages.begin(kPair ? 2 : 1, 1);
             accumulators.begin(1, kPair ? 2 * kStoreWarps : kStoreWarps);
+            pieces.begin(1, (kPair ? 2 : 1) * (kWorkWarp + 1)); // (every warp reads them)
             for (int i = 0; i < kStages; i++) mbarrier_init(&to_clear[i], 1);
         }
     };
-    static_assert(sizeof(Rings) <= 256, "room for the rings");
+    static_assert(sizeof(Rings) <= 512, "room for the rings");
 };
 
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
@@ -139,6 +140,44 @@ template <typename L> struct Hand {
     }
 };
 
+// Where a block (or pair) gets its work from: first the piece that it was launched for, then those of blocks that have not begun, so that all are
+// done at about the same time whatever their pieces take. (Dealt out in turn, 1072 equal tiles kept the SMs busy for 87 percent of the time.)
+template <typename L> struct Supply {
+    Block<L>& block;
+    Turn<L::kPieces> turn;
+    bool first = true;
+
+    // All warps but the one that gets work: the next piece, or -1. The same for all of them.
+    __device__ __forceinline__ int64_t next(int lane) {
+        if (first) {
+            first = false;
+            return blockIdx.x / (L::kPair ? 2 : 1);
+        }
+        bool ok = block.wait_full(block.rings->pieces, turn);
+        const int taken = ok ? taken_over(&block.rings->answers[turn.at]) : -1;
+        async_proxy_fence();
+        ok = __all_sync(kFullMask, ok);
+        if (lane == 0) Hand<L>::arrive(&block.rings->pieces.empty[turn.at]);
+        turn.next();
+        return !ok || taken < 0 ? -1 : taken / (L::kPair ? 2 : 1);
+    }
+    // One thread of the warp that gets work: asks for pieces until there are none. (Of a pair the first block asks, and both are told.)
+    __device__ __forceinline__ void get(int rank) {
+        for (;;) {
+            // (the second block's barriers know of its own answers alone; its places are free when the first block's are)
+            if (rank == 0 && !block.wait_empty(block.rings->pieces, turn)) return;
+            mbarrier_arrive_expect(&block.rings->pieces.full[turn.at], 16);
+            if (rank == 0) take_over<L::kPair>(&block.rings->answers[turn.at], &block.rings->pieces.full[turn.at]);
+            if (!block.wait_full(block.rings->pieces, turn)) return;
+            const bool more = taken_over(&block.rings->answers[turn.at]) >= 0;
+            async_proxy_fence();
+            Hand<L>::arrive(&block.rings->pieces.empty[turn.at]);
+            turn.next();
+            if (!more) return;
+        }
+    }
+};
+
 // ---------------------------------------------------------------------------------- rows
 // out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
 template <bool BF16, bool M_MN, int kColumns, bool kPair>
@@ -162,9 +201,11 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     Turn<2> tile;     // accumulator
     int64_t sent = 0; // boxes that this warp has fetched or stored
     auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
-    if (warp != kClearWarp) for (int64_t want = blockIdx.x / (kPair ? 2 : 1);; want += gridDim.x / (kPair ? 2 : 1)) {
+    Supply<L> supply{block};
+    if (warp == kWorkWarp && lane == 0) supply.get(rank);
+    if (warp < kWorkWarp) for (int64_t want = supply.next(lane); want >= 0; want = supply.next(lane)) {
         const GroupPiece piece = walk.find(want, lane);
-        if (!piece.found) break;
+        if (!piece.found) continue; // (there is a block for each piece that there could be)
         int64_t tile_row, tile_column;
         banded(piece.within, (piece.hi - piece.lo + L::kRows - 1) / L::kRows, column_tiles, tile_row, tile_column);
         const int64_t row = piece.lo + tile_row * L::kRows + rank * kTileRows; // of this block's half
@@ -270,15 +311,19 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     int64_t sent = 0;
     unsigned cleared = 0; // a bit for each place of the ring: the round of its to_clear
     auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
-    for (int64_t want = blockIdx.x / (kPair ? 2 : 1);; want += gridDim.x / (kPair ? 2 : 1)) {
+    Supply<L> supply{block};
+    if (warp == kWorkWarp && lane == 0) supply.get(rank);
+    if (warp < kWorkWarp) for (int64_t want = supply.next(lane); want >= 0; want = supply.next(lane)) {
         const GroupPiece piece = walk.find(want, lane);
-        if (!piece.found) break;
+        if (!piece.found) continue; // (there is a block for each piece that there could be)
         const int64_t part = piece.within / tiles;
         int64_t tile_row, tile_column;
         banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
         const int row = static_cast<int>(tile_row) * L::kRows + rank * kTileRows, column = static_cast<int>(tile_column) * kColumns;
         const int64_t lo = piece.lo + part * segment, hi = min(lo + segment, piece.hi);
         const int steps = static_cast<int>((hi - lo + kBoxDepth - 1) / kBoxDepth);
+        // the rows that do not fill a stage come first: they are cleared while the tile before is multiplied
+        const int left = static_cast<int>((hi - lo) % kBoxDepth);
         bool ok = true;
         if (warp == 0) {
             if (lane == 0) {
@@ -287,9 +332,9 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     if (!ok) break;
                     uint64_t* full = &block.rings->stages.full[stage.at];
                     const uint32_t a = stage_at(), b = a + L::kA;
-                    const int at = static_cast<int>(lo) + s * kBoxDepth;
+                    const int at = static_cast<int>(left == 0 ? lo + int64_t(s) * kBoxDepth : s == 0 ? hi - left : lo + int64_t(s - 1) * kBoxDepth);
                     const int own_column = column + rank * L::kOwnColumns;
-                    if (hi - lo - int64_t(s) * kBoxDepth >= kBoxDepth) {
+                    if (s > 0 || left == 0) {
                         H::expect(full);
 #pragma unroll
                         for (int i = 0; i < kTileRows / 64; i++) H::fetch(a + i * kBoxBytes, map_x, row + i * 64, at, 0, full);
@@ -313,8 +358,8 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 ok = block.wait_empty(block.rings->accumulators, tile);
                 tmem_fence_after_sync();
                 for (int s = 0; s < steps && ok; s++) {
-                    const int64_t left = hi - lo - int64_t(s) * kBoxDepth;
-                    if (kPair && left < kBoxDepth) ok = block.template wait<true>(&block.rings->stages.full[stage.at], stage.round); // cleared by both
+                    const bool cut = s == 0 && left > 0;
+                    if (kPair && cut) ok = block.template wait<true>(&block.rings->stages.full[stage.at], stage.round); // cleared by both
                     else ok = block.wait_full(block.rings->stages, stage);
                     if (!ok) break;
                     tmem_fence_after_sync();
@@ -322,7 +367,7 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     const uint64_t b = operand_descriptor(stage_at() + L::kA, kBoxBytes);
 #pragma unroll
                     for (int k = 0; k < kBoxDepth / 16; k++)
-                        if (k * 16 < left)
+                        if (!cut || k * 16 < left)
                             H::multiply(block.accumulator(tile), a + k * kDepthStep<true>, b + k * kDepthStep<true>, instruction, s + k > 0);
                     H::multiplied(&block.rings->stages.empty[stage.at]);
                     stage.next();
@@ -331,9 +376,7 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 tile.next();
             }
         } else if (warp == kClearWarp) {
-            const int left = static_cast<int>((hi - lo) % kBoxDepth); // rows of the last stage
             if (left > 0) {
-                stage.skip(steps - 1);
                 if (lane == 0) ok = block.wait(&block.rings->to_clear[stage.at], cleared >> stage.at & 1);
                 ok = __shfl_sync(kFullMask, ok, 0);
                 if (ok) ok = block.wait(&block.rings->to_clear[stage.at], cleared >> stage.at & 1); // (so that every lane has seen it)
@@ -348,10 +391,8 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     __syncwarp();
                     if (lane == 0) H::arrive(&block.rings->stages.full[stage.at]);
                 }
-                stage.next();
-            } else {
-                stage.skip(steps);
             }
+            stage.skip(steps);
         } else {
             const int quadrant = warp & 3;
             const int band = row + quadrant * 32, wide = min(columns - column, kColumns);
@@ -402,39 +443,22 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     block.end(warp);
 }
 
-// How many pairs of blocks can run at the same time: where an odd SM is left over in its part of the chip, fewer than half the SMs (asked once).
-int resident_pairs(const void* kernel, int device, const cudaLaunchConfig_t& config) {
-    static std::mutex mutex;
-    static std::map<std::pair<const void*, int>, int> known;
-    std::lock_guard<std::mutex> lock(mutex);
-    int& pairs = known[{kernel, device}];
-    if (pairs == 0) {
-        MOPS_CUDA_OK(cudaOccupancyMaxActiveClusters(&pairs, kernel, &config));
-        if (pairs < 1) pairs = 1;
-    }
-    return pairs;
-}
-
-// Launches as many blocks, or pairs of them, as there are pieces of work, or as fit the GPU at once.
+// Launches a block, or a pair of them, for each piece of work.
 template <typename L, typename... P, typename... A>
-void launch_blocks(const Call& call, void (*kernel)(P...), int64_t pieces, const A&... arguments) {
+void launch_blocks(const Call& call, const std::string& op, void (*kernel)(P...), int64_t pieces, const A&... arguments) {
     allow_dynamic_smem(kernel, call.device, L::kBytes);
-    if constexpr (!L::kPair) {
-        kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sm_count(call.device))), kThreads, L::kBytes, call.stream>>>(arguments...);
-    } else {
-        cudaLaunchConfig_t config{};
-        cudaLaunchAttribute cluster{};
-        cluster.id = cudaLaunchAttributeClusterDimension;
-        cluster.val.clusterDim.x = 2, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-        config.attrs = &cluster;
-        config.numAttrs = 1;
-        config.blockDim = dim3(kThreads);
-        config.dynamicSmemBytes = L::kBytes;
-        config.stream = call.stream;
-        config.gridDim = dim3(2);
-        config.gridDim = dim3(2 * static_cast<unsigned>(std::min<int64_t>(pieces, resident_pairs(reinterpret_cast<const void*>(kernel), call.device, config))));
-        MOPS_CUDA_OK(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
-    }
+    fits_int32(static_cast<size_t>(2 * pieces), "the number of tiles", op);
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = L::kPair ? 2 : 1, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    config.gridDim = dim3(static_cast<unsigned>(pieces) * (L::kPair ? 2 : 1));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = L::kBytes;
+    config.stream = call.stream;
+    MOPS_CUDA_OK(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
 }
 
 } // namespace
@@ -455,7 +479,7 @@ bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string
                                    : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], L::kOwnColumns);
         const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, p.columns, p.rows, 1, p.columns, 0, 32);
         const int64_t tiles = most_row_tiles(p.rows, p.groups, L::kRows) * ceil_div(p.columns, kColumns);
-        launch_blocks<L>(call, grouped_rows_mma<BF16, M_MN, kColumns, kPair>, tiles, x, m, out, static_cast<uint16_t*>(p.out.data), p.offsets,
+        launch_blocks<L>(call, op, grouped_rows_mma<BF16, M_MN, kColumns, kPair>, tiles, x, m, out, static_cast<uint16_t*>(p.out.data), p.offsets,
                          p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns), loose, call.status);
         note_kernel_f("grouped_rows_mma<%s,%s,%d,%s>", BF16 ? "bf16" : "f16", M_MN ? "columns" : "depth", kColumns, kPair ? "pair" : "block");
     };
@@ -504,7 +528,7 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         const int64_t segment = outer_segment(rows, tiles, kPair ? sms / 2 : sms), most_parts = most_outer_parts(rows, tiles, segment);
         float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * L::kRows * kColumns * sizeof(float)))
                                       : nullptr;
-        launch_blocks<L>(call, grouped_outer_mma<BF16, kColumns, kPair>, tiles * (rows / segment + p.groups), x, y, out,
+        launch_blocks<L>(call, op, grouped_outer_mma<BF16, kColumns, kPair>, tiles * (rows / segment + p.groups), x, y, out,
                          static_cast<uint16_t*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height),
                          static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {

@@ -88,6 +88,34 @@ __device__ __forceinline__ uint4 smem_load16(uint32_t address) {
     return v;
 }
 
+// ---- work that is handed out while the kernel runs: the grid has a block (or a pair) for each piece of work; those that run take over the places of
+// those that have not begun. The answer (16 bytes of shared memory, of both blocks of a pair) is counted on `bar`.
+template <bool kPair> __device__ __forceinline__ void take_over(void* answer, uint64_t* bar) {
+    if constexpr (kPair)
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.multicast::cluster::all.b128 [%0], [%1];\n" ::
+                         "r"(smem_address(answer)),
+                     "r"(smem_address(bar))
+                     : "memory");
+    else
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(smem_address(answer)),
+                     "r"(smem_address(bar))
+                     : "memory");
+}
+// Index of the (first) block whose place was taken over, or -1 if there is none left.
+__device__ __forceinline__ int taken_over(const void* answer) {
+    uint32_t taken, x;
+    asm volatile("{\n .reg .b128 a;\n .reg .pred p;\n .reg .b32 y, z, w;\n"
+                 " ld.shared.b128 a, [%2];\n"
+                 " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+                 " selp.u32 %0, 1, 0, p;\n"
+                 " mov.b32 %1, 0;\n"
+                 " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, a;\n}\n"
+                 : "=r"(taken), "=r"(x)
+                 : "r"(smem_address(answer))
+                 : "memory");
+    return taken ? static_cast<int>(x) : -1;
+}
+
 // ---- pairs of blocks (clusters of two), whose SMs multiply together: each has half of the rows of the accumulator in its tensor memory, and half of
 // either operand in its shared memory, at the same addresses. The first block of the pair issues the products.
 __device__ __forceinline__ unsigned pair_rank() {
