@@ -117,6 +117,120 @@ template <typename L> struct Block {
     __device__ uint32_t accumulator(const Turn<2>& turn) const { return rings->tmem + static_cast<uint32_t>(turn.at) * (L::kTmem / 2); }
 };
 
+// ------------------------------------------------------------------ pieces of work
+// A piece of work, as everybody in a block needs it.
+struct alignas(16) Piece {
+    int64_t lo, hi;  // rows of the tile's group from its first row on (of the first block, in a pair); outer products: the rows of its segment
+    int64_t slot;    // outer products: where its part goes, -1 if it is the whole
+    int group;       // -1: rows of no group
+    int row, column; // outer products: the tile's first row and column
+    int steps;       // stages
+};
+
+// A warp of each block gets pieces and works out what they are, while the others are at the ones before: to find a piece among groups takes a microsecond or two
+// of divisions and sums over lanes, which, done by the warps that copy, multiply and store, left the tensor cores idle between tiles. The first
+// piece is the one that the block (or pair) was launched for, then come those of blocks that have not begun; so all SMs are done at about the same
+// time, whatever their pieces take. L::kPieces pieces are known ahead; L::kReaders warps read them.
+template <int kPieces> struct Pieces {
+    Ring<kPieces> ring;
+    Piece piece[kPieces];
+    Ring<1> answers;
+    uint4 answer; // whose work was taken over
+    __device__ void begin(unsigned readers, bool pair) {
+        ring.begin(1, readers);
+        answers.begin(1, pair ? 2 : 1);
+    }
+};
+
+// The warp that gets them. decode(index, piece) says whether there is such a piece, and which (all lanes).
+template <typename L, typename Decode> __device__ __forceinline__ void hand_out(Block<L>& block, int rank, int lane, Decode decode) {
+    auto& pieces = block.rings->pieces;
+    Turn<1> asked;
+    Turn<L::kPieces> turn;
+    int64_t want = blockIdx.x / (L::kPair ? 2 : 1);
+    auto publish = [&](const Piece& p) {
+        bool ok = true;
+        if (lane == 0) {
+            ok = block.wait_empty(pieces.ring, turn);
+            if (ok) {
+                pieces.piece[turn.at] = p;
+                mbarrier_arrive(&pieces.ring.full[turn.at]);
+            }
+        }
+        turn.next();
+        return __shfl_sync(kFullMask, ok, 0) != 0;
+    };
+    for (;;) {
+        // the next one is on its way while this one is worked out; of a pair the first block asks, and both are told
+        bool ok = true;
+        if (lane == 0) {
+            if (rank == 0) ok = block.wait_empty(pieces.answers, asked);
+            if (ok) mbarrier_arrive_expect(&pieces.answers.full[0], 16);
+            if (ok && rank == 0) take_over<L::kPair>(&pieces.answer, &pieces.answers.full[0]);
+        }
+        if (!__shfl_sync(kFullMask, ok, 0)) return;
+        Piece p;
+        if (decode(want, p) && !publish(p)) return;
+        int taken = -1;
+        if (lane == 0) {
+            ok = block.wait_full(pieces.answers, asked);
+            if (ok) {
+                taken = taken_over(&pieces.answer);
+                async_proxy_fence();
+                if constexpr (L::kPair) pair_arrive(first_of_pair(&pieces.answers.empty[0]));
+                else mbarrier_arrive(&pieces.answers.empty[0]);
+            }
+        }
+        asked.next();
+        taken = __shfl_sync(kFullMask, taken, 0);
+        if (taken < 0) break;
+        want = taken / (L::kPair ? 2 : 1);
+    }
+    Piece end{};
+    end.steps = -1;
+    (void)publish(end);
+}
+
+// The other warps: the next piece, if there is one.
+template <typename L> struct Supply {
+    Block<L>& block;
+    Turn<L::kPieces> turn;
+    __device__ __forceinline__ bool next(Piece& p, int lane) {
+        auto& pieces = block.rings->pieces;
+        const bool ok = block.wait_full(pieces.ring, turn);
+        if (ok) p = pieces.piece[turn.at];
+        else p.steps = -1;
+        // (the vote waits for the loads: an arrival would overtake them)
+        const bool all = __all_sync(kFullMask, ok && p.lo >= 0 && p.slot >= -1 && p.steps >= -1);
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&pieces.ring.empty[turn.at]);
+        turn.next();
+        return all && p.steps >= 0;
+    }
+};
+
+// The pieces of products of rows: tiles of kRows rows by kColumns columns.
+template <int kRows, int kColumns> struct DecodeRows {
+    GroupWalk<RowTiles> walk;
+    int64_t column_tiles;
+    int steps, lane;
+    __device__ DecodeRows(const int32_t* offsets, int64_t groups, int64_t rows, int64_t columns, int steps, int lane)
+        : walk(offsets, groups, rows, -1, groups, RowTiles{kRows, (columns + kColumns - 1) / kColumns}),
+          column_tiles((columns + kColumns - 1) / kColumns), steps(steps), lane(lane) {}
+    __device__ bool operator()(int64_t want, Piece& p) {
+        const GroupPiece piece = walk.find(want, lane);
+        if (!piece.found) return false;
+        int64_t tile_row, tile_column;
+        banded(piece.within, (piece.hi - piece.lo + kRows - 1) / kRows, column_tiles, tile_row, tile_column);
+        const bool in_group = piece.group >= 0 && piece.group < walk.groups;
+        p.lo = piece.lo + tile_row * kRows, p.hi = piece.hi, p.slot = -1;
+        p.group = in_group ? static_cast<int>(piece.group) : -1;
+        p.row = 0, p.column = static_cast<int>(tile_column) * kColumns;
+        p.steps = in_group ? steps : 0;
+        return true;
+    }
+};
+
 // A group's rows are cut into segments of `segment` rows; the pieces of work are (segment, tile of the output). A group of more than one segment
 // leaves its tiles in `parts`, in f32, one after the other, and grouped_outer_join adds them up.
 struct OuterPieces {
@@ -143,6 +257,31 @@ __device__ __forceinline__ int64_t parts_before(const int32_t* __restrict__ offs
     }
     return warp_sum(n);
 }
+
+// The pieces of outer products: (segment, tile), kDepth rows to a stage.
+template <int kRows, int kColumns, int kDepth> struct DecodeOuter {
+    int64_t row_tiles, column_tiles, tiles, segment;
+    GroupWalk<OuterPieces> walk;
+    int lane;
+    __device__ DecodeOuter(const int32_t* offsets, int64_t groups, int64_t rows, int64_t height, int64_t columns, int64_t segment, int lane)
+        : row_tiles((height + kRows - 1) / kRows), column_tiles((columns + kColumns - 1) / kColumns), tiles(row_tiles * column_tiles),
+          segment(segment), walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles}), lane(lane) {}
+    __device__ bool operator()(int64_t want, Piece& p) {
+        const GroupPiece piece = walk.find(want, lane);
+        if (!piece.found) return false;
+        const int64_t part = piece.within / tiles;
+        int64_t tile_row, tile_column;
+        banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
+        p.lo = piece.lo + part * segment, p.hi = min(p.lo + segment, piece.hi);
+        p.slot = piece.hi - piece.lo > segment
+                     ? parts_before(walk.offsets, walk.groups, walk.rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within
+                     : -1;
+        p.group = static_cast<int>(piece.group);
+        p.row = static_cast<int>(tile_row) * kRows, p.column = static_cast<int>(tile_column) * kColumns;
+        p.steps = static_cast<int>((p.hi - p.lo + kDepth - 1) / kDepth);
+        return true;
+    }
+};
 
 // Adds up the parts of a tile, in the order of the rows.
 template <typename T, int kRows, int kColumns>
@@ -197,6 +336,24 @@ inline int64_t outer_segment(int64_t rows, int64_t tiles, int workers) {
 }
 // Room for the parts: a group of r > segment rows leaves at most 2 r / segment of each tile.
 inline int64_t most_outer_parts(int64_t rows, int64_t tiles, int64_t segment) { return tiles * (rows / segment * 2); }
+
+// Launches a block, or a pair of them, for each piece of work.
+template <typename L, typename... P, typename... A>
+void launch_blocks(const Call& call, const std::string& op, void (*kernel)(P...), int64_t pieces, const A&... arguments) {
+    allow_dynamic_smem(kernel, call.device, L::kBytes);
+    fits_int32(static_cast<size_t>(2 * pieces), "the number of tiles", op);
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = L::kPair ? 2 : 1, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    config.gridDim = dim3(static_cast<unsigned>(pieces) * (L::kPair ? 2 : 1));
+    config.blockDim = dim3(L::kThreads);
+    config.dynamicSmemBytes = L::kBytes;
+    config.stream = call.stream;
+    MOPS_CUDA_OK(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
+}
 
 template <typename T, int kRows, int kColumns>
 void join_outer(const Call& call, const OuterProblem& p, const float* parts, int64_t most_parts, int64_t tiles, int64_t segment,

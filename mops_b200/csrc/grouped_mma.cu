@@ -20,8 +20,8 @@ namespace mops_b200 {
 
 namespace {
 
-constexpr int kThreads = 256;   // the copying warp, the multiplying warp, four that store, the one that clears, the one that gets work
-constexpr int kClearWarp = 6, kWorkWarp = 7;
+constexpr int kThreads = 256;   // the copying warp, the multiplying warp, four that store, the one that clears, the one that gets pieces
+constexpr int kClearWarp = 6, kPieceWarp = 7;
 constexpr int kStoreWarps = 4;
 constexpr int kStaging = 32 * kBoxRow; // bytes: 32 rows of 64 values, of one warp
 
@@ -35,21 +35,21 @@ template <int kColumns, bool kPaired> struct Layout {
     static constexpr int kStage = kA + kB;
     static constexpr int kStagingAt = kStages * kStage;
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * 2 * kStaging;
-    static constexpr int kPieces = 2;                    // known ahead
+    static constexpr int kPieces = 3;                    // known ahead
+    static constexpr int kThreads = mops_b200::kThreads;
     static constexpr int kBytes = kRingsAt + 512 + 1024; // (boxes begin on multiples of 1024 bytes)
     static constexpr unsigned kTmem = 2 * kColumns;      // columns of tensor memory: two accumulators
     struct Rings {
         Ring<kStages> stages;
         Ring<2> accumulators;
         uint64_t to_clear[kStages]; // the copies of stages that are cleared in part before they count as full
-        Ring<kPieces> pieces;
-        uint4 answers[kPieces];     // whose work is taken over
+        Pieces<kPieces> pieces;
         uint32_t tmem;
         int gave_up;
         __device__ void begin() {
             stages.begin(kPair ? 2 : 1, 1);
             accumulators.begin(1, kPair ? 2 * kStoreWarps : kStoreWarps);
-            pieces.begin(1, (kPair ? 2 : 1) * (kWorkWarp + 1)); // (every warp reads them)
+            pieces.begin(kPieceWarp, kPair);
             for (int i = 0; i < kStages; i++) mbarrier_init(&to_clear[i], 1);
         }
     };
@@ -140,44 +140,6 @@ template <typename L> struct Hand {
     }
 };
 
-// Where a block (or pair) gets its work from: first the piece that it was launched for, then those of blocks that have not begun, so that all are
-// done at about the same time whatever their pieces take. (Dealt out in turn, 1072 equal tiles kept the SMs busy for 87 percent of the time.)
-template <typename L> struct Supply {
-    Block<L>& block;
-    Turn<L::kPieces> turn;
-    bool first = true;
-
-    // All warps but the one that gets work: the next piece, or -1. The same for all of them.
-    __device__ __forceinline__ int64_t next(int lane) {
-        if (first) {
-            first = false;
-            return blockIdx.x / (L::kPair ? 2 : 1);
-        }
-        bool ok = block.wait_full(block.rings->pieces, turn);
-        const int taken = ok ? taken_over(&block.rings->answers[turn.at]) : -1;
-        async_proxy_fence();
-        ok = __all_sync(kFullMask, ok);
-        if (lane == 0) Hand<L>::arrive(&block.rings->pieces.empty[turn.at]);
-        turn.next();
-        return !ok || taken < 0 ? -1 : taken / (L::kPair ? 2 : 1);
-    }
-    // One thread of the warp that gets work: asks for pieces until there are none. (Of a pair the first block asks, and both are told.)
-    __device__ __forceinline__ void get(int rank) {
-        for (;;) {
-            // (the second block's barriers know of its own answers alone; its places are free when the first block's are)
-            if (rank == 0 && !block.wait_empty(block.rings->pieces, turn)) return;
-            mbarrier_arrive_expect(&block.rings->pieces.full[turn.at], 16);
-            if (rank == 0) take_over<L::kPair>(&block.rings->answers[turn.at], &block.rings->pieces.full[turn.at]);
-            if (!block.wait_full(block.rings->pieces, turn)) return;
-            const bool more = taken_over(&block.rings->answers[turn.at]) >= 0;
-            async_proxy_fence();
-            Hand<L>::arrive(&block.rings->pieces.empty[turn.at]);
-            turn.next();
-            if (!more) return;
-        }
-    }
-};
-
 // ---------------------------------------------------------------------------------- rows
 // out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
 template <bool BF16, bool M_MN, int kColumns, bool kPair>
@@ -194,23 +156,17 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
-    const int64_t column_tiles = (columns + kColumns - 1) / kColumns;
-    const int steps = (depth + kBoxDepth - 1) / kBoxDepth;
-    GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{L::kRows, column_tiles});
+    if (warp == kPieceWarp)
+        hand_out(block, rank, lane, DecodeRows<L::kRows, kColumns>(offsets, groups, rows, columns, (depth + kBoxDepth - 1) / kBoxDepth, lane));
+    Supply<L> supply{block};
     Turn<L::kStages> stage;
     Turn<2> tile;     // accumulator
     int64_t sent = 0; // boxes that this warp has fetched or stored
     auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
-    Supply<L> supply{block};
-    if (warp == kWorkWarp && lane == 0) supply.get(rank);
-    if (warp < kWorkWarp) for (int64_t want = supply.next(lane); want >= 0; want = supply.next(lane)) {
-        const GroupPiece piece = walk.find(want, lane);
-        if (!piece.found) continue; // (there is a block for each piece that there could be)
-        int64_t tile_row, tile_column;
-        banded(piece.within, (piece.hi - piece.lo + L::kRows - 1) / L::kRows, column_tiles, tile_row, tile_column);
-        const int64_t row = piece.lo + tile_row * L::kRows + rank * kTileRows; // of this block's half
-        const int column = static_cast<int>(tile_column) * kColumns;
-        const bool in_group = piece.group >= 0 && piece.group < groups;
+    for (Piece piece; warp < kPieceWarp && supply.next(piece, lane);) {
+        const int64_t row = piece.lo + rank * kTileRows; // of this block's half
+        const int column = piece.column, steps = piece.steps;
+        const bool in_group = piece.group >= 0;
         bool ok = true;
         if (warp == 0) {
             if (lane == 0 && in_group) {
@@ -225,9 +181,9 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     if constexpr (M_MN) {
 #pragma unroll
                         for (int j = 0; j < L::kOwnColumns / 64; j++)
-                            H::fetch(b + j * kBoxBytes, map_m, own_column + j * 64, s * kBoxDepth, static_cast<int>(piece.group), full);
+                            H::fetch(b + j * kBoxBytes, map_m, own_column + j * 64, s * kBoxDepth, piece.group, full);
                     } else {
-                        H::fetch(b, map_m, s * kBoxDepth, own_column, static_cast<int>(piece.group), full);
+                        H::fetch(b, map_m, s * kBoxDepth, own_column, piece.group, full);
                     }
                     stage.next();
                     sent++;
@@ -303,25 +259,17 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
-    const int64_t row_tiles = (height + L::kRows - 1) / L::kRows, column_tiles = (columns + kColumns - 1) / kColumns;
-    const int64_t tiles = row_tiles * column_tiles;
-    GroupWalk<OuterPieces> walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles});
+    if (warp == kPieceWarp)
+        hand_out(block, rank, lane, DecodeOuter<L::kRows, kColumns, kBoxDepth>(offsets, groups, rows, height, columns, segment, lane));
+    Supply<L> supply{block};
     Turn<L::kStages> stage;
     Turn<2> tile;
     int64_t sent = 0;
     unsigned cleared = 0; // a bit for each place of the ring: the round of its to_clear
     auto stage_at = [&] { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
-    Supply<L> supply{block};
-    if (warp == kWorkWarp && lane == 0) supply.get(rank);
-    if (warp < kWorkWarp) for (int64_t want = supply.next(lane); want >= 0; want = supply.next(lane)) {
-        const GroupPiece piece = walk.find(want, lane);
-        if (!piece.found) continue; // (there is a block for each piece that there could be)
-        const int64_t part = piece.within / tiles;
-        int64_t tile_row, tile_column;
-        banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
-        const int row = static_cast<int>(tile_row) * L::kRows + rank * kTileRows, column = static_cast<int>(tile_column) * kColumns;
-        const int64_t lo = piece.lo + part * segment, hi = min(lo + segment, piece.hi);
-        const int steps = static_cast<int>((hi - lo + kBoxDepth - 1) / kBoxDepth);
+    for (Piece piece; warp < kPieceWarp && supply.next(piece, lane);) {
+        const int row = piece.row + rank * kTileRows, column = piece.column, steps = piece.steps;
+        const int64_t lo = piece.lo, hi = piece.hi;
         // the rows that do not fill a stage come first: they are cleared while the tile before is multiplied
         const int left = static_cast<int>((hi - lo) % kBoxDepth);
         bool ok = true;
@@ -401,11 +349,10 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 const uint32_t from = tmem_quadrant(block.accumulator(tile), quadrant);
                 const uint32_t staging = block.base + L::kStagingAt + quadrant * 2 * kStaging;
                 tmem_fence_after_sync();
-                if (piece.hi - piece.lo > segment) {
-                    const int64_t slot = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
-                    float* to = parts + (slot * L::kRows + rank * kTileRows + quadrant * 32 + lane) * kColumns;
+                if (piece.slot >= 0) {
+                    float* to = parts + (piece.slot * L::kRows + rank * kTileRows + quadrant * 32 + lane) * kColumns;
                     // (there are more parts than there is room for only where offsets descend, which is reported)
-                    for (int c = 0; c < wide && slot < most_parts; c += 32) {
+                    for (int c = 0; c < wide && piece.slot < most_parts; c += 32) {
                         uint32_t r[32];
                         tmem_load(from + c, r);
                         tmem_wait_load();
@@ -416,11 +363,11 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     }
                 } else {
                     const int here = min(height - band, 32);
-                    uint16_t* to = out + (piece.group * height + band) * static_cast<int64_t>(columns);
+                    uint16_t* to = out + (static_cast<int64_t>(piece.group) * height + band) * columns;
                     if (here > 0 && steps > 0) {
                         // (the copy engine leaves out what lies behind the output's last row)
                         for (int c = 0; c < wide; c += 64)
-                            store_columns<BF16>(from + c, staging, sent, map_out, to, band, static_cast<int>(piece.group),
+                            store_columns<BF16>(from + c, staging, sent, map_out, to, band, piece.group,
                                                         column + c, columns, loose ? here : 32, loose, lane);
                     } else { // a group without rows
                         for (int i = 0; i < here; i++)
@@ -441,24 +388,6 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     if (warp >= 2 && warp < kClearWarp && lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
-}
-
-// Launches a block, or a pair of them, for each piece of work.
-template <typename L, typename... P, typename... A>
-void launch_blocks(const Call& call, const std::string& op, void (*kernel)(P...), int64_t pieces, const A&... arguments) {
-    allow_dynamic_smem(kernel, call.device, L::kBytes);
-    fits_int32(static_cast<size_t>(2 * pieces), "the number of tiles", op);
-    cudaLaunchConfig_t config{};
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = L::kPair ? 2 : 1, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
-    config.gridDim = dim3(static_cast<unsigned>(pieces) * (L::kPair ? 2 : 1));
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = L::kBytes;
-    config.stream = call.stream;
-    MOPS_CUDA_OK(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
 }
 
 } // namespace

@@ -20,7 +20,7 @@ namespace mops_b200 {
 namespace {
 
 constexpr int kSplitWarps = 8, kStoreWarps = 8;
-constexpr int kMultiplyWarp = kSplitWarps + kStoreWarps, kCopyWarp = kMultiplyWarp + 1;
+constexpr int kMultiplyWarp = kSplitWarps + kStoreWarps, kCopyWarp = kMultiplyWarp + 1, kPieceWarp = kMultiplyWarp + 2;
 constexpr int kThreads = (kMultiplyWarp + 4) * 32; // (registers are dealt out to four warps at a time)
 constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kDepth = 32; // values of depth in a stage: a row of 128 bytes in f32
@@ -48,10 +48,13 @@ template <int kColumns> struct Layout {
     static constexpr int kStaging = 32 * 33 * 4; // bytes: 32 x 32 sums of a warp; rows begin one bank apart
     static constexpr int kStagingAt = kStagesAt + kStages * kStage;
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * kStaging;
-    static constexpr int kBytes = kRingsAt + 256 + 1024;
+    static constexpr int kBytes = kRingsAt + 512 + 1024;
     static constexpr unsigned kTmem = 2 * kColumns;
     static constexpr bool kPair = false;
+    static constexpr int kPieces = 3; // known ahead
+    static constexpr int kThreads = mops_b200::kThreads;
     struct Rings {
+        Pieces<kPieces> pieces;
         Ring<kRaws> raws;
         Ring<kStages> stages;
         Ring<2> accumulators;
@@ -62,9 +65,10 @@ template <int kColumns> struct Layout {
             raws.begin(1, kSplitWarps);
             stages.begin(kSplitWarps, 1);
             accumulators.begin(1, kStoreWarps);
+            pieces.begin(kStoreWarps + 2, false); // (those who store, copy and multiply)
         }
     };
-    static_assert(sizeof(Rings) <= 256, "room for the rings");
+    static_assert(sizeof(Rings) <= 512, "room for the rings");
 };
 
 // Operands of a stage. In f32: boxes of rows of 128 bytes, swizzled, K-major one of kRows rows, MN-major one for each 32 rows or columns, 32 rows of depth high.
@@ -172,13 +176,8 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
             for (int k = 0; k < A::kChunks; k++) A::load(a[k], from, k);
 #pragma unroll
             for (int k = 0; k < B::kChunks; k++) B::load(b[k], from + L::kRawA, k);
-            __syncwarp();
-            if (lane == 0) {
-                mbarrier_arrive(&block.rings->raws.empty[raw.at]);
-                ok = block.wait_empty(block.rings->stages, stage);
-            }
+            if (lane == 0) ok = block.wait_empty(block.rings->stages, stage);
             if (!__shfl_sync(kFullMask, ok, 0)) return;
-            raw.next();
             const uint32_t to = block.base + L::kStagesAt + static_cast<uint32_t>(stage.at) * L::kStage;
 #pragma unroll
             for (int k = 0; k < A::kChunks; k++) A::store(a[k], to, k, valid);
@@ -186,8 +185,14 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
             for (int k = 0; k < B::kChunks; k++) B::store(b[k], to + kParts * L::kA, k, valid);
             async_proxy_fence();
             __syncwarp();
-            if (lane == 0) mbarrier_arrive(&block.rings->stages.full[stage.at]);
+            if (lane == 0) {
+                mbarrier_arrive(&block.rings->stages.full[stage.at]);
+                // Not before what was loaded has been used: an arrival overtakes loads that are still queued, and the copy engine would write
+                // over what they are to read.
+                mbarrier_arrive(&block.rings->raws.empty[raw.at]);
+            }
             stage.next();
+            raw.next();
         }
     }
 
@@ -276,55 +281,37 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
-    const int64_t column_tiles = (columns + kColumns - 1) / kColumns;
-    const int steps = (depth + kDepth - 1) / kDepth;
     W work{block};
-    GroupWalk<RowTiles> walk(offsets, groups, rows, -1, groups, RowTiles{kTileRows, column_tiles});
-    struct Tile {
-        bool found, in_group;
-        int64_t row, hi;
-        int group, column;
-    };
-    int64_t want = blockIdx.x;
-    auto next = [&] {
-        const GroupPiece piece = walk.find(want, lane);
-        want += gridDim.x;
-        Tile t;
-        t.found = piece.found;
-        if (!t.found) return t;
-        int64_t tile_row, tile_column;
-        banded(piece.within, (piece.hi - piece.lo + kTileRows - 1) / kTileRows, column_tiles, tile_row, tile_column);
-        t.row = piece.lo + tile_row * kTileRows, t.hi = piece.hi;
-        t.group = static_cast<int>(piece.group), t.column = static_cast<int>(tile_column) * kColumns;
-        t.in_group = piece.group >= 0 && piece.group < groups;
-        return t;
-    };
+    Supply<L> supply{block};
+    Piece piece;
     if (warp < kSplitWarps) {
         fewer_registers<kSplitRegisters>();
         work.split(lane);
     } else if (warp < kMultiplyWarp) {
         more_registers<kStoreRegisters>();
         const int quadrant = warp & 3, half = (warp - kSplitWarps) / 4;
-        for (Tile t = next(); t.found; t = next()) {
+        while (supply.next(piece, lane)) {
             float sum[W::kOwn];
-            if (!work.collect(sum, t.in_group ? steps : 0, quadrant, half, lane)) break;
-            const int64_t row = t.row + quadrant * 32, column = t.column + half * W::kOwn;
-            work.store(sum, warp - kSplitWarps, out + row * columns + column, columns, t.hi - row, columns - column, lane);
+            if (!work.collect(sum, piece.steps, quadrant, half, lane)) break;
+            const int64_t row = piece.lo + quadrant * 32, column = piece.column + half * W::kOwn;
+            work.store(sum, warp - kSplitWarps, out + row * columns + column, columns, piece.hi - row, columns - column, lane);
         }
     } else {
         fewer_registers<kMultiplyRegisters>();
         bool ok = true;
         if (warp == kMultiplyWarp) {
-            for (Tile t = next(); t.found && ok; t = next()) {
-                if (lane == 0 && t.in_group) ok = work.multiply(steps);
+            while (ok && supply.next(piece, lane)) {
+                if (lane == 0) ok = work.multiply(piece.steps);
                 ok = __shfl_sync(kFullMask, ok, 0);
             }
+        } else if (warp == kPieceWarp) {
+            hand_out(block, 0, lane, DecodeRows<kTileRows, kColumns>(offsets, groups, rows, columns, (depth + kDepth - 1) / kDepth, lane));
         } else if (warp == kCopyWarp) {
-            for (Tile t = next(); t.found && ok; t = next()) {
-                if (lane == 0 && t.in_group)
-                    for (int s = 0; s < steps && ok; s++)
-                        ok = work.fetch(map_x, map_m, s * kDepth, static_cast<int>(t.row), M_MN ? t.column : s * kDepth,
-                                        M_MN ? s * kDepth : t.column, t.group, kDepth);
+            while (ok && supply.next(piece, lane)) {
+                if (lane == 0)
+                    for (int s = 0; s < piece.steps && ok; s++)
+                        ok = work.fetch(map_x, map_m, s * kDepth, static_cast<int>(piece.lo), M_MN ? piece.column : s * kDepth,
+                                        M_MN ? s * kDepth : piece.column, piece.group, kDepth);
                 ok = __shfl_sync(kFullMask, ok, 0);
             }
             if (lane == 0) {
@@ -352,66 +339,47 @@ grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
-    const int64_t row_tiles = (height + kTileRows - 1) / kTileRows, column_tiles = (columns + kColumns - 1) / kColumns;
-    const int64_t tiles = row_tiles * column_tiles;
     W work{block};
-    GroupWalk<OuterPieces> walk(offsets, groups, rows, 0, groups - 1, OuterPieces{segment, tiles});
-    struct Piece {
-        bool found, part;
-        int row, column, lo, hi, steps;
-        int64_t group, within;
-    };
-    int64_t want = blockIdx.x;
-    auto next = [&] {
-        const GroupPiece piece = walk.find(want, lane);
-        want += gridDim.x;
-        Piece t;
-        t.found = piece.found;
-        if (!t.found) return t;
-        t.group = piece.group, t.within = piece.within, t.part = piece.hi - piece.lo > segment;
-        const int64_t part = piece.within / tiles;
-        int64_t tile_row, tile_column;
-        banded(piece.within - part * tiles, row_tiles, column_tiles, tile_row, tile_column);
-        t.row = static_cast<int>(tile_row) * kTileRows, t.column = static_cast<int>(tile_column) * kColumns;
-        t.lo = static_cast<int>(piece.lo + part * segment), t.hi = static_cast<int>(min(t.lo + segment, piece.hi));
-        t.steps = (t.hi - t.lo + kDepth - 1) / kDepth;
-        return t;
-    };
+    Supply<L> supply{block};
+    Piece piece;
     if (warp < kSplitWarps) {
         fewer_registers<kSplitRegisters>();
         work.split(lane);
     } else if (warp < kMultiplyWarp) {
         more_registers<kStoreRegisters>();
         const int quadrant = warp & 3, half = (warp - kSplitWarps) / 4;
-        for (Piece t = next(); t.found; t = next()) {
+        while (supply.next(piece, lane)) {
             float sum[W::kOwn];
-            if (!work.collect(sum, t.steps, quadrant, half, lane)) break;
-            if (t.part) {
-                const int64_t slot = parts_before(offsets, groups, rows, t.group, OuterParts{segment, tiles}, lane) + t.within;
+            if (!work.collect(sum, piece.steps, quadrant, half, lane)) break;
+            if (piece.slot >= 0) {
                 // (there are more parts than there is room for only where offsets descend, which is reported)
-                if (slot >= most_parts) continue;
-                float* to = parts + (slot * kTileRows + quadrant * 32 + lane) * kColumns + half * W::kOwn;
+                if (piece.slot >= most_parts) continue;
+                float* to = parts + (piece.slot * kTileRows + quadrant * 32 + lane) * kColumns + half * W::kOwn;
 #pragma unroll
                 for (int i = 0; i < W::kOwn; i += 4)
                     *reinterpret_cast<float4*>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
             } else {
-                const int64_t row = t.row + quadrant * 32, column = t.column + half * W::kOwn;
-                work.store(sum, warp - kSplitWarps, out + (t.group * height + row) * columns + column, columns, height - row, columns - column, lane);
+                const int64_t row = piece.row + quadrant * 32, column = piece.column + half * W::kOwn;
+                work.store(sum, warp - kSplitWarps, out + (static_cast<int64_t>(piece.group) * height + row) * columns + column, columns, height - row,
+                           columns - column, lane);
             }
         }
     } else {
         fewer_registers<kMultiplyRegisters>();
         bool ok = true;
         if (warp == kMultiplyWarp) {
-            for (Piece t = next(); t.found && ok; t = next()) {
-                if (lane == 0) ok = work.multiply(t.steps);
+            while (ok && supply.next(piece, lane)) {
+                if (lane == 0) ok = work.multiply(piece.steps);
                 ok = __shfl_sync(kFullMask, ok, 0);
             }
+        } else if (warp == kPieceWarp) {
+            hand_out(block, 0, lane, DecodeOuter<kTileRows, kColumns, kDepth>(offsets, groups, rows, height, columns, segment, lane));
         } else if (warp == kCopyWarp) {
-            for (Piece t = next(); t.found && ok; t = next()) {
+            while (ok && supply.next(piece, lane)) {
+                const int lo = static_cast<int>(piece.lo), hi = static_cast<int>(piece.hi);
                 if (lane == 0)
-                    for (int s = 0; s < t.steps && ok; s++)
-                        ok = work.fetch(map_x, map_y, t.row, t.lo + s * kDepth, t.column, t.lo + s * kDepth, 0, min(t.hi - t.lo - s * kDepth, kDepth));
+                    for (int s = 0; s < piece.steps && ok; s++)
+                        ok = work.fetch(map_x, map_y, piece.row, lo + s * kDepth, piece.column, lo + s * kDepth, 0, min(hi - lo - s * kDepth, kDepth));
                 ok = __shfl_sync(kFullMask, ok, 0);
             }
             if (lane == 0) {
@@ -454,10 +422,8 @@ bool multiply_rows_split(const Call& call, const RowsProblem& p, const std::stri
                                    : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
         const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
         auto kernel = grouped_rows_split<M_MN, kColumns>;
-        allow_dynamic_smem(kernel, call.device, L::kBytes);
         check_registers(reinterpret_cast<const void*>(kernel), op);
-        kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kThreads, L::kBytes, call.stream>>>(
-            x, m, static_cast<float*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns),
+        launch_blocks<L>(call, op, kernel, tiles, x, m, static_cast<float*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns),
             call.status);
         note_kernel_f("grouped_rows_split<%s,%d>", M_MN ? "columns" : "depth", kColumns);
     };
@@ -486,11 +452,8 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
         float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
                                       : nullptr;
         auto kernel = grouped_outer_split<kColumns>;
-        allow_dynamic_smem(kernel, call.device, L::kBytes);
         check_registers(reinterpret_cast<const void*>(kernel), op);
-        const int64_t pieces = tiles * (rows / segment + p.groups);
-        kernel<<<static_cast<unsigned>(std::min<int64_t>(pieces, sms)), kThreads, L::kBytes, call.stream>>>(
-            x, y, static_cast<float*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns),
+        launch_blocks<L>(call, op, kernel, tiles * (rows / segment + p.groups), x, y, static_cast<float*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns),
             segment, call.status);
         if (rows > segment) {
             join_outer<float, kTileRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);

@@ -280,6 +280,26 @@ def test_grouped_matches_64_bits(dtype, rows, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,K,N", [([3] * 30, 96, 520), ([200, 0, 1, 300], 1000, 40), ([1, 2, 3], 1024, 72), ([5000, 300], 64, 264)])
+def test_grouped_gives_the_same_bits_every_time(dtype, rows, K, N):
+    """Many calls in a row: what the parts of a block hand to each other is never read too early or written over too soon."""
+    A, W = normal((sum(rows), K), dtype, 1), normal((len(rows), K, N), dtype, 2, K ** -0.5)
+    offsets, grad = offsets_of(rows), normal((sum(rows), N), dtype, 3)
+    A, W = A.requires_grad_(True), W.requires_grad_(True)
+
+    def step():
+        output = mt.grouped_matrix_product(A, W, offsets)
+        return [output.detach(), *torch.autograd.grad(output, [A, W], grad)]
+
+    first, differ = step(), torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(300):
+        for x, y in zip(step(), first):
+            differ += (x != y).any()
+    assert differ.item() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("K,N", [(64, 128), (72, 40), (33, 65)])
 def test_grouped_matrices_stored_the_other_way(dtype, K, N):
