@@ -300,8 +300,7 @@ grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t
     const int64_t n = (piece.hi - piece.lo + segment - 1) / segment;
     const int64_t first = parts_before(offsets, groups, rows, piece.group, OuterParts{segment, tiles}, lane) + piece.within;
     if (first + (n - 1) * tiles >= most_parts) return;
-    constexpr int kBlocks = kRows * kColumns / 8192; // to a tile: 32 values to a thread, four at a time
-    for (int at = (blockIdx.y * 256 + threadIdx.x) * 4; at < kRows * kColumns; at += kBlocks * 1024) {
+    for (int at = (blockIdx.y * 256 + threadIdx.x) * 4; at < kRows * kColumns; at += gridDim.y * 1024) { // four values at a time
         const int i = at / kColumns, j = at % kColumns;
         if (row + i >= height || column + j >= columns) continue;
         const float* from = parts + (first * kRows + i) * kColumns + j;
@@ -360,7 +359,9 @@ void join_outer(const Call& call, const OuterProblem& p, const float* parts, int
                 const std::string& op) {
     const int64_t rows = p.X.shape[0], joins = tiles * std::min<int64_t>(p.groups, rows / segment);
     fits_int32(static_cast<size_t>(joins), "the number of tiles", op);
-    grouped_outer_join<T, kRows, kColumns><<<dim3(static_cast<unsigned>(joins), kRows * kColumns / 8192), 256, 0, call.stream>>>(
+    // blocks to a tile: few where there are many tiles (most of which may be whole), up to one for each 1024 values
+    const int64_t most = kRows * kColumns / 1024, shares = std::min(most, std::max(most / 8, ceil_div(int64_t(sm_count(call.device)) * 8, joins)));
+    grouped_outer_join<T, kRows, kColumns><<<dim3(static_cast<unsigned>(joins), static_cast<unsigned>(shares)), 256, 0, call.stream>>>(
         static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(p.X.shape[1]),
         static_cast<int>(p.Y.shape[1]), segment);
     MOPS_CUDA_OK(cudaGetLastError());

@@ -45,7 +45,7 @@ template <int kColumns> struct Layout {
     static constexpr int kRaw = kRawA + kRawB, kStage = kParts * (kA + kB);
     static constexpr int kRaws = kColumns == 128 ? 3 : 4, kStages = 2;
     static constexpr int kStagesAt = kRaws * kRaw;
-    static constexpr int kStaging = 32 * 33 * 4; // bytes: 32 x 32 sums of a warp; rows begin one bank apart
+    static constexpr int kStaging = 32 * 32 * 4; // bytes: 32 x 32 sums of a warp
     static constexpr int kStagingAt = kStagesAt + kStages * kStage;
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * kStaging;
     static constexpr int kBytes = kRingsAt + 512 + 1024;
@@ -248,21 +248,39 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
         return true;
     }
 
-    // Writes them, 32 columns at a time through shared memory, a row after the other; rows of the output may begin anywhere.
-    __device__ __forceinline__ void store(const float (&sum)[kOwn], int warp, float* out, int64_t stride, int64_t here, int64_t wide, int lane) {
-        float* staging = reinterpret_cast<float*>(block.smem + L::kStagingAt + warp * L::kStaging);
+    // Writes them, 32 columns at a time through shared memory: by the copy engine, box by box, or where there are not all 32 rows of a box (`here`), or rows of the
+    // output begin anywhere (loose), a row after the other. out: the first value.
+    __device__ __forceinline__ void store(const float (&sum)[kOwn], int warp, const CUtensorMap& map, int column, int row, int slice, float* out,
+                                          int64_t stride, int64_t here, int64_t wide, bool loose, int lane) {
+        unsigned char* place = block.smem + L::kStagingAt + warp * L::kStaging;
         const int rows = static_cast<int>(min(here, int64_t(32)));
+        const bool box = !loose && rows == 32;
 #pragma unroll
         for (int c = 0; c < kOwn; c += 32) {
-            if (c >= wide) break;
+            if (c >= wide || rows <= 0) break;
+            if (lane == 0) boxes_left<0>();
+            __syncwarp();
+            if (box) {
+                const uint32_t to = smem_address(place);
 #pragma unroll
-            for (int j = 0; j < 32; j++) staging[lane * 33 + j] = sum[c + j];
-            __syncwarp();
-            if (c + lane < wide) {
+                for (int j = 0; j < 8; j++)
+                    smem_store16(to + lane * 128 + ((j ^ (lane & 7)) << 4),
+                                 make_uint4(__float_as_uint(sum[c + 4 * j]), __float_as_uint(sum[c + 4 * j + 1]),
+                                            __float_as_uint(sum[c + 4 * j + 2]), __float_as_uint(sum[c + 4 * j + 3])));
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) box_out(map, column + c, row, slice, to);
+            } else {
+                float* staging = reinterpret_cast<float*>(place);
+#pragma unroll
+                for (int j = 0; j < 32; j++) staging[lane * 32 + (j ^ lane)] = sum[c + j]; // (each lane another bank)
+                __syncwarp();
+                if (c + lane < wide) {
 #pragma unroll 8
-                for (int r = 0; r < rows; r++) out[r * stride + c + lane] = staging[r * 33 + lane];
+                    for (int r = 0; r < rows; r++) out[r * stride + c + lane] = staging[r * 32 + (lane ^ r)];
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
     }
 };
@@ -271,8 +289,9 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
 // out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
 template <bool M_MN, int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
-grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m, float* __restrict__ out,
-                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int depth, int columns, Status st) {
+grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_out,
+                   float* __restrict__ out, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int depth, int columns, bool loose,
+                   Status st) {
     extern __shared__ unsigned char raw[];
     using W = Work<false, M_MN, kColumns>;
     using L = typename W::L;
@@ -294,7 +313,8 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
             float sum[W::kOwn];
             if (!work.collect(sum, piece.steps, quadrant, half, lane)) break;
             const int64_t row = piece.lo + quadrant * 32, column = piece.column + half * W::kOwn;
-            work.store(sum, warp - kSplitWarps, out + row * columns + column, columns, piece.hi - row, columns - column, lane);
+            work.store(sum, warp - kSplitWarps, map_out, column, static_cast<int>(row), 0, out + row * columns + column, columns, piece.hi - row,
+                       columns - column, loose, lane);
         }
     } else {
         fewer_registers<kMultiplyRegisters>();
@@ -320,6 +340,7 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
             }
         }
     }
+    if (lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
 }
@@ -328,9 +349,9 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
 // out[g] = X[rows of g]^T Y[rows of g].
 template <int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
-grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y, float* __restrict__ out,
-                    float* __restrict__ parts, int64_t most_parts, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height,
-                    int columns, int64_t segment, Status st) {
+grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                    const __grid_constant__ CUtensorMap map_out, float* __restrict__ out, float* __restrict__ parts, int64_t most_parts, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height,
+                    int columns, int64_t segment, bool loose, Status st) {
     extern __shared__ unsigned char raw[];
     using W = Work<true, true, kColumns>;
     using L = typename W::L;
@@ -360,8 +381,10 @@ grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     *reinterpret_cast<float4*>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
             } else {
                 const int64_t row = piece.row + quadrant * 32, column = piece.column + half * W::kOwn;
-                work.store(sum, warp - kSplitWarps, out + (static_cast<int64_t>(piece.group) * height + row) * columns + column, columns, height - row,
-                           columns - column, lane);
+                // (the copy engine leaves out what lies behind the output's last row)
+                work.store(sum, warp - kSplitWarps, map_out, column, static_cast<int>(row), piece.group,
+                           out + (static_cast<int64_t>(piece.group) * height + row) * columns + column, columns,
+                           loose || row >= height ? height - row : 32, columns - column, loose, lane);
             }
         }
     } else {
@@ -388,6 +411,7 @@ grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             }
         }
     }
+    if (lane == 0) boxes_left<0>();
     __syncwarp();
     block.end(warp);
 }
@@ -420,11 +444,13 @@ bool multiply_rows_split(const Call& call, const RowsProblem& p, const std::stri
         const CUtensorMap x = tensor_map(p.X.type, p.X.data, p.depth, p.rows, 1, p.X.stride[0], 0, kTileRows);
         const CUtensorMap m = M_MN ? tensor_map(p.X.type, p.M.data, p.columns, p.depth, p.groups, stride, p.M.stride[0], kDepth)
                                    : tensor_map(p.X.type, p.M.data, p.depth, p.columns, p.groups, stride, p.M.stride[0], kColumns);
+        const bool loose = p.columns % 4 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
+        const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, p.columns, p.rows, 1, p.columns, 0, 32);
         const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
         auto kernel = grouped_rows_split<M_MN, kColumns>;
         check_registers(reinterpret_cast<const void*>(kernel), op);
-        launch_blocks<L>(call, op, kernel, tiles, x, m, static_cast<float*>(p.out.data), p.offsets, p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns),
-            call.status);
+        launch_blocks<L>(call, op, kernel, tiles, x, m, out, static_cast<float*>(p.out.data), p.offsets, p.groups, p.rows,
+                         static_cast<int>(p.depth), static_cast<int>(p.columns), loose, call.status);
         note_kernel_f("grouped_rows_split<%s,%d>", M_MN ? "columns" : "depth", kColumns);
     };
     auto by_width = [&](auto major) {
@@ -453,8 +479,10 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
                                       : nullptr;
         auto kernel = grouped_outer_split<kColumns>;
         check_registers(reinterpret_cast<const void*>(kernel), op);
-        launch_blocks<L>(call, op, kernel, tiles * (rows / segment + p.groups), x, y, static_cast<float*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height), static_cast<int>(columns),
-            segment, call.status);
+        const bool loose = columns % 4 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
+        const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
+        launch_blocks<L>(call, op, kernel, tiles * (rows / segment + p.groups), x, y, out, static_cast<float*>(p.out.data), parts, most_parts, p.offsets,
+                         p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {
             join_outer<float, kTileRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);
             scratch_free(call, parts);
