@@ -6,9 +6,10 @@
 // grows with the number of additions; so an accumulator takes kRun stages (64 values of depth) and is then added, rounded, to sums in
 // registers. An infinite or NaN operand gives NaN.
 //
-// The copy engine fetches boxes of f32 into one ring of stages; eight warps split them into the parts of a second ring; one thread issues the
-// products; eight warps add up what the accumulators hold and store the tiles. Bounded by shared memory, which moves 13 bytes for each byte of operand: in,
-// out, three halves in, and six times half a byte into each of the products.
+// The copy engine fetches boxes of f32 into one ring of stages; eight warps split them, the parts of the rows' operand go to tensor memory and those of the other to
+// a second ring; one thread issues the products; eight warps add up what the accumulators hold and store the tiles. Bounded by shared memory: of a stage of 64 values of
+// depth, 128 x 128, it moves 64 KB in, 64 KB out, 48 KB of parts in and 96 KB of them to the tensor cores. (With the parts of both operands in shared memory
+// it was 416 KB, and 2.0 us for such a stage.)
 #include <mutex>
 #include <set>
 
@@ -41,15 +42,18 @@ template <int kRegisters> __device__ __forceinline__ void fewer_registers() {
 
 template <int kColumns> struct Layout {
     static constexpr int kRawA = kTileRows * kDepth * 4, kRawB = kColumns * kDepth * 4; // bytes of a stage of f32
-    static constexpr int kA = kRawA / 2, kB = kRawB / 2;                                // of one part
-    static constexpr int kRaw = kRawA + kRawB, kStage = kParts * (kA + kB);
-    static constexpr int kRaws = kColumns == 128 ? 3 : 4, kStages = 2;
+    static constexpr int kB = kRawB / 2;                                                // of one part
+    static constexpr int kRaw = kRawA + kRawB, kStage = kParts * kB;
+    static constexpr int kRaws = kColumns == 128 ? 4 : 6, kStages = 2;
+    static constexpr int kPartColumns = kDepth / 2; // of tensor memory, of a part of the rows' operand
     static constexpr int kStagesAt = kRaws * kRaw;
     static constexpr int kStaging = 32 * 32 * 4; // bytes: 32 x 32 sums of a warp
     static constexpr int kStagingAt = kStagesAt + kStages * kStage;
     static constexpr int kRingsAt = kStagingAt + kStoreWarps * kStaging;
     static constexpr int kBytes = kRingsAt + 512 + 1024;
-    static constexpr unsigned kTmem = 2 * kColumns;
+    static constexpr unsigned kSums = 2 * kColumns; // columns of tensor memory of the accumulators; the parts come behind them
+    static constexpr unsigned kTmem = kColumns == 128 ? 512 : 256;
+    static_assert(kSums + kStages * kParts * kPartColumns <= kTmem, "room for the parts");
     static constexpr bool kPair = false;
     static constexpr int kPieces = 3; // known ahead
     static constexpr int kThreads = mops_b200::kThreads;
@@ -71,9 +75,57 @@ template <int kColumns> struct Layout {
     static_assert(sizeof(Rings) <= 512, "room for the rings");
 };
 
-// Operands of a stage. In f32: boxes of rows of 128 bytes, swizzled, K-major one of kRows rows, MN-major one for each 32 rows or columns, 32 rows of depth high.
-// In parts: K-major kRows rows of 64 bytes, MN-major boxes of 64 rows or columns, 32 rows of 128 bytes.
-template <bool MN, int kRows> struct Operand {
+// Cuts the top eight bits off each of two values and returns them side by side.
+__device__ __forceinline__ uint32_t cut_part(uint32_t& x, uint32_t& y) {
+    const uint32_t part = __byte_perm(x, y, 0x7632); // the upper halves
+    x = __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffff0000u));
+    y = __float_as_uint(__uint_as_float(y) - __uint_as_float(y & 0xffff0000u));
+    return part;
+}
+
+// Operands of a stage in f32: boxes of rows of 128 bytes, swizzled; K-major one of a row for each row or column of the operand, MN-major one for each 32 of
+// them, 32 rows of depth high.
+//
+// The rows' operand, by its lanes of tensor memory: warps w and w + 4 take 32 rows, half of the depth each.
+template <bool MN> struct RowOperand {
+    static constexpr int kBoxHeight = MN ? kDepth : kTileRows, kBoxes = MN ? kTileRows / 32 : 1, kHalf = kDepth / 2;
+    // (Eight neighbouring lanes read from different banks.)
+    __device__ static __forceinline__ void load(uint32_t (&x)[kHalf], uint32_t raw, int quadrant, int half, int lane) {
+        if constexpr (MN) {
+            const uint32_t box = raw + quadrant * (kDepth * 128) + lane % 4 * 4;
+#pragma unroll
+            for (int i = 0; i < kHalf; i++) {
+                const int d = half * kHalf + i;
+                x[i] = smem_load4(box + d * 128 + ((lane / 4 ^ (d & 7)) << 4));
+            }
+        } else {
+            const uint32_t row = raw + (quadrant * 32 + lane) * 128;
+#pragma unroll
+            for (int c = 0; c < kHalf / 4; c++) {
+                const uint4 v = smem_load16(row + (((half * (kHalf / 4) + c) ^ (lane & 7)) << 4));
+                x[4 * c] = v.x, x[4 * c + 1] = v.y, x[4 * c + 2] = v.z, x[4 * c + 3] = v.w;
+            }
+        }
+    }
+    // to: the stage's first column, in the warp's lanes
+    __device__ static __forceinline__ void store(uint32_t (&x)[kHalf], uint32_t to, int half, int valid) {
+        if constexpr (MN) { // rows of depth of another group
+#pragma unroll
+            for (int i = 0; i < kHalf; i++)
+                if (half * kHalf + i >= valid) x[i] = 0;
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            uint32_t w[kHalf / 2];
+#pragma unroll
+            for (int j = 0; j < kHalf / 2; j++) w[j] = cut_part(x[2 * j], x[2 * j + 1]);
+            tmem_store(to + p * (kDepth / 2) + half * (kHalf / 2), w);
+        }
+    }
+};
+
+// The columns' operand. In parts: K-major kRows rows of 64 bytes, MN-major boxes of 64 columns, 32 rows of 128 bytes.
+template <bool MN, int kRows> struct ColumnOperand {
     static constexpr int kChunks = kRows * kDepth / 8 / kSplitThreads; // of eight values, of a thread
     static constexpr int kPart = kRows * kDepth * 2;
     static constexpr int kBoxHeight = MN ? kDepth : kRows, kBoxes = MN ? kRows / 32 : 1;
@@ -114,13 +166,7 @@ template <bool MN, int kRows> struct Operand {
         for (int p = 0; p < kParts; p++) {
             uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                w[j] = __byte_perm(x[2 * j], x[2 * j + 1], 0x7632); // the upper halves
-                if (p + 1 == kParts) continue;
-#pragma unroll
-                for (int h = 2 * j; h < 2 * j + 2; h++)
-                    x[h] = __float_as_uint(__uint_as_float(x[h]) - __uint_as_float(x[h] & 0xffff0000u));
-            }
+            for (int j = 0; j < 4; j++) w[j] = cut_part(x[2 * j], x[2 * j + 1]);
             smem_store16(to + p * kPart, make_uint4(w[0], w[1], w[2], w[3]));
         }
     }
@@ -130,8 +176,8 @@ template <bool MN, int kRows> struct Operand {
 // What the parts of a block do, of both kernels.
 template <bool A_MN, bool B_MN, int kColumns> struct Work {
     using L = Layout<kColumns>;
-    using A = Operand<A_MN, kTileRows>;
-    using B = Operand<B_MN, kColumns>;
+    using A = RowOperand<A_MN>;
+    using B = ColumnOperand<B_MN, kColumns>;
     static constexpr int kOwn = kColumns / 2; // columns of a storing warp
 
     Block<L>& block;
@@ -162,7 +208,12 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
     }
 
     // A splitting warp, until no more stages come.
-    __device__ __forceinline__ void split(int lane) {
+    __device__ __forceinline__ uint32_t parts_at() const {
+        return block.rings->tmem + L::kSums + static_cast<uint32_t>(stage.at) * (kParts * L::kPartColumns);
+    }
+    __device__ __forceinline__ uint32_t stage_at() const { return block.base + L::kStagesAt + static_cast<uint32_t>(stage.at) * L::kStage; }
+
+    __device__ __forceinline__ void split(int warp, int lane) {
         for (;;) {
             bool ok = true;
             if (lane == 0) ok = block.wait_full(block.rings->raws, raw);
@@ -171,18 +222,19 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
             const int valid = *static_cast<volatile int*>(&block.rings->valid[raw.at]);
             if (valid < 0) return;
             const uint32_t from = block.base + static_cast<uint32_t>(raw.at) * L::kRaw;
-            uint4 a[A::kChunks][2], b[B::kChunks][2];
-#pragma unroll
-            for (int k = 0; k < A::kChunks; k++) A::load(a[k], from, k);
+            uint32_t a[A::kHalf];
+            uint4 b[B::kChunks][2];
+            A::load(a, from, warp & 3, warp / 4, lane);
 #pragma unroll
             for (int k = 0; k < B::kChunks; k++) B::load(b[k], from + L::kRawA, k);
             if (lane == 0) ok = block.wait_empty(block.rings->stages, stage);
             if (!__shfl_sync(kFullMask, ok, 0)) return;
-            const uint32_t to = block.base + L::kStagesAt + static_cast<uint32_t>(stage.at) * L::kStage;
+            tmem_fence_after_sync();
+            A::store(a, tmem_quadrant(parts_at(), warp), warp / 4, valid);
 #pragma unroll
-            for (int k = 0; k < A::kChunks; k++) A::store(a[k], to, k, valid);
-#pragma unroll
-            for (int k = 0; k < B::kChunks; k++) B::store(b[k], to + kParts * L::kA, k, valid);
+            for (int k = 0; k < B::kChunks; k++) B::store(b[k], stage_at(), k, valid);
+            tmem_wait_store();
+            tmem_fence_before_sync();
             async_proxy_fence();
             __syncwarp();
             if (lane == 0) {
@@ -198,21 +250,20 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
 
     // The multiplying thread: a tile.
     __device__ __forceinline__ bool multiply(int steps) {
-        constexpr uint32_t instruction = instruction_descriptor(true, A_MN, B_MN, kColumns);
+        constexpr uint32_t instruction = instruction_descriptor(true, false, B_MN, kColumns);
         constexpr int part_a[6] = {0, 2, 1, 0, 1, 0}, part_b[6] = {2, 0, 1, 1, 0, 0}; // small products first
         for (int s = 0; s < steps; s++) {
             if (s % kRun == 0 && !block.wait_empty(block.rings->accumulators, run)) return false;
             if (!block.wait_full(block.rings->stages, stage)) return false;
             tmem_fence_after_sync();
-            const uint32_t at = block.base + L::kStagesAt + static_cast<uint32_t>(stage.at) * L::kStage;
-            const uint64_t a = A::descriptor(at), b = B::descriptor(at + kParts * L::kA);
-            const uint32_t accumulator = block.accumulator(run);
+            const uint32_t a = parts_at(), accumulator = block.rings->tmem + static_cast<uint32_t>(run.at) * kColumns;
+            const uint64_t b = B::descriptor(stage_at());
 #pragma unroll
             for (int i = 0; i < 6; i++)
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; k++)
-                    umma(accumulator, a + (part_a[i] * (L::kA >> 4) + k * A::kStep), b + (part_b[i] * (L::kB >> 4) + k * B::kStep), instruction,
-                         s % kRun + i + k > 0);
+                    umma_from_tmem(accumulator, a + part_a[i] * L::kPartColumns + k * 8, b + (part_b[i] * (L::kB >> 4) + k * B::kStep), instruction,
+                                   s % kRun + i + k > 0);
             umma_arrive(&block.rings->stages.empty[stage.at]);
             stage.next();
             if ((s + 1) % kRun == 0 || s + 1 == steps) {
@@ -230,7 +281,7 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
         for (int s = 0; s < steps; s += kRun) {
             if (!block.wait_full(block.rings->accumulators, run)) return false;
             tmem_fence_after_sync();
-            const uint32_t from = tmem_quadrant(block.accumulator(run), quadrant) + half * kOwn;
+            const uint32_t from = tmem_quadrant(block.rings->tmem + static_cast<uint32_t>(run.at) * kColumns, quadrant) + half * kOwn;
 #pragma unroll
             for (int c = 0; c < kOwn; c += 32) {
                 uint32_t r[32];
@@ -305,7 +356,7 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
     Piece piece;
     if (warp < kSplitWarps) {
         fewer_registers<kSplitRegisters>();
-        work.split(lane);
+        work.split(warp, lane);
     } else if (warp < kMultiplyWarp) {
         more_registers<kStoreRegisters>();
         const int quadrant = warp & 3, half = (warp - kSplitWarps) / 4;
@@ -365,7 +416,7 @@ grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     Piece piece;
     if (warp < kSplitWarps) {
         fewer_registers<kSplitRegisters>();
-        work.split(lane);
+        work.split(warp, lane);
     } else if (warp < kMultiplyWarp) {
         more_registers<kStoreRegisters>();
         const int quadrant = warp & 3, half = (warp - kSplitWarps) / 4;

@@ -39,6 +39,13 @@ __device__ __forceinline__ void umma(uint32_t accumulator, uint64_t a, uint64_t 
                  "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate))
                  : "memory");
 }
+// With the rows' operand in tensor memory: a row to a lane, two values of depth to a column.
+__device__ __forceinline__ void umma_from_tmem(uint32_t accumulator, uint32_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(accumulator),
+                 "r"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate))
+                 : "memory");
+}
 // Arrives on `bar` when the products issued so far by this thread are done.
 __device__ __forceinline__ void umma_arrive(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_address(bar))
@@ -80,6 +87,11 @@ __device__ __forceinline__ void smem_store16(uint32_t address, uint4 v) {
 __device__ __forceinline__ uint16_t smem_load2(uint32_t address) {
     uint16_t v;
     asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t smem_load4(uint32_t address) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(address) : "memory");
     return v;
 }
 __device__ __forceinline__ uint4 smem_load16(uint32_t address) {
