@@ -122,7 +122,7 @@ grouped_outer_plain(T* __restrict__ out, const T* __restrict__ X, int64_t x_stri
 const char* const kIndexNames[] = {"offsets"};
 
 void multiply_rows(const Call& call, const RowsProblem& p, const std::string& op) {
-    if (p.rows == 0 || p.columns == 0 || multiply_rows_mma(call, p, op) ||
+    if (p.rows == 0 || p.columns == 0 || multiply_rows_few(call, p, op) || multiply_rows_mma(call, p, op) ||
         multiply_rows_split(call, p, op))
         return;
     for_type(p.X.type, [&](auto zero) {

@@ -21,6 +21,9 @@ struct OuterProblem {
     int64_t groups;
 };
 
+// A few rows in all, as single tokens are (grouped_few.cu): false if there are too many.
+bool multiply_rows_few(const Call& call, const RowsProblem& p, const std::string& op);
+
 // On arrays that the copy engine can fetch (pack.hpp); f16 and bf16 in grouped_mma.cu, f32 in grouped_split.cu. false: not taken on
 // (another type, or nothing to multiply).
 bool multiply_rows_mma(const Call& call, const RowsProblem& p, const std::string& op);

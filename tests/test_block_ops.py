@@ -301,6 +301,20 @@ def test_grouped_gives_the_same_bits_every_time(dtype, rows, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("other_way", [False, True])
+@pytest.mark.parametrize("before,rows,after,K,N", [
+    (0, [1], 0, 4096, 8), (1, [0, 2, 0], 2, 1096, 2056), (0, [1] * 20 + [0] * 30 + [12], 0, 584, 136), (3, [17, 0, 1], 4, 264, 392),
+    (0, [32], 0, 2048, 264), (0, [9, 70, 0, 20], 1, 2120, 2072), (5, [60, 0, 63], 0, 2048, 40), (0, [2, 5, 1, 0, 3], 0, 1536, 1024),
+    (0, [0, 0, 0], 7, 128, 128), (0, [33], 0, 2056, 2304)])
+def test_grouped_few_rows(dtype, other_way, before, rows, after, K, N):
+    """Single tokens: the depth is cut into parts, the rows of no group are zero."""
+    R = before + sum(rows) + after
+    W = normal((len(rows), N, K), dtype, 2, K ** -0.5).transpose(1, 2) if other_way else normal((len(rows), K, N), dtype, 2, K ** -0.5)
+    check_grouped(normal((R, K), dtype, 1), W, offsets_of(rows) + before, normal((R, N), dtype, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("K,N", [(64, 128), (72, 40), (33, 65)])
 def test_grouped_matrices_stored_the_other_way(dtype, K, N):
     rows = [100, 0, 37, 260]
