@@ -74,7 +74,34 @@ tensor_list first_derivative(const tensor_list& differentiable, const Args&... a
     return at::GradMode::is_enabled() || tangent ? Backward::apply(args...) : Backward::run(args...);
 }
 
+// Whether a call leaves something to differentiate (or to refuse to). What does not, goes without a Function, whose node and saved variables take
+// the host as long as the rest of a call.
+bool differentiated(std::initializer_list<const Tensor*> arguments) {
+    const bool recorded = at::GradMode::is_enabled();
+    for (const Tensor* t : arguments)
+        if (t->defined() && ((recorded && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
+    return false;
+}
+
 // ====================================================================== embedding_lookup
+// Arguments are replaced by what the kernels take.
+Tensor run_embedding_lookup(Tensor& W, Tensor& indices, double scale, int64_t padding_index) {
+    static constexpr const char* op = "embedding_lookup";
+    same_device({W, indices});
+    block_types({W});
+    int32_indices({indices});
+    ndim(W, 2, "W", op);
+    ndim(indices, 1, "indices", op);
+    cuda_only(W, op);
+    if (padding_index < -1 || padding_index >= W.size(0))
+        C10_THROW_ERROR(ValueError, "padding_index " + std::to_string(padding_index) + " is not a row of W in " + op);
+    W = rows_of(W);
+    indices = indices.contiguous();
+    Tensor output = torch::empty({indices.size(0), W.size(1)}, W.options());
+    on_stream_of(W, [&] { checked(mops_b200_cuda_embedding_lookup(array(output), array(W), array(indices), scale)); });
+    return output;
+}
+
 struct EmbeddingLookupBackward : torch::autograd::Function<EmbeddingLookupBackward> {
     static tensor_list run(const Tensor& grad_output, const Tensor& indices, int64_t rows, double scale, int64_t padding_index) {
         Tensor grad_W = torch::empty({rows, grad_output.size(1)}, grad_output.options());
@@ -93,19 +120,7 @@ struct EmbeddingLookupBackward : torch::autograd::Function<EmbeddingLookupBackwa
 
 struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
     static Tensor forward(AutogradContext* ctx, Tensor W, Tensor indices, double scale, int64_t padding_index) {
-        static constexpr const char* op = "embedding_lookup";
-        same_device({W, indices});
-        block_types({W});
-        int32_indices({indices});
-        ndim(W, 2, "W", op);
-        ndim(indices, 1, "indices", op);
-        cuda_only(W, op);
-        if (padding_index < -1 || padding_index >= W.size(0))
-            C10_THROW_ERROR(ValueError, "padding_index " + std::to_string(padding_index) + " is not a row of W in " + op);
-        W = rows_of(W);
-        indices = indices.contiguous();
-        Tensor output = torch::empty({indices.size(0), W.size(1)}, W.options());
-        on_stream_of(W, [&] { checked(mops_b200_cuda_embedding_lookup(array(output), array(W), array(indices), scale)); });
+        Tensor output = run_embedding_lookup(W, indices, scale, padding_index);
         ctx->save_for_backward({indices});
         ctx->saved_data["rows"] = W.size(0);
         ctx->saved_data["scale"] = scale;
@@ -127,6 +142,23 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
 Tensor matrices_of(const Tensor& W) {
     if (W.is_neg() || W.is_conj()) return W.resolve_neg().resolve_conj().contiguous();
     return W.stride(2) == 1 || W.stride(1) == 1 ? W : W.contiguous();
+}
+
+Tensor run_grouped_matrix_product(Tensor& A, Tensor& W, Tensor& offsets) {
+    static constexpr const char* op = "grouped_matrix_product";
+    same_device({A, W, offsets});
+    block_types({A, W});
+    int32_indices({offsets});
+    ndim(A, 2, "A", op);
+    ndim(W, 3, "W", op);
+    ndim(offsets, 1, "offsets", op);
+    cuda_only(A, op);
+    A = rows_of(A);
+    W = matrices_of(W);
+    offsets = offsets.contiguous();
+    Tensor output = torch::empty({A.size(0), W.size(2)}, A.options());
+    on_stream_of(A, [&] { checked(mops_b200_cuda_grouped_matrix_product(array(output), array(A), array(W), array(offsets))); });
+    return output;
 }
 
 struct GroupedMatrixProductBackward : torch::autograd::Function<GroupedMatrixProductBackward> {
@@ -151,19 +183,7 @@ struct GroupedMatrixProductBackward : torch::autograd::Function<GroupedMatrixPro
 
 struct GroupedMatrixProduct : torch::autograd::Function<GroupedMatrixProduct> {
     static Tensor forward(AutogradContext* ctx, Tensor A, Tensor W, Tensor offsets) {
-        static constexpr const char* op = "grouped_matrix_product";
-        same_device({A, W, offsets});
-        block_types({A, W});
-        int32_indices({offsets});
-        ndim(A, 2, "A", op);
-        ndim(W, 3, "W", op);
-        ndim(offsets, 1, "offsets", op);
-        cuda_only(A, op);
-        A = rows_of(A);
-        W = matrices_of(W);
-        offsets = offsets.contiguous();
-        Tensor output = torch::empty({A.size(0), W.size(2)}, A.options());
-        on_stream_of(A, [&] { checked(mops_b200_cuda_grouped_matrix_product(array(output), array(A), array(W), array(offsets))); });
+        Tensor output = run_grouped_matrix_product(A, W, offsets);
         ctx->save_for_backward({A, W, offsets});
         return output;
     }
@@ -177,6 +197,31 @@ struct GroupedMatrixProduct : torch::autograd::Function<GroupedMatrixProduct> {
 };
 
 // =================================================================== gated_residual_norm
+// (gate: none if it is not defined)
+tensor_list run_gated_residual_norm(Tensor& residual, Tensor& branch, Tensor& gate, Tensor& scale, Tensor& weight_branch, Tensor& weight_output,
+                                    double epsilon) {
+    static constexpr const char* op = "gated_residual_norm";
+    tensor_list all = {residual, branch, scale, weight_branch, weight_output};
+    if (gate.defined()) all.push_back(gate);
+    same_device(all);
+    block_types(all);
+    ndim(residual, 2, "residual", op);
+    ndim(branch, 2, "branch", op);
+    if (gate.defined()) ndim(gate, 2, "gate", op);
+    ndim(scale, 1, "scale", op);
+    ndim(weight_branch, 1, "weight_branch", op);
+    ndim(weight_output, 1, "weight_output", op);
+    cuda_only(residual, op);
+    for (Tensor* t : {&residual, &branch, &scale, &weight_branch, &weight_output}) *t = rows_of(*t);
+    if (gate.defined()) gate = rows_of(gate);
+    Tensor stream = torch::empty(residual.sizes(), residual.options()), normed = torch::empty(residual.sizes(), residual.options());
+    on_stream_of(residual, [&] {
+        checked(mops_b200_cuda_gated_residual_norm(array(stream), array(normed), array(residual), array(branch), array(gate), array(scale),
+                                                   array(weight_branch), array(weight_output), epsilon));
+    });
+    return {stream, normed};
+}
+
 struct GatedResidualNormBackward : torch::autograd::Function<GatedResidualNormBackward> {
     // need: one bit for each input, in order
     static tensor_list run(const Tensor& grad_stream, const Tensor& grad_normed, const Tensor& residual, const Tensor& branch,
@@ -207,30 +252,11 @@ struct GatedResidualNormBackward : torch::autograd::Function<GatedResidualNormBa
 struct GatedResidualNorm : torch::autograd::Function<GatedResidualNorm> {
     static tensor_list forward(AutogradContext* ctx, Tensor residual, Tensor branch, std::optional<Tensor> optional_gate,
                                Tensor scale, Tensor weight_branch, Tensor weight_output, double epsilon) {
-        static constexpr const char* op = "gated_residual_norm";
         Tensor gate = optional_gate.value_or(Tensor());
-        tensor_list all = {residual, branch, scale, weight_branch, weight_output};
-        if (gate.defined()) all.push_back(gate);
-        same_device(all);
-        block_types(all);
-        ndim(residual, 2, "residual", op);
-        ndim(branch, 2, "branch", op);
-        if (gate.defined()) ndim(gate, 2, "gate", op);
-        ndim(scale, 1, "scale", op);
-        ndim(weight_branch, 1, "weight_branch", op);
-        ndim(weight_output, 1, "weight_output", op);
-        cuda_only(residual, op);
-        for (Tensor* t : {&residual, &branch, &scale, &weight_branch, &weight_output}) *t = rows_of(*t);
-        if (gate.defined()) gate = rows_of(gate);
-        Tensor stream = torch::empty(residual.sizes(), residual.options()), normed = torch::empty_like(stream);
-        on_stream_of(residual, [&] {
-            checked(mops_b200_cuda_gated_residual_norm(array(stream), array(normed), array(residual), array(branch),
-                                                       array(gate), array(scale), array(weight_branch),
-                                                       array(weight_output), epsilon));
-        });
+        tensor_list r = run_gated_residual_norm(residual, branch, gate, scale, weight_branch, weight_output, epsilon);
         ctx->save_for_backward({residual, branch, gate, scale, weight_branch, weight_output});
         ctx->saved_data["epsilon"] = epsilon;
-        return {stream, normed};
+        return r;
     }
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         auto s = ctx->get_saved_variables();
@@ -252,15 +278,20 @@ struct GatedResidualNorm : torch::autograd::Function<GatedResidualNorm> {
 
 // ------------------------------------------------------------------ registered entry points
 Tensor embedding_lookup(Tensor W, Tensor indices, double scale, int64_t padding_index) {
-    return EmbeddingLookup::apply(W, indices, scale, padding_index);
+    return differentiated({&W}) ? EmbeddingLookup::apply(W, indices, scale, padding_index)
+                                : run_embedding_lookup(W, indices, scale, padding_index);
 }
 
-Tensor grouped_matrix_product(Tensor A, Tensor W, Tensor offsets) { return GroupedMatrixProduct::apply(A, W, offsets); }
+Tensor grouped_matrix_product(Tensor A, Tensor W, Tensor offsets) {
+    return differentiated({&A, &W}) ? GroupedMatrixProduct::apply(A, W, offsets) : run_grouped_matrix_product(A, W, offsets);
+}
 
 std::tuple<Tensor, Tensor> gated_residual_norm(Tensor residual, Tensor branch, std::optional<Tensor> gate, Tensor scale,
                                                Tensor weight_branch, Tensor weight_output, double epsilon) {
-    auto r = GatedResidualNorm::apply(residual, branch, gate, scale, weight_branch,
-                                      weight_output, epsilon);
+    Tensor given = gate.value_or(Tensor());
+    auto r = differentiated({&residual, &branch, &given, &scale, &weight_branch, &weight_output})
+                 ? GatedResidualNorm::apply(residual, branch, gate, scale, weight_branch, weight_output, epsilon)
+                 : run_gated_residual_norm(residual, branch, given, scale, weight_branch, weight_output, epsilon);
     return {r[0], r[1]};
 }
 
