@@ -327,11 +327,14 @@ grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t
 }
 
 // How many rows a segment has. Where a group has tiles for all `workers` (blocks, or pairs), its rows are not cut: what parts cost to write and to join is
-// that of some 800 rows of a tile. Where it has fewer, segments are such that, were all rows in one group, there would be one and a half pieces for
-// each worker, but have 1024 rows at least (6000 rows of 24 groups, 1024 x 768 in bf16: 54 us with three pieces and 256 rows, 28 us uncut; 100 003 of 20 groups, 128 x 128
-// in f32: 62 and 54 us).
-inline int64_t outer_segment(int64_t rows, int64_t tiles, int workers) {
+// that of some 800 rows of a tile. Where all groups together have tiles for half of the workers at most, segments are such that there are no more pieces than workers, as a group
+// leaves one that is not full (30 000 rows of 8 groups, 128 x 128 in f32: 25 us; of 1024 rows 45; 100 003 rows of 20: 45.6 and 50.3). In between they are such that,
+// were all rows in one group, there would be one and a half pieces for each worker, but have 1024 rows at least (6000 rows of 24 groups, 1024 x 768 in bf16: 28 us; with three
+// pieces and 256 rows 54).
+inline int64_t outer_segment(int64_t rows, int64_t groups, int64_t tiles, int workers) {
     if (tiles >= workers) return std::max<int64_t>(rows, 1);
+    const int64_t others = workers - groups * tiles; // that do not work on the last segment of a group
+    if (2 * others >= workers) return std::max<int64_t>(ceil_div(rows * tiles, others * kBoxDepth) * kBoxDepth, 256);
     return std::max<int64_t>(ceil_div(2 * rows * tiles, int64_t(workers) * 3 * kBoxDepth) * kBoxDepth, 1024);
 }
 // Room for the parts: a group of r > segment rows leaves at most 2 r / segment of each tile.

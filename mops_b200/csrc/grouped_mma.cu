@@ -454,7 +454,7 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         const CUtensorMap y = tensor_map(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, 64);
         const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
         const int64_t tiles = ceil_div(height, L::kRows) * ceil_div(columns, kColumns);
-        const int64_t segment = outer_segment(rows, tiles, kPair ? sms / 2 : sms), most_parts = most_outer_parts(rows, tiles, segment);
+        const int64_t segment = outer_segment(rows, p.groups, tiles, kPair ? sms / 2 : sms), most_parts = most_outer_parts(rows, tiles, segment);
         float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * L::kRows * kColumns * sizeof(float)))
                                       : nullptr;
         launch_blocks<L>(call, op, grouped_outer_mma<BF16, kColumns, kPair>, tiles * (rows / segment + p.groups), x, y, out,

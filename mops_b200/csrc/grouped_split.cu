@@ -525,7 +525,7 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
         const CUtensorMap x = tensor_map(p.X.type, p.X.data, height, rows, 1, p.X.stride[0], 0, kDepth);
         const CUtensorMap y = tensor_map(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, kDepth);
         const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
-        const int64_t segment = outer_segment(rows, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
+        const int64_t segment = outer_segment(rows, p.groups, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
         float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
                                       : nullptr;
         auto kernel = grouped_outer_split<kColumns>;
