@@ -34,51 +34,60 @@ struct Divider {
 // work whatever the width of a row, and a single token still uses many SMs.
 constexpr int kPacksPerThread = 4;
 
+// Writes what this call does not read again: the line goes to memory before others do.
+template <typename T, int N> __device__ __forceinline__ void store_through(T* to, const Pack<T, N>& v) {
+    if constexpr (N * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&v));
+    else *reinterpret_cast<Pack<T, N>*>(to) = v;
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
 embedding_rows(T* __restrict__ output, const T* __restrict__ W, int64_t stride, const int32_t* __restrict__ indices,
                int64_t index_stride, int64_t tokens, int64_t rows, uint32_t packs, Divider by_packs, Sum<T> scale, Status st) {
     const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * kPacksPerThread);
-    const int64_t t0 = first / packs;
+    const int64_t t0 = first >> 32 ? first / packs : by_packs.divide(static_cast<uint32_t>(first));
     const uint32_t p0 = static_cast<uint32_t>(first - t0 * packs);
-    Pack<T, N> value[kPacksPerThread];
+    // all indices, then all values: each load of a thread is on its way before the first is waited for
     int64_t token[kPacksPerThread];
     uint32_t pack[kPacksPerThread];
+    int32_t row[kPacksPerThread];
 #pragma unroll
     for (int k = 0; k < kPacksPerThread; k++) {
         const uint32_t at = p0 + k * kThreads + threadIdx.x;
         const uint32_t t = by_packs.divide(at);
         token[k] = t0 + t;
         pack[k] = at - t * packs;
-        if (token[k] >= tokens) continue;
-        const int32_t row = __ldg(indices + token[k] * index_stride);
-        if (static_cast<uint32_t>(row) < static_cast<uint64_t>(rows)) {
-            value[k] = *reinterpret_cast<const Pack<T, N>*>(W + row * stride + static_cast<int64_t>(pack[k]) * N);
-        } else {
-            if (pack[k] == 0) report_bad_index(st, 0);
+        row[k] = __ldg(indices + min(token[k], tokens - 1) * index_stride);
+    }
+    Pack<T, N> value[kPacksPerThread];
 #pragma unroll
-            for (int i = 0; i < N; i++) value[k].v[i] = narrow<T>(0);
-        }
+    for (int k = 0; k < kPacksPerThread; k++) {
+#pragma unroll
+        for (int i = 0; i < N; i++) value[k].v[i] = narrow<T>(0);
+        if (static_cast<uint32_t>(row[k]) < static_cast<uint64_t>(rows))
+            value[k] = *reinterpret_cast<const Pack<T, N>*>(W + row[k] * stride + static_cast<int64_t>(pack[k]) * N);
     }
 #pragma unroll
     for (int k = 0; k < kPacksPerThread; k++) {
         if (token[k] >= tokens) continue;
+        if (static_cast<uint32_t>(row[k]) >= static_cast<uint64_t>(rows) && pack[k] == 0) report_bad_index(st, 0);
 #pragma unroll
         for (int i = 0; i < N; i++) value[k].v[i] = narrow<T>(widen(value[k].v[i]) * scale);
-        *reinterpret_cast<Pack<T, N>*>(output + (token[k] * packs + pack[k]) * N) = value[k];
+        store_through(output + (token[k] * packs + pack[k]) * N, value[k]);
     }
 }
 
 // ------------------------------------------------------------------------------ gradient
 // Few tokens: one block sorts them, in shared memory, while the others clear the rows of grad_W that no token asks for, which takes
-// longer. Digits of eight bits, lowest first, every pass stable: a warp's keys in order, warps in order.
+// longer. Digits of up to nine bits (so that 2^18 rows take two passes of 13 us), lowest first, every pass stable: a warp's keys in order, warps in order.
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderItems = 16;
 constexpr int kFewTokens = kOrderThreads * kOrderItems;
 struct OrderMemory {
     int32_t keys[kFewTokens];
     uint16_t values[kFewTokens];
-    uint16_t counts[kOrderWarps][256]; // then: how many of a digit earlier warps have
-    int32_t of_warp[8], first[256];       // of each digit
+    uint16_t counts[kOrderWarps][kDigits]; // then: how many of a digit earlier warps have
+    int32_t of_warp[kDigits / 32], first[kDigits]; // of each digit
 };
 constexpr int kFlags = sizeof(OrderMemory); // rows that a block looks at together, a byte each
 
@@ -87,7 +96,7 @@ constexpr int kFlags = sizeof(OrderMemory); // rows that a block looks at togeth
 __device__ __forceinline__ unsigned lanes_with(int digit, bool in) {
     unsigned peers = __ballot_sync(kFullMask, in);
 #pragma unroll
-    for (int bit = 0; bit < 8; bit++) {
+    for (int bit = 0; bit < kDigitBits; bit++) {
         const unsigned set = __ballot_sync(kFullMask, digit >> bit & 1);
         peers &= digit >> bit & 1 ? set : ~set;
     }
@@ -95,7 +104,7 @@ __device__ __forceinline__ unsigned lanes_with(int digit, bool in) {
 }
 
 __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ sorted, int32_t* __restrict__ permutation,
-                                         const int32_t* __restrict__ indices, int tokens, int32_t rows, int32_t dropped, int passes, const Status& st) {
+                                         const int32_t* __restrict__ indices, int tokens, int32_t rows, int32_t dropped, int passes, int digit_bits, const Status& st) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rounds = (tokens + kOrderThreads - 1) / kOrderThreads, first = warp * rounds * 32 + lane;
     int32_t key[kOrderItems];
@@ -114,31 +123,44 @@ __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ s
         if (outside || key[r] == dropped) key[r] = rows;
     }
     if (bad && rows > 0) report_bad_index(st, 0);
+    const int mask = (1 << digit_bits) - 1;
     for (int pass = 0; pass < passes; pass++) {
-        const int shift = 8 * pass;
-        for (int i = tid; i < kOrderWarps * 256 / 2; i += kOrderThreads) reinterpret_cast<uint32_t*>(m.counts)[i] = 0;
+        const int shift = digit_bits * pass;
+        for (int i = tid; i < kOrderWarps * kDigits / 2; i += kOrderThreads) reinterpret_cast<uint32_t*>(m.counts)[i] = 0;
         __syncthreads();
         // each warp counts its digits
+        constexpr int kSide = 2; // side by side
 #pragma unroll
-        for (int r = 0; r < kOrderItems; r++) {
-            if (r >= rounds) break;
-            const bool in = first + r * 32 < tokens;
-            const int digit = key[r] >> shift & 255;
-            const unsigned peers = lanes_with(digit, in);
-            const int rank = __popc(peers & ((1u << lane) - 1));
-            if (in) value[r] |= static_cast<uint32_t>(m.counts[warp][digit] + rank) << 16;
-            __syncwarp();
-            if (in && rank == 0) m.counts[warp][digit] += __popc(peers);
-            __syncwarp();
+        for (int r0 = 0; r0 < kOrderItems; r0 += kSide) {
+            if (r0 >= rounds) break;
+            unsigned peers[kSide];
+#pragma unroll
+            for (int u = 0; u < kSide; u++) peers[u] = lanes_with(key[r0 + u] >> shift & mask, r0 + u < rounds && first + (r0 + u) * 32 < tokens);
+#pragma unroll
+            for (int u = 0; u < kSide; u++) {
+                const int r = r0 + u, digit = key[r] >> shift & mask;
+                const bool in = peers[u] >> lane & 1;
+                const int rank = __popc(peers[u] & ((1u << lane) - 1));
+                if (in) value[r] |= static_cast<uint32_t>(m.counts[warp][digit] + rank) << 16;
+                __syncwarp();
+                if (in && rank == 0) m.counts[warp][digit] += __popc(peers[u]);
+                __syncwarp();
+            }
         }
         __syncthreads();
         // where each warp's keys of a digit go: behind smaller digits, and behind earlier warps
         int total = 0, up_to = 0;
-        if (tid < 256) {
-            for (int w = 0; w < kOrderWarps; w++) {
-                const int n = m.counts[w][tid];
-                m.counts[w][tid] = static_cast<uint16_t>(total);
-                total += n;
+        if (tid < kDigits) {
+#pragma unroll
+            for (int w0 = 0; w0 < kOrderWarps; w0 += 16) {
+                int n[16];
+#pragma unroll
+                for (int w = 0; w < 16; w++) n[w] = m.counts[w0 + w][tid];
+#pragma unroll
+                for (int w = 0; w < 16; w++) {
+                    m.counts[w0 + w][tid] = static_cast<uint16_t>(total);
+                    total += n[w];
+                }
             }
             up_to = total;
 #pragma unroll
@@ -149,7 +171,7 @@ __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ s
             if (lane == 31) m.of_warp[warp] = up_to;
         }
         __syncthreads();
-        if (tid < 256) {
+        if (tid < kDigits) {
             int base = up_to - total;
             for (int w = 0; w < warp; w++) base += m.of_warp[w];
             m.first[tid] = base;
@@ -158,7 +180,7 @@ __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ s
 #pragma unroll
         for (int r = 0; r < kOrderItems; r++) {
             if (r >= rounds || first + r * 32 >= tokens) break;
-            const int digit = key[r] >> shift & 255;
+            const int digit = key[r] >> shift & mask;
             const int to = m.first[digit] + m.counts[warp][digit] + (value[r] >> 16);
             m.keys[to] = key[r];
             m.values[to] = static_cast<uint16_t>(value[r]);
@@ -198,7 +220,7 @@ __device__ __forceinline__ void clear_rows(unsigned char* flags, T* __restrict__
             const uint32_t all = static_cast<uint32_t>(min(group, here - r0)) * packs;
             for (uint32_t i = threadIdx.x; i < all; i += kOrderThreads) {
                 const uint32_t r = r0 + by_packs.divide(i), p = i - (r - r0) * packs;
-                if (!flags[r]) *reinterpret_cast<Pack<T, N>*>(grad_W + ((row0 + r) * packs + p) * N) = zero;
+                if (!flags[r]) store_through(grad_W + ((row0 + r) * packs + p) * N, zero);
             }
         }
     }
@@ -207,10 +229,10 @@ __device__ __forceinline__ void clear_rows(unsigned char* flags, T* __restrict__
 template <typename T, int N>
 __global__ void __launch_bounds__(kOrderThreads, 1)
 embedding_order(T* __restrict__ grad_W, int32_t* __restrict__ sorted, int32_t* __restrict__ permutation, const int32_t* __restrict__ indices,
-                int tokens, int32_t rows, int32_t dropped, int passes, uint32_t packs, Divider by_packs, Status st) {
+                int tokens, int32_t rows, int32_t dropped, int passes, int digit_bits, uint32_t packs, Divider by_packs, Status st) {
     extern __shared__ __align__(16) unsigned char memory[];
     if (blockIdx.x == 0) {
-        sort_few(*reinterpret_cast<OrderMemory*>(memory), sorted, permutation, indices, tokens, rows, dropped, passes, st);
+        sort_few(*reinterpret_cast<OrderMemory*>(memory), sorted, permutation, indices, tokens, rows, dropped, passes, digit_bits, st);
     } else {
         const int64_t blocks = gridDim.x - 1, b = blockIdx.x - 1;
         clear_rows<T, N>(memory, grad_W, indices, tokens, rows * b / blocks, rows * (b + 1) / blocks, dropped, packs, by_packs);
@@ -242,7 +264,7 @@ __device__ __forceinline__ void clear_some_rows(int64_t row0, T* __restrict__ gr
     for (int r = threadIdx.x / 32; r < here; r += kWarps) {
         if (!empty[r]) continue;
         for (uint32_t p = threadIdx.x % 32; p < packs; p += 32)
-            *reinterpret_cast<Pack<T, N>*>(grad_W + ((row0 + r) * packs + p) * N) = zero;
+            store_through(grad_W + ((row0 + r) * packs + p) * N, zero);
     }
 }
 
@@ -515,12 +537,13 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
             if (tokens <= kFewTokens) {
                 int bits = 1;
                 while ((int64_t(1) << bits) < rows + 1) bits++;
+                const int passes = (bits + kDigitBits - 1) / kDigitBits;
                 auto kernel = embedding_order<T, N>;
                 allow_dynamic_smem(kernel, call.device, sizeof(OrderMemory));
                 const int64_t blocks = std::min<int64_t>(ceil_div(rows * packs, 4 * kOrderThreads), sm_count(call.device) - 1);
                 kernel<<<grid_of(1 + blocks, op), kOrderThreads, sizeof(OrderMemory), call.stream>>>(
                     out, sorted, permutation, given, static_cast<int>(tokens), static_cast<int32_t>(rows), static_cast<int32_t>(padding_index),
-                    (bits + 7) / 8, static_cast<uint32_t>(packs), Divider(static_cast<uint32_t>(packs)), call.status);
+                    passes, (bits + passes - 1) / passes, static_cast<uint32_t>(packs), Divider(static_cast<uint32_t>(packs)), call.status);
                 note_kernel_f("embedding_order<%s,%d>", array_type_name<T>(), N);
                 clear_blocks = 0;
                 if (tokens == 0) return;
