@@ -31,7 +31,8 @@ struct Divider {
 
 // ------------------------------------------------------------------------------ forward
 // The output is cut into packs of N values, rows one after the other, and a block takes 1024 packs in a row; so blocks have the same
-// work whatever the width of a row, and a single token still uses many SMs.
+// work whatever the width of a row. Bounded by memory: 65 536 tokens of 2048 columns in bf16 take 66 us, in which 93 MB
+// are read and 268 MB written (5.4 TB/s); with a thread's loads one after the other and ordinary stores 95 us.
 constexpr int kPacksPerThread = 4;
 
 // Writes what this call does not read again: the line goes to memory before others do.
@@ -196,6 +197,8 @@ __device__ __forceinline__ void sort_few(OrderMemory& m, int32_t* __restrict__ s
     for (int i = tid; i < tokens; i += kOrderThreads) sorted[i] = m.keys[i], permutation[i] = m.values[i];
 }
 
+// (16 384 tokens among 100 003 rows of 1024 columns in bf16: 35 us. The sort's two passes take 34, bound by the instructions and shared-memory accesses of one SM; the
+// clearing of 170 MB, beside it, some 30.)
 // Clears the rows [lo, hi) that no token asks for. A block marks in shared memory which ones are, kFlags rows at a time.
 template <typename T, int N>
 __device__ __forceinline__ void clear_rows(unsigned char* flags, T* __restrict__ grad_W, const int32_t* __restrict__ indices, int tokens,
@@ -271,7 +274,7 @@ __device__ __forceinline__ void clear_some_rows(int64_t row0, T* __restrict__ gr
 // The sorted tokens are cut into chunks. A warp takes a chunk and a slab of 32 N columns and adds up the rows of grad_output, token
 // by token. A run of equal tokens that lies inside a chunk goes to its row of grad_W at once; of one
 // that a chunk's end cuts, each chunk leaves a partial sum (place 0: the run had begun before the chunk;
-// place 1: it begins in it and goes on after it), and embedding_join adds those up.
+// place 1: it begins in it and goes on after it), and embedding_join adds those up. Bounded by memory: 200 003 tokens of 256 columns in f32 43.5 us, 4.7 TB/s.
 // The first clear_blocks blocks clear rows instead.
 constexpr int kRowsInFlight = 8; // loads of a warp under way
 

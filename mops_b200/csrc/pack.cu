@@ -12,6 +12,8 @@ struct Jobs {
     Packing::Job job[Packing::kMost];
 };
 
+// Arrays whose rows begin anywhere, as a user's odd widths are, cannot be fetched by the copy engine; a copy of them costs less than tiles put together value by value
+// (3001 rows of 7 groups, 509 x 771 in bf16, forward and gradients: 200 us so, 89 with copies; the copies of A and W, 7 MB, take some 5 us of it).
 // A thread copies 16 bytes: from the two vectors that they lie in (16-bit values: they begin at any multiple of 2 bytes) where both are inside of the
 // array, else value by value.
 template <typename T>

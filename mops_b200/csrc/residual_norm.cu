@@ -26,7 +26,8 @@ namespace mops_b200 {
 namespace {
 
 // ---------------------------------------------------------------------------- rows of any length
-// A block takes a row after another and reads it as often as it needs it.
+// A block takes a row after another and reads it as often as it needs it. 500 rows of 100 000 columns in bf16: 880 us, backward 1.94 ms; bounded by the latency of
+// one load after the other.
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
@@ -158,7 +159,7 @@ residual_norm_vjp_plain(Gradients<T> g, Inputs<T> in) {
 // ---------------------------------------------------------------- rows that fit into registers
 // A team of threads (a warp, or a block) takes one row after another, each thread kPacks packs of N values: kPacks * N values of each
 // array. The next row's values are on their way while this one is worked on. Blocks stay for the whole call, so that scales and weights are read
-// once and the sums over rows stay in registers until the end.
+// once and the sums over rows stay in registers until the end. Where rows are not whole packs: 20 000 rows of 250 columns in f32 23.8 us (4.2 TB/s), backward 59 us.
 constexpr int kTeamThreads = 512; // at most (so a thread has 128 registers)
 // Values of a thread, in 16-byte packs or one by one: eight of them (f64: four), or twice as many for long rows.
 template <typename T> constexpr int kFewValues = sizeof(T) == 8 ? 4 : 8;
@@ -358,7 +359,8 @@ residual_norm_rows(T* __restrict__ stream, T* __restrict__ normed, const __grid_
 }
 
 // Rows that a block shares and whose packs are whole: the rows of the inputs come into shared memory by bulk copies, kRing rows ahead, which
-// leaves registers for two blocks on an SM: while one waits at a barrier the other works.
+// leaves registers for two blocks on an SM: while one waits at a barrier the other works. Bounded by memory: 16 384 rows of 4096 columns in bf16 take 110 to 119 us (670 MB, 5.6 to 6.1 TB/s),
+// backward 202 us (1.07 GB, 5.3 TB/s); 20 011 of 1000 in f32, a gate for each row, 55 and 83 us (5.8 and 6.1 TB/s). In registers alone the first took 287 and 438 us.
 template <typename T, int kInputs, int kRing> struct RowRing {
     unsigned char* places;
     uint64_t* full;
