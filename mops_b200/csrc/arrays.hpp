@@ -121,6 +121,26 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Pack {
 };
 template <typename T> constexpr int kPack = 16 / static_cast<int>(sizeof(T));
 
+// Writes what this call does not read again: the line goes to memory before others do.
+template <typename T, int N> __device__ __forceinline__ void store_through(T* to, const Pack<T, N>& v) {
+    if constexpr (N * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&v));
+    else *reinterpret_cast<Pack<T, N>*>(to) = v;
+}
+
+// x / d for x < 2^32, by a multiplication: d times the rounded-up quotient 2^(32 + s) / d exceeds 2^(32 + s) by less than 2^s
+// when 2^s >= d.
+struct Divider {
+    uint32_t d, shift;
+    uint64_t factor;
+    explicit Divider(uint32_t divisor) : d(divisor), shift(0) {
+        while ((uint64_t(1) << shift) < d) shift++;
+        factor = ((uint64_t(1) << (32 + shift)) + d - 1) / d;
+    }
+    __device__ __forceinline__ uint32_t divide(uint32_t x) const {
+        return static_cast<uint32_t>((__umul64hi(factor << (31 - shift), uint64_t(x) << 1)));
+    }
+};
+
 inline bool aligned16(const Array& a) {
     if (a.data == nullptr) return true;
     const int64_t bytes = type_bytes(a.type);

@@ -15,31 +15,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// x / d for x < 2^32, by a multiplication: d times the rounded-up quotient 2^(32 + s) / d exceeds 2^(32 + s) by less than 2^s
-// when 2^s >= d.
-struct Divider {
-    uint32_t d, shift;
-    uint64_t factor;
-    explicit Divider(uint32_t divisor) : d(divisor), shift(0) {
-        while ((uint64_t(1) << shift) < d) shift++;
-        factor = ((uint64_t(1) << (32 + shift)) + d - 1) / d;
-    }
-    __device__ __forceinline__ uint32_t divide(uint32_t x) const {
-        return static_cast<uint32_t>((__umul64hi(factor << (31 - shift), uint64_t(x) << 1)));
-    }
-};
-
 // ------------------------------------------------------------------------------ forward
 // The output is cut into packs of N values, rows one after the other, and a block takes 1024 packs in a row; so blocks have the same
 // work whatever the width of a row. Bounded by memory: 65 536 tokens of 2048 columns in bf16 take 66 us, in which 93 MB
 // are read and 268 MB written (5.4 TB/s); with a thread's loads one after the other and ordinary stores 95 us.
 constexpr int kPacksPerThread = 4;
-
-// Writes what this call does not read again: the line goes to memory before others do.
-template <typename T, int N> __device__ __forceinline__ void store_through(T* to, const Pack<T, N>& v) {
-    if constexpr (N * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&v));
-    else *reinterpret_cast<Pack<T, N>*>(to) = v;
-}
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)

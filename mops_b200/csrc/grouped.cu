@@ -143,7 +143,7 @@ void multiply_outer(const Call& call, const OuterProblem& p, const std::string& 
     const Array &out = p.out, &X = p.X, &Y = p.Y;
     const int32_t* offsets = p.offsets;
     const int64_t groups = p.groups, rows = X.shape[0], height = X.shape[1], columns = Y.shape[1];
-    if (groups == 0 || height == 0 || columns == 0 || multiply_outer_mma(call, p, op) ||
+    if (groups == 0 || height == 0 || columns == 0 || multiply_outer_few(call, p, op) || multiply_outer_mma(call, p, op) ||
         multiply_outer_split(call, p, op))
         return;
     fits_int32(static_cast<size_t>(groups), "the number of groups", op);
@@ -197,7 +197,7 @@ void grouped_matrix_product(Array output, Array A, Array W, Array offsets) {
     if (output.shape[0] == 0 || output.shape[1] == 0) return;
     Call call = begin_call();
     Packing packing(call);
-    if (on_tensor_cores(A, W)) {
+    if (on_tensor_cores(A, W) && !straight_rows(W, A.shape[0], W.stride[2] == 1)) {
         packing.add(A);
         packing.add(W);
         packing.run();
@@ -233,9 +233,11 @@ void grouped_matrix_product_vjp(Array grad_A, Array grad_W, Array grad_output, A
     Call call = begin_call();
     Packing packing(call);
     if (on_tensor_cores(A, W)) {
-        packing.add(grad_output);
-        if (need_A) packing.add(W);
-        if (need_W) packing.add(A);
+        const bool rows_packed = need_A && !straight_rows(W, A.shape[0], W.stride[1] == 1);
+        const bool outer_packed = need_W && !straight_outer(A.shape[0], W.shape[0], W.shape[1], W.shape[2], A.type);
+        if (rows_packed || outer_packed) packing.add(grad_output);
+        if (rows_packed) packing.add(W);
+        if (outer_packed) packing.add(A);
         packing.run();
     }
     const int32_t* starts = static_cast<const int32_t*>(offsets.data);

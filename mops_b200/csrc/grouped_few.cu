@@ -7,7 +7,7 @@
 // 16 bits: the tensor cores with the operands the other way round. The matrix gives the 128 rows of the accumulator, the rows of X its 16 or 64 columns, so that
 // little is fetched besides the matrix. In bf16, 16 rows of 32 groups, 2048 x 1536 (12 of them used, 75 MB): 16.3 us, 4.6 TB/s, which is bounded by how fast the copies of a block
 // that has just begun get under way; tiles of 128 rows, whose blocks fetch as much of X as of the matrices, 23.0 us. Two rows of 16 groups, 4096 x 1024: 8.4 and 25.7 us.
-// f32 and f64: the ordinary units, straight from the loads. In f32 the first of them takes 43 us (3.5 TB/s; tiles of 128 rows 61), eight rows of 8 groups, 128 x 128, 4.6 (9.0); bounded
+// f32, f64 and matrices whose rows begin anywhere: the ordinary units, straight from the loads. In f32 the first of them takes 43 us (3.5 TB/s; tiles of 128 rows 61), eight rows of 8 groups, 128 x 128, 4.6 (9.0); bounded
 // by the loads that a block's registers can hold.
 #include <cooperative_groups.h>
 
@@ -190,7 +190,8 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kRows = 4;         // of a block
 constexpr int kMostRows = 64;    // of a call
 constexpr int kChunk = 1024;     // values of depth of the rows that are in shared memory at a time
-constexpr int kInFlight = 8;     // loads of a thread
+// (loads of a thread under way: 128 bytes where they are whole packs)
+template <typename T, int N> constexpr int kInFlight = N > 1 ? 8 : 16;
 
 template <typename T> struct Few {
     T* out;
@@ -220,12 +221,13 @@ __device__ __forceinline__ void join_parts(Sum<T>* part, const Few<T>& p, int64_
     if (parts > 1) cluster.sync(); // (nobody leaves while others read its sums)
 }
 
-// Columns that are neighbours in memory (depth x columns). Sixteen threads side by side take a pack of columns each, sixteen such rows of threads every sixteenth value of depth.
-template <typename T>
+// Columns that are neighbours in memory (depth x columns). kAcross threads side by side take a pack of N columns each, the rows of such threads every kDown-th value of depth.
+template <int N> constexpr int kAcross = N > 1 ? 16 : 64;
+template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
 few_rows_columns(const __grid_constant__ Few<T> p, Status st) {
     using S = Sum<T>;
-    constexpr int N = kPack<T>, kAcross = 16, kDown = kThreads / kAcross, kColumns = kAcross * N;
+    constexpr int kAcross = mops_b200::kAcross<N>, kInFlight = mops_b200::kInFlight<T, N>, kDown = kThreads / kAcross, kColumns = kAcross * N;
     __shared__ S x[kRows][kChunk];
     __shared__ S sums[kDown][kRows * kColumns / 4]; // a quarter of the columns at a time
     __shared__ S part[kRows * kColumns];
@@ -281,11 +283,11 @@ few_rows_columns(const __grid_constant__ Few<T> p, Status st) {
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         __syncthreads();
-        if (across / 4 == q) {
+        if (across / (kAcross / 4) == q) {
 #pragma unroll
             for (int r = 0; r < kRows; r++)
 #pragma unroll
-                for (int i = 0; i < N; i++) sums[down][r * (kColumns / 4) + across % 4 * N + i] = sum[r][i];
+                for (int i = 0; i < N; i++) sums[down][r * (kColumns / 4) + across % (kAcross / 4) * N + i] = sum[r][i];
         }
         __syncthreads();
         for (int i = threadIdx.x; i < kRows * kColumns / 4; i += kThreads) {
@@ -298,12 +300,12 @@ few_rows_columns(const __grid_constant__ Few<T> p, Status st) {
     join_parts<T, kColumns>(part, p, row, here, column);
 }
 
-// Depth that is neighbours in memory (columns x depth). A warp takes four columns, its lanes packs of the depth.
-template <typename T>
+// Depth that is neighbours in memory (columns x depth). A warp takes four columns, its lanes packs of N values of the depth.
+template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
 few_rows_depth(const __grid_constant__ Few<T> p, Status st) {
     using S = Sum<T>;
-    constexpr int N = kPack<T>, kOwn = 4, kColumns = kWarps * kOwn;
+    constexpr int kOwn = 4, kColumns = kWarps * kOwn, kInFlight = 4 * mops_b200::kInFlight<T, N> / (N > 1 ? 4 : 2);
     __shared__ alignas(16) T x[kRows][kChunk];
     __shared__ S part[kRows * kColumns];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -369,7 +371,84 @@ few_rows_depth(const __grid_constant__ Few<T> p, Status st) {
     join_parts<T, kColumns>(part, p, row, here, column);
 }
 
+// ------------------------------------------------------------------- outer products of few rows
+// out[g] = X[rows of g]^T Y[rows of g], of which most are zero or the product of one or two rows: what counts is to write them. A thread has 16 bytes of the output at a time,
+// wherever matrices and their rows begin, and adds up the products of its group's rows in f32 (f64), read through the L1, value by value, which bounds it. 16 rows of 56 groups,
+// 1195 x 33 in bf16 (4.4 MB): 7 us, tiles on the tensor cores 25 and a copy of the operands. Large matrices are better off there (18 rows of 13 groups, 1754 x 2693, 123 MB: 71 us, here 89).
+constexpr int kOuterTurns = 2;
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+few_outer(T* __restrict__ out, const T* __restrict__ X, int64_t x_stride, const T* __restrict__ Y, int64_t y_stride, const int32_t* __restrict__ offsets,
+          int64_t groups, int64_t rows, uint32_t columns, Divider by_columns, uint32_t values, Status st) {
+    using S = Sum<T>;
+    constexpr int N = kPack<T>;
+    if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(offsets, groups, rows, st);
+    int64_t lo, hi;
+    group_bounds(offsets, groups, rows, blockIdx.y, lo, hi);
+    out += static_cast<int64_t>(blockIdx.y) * values; // the group's matrix
+    // how far it begins behind a multiple of 16 bytes
+    const uint32_t head = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T));
+    uint32_t at = (blockIdx.x * (kThreads * kOuterTurns) + threadIdx.x) * N; // counted from there
+    for (int turn = 0; turn < kOuterTurns; turn++, at += kThreads * N) {
+        if (at >= values + head) break;
+        if (at >= head && at + N <= values + head) {
+            const uint32_t v = at - head;
+            uint32_t j;
+            S sum[N];
+#pragma unroll
+            for (int u = 0; u < N; u++) sum[u] = 0;
+            if (lo < hi) {
+                const uint32_t i = by_columns.divide(v);
+                j = v - i * columns;
+                for (int64_t r = lo; r < hi; r++) {
+                    const T *x = X + r * x_stride + i, *y = Y + r * y_stride;
+                    S factor = widen(*x);
+                    uint32_t c = j;
+#pragma unroll
+                    for (int u = 0; u < N; u++) {
+                        sum[u] += factor * widen(y[c]);
+                        if (++c == columns) {
+                            c = 0;
+                            if (u + 1 < N) factor = widen(*++x);
+                        }
+                    }
+                }
+            }
+            Pack<T, N> result;
+#pragma unroll
+            for (int u = 0; u < N; u++) result.v[u] = narrow<T>(sum[u]);
+            store_through(out + v, result);
+        } else { // the matrix begins or ends in here
+            for (uint32_t a = max(at, head); a < min(at + N, values + head); a++) {
+                const uint32_t i = by_columns.divide(a - head), j = a - head - i * columns;
+                S sum = 0;
+                for (int64_t r = lo; r < hi; r++) sum += widen(X[r * x_stride + i]) * widen(Y[r * y_stride + j]);
+                out[a - head] = narrow<T>(sum);
+            }
+        }
+    }
+}
+
 } // namespace
+
+bool straight_rows(const Array& M, int64_t rows, bool by_columns) {
+    const int64_t groups = M.shape[0], bytes = type_bytes(M.type);
+    if (rows > kMostRows / (bytes == 2 ? 2 : 1)) return false;
+    // Where many rows share matrices the tiles of 128 rows read them once for all; those of f32 take long for few rows, and the next four find the matrix in L2 (32 rows of a
+    // group, 1024 x 1024: 22 us so, 30 in tiles; 4096 x 4096: 147 and 113, 8 rows 45 and 113).
+    if (rows > kRows * groups && !(bytes == 4 && (rows <= 16 || (rows <= 32 && M.shape[1] * M.shape[2] <= 1 << 23)))) return false;
+    if (bytes != 2) return true;
+    // 16 bits: only what the copy engine cannot fetch.
+    const int inner = M.stride[2] == 1 ? 2 : 1, outer = 3 - inner;
+    if (boxable(M.type, M.data, M.shape[inner], M.shape[outer], groups, M.stride[outer], M.stride[0])) return false;
+    // Columns one by one come at 1.3 TB/s, and copies, of all matrices, with the tensor cores behind them, at 1.5 (13 matrices of 1754 x 2693, all used: 120 and 84 us); with the depth along
+    // rows it is 2 TB/s. So copies it is for large matrices by columns of which most are used.
+    return !by_columns || std::min(rows, groups) * 3 <= groups * 2 || groups * M.shape[1] * M.shape[2] * bytes <= 16 << 20;
+}
+
+bool straight_outer(int64_t rows, int64_t groups, int64_t height, int64_t columns, int32_t type) {
+    return rows <= 64 && rows <= 2 * groups && groups <= 65535 && groups * height * columns * type_bytes(type) <= 16 << 20;
+}
 
 bool multiply_rows_few(const Call& call, const RowsProblem& p, const std::string& op) {
     if (p.depth == 0 || p.groups == 0) return false;
@@ -377,6 +456,28 @@ bool multiply_rows_few(const Call& call, const RowsProblem& p, const std::string
     const int64_t stride = mn ? p.depth_stride : p.column_stride;
     const int64_t inner = mn ? p.columns : p.depth, outer = mn ? p.depth : p.columns;
     const int64_t sms = sm_count(call.device);
+    if (straight_rows(p.M, p.rows, mn)) {
+        for_type(p.X.type, [&](auto zero) {
+            using T = decltype(zero);
+            auto launch = [&](auto width) {
+                constexpr int N = decltype(width)::value;
+                const int64_t across = ceil_div(p.columns, mn ? kAcross<N> * N : kWarps * 4), pieces = std::min<int64_t>(p.rows, p.groups + p.rows / kRows);
+                const int parts = parts_of_depth(across * pieces, sms * 4, p.depth, 128);
+                const Few<T> few{static_cast<T*>(p.out.data), static_cast<const T*>(p.X.data), static_cast<const T*>(p.M.data), p.X.stride[0], p.M.stride[0],
+                                 stride, p.offsets, p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns)};
+                Clusters clusters(call, op, across, parts, pieces, kThreads, 0);
+                MOPS_CUDA_OK(cudaLaunchKernelEx(&clusters.config, mn ? few_rows_columns<T, N> : few_rows_depth<T, N>, few, call.status));
+                note_kernel_f("few_rows_%s<%s,%d>, %d parts", mn ? "columns" : "depth", array_type_name<T>(), N, parts);
+            };
+            if constexpr (sizeof(T) > 2)
+                if (inner % kPack<T> == 0 && boxable(p.X.type, p.M.data, inner, outer, p.groups, stride, p.M.stride[0])) {
+                    launch(std::integral_constant<int, kPack<T>>());
+                    return;
+                }
+            launch(std::integral_constant<int, 1>());
+        });
+        return true;
+    }
     if (p.X.type == MOPS_B200_F16 || p.X.type == MOPS_B200_BF16) {
         // Up to 32 rows the accumulators have 16 columns, up to 128 of deep matrices 64 (64 rows of 32 groups, 2048 x 1536: 29.5 us, with 16 columns 36.8). More rows, and
         // shallow matrices, are left to the tiles of 128 rows (200 rows of 8 groups, 2048 x 1536: 18.5 us here, 17.1 there; 48 of 2, 1024 x 1024: 11.7 and 9.8).
@@ -410,22 +511,22 @@ bool multiply_rows_few(const Call& call, const RowsProblem& p, const std::string
         else by_major(__half());
         return true;
     }
-    // Where many rows share matrices the tiles of 128 rows read them once for all.
-    if (p.rows > kMostRows || p.rows > kRows * p.groups || inner % (16 / type_bytes(p.X.type)) != 0 ||
-        !boxable(p.X.type, p.M.data, inner, outer, p.groups, stride, p.M.stride[0]))
-        return false;
-    auto launch = [&](auto zero) {
+    return false;
+}
+
+bool multiply_outer_few(const Call& call, const OuterProblem& p, const std::string& op) {
+    const int64_t rows = p.X.shape[0], height = p.X.shape[1], columns = p.Y.shape[1];
+    if (!straight_outer(rows, p.groups, height, columns, p.X.type)) return false;
+    for_type(p.X.type, [&](auto zero) {
         using T = decltype(zero);
-        const int64_t across = ceil_div(p.columns, mn ? 16 * kPack<T> : kWarps * 4), pieces = std::min<int64_t>(p.rows, p.groups + p.rows / kRows);
-        const int parts = parts_of_depth(across * pieces, sms * 4, p.depth, 128);
-        const Few<T> few{static_cast<T*>(p.out.data), static_cast<const T*>(p.X.data), static_cast<const T*>(p.M.data), p.X.stride[0], p.M.stride[0],
-                         stride, p.offsets, p.groups, p.rows, static_cast<int>(p.depth), static_cast<int>(p.columns)};
-        Clusters clusters(call, op, across, parts, pieces, kThreads, 0);
-        MOPS_CUDA_OK(cudaLaunchKernelEx(&clusters.config, mn ? few_rows_columns<T> : few_rows_depth<T>, few, call.status));
-        note_kernel_f("few_rows_%s<%s>, %d parts", mn ? "columns" : "depth", array_type_name<T>(), parts);
-    };
-    if (p.X.type == MOPS_B200_F32) launch(float());
-    else launch(double());
+        const int64_t values = height * columns;
+        few_outer<T><<<dim3(static_cast<unsigned>(ceil_div(values + kPack<T>, int64_t(kThreads) * kOuterTurns * kPack<T>)), static_cast<unsigned>(p.groups)), kThreads, 0,
+                       call.stream>>>(static_cast<T*>(p.out.data), static_cast<const T*>(p.X.data), p.X.stride[0], static_cast<const T*>(p.Y.data), p.Y.stride[0],
+                                      p.offsets, p.groups, rows, static_cast<uint32_t>(columns), Divider(static_cast<uint32_t>(columns)),
+                                      static_cast<uint32_t>(values), call.status);
+        note_kernel_f("few_outer<%s>", array_type_name<T>());
+    });
+    MOPS_CUDA_OK(cudaGetLastError());
     return true;
 }
 

@@ -23,6 +23,11 @@ struct OuterProblem {
 
 // A few rows in all, as single tokens are (grouped_few.cu): false if there are too many.
 bool multiply_rows_few(const Call& call, const RowsProblem& p, const std::string& op);
+bool multiply_outer_few(const Call& call, const OuterProblem& p, const std::string& op);
+// Whether they take the arrays as they are, wherever rows begin: products of `rows` rows with the matrices M (by_columns: whose columns, not
+// whose depth, are neighbours in memory), and outer products of height x columns.
+bool straight_rows(const Array& M, int64_t rows, bool by_columns);
+bool straight_outer(int64_t rows, int64_t groups, int64_t height, int64_t columns, int32_t type);
 
 // On arrays that the copy engine can fetch (pack.hpp); f16 and bf16 in grouped_mma.cu, f32 in grouped_split.cu. false: not taken on
 // (another type, or nothing to multiply).

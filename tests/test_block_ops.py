@@ -315,6 +315,42 @@ def test_grouped_few_rows(dtype, other_way, before, rows, after, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("before,rows,K,N", [
+    (0, [1] * 13 + [0] * 7 + [5], 175, 269), (2, [0, 3, 0, 0, 1], 1, 1), (0, [1, 2, 0, 1], 3, 5), (0, [2] * 30, 1001, 7), (1, [0, 0, 1, 0, 31] + [0] * 20, 67, 2051),
+    (0, [0, 40] + [0] * 20, 130, 3)])
+def test_grouped_few_rows_of_odd_matrices(dtype, before, rows, K, N):
+    """Matrices whose rows begin anywhere are read as they are, and most of the gradients of matrices are zero."""
+    R = before + sum(rows)
+    check_grouped(normal((R, K), dtype, 1), normal((len(rows), K, N), dtype, 2, K ** -0.5), offsets_of(rows) + before, normal((R, N), dtype, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(5, 3), (24, 40), (129, 67)])
+@pytest.mark.parametrize("shift", [1, 3, 5])
+def test_grouped_few_rows_outputs_begin_anywhere(dtype, K, N, shift):
+    from mops_b200 import _lib
+    rows = [1, 0, 3, 0, 0, 2]
+    G, R = len(rows), sum(rows)
+    A, W, offsets, grad = normal((R, K), dtype, 1), normal((G, K, N), dtype, 2, K ** -0.5), offsets_of(rows), normal((R, N), dtype, 3)
+    room = torch.full((G * K * N + R * K + R * N + 64,), 7.0, dtype=dtype, device="cuda")
+    views, at = [], shift
+    for shape in ((R, N), (R, K), (G, K, N)):
+        views.append(room[at:at + int(np.prod(shape))].view(shape))
+        at += int(np.prod(shape))
+    array = lambda t: _lib.make_array(t.data_ptr(), str(t.dtype).split(".")[1], tuple(t.shape), t.stride())
+    torch.cuda.synchronize()
+    _lib.call("mops_b200_cuda_grouped_matrix_product", [array(t) for t in (views[0], A, W, offsets)])
+    _lib.call("mops_b200_cuda_grouped_matrix_product_vjp", [array(t) for t in (views[1], views[2], grad, A, W, offsets)])
+    want = grouped_plain(A, W, offsets, grad)
+    terms = grouped_plain(A.abs(), W.abs(), offsets, grad.abs())
+    for g, w, t, n, what in zip(views, want, terms, (K, N, 3), ("output", "grad_A", "grad_W")):
+        close(g, w, t, n, what)
+    assert (room[:shift] == 7).all() and (room[at:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("K,N", [(64, 128), (72, 40), (33, 65)])
 def test_grouped_matrices_stored_the_other_way(dtype, K, N):
     rows = [100, 0, 37, 260]
