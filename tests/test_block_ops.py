@@ -180,6 +180,28 @@ def test_embedding_matches_64_bits(dtype, tokens, rows, columns, padding):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,rows,columns", [(3, 40, 1), (0, 33, 7), (50, 5000, 3), (20, 300, 1586), (700, 90000, 5), (17000, 70001, 3), (17001, 300, 33),
+                                                 (16500, 90000, 8)])
+@pytest.mark.parametrize("shift", [0, 1, 5])
+def test_embedding_gradient_clears_every_row_wherever_it_begins(dtype, tokens, rows, columns, shift):
+    import ctypes
+    from mops_b200 import _lib
+    gen = torch.Generator(device="cuda").manual_seed(rows + columns)
+    indices = torch.randint(rows, (tokens,), generator=gen, device="cuda", dtype=torch.int32)
+    grad = normal((tokens, columns), dtype, 2)
+    room = torch.full((rows * columns + 16,), 7.0, dtype=dtype, device="cuda")
+    got = room[shift:shift + rows * columns].view(rows, columns)
+    array = lambda t: _lib.make_array(t.data_ptr(), str(t.dtype).split(".")[1], tuple(t.shape), t.stride())
+    torch.cuda.synchronize()
+    _lib.call("mops_b200_cuda_embedding_lookup_vjp", [array(got), array(grad), array(indices), ctypes.c_double(1.0), ctypes.c_int64(-1)])
+    sums = torch.zeros(rows, columns, dtype=torch.float64, device="cuda").index_add_(0, indices.long(), grad.double())
+    absolute = torch.zeros_like(sums).index_add_(0, indices.long(), grad.double().abs())
+    close(got, sums, absolute, max(int(torch.bincount(indices, minlength=1).max()), 1), "grad_W")
+    assert (room[:shift] == 7).all() and (room[shift + rows * columns:] == 7).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_embedding_on_strided_and_shifted_tensors(dtype):
     base = normal((50, 80), dtype, 3)
