@@ -286,8 +286,9 @@ class _Arena:
         else:
             self.device = first.device
             self.host = False
-        taken = (torch.float32, torch.float64) + ((torch.float16, torch.bfloat16) if half else ())
-        self.dtype = {_dtype_name(torch.empty(0, dtype=t)): t for t in taken}.get(_dtype_name(first))
+        name = _dtype_name(first)
+        taken = ("float32", "float64", "float16", "bfloat16") if half else ("float32", "float64")
+        self.dtype = getattr(torch, name) if name in taken else None
         if self.dtype is None:
             raise TypeError("Unsupported dtype detected. Only float32" + (
                 ", float64, float16 and bfloat16" if half else " and float64") + " are supported")
