@@ -141,13 +141,15 @@ struct Divider {
     }
 };
 
-inline bool aligned16(const Array& a) {
+// Whether rows begin on multiples of so many bytes and are made of them.
+inline bool aligned(const Array& a, int64_t to) {
     if (a.data == nullptr) return true;
     const int64_t bytes = type_bytes(a.type);
-    bool ok = reinterpret_cast<uintptr_t>(a.data) % 16 == 0 && a.shape[a.dimensions - 1] * bytes % 16 == 0;
-    for (int d = 0; d + 1 < a.dimensions; d++) ok = ok && a.stride[d] * bytes % 16 == 0;
+    bool ok = reinterpret_cast<uintptr_t>(a.data) % to == 0 && a.shape[a.dimensions - 1] * bytes % to == 0;
+    for (int d = 0; d + 1 < a.dimensions; d++) ok = ok && a.stride[d] * bytes % to == 0;
     return ok;
 }
+inline bool aligned16(const Array& a) { return aligned(a, 16); }
 
 template <typename T> inline const char* array_type_name() {
     return std::is_same<T, float>::value    ? "f32"

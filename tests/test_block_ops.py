@@ -181,6 +181,19 @@ def test_embedding_matches_64_bits(dtype, tokens, rows, columns, padding):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("columns", [2, 6, 12, 20, 34, 258])
+def test_embedding_rows_of_8_and_4_bytes(dtype, columns):
+    W, grad = normal((61, columns), dtype, 1).requires_grad_(True), normal((700, columns), dtype, 2)
+    indices = (torch.arange(700, device="cuda", dtype=torch.int32) * 7) % 53
+    output = mt.embedding_lookup(W, indices, 1.75)
+    got, = torch.autograd.grad(output, [W], grad)
+    want, sums, absolute, n = embedding_plain(W.detach(), indices, 1.75, grad, -1)
+    close(output.detach(), want, want.abs(), 1, "output")
+    close(got, sums, absolute, n, "grad_W")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tokens,rows,columns", [(3, 40, 1), (0, 33, 7), (50, 5000, 3), (20, 300, 1586), (700, 90000, 5), (17000, 70001, 3), (17001, 300, 33),
                                                  (16500, 90000, 8)])
 @pytest.mark.parametrize("shift", [0, 1, 5])
