@@ -6,6 +6,7 @@
 #define MOPS_B200_GROUP_TILES_CUH
 
 #include "device.cuh"
+#include "group_ranges.hpp"
 
 namespace mops_b200 {
 
@@ -13,9 +14,8 @@ namespace mops_b200 {
 // first group; g == groups: those behind the last one.
 __device__ __forceinline__ void group_bounds(const int32_t* __restrict__ offsets, int64_t groups, int64_t rows,
                                              int64_t g, int64_t& lo, int64_t& hi) {
-    lo = g < 0 ? 0 : min(max(int64_t(__ldg(offsets + g)), int64_t(0)), rows);
-    hi = g >= groups ? rows : min(max(int64_t(__ldg(offsets + g + 1)), int64_t(0)), rows);
-    hi = max(lo, hi);
+    const RowRange r = rows_between(g < 0 ? 0 : int64_t(__ldg(offsets + g)), g >= groups ? rows : int64_t(__ldg(offsets + g + 1)), rows);
+    lo = r.lo, hi = r.hi;
 }
 
 // The rows [lo, hi) of a group and which of its pieces is meant; found == false: there is no such piece.

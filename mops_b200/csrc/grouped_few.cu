@@ -31,11 +31,9 @@ struct FewRows { // pieces: up to `most` rows of a group
 // The rows of no group: zeros in kColumns columns.
 template <typename T, int kColumns, int kThreads>
 __device__ __forceinline__ void clear_others(T* __restrict__ out, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int column, int columns) {
-    int64_t lo, hi, ignored;
-    group_bounds(offsets, groups, rows, -1, ignored, lo);
-    group_bounds(offsets, groups, rows, groups, hi, ignored);
-    for (int64_t r = lo > 0 ? 0 : hi; r < rows; r = r + 1 == lo ? hi : r + 1)
+    for_rows_of_no_group(__ldg(offsets), __ldg(offsets + groups), rows, [&](int64_t r) {
         for (int c = threadIdx.x; c < kColumns && column + c < columns; c += kThreads) out[r * columns + column + c] = T(0);
+    });
 }
 
 // How many parts the depth is cut into: until there are `enough` blocks, of `least` values of depth at least.
