@@ -33,8 +33,20 @@ constexpr int kWarps = kThreads / 32;
 
 enum Gate : int { kNoGate = 0, kRowGate = 1, kFullGate = 2 };
 
-template <typename S> __device__ __forceinline__ S sigmoid(S v) { return S(1) / (S(1) + exp(-v)); }
-template <> __device__ __forceinline__ float sigmoid<float>(float v) { return 1.0f / (1.0f + expf(-v)); }
+__device__ __forceinline__ float exponential(float v) { return expf(v); }
+__device__ __forceinline__ double exponential(double v) { return exp(v); }
+
+// z = sigmoid(v) = 1 / (1 + e) with e = exp(-v), and 1 - z as e z: 1 - z itself would be what z was rounded by for large v (in f32 nothing is left of it from v = 17 on).
+// Where e is infinite z is 0, and so is everything that 1 - z is multiplied with.
+__device__ __forceinline__ float complement(float e, float z) { return fminf(e, 3.402823466e38f) * z; }
+__device__ __forceinline__ double complement(double e, double z) {
+    return __hiloint2double(min(__double2hiint(e), 0x7fefffff), __double2loint(e)) * z; // (the largest finite power of e: e is not negative)
+}
+template <typename S> __device__ __forceinline__ S sigmoid(S v, S& one_minus) {
+    const S e = exponential(-v), z = S(1) / (S(1) + e);
+    one_minus = complement(e, z);
+    return z;
+}
 template <typename S> __device__ __forceinline__ S inverse_root(S v) { return S(1) / sqrt(v); }
 template <> __device__ __forceinline__ float inverse_root<float>(float v) { return rsqrtf(v); }
 
@@ -62,9 +74,13 @@ template <typename T> struct Inputs {
     double epsilon;
 };
 
+template <typename T, int GATE> __device__ __forceinline__ Sum<T> gate_of(const Inputs<T>& in, int64_t row, int64_t c, Sum<T>& one_minus) {
+    if constexpr (GATE == kNoGate) return one_minus = 0, Sum<T>(1);
+    else return sigmoid<Sum<T>>(widen(in.gate[row * in.gate_stride + (GATE == kFullGate ? c : 0)]), one_minus);
+}
 template <typename T, int GATE> __device__ __forceinline__ Sum<T> gate_of(const Inputs<T>& in, int64_t row, int64_t c) {
-    if constexpr (GATE == kNoGate) return 1;
-    else return sigmoid<Sum<T>>(widen(in.gate[row * in.gate_stride + (GATE == kFullGate ? c : 0)]));
+    Sum<T> one_minus;
+    return gate_of<T, GATE>(in, row, c, one_minus);
 }
 
 template <typename T, int GATE>
@@ -133,13 +149,14 @@ residual_norm_vjp_plain(Gradients<T> g, Inputs<T> in) {
         auto ds_of = [&](int64_t c, S y) { return widen(gs[c]) + r * widen(in.weight_output[c]) * widen(gh[c]) - y * back; };
         sum[0] = sum[1] = 0;
         for (int64_t c = threadIdx.x; c < in.columns; c += kThreads) {
-            const S z = gate_of<T, GATE>(in, row, c), y = stream(c, z), ds = ds_of(c, y), n = widen(b[c]) * q;
+            S one_minus;
+            const S z = gate_of<T, GATE>(in, row, c, one_minus), y = stream(c, z), ds = ds_of(c, y), n = widen(b[c]) * q;
             const S full = ds * widen(in.scale[c]) * widen(in.weight_branch[c]) * n;
             sum[0] += full * z;
             if (g.residual != nullptr) g.residual[row * in.columns + c] = narrow<T>(ds);
             if constexpr (GATE == kFullGate)
-                if (g.gate != nullptr) g.gate[row * in.columns + c] = narrow<T>(full * z * (1 - z));
-            if constexpr (GATE == kRowGate) sum[1] += full * z * (1 - z);
+                if (g.gate != nullptr) g.gate[row * in.columns + c] = narrow<T>(full * z * one_minus);
+            if constexpr (GATE == kRowGate) sum[1] += full * z * one_minus;
             own[c] += ds * z * n;
             own[in.columns + c] += widen(gh[c]) * y * r;
         }
@@ -231,24 +248,37 @@ template <typename T, int N, int kPacks> struct alignas(16) Values {
             if (k * team + member < packs)
                 *reinterpret_cast<Pack<T, N>*>(first + k * team * N) = *reinterpret_cast<const Pack<T, N>*>(&v[k * N]);
     }
+    // What is computed from the values behind this is computed anew, not kept from before.
+    __device__ __forceinline__ void forget() {
+        uint32_t* w = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(N * kPacks * sizeof(T) / 4); i++) asm volatile("" : "+r"(w[i]));
+    }
     __device__ __forceinline__ Pair<Sum<T>> operator[](int i) const { return widen2(&v[2 * i]); }
     __device__ __forceinline__ void set(int i, Pair<Sum<T>> value) { narrow2(&v[2 * i], value); }
 };
 
-// sigmoid(v). In f32 and f64 with the functions of the mathematical library; of 16-bit gates, whose results are rounded to as many bits, by
-// the approximate instructions (2^v within 2 units of the 22nd bit, 1 / v within 1 of the 23rd).
-template <typename T> __device__ __forceinline__ Pair<Sum<T>> gates(Pair<Sum<T>> v) {
+// sigmoid(v), and 1 - sigmoid(v). In f32 and f64 with the functions of the mathematical library; of 16-bit gates, whose results are rounded to as many bits, by
+// the approximate instructions (2^v within 2 units of the 22nd bit, 1 / v within 1 of the 23rd), so that e^-v is off by some 2^-21 + |v| 2^-23 of itself, and 1 - sigmoid(v), which is made
+// without a difference that cancels, as well.
+template <typename T> __device__ __forceinline__ Pair<Sum<T>> gates(Pair<Sum<T>> v, Pair<Sum<T>>& one_minus) {
     if constexpr (sizeof(T) == 2) {
-        Pair<float> e = v * -1.44269504f;
+        Pair<float> e = v * -1.44269504f, z;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
-        e = e + both(1.0f);
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
-        return e;
+        z = e + both(1.0f);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(z.x) : "f"(z.x));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(z.y) : "f"(z.y));
+        one_minus = Pair<float>{fminf(e.x, 3.402823466e38f), fminf(e.y, 3.402823466e38f)} * z;
+        return z;
     } else {
-        return {sigmoid<Sum<T>>(v.x), sigmoid<Sum<T>>(v.y)};
+        const Sum<T> x = sigmoid<Sum<T>>(v.x, one_minus.x);
+        return {x, sigmoid<Sum<T>>(v.y, one_minus.y)};
     }
+}
+template <typename T> __device__ __forceinline__ Pair<Sum<T>> gates(Pair<Sum<T>> v) {
+    Pair<Sum<T>> one_minus;
+    return gates<T>(v, one_minus);
 }
 
 // A thread's own weights: scale * weight_branch, where registers are short in shared memory, and weight_output.
@@ -479,7 +509,8 @@ template <typename T, int GATE, int N, int kPacks, bool kShared> struct RowBackw
         Pair<S> sum = both(S(0));
 #pragma unroll
         for (int i = 0; i < kPairs; i++) {
-            const Pair<S> z = GATE == kFullGate ? gates<T>(g[i]) : both(z_row);
+            Pair<S> one_minus;
+            const Pair<S> z = GATE == kFullGate ? gates<T>(g[i], one_minus) : both(z_row);
             const Pair<S> n = b[i] * q, h = gh[i] * r;
             of_output[i] = fma2(h, y[i], of_output[i]);
             const Pair<S> ds = fma2(weights.p[i], h, fma2(y[i], both(back), gs[i]));
@@ -489,7 +520,7 @@ template <typename T, int GATE, int N, int kPacks, bool kShared> struct RowBackw
             y[i] = dz * weights.sw(i);
             const Pair<S> all = y[i] * n;
             sum = sum + all;
-            if constexpr (GATE == kFullGate) out_gate.set(i, fma2(all, z * S(-1), all));
+            if constexpr (GATE == kFullGate) out_gate.set(i, all * one_minus);
         }
         return total(sum);
     }
@@ -510,9 +541,16 @@ template <typename T, int GATE, int N, int kPacks, bool kShared> struct RowBackw
         }
     }
 };
-template <typename T, int GATE> __device__ __forceinline__ Sum<T> row_gate(const Inputs<T>& in, int64_t row) {
-    if constexpr (GATE == kRowGate) return gates<T>(both(widen(in.gate[row * in.gate_stride]))).x;
-    else return 1;
+// The gate of a row. 1 minus it, which only one thread of the team needs, later, it leaves in shared memory: registers are short.
+template <typename T, int GATE> __device__ __forceinline__ Sum<T> row_gate(const Inputs<T>& in, int64_t row, int member, Sum<T>& one_minus) {
+    if constexpr (GATE == kRowGate) {
+        Pair<Sum<T>> other;
+        const Sum<T> z = gates<T>(both(widen(in.gate[row * in.gate_stride])), other).x;
+        if (member == 0) one_minus = other.x;
+        return z;
+    } else {
+        return 1;
+    }
 }
 
 template <typename T, int GATE, int N, int kPacks>
@@ -521,6 +559,7 @@ residual_norm_vjp_rows(const __grid_constant__ Gradients<T> grad, const __grid_c
     using S = Sum<T>;
     using V = Values<T, N, kPacks>;
     __shared__ typename TeamSums<S>::Place shared[2];
+    __shared__ S one_minus[kTeamThreads / 32];
     const int member = threadIdx.x % team, teams = blockDim.x / team, packs = static_cast<int>(in.columns / N);
     TeamSums<S> sums(shared, team);
     Weights<T, N, kPacks, false> weights;
@@ -535,18 +574,19 @@ residual_norm_vjp_rows(const __grid_constant__ Gradients<T> grad, const __grid_c
         gh.load(grad.normed + row * grad.normed_stride + member * N, member, team, packs);
         if constexpr (GATE == kFullGate) g.load(in.gate + row * in.gate_stride + member * N, member, team, packs);
         gs.load(grad.stream + row * grad.stream_stride + member * N, member, team, packs);
-        const S z_row = row_gate<T, GATE>(in, row);
+        const S z_row = row_gate<T, GATE>(in, row, member, one_minus[threadIdx.x / 32]);
         S of_b = work.squares_of(b), squares, products;
         sums.add_up(of_b);
         const S q = work.inverse_rms(of_b);
         work.forward(x, b, g, z_row, gh, q, squares, products);
         sums.add_up(squares, products);
+        if constexpr (GATE == kFullGate) g.forget(); // (else gates and their exponentials stay in registers that there are not)
         S sum = work.backward(out, out_gate, b, g, z_row, gs, gh, q, squares, products);
         const int64_t at = row * in.columns + member * N;
         if (grad.residual != nullptr) out.store(grad.residual + at, member, team, packs);
         if (GATE == kFullGate && grad.gate != nullptr) out_gate.store(grad.gate + at, member, team, packs);
         sums.add_up(sum);
-        if (GATE == kRowGate && grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(sum * (1 - z_row));
+        if (GATE == kRowGate && grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(sum * one_minus[threadIdx.x / 32]);
         work.branch(out, b, q, sum);
         if (grad.branch != nullptr) out.store(grad.branch + at, member, team, packs);
     }
@@ -568,6 +608,7 @@ residual_norm_vjp_staged(const __grid_constant__ Gradients<T> grad, const __grid
     extern __shared__ __align__(128) unsigned char stages[];
     __shared__ typename TeamSums<S>::Place shared[2];
     __shared__ uint64_t full[kBackwardRing];
+    __shared__ S one_minus;
     const int member = threadIdx.x, team = blockDim.x, packs = static_cast<int>(in.columns / N), columns = static_cast<int>(in.columns);
     RowRing<T, kInputs, kBackwardRing> ring(stages, full, in.columns);
     TeamSums<S> sums(shared, team); // (ends with a barrier: a team of one warp does not come here)
@@ -594,7 +635,7 @@ residual_norm_vjp_staged(const __grid_constant__ Gradients<T> grad, const __grid
     S of_b = work.squares_of(b);
     sums.add_up(of_b);
     while (row < in.rows) {
-        const S z_row = row_gate<T, GATE>(in, row), q = work.inverse_rms(of_b);
+        const S z_row = row_gate<T, GATE>(in, row, member, one_minus), q = work.inverse_rms(of_b);
         const T* first = ring.row() + member * N;
         const int place = ring.at;
         V out;
@@ -633,7 +674,7 @@ residual_norm_vjp_staged(const __grid_constant__ Gradients<T> grad, const __grid
         of_b = work.squares_of(next_b);
         sums.add_up(sum, of_b);
         fetch(row + kBackwardRing * step, place); // (everybody is done with it)
-        if (GATE == kRowGate && grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(sum * (1 - z_row));
+        if (GATE == kRowGate && grad.gate != nullptr && member == 0) grad.gate[row] = narrow<T>(sum * one_minus);
         work.branch(out, b, q, sum);
         if (grad.branch != nullptr) out.store(grad.branch + at, member, team, packs);
         b = next_b;
