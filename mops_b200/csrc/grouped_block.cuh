@@ -47,7 +47,8 @@ __device__ __forceinline__ void banded(int64_t at, int64_t rows, int64_t columns
 
 // What the kernels share: setting up, waiting and leaving. A wait that runs out is reported, and everybody leaves. L says how shared memory is
 // laid out, how many columns of tensor memory there are, what the rings are (L::Rings, with begin(), `tmem` and `gave_up`), and whether two blocks
-// work as a pair (L::kPair).
+// work as a pair (L::kPair), and whether warps compute sums again (L::kRepairs): how long others wait for them, `patience`, then grows by the time that takes.
+constexpr long long kPatience = 2000000000; // clocks
 template <typename L> struct Block {
     unsigned char* smem;
     typename L::Rings* rings;
@@ -92,8 +93,14 @@ template <typename L> struct Block {
     template <bool kOfPair = false> __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity) {
         if (passed<kOfPair>(bar, parity)) return true;
         const long long start = clock64();
-        while (*static_cast<volatile int*>(&rings->gave_up) == 0 && clock64() - start < 2000000000LL)
-            if (passed<kOfPair>(bar, parity)) return true;
+        if constexpr (L::kRepairs) {
+            while (clock64() - start < *static_cast<volatile long long*>(&rings->patience))
+                if (passed<kOfPair>(bar, parity)) return true;
+            *static_cast<volatile long long*>(&rings->patience) = 0; // (of everybody)
+        } else {
+            while (*static_cast<volatile int*>(&rings->gave_up) == 0 && clock64() - start < kPatience)
+                if (passed<kOfPair>(bar, parity)) return true;
+        }
         if (atomicExch(&rings->gave_up, 1) == 0) report_stalled(st);
         return false;
     }

@@ -63,7 +63,7 @@ struct Clusters {
 // ---------------------------------------------------------------------------------- 16 bits
 constexpr int kTileThreads = 128;
 template <int kRows_> struct FewLayout {
-    static constexpr bool kPair = false;
+    static constexpr bool kPair = false, kRepairs = false;
     static constexpr int kM = kTileRows * kBoxRow, kX = kRows_ * kBoxRow, kStage = kM + kX;
     static constexpr int kStages = 5 * (kTileRows + 16) / (kTileRows + kRows_); // some 90 KB, for two blocks on an SM
     static constexpr int kRingsAt = kStages * kStage;

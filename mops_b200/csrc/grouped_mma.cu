@@ -31,7 +31,7 @@ constexpr int kStaging = 32 * kBoxRow; // bytes: 32 rows of 64 values, of one wa
 
 // What a block keeps in shared memory.
 template <int kColumns, bool kPaired> struct Layout {
-    static constexpr bool kPair = kPaired;
+    static constexpr bool kPair = kPaired, kRepairs = false;
     static constexpr int kOwnColumns = kPair ? kColumns / 2 : kColumns; // that a block fetches
     static constexpr int kRows = kPair ? 2 * kTileRows : kTileRows;     // of a tile
     static constexpr int kStages = kOwnColumns == 256 ? 4 : kOwnColumns == 128 ? 6 : 8;

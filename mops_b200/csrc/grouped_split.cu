@@ -1,10 +1,12 @@
 // grouped_matrix_product on tensor cores, for f32.
 //
-// A value is split into three bf16 parts of eight bits each, by cutting bits off, so that the parts add up to the value exactly: x = x0 + x1 +
-// x2. Of the nine products of parts the six of up to 2^-16 of the largest are computed, the small ones first; the three left out are about
+// A value is split into three bf16 parts of eight bits each, by cutting bits off, so that the parts add up to the value: x = x0 + x1 +
+// x2 (of values below some 2^-110 the bits under 2^-133, the smallest bf16, are lost). Of the nine products of parts the six of up to 2^-16 of the largest are computed, the small ones first; the three left out are about
 // 2^-24 of the result, as a rounding to f32 is. The tensor cores add to their f32 accumulators by cutting off what does not fit, an error of one sign that
 // grows with the number of additions; so an accumulator takes kRun stages (64 values of depth) and is then added, rounded, to sums in
-// registers. An infinite or NaN operand gives NaN.
+// registers. That is the choice here: f32 results whose error is about twice that of f32 products and sums rounded one by one (K = 128, normal values: 4.0e-7 and 2.0e-7 of the norm), at two to
+// three times the rate that the ordinary units could reach (74 TFLOP/s). Calls of few rows (grouped_few.cu) go to those. Sums that come out as NaN, as they do wherever an operand is infinite, are computed again by the ordinary units (repair()), so
+// infinities come out as f32 arithmetic has them.
 //
 // The copy engine fetches boxes of f32 into one ring of stages; eight warps split them, the parts of the rows' operand go to tensor memory and those of the other to
 // a second ring; one thread issues the products; eight warps add up what the accumulators hold and store the tiles. Bounded by shared memory: of a stage of 64 values of
@@ -55,7 +57,7 @@ template <int kColumns> struct Layout {
     static constexpr unsigned kSums = 2 * kColumns; // columns of tensor memory of the accumulators; the parts come behind them
     static constexpr unsigned kTmem = kColumns == 128 ? 512 : 256;
     static_assert(kSums + kStages * kParts * kPartColumns <= kTmem, "room for the parts");
-    static constexpr bool kPair = false;
+    static constexpr bool kPair = false, kRepairs = true;
     static constexpr int kPieces = 3; // known ahead
     static constexpr int kThreads = mops_b200::kThreads;
     struct Rings {
@@ -66,7 +68,9 @@ template <int kColumns> struct Layout {
         int valid[kRaws]; // rows of depth that a raw stage has (MN-major); -1: there are no more
         uint32_t tmem;
         int gave_up;
+        long long patience;
         __device__ void begin() {
+            patience = kPatience;
             raws.begin(1, kSplitWarps);
             stages.begin(kSplitWarps, 1);
             accumulators.begin(1, kStoreWarps);
@@ -172,6 +176,42 @@ template <bool MN, int kRows> struct ColumnOperand {
         }
     }
     __device__ static __forceinline__ uint64_t descriptor(uint32_t at) { return operand_descriptor<kPartRow>(at, kDepth * 128); }
+};
+
+// The operands in global memory: value (i, j) of a product is the sum of a[i * a_row + d * a_step] * b[j * b_column + d * b_step] over d < depth.
+struct Terms {
+    const float *a, *b;
+    int64_t a_row, a_step, b_column, b_step;
+    int depth;
+    int rows, columns; // that there are from the warp's first ones on
+
+    // By the warp: lanes take every 32nd value of depth. (The sum's order is another one than that of a thread by itself; this is for sums that are infinite or NaN.)
+    __device__ __forceinline__ float product(int i, int j, int lane) const {
+        const float *x = a + i * a_row, *y = b + j * b_column;
+        constexpr int kInFlight = 8;
+        float sum = 0;
+        for (int d0 = 0; d0 < depth; d0 += 32 * kInFlight) {
+            float u[kInFlight], v[kInFlight];
+#pragma unroll
+            for (int k = 0; k < kInFlight; k++) {
+                const int d = d0 + k * 32 + lane;
+                u[k] = d < depth ? x[d * a_step] : 0.f;
+                v[k] = d < depth ? y[d * b_step] : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < kInFlight; k++) sum += u[k] * v[k];
+            if (__any_sync(kFullMask, sum != sum)) break; // it stays so
+        }
+        return warp_sum(sum);
+    }
+    // Whether the first few terms already say that value (i, j) is NaN, as where nothing else is left.
+    __device__ __forceinline__ bool nan_at_once(int i, int j) const {
+        float sum = 0;
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+            if (d < depth) sum += a[i * a_row + d * a_step] * b[j * b_column + d * b_step];
+        return sum != sum;
+    }
 };
 
 // What the parts of a block do, of both kernels.
@@ -300,13 +340,45 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
         return true;
     }
 
+    // An infinite value has no second and third part (inf - inf), so that all sums of its row, or of its column, come out as NaN. Those are computed again, as the
+    // ordinary units do it, and written over what has been stored. out: the warp's first value. (All of it in one place, behind the stores: a look at every sum in front of them, and a copy
+    // of this for each of them, took 2 of 33 us of a product of 128 values in depth.)
+    template <typename MakeTerms> __device__ __forceinline__ void repair(const float (&sum)[kOwn], int warp, int lane, float* out, int64_t stride, MakeTerms make) {
+        long long start = clock64();
+        const Terms terms = make();
+        float* const staging = reinterpret_cast<float*>(block.smem + L::kStagingAt + warp * L::kStaging) + lane * 32;
+        if (lane == 0) boxes_written();
+        __syncwarp();
+#pragma unroll 1
+        for (int c = 0; c < kOwn; c += 32) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) staging[j ^ lane] = c == 0 ? sum[j] : sum[kOwn - 32 + j]; // (each lane another bank)
+#pragma unroll 1
+            for (int j = 0; j < 32 && c + j < terms.columns; j++) {
+                const float value = staging[j ^ lane];
+                unsigned bad = __ballot_sync(kFullMask, lane < terms.rows && value != value && !terms.nan_at_once(lane, c + j));
+                for (; bad != 0; bad &= bad - 1) {
+                    const int i = __ffs(bad) - 1;
+                    const float again = terms.product(i, c + j, lane);
+                    if (lane == i) out[i * stride + c + j] = again;
+                }
+                const long long now = clock64(); // (so long others wait longer for this warp)
+                if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&block.rings->patience), static_cast<unsigned long long>(now - start));
+                start = now;
+            }
+        }
+        __syncwarp();
+    }
+
     // Writes them, 32 columns at a time through shared memory: by the copy engine, box by box, or where there are not all 32 rows of a box (`here`), or rows of the
-    // output begin anywhere (loose), a row after the other. out: the first value.
-    __device__ __forceinline__ void store(const float (&sum)[kOwn], int warp, const CUtensorMap& map, int column, int row, int slice, float* out,
+    // output begin anywhere (loose), a row after the other. out: the first value. Returns whether there are sums to repair: some are NaN in the lane's first column, or in the
+    // first row.
+    __device__ __forceinline__ bool store(const float (&sum)[kOwn], int warp, const CUtensorMap& map, int column, int row, int slice, float* out,
                                           int64_t stride, int64_t here, int64_t wide, bool loose, int lane) {
         unsigned char* place = block.smem + L::kStagingAt + warp * L::kStaging;
         const int rows = static_cast<int>(min(here, int64_t(32)));
         const bool box = !loose && rows == 32;
+        bool odd = sum[0] != sum[0];
 #pragma unroll
         for (int c = 0; c < kOwn; c += 32) {
             if (c >= wide || rows <= 0) break;
@@ -321,12 +393,14 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
                                             __float_as_uint(sum[c + 4 * j + 2]), __float_as_uint(sum[c + 4 * j + 3])));
                 async_proxy_fence();
                 __syncwarp();
+                odd |= isnan(*reinterpret_cast<const float*>(place + lane * 4));
                 if (lane == 0) box_out(map, column + c, row, slice, to);
             } else {
                 float* staging = reinterpret_cast<float*>(place);
 #pragma unroll
                 for (int j = 0; j < 32; j++) staging[lane * 32 + (j ^ lane)] = sum[c + j]; // (each lane another bank)
                 __syncwarp();
+                odd |= isnan(staging[lane]);
                 if (c + lane < wide) {
 #pragma unroll 8
                     for (int r = 0; r < rows; r++) out[r * stride + c + lane] = staging[r * 32 + (lane ^ r)];
@@ -334,16 +408,29 @@ template <bool A_MN, bool B_MN, int kColumns> struct Work {
                 __syncwarp();
             }
         }
+        return __any_sync(kFullMask, odd && rows > 0);
+    }
+    // The same of sums that go elsewhere.
+    __device__ __forceinline__ static bool any_nan(const float (&sum)[kOwn]) {
+        float check[8] = {}; // (side by side)
+#pragma unroll
+        for (int i = 0; i < kOwn; i++) check[i % 8] = fmaf(sum[i], 0.f, check[i % 8]);
+        const float all = (check[0] + check[1] + (check[2] + check[3])) + (check[4] + check[5] + (check[6] + check[7]));
+        return __any_sync(kFullMask, isnan(all));
     }
 };
 
 // ---------------------------------------------------------------------------------- rows
 // out[r,:] = X[r,:] M[group of r]. M_MN: the columns of M are neighbours in memory, else its depth is.
+struct RowOperands {
+    const float *x, *m;
+    int64_t x_stride, group_stride, depth_stride, column_stride; // of m the last three
+};
 template <bool M_MN, int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_out,
-                   float* __restrict__ out, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int depth, int columns, bool loose,
-                   Status st) {
+                   float* __restrict__ out, const __grid_constant__ RowOperands from, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int depth,
+                   int columns, bool loose, Status st) {
     extern __shared__ unsigned char raw[];
     using W = Work<false, M_MN, kColumns>;
     using L = typename W::L;
@@ -365,8 +452,12 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
             float sum[W::kOwn];
             if (!work.collect(sum, piece.steps, quadrant, half, lane)) break;
             const int64_t row = piece.lo + quadrant * 32, column = piece.column + half * W::kOwn;
-            work.store(sum, warp - kSplitWarps, map_out, column, static_cast<int>(row), 0, out + row * columns + column, columns, piece.hi - row,
-                       columns - column, loose, lane);
+            if (work.store(sum, warp - kSplitWarps, map_out, column, static_cast<int>(row), 0, out + row * columns + column, columns, piece.hi - row,
+                           columns - column, loose, lane))
+                work.repair(sum, warp - kSplitWarps, lane, out + row * columns + column, columns, [&] {
+                    return Terms{from.x + row * from.x_stride, from.m + piece.group * from.group_stride + column * from.column_stride, from.x_stride, 1, from.column_stride,
+                                 from.depth_stride, depth, static_cast<int>(min(piece.hi - row, int64_t(32))), static_cast<int>(columns - column)};
+                });
         }
     } else {
         fewer_registers<kMultiplyRegisters>();
@@ -399,11 +490,15 @@ grouped_rows_split(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
 // ------------------------------------------------------------------------- outer products
 // out[g] = X[rows of g]^T Y[rows of g].
+struct OuterOperands {
+    const float *x, *y;
+    int64_t x_stride, y_stride;
+};
 template <int kColumns>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
-                    const __grid_constant__ CUtensorMap map_out, float* __restrict__ out, float* __restrict__ parts, int64_t most_parts, const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height,
-                    int columns, int64_t segment, bool loose, Status st) {
+                    const __grid_constant__ CUtensorMap map_out, float* __restrict__ out, float* __restrict__ parts, int64_t most_parts, const __grid_constant__ OuterOperands from,
+                    const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment, bool loose, Status st) {
     extern __shared__ unsigned char raw[];
     using W = Work<true, true, kColumns>;
     using L = typename W::L;
@@ -424,20 +519,29 @@ grouped_outer_split(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         while (supply.next(piece, lane)) {
             float sum[W::kOwn];
             if (!work.collect(sum, piece.steps, quadrant, half, lane)) break;
+            const int64_t row = piece.row + quadrant * 32, column = piece.column + half * W::kOwn;
+            float* to = out + (static_cast<int64_t>(piece.group) * height + row) * columns + column;
+            int64_t stride = columns;
+            bool odd;
             if (piece.slot >= 0) {
                 // (there are more parts than there is room for only where offsets descend, which is reported)
                 if (piece.slot >= most_parts) continue;
-                float* to = parts + (piece.slot * kTileRows + quadrant * 32 + lane) * kColumns + half * W::kOwn;
+                to = parts + (piece.slot * kTileRows + quadrant * 32) * kColumns + half * W::kOwn;
+                stride = kColumns;
 #pragma unroll
                 for (int i = 0; i < W::kOwn; i += 4)
-                    *reinterpret_cast<float4*>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+                    *reinterpret_cast<float4*>(to + lane * kColumns + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+                odd = W::any_nan(sum);
             } else {
-                const int64_t row = piece.row + quadrant * 32, column = piece.column + half * W::kOwn;
                 // (the copy engine leaves out what lies behind the output's last row)
-                work.store(sum, warp - kSplitWarps, map_out, column, static_cast<int>(row), piece.group,
-                           out + (static_cast<int64_t>(piece.group) * height + row) * columns + column, columns,
-                           loose || row >= height ? height - row : 32, columns - column, loose, lane);
+                odd = work.store(sum, warp - kSplitWarps, map_out, column, static_cast<int>(row), piece.group, to, columns,
+                                 loose || row >= height ? height - row : 32, columns - column, loose, lane);
             }
+            if (odd)
+                work.repair(sum, warp - kSplitWarps, lane, to, stride, [&] {
+                    return Terms{from.x + piece.lo * from.x_stride + row, from.y + piece.lo * from.y_stride + column, 1, from.x_stride, 1, from.y_stride,
+                                 static_cast<int>(piece.hi - piece.lo), static_cast<int>(height - row), static_cast<int>(columns - column)};
+                });
         }
     } else {
         fewer_registers<kMultiplyRegisters>();
@@ -501,7 +605,8 @@ bool multiply_rows_split(const Call& call, const RowsProblem& p, const std::stri
         const int64_t tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kColumns);
         auto kernel = grouped_rows_split<M_MN, kColumns>;
         check_registers(reinterpret_cast<const void*>(kernel), op);
-        launch_blocks<L>(call, op, kernel, tiles, x, m, out, static_cast<float*>(p.out.data), p.offsets, p.groups, p.rows,
+        const RowOperands from{static_cast<const float*>(p.X.data), static_cast<const float*>(p.M.data), p.X.stride[0], p.M.stride[0], p.depth_stride, p.column_stride};
+        launch_blocks<L>(call, op, kernel, tiles, x, m, out, static_cast<float*>(p.out.data), from, p.offsets, p.groups, p.rows,
                          static_cast<int>(p.depth), static_cast<int>(p.columns), loose, call.status);
         note_kernel_f("grouped_rows_split<%s,%d>", M_MN ? "columns" : "depth", kColumns);
     };
@@ -533,7 +638,8 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
         check_registers(reinterpret_cast<const void*>(kernel), op);
         const bool loose = columns % 4 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
         const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
-        launch_blocks<L>(call, op, kernel, tiles * (rows / segment + p.groups), x, y, out, static_cast<float*>(p.out.data), parts, most_parts, p.offsets,
+        const OuterOperands from{static_cast<const float*>(p.X.data), static_cast<const float*>(p.Y.data), p.X.stride[0], p.Y.stride[0]};
+        launch_blocks<L>(call, op, kernel, tiles * (rows / segment + p.groups), x, y, out, static_cast<float*>(p.out.data), parts, most_parts, from, p.offsets,
                          p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {
             join_outer<float, kTileRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);

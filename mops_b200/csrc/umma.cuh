@@ -76,6 +76,11 @@ __device__ __forceinline__ void box_out(const CUtensorMap& map, int inner, int o
 template <int N> __device__ __forceinline__ void boxes_left() {
     asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
 }
+// Until all boxes that this thread sent out are in global memory, where ordinary stores may follow.
+__device__ __forceinline__ void boxes_written() {
+    asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+    asm volatile("fence.proxy.async;\n" ::: "memory");
+}
 __device__ __forceinline__ void map_prefetch(const CUtensorMap& map) {
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
 }
