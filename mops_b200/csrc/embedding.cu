@@ -538,9 +538,9 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
     if (rows == 0 || columns == 0) return;
     Call call = begin_call();
     const size_t index_room = (static_cast<size_t>(tokens) * sizeof(int32_t) + 255) / 256 * 256;
-    unsigned char* order = static_cast<unsigned char*>(scratch_alloc(call, 2 * index_room + 256));
-    int32_t* sorted = reinterpret_cast<int32_t*>(order);
-    int32_t* permutation = reinterpret_cast<int32_t*>(order + index_room);
+    Scratch order(call, 2 * index_room + 256);
+    int32_t* sorted = order.as<int32_t>();
+    int32_t* permutation = reinterpret_cast<int32_t*>(order.as<unsigned char>() + index_room);
     const int32_t* given = static_cast<const int32_t*>(indices.data);
     for_type(grad_W.type, [&](auto zero) {
         using T = decltype(zero);
@@ -572,7 +572,8 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
             const int chunk = static_cast<int>(std::min<int64_t>(ceil_div(of_warp, 16) * 16, 256));
             const int64_t chunks = ceil_div(tokens, chunk);
             using P = Sums<Sum<T>, N>;
-            P* partial = static_cast<P*>(scratch_alloc(call, static_cast<size_t>(2 * chunks * slabs * 32) * sizeof(P)));
+            Scratch sums(call, static_cast<size_t>(2 * chunks * slabs * 32) * sizeof(P));
+            P* partial = sums.as<P>();
             embedding_sums<T, N><<<grid_of(clear_blocks + ceil_div(chunks * slabs, kWarps), op), kThreads, 0, call.stream>>>(
                 out, static_cast<const T*>(grad_output.data), grad_output.stride[0], sorted, permutation, tokens, rows,
                 columns, chunk, chunks, slabs, static_cast<Sum<T>>(scale), partial, clear_blocks);
@@ -580,12 +581,12 @@ void embedding_lookup_vjp(Array grad_W, Array grad_output, Array indices, double
                 embedding_join<T, N>
                     <<<dim3(grid_of(ceil_div(chunks, kWarps), op), static_cast<unsigned>(std::min<int64_t>(slabs, 65535))), kThreads, 0, call.stream>>>(
                         out, sorted, tokens, rows, columns, chunk, chunks, slabs, static_cast<Sum<T>>(scale), partial);
-            scratch_free(call, partial);
+            sums.free();
             note_kernel_f("embedding_sums<%s,%d>", array_type_name<T>(), N);
         };
         widest<T>(grad_W, grad_output, launch);
     });
-    scratch_free(call, order);
+    order.free();
     end_call(call, op.c_str(), kIndexNames, 1);
 }
 

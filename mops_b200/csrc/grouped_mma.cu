@@ -459,14 +459,15 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         const CUtensorMap out = loose ? x : tensor_map(p.X.type, p.out.data, columns, height, p.groups, columns, height * columns, 32);
         const int64_t tiles = ceil_div(height, L::kRows) * ceil_div(columns, kColumns);
         const int64_t segment = outer_segment(rows, p.groups, tiles, kPair ? sms / 2 : sms), most_parts = most_outer_parts(rows, tiles, segment);
-        float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * L::kRows * kColumns * sizeof(float)))
-                                      : nullptr;
+        Scratch room(call);
+        if (rows > segment) room.take(static_cast<size_t>(most_parts) * L::kRows * kColumns * sizeof(float));
+        float* parts = room.as<float>();
         launch_blocks<L>(call, op, grouped_outer_mma<BF16, kColumns, kPair>, tiles * (rows / segment + p.groups), x, y, out,
                          static_cast<uint16_t*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height),
                          static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {
             join_outer<T, L::kRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);
-            scratch_free(call, parts);
+            room.free();
         }
         note_kernel_f("grouped_outer_mma<%s,%d,%s>", BF16 ? "bf16" : "f16", kColumns, kPair ? "pair" : "block");
     };

@@ -632,8 +632,9 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
         const CUtensorMap y = tensor_map(p.X.type, p.Y.data, columns, rows, 1, p.Y.stride[0], 0, kDepth);
         const int64_t tiles = ceil_div(height, kTileRows) * ceil_div(columns, kColumns);
         const int64_t segment = outer_segment(rows, p.groups, tiles, sms), most_parts = most_outer_parts(rows, tiles, segment);
-        float* parts = rows > segment ? static_cast<float*>(scratch_alloc(call, static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float)))
-                                      : nullptr;
+        Scratch room(call);
+        if (rows > segment) room.take(static_cast<size_t>(most_parts) * kTileRows * kColumns * sizeof(float));
+        float* parts = room.as<float>();
         auto kernel = grouped_outer_split<kColumns>;
         check_registers(reinterpret_cast<const void*>(kernel), op);
         const bool loose = columns % 4 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
@@ -643,7 +644,7 @@ bool multiply_outer_split(const Call& call, const OuterProblem& p, const std::st
                          p.groups, rows, static_cast<int>(height), static_cast<int>(columns), segment, loose, call.status);
         if (rows > segment) {
             join_outer<float, kTileRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);
-            scratch_free(call, parts);
+            room.free();
         }
         note_kernel_f("grouped_outer_split<%d>", kColumns);
     };

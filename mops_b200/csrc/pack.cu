@@ -67,10 +67,11 @@ void Packing::add(Array& a) {
         boxable(a.type, a.data, a.shape[inner], a.shape[outer], slices, a.stride[outer], slice_stride))
         return;
     const int64_t bytes = type_bytes(a.type), values = 16 / bytes, packs = ceil_div(a.shape[inner], values);
-    Job& j = jobs_[n_++];
+    Job& j = jobs_[n_];
     type_ = a.type;
     j.from = a.data;
     j.to = scratch_alloc(call_, static_cast<size_t>(slices * a.shape[outer] * packs) * 16);
+    n_++;
     j.outer = a.shape[outer], j.outer_stride = a.stride[outer], j.slices = slices, j.slice_stride = slice_stride;
     j.inner = a.shape[inner], j.packs = packs;
     j.begin = static_cast<const unsigned char*>(a.data);
@@ -96,8 +97,7 @@ void Packing::run() {
 }
 
 void Packing::release() {
-    for (int i = 0; i < n_; i++) scratch_free(call_, jobs_[i].to);
-    n_ = 0;
+    while (n_ > 0) scratch_free(call_, jobs_[--n_].to);
 }
 
 } // namespace mops_b200

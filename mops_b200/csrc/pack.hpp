@@ -11,6 +11,12 @@ namespace mops_b200 {
 class Packing {
   public:
     explicit Packing(const Call& call) : call_(call) {}
+    ~Packing() {
+        try {
+            release();
+        } catch (...) { // (there is an exception already)
+        }
+    }
     Packing(const Packing&) = delete;
     Packing& operator=(const Packing&) = delete;
 

@@ -889,12 +889,12 @@ void gated_residual_norm_vjp(Array grad_residual, Array grad_branch, Array grad_
         auto data = [](const Array& a) { return static_cast<T*>(a.data); };
         const bool of_columns = grad_scale.data != nullptr || grad_weight_branch.data != nullptr || grad_weight_output.data != nullptr;
         int64_t blocks = 0;
-        Sum<T>* sums = nullptr;
+        Scratch of_blocks(call);
         auto room = [&](int64_t for_blocks) {
             blocks = for_blocks;
-            sums = static_cast<Sum<T>*>(scratch_alloc(call, static_cast<size_t>(2 * blocks * columns) * sizeof(Sum<T>)));
+            of_blocks.take(static_cast<size_t>(2 * blocks * columns) * sizeof(Sum<T>));
             return Gradients<T>{data(grad_residual), data(grad_branch), data(grad_gate), data(grad_stream), data(grad_normed),
-                                grad_stream.stride[0], grad_normed.stride[0], sums};
+                                grad_stream.stride[0], grad_normed.stride[0], of_blocks.as<Sum<T>>()};
         };
         for_gate(kind, [&](auto g) {
             constexpr int GATE = decltype(g)::value;
@@ -934,9 +934,9 @@ void gated_residual_norm_vjp(Array grad_residual, Array grad_branch, Array grad_
         MOPS_CUDA_OK(cudaGetLastError());
         if (of_columns)
             residual_norm_columns<T><<<static_cast<unsigned>(ceil_div(columns, kColumnsAtOnce)), kColumnThreads, 0, call.stream>>>(
-                data(grad_scale), data(grad_weight_branch), data(grad_weight_output), data(scale), data(weight_branch), sums,
+                data(grad_scale), data(grad_weight_branch), data(grad_weight_output), data(scale), data(weight_branch), of_blocks.as<Sum<T>>(),
                 blocks, columns);
-        if (sums != nullptr) scratch_free(call, sums);
+        of_blocks.free();
     });
     end_call(call, op.c_str(), nullptr, 0);
 }

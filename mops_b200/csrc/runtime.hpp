@@ -96,6 +96,35 @@ bool get_wait();
 void* scratch_alloc(const Call& call, size_t bytes);
 void scratch_free(const Call& call, void* ptr);
 
+// Scratch memory of a scope, given back also where an exception leaves it.
+class Scratch {
+  public:
+    explicit Scratch(const Call& call) : call_(call) {}
+    Scratch(const Call& call, size_t bytes) : call_(call) { take(bytes); }
+    Scratch(const Scratch&) = delete;
+    Scratch& operator=(const Scratch&) = delete;
+    ~Scratch() {
+        try {
+            free();
+        } catch (...) { // (there is an exception already)
+        }
+    }
+    void take(size_t bytes) {
+        free();
+        ptr_ = scratch_alloc(call_, bytes);
+    }
+    void free() {
+        void* ptr = ptr_;
+        ptr_ = nullptr;
+        scratch_free(call_, ptr);
+    }
+    template <typename T> T* as() const { return static_cast<T*>(ptr_); }
+
+  private:
+    const Call& call_;
+    void* ptr_ = nullptr;
+};
+
 // ---- reusable device tables ("plans")
 // Every operation first turns its index (and coefficient) arrays into a device table: the
 // segment offsets of a scatter index, HPE's packed monomial records, SAP's sorted triplets,

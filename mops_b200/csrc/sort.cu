@@ -177,8 +177,8 @@ void sort_keys_by(const Call& call, int32_t* sorted, int32_t* permutation, const
     const size_t hist_bytes = static_cast<size_t>(256) * blocks * sizeof(int32_t);
     const size_t buf_bytes = (static_cast<size_t>(n) * sizeof(int32_t) + 255) / 256 * 256;
     const size_t hist_room = (hist_bytes + 255) / 256 * 256;
-    unsigned char* scratch = static_cast<unsigned char*>(
-        scratch_alloc(call, hist_room + 1024 + (passes > 1 ? 4 * buf_bytes : 0)));
+    Scratch room(call, hist_room + 1024 + (passes > 1 ? 4 * buf_bytes : 0));
+    unsigned char* scratch = room.as<unsigned char>();
     int32_t* hist = reinterpret_cast<int32_t*>(scratch);
     int32_t* totals = reinterpret_cast<int32_t*>(scratch + hist_room);
     unsigned char* bufs = scratch + hist_room + 1024;
@@ -202,7 +202,7 @@ void sort_keys_by(const Call& call, int32_t* sorted, int32_t* permutation, const
         vals_in = vals_out;
     }
     note_kernel_f("radix sort, %d passes", passes);
-    scratch_free(call, scratch);
+    room.free();
 }
 } // namespace
 
