@@ -23,15 +23,14 @@ namespace mops_b200 {
 
 // What a thread keeps for a (device, stream): calls on one stream run in order, so a call's status
 // words and workspace cannot be overwritten before its own kernels are done with them, and calls on
-// different streams (which may overlap) never share them. Status words are never freed (kernels of
-// captured graphs hold their address) but handed on, with the workspace, to later streams.
+// different streams (which may overlap) never share them. Status words are never freed but handed on, with the
+// workspace, to later streams. (Those of a graph that is being captured: graph_words().)
 struct StreamState {
     Status status{};
     unsigned char* workspace = nullptr;
     size_t size = 0, used = 0;
     size_t wanted = 0; // by the previous call
     bool pending = false; // a call may still be running (it did not wait, or ended with an exception)
-    bool captured = false; // a graph holds the address of the status words
     uint64_t last_call = 0;
 };
 
@@ -47,6 +46,7 @@ struct RelaxedCapture {
 constexpr size_t kMostWorkspace = 4 << 20; // bytes per (thread, device, stream)
 constexpr int kMostWorkspaces = 16;        // per thread
 constexpr size_t kMostStreams = 64;        // per thread, before states of old streams are handed on
+constexpr size_t kMostCaptures = 16;       // per thread, that it remembers
 
 struct ThreadState {
     cudaStream_t stream = nullptr;
@@ -55,6 +55,7 @@ struct ThreadState {
     // by device and stream id: a handle may come back for another stream, an id does not
     std::map<std::pair<int, unsigned long long>, StreamState> streams;
     std::vector<std::pair<int, StreamState>> spare; // (device, state) of streams that have gone
+    std::map<std::pair<int, unsigned long long>, StreamState> captures; // by device and the capture's id
     uint64_t calls = 0;
     std::pair<int, unsigned long long> last_key{-1, 0};
     StreamState* last = nullptr; // of the previous call
@@ -125,13 +126,13 @@ void zero_words(uint32_t* dev, int words) {
 }
 
 // Ids of streams never come back, so a program that makes a stream per step would leave a state behind
-// each time. At kMostStreams the older half of them (but for graphs') goes to `spare`, once the device
+// each time. At kMostStreams the older half of them goes to `spare`, once the device
 // has been waited for if any of their calls may still run: one wait in kMostStreams / 2 new streams.
 // Where it cannot be waited for, the states stay.
 void retire_streams(int device) {
     std::vector<std::pair<uint64_t, std::pair<int, unsigned long long>>> old;
     for (const auto& s : g_thread.streams)
-        if (s.first.first == device && !s.second.captured) old.push_back({s.second.last_call, s.first});
+        if (s.first.first == device) old.push_back({s.second.last_call, s.first});
     std::sort(old.begin(), old.end());
     old.resize(std::min(old.size(), kMostStreams / 2));
     const RelaxedCapture relaxed;
@@ -150,10 +151,10 @@ void retire_streams(int device) {
     }
 }
 
-StreamState& state_of(const std::pair<int, unsigned long long>& key, bool capturing) {
+StreamState& state_of(const std::pair<int, unsigned long long>& key) {
     auto it = g_thread.streams.find(key);
     if (it != g_thread.streams.end()) return it->second;
-    if (g_thread.streams.size() >= kMostStreams && !capturing) retire_streams(key.first);
+    if (g_thread.streams.size() >= kMostStreams) retire_streams(key.first);
     // (a spare one with a workspace rather than one without)
     auto spare = g_thread.spare.end();
     for (auto s = g_thread.spare.begin(); s != g_thread.spare.end(); ++s)
@@ -174,6 +175,92 @@ StreamState& state_of(const std::pair<int, unsigned long long>& key, bool captur
     }
     return g_thread.streams.emplace(key, state).first->second;
 }
+
+// Status words of graphs. The kernels of a captured graph hold the address of their words for as long as the graph, or what was instantiated from it, may
+// run. So the graph itself keeps them, as a user object, and they are free again when it has gone. They come from slabs, of which there are as many as the graphs
+// that are there at a time need.
+struct GraphWords {
+    Status status{};
+    int device;
+};
+struct GraphWordsPool {
+    std::mutex mutex;
+    std::map<int, std::vector<GraphWords*>> free; // by device
+};
+GraphWordsPool& graph_words_pool() {
+    static GraphWordsPool* const pool = new GraphWordsPool; // (graphs may go after everything else has)
+    return *pool;
+}
+constexpr int kSlabWords = 64;
+
+void CUDART_CB graph_gone(void* p) { // (no CUDA calls in here)
+    GraphWords* const words = static_cast<GraphWords*>(p);
+    GraphWordsPool& pool = graph_words_pool();
+    std::lock_guard<std::mutex> lock(pool.mutex);
+    pool.free[words->device].push_back(words);
+}
+
+// Words, all zero, for calls on `stream`, which is being captured.
+Status graph_words(int device, cudaStream_t stream) {
+    GraphWordsPool& pool = graph_words_pool();
+    GraphWords* words = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(pool.mutex);
+        std::vector<GraphWords*>& free = pool.free[device];
+        if (free.empty()) {
+            void *host = nullptr, *dev = nullptr;
+            constexpr size_t bytes = kSlabWords * kStatusWords * sizeof(uint32_t);
+            MOPS_CUDA_OK(cudaHostAlloc(&host, bytes, cudaHostAllocMapped | cudaHostAllocPortable));
+            MOPS_CUDA_OK(cudaMalloc(&dev, bytes));
+            for (int i = 0; i < kSlabWords; i++) {
+                GraphWords* const w = new GraphWords;
+                w->status.host = static_cast<uint32_t*>(host) + i * kStatusWords;
+                w->status.dev = static_cast<uint32_t*>(dev) + i * kStatusWords;
+                w->device = device;
+                free.push_back(w);
+            }
+        }
+        words = free.back();
+        free.pop_back();
+    }
+    try {
+        // (of a graph that has gone they hold the numbers of its calls)
+        for (int i = 0; i < kStatusWords; i++) static_cast<volatile uint32_t*>(words->status.host)[i] = 0;
+        zero_words(words->status.dev, kStatusWords);
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        cudaGraph_t graph = nullptr;
+        MOPS_CUDA_OK(cudaStreamGetCaptureInfo_v2(stream, &capture, nullptr, &graph, nullptr, nullptr));
+        if (capture != cudaStreamCaptureStatusActive) throw std::runtime_error("the capture of the stream into a graph has been invalidated");
+        cudaUserObject_t object = nullptr;
+        MOPS_CUDA_OK(cudaUserObjectCreate(&object, words, graph_gone, 1, cudaUserObjectNoDestructorSync));
+        const cudaError_t err = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+        if (err != cudaSuccess) {
+            words = nullptr; // (they go back with the object)
+            (void)cudaUserObjectRelease(object, 1);
+            MOPS_CUDA_OK(err);
+        }
+        return words->status;
+    } catch (...) {
+        if (words != nullptr) graph_gone(words);
+        throw;
+    }
+}
+
+// What this thread keeps for a capture. It forgets the oldest of many: a later call in that one gets other words.
+StreamState& state_of_capture(const std::pair<int, unsigned long long>& key, cudaStream_t stream) {
+    auto it = g_thread.captures.find(key);
+    if (it != g_thread.captures.end()) return it->second;
+    StreamState state{};
+    state.status = graph_words(key.first, stream);
+    while (g_thread.captures.size() >= kMostCaptures) {
+        auto oldest = g_thread.captures.begin();
+        for (auto c = g_thread.captures.begin(); c != g_thread.captures.end(); ++c)
+            if (c->second.last_call < oldest->second.last_call) oldest = c;
+        g_thread.captures.erase(oldest);
+    }
+    g_thread.last = nullptr;
+    return g_thread.captures.emplace(key, state).first->second;
+}
 } // namespace
 
 Call begin_call() {
@@ -183,7 +270,7 @@ Call begin_call() {
     call.wait = g_thread.wait;
 
     g_thread.kernels.clear();
-    // The id of a stream cannot be asked for while it is captured into a graph; that of the capture stands for it then, so
+    // The id of a stream cannot be asked for while it is captured into a graph; that of the capture stands for it then, and
     // each graph has status words of its own.
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
@@ -194,13 +281,12 @@ Call begin_call() {
     const auto key = std::make_pair(call.device, id);
     if (g_thread.last == nullptr || key != g_thread.last_key) {
         const RelaxedCapture relaxed; // (a first call allocates)
-        g_thread.last = &state_of(key, call.capturing);
+        g_thread.last = call.capturing ? &state_of_capture(key, call.stream) : &state_of(key);
         g_thread.last_key = key;
     }
     call.state = g_thread.last;
     call.state->used = 0;
     call.state->pending = true;
-    call.state->captured |= call.capturing;
     call.state->last_call = ++g_thread.calls;
     call.status = call.state->status;
     g_thread.epoch += 1;
