@@ -176,8 +176,10 @@ void check_common(Array& A, Array& W, const char* w_name, Array& offsets, Array&
     for (int64_t n : {A.shape[0], A.shape[1], W.shape[0], W.shape[2]}) fits_int32(static_cast<size_t>(n), "a size", op);
 }
 
-// One of the last two dimensions of W lies value by value in memory.
-void check_matrices(const Array& W, const char* name, const std::string& op) {
+// One of the last two dimensions of W lies value by value in memory. (So does one of size 1, whatever its stride; matrices of one row whose columns lie apart are
+// columns of one value each.)
+void check_matrices(Array& W, const char* name, const std::string& op) {
+    if (W.shape[1] == 1 && W.stride[2] != 1) W.stride[1] = 1;
     if (W.stride[2] != 1 && W.stride[1] != 1)
         throw std::runtime_error(std::string(name) + " must have a stride of 1 in one of its last two dimensions in " + op);
 }

@@ -1,9 +1,11 @@
-"""grouped_matrix_product: operands that are infinite or NaN, whatever kernel multiplies them, and the precision of deep f32 sums."""
+"""grouped_matrix_product: operands that are infinite or NaN, whatever kernel multiplies them, the precision of deep f32 sums, and matrices of one row."""
 import pytest
 import torch
 
 import mops_b200
-from test_block_ops import DTYPES, normal, offsets_of
+import mops_b200.torch as mt
+from mops_b200 import _lib
+from test_block_ops import DTYPES, check_grouped, normal, offsets_of
 
 
 def kinds(t):
@@ -109,3 +111,25 @@ def test_deep_sums_of_one_sign_in_f32(what, depth):
         want = A.double() @ W[0].double()
     bound = 3 * 2.0 ** -23 + 24 * 2.0 ** -22 + (depth / 64 + 1) * 2.0 ** -24
     assert ((got.double() - want).abs() / want).max().item() <= bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [[2, 1], [70, 0, 200]])
+@pytest.mark.parametrize("N", [1, 3, 40, 129])
+def test_matrices_of_one_row_whose_columns_lie_apart(dtype, rows, N):
+    """Strides of a dimension of one value mean nothing: with one column of a wider array the other way round, the only stride of 1 is such a one."""
+    G, R = len(rows), sum(rows)
+    wide = normal((G, N, 5), dtype, 1)
+    W = wide[:, :, 2:3].transpose(1, 2)
+    check_grouped(normal((R, 1), dtype, 2), W.detach(), offsets_of(rows), normal((R, N), dtype, 3))
+    check_grouped(normal((R, N), dtype, 2), wide[:, :, 1:2].detach(), offsets_of(rows), normal((R, 1), dtype, 3))
+    # through the C ABI
+    A, offsets, out = normal((R, 1), dtype, 2), offsets_of(rows), torch.empty(R, N, dtype=dtype, device="cuda")
+    array = lambda t, stride=None: _lib.make_array(t.data_ptr(), str(t.dtype).split(".")[1], tuple(t.shape), stride or t.stride())
+    torch.cuda.synchronize()
+    for stride in (1, 7, 5 * N):
+        out.fill_(7)
+        torch.cuda.synchronize()
+        _lib.call("mops_b200_cuda_grouped_matrix_product", [array(out), array(A), array(W, (5 * N, stride, 5)), array(offsets)])
+        assert torch.equal(out, mt.grouped_matrix_product(A, W.contiguous(), offsets))
