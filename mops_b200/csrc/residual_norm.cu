@@ -416,6 +416,13 @@ template <typename T, int kInputs, int kRing> struct RowRing {
     __device__ __forceinline__ void next() {
         if (++at == kRing) at = 0, round ^= 1;
     }
+    // A wait ran out: reports that, and the copying thread stays until the copies that may be under way, to this place and the next ones, are there (or another wait runs
+    // out), as the block's shared memory is another one's afterwards. rows: that are left, from the one waited for on; places: that are filled at most.
+    __device__ void give_up(const Status& st, int64_t rows, int places) {
+        report_stalled(st);
+        if (threadIdx.x != 0) return;
+        for (int i = 0; i < places && i < rows; i++, next()) (void)wait();
+    }
 };
 constexpr int kForwardRing = 3, kBackwardRing = 2;
 
@@ -446,10 +453,7 @@ residual_norm_staged(T* __restrict__ stream, T* __restrict__ normed, const __gri
     RowForward<T, GATE, N, kPacks> work(in);
     for (; row < in.rows; row += step, ring.next()) {
         const T gate = GATE == kRowGate ? in.gate[row * in.gate_stride] : T{};
-        if (!ring.wait()) {
-            report_stalled(st);
-            return;
-        }
+        if (!ring.wait()) return ring.give_up(st, (in.rows - row + step - 1) / step, kForwardRing);
         const T* first = ring.row() + member * N;
         V x, b, g, out;
         x.clear(), b.clear(), g.clear();
@@ -625,10 +629,7 @@ residual_norm_vjp_staged(const __grid_constant__ Gradients<T> grad, const __grid
     Weights<T, N, kPacks, true> weights;
     weights.load(in, member, team, packs, reinterpret_cast<S*>(stages + kBackwardRing * kInputs * ring.row_bytes));
     RowBackward<T, GATE, N, kPacks, true> work(weights, in);
-    if (!ring.wait()) { // (a block has at least one row)
-        report_stalled(st);
-        return;
-    }
+    if (!ring.wait()) return ring.give_up(st, (in.rows - row + step - 1) / step, kBackwardRing); // (a block has at least one row)
     V b;
     b.clear();
     b.load(ring.row() + member * N, member, team, packs);
@@ -665,10 +666,7 @@ residual_norm_vjp_staged(const __grid_constant__ Gradients<T> grad, const __grid
         V next_b;
         next_b.clear();
         if (row + step < in.rows) {
-            if (!ring.wait()) {
-                report_stalled(st);
-                return;
-            }
+            if (!ring.wait()) return ring.give_up(st, 1, 1);
             next_b.load(ring.row() + member * N, member, team, packs);
         }
         of_b = work.squares_of(next_b);
