@@ -177,7 +177,10 @@ template <typename L, typename Decode> __device__ __forceinline__ void hand_out(
         }
         if (!__shfl_sync(kFullMask, ok, 0)) return;
         Piece p;
-        if (decode(want, p) && !publish(p)) return;
+        if (decode(want, p) && !publish(p)) {
+            if (lane == 0) (void)mbarrier_wait(&pieces.answers.full[0], asked.round); // (the answer that is on its way into shared memory)
+            return;
+        }
         int taken = -1;
         if (lane == 0) {
             ok = block.wait_full(pieces.answers, asked);
