@@ -60,7 +60,7 @@ embedding_rows(T* __restrict__ output, const T* __restrict__ W, int64_t stride, 
 
 // ------------------------------------------------------------------------------ gradient
 // Few tokens: one block sorts them, in shared memory, while the others clear the rows of grad_W that no token asks for, which takes
-// longer. Digits of up to nine bits (so that 2^18 rows take two passes of 13 us), lowest first, every pass stable: a warp's keys in order, warps in order.
+// longer. Digits of up to nine bits (so that 2^18 rows take two passes), lowest first, every pass stable: a warp's keys in order, warps in order.
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderItems = 16;
 constexpr int kFewTokens = kOrderThreads * kOrderItems;

@@ -11,8 +11,8 @@
 // The copy engine fetches boxes of f32 into one ring of stages; eight warps split them, the parts of the rows' operand go to tensor memory and those of the other to
 // a second ring; one thread issues the products; eight warps add up what the accumulators hold and store the tiles. Bounded by shared memory: of a stage of 64 values of
 // depth, 128 x 128, it moves 64 KB in, 64 KB out, 48 KB of parts in and 96 KB of them to the tensor cores. (With the parts of both operands in shared memory
-// it was 416 KB, and 2.0 us for such a stage.) 16 384 rows of 8 groups, 1024 x 1024: 202 us (171 TFLOP/s, 1.02 P of bf16), gradients 195 and 265. Shallow products are bounded by memory and by the
-// number of tiles: 100 003 rows of 20 groups, 128 x 128: 33 us, of which a tile on every SM takes 4.1 (4.5 TB/s) and beginning and end 6.5.
+// it was 416 KB, and 2.0 us for such a stage.) 16 384 rows of 8 groups, 1024 x 1024: 209 us (164 TFLOP/s, 0.99 P of bf16), gradients 204 and 269. Shallow products are bounded by memory and by the
+// number of tiles: 100 003 rows of 20 groups, 128 x 128: 34 us, of which a tile on every SM takes 4.1 (4.5 TB/s) and beginning and end 6.5.
 #include <mutex>
 #include <set>
 

@@ -390,7 +390,7 @@ residual_norm_rows(T* __restrict__ stream, T* __restrict__ normed, const __grid_
 
 // Rows that a block shares and whose packs are whole: the rows of the inputs come into shared memory by bulk copies, kRing rows ahead, which
 // leaves registers for two blocks on an SM: while one waits at a barrier the other works. Bounded by memory: 16 384 rows of 4096 columns in bf16 take 110 to 119 us (670 MB, 5.6 to 6.1 TB/s),
-// backward 202 us (1.07 GB, 5.3 TB/s); 20 011 of 1000 in f32, a gate for each row, 55 and 83 us (5.8 and 6.1 TB/s). In registers alone the first took 287 and 438 us.
+// backward 206 us (1.07 GB, 5.2 TB/s); 20 011 of 1000 in f32, a gate for each row, 55 and 82 to 86 us (5.8 and 5.6 to 5.9 TB/s). In registers alone the first took 287 and 438 us.
 template <typename T, int kInputs, int kRing> struct RowRing {
     unsigned char* places;
     uint64_t* full;
