@@ -187,7 +187,7 @@ MOPS_EXPORT int mops_b200_get_wait(void);
  * which the kernels report unsorted or out-of-range indices are kept per (calling thread,
  * device, stream): calls that one thread issues on one stream run in order and share them
  * safely; calls on different streams, which may overlap on the GPU when wait == 0, each have
- * their own. Do not hand one thread's stream to mops_b200_set_stream of another thread while
+ * their own, and so has each graph that calls are captured into, for as long as it exists. Do not hand one thread's stream to mops_b200_set_stream of another thread while
  * asynchronous calls of both are in flight on it unless the application orders them itself. */
 
 /* ---- Plans: device tables built once and reused (no counterpart in the reference, which
