@@ -288,6 +288,40 @@ MOPS_EXPORT int mops_b200_cuda_gated_residual_norm_vjp(
     mops_b200_array_t branch, mops_b200_array_t gate, mops_b200_array_t scale, mops_b200_array_t weight_branch,
     mops_b200_array_t weight_output, double epsilon);
 
+/* The gated feed-forward layer of groups: W[g] holds the N columns of the gate, then those of the values (K x 2N), and
+ * output[r,j] = f(A[r,:] W[g,:,j]) * (A[r,:] W[g,:,N+j]) for the rows offsets[g] <= r < offsets[g+1] of group g; zeros for
+ * rows of no group. f is one of MOPS_B200_SILU (u sigmoid(u)) and MOPS_B200_GELU (u Phi(u), by the error function). Offsets and
+ * the ways W and grad_W may be stored: as of the grouped product. */
+enum { MOPS_B200_SILU = 0, MOPS_B200_GELU = 1 };
+MOPS_EXPORT int mops_b200_cuda_grouped_gated_product(mops_b200_array_t output, mops_b200_array_t A,
+                                                     mops_b200_array_t W, mops_b200_array_t offsets,
+                                                     int32_t activation);
+MOPS_EXPORT int mops_b200_cuda_grouped_gated_product_vjp(mops_b200_array_t grad_A, mops_b200_array_t grad_W,
+                                                         mops_b200_array_t grad_output, mops_b200_array_t A,
+                                                         mops_b200_array_t W, mops_b200_array_t offsets,
+                                                         int32_t activation);
+
+/* The cross entropy of a softmax over the rows of a table (V x C, as that of embedding_lookup), without the logits
+ * x[r,v] = scale * A[r,:] . W[v,:] (scale > 0) in memory:
+ * log_sum[r] = log sum_v exp(x[r,v]), loss[r] = log_sum[r] - x[r,targets[r]], in f32 (f64 for f64). A row whose target is ignore_index
+ * has zeros and no gradient, whatever stands in it; so has one whose target is no row of W, which is reported as an error. */
+MOPS_EXPORT int mops_b200_cuda_linear_cross_entropy(mops_b200_array_t loss, mops_b200_array_t log_sum,
+                                                    mops_b200_array_t A, mops_b200_array_t W,
+                                                    mops_b200_array_t targets, double scale, int64_t ignore_index);
+/* Gradients for those of loss and log_sum (an array of 0 dimensions: zeros); loss and log_sum are the forward call's. */
+MOPS_EXPORT int mops_b200_cuda_linear_cross_entropy_vjp(
+    mops_b200_array_t grad_A, mops_b200_array_t grad_W, mops_b200_array_t grad_loss, mops_b200_array_t grad_log_sum,
+    mops_b200_array_t loss, mops_b200_array_t log_sum, mops_b200_array_t A, mops_b200_array_t W,
+    mops_b200_array_t targets, double scale, int64_t ignore_index);
+
+/* norm[0] = the root of the sum of squares of all values of n contiguous arrays, whose types may differ. norm: one value, f64 if one of the
+ * arrays is, else f32. The squares are f32 products (f64 for f64), their sums f64 beyond a few hundred of them. */
+MOPS_EXPORT int mops_b200_cuda_gradient_norm(mops_b200_array_t norm, const mops_b200_array_t* gradients, int64_t n);
+/* outputs[i] = gradients[i] * max_norm / norm where norm > max_norm (>= 0), else gradients[i]; so they are where the norm is not finite. An output
+ * has the type and size of its gradient, and may be that gradient (which is then written only where it changes); other than that no two of the arrays overlap. */
+MOPS_EXPORT int mops_b200_cuda_clip_gradient_norm(mops_b200_array_t norm, const mops_b200_array_t* outputs,
+                                                  const mops_b200_array_t* gradients, int64_t n, double max_norm);
+
 /* Names (with template arguments) of the main kernels the calling thread's last mops_cuda_*
  * call dispatched to, "; "-separated; valid until that thread's next call. For tools that
  * pair a timing with the profile of the same kernel instantiation. */

@@ -19,8 +19,10 @@ Accepted arrays
 
 Beside the five operations stand the operators of the block around them, with gradients:
 ``embedding_lookup`` (a row of a table for every atom or token), ``grouped_matrix_product`` (a matrix for
-each group of rows) and ``gated_residual_norm`` (the residual connection with its gate and norms). They
-also take float16 and bfloat16.
+each group of rows), ``gated_residual_norm`` (the residual connection with its gate and norms),
+``grouped_gated_product`` (the gated feed-forward layer of each group) and ``linear_cross_entropy`` (the loss
+over a large table, without its logits); ``gradient_norm`` and ``clip_gradient_norm`` take all gradients of a
+model together. They also take float16 and bfloat16.
 
 Differences from the reference front end: no CuPy dispatch (CuPy is replaced by torch CUDA
 tensors); OPSAW and SASAW run on the GPU instead of raising "CUDA implementation does not
@@ -294,9 +296,10 @@ class _Arena:
                 ", float64, float16 and bfloat16" if half else " and float64") + " are supported")
         self.suffix = "f64" if self.dtype == torch.float64 else "f32"
 
-    def floats(self, x):
+    def floats(self, x, dtype=None):
+        """``dtype``: that of ``x``, if it is another one than the call's."""
         t = self.torch.from_numpy(np.ascontiguousarray(x)) if isinstance(x, np.ndarray) else x
-        if t.dtype != self.dtype:
+        if t.dtype != (dtype or self.dtype):
             raise TypeError("all floating-point arrays of one call must have the same dtype")
         if self.queue is not None and not t.is_cuda:
             dev, ready = self.queue.operand(t.contiguous())
@@ -320,14 +323,19 @@ class _Arena:
             return dev
         return t.to(self.device, non_blocking=True).to(self.torch.int32).contiguous()
 
-    def empty(self, shape):
-        shape = tuple(int(s) for s in shape)
+    def empty(self, shape, dtype=None):
+        shape, dtype = tuple(int(s) for s in shape), dtype or self.dtype
         if self.queue is not None:
             with self.torch.cuda.stream(self.queue.compute):
-                t = self.torch.empty(shape, dtype=self.dtype, device=self.device)
+                t = self.torch.empty(shape, dtype=dtype, device=self.device)
             self.queue._keep.append(t)
             return t
-        return self.torch.empty(shape, dtype=self.dtype, device=self.device)
+        return self.torch.empty(shape, dtype=dtype, device=self.device)
+
+    @property
+    def sum_dtype(self):
+        """Of results that are not rounded to 16 bits."""
+        return self.torch.float64 if self.dtype == self.torch.float64 else self.torch.float32
 
     def back(self, t):
         """Result to where the inputs live. Pinned host inputs get pinned host results (from
@@ -774,3 +782,120 @@ def gated_residual_norm_vjp(grad_stream, grad_normed, residual, branch, gate, sc
     gradients = [None if x is None else m.empty(x.shape) for x in inputs]
     m.run_arrays(op, *gradients, m.rows(grad_stream), m.rows(grad_normed), *inputs, ctypes.c_double(epsilon))
     return tuple(m.back(x) for x in gradients)
+
+
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _activation(name, operation):
+    if name not in _ACTIVATIONS:
+        raise ValueError(f"`activation` must be one of {', '.join(_ACTIVATIONS)} in {operation}, got {name!r}")
+    return ctypes.c_int32(_ACTIVATIONS[name])
+
+
+def grouped_gated_product(A, W, offsets, activation="silu"):
+    """The gated feed-forward layer of groups of rows. ``W[g]`` holds the N columns of the gate, then those of the
+    values: ``output[r,:] = f(A[r,:] @ W[g][:, :N]) * (A[r,:] @ W[g][:, N:])`` for the rows
+    ``offsets[g] <= r < offsets[g+1]`` of group g; zeros for rows of no group. ``activation``: ``"silu"`` or ``"gelu"``
+    (by the error function)."""
+    op = "grouped_gated_product"
+    _grouped_common(op, A, W, offsets)
+    f = _activation(activation, op)
+    m = _Arena(A, half=True)
+    A_, W_, o_ = m.rows(A), m.rows(W), m.ints(offsets)
+    out = m.empty((A_.shape[0], W_.shape[2] // 2))
+    m.run_arrays(op, out, A_, W_, o_, f)
+    return m.back(out)
+
+
+def grouped_gated_product_vjp(grad_output, A, W, offsets, activation="silu", compute_grad_A=True, compute_grad_W=True):
+    op = "grouped_gated_product_vjp"
+    _check(grad_output, 2, "f", op, "grad_output")
+    _grouped_common(op, A, W, offsets)
+    f = _activation(activation, op)
+    m = _Arena(A, half=True)
+    g_, A_, W_, o_ = m.rows(grad_output), m.rows(A), m.rows(W), m.ints(offsets)
+    gA = m.empty(A_.shape) if compute_grad_A else None
+    gW = m.empty(W_.shape) if compute_grad_W else None
+    m.run_arrays(op, gA, gW, g_, A_, W_, o_, f)
+    return m.back(gA), m.back(gW)
+
+
+def _loss_check(op, A, W, targets, scale, ignore_index):
+    _check(A, 2, "f", op, "A"); _check(W, 2, "f", op, "W"); _check(targets, 1, "i", op, "targets")
+    _check_real(scale, op, "scale"); _check_scalar(ignore_index, op, "ignore_index")
+
+
+def linear_cross_entropy(A, W, targets, scale=1.0, ignore_index=-1):
+    """The cross entropy of a softmax over the rows of a table, whose logits ``x = scale * A @ W.T`` are not kept: returns
+    ``loss[r] = log_sum[r] - x[r, targets[r]]`` and ``log_sum[r] = log(sum(exp(x[r])))``, float32 (float64 for
+    float64). Rows whose target is ``ignore_index`` have zeros and no gradient, whatever stands in them."""
+    op = "linear_cross_entropy"
+    _loss_check(op, A, W, targets, scale, ignore_index)
+    m = _Arena(A, half=True)
+    A_, W_, t_ = m.rows(A), m.rows(W), m.ints(targets)
+    loss, log_sum = (m.empty((A_.shape[0],), m.sum_dtype) for _ in range(2))
+    m.run_arrays(op, loss, log_sum, A_, W_, t_, ctypes.c_double(scale), ctypes.c_int64(ignore_index))
+    return m.back(loss), m.back(log_sum)
+
+
+def linear_cross_entropy_vjp(grad_loss, grad_log_sum, loss, log_sum, A, W, targets, scale=1.0, ignore_index=-1,
+                             compute_grad_A=True, compute_grad_W=True):
+    """Gradients of (A, W). ``loss`` and ``log_sum`` are the results of the forward call; ``grad_loss`` or ``grad_log_sum``
+    may be None (zeros)."""
+    op = "linear_cross_entropy_vjp"
+    for g, name in ((grad_loss, "grad_loss"), (grad_log_sum, "grad_log_sum"), (loss, "loss"), (log_sum, "log_sum")):
+        if g is not None or name in ("loss", "log_sum"):
+            _check(g, 1, "f", op, name)
+    _loss_check(op, A, W, targets, scale, ignore_index)
+    m = _Arena(A, half=True)
+    given = [None if g is None else m.floats(g, m.sum_dtype) for g in (grad_loss, grad_log_sum, loss, log_sum)]
+    A_, W_, t_ = m.rows(A), m.rows(W), m.ints(targets)
+    gA = m.empty(A_.shape) if compute_grad_A else None
+    gW = m.empty(W_.shape) if compute_grad_W else None
+    m.run_arrays(op, gA, gW, *given, A_, W_, t_, ctypes.c_double(scale), ctypes.c_int64(ignore_index))
+    return m.back(gA), m.back(gW)
+
+
+def _gradients(op, gradients):
+    gradients = list(gradients)
+    if not gradients:
+        raise ValueError(f"no gradients in {op}")
+    for g in gradients:
+        if not _is_array(g):
+            raise TypeError(f"`gradients` must be arrays in {op}, got {type(g)}")
+        if not _is_floating(g):
+            raise TypeError(f"Wrong dtype for gradients in {op}: got {_dtype_name(g)}")
+    m = _Arena(gradients[0], half=True)
+    torch = _torch()
+    on_device = []
+    for g in gradients:
+        if _Arena(g, half=True).host != m.host:
+            raise TypeError(f"`gradients` must all be host arrays or all be on the device in {op}")
+        on_device.append(m.floats(g, getattr(torch, _dtype_name(g))))
+    wide = any(t.dtype == torch.float64 for t in on_device)
+    return m, on_device, m.empty((1,), torch.float64 if wide else torch.float32)
+
+
+def _table(tensors):
+    return (_lib.Array * len(tensors))(*[_lib.make_array(t.data_ptr(), _dtype_name(t), (t.numel(),), (1,)) for t in tensors])
+
+
+def gradient_norm(gradients):
+    """The root of the sum of squares of all values of a list of arrays, whose types may differ: one value, float32 (float64
+    if one of the arrays is)."""
+    op = "gradient_norm"
+    m, tensors, norm = _gradients(op, gradients)
+    m.run_arrays(op, norm, _table(tensors), ctypes.c_int64(len(tensors)))
+    return m.back(norm)[0]
+
+
+def clip_gradient_norm(gradients, max_norm):
+    """Returns the norm of all gradients together and the list of them, scaled to ``max_norm`` where the norm is larger. They are
+    copied as they are where the norm is not finite."""
+    op = "clip_gradient_norm"
+    _check_real(max_norm, op, "max_norm")
+    m, tensors, norm = _gradients(op, gradients)
+    clipped = [m.empty(t.shape, t.dtype) for t in tensors]
+    m.run_arrays(op, norm, _table(clipped), _table(tensors), ctypes.c_int64(len(tensors)), ctypes.c_double(max_norm))
+    return m.back(norm)[0], [m.back(t) for t in clipped]

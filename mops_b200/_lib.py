@@ -35,7 +35,10 @@ EXTENSION_SYMBOLS = ("mops_b200_set_stream", "mops_b200_get_stream", "mops_b200_
                      "mops_b200_cuda_sparse_accumulation_scatter_add_with_weights_noalloc_f64",
                      "mops_b200_cuda_embedding_lookup", "mops_b200_cuda_embedding_lookup_vjp",
                      "mops_b200_cuda_grouped_matrix_product", "mops_b200_cuda_grouped_matrix_product_vjp",
-                     "mops_b200_cuda_gated_residual_norm", "mops_b200_cuda_gated_residual_norm_vjp")
+                     "mops_b200_cuda_gated_residual_norm", "mops_b200_cuda_gated_residual_norm_vjp",
+                     "mops_b200_cuda_grouped_gated_product", "mops_b200_cuda_grouped_gated_product_vjp",
+                     "mops_b200_cuda_linear_cross_entropy", "mops_b200_cuda_linear_cross_entropy_vjp",
+                     "mops_b200_cuda_gradient_norm", "mops_b200_cuda_clip_gradient_norm")
 
 
 class MopsError(Exception):

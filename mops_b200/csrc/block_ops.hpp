@@ -22,6 +22,16 @@ void gated_residual_norm_vjp(Array grad_residual, Array grad_branch, Array grad_
                              Array residual, Array branch, Array gate, Array scale, Array weight_branch,
                              Array weight_output, double epsilon);
 
+void grouped_gated_product(Array output, Array A, Array W, Array offsets, int32_t activation);
+void grouped_gated_product_vjp(Array grad_A, Array grad_W, Array grad_output, Array A, Array W, Array offsets, int32_t activation);
+
+void linear_cross_entropy(Array loss, Array log_sum, Array A, Array W, Array targets, double scale, int64_t ignore_index);
+void linear_cross_entropy_vjp(Array grad_A, Array grad_W, Array grad_loss, Array grad_log_sum, Array loss, Array log_sum, Array A, Array W,
+                              Array targets, double scale, int64_t ignore_index);
+
+void gradient_norm(Array norm, const Array* gradients, int64_t n);
+void clip_gradient_norm(Array norm, const Array* outputs, const Array* gradients, int64_t n, double max_norm);
+
 } // namespace mops_b200
 
 #endif

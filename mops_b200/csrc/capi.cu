@@ -190,6 +190,22 @@ BLOCK_ENTRY(gated_residual_norm_vjp,
             grad_residual, grad_branch, grad_gate, grad_scale, grad_weight_branch, grad_weight_output, grad_stream,
             grad_normed, residual, branch, gate, scale, weight_branch, weight_output, epsilon)
 
+BLOCK_ENTRY(grouped_gated_product, (Array output, Array A, Array W, Array offsets, int32_t activation), output, A, W, offsets,
+            activation)
+BLOCK_ENTRY(grouped_gated_product_vjp,
+            (Array grad_A, Array grad_W, Array grad_output, Array A, Array W, Array offsets, int32_t activation), grad_A,
+            grad_W, grad_output, A, W, offsets, activation)
+BLOCK_ENTRY(linear_cross_entropy,
+            (Array loss, Array log_sum, Array A, Array W, Array targets, double scale, int64_t ignore_index), loss, log_sum, A,
+            W, targets, scale, ignore_index)
+BLOCK_ENTRY(linear_cross_entropy_vjp,
+            (Array grad_A, Array grad_W, Array grad_loss, Array grad_log_sum, Array loss, Array log_sum, Array A, Array W,
+             Array targets, double scale, int64_t ignore_index),
+            grad_A, grad_W, grad_loss, grad_log_sum, loss, log_sum, A, W, targets, scale, ignore_index)
+BLOCK_ENTRY(gradient_norm, (Array norm, const Array* gradients, int64_t n), norm, gradients, n)
+BLOCK_ENTRY(clip_gradient_norm, (Array norm, const Array* outputs, const Array* gradients, int64_t n, double max_norm), norm,
+            outputs, gradients, n, max_norm)
+
 extern "C" int mops_b200_plan_create(mops_b200_plan_t** plan) {
     return guarded([&] {
         if (plan == nullptr) throw std::runtime_error("mops_b200_plan_create: plan is NULL");

@@ -1,0 +1,368 @@
+// linear_cross_entropy: the cross entropy of a softmax over the rows of a table, without the logits.
+//
+//   x[r,v] = scale A[r,:] . W[v,:]
+//   log_sum[r] = log sum_v exp(x[r,v]), loss[r] = log_sum[r] - x[r,t_r]
+//   dx[r,v] = (grad_loss[r] + grad_log_sum[r]) exp(x[r,v] - log_sum[r]) - grad_loss[r] [v = t_r]
+//   grad_A = scale dx W, grad_W = scale dx^T A
+//
+// A piece of the vocabulary at a time: its logits are a product into scratch memory, of which sums are taken, or which become dx where they stand and are multiplied by the
+// piece's rows of W and, the other way, by A. The gradients compute the logits again. Here: f32 and f64; f16 and bf16 are widened to f32.
+#include "block_ops.hpp"
+#include "convert.cuh"
+#include "grouped_mma.hpp"
+#include "loss_rows.cuh"
+#include "pack.hpp"
+
+namespace mops_b200 {
+namespace {
+
+constexpr int kPrepareThreads = 1024, kPrepareRows = 8;
+constexpr int64_t kPartColumns = 4096;             // of a part of a row's sums, at most
+constexpr int64_t kMostLogits = int64_t(64) << 20; // of a piece
+
+// Numbers the rows that have a target, by one block; the others get zeros, if loss is given.
+template <typename S>
+__global__ void __launch_bounds__(kPrepareThreads)
+loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, const int32_t* __restrict__ targets, int64_t rows, int64_t vocabulary,
+             int64_t ignored, Status st) {
+    __shared__ int of_warp[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int before = 0;
+    bool bad = false;
+    for (int64_t r0 = 0; r0 < rows; r0 += kPrepareThreads * kPrepareRows) {
+        const int64_t r = r0 + static_cast<int64_t>(threadIdx.x) * kPrepareRows;
+        unsigned keep = 0;
+#pragma unroll
+        for (int k = 0; k < kPrepareRows; k++)
+            if (r + k < rows) {
+                const int64_t t = targets[r + k];
+                const bool in = t >= 0 && t < vocabulary && t != ignored;
+                keep |= static_cast<unsigned>(in) << k;
+                bad |= !in && t != ignored;
+            }
+        const int own = __popc(keep);
+        int up_to = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(kFullMask, up_to, d);
+            if (lane >= d) up_to += v;
+        }
+        if (lane == 31) of_warp[warp] = up_to;
+        __syncthreads();
+        int all = of_warp[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(kFullMask, all, d);
+            if (lane >= d) all += v;
+        }
+        const int in_front = __shfl_sync(kFullMask, all, (warp + 31) & 31), total = __shfl_sync(kFullMask, all, 31);
+        int i = before + up_to - own + (warp > 0 ? in_front : 0);
+#pragma unroll
+        for (int k = 0; k < kPrepareRows; k++)
+            if (r + k < rows) {
+                const bool in = keep >> k & 1;
+                to.place[r + k] = in ? i : -1;
+                if (in) to.order[i++] = static_cast<int32_t>(r + k);
+                else if (loss != nullptr) loss[r + k] = log_sum[r + k] = S(0);
+            }
+        before += total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) to.offsets[0] = 0, to.offsets[1] = before;
+    if (bad) report_bad_index(st, 0);
+}
+
+// to[i,:] = from[order[i],:]
+template <typename To, typename From>
+__global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
+loss_gather(To* __restrict__ to, int64_t to_stride, const From* __restrict__ from, int64_t stride, const LossRows rows, int64_t columns) {
+    const int64_t kept = rows.offsets[1];
+    for (int64_t i = first_row(); i < kept; i += row_step()) {
+        const int64_t r = rows.order[i];
+        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[i * to_stride + c] = convert<To>(from[r * stride + c]);
+    }
+}
+
+// to[r,:] = from[place[r],:], zeros for rows that have no place
+template <typename To, typename From>
+__global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
+loss_scatter(To* __restrict__ to, const From* __restrict__ from, const LossRows rows, int64_t n, int64_t columns) {
+    for (int64_t r = first_row(); r < n; r += row_step()) {
+        const int64_t i = rows.place[r];
+        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[r * columns + c] = i >= 0 ? convert<To>(from[i * columns + c]) : To(0);
+    }
+}
+
+template <typename S>
+__global__ void __launch_bounds__(256)
+add_values(S* __restrict__ to, const S* __restrict__ from, int64_t n) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) to[i] += from[i];
+}
+
+// The sums of parts of `part` columns of a piece's logits. A block to a part.
+template <typename S>
+__global__ void __launch_bounds__(256)
+loss_sums(PartSum<S>* __restrict__ parts, int64_t n, int64_t first_part, S* __restrict__ at_target, const S* __restrict__ logits, int64_t columns, S scale,
+          const int32_t* __restrict__ targets, int64_t first_column, int64_t part, const LossRows rows) {
+    __shared__ PartSum<S> of_warp[8];
+    const int64_t i = blockIdx.x, c0 = static_cast<int64_t>(blockIdx.y) * part;
+    if (i >= rows.offsets[1]) return;
+    const S* x = logits + i * columns;
+    const int64_t end = min(c0 + part, columns);
+    S top = -S(INFINITY);
+    for (int64_t c = c0 + threadIdx.x; c < end; c += 256) top = fmax(top, scale * x[c]);
+    const S base = PartSum<S>::from(top);
+    S sum = 0;
+    for (int64_t c = c0 + threadIdx.x; c < end; c += 256) sum += exp(scale * x[c] - base);
+    PartSum<S> all{top, sum};
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        PartSum<S> other;
+        other.top = __shfl_down_sync(kFullMask, all.top, d);
+        other.sum = __shfl_down_sync(kFullMask, all.sum, d);
+        all.join(other);
+    }
+    if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = all;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 8; w++) all.join(of_warp[w]);
+    parts[i * n + first_part + blockIdx.y] = all;
+    const int64_t t = targets[rows.order[i]] - first_column;
+    if (t >= c0 && t < end) at_target[i] = scale * x[t];
+}
+
+// The logits of a piece become scale dx.
+template <typename S>
+__global__ void __launch_bounds__(256)
+loss_gradient(S* __restrict__ logits, int64_t columns, S scale, const S* __restrict__ grad_loss, const S* __restrict__ grad_log_sum,
+              const S* __restrict__ log_sum, const int32_t* __restrict__ targets, int64_t first_column, int64_t part, const LossRows rows) {
+    const int64_t i = blockIdx.x, c0 = static_cast<int64_t>(blockIdx.y) * part;
+    if (i >= rows.offsets[1]) return;
+    const int64_t r = rows.order[i], t = targets[r] - first_column;
+    const S of_loss = grad_loss != nullptr ? grad_loss[r] : S(0), of_sum = grad_log_sum != nullptr ? grad_log_sum[r] : S(0);
+    const S both = (of_loss + of_sum) * scale, base = log_sum[r];
+    S* x = logits + i * columns;
+    for (int64_t c = c0 + threadIdx.x; c < min(c0 + part, columns); c += 256) {
+        S d = both * exp(scale * x[c] - base);
+        if (c == t) d -= of_loss * scale;
+        x[c] = d;
+    }
+}
+
+const char* const kIndexNames[] = {"targets"};
+
+// Sizes and types; the results have the type of sums.
+void check_loss(Array& A, Array& W, Array& targets, Array& loss, Array& log_sum, double scale, const std::string& op) {
+    check_floating(A.type, "A", op);
+    check_array(A, "A", 2, A.type, op);
+    check_array(W, "W", 2, A.type, op);
+    check_array(targets, "targets", 1, MOPS_B200_I32, op);
+    const int32_t sums = A.type == MOPS_B200_F64 ? MOPS_B200_F64 : MOPS_B200_F32;
+    check_array(loss, "loss", 1, sums, op);
+    check_array(log_sum, "log_sum", 1, sums, op);
+    check_size(A.shape[1], "A", 1, W.shape[1], "W", 1, op);
+    check_size(targets.shape[0], "targets", 0, A.shape[0], "A", 0, op);
+    check_size(loss.shape[0], "loss", 0, A.shape[0], "A", 0, op);
+    check_size(log_sum.shape[0], "log_sum", 0, A.shape[0], "A", 0, op);
+    check_rows(A, "A", op);
+    check_rows(W, "W", op);
+    check_rows(targets, "targets", op);
+    check_output(loss, "loss", op);
+    check_output(log_sum, "log_sum", op);
+    if (W.shape[0] == 0) throw std::runtime_error("W must have a row in " + op);
+    if (!(scale > 0) || std::isinf(scale)) throw std::runtime_error("scale must be positive and finite in " + op);
+    for (int64_t n : {A.shape[0], A.shape[1], W.shape[0]}) fits_int32(static_cast<size_t>(n), "a size", op);
+}
+
+LossRows take_rows(Scratch& room, int64_t rows) {
+    room.take(static_cast<size_t>(2 * rows + 4) * sizeof(int32_t));
+    int32_t* p = room.as<int32_t>();
+    return {p, p + 4, p + 4 + rows};
+}
+
+unsigned blocks_for(const Call& call, int64_t n) {
+    return static_cast<unsigned>(std::min<int64_t>(ceil_div(n, 256), int64_t(sm_count(call.device)) * 16));
+}
+
+// What forward and backward share: the rows that count, gathered and as the products want them, W likewise, and the logits of a piece.
+template <typename S> struct Pieces {
+    const Call& call;
+    const std::string& op;
+    Scratch room_rows, room_A, room_W, room_logits;
+    Packing packing;
+    LossRows rows;
+    Array A, W, logits;
+    int64_t width, part; // columns of a piece, and of a part of it
+    static constexpr int32_t kType = sizeof(S) == 8 ? MOPS_B200_F64 : MOPS_B200_F32;
+
+    Pieces(const Call& call, const std::string& op, const Array& a, const Array& w)
+        : call(call), op(op), room_rows(call), room_A(call), room_W(call), room_logits(call), packing(call), W(w) {
+        const int64_t n = a.shape[0], columns = a.shape[1];
+        rows = take_rows(room_rows, n);
+        room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
+        A = contiguous(room_A.as<void>(), kType, n, columns);
+        if (w.type != kType) {
+            room_W.take(static_cast<size_t>(values_of(w)) * sizeof(S) + 16);
+            W = converted(call, w, room_W.as<S>(), kType);
+        }
+        width = std::max<int64_t>(kMostLogits / n, 256);
+        width = width >= kPartColumns ? width / kPartColumns * kPartColumns : width / 256 * 256;
+        part = std::min(width, kPartColumns);
+        width = std::min(width, W.shape[0]);
+        room_logits.take(static_cast<size_t>(n * width) * sizeof(S) + 16);
+    }
+    void gather(const Array& a) {
+        if (a.shape[1] == 0) return;
+        for_type(a.type, [&](auto zero) {
+            using From = decltype(zero);
+            loss_gather<S, From><<<row_blocks(call, a.shape[0]), row_threads(), 0, call.stream>>>(
+                static_cast<S*>(A.data), a.shape[1], static_cast<const From*>(a.data), a.stride[0], rows, a.shape[1]);
+        });
+        MOPS_CUDA_OK(cudaGetLastError());
+        if (kType == MOPS_B200_F32 && !straight_rows(matrices(0, W.shape[0]), A.shape[0], false)) {
+            packing.add(A);
+            packing.add(W);
+            packing.run();
+        }
+    }
+    // The rows v0 .. v1 of W as the single group's matrix, C x (v1 - v0).
+    Array matrices(int64_t v0, int64_t v1) const {
+        Array m = contiguous(static_cast<S*>(W.data) + v0 * W.stride[0], kType, 1, W.shape[1], v1 - v0);
+        m.stride[1] = 1, m.stride[2] = W.stride[0];
+        return m;
+    }
+    template <typename F> void for_each(F&& f) {
+        for (int64_t v0 = 0; v0 < W.shape[0]; v0 += width) {
+            const int64_t v1 = std::min(v0 + width, W.shape[0]);
+            const Array m = matrices(v0, v1);
+            logits = contiguous(room_logits.as<void>(), kType, A.shape[0], v1 - v0);
+            multiply_rows(call, {logits, A, m, m.stride[1], m.stride[2], rows.offsets, 1, A.shape[0], A.shape[1], v1 - v0}, op);
+            const dim3 grid(static_cast<unsigned>(A.shape[0]), static_cast<unsigned>(ceil_div(v1 - v0, part)));
+            f(v0, v1, grid, static_cast<S*>(logits.data));
+            MOPS_CUDA_OK(cudaGetLastError());
+        }
+    }
+};
+
+template <typename S>
+void loss_forward(const Call& call, const Array& loss, const Array& log_sum, const Array& A, const Array& W, const Array& targets, double scale,
+                  int64_t ignored, const std::string& op) {
+    Pieces<S> pieces(call, op, A, W);
+    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.part);
+    const int32_t* t = static_cast<const int32_t*>(targets.data);
+    loss_prepare<S><<<1, kPrepareThreads, 0, call.stream>>>(pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), t, n, W.shape[0], ignored,
+                                                            call.status);
+    pieces.gather(A);
+    Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<S>) + static_cast<size_t>(n) * sizeof(S));
+    PartSum<S>* sums = room.as<PartSum<S>>();
+    S* at_target = reinterpret_cast<S*>(sums + n * parts);
+    pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
+        loss_sums<S><<<grid, 256, 0, call.stream>>>(sums, parts, v0 / pieces.part, at_target, logits, v1 - v0, static_cast<S>(scale), t, v0, pieces.part,
+                                                     pieces.rows);
+    });
+    loss_join<S><<<static_cast<unsigned>(n), 128, 0, call.stream>>>(static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), sums, parts, at_target, pieces.rows);
+    MOPS_CUDA_OK(cudaGetLastError());
+    note_kernel_f("loss_sums<%s>", scalar_name<S>());
+}
+
+template <typename S>
+void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, const Array& grad_loss, const Array& grad_log_sum, const Array& log_sum,
+                   const Array& A, const Array& W, const Array& targets, double scale, int64_t ignored, const std::string& op) {
+    Pieces<S> pieces(call, op, A, W);
+    const int64_t n = A.shape[0], columns = A.shape[1];
+    const int32_t* t = static_cast<const int32_t*>(targets.data);
+    loss_prepare<S><<<1, kPrepareThreads, 0, call.stream>>>(pieces.rows, static_cast<S*>(nullptr), static_cast<S*>(nullptr), t, n, W.shape[0], ignored, call.status);
+    if (columns == 0) return;
+    pieces.gather(A);
+    const bool need_A = grad_A.data != nullptr, need_W = grad_W.data != nullptr, widened = A.type != pieces.kType;
+    Scratch room_A(call), room_more(call), room_W(call);
+    const size_t bytes = static_cast<size_t>(n * columns) * sizeof(S);
+    if (need_A) room_A.take(bytes);
+    if (need_A && pieces.width < W.shape[0]) room_more.take(bytes);
+    if (need_W && widened) room_W.take(static_cast<size_t>(pieces.width * columns) * sizeof(S));
+    pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
+        loss_gradient<S><<<grid, 256, 0, call.stream>>>(logits, v1 - v0, static_cast<S>(scale), static_cast<const S*>(grad_loss.data),
+                                                        static_cast<const S*>(grad_log_sum.data), static_cast<const S*>(log_sum.data), t, v0, pieces.part, pieces.rows);
+        Array m = pieces.matrices(v0, v1), dx = pieces.logits, a = pieces.A;
+        m.shape[1] = v1 - v0, m.shape[2] = columns; // (v1 - v0) x C
+        std::swap(m.stride[1], m.stride[2]);
+        Packing packing(call);
+        if (pieces.kType == MOPS_B200_F32) {
+            const bool rows_packed = need_A && !straight_rows(m, n, true), outer_packed = need_W && !straight_outer(n, 1, v1 - v0, columns, pieces.kType);
+            if (rows_packed || outer_packed) packing.add(dx);
+            if (rows_packed) packing.add(m);
+            if (outer_packed) packing.add(a);
+            packing.run();
+        }
+        if (need_A) {
+            S* to = v0 == 0 ? room_A.as<S>() : room_more.as<S>();
+            multiply_rows(call, {contiguous(to, pieces.kType, n, columns), dx, m, m.stride[1], 1, pieces.rows.offsets, 1, n, v1 - v0, columns}, op);
+            if (v0 > 0) add_values<S><<<blocks_for(call, n * columns), 256, 0, call.stream>>>(room_A.as<S>(), to, n * columns);
+        }
+        if (need_W) {
+            char* to = static_cast<char*>(grad_W.data) + v0 * columns * type_bytes(grad_W.type);
+            const Array part = contiguous(widened ? room_W.as<void>() : to, pieces.kType, 1, v1 - v0, columns);
+            multiply_outer(call, {part, dx, a, pieces.rows.offsets, 1}, op);
+            if (widened)
+                for_type(grad_W.type, [&](auto zero) {
+                    using T = decltype(zero);
+                    (void)converted(call, part, reinterpret_cast<T*>(to), grad_W.type);
+                });
+        }
+        packing.release();
+    });
+    if (need_A)
+        for_type(grad_A.type, [&](auto zero) {
+            using T = decltype(zero);
+            loss_scatter<T, S><<<row_blocks(call, n), row_threads(), 0, call.stream>>>(static_cast<T*>(grad_A.data), room_A.as<S>(), pieces.rows, n, columns);
+        });
+    MOPS_CUDA_OK(cudaGetLastError());
+    note_kernel_f("loss_gradient<%s>", scalar_name<S>());
+}
+
+} // namespace
+
+void linear_cross_entropy(Array loss, Array log_sum, Array A, Array W, Array targets, double scale, int64_t ignore_index) {
+    const std::string op = "cuda_linear_cross_entropy";
+    check_loss(A, W, targets, loss, log_sum, scale, op);
+    if (A.shape[0] == 0) return;
+    Call call = begin_call();
+    if (A.type == MOPS_B200_F64) loss_forward<double>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
+    else loss_forward<float>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
+    end_call(call, op.c_str(), kIndexNames, 1);
+}
+
+void linear_cross_entropy_vjp(Array grad_A, Array grad_W, Array grad_loss, Array grad_log_sum, Array loss, Array log_sum, Array A, Array W,
+                              Array targets, double scale, int64_t ignore_index) {
+    const std::string op = "cuda_linear_cross_entropy_vjp";
+    check_loss(A, W, targets, loss, log_sum, scale, op);
+    auto given = [&](Array& g, const char* name) {
+        if (g.data == nullptr && g.dimensions == 0) return;
+        check_array(g, name, 1, loss.type, op);
+        check_size(g.shape[0], name, 0, A.shape[0], "A", 0, op);
+        check_output(g, name, op);
+    };
+    given(grad_loss, "grad_loss");
+    given(grad_log_sum, "grad_log_sum");
+    auto wanted = [&](Array& g, const char* name, const Array& of, const char* of_name) {
+        if (g.data == nullptr) return;
+        check_array(g, name, 2, A.type, op);
+        for (int d = 0; d < 2; d++) check_size(g.shape[d], name, d, of.shape[d], of_name, d, op);
+        check_output(g, name, op);
+    };
+    wanted(grad_A, "grad_A", A, "A");
+    wanted(grad_W, "grad_W", W, "W");
+    if (grad_A.data == nullptr && grad_W.data == nullptr) return;
+    Call call = begin_call();
+    if (A.shape[0] == 0) {
+        if (grad_W.data != nullptr)
+            MOPS_CUDA_OK(cudaMemsetAsync(grad_W.data, 0, static_cast<size_t>(values_of(grad_W) * type_bytes(grad_W.type)), call.stream));
+    } else if (A.type == MOPS_B200_F64) {
+        loss_backward<double>(call, grad_A, grad_W, grad_loss, grad_log_sum, log_sum, A, W, targets, scale, ignore_index, op);
+    } else {
+        loss_backward<float>(call, grad_A, grad_W, grad_loss, grad_log_sum, log_sum, A, W, targets, scale, ignore_index, op);
+    }
+    end_call(call, op.c_str(), kIndexNames, 1);
+}
+
+} // namespace mops_b200

@@ -1,0 +1,199 @@
+// grouped_gated_product: the gated feed-forward layer of groups of rows. W[g] holds the N columns of the gate and, behind them, those of the values.
+//
+//   U = A[r,:] W[g][:, :N], V = A[r,:] W[g][:, N:]       for offsets[g] <= r < offsets[g+1]
+//   output[r,:] = f(U) V
+//   dV = grad_output f(U), dU = grad_output V f'(U)
+//   grad_A[r,:] = [dU dV] W[g]^T, grad_W[g] = A[rows of g]^T [dU dV]
+//
+// Here: f32 and f64. U and V, side by side in scratch memory, are one grouped product; a pass over them makes the output of them, or, where
+// they stood, dU and dV, of which the gradients are the grouped products that they are for a plain layer. f16 and bf16 are widened to f32 for that, so U, V, dU and dV are never
+// rounded to 16 bits.
+#include "activation.cuh"
+#include "block_ops.hpp"
+#include "convert.cuh"
+#include "grouped_mma.hpp"
+#include "pack.hpp"
+
+namespace mops_b200 {
+namespace {
+
+// out[r,j] = f(u) v
+template <int kActivation, typename T, typename S>
+__global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
+gate_rows(T* __restrict__ out, const S* __restrict__ uv, int64_t rows, int64_t columns) {
+    for (int64_t r = first_row(); r < rows; r += row_step())
+        for (int64_t j = threadIdx.x; j < columns; j += kRowThreads) {
+            const S u = uv[r * 2 * columns + j], v = uv[r * 2 * columns + columns + j];
+            out[r * columns + j] = narrow<T>(Gate<kActivation, S>(u).value * v);
+        }
+}
+
+// u, v become dU, dV
+template <int kActivation, typename T, typename S>
+__global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
+gate_rows_vjp(S* __restrict__ uv, const T* __restrict__ grad, int64_t grad_stride, int64_t rows, int64_t columns) {
+    for (int64_t r = first_row(); r < rows; r += row_step())
+        for (int64_t j = threadIdx.x; j < columns; j += kRowThreads) {
+            S *u = uv + r * 2 * columns + j, *v = u + columns;
+            const Gate<kActivation, S> gate(*u);
+            const S g = widen(grad[r * grad_stride + j]);
+            *u = g * *v * gate.slope;
+            *v = g * gate.value;
+        }
+}
+
+template <typename F> void for_activation(int32_t activation, F&& f) {
+    if (activation == MOPS_B200_SILU) f(std::integral_constant<int, MOPS_B200_SILU>());
+    else f(std::integral_constant<int, MOPS_B200_GELU>());
+}
+
+const char* const kIndexNames[] = {"offsets"};
+
+void check_gated(Array& A, Array& W, Array& offsets, Array& rows, const char* rows_name, int32_t activation, const std::string& op) {
+    check_floating(A.type, "A", op);
+    check_array(A, "A", 2, A.type, op);
+    check_array(W, "W", 3, A.type, op);
+    check_array(rows, rows_name, 2, A.type, op);
+    check_array(offsets, "offsets", 1, MOPS_B200_I32, op);
+    check_size(A.shape[1], "A", 1, W.shape[1], "W", 1, op);
+    check_size(rows.shape[0], rows_name, 0, A.shape[0], "A", 0, op);
+    if (W.shape[2] % 2 != 0) throw std::runtime_error("W must have as many columns for the gate as for the values, an even number in all, in " + op);
+    check_size(rows.shape[1], rows_name, 1, W.shape[2] / 2, "one half of W", 2, op);
+    check_size(offsets.shape[0], "offsets", 0, W.shape[0] + 1, "the groups of W (and one)", 0, op);
+    check_rows(A, "A", op);
+    check_matrices(W, "W", op);
+    if (offsets.stride[0] != 1) throw std::runtime_error("offsets must be contiguous in " + op);
+    for (int64_t n : {A.shape[0], A.shape[1], W.shape[0], W.shape[2]}) fits_int32(static_cast<size_t>(n), "a size", op);
+    if (activation != MOPS_B200_SILU && activation != MOPS_B200_GELU)
+        throw std::runtime_error("unknown activation " + std::to_string(activation) + " in " + op);
+}
+
+// In f32 (f64 for f64), what the products are made of: A and W, widened where they have 16 bits, and U and V side by side.
+struct Widened {
+    Scratch room_A, room_W, room_uv;
+    Packing packing;
+    Array A, W, uv;
+    int32_t type;
+    Widened(const Call& call, const Array& a, const Array& w, const int32_t* offsets, const std::string& op)
+        : room_A(call), room_W(call), room_uv(call), packing(call), A(a), W(w), type(a.type == MOPS_B200_F64 ? MOPS_B200_F64 : MOPS_B200_F32) {
+        if (type != a.type) {
+            room_A.take(static_cast<size_t>(values_of(a)) * 4 + 16);
+            room_W.take(static_cast<size_t>(values_of(w)) * 4 + 16);
+            A = converted(call, a, room_A.as<float>(), type);
+            W = converted(call, w, room_W.as<float>(), type);
+        }
+        if (type == MOPS_B200_F32 && W.shape[0] > 0 && W.shape[1] > 0 && !straight_rows(W, A.shape[0], W.stride[2] == 1)) {
+            packing.add(A);
+            packing.add(W);
+            packing.run();
+        }
+        room_uv.take(static_cast<size_t>(A.shape[0] * W.shape[2] * type_bytes(type)) + 16);
+        uv = contiguous(room_uv.as<void>(), type, A.shape[0], W.shape[2]);
+        multiply_rows(call, {uv, A, W, W.stride[1], W.stride[2], offsets, W.shape[0], A.shape[0], A.shape[1], W.shape[2]}, op);
+    }
+};
+
+// f(T(), S()) with T the type and S that of sums
+template <typename F> void for_types(int32_t type, F&& f) {
+    for_type(type, [&](auto zero) { f(zero, Sum<decltype(zero)>()); });
+}
+
+} // namespace
+
+void grouped_gated_product(Array output, Array A, Array W, Array offsets, int32_t activation) {
+    const std::string op = "cuda_grouped_gated_product";
+    check_gated(A, W, offsets, output, "output", activation, op);
+    check_output(output, "output", op);
+    if (output.shape[0] == 0 || output.shape[1] == 0) return;
+    Call call = begin_call();
+    const int32_t* starts = static_cast<const int32_t*>(offsets.data);
+    Widened wide(call, A, W, starts, op);
+    for_types(A.type, [&](auto zero, auto sum) {
+        using T = decltype(zero);
+        using S = decltype(sum);
+        for_activation(activation, [&](auto f) {
+            gate_rows<decltype(f)::value, T, S><<<row_blocks(call, output.shape[0]), row_threads(), 0, call.stream>>>(
+                static_cast<T*>(output.data), static_cast<const S*>(wide.uv.data), output.shape[0], output.shape[1]);
+        });
+        note_kernel_f("gate_rows<%s>", array_type_name<T>());
+    });
+    MOPS_CUDA_OK(cudaGetLastError());
+    end_call(call, op.c_str(), kIndexNames, 1);
+}
+
+void grouped_gated_product_vjp(Array grad_A, Array grad_W, Array grad_output, Array A, Array W, Array offsets, int32_t activation) {
+    const std::string op = "cuda_grouped_gated_product_vjp";
+    check_gated(A, W, offsets, grad_output, "grad_output", activation, op);
+    check_rows(grad_output, "grad_output", op);
+    const bool need_A = grad_A.data != nullptr, need_W = grad_W.data != nullptr;
+    if (need_A) {
+        check_array(grad_A, "grad_A", 2, A.type, op);
+        for (int d = 0; d < 2; d++) check_size(grad_A.shape[d], "grad_A", d, A.shape[d], "A", d, op);
+        check_output(grad_A, "grad_A", op);
+    }
+    bool turned = false; // grad_W[g] is stored column by column
+    if (need_W) {
+        check_array(grad_W, "grad_W", 3, A.type, op);
+        for (int d = 0; d < 3; d++) check_size(grad_W.shape[d], "grad_W", d, W.shape[d], "W", d, op);
+        turned = grad_W.stride[2] != 1;
+        if (turned) std::swap(grad_W.shape[1], grad_W.shape[2]), std::swap(grad_W.stride[1], grad_W.stride[2]);
+        check_output(grad_W, "grad_W", op);
+    }
+    if (!need_A && !need_W) return;
+    Call call = begin_call();
+    const int32_t* starts = static_cast<const int32_t*>(offsets.data);
+    const int64_t rows = A.shape[0], columns = W.shape[2];
+    Widened wide(call, A, W, starts, op);
+    if (rows > 0 && columns > 0) {
+        for_types(A.type, [&](auto zero, auto sum) {
+            using T = decltype(zero);
+            using S = decltype(sum);
+            for_activation(activation, [&](auto f) {
+                gate_rows_vjp<decltype(f)::value, T, S><<<row_blocks(call, rows), row_threads(), 0, call.stream>>>(
+                    static_cast<S*>(wide.uv.data), static_cast<const T*>(grad_output.data), grad_output.stride[0], rows, columns / 2);
+            });
+            note_kernel_f("gate_rows_vjp<%s>", array_type_name<T>());
+        });
+        MOPS_CUDA_OK(cudaGetLastError());
+    }
+    // as of a plain layer whose output's gradient is dU and dV
+    Packing packing(call);
+    if (wide.type == MOPS_B200_F32 && rows > 0 && A.shape[1] > 0 && W.shape[0] > 0 && columns > 0) {
+        const bool rows_packed = need_A && !straight_rows(wide.W, rows, wide.W.stride[1] == 1);
+        const bool outer_packed = need_W && !straight_outer(rows, W.shape[0], W.shape[1], columns, wide.type);
+        if (rows_packed || outer_packed) packing.add(wide.uv);
+        if (rows_packed) packing.add(wide.W);
+        if (outer_packed) packing.add(wide.A);
+        packing.run();
+    }
+    const bool widened = wide.type != A.type;
+    Scratch room(call);
+    auto result = [&](Array& gradient, auto&& make) { // in the type of the products, and rounded where that is another one
+        Array to = gradient;
+        if (widened) {
+            room.take(static_cast<size_t>(values_of(gradient)) * 4 + 16);
+            to.data = room.as<void>();
+            to.type = wide.type;
+        }
+        make(to);
+        if (widened)
+            for_type(A.type, [&](auto zero) {
+                using T = decltype(zero);
+                (void)converted(call, to, static_cast<T*>(gradient.data), A.type);
+            });
+    };
+    if (need_A)
+        result(grad_A, [&](const Array& to) {
+            multiply_rows(call, {to, wide.uv, wide.W, wide.W.stride[2], wide.W.stride[1], starts, W.shape[0], rows, columns, A.shape[1]}, op);
+        });
+    if (need_W)
+        result(grad_W, [&](const Array& to) {
+            if (turned) multiply_outer(call, {to, wide.uv, wide.A, starts, W.shape[0]}, op);
+            else multiply_outer(call, {to, wide.A, wide.uv, starts, W.shape[0]}, op);
+        });
+    room.free();
+    packing.release();
+    end_call(call, op.c_str(), kIndexNames, 1);
+}
+
+} // namespace mops_b200

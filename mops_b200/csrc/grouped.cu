@@ -122,6 +122,8 @@ grouped_outer_plain(T* __restrict__ out, const T* __restrict__ X, int64_t x_stri
 
 const char* const kIndexNames[] = {"offsets"};
 
+} // namespace
+
 void multiply_rows(const Call& call, const RowsProblem& p, const std::string& op) {
     if (p.rows == 0 || p.columns == 0 || multiply_rows_few(call, p, op) || multiply_rows_mma(call, p, op) ||
         multiply_rows_split(call, p, op))
@@ -159,6 +161,8 @@ void multiply_outer(const Call& call, const OuterProblem& p, const std::string& 
     MOPS_CUDA_OK(cudaGetLastError());
 }
 
+namespace {
+
 // Sizes and types of rows (R x K), matrices (G x K x N) and offsets (G + 1).
 void check_common(Array& A, Array& W, const char* w_name, Array& offsets, Array& rows, const char* rows_name,
                   const std::string& op) {
@@ -176,13 +180,16 @@ void check_common(Array& A, Array& W, const char* w_name, Array& offsets, Array&
     for (int64_t n : {A.shape[0], A.shape[1], W.shape[0], W.shape[2]}) fits_int32(static_cast<size_t>(n), "a size", op);
 }
 
-// One of the last two dimensions of W lies value by value in memory. (So does one of size 1, whatever its stride; matrices of one row whose columns lie apart are
-// columns of one value each.)
+} // namespace
+
+// (So does one of size 1, whatever its stride; matrices of one row whose columns lie apart are columns of one value each.)
 void check_matrices(Array& W, const char* name, const std::string& op) {
     if (W.shape[1] == 1 && W.stride[2] != 1) W.stride[1] = 1;
     if (W.stride[2] != 1 && W.stride[1] != 1)
         throw std::runtime_error(std::string(name) + " must have a stride of 1 in one of its last two dimensions in " + op);
 }
+
+namespace {
 
 // Whether there are products to compute that the tensor cores take on (the other problems go to the kernels of this file).
 bool on_tensor_cores(const Array& A, const Array& W) {

@@ -21,6 +21,13 @@ struct OuterProblem {
     int64_t groups;
 };
 
+// By whichever kernels fit (grouped.cu). Arrays of 16 and 32 bits are such that the copy engine can fetch them (pack.hpp), unless straight_rows() or
+// straight_outer() say that this does not matter.
+void multiply_rows(const Call& call, const RowsProblem& p, const std::string& op);
+void multiply_outer(const Call& call, const OuterProblem& p, const std::string& op);
+// One of the last two dimensions of W lies value by value in memory.
+void check_matrices(Array& W, const char* name, const std::string& op);
+
 // A few rows in all, as single tokens are (grouped_few.cu): false if there are too many.
 bool multiply_rows_few(const Call& call, const RowsProblem& p, const std::string& op);
 bool multiply_outer_few(const Call& call, const OuterProblem& p, const std::string& op);

@@ -1,5 +1,5 @@
-// torch operators of the block: torch.ops.mops.embedding_lookup, grouped_matrix_product and gated_residual_norm, with
-// their gradients (first derivatives; second ones are refused). CUDA tensors of float32, float64, float16 or bfloat16. Rows may lie apart
+// torch operators of the block: torch.ops.mops.embedding_lookup, grouped_matrix_product, gated_residual_norm, grouped_gated_product and
+// linear_cross_entropy, with their gradients (first derivatives; second ones are refused), and the norm of gradients. CUDA tensors of float32, float64, float16 or bfloat16. Rows may lie apart
 // (any strides but that of the last dimension); anything else is made contiguous. Kernels run on torch's current stream of the tensors'
 // device without synchronising it, so an index out of range is not reported: its row is zero, and it gives no gradient.
 #include "torch_common.hpp"
@@ -276,7 +276,217 @@ struct GatedResidualNorm : torch::autograd::Function<GatedResidualNorm> {
     }
 };
 
+// ================================================================= grouped_gated_product
+int32_t activation_of(const std::string& name, const char* op) {
+    if (name == "silu") return MOPS_B200_SILU;
+    if (name == "gelu") return MOPS_B200_GELU;
+    C10_THROW_ERROR(ValueError, "activation must be one of silu, gelu in " + std::string(op) + ", found " + name);
+}
+
+Tensor run_grouped_gated_product(Tensor& A, Tensor& W, Tensor& offsets, int32_t activation) {
+    static constexpr const char* op = "grouped_gated_product";
+    same_device({A, W, offsets});
+    block_types({A, W});
+    int32_indices({offsets});
+    ndim(A, 2, "A", op);
+    ndim(W, 3, "W", op);
+    ndim(offsets, 1, "offsets", op);
+    cuda_only(A, op);
+    A = rows_of(A);
+    W = matrices_of(W);
+    offsets = offsets.contiguous();
+    Tensor output = torch::empty({A.size(0), W.size(2) / 2}, A.options());
+    on_stream_of(A, [&] { checked(mops_b200_cuda_grouped_gated_product(array(output), array(A), array(W), array(offsets), activation)); });
+    return output;
+}
+
+struct GroupedGatedProductBackward : torch::autograd::Function<GroupedGatedProductBackward> {
+    static tensor_list run(const Tensor& grad_output, const Tensor& A, const Tensor& W, const Tensor& offsets, int64_t activation, bool need_A,
+                           bool need_W) {
+        Tensor grad_A = empty_if(need_A, A.sizes(), A), grad_W;
+        if (need_W) // stored the way round that W is
+            grad_W = W.stride(2) == 1 ? torch::empty(W.sizes(), W.options())
+                                      : torch::empty({W.size(0), W.size(2), W.size(1)}, W.options()).transpose(1, 2);
+        on_stream_of(A, [&] {
+            checked(mops_b200_cuda_grouped_gated_product_vjp(array(grad_A), array(grad_W), array(grad_output), array(A), array(W), array(offsets),
+                                                             static_cast<int32_t>(activation)));
+        });
+        return {grad_A, grad_W};
+    }
+    static tensor_list forward(AutogradContext*, Tensor grad_output, Tensor A, Tensor W, Tensor offsets, int64_t activation, bool need_A,
+                               bool need_W) {
+        return all_defined(run(grad_output, A, W, offsets, activation, need_A, need_W), A);
+    }
+    static tensor_list backward(AutogradContext*, tensor_list) { no_second_derivative("grouped_gated_product"); }
+};
+
+struct GroupedGatedProduct : torch::autograd::Function<GroupedGatedProduct> {
+    static Tensor forward(AutogradContext* ctx, Tensor A, Tensor W, Tensor offsets, int64_t activation) {
+        Tensor output = run_grouped_gated_product(A, W, offsets, static_cast<int32_t>(activation));
+        ctx->save_for_backward({A, W, offsets});
+        ctx->saved_data["activation"] = activation;
+        return output;
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        auto s = ctx->get_saved_variables();
+        const Tensor grad_output = rows_of(grads[0]);
+        auto r = first_derivative<GroupedGatedProductBackward>({grad_output, s[0], s[1]}, grad_output, s[0], s[1], s[2],
+                                                               ctx->saved_data["activation"].toInt(), ctx->needs_input_grad(0),
+                                                               ctx->needs_input_grad(1));
+        return {if_needed(r[0], ctx->needs_input_grad(0)), if_needed(r[1], ctx->needs_input_grad(1)), Tensor(), Tensor()};
+    }
+};
+
+// ================================================================== linear_cross_entropy
+at::TensorOptions options_of_sums(const Tensor& t) { return t.options().dtype(t.scalar_type() == torch::kF64 ? torch::kF64 : torch::kF32); }
+
+tensor_list run_linear_cross_entropy(Tensor& A, Tensor& W, Tensor& targets, double scale, int64_t ignore_index) {
+    static constexpr const char* op = "linear_cross_entropy";
+    same_device({A, W, targets});
+    block_types({A, W});
+    int32_indices({targets});
+    ndim(A, 2, "A", op);
+    ndim(W, 2, "W", op);
+    ndim(targets, 1, "targets", op);
+    cuda_only(A, op);
+    A = rows_of(A);
+    W = rows_of(W);
+    targets = targets.contiguous();
+    Tensor loss = torch::empty({A.size(0)}, options_of_sums(A)), log_sum = torch::empty({A.size(0)}, options_of_sums(A));
+    on_stream_of(A, [&] {
+        checked(mops_b200_cuda_linear_cross_entropy(array(loss), array(log_sum), array(A), array(W), array(targets), scale, ignore_index));
+    });
+    return {loss, log_sum};
+}
+
+struct LinearCrossEntropyBackward : torch::autograd::Function<LinearCrossEntropyBackward> {
+    static tensor_list run(const std::optional<Tensor>& grad_loss, const std::optional<Tensor>& grad_log_sum, const Tensor& loss, const Tensor& log_sum,
+                           const Tensor& A, const Tensor& W, const Tensor& targets, double scale, int64_t ignore_index, bool need_A, bool need_W) {
+        Tensor grad_A = empty_if(need_A, A.sizes(), A), grad_W = empty_if(need_W, W.sizes(), W);
+        on_stream_of(A, [&] {
+            checked(mops_b200_cuda_linear_cross_entropy_vjp(array(grad_A), array(grad_W), array(grad_loss.value_or(Tensor())),
+                                                            array(grad_log_sum.value_or(Tensor())), array(loss), array(log_sum), array(A), array(W),
+                                                            array(targets), scale, ignore_index));
+        });
+        return {grad_A, grad_W};
+    }
+    static tensor_list forward(AutogradContext*, std::optional<Tensor> grad_loss, std::optional<Tensor> grad_log_sum, Tensor loss, Tensor log_sum,
+                               Tensor A, Tensor W, Tensor targets, double scale, int64_t ignore_index, bool need_A, bool need_W) {
+        return all_defined(run(grad_loss, grad_log_sum, loss, log_sum, A, W, targets, scale, ignore_index, need_A, need_W), A);
+    }
+    static tensor_list backward(AutogradContext*, tensor_list) { no_second_derivative("linear_cross_entropy"); }
+};
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+    static tensor_list forward(AutogradContext* ctx, Tensor A, Tensor W, Tensor targets, double scale, int64_t ignore_index) {
+        tensor_list r = run_linear_cross_entropy(A, W, targets, scale, ignore_index);
+        ctx->save_for_backward({A, W, targets, r[0], r[1]});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["ignore_index"] = ignore_index;
+        ctx->set_materialize_grads(false);
+        return r;
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        auto s = ctx->get_saved_variables();
+        std::optional<Tensor> given[2];
+        for (int i = 0; i < 2; i++)
+            if (grads[i].defined()) given[i] = rows_of(grads[i]);
+        if (!given[0] && !given[1]) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        auto r = first_derivative<LinearCrossEntropyBackward>(
+            {given[0].value_or(Tensor()), given[1].value_or(Tensor()), s[0], s[1]}, given[0], given[1], s[3].detach(), s[4].detach(), s[0], s[1], s[2],
+            ctx->saved_data["scale"].toDouble(), ctx->saved_data["ignore_index"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        return {if_needed(r[0], ctx->needs_input_grad(0)), if_needed(r[1], ctx->needs_input_grad(1)), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ==================================================================== norm of gradients
+// All on one device and of types that there are; not differentiated.
+void check_gradients(const tensor_list& gradients, const char* op) {
+    if (gradients.empty()) C10_THROW_ERROR(ValueError, "no gradients in " + std::string(op));
+    same_device(gradients);
+    for (const Tensor& g : gradients) {
+        block_types({g});
+        if (differentiated({&g})) C10_THROW_ERROR(NotImplementedError, "derivatives are not supported in CUDA for " + std::string(op));
+    }
+    cuda_only(gradients[0], op);
+}
+
+// A tensor whose values fill a piece of memory, as one dimension.
+mops_b200_array_t flat(const Tensor& t) {
+    mops_b200_array_t a = array(t.dim() == 1 ? t : t.as_strided({t.numel()}, {1}));
+    a.stride[0] = 1;
+    return a;
+}
+bool is_flat(const Tensor& t) { return !t.is_neg() && !t.is_conj() && t.is_non_overlapping_and_dense(); }
+
+std::vector<mops_b200_array_t> table_of(const tensor_list& tensors) {
+    std::vector<mops_b200_array_t> r;
+    r.reserve(tensors.size());
+    for (const Tensor& t : tensors) r.push_back(flat(t));
+    return r;
+}
+
+// A scalar tensor for the norm, and the view of it that the library writes.
+Tensor empty_norm(const tensor_list& gradients) {
+    bool wide = false;
+    for (const Tensor& g : gradients) wide |= g.scalar_type() == torch::kF64;
+    return torch::empty({}, gradients[0].options().dtype(wide ? torch::kF64 : torch::kF32));
+}
+
+tensor_list all_flat(const tensor_list& gradients) {
+    tensor_list r;
+    for (const Tensor& g : gradients) r.push_back(is_flat(g) ? g : g.resolve_neg().resolve_conj().contiguous());
+    return r;
+}
+
+Tensor gradient_norm(tensor_list gradients) {
+    check_gradients(gradients, "gradient_norm");
+    gradients = all_flat(gradients);
+    Tensor norm = empty_norm(gradients);
+    const auto table = table_of(gradients);
+    on_stream_of(norm, [&] { checked(mops_b200_cuda_gradient_norm(flat(norm), table.data(), static_cast<int64_t>(table.size()))); });
+    return norm;
+}
+
+std::tuple<Tensor, tensor_list> clip_gradient_norm(tensor_list gradients, double max_norm) {
+    check_gradients(gradients, "clip_gradient_norm");
+    gradients = all_flat(gradients);
+    Tensor norm = empty_norm(gradients);
+    tensor_list clipped;
+    for (const Tensor& g : gradients) clipped.push_back(torch::empty_like(g));
+    const auto table = table_of(gradients), results = table_of(clipped);
+    on_stream_of(norm, [&] {
+        checked(mops_b200_cuda_clip_gradient_norm(flat(norm), results.data(), table.data(), static_cast<int64_t>(table.size()), max_norm));
+    });
+    return {norm, clipped};
+}
+
+Tensor clip_gradient_norm_(tensor_list gradients, double max_norm) {
+    static constexpr const char* op = "clip_gradient_norm_";
+    check_gradients(gradients, op);
+    for (const Tensor& g : gradients)
+        if (!is_flat(g)) C10_THROW_ERROR(ValueError, "gradients must fill their memory without gaps in " + std::string(op));
+    Tensor norm = empty_norm(gradients);
+    const auto table = table_of(gradients);
+    on_stream_of(norm, [&] {
+        checked(mops_b200_cuda_clip_gradient_norm(flat(norm), table.data(), table.data(), static_cast<int64_t>(table.size()), max_norm));
+    });
+    for (Tensor& g : gradients) g.unsafeGetTensorImpl()->bump_version();
+    return norm;
+}
+
 // ------------------------------------------------------------------ registered entry points
+Tensor grouped_gated_product(Tensor A, Tensor W, Tensor offsets, std::string activation) {
+    const int32_t f = activation_of(activation, "grouped_gated_product");
+    return differentiated({&A, &W}) ? GroupedGatedProduct::apply(A, W, offsets, static_cast<int64_t>(f)) : run_grouped_gated_product(A, W, offsets, f);
+}
+
+std::tuple<Tensor, Tensor> linear_cross_entropy(Tensor A, Tensor W, Tensor targets, double scale, int64_t ignore_index) {
+    auto r = differentiated({&A, &W}) ? LinearCrossEntropy::apply(A, W, targets, scale, ignore_index)
+                                      : run_linear_cross_entropy(A, W, targets, scale, ignore_index);
+    return {r[0], r[1]};
+}
+
 Tensor embedding_lookup(Tensor W, Tensor indices, double scale, int64_t padding_index) {
     return differentiated({&W}) ? EmbeddingLookup::apply(W, indices, scale, padding_index)
                                 : run_embedding_lookup(W, indices, scale, padding_index);
@@ -303,4 +513,10 @@ TORCH_LIBRARY_FRAGMENT(mops, m) {
     m.def("gated_residual_norm(Tensor residual, Tensor branch, Tensor? gate, Tensor scale, Tensor weight_branch, "
           "Tensor weight_output, float epsilon=1e-6) -> (Tensor, Tensor)",
           gated_residual_norm);
+    m.def("grouped_gated_product(Tensor A, Tensor W, Tensor offsets, str activation='silu') -> Tensor", grouped_gated_product);
+    m.def("linear_cross_entropy(Tensor A, Tensor W, Tensor targets, float scale=1.0, int ignore_index=-1) -> (Tensor loss, Tensor log_sum)",
+          linear_cross_entropy);
+    m.def("gradient_norm(Tensor[] gradients) -> Tensor", gradient_norm);
+    m.def("clip_gradient_norm(Tensor[] gradients, float max_norm) -> (Tensor norm, Tensor[] clipped)", clip_gradient_norm);
+    m.def("clip_gradient_norm_(Tensor(a!)[] gradients, float max_norm) -> Tensor", clip_gradient_norm_);
 }

@@ -15,6 +15,16 @@ float16 and bfloat16:
 * ``gated_residual_norm(residual, branch, gate, scale, weight_branch, weight_output, epsilon=1e-6)``:
   ``stream = residual + scale * weight_branch * sigmoid(gate) * branch / rms(branch)`` and
   ``weight_output * stream / rms(stream)``.
+* ``grouped_gated_product(A, W, offsets, activation="silu")``: the gated feed-forward layer of each group, ``W`` of G x K x 2N with the gate's
+  columns first: ``f(A[r] @ W[g][:, :N]) * (A[r] @ W[g][:, N:])``, f silu or gelu.
+* ``linear_cross_entropy(A, W, targets, scale=1.0, ignore_index=-1)``: ``loss`` and ``log_sum`` of each row, of the logits
+  ``scale * A @ W.T``, which are not kept. Rows whose target is ``ignore_index`` have zeros and no gradient.
+
+And for all gradients of a model together, whose types may differ (not differentiable):
+
+* ``gradient_norm(gradients)``: the root of the sum of squares of all their values.
+* ``clip_gradient_norm(gradients, max_norm)``: that norm, and the gradients scaled to ``max_norm`` where it is larger;
+  ``clip_gradient_norm_`` scales them in place and returns the norm. Where the norm is not finite they stay as they are.
 """
 import os
 
@@ -37,6 +47,11 @@ sparse_accumulation_scatter_add_with_weights = (
 embedding_lookup = torch.ops.mops.embedding_lookup
 grouped_matrix_product = torch.ops.mops.grouped_matrix_product
 gated_residual_norm = torch.ops.mops.gated_residual_norm
+grouped_gated_product = torch.ops.mops.grouped_gated_product
+linear_cross_entropy = torch.ops.mops.linear_cross_entropy
+gradient_norm = torch.ops.mops.gradient_norm
+clip_gradient_norm = torch.ops.mops.clip_gradient_norm
+clip_gradient_norm_ = torch.ops.mops.clip_gradient_norm_
 
 __all__ = [
     "homogeneous_polynomial_evaluation",
@@ -47,4 +62,9 @@ __all__ = [
     "embedding_lookup",
     "grouped_matrix_product",
     "gated_residual_norm",
+    "grouped_gated_product",
+    "linear_cross_entropy",
+    "gradient_norm",
+    "clip_gradient_norm",
+    "clip_gradient_norm_",
 ]
