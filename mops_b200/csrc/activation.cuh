@@ -2,6 +2,8 @@
 #ifndef MOPS_B200_ACTIVATION_CUH
 #define MOPS_B200_ACTIVATION_CUH
 
+#include <type_traits>
+
 #include "../../include/mops.h"
 #include "device.cuh"
 
@@ -22,6 +24,26 @@ template <int kActivation, typename S> struct Gate {
         }
     }
 };
+
+// The same for results that are rounded to 16 bits: exponentials and quotients to some 2^-21.
+template <int kActivation> struct FastGate {
+    float value, slope;
+    __device__ __forceinline__ explicit FastGate(float u) {
+        if constexpr (kActivation == MOPS_B200_SILU) {
+            const float s = __fdividef(1.f, 1.f + __expf(-u)); // (0 where the exponential is beyond 2^126)
+            value = u * s;
+            slope = fmaf(value, 1.f - s, s);
+        } else {
+            const Gate<kActivation, float> gate(u);
+            value = gate.value, slope = gate.slope;
+        }
+    }
+};
+
+template <typename F> void for_activation(int32_t activation, F&& f) {
+    if (activation == MOPS_B200_SILU) f(std::integral_constant<int, MOPS_B200_SILU>());
+    else f(std::integral_constant<int, MOPS_B200_GELU>());
+}
 
 } // namespace mops_b200
 

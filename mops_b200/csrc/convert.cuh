@@ -21,15 +21,15 @@ template <typename To, typename From> __device__ __forceinline__ To convert(From
     else return narrow<To>(static_cast<Sum<To>>(widen(v)));
 }
 
-// to[row][i] = from[slice of the row][row of the slice][i], `slices` x `outer` rows of `inner` values.
+// to[slice][row][i] = from[slice][row][i], `slices` x `outer` rows of `inner` values.
 template <typename To, typename From>
 static __global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
-convert_rows(To* __restrict__ to, int64_t to_stride, const From* __restrict__ from, int64_t slices, int64_t outer, int64_t inner, int64_t slice_stride,
+convert_rows(To* __restrict__ to, int64_t to_slice_stride, int64_t to_stride, const From* __restrict__ from, int64_t slices, int64_t outer, int64_t inner, int64_t slice_stride,
              int64_t outer_stride) {
     for (int64_t row = first_row(); row < slices * outer; row += row_step()) {
         const int64_t slice = row / outer;
         const From* p = from + slice * slice_stride + (row - slice * outer) * outer_stride;
-        To* q = to + row * to_stride;
+        To* q = to + slice * to_slice_stride + (row - slice * outer) * to_stride;
         for (int64_t i = threadIdx.x; i < inner; i += kRowThreads) q[i] = convert<To>(p[i]);
     }
 }
@@ -47,7 +47,7 @@ template <typename To> Array converted(const Call& call, const Array& a, To* to,
         for_type(a.type, [&](auto zero) {
             using From = decltype(zero);
             convert_rows<To, From><<<row_blocks(call, slices * a.shape[outer]), row_threads(), 0, call.stream>>>(
-                to, a.shape[inner], static_cast<const From*>(a.data), slices, a.shape[outer], a.shape[inner], a.dimensions == 3 ? a.stride[0] : 0, a.stride[outer]);
+                to, a.shape[inner] * a.shape[outer], a.shape[inner], static_cast<const From*>(a.data), slices, a.shape[outer], a.shape[inner], a.dimensions == 3 ? a.stride[0] : 0, a.stride[outer]);
         });
     MOPS_CUDA_OK(cudaGetLastError());
     return r;

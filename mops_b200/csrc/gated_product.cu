@@ -7,10 +7,11 @@
 //
 // Here: f32 and f64. U and V, side by side in scratch memory, are one grouped product; a pass over them makes the output of them, or, where
 // they stood, dU and dV, of which the gradients are the grouped products that they are for a plain layer. f16 and bf16 are widened to f32 for that, so U, V, dU and dV are never
-// rounded to 16 bits.
+// rounded to 16 bits; that is done where there are few rows to differentiate, the rest of f16 and bf16 is in gated_mma.cu.
 #include "activation.cuh"
 #include "block_ops.hpp"
 #include "convert.cuh"
+#include "gated_mma.hpp"
 #include "grouped_mma.hpp"
 #include "pack.hpp"
 
@@ -40,11 +41,6 @@ gate_rows_vjp(S* __restrict__ uv, const T* __restrict__ grad, int64_t grad_strid
             *u = g * *v * gate.slope;
             *v = g * gate.value;
         }
-}
-
-template <typename F> void for_activation(int32_t activation, F&& f) {
-    if (activation == MOPS_B200_SILU) f(std::integral_constant<int, MOPS_B200_SILU>());
-    else f(std::integral_constant<int, MOPS_B200_GELU>());
 }
 
 const char* const kIndexNames[] = {"offsets"};
@@ -93,6 +89,82 @@ struct Widened {
     }
 };
 
+// ---- f16 and bf16 on tensor cores
+// A and W as the copy engine can fetch them, or copies: rows of A whole packs apart, and of W both halves, with zeros behind the columns of either up to a multiple of 8. `padded`: gradients
+// are to be taken, too, whose products go along both halves at once.
+struct Boxed {
+    const Call& call;
+    Packing packing;
+    Scratch room;
+    GatedProblem p;
+    int64_t real_columns; // of a half
+    Boxed(const Call& call, const Array& A, const Array& W, const int32_t* offsets, int32_t activation, bool gradients)
+        : call(call), packing(call), room(call), p{A, W, offsets, W.shape[0], A.shape[0], A.shape[1], W.shape[2] / 2, activation}, real_columns(W.shape[2] / 2) {
+        packing.add(p.A);
+        const int64_t columns = real_columns;
+        if (columns % 8 != 0 && (gradients || p.by_columns())) {
+            const int64_t groups = p.groups, depth = p.depth, wide = (columns + 7) / 8 * 8, deep = (depth + 7) / 8 * 8;
+            p.columns = wide;
+            p.W = p.by_columns() ? contiguous(nullptr, A.type, groups, depth, 2 * wide) : contiguous(nullptr, A.type, groups, 2 * wide, deep);
+            const size_t bytes = static_cast<size_t>(values_of(p.W)) * 2;
+            room.take(bytes);
+            p.W.data = room.as<void>();
+            if (W.stride[2] != 1) std::swap(p.W.shape[1], p.W.shape[2]), std::swap(p.W.stride[1], p.W.stride[2]), p.W.shape[1] = depth;
+            MOPS_CUDA_OK(cudaMemsetAsync(p.W.data, 0, bytes, call.stream));
+            copy_halves(p.W, wide, W, columns);
+        } else {
+            packing.add(p.W);
+        }
+        packing.run();
+    }
+    // The halves of `from` (of `n` columns each) go where those of `to` (of `m`, n or more there or here) are; both are stored the same way round.
+    void copy_halves(const Array& to, int64_t m, const Array& from, int64_t n) {
+        const bool by_columns = from.stride[2] == 1;
+        const int64_t columns = std::min(m, n), outer = by_columns ? from.shape[1] : columns, inner = by_columns ? columns : from.shape[1];
+        for (int half = 0; half < 2; half++) // (their values are only moved)
+            convert_rows<uint16_t, uint16_t><<<row_blocks(call, from.shape[0] * outer), row_threads(), 0, call.stream>>>(
+                static_cast<uint16_t*>(to.data) + half * m * to.stride[2], to.stride[0], by_columns ? to.stride[1] : to.stride[2],
+                static_cast<const uint16_t*>(from.data) + half * n * from.stride[2], from.shape[0], outer, inner, from.stride[0],
+                by_columns ? from.stride[1] : from.stride[2]);
+        MOPS_CUDA_OK(cudaGetLastError());
+    }
+};
+
+bool sixteen_bits(const Array& A, const Array& W) {
+    return (A.type == MOPS_B200_F16 || A.type == MOPS_B200_BF16) && A.shape[0] > 0 && A.shape[1] > 0 && W.shape[0] > 0 && W.shape[2] > 0;
+}
+
+// Up to so many rows gradients are computed in f32 throughout: rounded to 16 bits, dU and dV of a few rows are few values, whose errors do not average out.
+constexpr int64_t kFewGradients = 64;
+
+void gradients_16(const Call& call, const Array& grad_A, const Array& grad_W, bool turned, const Array& grad_output, const Array& A, const Array& W, const int32_t* offsets,
+                  int32_t activation, const std::string& op) {
+    Boxed boxed(call, A, W, offsets, activation, true);
+    const GatedProblem& p = boxed.p;
+    Scratch room(call, static_cast<size_t>(p.rows * 2 * p.columns) * 2);
+    const Array duv = contiguous(room.as<void>(), A.type, p.rows, 2 * p.columns);
+    gated_rows_vjp_mma(call, p, duv.data, grad_output, op);
+    if (grad_A.data != nullptr)
+        multiply_rows(call, {grad_A, duv, p.W, p.W.stride[2], p.W.stride[1], offsets, p.groups, p.rows, 2 * p.columns, p.depth}, op);
+    if (grad_W.data == nullptr) return;
+    Array to = grad_W;
+    Scratch room_W(call);
+    const bool padded = p.columns != boxed.real_columns;
+    if (padded) { // the products of the columns that there are not, too
+        to = turned ? contiguous(nullptr, A.type, p.groups, 2 * p.columns, p.depth) : contiguous(nullptr, A.type, p.groups, p.depth, 2 * p.columns);
+        room_W.take(static_cast<size_t>(values_of(to)) * 2);
+        to.data = room_W.as<void>();
+    }
+    if (turned) multiply_outer(call, {to, duv, p.A, offsets, p.groups}, op);
+    else multiply_outer(call, {to, p.A, duv, offsets, p.groups}, op);
+    if (padded) {
+        Array result = grad_W;
+        if (turned)
+            for (Array* a : {&to, &result}) std::swap(a->shape[1], a->shape[2]), std::swap(a->stride[1], a->stride[2]);
+        boxed.copy_halves(result, boxed.real_columns, to, p.columns);
+    }
+}
+
 // f(T(), S()) with T the type and S that of sums
 template <typename F> void for_types(int32_t type, F&& f) {
     for_type(type, [&](auto zero) { f(zero, Sum<decltype(zero)>()); });
@@ -107,6 +179,12 @@ void grouped_gated_product(Array output, Array A, Array W, Array offsets, int32_
     if (output.shape[0] == 0 || output.shape[1] == 0) return;
     Call call = begin_call();
     const int32_t* starts = static_cast<const int32_t*>(offsets.data);
+    if (sixteen_bits(A, W)) {
+        Boxed boxed(call, A, W, starts, activation, false);
+        gated_rows_mma(call, boxed.p, output, op);
+        end_call(call, op.c_str(), kIndexNames, 1);
+        return;
+    }
     Widened wide(call, A, W, starts, op);
     for_types(A.type, [&](auto zero, auto sum) {
         using T = decltype(zero);
@@ -143,6 +221,11 @@ void grouped_gated_product_vjp(Array grad_A, Array grad_W, Array grad_output, Ar
     Call call = begin_call();
     const int32_t* starts = static_cast<const int32_t*>(offsets.data);
     const int64_t rows = A.shape[0], columns = W.shape[2];
+    if (sixteen_bits(A, W) && rows > kFewGradients) {
+        gradients_16(call, grad_A, grad_W, turned, grad_output, A, W, starts, activation, op);
+        end_call(call, op.c_str(), kIndexNames, 1);
+        return;
+    }
     Widened wide(call, A, W, starts, op);
     if (rows > 0 && columns > 0) {
         for_types(A.type, [&](auto zero, auto sum) {
