@@ -6,7 +6,8 @@
 //   grad_A = scale dx W, grad_W = scale dx^T A
 //
 // A piece of the vocabulary at a time: its logits are a product into scratch memory, of which sums are taken, or which become dx where they stand and are multiplied by the
-// piece's rows of W and, the other way, by A. The gradients compute the logits again. Here: f32 and f64; f16 and bf16 are widened to f32.
+// piece's rows of W and, the other way, by A. The gradients compute the logits again. Here: f32 and f64, and f16 and bf16, widened to f32, where there are few rows to differentiate; the rest of
+// them is in cross_entropy_mma.cu.
 #include "block_ops.hpp"
 #include "convert.cuh"
 #include "grouped_mma.hpp"
@@ -24,10 +25,11 @@ constexpr int64_t kMostLogits = int64_t(64) << 20; // of a piece
 template <typename S>
 __global__ void __launch_bounds__(kPrepareThreads)
 loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, const int32_t* __restrict__ targets, int64_t rows, int64_t vocabulary,
-             int64_t ignored, Status st) {
+             int64_t ignored, const S* __restrict__ grad_loss, const S* __restrict__ grad_log_sum, Status st) {
     __shared__ int of_warp[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int before = 0;
+    float largest[3] = {}; // of the gradients of losses, of sums, of both together
     bool bad = false;
     for (int64_t r0 = 0; r0 < rows; r0 += kPrepareThreads * kPrepareRows) {
         const int64_t r = r0 + static_cast<int64_t>(threadIdx.x) * kPrepareRows;
@@ -62,11 +64,37 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
             if (r + k < rows) {
                 const bool in = keep >> k & 1;
                 to.place[r + k] = in ? i : -1;
-                if (in) to.order[i++] = static_cast<int32_t>(r + k);
-                else if (loss != nullptr) loss[r + k] = log_sum[r + k] = S(0);
+                if (in) {
+                    to.order[i] = static_cast<int32_t>(r + k);
+                    to.target[i++] = targets[r + k];
+                    const float l = grad_loss != nullptr ? static_cast<float>(fabs(grad_loss[r + k])) : 0.f;
+                    const float m = grad_log_sum != nullptr ? static_cast<float>(fabs(grad_log_sum[r + k])) : 0.f;
+                    const float all[3] = {l, m, l + m};
+#pragma unroll
+                    for (int q = 0; q < 3; q++)
+                        if (all[q] <= 3e38f) largest[q] = fmaxf(largest[q], all[q]); // (infinities keep to their rows)
+                } else if (loss != nullptr) {
+                    loss[r + k] = log_sum[r + k] = S(0);
+                }
             }
         before += total;
         __syncthreads();
+    }
+    if (grad_loss != nullptr || grad_log_sum != nullptr) {
+        __shared__ float most[3][kPrepareThreads / 32];
+#pragma unroll
+        for (int q = 0; q < 3; q++) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) largest[q] = fmaxf(largest[q], __shfl_xor_sync(kFullMask, largest[q], d));
+            if (lane == 0) most[q][warp] = largest[q];
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < kPrepareThreads / 32; w++)
+                for (int q = 0; q < 3; q++) largest[q] = fmaxf(largest[q], most[q][w]);
+            // (small gradients of sums are left out: 16-bit units are those of the losses', so that -1 stays -1)
+            *to.unit = largest[1] <= 2 * largest[0] ? largest[0] : largest[2];
+        }
     }
     if (threadIdx.x == 0) to.offsets[0] = 0, to.offsets[1] = before;
     if (bad) report_bad_index(st, 0);
@@ -151,6 +179,19 @@ loss_gradient(S* __restrict__ logits, int64_t columns, S scale, const S* __restr
 
 const char* const kIndexNames[] = {"targets"};
 
+} // namespace
+
+template <typename S>
+void prepare_rows(const Call& call, const LossRows& to, S* loss, S* log_sum, const Array& targets, int64_t vocabulary, int64_t ignored, const S* grad_loss,
+                  const S* grad_log_sum) {
+    loss_prepare<S><<<1, kPrepareThreads, 0, call.stream>>>(to, loss, log_sum, static_cast<const int32_t*>(targets.data), targets.shape[0], vocabulary, ignored, grad_loss,
+                                                            grad_log_sum, call.status);
+    MOPS_CUDA_OK(cudaGetLastError());
+}
+template void prepare_rows(const Call&, const LossRows&, float*, float*, const Array&, int64_t, int64_t, const float*, const float*);
+
+namespace {
+
 // Sizes and types; the results have the type of sums.
 void check_loss(Array& A, Array& W, Array& targets, Array& loss, Array& log_sum, double scale, const std::string& op) {
     check_floating(A.type, "A", op);
@@ -172,12 +213,6 @@ void check_loss(Array& A, Array& W, Array& targets, Array& loss, Array& log_sum,
     if (W.shape[0] == 0) throw std::runtime_error("W must have a row in " + op);
     if (!(scale > 0) || std::isinf(scale)) throw std::runtime_error("scale must be positive and finite in " + op);
     for (int64_t n : {A.shape[0], A.shape[1], W.shape[0]}) fits_int32(static_cast<size_t>(n), "a size", op);
-}
-
-LossRows take_rows(Scratch& room, int64_t rows) {
-    room.take(static_cast<size_t>(2 * rows + 4) * sizeof(int32_t));
-    int32_t* p = room.as<int32_t>();
-    return {p, p + 4, p + 4 + rows};
 }
 
 unsigned blocks_for(const Call& call, int64_t n) {
@@ -250,8 +285,7 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
     Pieces<S> pieces(call, op, A, W);
     const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.part);
     const int32_t* t = static_cast<const int32_t*>(targets.data);
-    loss_prepare<S><<<1, kPrepareThreads, 0, call.stream>>>(pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), t, n, W.shape[0], ignored,
-                                                            call.status);
+    prepare_rows<S>(call, pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), targets, W.shape[0], ignored, nullptr, nullptr);
     pieces.gather(A);
     Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<S>) + static_cast<size_t>(n) * sizeof(S));
     PartSum<S>* sums = room.as<PartSum<S>>();
@@ -260,7 +294,8 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
         loss_sums<S><<<grid, 256, 0, call.stream>>>(sums, parts, v0 / pieces.part, at_target, logits, v1 - v0, static_cast<S>(scale), t, v0, pieces.part,
                                                      pieces.rows);
     });
-    loss_join<S><<<static_cast<unsigned>(n), 128, 0, call.stream>>>(static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), sums, parts, at_target, pieces.rows);
+    loss_join<S><<<static_cast<unsigned>(n), 128, 0, call.stream>>>(static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), sums, parts, at_target, pieces.rows, t, W.shape[0], ignored,
+                                                            call.status);
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("loss_sums<%s>", scalar_name<S>());
 }
@@ -271,7 +306,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     Pieces<S> pieces(call, op, A, W);
     const int64_t n = A.shape[0], columns = A.shape[1];
     const int32_t* t = static_cast<const int32_t*>(targets.data);
-    loss_prepare<S><<<1, kPrepareThreads, 0, call.stream>>>(pieces.rows, static_cast<S*>(nullptr), static_cast<S*>(nullptr), t, n, W.shape[0], ignored, call.status);
+    prepare_rows<S>(call, pieces.rows, nullptr, nullptr, targets, W.shape[0], ignored, nullptr, nullptr);
     if (columns == 0) return;
     pieces.gather(A);
     const bool need_A = grad_A.data != nullptr, need_W = grad_W.data != nullptr, widened = A.type != pieces.kType;
@@ -320,6 +355,11 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     note_kernel_f("loss_gradient<%s>", scalar_name<S>());
 }
 
+bool sixteen_bits(const Array& A) { return (A.type == MOPS_B200_F16 || A.type == MOPS_B200_BF16) && A.shape[1] > 0; }
+
+// Up to so many rows gradients are computed in f32 throughout: a row's gradient is for the most part that of its target, whose rounding to 16 bits would be an error of the row as a whole.
+constexpr int64_t kFewGradients = 256;
+
 } // namespace
 
 void linear_cross_entropy(Array loss, Array log_sum, Array A, Array W, Array targets, double scale, int64_t ignore_index) {
@@ -327,7 +367,8 @@ void linear_cross_entropy(Array loss, Array log_sum, Array A, Array W, Array tar
     check_loss(A, W, targets, loss, log_sum, scale, op);
     if (A.shape[0] == 0) return;
     Call call = begin_call();
-    if (A.type == MOPS_B200_F64) loss_forward<double>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
+    if (sixteen_bits(A)) loss_forward_mma(call, {A, W, targets, scale, ignore_index}, loss, log_sum, op);
+    else if (A.type == MOPS_B200_F64) loss_forward<double>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
     else loss_forward<float>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
     end_call(call, op.c_str(), kIndexNames, 1);
 }
@@ -357,6 +398,8 @@ void linear_cross_entropy_vjp(Array grad_A, Array grad_W, Array grad_loss, Array
     if (A.shape[0] == 0) {
         if (grad_W.data != nullptr)
             MOPS_CUDA_OK(cudaMemsetAsync(grad_W.data, 0, static_cast<size_t>(values_of(grad_W) * type_bytes(grad_W.type)), call.stream));
+    } else if (sixteen_bits(A) && A.shape[0] > kFewGradients) {
+        loss_backward_mma(call, {A, W, targets, scale, ignore_index}, grad_A, grad_W, grad_loss, grad_log_sum, loss, log_sum, op);
     } else if (A.type == MOPS_B200_F64) {
         loss_backward<double>(call, grad_A, grad_W, grad_loss, grad_log_sum, log_sum, A, W, targets, scale, ignore_index, op);
     } else {

@@ -39,7 +39,7 @@ template <bool BF16, int kActivation, int kColumns> struct GateStore {
     int64_t row = 0;
     int here = 0, column = 0;
     __device__ GateStore(const Args& a, uint32_t staging, int lane) : out{a.map, a.out, a.stride, a.columns, a.loose}, staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(int64_t r, int h, int c) { row = r, here = h, column = c; }
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) { row = r, here = h, column = piece.column; }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
         if (column + part * 64 >= out.columns) return;
         uint4 values[8];
@@ -83,7 +83,7 @@ template <bool BF16, int kActivation, int kColumns> struct GateStoreVjp {
     __device__ GateStoreVjp(const Args& a, uint32_t staging, int lane)
         : a(a), out_u{a.map_u, a.out, 2 * int64_t(a.columns), a.columns, false}, out_v{a.map_v, a.out + a.columns, 2 * int64_t(a.columns), a.columns, false},
           staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(int64_t r, int h, int c) { row = r, here = h, column = c; }
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) { row = r, here = h, column = piece.column; }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
         const int first = column + part * 64;
         if (first >= a.columns) return;

@@ -297,7 +297,8 @@ template <int kRows, int kColumns, int kDepth> struct DecodeOuter {
 template <typename T, int kRows, int kColumns>
 static __global__ void __launch_bounds__(256)
 grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t most_parts,
-                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment) {
+                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment,
+                   const float* __restrict__ factor) {
     const int lane = threadIdx.x & 31;
     const int64_t row_tiles = (height + kRows - 1) / kRows, column_tiles = (columns + kColumns - 1) / kColumns;
     const int64_t tiles = row_tiles * column_tiles;
@@ -329,6 +330,7 @@ grouped_outer_join(T* __restrict__ out, const float* __restrict__ parts, int64_t
             sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
         T* to = out + (piece.group * height + row + i) * columns + column + j;
+        if (factor != nullptr) sum.x *= *factor, sum.y *= *factor, sum.z *= *factor, sum.w *= *factor;
         const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -377,7 +379,7 @@ void join_outer(const Call& call, const OuterProblem& p, const float* parts, int
     const int64_t most = kRows * kColumns / 1024, shares = std::min(most, std::max(most / 8, ceil_div(int64_t(sm_count(call.device)) * 8, joins)));
     grouped_outer_join<T, kRows, kColumns><<<dim3(static_cast<unsigned>(joins), static_cast<unsigned>(shares)), 256, 0, call.stream>>>(
         static_cast<T*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(p.X.shape[1]),
-        static_cast<int>(p.Y.shape[1]), segment);
+        static_cast<int>(p.Y.shape[1]), segment, p.factor);
     MOPS_CUDA_OK(cudaGetLastError());
 }
 

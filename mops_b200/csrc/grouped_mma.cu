@@ -74,17 +74,23 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint
 }
 
 // Writes the 64 columns that follow `column` of a warp's 32 rows of an accumulator, `here` of which are the group's: all of them by the copy engine,
-// fewer each lane its row. Where rows of the output begin anywhere (loose), a row after the other, value by value. out: the first row of the band.
-template <bool BF16>
+// fewer each lane its row. Where rows of the output begin anywhere (loose), a row after the other, value by value. out: the first row of the band. kScaled: times `factor`.
+template <bool BF16, bool kScaled = false>
 __device__ __forceinline__ void store_columns(uint32_t accumulator, uint32_t staging, int64_t& sent, const CUtensorMap& map,
                                               uint16_t* __restrict__ out, int row, int slice, int column, int columns, int here, bool loose,
-                                              int lane) {
+                                              int lane, float factor = 1.f) {
     uint32_t r[2][32];
     tmem_load(accumulator, r[0]);
     tmem_load(accumulator + 32, r[1]);
     tmem_wait_load();
     tmem_pin(r[0]);
     tmem_pin(r[1]);
+    if constexpr (kScaled) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < 32; j++) r[h][j] = __float_as_uint(__uint_as_float(r[h][j]) * factor);
+    }
     uint4 v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) {
@@ -250,13 +256,13 @@ grouped_rows_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 }
 
 // ------------------------------------------------------------------------- outer products
-// out[g] = X[rows of g]^T Y[rows of g].
-template <bool BF16, int kColumns, bool kPair>
+// out[g] = X[rows of g]^T Y[rows of g], kScaled: times *factor.
+template <bool BF16, int kColumns, bool kPair, bool kScaled>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                   const __grid_constant__ CUtensorMap map_out, uint16_t* __restrict__ out, float* __restrict__ parts, int64_t most_parts,
                   const int32_t* __restrict__ offsets, int64_t groups, int64_t rows, int height, int columns, int64_t segment,
-                  bool loose, Status st) {
+                  bool loose, const float* __restrict__ factor, Status st) {
     extern __shared__ unsigned char raw[];
     using L = Layout<kColumns, kPair>;
     using H = Hand<L>;
@@ -265,6 +271,7 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     Block<L> block(raw, st);
     block.begin(warp);
     if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
+    const float scaled = kScaled ? __ldg(factor) : 1.f;
 
     if (warp == kPieceWarp)
         hand_out(block, rank, lane, DecodeOuter<L::kRows, kColumns, kBoxDepth>(offsets, groups, rows, height, columns, segment, lane));
@@ -374,8 +381,8 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     if (here > 0 && steps > 0) {
                         // (the copy engine leaves out what lies behind the output's last row)
                         for (int c = 0; c < wide; c += 64)
-                            store_columns<BF16>(from + c, staging, sent, map_out, to, band, piece.group,
-                                                        column + c, columns, loose ? here : 32, loose, lane);
+                            store_columns<BF16, kScaled>(from + c, staging, sent, map_out, to, band, piece.group,
+                                                         column + c, columns, loose ? here : 32, loose, lane, scaled);
                     } else { // a group without rows
                         for (int i = 0; i < here; i++)
                             for (int c = lane; c < wide; c += 32) to[static_cast<int64_t>(i) * columns + column + c] = 0;
@@ -452,8 +459,8 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
     if (rows == 0) return false;
     const bool loose = columns % 8 != 0 || reinterpret_cast<uintptr_t>(p.out.data) % 16 != 0;
     const int sms = sm_count(call.device);
-    auto launch = [&](auto type, auto width, auto paired) {
-        constexpr bool BF16 = decltype(type)::value, kPair = decltype(paired)::value;
+    auto launch_as = [&](auto type, auto width, auto paired, auto with_factor) {
+        constexpr bool BF16 = decltype(type)::value, kPair = decltype(paired)::value, kScaled = decltype(with_factor)::value;
         constexpr int kColumns = decltype(width)::value;
         using L = Layout<kColumns, kPair>;
         using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
@@ -465,14 +472,18 @@ bool multiply_outer_mma(const Call& call, const OuterProblem& p, const std::stri
         Scratch room(call);
         if (rows > segment) room.take(static_cast<size_t>(most_parts) * L::kRows * kColumns * sizeof(float));
         float* parts = room.as<float>();
-        launch_blocks<L>(call, op, grouped_outer_mma<BF16, kColumns, kPair>, tiles * (rows / segment + p.groups), x, y, out,
+        launch_blocks<L>(call, op, grouped_outer_mma<BF16, kColumns, kPair, kScaled>, tiles * (rows / segment + p.groups), x, y, out,
                          static_cast<uint16_t*>(p.out.data), parts, most_parts, p.offsets, p.groups, rows, static_cast<int>(height),
-                         static_cast<int>(columns), segment, loose, call.status);
+                         static_cast<int>(columns), segment, loose, p.factor, call.status);
         if (rows > segment) {
             join_outer<T, L::kRows, kColumns>(call, p, parts, most_parts, tiles, segment, op);
             room.free();
         }
         note_kernel_f("grouped_outer_mma<%s,%d,%s>", BF16 ? "bf16" : "f16", kColumns, kPair ? "pair" : "block");
+    };
+    auto launch = [&](auto type, auto width, auto paired) {
+        if (p.factor != nullptr) launch_as(type, width, paired, std::true_type());
+        else launch_as(type, width, paired, std::false_type());
     };
     auto by_width = [&](auto type) {
         using std::integral_constant;

@@ -14,11 +14,12 @@ struct RowsProblem {
     int64_t groups, rows, depth, columns;
 };
 
-// out[g] = X[rows of g]^T Y[rows of g]; out is contiguous.
+// out[g] = X[rows of g]^T Y[rows of g]; out is contiguous. factor: in device memory, of 16-bit results on tensor cores (more than two rows for each group) alone.
 struct OuterProblem {
     Array out, X, Y;
     const int32_t* offsets;
     int64_t groups;
+    const float* factor = nullptr;
 };
 
 // By whichever kernels fit (grouped.cu). Arrays of 16 and 32 bits are such that the copy engine can fetch them (pack.hpp), unless straight_rows() or

@@ -7,7 +7,7 @@
 //
 // E has: kHalves, kStoreWarps (4 or 8), kStaging (bytes of shared memory of each of them), Args (among the kernel's arguments), and
 //   E(args, staging, lane)                            what a storing warp keeps
-//   begin(row, here, column)                          before the accumulator is there: what can be loaded. The warp's first row, how many rows it has, the tile's first column
+//   begin(piece, row, here)                           before the accumulator is there: what can be loaded. The warp's first row, and how many it has
 //   store(accumulator, part)                          the warp's part of the columns (0 of 1, or of 2)
 //   clear()                                           rows of no group
 //   end()                                             before the block leaves
@@ -152,6 +152,25 @@ template <int kRows, int kColumns> struct DecodeTable {
     }
 };
 
+// The same with the depth cut into slices of `slice_steps` stages: a piece's first stage is in p.slot, its slice in p.row.
+template <int kRows, int kColumns> struct DecodeSlices {
+    DecodeTable<kRows, kColumns> table;
+    int slice_steps;
+    __device__ DecodeSlices(const int32_t* offsets, int64_t slices, int64_t rows, int64_t columns, int steps, int lane)
+        : table(offsets, 1, rows, columns, steps, lane), slice_steps((steps + static_cast<int>(slices) - 1) / static_cast<int>(slices)) {}
+    __device__ bool operator()(int64_t want, Piece& p) const {
+        const int64_t tiles = table.row_tiles * table.column_tiles;
+        if (tiles == 0) return false;
+        const int64_t slice = want / tiles, first = slice * slice_steps;
+        if (first >= table.steps) return false;
+        (void)table(want - slice * tiles, p);
+        p.slot = first, p.row = static_cast<int>(slice);
+        p.steps = static_cast<int>(min(int64_t(slice_steps), table.steps - first));
+        return true;
+    }
+};
+template <template <int, int> class Decode> constexpr bool kOneGroup = !std::is_same<Decode<1, 1>, DecodeRows<1, 1>>::value;
+
 // a_bytes: of a box of the first operand, which may have fewer than 128 rows where there are no more (what stands in the others does not matter). B_MN: the columns of the second operand are
 // neighbours in memory, else its depth is. map_b1: its second half.
 template <bool BF16, bool B_MN, int kColumns, bool kPair, typename E, template <int, int> class Decode>
@@ -165,7 +184,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
-    if constexpr (!std::is_same<Decode<1, 1>, DecodeTable<1, 1>>::value)
+    if constexpr (!kOneGroup<Decode>)
         if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
     auto stage_at = [&](const Turn<L::kStages>& stage) { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
     if (warp == kTilePieceWarp) {
@@ -183,7 +202,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     if (!ok) break;
                     uint64_t* full = &block.rings->stages.full[stage.at];
                     const uint32_t a = stage_at(stage), b = a + L::kA;
-                    const int deep = s * kBoxDepth;
+                    const int deep = (std::is_same<Decode<1, 1>, DecodeSlices<1, 1>>::value ? static_cast<int>(piece.slot) + s : s) * kBoxDepth;
                     H::expect(full, static_cast<uint32_t>(a_bytes) + L::kB);
                     H::fetch(a, map_a, deep, row, 0, full);
                     if constexpr (!E::kHalves) {
@@ -256,7 +275,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (Piece piece; supply.next(piece, lane);) {
             const int64_t row = piece.lo + rank * kTileRows + quadrant * 32;
             const int here = static_cast<int>(min(max(piece.hi - row, int64_t(0)), int64_t(32)));
-            work.begin(row, here, piece.column);
+            work.begin(piece, row, here);
             if (piece.group < 0) {
                 if (part == 0) work.clear();
                 continue;
@@ -280,6 +299,7 @@ struct TileProblem {
     Array A;            // rows x depth, boxable
     const int32_t* offsets;
     int64_t groups, rows, depth, columns;
+    int64_t slices = 1; // of the depth (DecodeSlices)
 };
 
 // The second operand, or a half of it: value (d, j) of group g at g * group_stride + d * depth_stride + j * column_stride, boxable.
@@ -302,9 +322,10 @@ void launch_tiles(const Call& call, const std::string& op, const TileProblem& p,
                     : tensor_map(type, o.data, p.depth, p.columns, p.groups, o.column_stride, o.group_stride, E::kHalves ? kColumns / 2 : L::kOwnColumns);
     };
     const CUtensorMap b0 = map_of(b[0]), b1 = E::kHalves ? map_of(b[1]) : b0;
-    const int64_t tiles = (std::is_same<Decode<1, 1>, DecodeTable<1, 1>>::value ? ceil_div(p.rows, L::kRows) : most_row_tiles(p.rows, p.groups, L::kRows)) *
+    const int64_t tiles = (kOneGroup<Decode> ? ceil_div(p.rows, L::kRows) * p.slices : most_row_tiles(p.rows, p.groups, L::kRows)) *
                           ceil_div(p.columns, L::kTileColumns);
-    launch_blocks<L>(call, op, tile_rows<BF16, B_MN, kColumns, kPair, E, Decode>, tiles, a, b0, b1, box * kBoxRow, args, p.offsets, p.groups, p.rows,
+    launch_blocks<L>(call, op, tile_rows<BF16, B_MN, kColumns, kPair, E, Decode>, tiles, a, b0, b1, box * kBoxRow, args, p.offsets,
+                     kOneGroup<Decode> ? p.slices : p.groups, p.rows,
                      static_cast<int>(p.depth), static_cast<int>(p.columns), call.status);
 }
 

@@ -445,7 +445,7 @@ def some_targets(R, V, kept, seed=5, ignored=-1):
 @pytest.mark.parametrize("R,V,C,kept", [
     (1, 1, 1, 1.0), (1, 2, 8, 1.0), (2, 5, 3, 1.0), (1, 5000, 64, 1.0), (3, 257, 40, 0.5), (8, 1000, 1030, 1.0), (31, 4097, 72, 0.8), (64, 63, 16, 1.0),
     (130, 300, 64, 0.9), (257, 1000, 129, 0.5), (300, 8200, 96, 0.95), (400, 129, 256, 0.7), (700, 5003, 203, 0.3), (1025, 2, 40, 0.9),
-    (2000, 77, 520, 1.0), (513, 12345, 8, 0.9), (300, 100, 1, 1.0), (5000, 600, 136, 0.02), (385, 3000, 700, 0.99)])
+    (2000, 77, 520, 1.0), (513, 12345, 8, 0.9), (2049, 3000, 64, 0.9), (4100, 511, 72, 0.4), (300, 70001, 24, 0.9), (3000, 50001, 16, 0.9), (300, 100, 1, 1.0), (5000, 600, 136, 0.02), (385, 3000, 700, 0.99)])
 def test_loss_matches_64_bits(dtype, R, V, C, kept):
     A, W = normal((R, C), dtype, 1, 2.0), normal((V, C), dtype, 2, C ** -0.5)
     check_loss(A, W, some_targets(R, V, kept), 1.25)
@@ -540,6 +540,17 @@ def test_loss_of_large_and_infinite_logits(dtype, R):
     assert (log_sum[0::2] == float("inf")).all() and (loss[0::4] == float("inf")).all()
     assert (log_sum[1::2] - math.log(V - 1)).abs().max() < 1e-5
     assert (loss[1::4] - math.log(V - 1)).abs().max() < 1e-5 and (loss[3::4] == float("inf")).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [9, 300, 2100])
+@pytest.mark.parametrize("far", [-4.0, 4.0])
+def test_loss_of_logits_far_from_zero(dtype, R, far):
+    """All logits beyond what exponentials can be taken of, to either side."""
+    V, C = 1300, 16
+    A, W = 5 + normal((R, C), dtype, 1, 0.01), far + normal((V, C), dtype, 2, 0.05)
+    check_loss(A, W, some_targets(R, V, 0.9))
 
 
 @pytest.mark.gpu
