@@ -3,7 +3,7 @@
 //   norm = sqrt(sum over all tensors of x^2), output = x min(1, max_norm / norm)
 //
 // Bounded by memory: 2 bytes a value for the norm of bf16, and 4 for its scaling, which has to read again what the norm was taken of. All tensors go in one launch, as a table among the kernel's
-// arguments (so a captured graph keeps it): their values are cut into chunks of 32 KB, of which a block takes every so many-th, and the second kernel goes through them backwards, so that it
+// arguments (so a captured graph keeps it): their values are cut into chunks, of which a block takes every so many-th, and the second kernel goes through them backwards, so that it
 // finds what was read last in L2.
 #include <vector>
 
@@ -14,9 +14,9 @@ namespace mops_b200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 32768;  // bytes
+// Packs of 16 bytes that a thread has under way, and blocks of an SM: while squares are added up, and while values are scaled.
+constexpr int kSumPacks = 8, kSumBlocks = 4, kScalePacks = 4, kScaleBlocks = 6;
 constexpr int kMostTensors = 448; // of a launch, whose arguments have 32 KB
-constexpr int kBlocks = 4;     // of an SM
 
 struct Entry {
     const void* from;
@@ -26,7 +26,7 @@ struct Entry {
     int32_t type;
 };
 template <int kMost> struct Table {
-    int n;
+    int n, chunk; // bytes
     int64_t chunks;
     Entry entry[kMost];
 };
@@ -45,19 +45,10 @@ template <int kMost> __device__ __forceinline__ Chunk find_chunk(const Table<kMo
     }
     Chunk c;
     c.entry = &table.entry[lo];
-    const int64_t size = kChunk / (c.entry->type == MOPS_B200_F64 ? 8 : c.entry->type == MOPS_B200_F32 ? 4 : 2);
+    const int64_t size = table.chunk / (c.entry->type == MOPS_B200_F64 ? 8 : c.entry->type == MOPS_B200_F32 ? 4 : 2);
     c.lo = (chunk - c.entry->first) * size;
     c.hi = min(c.lo + size, c.entry->values);
     return c;
-}
-
-// Calls body(first value, N values) for packs of a chunk, and body(value, 1) for what does not fill one; the same threads take the same values wherever a tensor begins.
-template <typename T, typename F> __device__ __forceinline__ void for_packs(const Chunk& c, F&& body) {
-    constexpr int N = kPack<T>;
-    const int64_t whole = c.lo + (c.hi - c.lo) / N * N;
-#pragma unroll 4
-    for (int64_t i = c.lo + threadIdx.x * N; i < whole; i += kThreads * N) body(i, std::integral_constant<int, N>());
-    for (int64_t i = whole + threadIdx.x; i < c.hi; i += kThreads) body(i, std::integral_constant<int, 1>());
 }
 
 // N values from or to anywhere; `aligned`: to multiples of 16 bytes.
@@ -75,6 +66,25 @@ template <int N, typename T> __device__ __forceinline__ void store_pack(T* p, co
     }
 #pragma unroll
     for (int k = 0; k < N; k++) p[k] = v.v[k];
+}
+
+// Calls body(where, pack) for packs of a chunk's n values, kInFlight of which a thread loads before it goes on with the first, and for single values where they do not fill one; the same threads take the
+// same values wherever a tensor begins.
+template <int kInFlight, typename T, typename F> __device__ __forceinline__ void for_packs(const T* __restrict__ p, int n, bool aligned, F&& body) {
+    constexpr int N = kPack<T>;
+    const int whole = n / N * N;
+    int i = threadIdx.x * N;
+    if (aligned)
+        for (; i + (kInFlight - 1) * kThreads * N < whole; i += kInFlight * kThreads * N) {
+            Pack<T, N> v[kInFlight];
+#pragma unroll
+            for (int k = 0; k < kInFlight; k++) v[k] = *reinterpret_cast<const Pack<T, N>*>(p + i + k * kThreads * N);
+#pragma unroll
+            for (int k = 0; k < kInFlight; k++) body(i + k * kThreads * N, v[k]);
+        }
+#pragma unroll 1
+    for (; i < whole; i += kThreads * N) body(i, load_pack<N>(p + i, aligned));
+    for (i = whole + threadIdx.x; i < n; i += kThreads) body(i, load_pack<1>(p + i, true));
 }
 
 template <typename F> __device__ __forceinline__ void with_type(int32_t type, F&& f) {
@@ -97,7 +107,7 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 template <int kMost>
-__global__ void __launch_bounds__(kThreads, kBlocks)
+__global__ void __launch_bounds__(kThreads, kSumBlocks)
 sum_squares(double* __restrict__ sums, const __grid_constant__ Table<kMost> table) {
     double sum = 0;
     for (int64_t chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
@@ -105,12 +115,11 @@ sum_squares(double* __restrict__ sums, const __grid_constant__ Table<kMost> tabl
         with_type(c.entry->type, [&](auto zero) {
             using T = decltype(zero);
             using S = Sum<T>;
-            const T* p = static_cast<const T*>(c.entry->from);
+            const T* p = static_cast<const T*>(c.entry->from) + c.lo;
             S part[kPack<T>] = {};
             const bool aligned = reinterpret_cast<uintptr_t>(p) % 16 == 0;
-            for_packs<T>(c, [&](int64_t i, auto width) {
-                constexpr int N = decltype(width)::value;
-                const Pack<T, N> v = load_pack<N>(p + i, aligned || N == 1);
+            for_packs<kSumPacks>(p, static_cast<int>(c.hi - c.lo), aligned, [&](int, const auto& v) {
+                constexpr int N = sizeof(v) / sizeof(T);
 #pragma unroll
                 for (int k = 0; k < N; k++) {
                     const S x = widen(v.v[k]);
@@ -143,7 +152,7 @@ join_norm(void* __restrict__ norm, bool wide, const double* __restrict__ sums, i
 }
 
 template <int kMost>
-__global__ void __launch_bounds__(kThreads, kBlocks)
+__global__ void __launch_bounds__(kThreads, kScaleBlocks)
 scale_values(void* norm, bool wide, const double* __restrict__ sums, int n, double max_norm, const __grid_constant__ Table<kMost> table) {
     const double value = join_sums(sums, n);
     if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) write_norm(norm, wide, value);
@@ -154,14 +163,13 @@ scale_values(void* norm, bool wide, const double* __restrict__ sums, int n, doub
         with_type(c.entry->type, [&](auto zero) {
             using T = decltype(zero);
             using S = Sum<T>;
-            const T* p = static_cast<const T*>(c.entry->from);
-            T* q = static_cast<T*>(c.entry->to);
+            const T* p = static_cast<const T*>(c.entry->from) + c.lo;
+            T* q = static_cast<T*>(c.entry->to) + c.lo;
             const S f = static_cast<S>(factor);
             const bool as_it_is = factor == 1.0;
             const bool from_aligned = reinterpret_cast<uintptr_t>(p) % 16 == 0, to_aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0;
-            for_packs<T>(c, [&](int64_t i, auto width) {
-                constexpr int N = decltype(width)::value;
-                Pack<T, N> v = load_pack<N>(p + i, from_aligned || N == 1);
+            for_packs<kScalePacks>(p, static_cast<int>(c.hi - c.lo), from_aligned, [&](int i, auto v) {
+                constexpr int N = sizeof(v) / sizeof(T);
                 if (!as_it_is) {
 #pragma unroll
                     for (int k = 0; k < N; k++) v.v[k] = narrow<T>(widen(v.v[k]) * f);
@@ -215,17 +223,23 @@ Tensors check_tensors(Array& norm, const Array* outputs, const Array* gradients,
     return t;
 }
 
-template <typename F> void for_tables(const Tensors& t, F&& f) {
+// Chunks of 8 KB where that leaves no block without one, up to 128 KB where there are several for each: a block that goes on to another chunk has nothing under way meanwhile.
+template <typename F> void for_tables(const Tensors& t, int64_t blocks, F&& f) {
+    int64_t bytes = 0;
+    for (const Entry& e : t.entries) bytes += e.values * type_bytes(e.type);
+    int chunk = 8192;
+    while (chunk < 131072 && bytes / chunk > 4 * blocks) chunk *= 2;
     auto go = [&](auto most) {
         constexpr int kMost = decltype(most)::value;
         for (size_t at = 0; at < t.entries.size(); at += kMost) {
             Table<kMost> table;
             table.n = static_cast<int>(std::min<size_t>(kMost, t.entries.size() - at));
+            table.chunk = chunk;
             table.chunks = 0;
             for (int i = 0; i < table.n; i++) {
                 table.entry[i] = t.entries[at + i];
                 table.entry[i].first = table.chunks;
-                table.chunks += ceil_div(table.entry[i].values * type_bytes(table.entry[i].type), kChunk);
+                table.chunks += ceil_div(table.entry[i].values * type_bytes(table.entry[i].type), chunk);
             }
             f(table, most);
         }
@@ -238,12 +252,12 @@ void norm_of(Array norm, const Array* outputs, const Array* gradients, int64_t n
     const Tensors t = check_tensors(norm, outputs, gradients, n, op);
     if (outputs != nullptr && !(max_norm >= 0)) throw std::runtime_error("max_norm must not be negative in " + op);
     Call call = begin_call();
-    const int64_t most = int64_t(sm_count(call.device)) * kBlocks, launches = ceil_div(static_cast<int64_t>(t.entries.size()), 32);
+    const int64_t most = int64_t(sm_count(call.device)) * kSumBlocks, most_scaling = int64_t(sm_count(call.device)) * kScaleBlocks, launches = ceil_div(static_cast<int64_t>(t.entries.size()), 32);
     Scratch room(call, static_cast<size_t>(most * std::max<int64_t>(launches, 1)) * sizeof(double));
     double* sums = room.as<double>();
     const bool wide = norm.type == MOPS_B200_F64;
     int64_t parts = 0;
-    for_tables(t, [&](const auto& table, auto most_tensors) {
+    for_tables(t, most, [&](const auto& table, auto most_tensors) {
         const int64_t blocks = std::min(table.chunks, most);
         sum_squares<decltype(most_tensors)::value><<<static_cast<unsigned>(blocks), kThreads, 0, call.stream>>>(sums + parts, table);
         parts += blocks;
@@ -251,8 +265,8 @@ void norm_of(Array norm, const Array* outputs, const Array* gradients, int64_t n
     MOPS_CUDA_OK(cudaGetLastError());
     bool written = false;
     if (outputs != nullptr)
-        for_tables(t, [&](const auto& table, auto most_tensors) {
-            const int64_t blocks = std::min(table.chunks, most);
+        for_tables(t, most, [&](const auto& table, auto most_tensors) {
+            const int64_t blocks = std::min(table.chunks, most_scaling);
             scale_values<decltype(most_tensors)::value><<<static_cast<unsigned>(blocks), kThreads, 0, call.stream>>>(
                 written ? nullptr : norm.data, wide, sums, static_cast<int>(parts), max_norm, table);
             written = true;

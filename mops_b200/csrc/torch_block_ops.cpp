@@ -4,6 +4,8 @@
 // device without synchronising it, so an index out of range is not reported: its row is zero, and it gives no gradient.
 #include "torch_common.hpp"
 
+#include <ATen/cuda/EmptyTensor.h>
+
 namespace {
 
 using namespace mops_torch;
@@ -404,16 +406,26 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 void check_gradients(const tensor_list& gradients, const char* op) {
     if (gradients.empty()) C10_THROW_ERROR(ValueError, "no gradients in " + std::string(op));
     same_device(gradients);
+    const bool recorded = at::GradMode::is_enabled();
     for (const Tensor& g : gradients) {
-        block_types({g});
-        if (differentiated({&g})) C10_THROW_ERROR(NotImplementedError, "derivatives are not supported in CUDA for " + std::string(op));
+        const auto type = g.scalar_type();
+        if (type != torch::kF64 && type != torch::kF32 && type != torch::kF16 && type != torch::kBFloat16) block_types({g}); // (says why not)
+        if ((recorded && g.requires_grad()) || g._fw_grad(/*level=*/0).defined())
+            C10_THROW_ERROR(NotImplementedError, "derivatives are not supported in CUDA for " + std::string(op));
     }
     cuda_only(gradients[0], op);
 }
 
 // A tensor whose values fill a piece of memory, as one dimension.
 mops_b200_array_t flat(const Tensor& t) {
-    mops_b200_array_t a = array(t.dim() == 1 ? t : t.as_strided({t.numel()}, {1}));
+    mops_b200_array_t a{};
+    a.data = t.data_ptr();
+    a.type = t.scalar_type() == torch::kF64         ? MOPS_B200_F64
+             : t.scalar_type() == torch::kF16       ? MOPS_B200_F16
+             : t.scalar_type() == torch::kBFloat16  ? MOPS_B200_BF16
+                                                    : MOPS_B200_F32;
+    a.dimensions = 1;
+    a.shape[0] = t.numel();
     a.stride[0] = 1;
     return a;
 }
@@ -433,15 +445,39 @@ Tensor empty_norm(const tensor_list& gradients) {
     return torch::empty({}, gradients[0].options().dtype(wide ? torch::kF64 : torch::kF32));
 }
 
-tensor_list all_flat(const tensor_list& gradients) {
+void make_flat(tensor_list& gradients) {
+    for (Tensor& g : gradients)
+        if (!is_flat(g)) g = g.resolve_neg().resolve_conj().contiguous();
+}
+
+// Tensors like these. Many small ones share one piece of memory: to ask for each would take the host longer than all of them the kernels (two dozen tensors of some 10^5 values: 58 us a call,
+// 23 together).
+constexpr int64_t kMostShared = 16 << 20; // bytes
+tensor_list empty_like_all(const tensor_list& tensors) {
     tensor_list r;
-    for (const Tensor& g : gradients) r.push_back(is_flat(g) ? g : g.resolve_neg().resolve_conj().contiguous());
+    r.reserve(tensors.size());
+    const c10::cuda::CUDAGuard guard(tensors[0].device());
+    const auto places = [](const Tensor& t) { return (t.numel() * static_cast<int64_t>(t.element_size()) + 511) / 512 * 512; };
+    int64_t bytes = 0;
+    for (const Tensor& t : tensors) bytes += places(t);
+    if (tensors.size() < 2 || bytes > kMostShared) {
+        for (const Tensor& t : tensors) r.push_back(at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.options()));
+        return r;
+    }
+    const Tensor all = at::detail::empty_cuda({bytes}, torch::kByte, tensors[0].device(), std::nullopt);
+    int64_t at = 0;
+    for (const Tensor& t : tensors) {
+        Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), t.dtype());
+        part.unsafeGetTensorImpl()->set_sizes_and_strides(t.sizes(), t.strides(), at / static_cast<int64_t>(t.element_size()));
+        r.push_back(std::move(part));
+        at += places(t);
+    }
     return r;
 }
 
 Tensor gradient_norm(tensor_list gradients) {
     check_gradients(gradients, "gradient_norm");
-    gradients = all_flat(gradients);
+    make_flat(gradients);
     Tensor norm = empty_norm(gradients);
     const auto table = table_of(gradients);
     on_stream_of(norm, [&] { checked(mops_b200_cuda_gradient_norm(flat(norm), table.data(), static_cast<int64_t>(table.size()))); });
@@ -450,10 +486,9 @@ Tensor gradient_norm(tensor_list gradients) {
 
 std::tuple<Tensor, tensor_list> clip_gradient_norm(tensor_list gradients, double max_norm) {
     check_gradients(gradients, "clip_gradient_norm");
-    gradients = all_flat(gradients);
+    make_flat(gradients);
     Tensor norm = empty_norm(gradients);
-    tensor_list clipped;
-    for (const Tensor& g : gradients) clipped.push_back(torch::empty_like(g));
+    tensor_list clipped = empty_like_all(gradients);
     const auto table = table_of(gradients), results = table_of(clipped);
     on_stream_of(norm, [&] {
         checked(mops_b200_cuda_clip_gradient_norm(flat(norm), results.data(), table.data(), static_cast<int64_t>(table.size()), max_norm));
