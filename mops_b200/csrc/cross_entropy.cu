@@ -6,13 +6,15 @@
 //   grad_A = scale dx W, grad_W = scale dx^T A
 //
 // A piece of the vocabulary at a time: its logits are a product into scratch memory, of which sums are taken, or which become dx where they stand and are multiplied by the
-// piece's rows of W and, the other way, by A. The gradients compute the logits again. Here: f32 and f64, and f16 and bf16, widened to f32, where there are few rows to differentiate; the rest of
+// piece's rows of W and, the other way, by A. The gradients compute the logits again. In f32 the logits of more than a few rows are worked on where they are summed (LossStore32, GradientStore32)
+// and never stored. Here: f32 and f64, and f16 and bf16, widened to f32, where there are few rows to differentiate; the rest of
 // them is in cross_entropy_mma.cu.
 #include "block_ops.hpp"
 #include "convert.cuh"
 #include "grouped_mma.hpp"
 #include "loss_rows.cuh"
 #include "pack.hpp"
+#include "split_rows.cuh"
 
 namespace mops_b200 {
 namespace {
@@ -177,6 +179,107 @@ loss_gradient(S* __restrict__ logits, int64_t columns, S scale, const S* __restr
     }
 }
 
+// ---- f32, where the logits are summed: a lane has 64 of its row
+struct LossStore32 {
+    static constexpr bool kHalves = false;
+    static constexpr int kOwn = kSplitColumns / 2;
+    struct Args {
+        PartSum<float>* parts;
+        int64_t n;
+        float* at_target;
+        const int32_t* target;
+        int columns;
+        float scale;
+    };
+    const Args& a;
+    int lane;
+    int64_t row = 0;
+    int here = 0, first = 0, target = -1;
+    __device__ LossStore32(const Args& a, uint32_t, int lane) : a(a), lane(lane) {}
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
+        row = r + lane, here = h, first = piece.column + half * kOwn;
+        target = lane < here ? a.target[row] : -1;
+    }
+    __device__ __forceinline__ void store(float (&sum)[kOwn]) const {
+        const int wide = min(a.columns - first, kOwn);
+        if (wide <= 0) return;
+        const int at = target - first;
+        if (__any_sync(kFullMask, at >= 0 && at < wide)) {
+            float x = 0;
+#pragma unroll
+            for (int j = 0; j < kOwn; j++)
+                if (j == at) x = sum[j];
+            if (at >= 0 && at < wide) a.at_target[row] = x * a.scale;
+        }
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < kOwn; j++) {
+            if (wide < kOwn && j >= wide) sum[j] = -INFINITY;
+            most[j % 4] = fmaxf(most[j % 4], sum[j]);
+        }
+        PartSum<float> part{fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * a.scale, 0.f};
+        const float base = PartSum<float>::from(part.top);
+        float all[4] = {};
+#pragma unroll
+        for (int j = 0; j < kOwn; j++) all[j % 4] += expf(fmaf(sum[j], a.scale, -base));
+        part.sum = (all[0] + all[1]) + (all[2] + all[3]);
+        if (lane < here) a.parts[row * a.n + first / kOwn] = part;
+    }
+    __device__ __forceinline__ void clear() const {}
+    __device__ __forceinline__ void end() const {}
+};
+
+struct GradientStore32 {
+    static constexpr bool kHalves = false;
+    static constexpr int kOwn = kSplitColumns / 2;
+    struct Args {
+        CUtensorMap map;
+        float* out;
+        int64_t stride;
+        int columns, first_column; // of the piece
+        float scale;
+        const float *grad_loss, *grad_log_sum, *log_sum;
+        LossRows rows;
+    };
+    const Args& a;
+    BoxOut32 out;
+    uint32_t staging;
+    int lane;
+    int64_t row = 0;
+    int here = 0, first = 0, target = -1;
+    float base = 0, both = 0, of_loss = 0; // with the scale of the gradients
+    __device__ GradientStore32(const Args& a, uint32_t staging, int lane) : a(a), out{a.map, a.out, a.stride, a.columns, false}, staging(staging), lane(lane) {}
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
+        row = r, here = h, first = piece.column + half * kOwn;
+        if (lane < here) {
+            const int64_t of = a.rows.order[row + lane];
+            target = a.rows.target[row + lane] - a.first_column;
+            const float l = a.grad_loss != nullptr ? a.grad_loss[of] : 0.f, m = a.grad_log_sum != nullptr ? a.grad_log_sum[of] : 0.f;
+            base = a.log_sum[of], both = (l + m) * a.scale, of_loss = l * a.scale;
+        }
+    }
+    __device__ __forceinline__ void store(const float (&sum)[kOwn]) const {
+#pragma unroll
+        for (int c = 0; c < kOwn; c += 32) {
+            if (first + c >= a.columns) return;
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = both * expf(fmaf(sum[c + j], a.scale, -base));
+            const int at = target - first - c;
+            if (__any_sync(kFullMask, at >= 0 && at < 32)) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (j == at) v[j] -= of_loss;
+            }
+            out.put(v, staging, row, here, first + c, lane);
+        }
+    }
+    __device__ __forceinline__ void clear() const {}
+    __device__ __forceinline__ void end() const {
+        if (lane == 0) boxes_left<0>();
+    }
+};
+
 const char* const kIndexNames[] = {"targets"};
 
 } // namespace
@@ -228,6 +331,7 @@ template <typename S> struct Pieces {
     LossRows rows;
     Array A, W, logits;
     int64_t width, part; // columns of a piece, and of a part of it
+    bool fused;          // worked on where they are summed
     static constexpr int32_t kType = sizeof(S) == 8 ? MOPS_B200_F64 : MOPS_B200_F32;
 
     Pieces(const Call& call, const std::string& op, const Array& a, const Array& w)
@@ -244,8 +348,10 @@ template <typename S> struct Pieces {
         width = width >= kPartColumns ? width / kPartColumns * kPartColumns : width / 256 * 256;
         part = std::min(width, kPartColumns);
         width = std::min(width, W.shape[0]);
-        room_logits.take(static_cast<size_t>(n * width) * sizeof(S) + 16);
+        fused = kType == MOPS_B200_F32 && columns > 0 && !straight_rows(matrices(0, W.shape[0]), n, false);
     }
+    void take_logits() { room_logits.take(static_cast<size_t>(A.shape[0] * (width + 3)) * sizeof(S) + 16); }
+    TileProblem problem(int64_t columns) const { return {A, rows.offsets, 1, A.shape[0], A.shape[1], columns}; }
     void gather(const Array& a) {
         if (a.shape[1] == 0) return;
         for_type(a.type, [&](auto zero) {
@@ -267,6 +373,7 @@ template <typename S> struct Pieces {
         return m;
     }
     template <typename F> void for_each(F&& f) {
+        take_logits();
         for (int64_t v0 = 0; v0 < W.shape[0]; v0 += width) {
             const int64_t v1 = std::min(v0 + width, W.shape[0]);
             const Array m = matrices(v0, v1);
@@ -283,14 +390,22 @@ template <typename S>
 void loss_forward(const Call& call, const Array& loss, const Array& log_sum, const Array& A, const Array& W, const Array& targets, double scale,
                   int64_t ignored, const std::string& op) {
     Pieces<S> pieces(call, op, A, W);
-    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.part);
+    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.fused ? LossStore32::kOwn : pieces.part);
     const int32_t* t = static_cast<const int32_t*>(targets.data);
     prepare_rows<S>(call, pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), targets, W.shape[0], ignored, nullptr, nullptr);
     pieces.gather(A);
     Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<S>) + static_cast<size_t>(n) * sizeof(S));
     PartSum<S>* sums = room.as<PartSum<S>>();
     S* at_target = reinterpret_cast<S*>(sums + n * parts);
-    pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
+    if constexpr (sizeof(S) == 4) {
+        if (pieces.fused) {
+            const LossStore32::Args args{sums, parts, at_target, pieces.rows.target, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
+            const TileOperand w{pieces.W.data, 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
+            launch_split<false, LossStore32, DecodeTable>(call, op, pieces.problem(W.shape[0]), operands, args);
+            note_kernel("loss_rows_split");
+        }
+    }
+    if (!pieces.fused) pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
         loss_sums<S><<<grid, 256, 0, call.stream>>>(sums, parts, v0 / pieces.part, at_target, logits, v1 - v0, static_cast<S>(scale), t, v0, pieces.part,
                                                      pieces.rows);
     });
@@ -315,10 +430,8 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     if (need_A) room_A.take(bytes);
     if (need_A && pieces.width < W.shape[0]) room_more.take(bytes);
     if (need_W && widened) room_W.take(static_cast<size_t>(pieces.width * columns) * sizeof(S));
-    pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
-        loss_gradient<S><<<grid, 256, 0, call.stream>>>(logits, v1 - v0, static_cast<S>(scale), static_cast<const S*>(grad_loss.data),
-                                                        static_cast<const S*>(grad_log_sum.data), static_cast<const S*>(log_sum.data), t, v0, pieces.part, pieces.rows);
-        Array m = pieces.matrices(v0, v1), dx = pieces.logits, a = pieces.A;
+    auto multiply = [&](int64_t v0, int64_t v1, Array dx) {
+        Array m = pieces.matrices(v0, v1), a = pieces.A;
         m.shape[1] = v1 - v0, m.shape[2] = columns; // (v1 - v0) x C
         std::swap(m.stride[1], m.stride[2]);
         Packing packing(call);
@@ -345,7 +458,31 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
                 });
         }
         packing.release();
-    });
+    };
+    if (pieces.fused) {
+        if constexpr (sizeof(S) == 4) {
+            pieces.take_logits();
+            const int64_t stride = (pieces.width + 3) / 4 * 4;
+            for (int64_t v0 = 0; v0 < W.shape[0]; v0 += pieces.width) {
+                const int64_t v1 = std::min(v0 + pieces.width, W.shape[0]);
+                Array dx = contiguous(pieces.room_logits.template as<void>(), pieces.kType, n, v1 - v0);
+                dx.stride[0] = stride;
+                const GradientStore32::Args args{tensor_map(pieces.kType, dx.data, v1 - v0, n, 1, stride, 0, 32), static_cast<float*>(dx.data), stride,
+                                                 static_cast<int>(v1 - v0), static_cast<int>(v0), static_cast<float>(scale), static_cast<const float*>(grad_loss.data),
+                                                 static_cast<const float*>(grad_log_sum.data), static_cast<const float*>(log_sum.data), pieces.rows};
+                const TileOperand w{static_cast<float*>(pieces.W.data) + v0 * pieces.W.stride[0], 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
+                launch_split<false, GradientStore32, DecodeTable>(call, op, pieces.problem(v1 - v0), operands, args);
+                multiply(v0, v1, dx);
+                MOPS_CUDA_OK(cudaGetLastError());
+            }
+        }
+    } else {
+        pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
+            loss_gradient<S><<<grid, 256, 0, call.stream>>>(logits, v1 - v0, static_cast<S>(scale), static_cast<const S*>(grad_loss.data),
+                                                            static_cast<const S*>(grad_log_sum.data), static_cast<const S*>(log_sum.data), t, v0, pieces.part, pieces.rows);
+            multiply(v0, v1, pieces.logits);
+        });
+    }
     if (need_A)
         for_type(grad_A.type, [&](auto zero) {
             using T = decltype(zero);

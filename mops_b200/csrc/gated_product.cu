@@ -5,9 +5,9 @@
 //   dV = grad_output f(U), dU = grad_output V f'(U)
 //   grad_A[r,:] = [dU dV] W[g]^T, grad_W[g] = A[rows of g]^T [dU dV]
 //
-// Here: f32 and f64. U and V, side by side in scratch memory, are one grouped product; a pass over them makes the output of them, or, where
-// they stood, dU and dV, of which the gradients are the grouped products that they are for a plain layer. f16 and bf16 are widened to f32 for that, so U, V, dU and dV are never
-// rounded to 16 bits; that is done where there are few rows to differentiate, the rest of f16 and bf16 is in gated_mma.cu.
+// On tensor cores U and V are gated where they are summed (gated_mma.cu, gated_split.cu). Here: f64, and f32 in the forms that those leave to other kernels (few rows, halves that begin anywhere). U and V, side by
+// side in scratch memory, are one grouped product; a pass over them makes the output of them, or, where they stood, dU and dV, of which the gradients are the grouped products that they are for a plain
+// layer. f16 and bf16 are widened to f32 where there are few rows to differentiate.
 #include "activation.cuh"
 #include "block_ops.hpp"
 #include "convert.cuh"
@@ -64,14 +64,17 @@ void check_gated(Array& A, Array& W, Array& offsets, Array& rows, const char* ro
         throw std::runtime_error("unknown activation " + std::to_string(activation) + " in " + op);
 }
 
-// In f32 (f64 for f64), what the products are made of: A and W, widened where they have 16 bits, and U and V side by side.
+// In f32 (f64 for f64), what the products are made of: A and W, widened where they have 16 bits, and U and V, or dU and dV, side by side.
 struct Widened {
+    const Call& call;
+    const std::string& op;
     Scratch room_A, room_W, room_uv;
     Packing packing;
     Array A, W, uv;
     int32_t type;
-    Widened(const Call& call, const Array& a, const Array& w, const int32_t* offsets, const std::string& op)
-        : room_A(call), room_W(call), room_uv(call), packing(call), A(a), W(w), type(a.type == MOPS_B200_F64 ? MOPS_B200_F64 : MOPS_B200_F32) {
+    bool fused = false; // gated where they are summed
+    Widened(const Call& call, const Array& a, const Array& w, const std::string& op)
+        : call(call), op(op), room_A(call), room_W(call), room_uv(call), packing(call), A(a), W(w), type(a.type == MOPS_B200_F64 ? MOPS_B200_F64 : MOPS_B200_F32) {
         if (type != a.type) {
             room_A.take(static_cast<size_t>(values_of(a)) * 4 + 16);
             room_W.take(static_cast<size_t>(values_of(w)) * 4 + 16);
@@ -82,9 +85,18 @@ struct Widened {
             packing.add(A);
             packing.add(W);
             packing.run();
+            fused = A.shape[0] > 0 && W.shape[2] > 0 && (W.stride[2] != 1 || W.shape[2] % 8 == 0);
         }
+    }
+    GatedProblem problem(const int32_t* offsets, int32_t activation) const {
+        return {A, W, offsets, W.shape[0], A.shape[0], A.shape[1], W.shape[2] / 2, activation};
+    }
+    void take_uv() {
         room_uv.take(static_cast<size_t>(A.shape[0] * W.shape[2] * type_bytes(type)) + 16);
         uv = contiguous(room_uv.as<void>(), type, A.shape[0], W.shape[2]);
+    }
+    void multiply(const int32_t* offsets) {
+        take_uv();
         multiply_rows(call, {uv, A, W, W.stride[1], W.stride[2], offsets, W.shape[0], A.shape[0], A.shape[1], W.shape[2]}, op);
     }
 };
@@ -185,7 +197,13 @@ void grouped_gated_product(Array output, Array A, Array W, Array offsets, int32_
         end_call(call, op.c_str(), kIndexNames, 1);
         return;
     }
-    Widened wide(call, A, W, starts, op);
+    Widened wide(call, A, W, op);
+    if (wide.fused && A.type == MOPS_B200_F32) {
+        gated_rows_split(call, wide.problem(starts, activation), output, op);
+        end_call(call, op.c_str(), kIndexNames, 1);
+        return;
+    }
+    wide.multiply(starts);
     for_types(A.type, [&](auto zero, auto sum) {
         using T = decltype(zero);
         using S = decltype(sum);
@@ -226,8 +244,20 @@ void grouped_gated_product_vjp(Array grad_A, Array grad_W, Array grad_output, Ar
         end_call(call, op.c_str(), kIndexNames, 1);
         return;
     }
-    Widened wide(call, A, W, starts, op);
-    if (rows > 0 && columns > 0) {
+    Widened wide(call, A, W, op);
+    if (wide.fused) {
+        Scratch room(call);
+        Array grad = grad_output;
+        if (A.type != wide.type) {
+            room.take(static_cast<size_t>(values_of(grad)) * 4 + 16);
+            grad = converted(call, grad_output, room.as<float>(), wide.type);
+        }
+        wide.take_uv();
+        gated_rows_vjp_split(call, wide.problem(starts, activation), wide.uv, grad, op);
+    } else {
+        wide.multiply(starts);
+    }
+    if (!wide.fused && rows > 0 && columns > 0) {
         for_types(A.type, [&](auto zero, auto sum) {
             using T = decltype(zero);
             using S = decltype(sum);

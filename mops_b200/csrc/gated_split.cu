@@ -1,0 +1,131 @@
+// grouped_gated_product on tensor cores, for f32: products in three bf16 parts (grouped_split.cu), whose sums of U and V are gated in registers.
+#include "activation.cuh"
+#include "gated_mma.hpp"
+#include "split_rows.cuh"
+
+namespace mops_b200 {
+namespace {
+
+template <int kActivation> struct GateStore32 {
+    static constexpr bool kHalves = true;
+    struct Args {
+        CUtensorMap map;
+        float* out;
+        int columns;
+        bool loose;
+    };
+    BoxOut32 out;
+    uint32_t staging;
+    int lane;
+    int64_t row = 0;
+    int here = 0, column = 0;
+    __device__ GateStore32(const Args& a, uint32_t staging, int lane) : out{a.map, a.out, a.columns, a.columns, a.loose}, staging(staging), lane(lane) {}
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) { row = r, here = h, column = piece.column + half * 32; }
+    __device__ __forceinline__ void store(const float (&sum)[64]) const {
+        if (column >= out.columns) return;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = Gate<kActivation, float>(sum[j]).value * sum[32 + j];
+        out.put(v, staging, row, here, column, lane);
+    }
+    __device__ __forceinline__ void clear() const { out.clear(row, here, column, kSplitColumns / 2, lane); }
+    __device__ __forceinline__ void end() const {
+        if (lane == 0) boxes_left<0>();
+    }
+};
+
+template <int kActivation> struct GateStoreVjp32 {
+    static constexpr bool kHalves = true;
+    struct Args {
+        CUtensorMap map_u, map_v;
+        float* out;
+        int64_t stride;
+        int columns; // of dU
+        bool loose;
+        const float* grad;
+        int64_t grad_stride;
+        bool grad_aligned; // rows begin on multiples of 16 bytes
+    };
+    const Args& a;
+    BoxOut32 out_u, out_v;
+    uint32_t staging;
+    int lane;
+    int64_t row = 0;
+    int here = 0, column = 0;
+    __device__ GateStoreVjp32(const Args& a, uint32_t staging, int lane)
+        : a(a), out_u{a.map_u, a.out, a.stride, a.columns, a.loose}, out_v{a.map_v, a.out + a.columns, a.stride, a.columns, a.loose}, staging(staging), lane(lane) {}
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) { row = r, here = h, column = piece.column + half * 32; }
+    __device__ __forceinline__ void store(const float (&sum)[64]) const {
+        if (column >= a.columns) return;
+        const float* from = a.grad + (row + lane) * a.grad_stride + column;
+        float u[32], v[32];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int n = lane < here ? a.columns - column - 4 * j : 0; // values that there are
+            float4 g = make_float4(0, 0, 0, 0);
+            if (a.grad_aligned && n >= 4) g = *reinterpret_cast<const float4*>(from + 4 * j);
+            else {
+                if (n > 0) g.x = from[4 * j];
+                if (n > 1) g.y = from[4 * j + 1];
+                if (n > 2) g.z = from[4 * j + 2];
+                if (n > 3) g.w = from[4 * j + 3];
+            }
+            const float d[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const Gate<kActivation, float> gate(sum[4 * j + k]);
+                u[4 * j + k] = d[k] * sum[32 + 4 * j + k] * gate.slope;
+                v[4 * j + k] = d[k] * gate.value;
+            }
+        }
+        out_u.put(u, staging, row, here, column, lane);
+        out_v.put(v, staging, row, here, column, lane);
+    }
+    __device__ __forceinline__ void clear() const {} // (nothing reads those of rows of no group)
+    __device__ __forceinline__ void end() const {
+        if (lane == 0) boxes_left<0>();
+    }
+};
+
+template <typename E> void launch_gated(const Call& call, const GatedProblem& p, const typename E::Args& args, const char* name, const std::string& op) {
+    const TileProblem problem{p.A, p.offsets, p.groups, p.rows, p.depth, p.columns};
+    const TileOperand halves[2] = {{p.half(0), p.W.stride[1], p.W.stride[2], p.W.stride[0]}, {p.half(1), p.W.stride[1], p.W.stride[2], p.W.stride[0]}};
+    if (p.by_columns()) launch_split<true, E, DecodeRows>(call, op, problem, halves, args);
+    else launch_split<false, E, DecodeRows>(call, op, problem, halves, args);
+    note_kernel_f("%s<%s>", name, p.by_columns() ? "columns" : "depth");
+    MOPS_CUDA_OK(cudaGetLastError());
+}
+
+} // namespace
+
+void gated_rows_split(const Call& call, const GatedProblem& p, const Array& output, const std::string& op) {
+    for_activation(p.activation, [&](auto activation) {
+        using E = GateStore32<decltype(activation)::value>;
+        const int64_t columns = output.shape[1];
+        typename E::Args args{};
+        args.loose = columns % 4 != 0 || reinterpret_cast<uintptr_t>(output.data) % 16 != 0;
+        if (!args.loose) args.map = tensor_map(MOPS_B200_F32, output.data, columns, p.rows, 1, columns, 0, 32);
+        args.out = static_cast<float*>(output.data), args.columns = static_cast<int>(columns);
+        launch_gated<E>(call, p, args, "gated_rows_split", op);
+    });
+}
+
+void gated_rows_vjp_split(const Call& call, const GatedProblem& p, const Array& to, const Array& grad, const std::string& op) {
+    for_activation(p.activation, [&](auto activation) {
+        using E = GateStoreVjp32<decltype(activation)::value>;
+        const int64_t columns = grad.shape[1];
+        typename E::Args args{};
+        float* out = static_cast<float*>(to.data);
+        args.loose = columns % 4 != 0;
+        if (!args.loose) {
+            args.map_u = tensor_map(MOPS_B200_F32, out, columns, p.rows, 1, to.stride[0], 0, 32);
+            args.map_v = tensor_map(MOPS_B200_F32, out + columns, columns, p.rows, 1, to.stride[0], 0, 32);
+        }
+        args.out = out, args.stride = to.stride[0], args.columns = static_cast<int>(columns);
+        args.grad = static_cast<const float*>(grad.data), args.grad_stride = grad.stride[0];
+        args.grad_aligned = reinterpret_cast<uintptr_t>(grad.data) % 16 == 0 && grad.stride[0] % 4 == 0;
+        launch_gated<E>(call, p, args, "gated_rows_vjp_split", op);
+    });
+}
+
+} // namespace mops_b200
