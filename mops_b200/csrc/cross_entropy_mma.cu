@@ -41,7 +41,7 @@ template <int kColumns> struct LossStore {
     int64_t row = 0;
     int here = 0, column = 0, target = -1;
     __device__ LossStore(const Args& a, uint32_t, int lane) : a(a), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) {
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) {
         row = r + lane, here = h, column = piece.column;
         target = lane < here ? a.target[row] : -1;
     }
@@ -113,7 +113,7 @@ template <bool BF16, int kColumns> struct GradientStore {
     int here = 0, column = 0;
     RowFactors f{};
     __device__ GradientStore(const Args& a, uint32_t staging, int lane) : a(a), out{a.map, a.out, a.stride, a.columns, false}, staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) {
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) {
         row = r, here = h, column = piece.column;
         if (lane < here) {
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(a.factors + row + lane));
@@ -179,7 +179,7 @@ template <int kColumns> struct SumStore {
     int64_t row = 0;
     int here = 0, column = 0, slice = 0;
     __device__ SumStore(const Args& a, uint32_t staging, int lane) : a(a), staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) { row = r, here = h, column = piece.column, slice = piece.row; }
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) { row = r, here = h, column = piece.column, slice = piece.row; }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
 #pragma unroll 1
         for (int c = part * kOwn; c < part * kOwn + kOwn; c += 32) {

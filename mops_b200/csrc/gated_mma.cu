@@ -39,7 +39,7 @@ template <bool BF16, int kActivation, int kColumns> struct GateStore {
     int64_t row = 0;
     int here = 0, column = 0;
     __device__ GateStore(const Args& a, uint32_t staging, int lane) : out{a.map, a.out, a.stride, a.columns, a.loose}, staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) { row = r, here = h, column = piece.column; }
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) { row = r, here = h, column = piece.column; }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
         if (column + part * 64 >= out.columns) return;
         uint4 values[8];
@@ -80,28 +80,24 @@ template <bool BF16, int kActivation, int kColumns> struct GateStoreVjp {
     int lane;
     int64_t row = 0;
     int here = 0, column = 0;
+    bool fetched = false; // the gradient's rows are in the staging memory
     __device__ GateStoreVjp(const Args& a, uint32_t staging, int lane)
         : a(a), out_u{a.map_u, a.out, 2 * int64_t(a.columns), a.columns, false}, out_v{a.map_v, a.out + a.columns, 2 * int64_t(a.columns), a.columns, false},
           staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h) { row = r, here = h, column = piece.column; }
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int part) {
+        row = r, here = h, column = piece.column;
+        const int first = column + part * 64;
+        fetched = a.grad_aligned && piece.group >= 0 && here > 0 && first + 64 <= a.grad_columns;
+        if (fetched) RowsIn::fetch(staging, a.grad + row * a.grad_stride + first, a.grad_stride * 2, here, lane);
+    }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
         const int first = column + part * 64;
         if (first >= a.columns) return;
         uint4 grad_u[8], grad_v[8];
         const T* from = a.grad + (row + lane) * a.grad_stride + first;
+        if (fetched) RowsIn::wait();
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            Pack<T, 8> g[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int c = h * 32 + j * 8, n = lane < here ? a.grad_columns - first - c : 0; // values that there are
-                if (a.grad_aligned && n >= 8) {
-                    g[j] = *reinterpret_cast<const Pack<T, 8>*>(from + c);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) g[j].v[k] = k < n ? from[c + k] : T(0.f);
-                }
-            }
             uint32_t u[32], v[32];
             tmem_load(accumulator + part * 64 + h * 32, u);
             tmem_load(accumulator + kColumns / 2 + part * 64 + h * 32, v);
@@ -110,6 +106,14 @@ template <bool BF16, int kActivation, int kColumns> struct GateStoreVjp {
             tmem_pin(v);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
+                Pack<T, 8> g;
+                if (fetched) {
+                    *reinterpret_cast<uint4*>(&g) = RowsIn::chunk(staging, h * 4 + j, lane);
+                } else {
+                    const int c = h * 32 + j * 8, n = lane < here ? a.grad_columns - first - c : 0; // values that there are
+#pragma unroll
+                    for (int k = 0; k < 8; k++) g.v[k] = k < n ? from[c + k] : T(0.f);
+                }
                 uint32_t du[4], dv[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -118,7 +122,7 @@ template <bool BF16, int kActivation, int kColumns> struct GateStoreVjp {
                     for (int i = 0; i < 2; i++) {
                         const int at = j * 8 + k * 2 + i;
                         const FastGate<kActivation> gate(__uint_as_float(u[at]));
-                        const float d = widen(g[j].v[k * 2 + i]);
+                        const float d = widen(g.v[k * 2 + i]);
                         x[i] = d * __uint_as_float(v[at]) * gate.slope;
                         y[i] = d * gate.value;
                     }
@@ -129,6 +133,7 @@ template <bool BF16, int kActivation, int kColumns> struct GateStoreVjp {
                 grad_v[h * 4 + j] = make_uint4(dv[0], dv[1], dv[2], dv[3]);
             }
         }
+        __syncwarp();
         out_u.put(grad_u, staging, row, here, first, lane);
         out_v.put(grad_v, staging, row, here, first, lane);
     }

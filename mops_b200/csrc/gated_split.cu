@@ -21,12 +21,11 @@ template <int kActivation> struct GateStore32 {
     int here = 0, column = 0;
     __device__ GateStore32(const Args& a, uint32_t staging, int lane) : out{a.map, a.out, a.columns, a.columns, a.loose}, staging(staging), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) { row = r, here = h, column = piece.column + half * 32; }
-    __device__ __forceinline__ void store(const float (&sum)[64]) const {
+    __device__ __forceinline__ void store(float (&sum)[64]) const {
         if (column >= out.columns) return;
-        float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = Gate<kActivation, float>(sum[j]).value * sum[32 + j];
-        out.put(v, staging, row, here, column, lane);
+        for (int j = 0; j < 32; j++) sum[j] = Gate<kActivation, float>(sum[j]).value * sum[32 + j];
+        out.put(reinterpret_cast<const float(&)[32]>(sum[0]), staging, row, here, column, lane);
     }
     __device__ __forceinline__ void clear() const { out.clear(row, here, column, kSplitColumns / 2, lane); }
     __device__ __forceinline__ void end() const {
@@ -54,32 +53,33 @@ template <int kActivation> struct GateStoreVjp32 {
     int here = 0, column = 0;
     __device__ GateStoreVjp32(const Args& a, uint32_t staging, int lane)
         : a(a), out_u{a.map_u, a.out, a.stride, a.columns, a.loose}, out_v{a.map_v, a.out + a.columns, a.stride, a.columns, a.loose}, staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) { row = r, here = h, column = piece.column + half * 32; }
-    __device__ __forceinline__ void store(const float (&sum)[64]) const {
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
+        row = r, here = h, column = piece.column + half * 32;
+        if (lane < here && column < a.columns) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(a.grad + (row + lane) * a.grad_stride + column));
+    }
+    __device__ __forceinline__ void store(float (&sum)[64]) const { // (the sums become dU and dV where they are)
         if (column >= a.columns) return;
         const float* from = a.grad + (row + lane) * a.grad_stride + column;
-        float u[32], v[32];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int n = lane < here ? a.columns - column - 4 * j : 0; // values that there are
-            float4 g = make_float4(0, 0, 0, 0);
-            if (a.grad_aligned && n >= 4) g = *reinterpret_cast<const float4*>(from + 4 * j);
-            else {
-                if (n > 0) g.x = from[4 * j];
-                if (n > 1) g.y = from[4 * j + 1];
-                if (n > 2) g.z = from[4 * j + 2];
-                if (n > 3) g.w = from[4 * j + 3];
+            alignas(16) float d[4];
+            if (a.grad_aligned && n >= 4) {
+                *reinterpret_cast<float4*>(d) = *reinterpret_cast<const float4*>(from + 4 * j);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) d[k] = k < n ? from[4 * j + k] : 0.f;
             }
-            const float d[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const Gate<kActivation, float> gate(sum[4 * j + k]);
-                u[4 * j + k] = d[k] * sum[32 + 4 * j + k] * gate.slope;
-                v[4 * j + k] = d[k] * gate.value;
+                float &u = sum[4 * j + k], &v = sum[32 + 4 * j + k];
+                const Gate<kActivation, float> gate(u);
+                u = d[k] * v * gate.slope;
+                v = d[k] * gate.value;
             }
         }
-        out_u.put(u, staging, row, here, column, lane);
-        out_v.put(v, staging, row, here, column, lane);
+        out_u.put(reinterpret_cast<const float(&)[32]>(sum[0]), staging, row, here, column, lane);
+        out_v.put(reinterpret_cast<const float(&)[32]>(sum[32]), staging, row, here, column, lane);
     }
     __device__ __forceinline__ void clear() const {} // (nothing reads those of rows of no group)
     __device__ __forceinline__ void end() const {

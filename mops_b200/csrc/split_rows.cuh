@@ -60,13 +60,16 @@ split_rows(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
             float sum[W::kOwn];
             if (!work.template collect<E::kHalves>(sum, piece.steps, quadrant, half, lane)) break;
             if (here <= 0) continue;
-            if (W::any_nan(sum, lane < here))
+            if (W::any_nan(sum, lane < here)) {
+                RowsIn::wait();
                 work.mend(sum, warp - kSplitWarps, lane, [&](int c) {
                     const int column = piece.column + (E::kHalves ? half * 32 : half * W::kOwn + c);
                     return Terms{from.x + row * from.x_stride,
                                  from.m[E::kHalves && c > 0 ? 1 : 0] + piece.group * from.group_stride + column * from.column_stride,
                                  from.x_stride, 1, from.column_stride, from.depth_stride, depth, here, columns - column};
                 });
+                result.begin(piece, row, here, half); // (what it had in the staging memory has been written over)
+            }
             result.store(sum);
         }
         result.end();

@@ -7,7 +7,7 @@
 //
 // E has: kHalves, kStoreWarps (4 or 8), kStaging (bytes of shared memory of each of them), Args (among the kernel's arguments), and
 //   E(args, staging, lane)                            what a storing warp keeps
-//   begin(piece, row, here)                           before the accumulator is there: what can be loaded. The warp's first row, and how many it has
+//   begin(piece, row, here, part)                     before the accumulator is there: what can be loaded. The warp's first row, how many it has, and its part of the columns
 //   store(accumulator, part)                          the warp's part of the columns (0 of 1, or of 2)
 //   clear()                                           rows of no group
 //   end()                                             before the block leaves
@@ -130,6 +130,30 @@ struct BoxOut {
         for (int i = 0; i < here; i++)
             for (int c = lane; c < wide && column + c < columns; c += 32) out[(row + i) * stride + column + c] = 0;
     }
+};
+
+// Rows of 128 bytes that a warp has in its staging memory before its accumulator is there: a row for each lane, laid out as a box is.
+struct RowsIn {
+    // from: the first row's first byte, all on multiples of 16 bytes. `here` rows; the others are left as they are.
+    __device__ static __forceinline__ void fetch(uint32_t staging, const void* from, int64_t stride, int here, int lane) {
+        if (lane == 0) boxes_left<0>();
+        __syncwarp();
+        const int c = lane % 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = i * 4 + lane / 8;
+            if (r < here)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(staging + r * kBoxRow + ((c ^ (r & 7)) << 4)),
+                             "l"(static_cast<const unsigned char*>(from) + r * stride + c * 16)
+                             : "memory");
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
+    __device__ static __forceinline__ void wait() {
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        __syncwarp();
+    }
+    __device__ static __forceinline__ uint4 chunk(uint32_t staging, int c, int lane) { return smem_load16(staging + lane * kBoxRow + ((c ^ (lane & 7)) << 4)); }
 };
 
 // Rows of a single group, from the first on: as many as offsets[1] says, or all.
@@ -275,7 +299,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (Piece piece; supply.next(piece, lane);) {
             const int64_t row = piece.lo + rank * kTileRows + quadrant * 32;
             const int here = static_cast<int>(min(max(piece.hi - row, int64_t(0)), int64_t(32)));
-            work.begin(piece, row, here);
+            work.begin(piece, row, here, part);
             if (piece.group < 0) {
                 if (part == 0) work.clear();
                 continue;
