@@ -28,61 +28,73 @@ template <typename S>
 __global__ void __launch_bounds__(kPrepareThreads)
 loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, const int32_t* __restrict__ targets, int64_t rows, int64_t vocabulary,
              int64_t ignored, const S* __restrict__ grad_loss, const S* __restrict__ grad_log_sum, Status st) {
-    __shared__ int of_warp[32];
+    constexpr int kRuns = kPrepareRows * kPrepareThreads / 32; // of 32 rows each
+    __shared__ int in_run[kRuns], in_front[kRuns + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool gradients = grad_loss != nullptr || grad_log_sum != nullptr;
     int before = 0;
     float largest[3] = {}; // of the gradients of losses, of sums, of both together
     bool bad = false;
     for (int64_t r0 = 0; r0 < rows; r0 += kPrepareThreads * kPrepareRows) {
-        const int64_t r = r0 + static_cast<int64_t>(threadIdx.x) * kPrepareRows;
-        unsigned keep = 0;
+        int32_t target[kPrepareRows];
+        unsigned kept[kPrepareRows];
 #pragma unroll
-        for (int k = 0; k < kPrepareRows; k++)
-            if (r + k < rows) {
-                const int64_t t = targets[r + k];
-                const bool in = t >= 0 && t < vocabulary && t != ignored;
-                keep |= static_cast<unsigned>(in) << k;
-                bad |= !in && t != ignored;
-            }
-        const int own = __popc(keep);
-        int up_to = own;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(kFullMask, up_to, d);
-            if (lane >= d) up_to += v;
+        for (int k = 0; k < kPrepareRows; k++) {
+            const int64_t r = r0 + k * kPrepareThreads + threadIdx.x;
+            target[k] = r < rows ? targets[r] : 0;
         }
-        if (lane == 31) of_warp[warp] = up_to;
+#pragma unroll
+        for (int k = 0; k < kPrepareRows; k++) {
+            const int64_t r = r0 + k * kPrepareThreads + threadIdx.x, t = target[k];
+            const bool in = r < rows && t >= 0 && t < vocabulary && t != ignored;
+            bad |= r < rows && !in && t != ignored;
+            kept[k] = __ballot_sync(kFullMask, in);
+            if (lane == 0) in_run[k * (kPrepareThreads / 32) + warp] = __popc(kept[k]);
+        }
         __syncthreads();
-        int all = of_warp[lane];
+        if (warp == 0) { // the runs in front of each
+            constexpr int kEach = kRuns / 32;
+            int sum = 0, own[kEach];
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(kFullMask, all, d);
-            if (lane >= d) all += v;
+            for (int i = 0; i < kEach; i++) own[i] = in_run[lane * kEach + i], sum += own[i];
+            int up_to = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(kFullMask, up_to, d);
+                if (lane >= d) up_to += v;
+            }
+            int at = up_to - sum;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) in_front[lane * kEach + i] = at, at += own[i];
+            if (lane == 31) in_front[kRuns] = at;
         }
-        const int in_front = __shfl_sync(kFullMask, all, (warp + 31) & 31), total = __shfl_sync(kFullMask, all, 31);
-        int i = before + up_to - own + (warp > 0 ? in_front : 0);
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kPrepareRows; k++)
-            if (r + k < rows) {
-                const bool in = keep >> k & 1;
-                to.place[r + k] = in ? i : -1;
-                if (in) {
-                    to.order[i] = static_cast<int32_t>(r + k);
-                    to.target[i++] = targets[r + k];
-                    const float l = grad_loss != nullptr ? static_cast<float>(fabs(grad_loss[r + k])) : 0.f;
-                    const float m = grad_log_sum != nullptr ? static_cast<float>(fabs(grad_log_sum[r + k])) : 0.f;
+        for (int k = 0; k < kPrepareRows; k++) {
+            const int64_t r = r0 + k * kPrepareThreads + threadIdx.x;
+            if (r >= rows) continue;
+            const bool in = kept[k] >> lane & 1;
+            const int i = before + in_front[k * (kPrepareThreads / 32) + warp] + __popc(kept[k] & ((1u << lane) - 1));
+            to.place[r] = in ? i : -1;
+            if (in) {
+                to.order[i] = static_cast<int32_t>(r);
+                to.target[i] = target[k];
+                if (gradients) {
+                    const float l = grad_loss != nullptr ? static_cast<float>(fabs(grad_loss[r])) : 0.f;
+                    const float m = grad_log_sum != nullptr ? static_cast<float>(fabs(grad_log_sum[r])) : 0.f;
                     const float all[3] = {l, m, l + m};
 #pragma unroll
                     for (int q = 0; q < 3; q++)
                         if (all[q] <= 3e38f) largest[q] = fmaxf(largest[q], all[q]); // (infinities keep to their rows)
-                } else if (loss != nullptr) {
-                    loss[r + k] = log_sum[r + k] = S(0);
                 }
+            } else if (loss != nullptr) {
+                loss[r] = log_sum[r] = S(0);
             }
-        before += total;
+        }
+        before += in_front[kRuns];
         __syncthreads();
     }
-    if (grad_loss != nullptr || grad_log_sum != nullptr) {
+    if (gradients) {
         __shared__ float most[3][kPrepareThreads / 32];
 #pragma unroll
         for (int q = 0; q < 3; q++) {
@@ -409,9 +421,7 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
         loss_sums<S><<<grid, 256, 0, call.stream>>>(sums, parts, v0 / pieces.part, at_target, logits, v1 - v0, static_cast<S>(scale), t, v0, pieces.part,
                                                      pieces.rows);
     });
-    loss_join<S><<<static_cast<unsigned>(n), 128, 0, call.stream>>>(static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), sums, parts, at_target, pieces.rows, t, W.shape[0], ignored,
-                                                            call.status);
-    MOPS_CUDA_OK(cudaGetLastError());
+    join_rows<S>(call, loss, log_sum, sums, parts, at_target, pieces.rows, targets, W.shape[0], ignored);
     note_kernel_f("loss_sums<%s>", scalar_name<S>());
 }
 

@@ -229,21 +229,22 @@ struct FactorArgs {
     float scale, units; // units: that are 1, 2^14 for f16
 };
 __global__ void __launch_bounds__(kGatherThreads)
-gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const uint16_t* __restrict__ from, int64_t stride, bool aligned, const LossRows rows, int64_t columns,
-            const FactorArgs f) {
+gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const __half* __restrict__ from, int64_t stride, bool aligned, const unsigned char* begin,
+            const unsigned char* end, const LossRows rows, int64_t columns, const FactorArgs f) {
     const int64_t kept = rows.offsets[1];
     const int lane = threadIdx.x & 31;
     const float unit = f.factors != nullptr ? *rows.unit : 0.f;
     if (f.factors != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *f.factor = unit * f.scale / f.units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kGatherThreads / 32) + threadIdx.x / 32; i < kept; i += static_cast<int64_t>(gridDim.x) * (kGatherThreads / 32)) {
         const int64_t r = rows.order[i];
+        const __half* p = from + r * stride;
+        uint4* q = reinterpret_cast<uint4*>(to + i * to_stride);
         if (aligned) {
-            const uint4* p = reinterpret_cast<const uint4*>(from + r * stride);
-            uint4* q = reinterpret_cast<uint4*>(to + i * to_stride);
 #pragma unroll 4
-            for (int64_t c = lane; c < columns / 8; c += 32) q[c] = __ldg(p + c);
+            for (int64_t c = lane; c < columns / 8; c += 32) q[c] = __ldg(reinterpret_cast<const uint4*>(p) + c);
         } else {
-            for (int64_t c = lane; c < columns; c += 32) to[i * to_stride + c] = from[r * stride + c];
+#pragma unroll 2
+            for (int64_t c = lane; c < to_stride / 8; c += 32) q[c] = load_anywhere<__half>(p + c * 8, columns - c * 8, begin, end);
         }
         if (f.factors != nullptr && lane == 0) {
             const float of_loss = f.grad_loss != nullptr ? f.grad_loss[r] : 0.f, of_sum = f.grad_log_sum != nullptr ? f.grad_log_sum[r] : 0.f;
@@ -254,36 +255,38 @@ gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const uint16_t* __rest
     }
 }
 
-// grad_A[r,:] = factor times the sums of row place[r], zeros for rows that have no place.
+// grad_A[r,:] = factor times the sums of row place[r], zeros for rows that have no place. Four columns to a thread; the sums have room up to a multiple of 4.
 template <typename T>
 __global__ void __launch_bounds__(kGatherThreads)
-scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int64_t slices, int64_t stride, const LossRows rows, int64_t n, int64_t columns, bool by_four,
+scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int slices, int64_t stride, const LossRows rows, int64_t n, int columns, bool by_four,
              const float* __restrict__ factor) {
-    const int lane = threadIdx.x & 31;
     const float f = *factor;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kGatherThreads / 32) + threadIdx.x / 32; r < n; r += static_cast<int64_t>(gridDim.x) * (kGatherThreads / 32)) {
+    const int quads = static_cast<int>(stride / 4), per = (quads + gridDim.y - 1) / gridDim.y;
+    const int begin = blockIdx.y * per, end = min(begin + per, quads);
+    const int64_t slice = n * stride;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; r < n; r += static_cast<int64_t>(gridDim.x) * blockDim.y) {
         const int64_t i = rows.place[r];
-        const float* from = sums + i * stride;
-        T* p = to + r * columns;
-        if (by_four) {
-            for (int64_t c = lane * 4; c < columns; c += 128) {
-                float4 v = make_float4(0, 0, 0, 0);
-                if (i >= 0)
-                    for (int64_t s = 0; s < slices; s++) {
-                        const float4 w = *reinterpret_cast<const float4*>(from + s * n * stride + c);
-                        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                    }
-                Pack<T, 4> out;
+#pragma unroll 2
+        for (int q = begin + threadIdx.x; q < end; q += blockDim.x) {
+            Pack<T, 4> out;
+            if (i >= 0) {
+                const float* from = sums + i * stride + 4 * q;
+                float4 v = *reinterpret_cast<const float4*>(from);
+                for (int s = 1; s < slices; s++) {
+                    const float4 w = *reinterpret_cast<const float4*>(from + s * slice);
+                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                }
                 out.v[0] = narrow<T>(v.x * f), out.v[1] = narrow<T>(v.y * f), out.v[2] = narrow<T>(v.z * f), out.v[3] = narrow<T>(v.w * f);
-                if (i < 0) out.v[0] = out.v[1] = out.v[2] = out.v[3] = T(0.f);
-                *reinterpret_cast<Pack<T, 4>*>(p + c) = out;
+            } else {
+                out.v[0] = out.v[1] = out.v[2] = out.v[3] = T(0.f);
             }
-        } else {
-            for (int64_t c = lane; c < columns; c += 32) {
-                float v = 0;
-                if (i >= 0)
-                    for (int64_t s = 0; s < slices; s++) v += from[s * n * stride + c];
-                p[c] = i >= 0 ? narrow<T>(v * f) : T(0.f);
+            T* p = to + r * columns + 4 * q;
+            if (by_four) {
+                *reinterpret_cast<Pack<T, 4>*>(p) = out;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (4 * q + k < columns) p[k] = out.v[k];
             }
         }
     }
@@ -302,8 +305,10 @@ Array gathered(const Call& call, Scratch& room, const Array& A, const LossRows& 
     Array to = contiguous(room.as<void>(), A.type, A.shape[0], A.shape[1]);
     to.stride[0] = stride;
     const bool aligned = A.shape[1] % 8 == 0 && A.stride[0] % 8 == 0 && reinterpret_cast<uintptr_t>(A.data) % 16 == 0;
-    gather_rows<<<warps_for(call, A.shape[0]), kGatherThreads, 0, call.stream>>>(static_cast<uint16_t*>(to.data), stride, static_cast<const uint16_t*>(A.data),
-                                                                                  A.stride[0], aligned, rows, A.shape[1], factors);
+    const unsigned char* begin = static_cast<const unsigned char*>(A.data);
+    gather_rows<<<warps_for(call, A.shape[0]), kGatherThreads, 0, call.stream>>>(static_cast<uint16_t*>(to.data), stride, static_cast<const __half*>(A.data), A.stride[0],
+                                                                                  aligned, begin, begin + ((A.shape[0] - 1) * A.stride[0] + A.shape[1]) * 2, rows,
+                                                                                  A.shape[1], factors);
     MOPS_CUDA_OK(cudaGetLastError());
     return to;
 }
@@ -313,8 +318,8 @@ template <typename F> void for_sixteen(int32_t type, F&& f) {
     else f(std::false_type());
 }
 
-// Whether rows are numbered and gathered in front of a forward pass: of few rows those without a target cost less than the two kernels that does.
-constexpr int64_t kGatherFrom = 2048;
+// Whether rows are numbered and gathered in front of a forward pass, which takes some 10 us: where all of them take 50 us or more on the tensor cores.
+bool worth_gathering(int64_t rows, int64_t vocabulary, int64_t columns) { return rows >= 512 && 2.0 * rows * vocabulary * columns >= 5e10; }
 
 } // namespace
 
@@ -326,7 +331,7 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
     Array A = p.A, W = p.W;
     LossRows rows{};
     const int32_t* targets = static_cast<const int32_t*>(p.targets.data);
-    const bool gather = n >= kGatherFrom;
+    const bool gather = worth_gathering(n, vocabulary, p.A.shape[1]);
     if (gather) {
         rows = take_rows(room_rows, n);
         prepare_rows<float>(call, rows, static_cast<float*>(loss.data), static_cast<float*>(log_sum.data), p.targets, vocabulary, p.ignored, nullptr, nullptr);
@@ -355,9 +360,7 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
         else launch(integral_constant<int, 256>(), std::true_type());
     });
     MOPS_CUDA_OK(cudaGetLastError());
-    loss_join<float><<<static_cast<unsigned>(n), 128, 0, call.stream>>>(static_cast<float*>(loss.data), static_cast<float*>(log_sum.data), sums, parts, at_target, rows,
-                                                                         targets, vocabulary, p.ignored, call.status);
-    MOPS_CUDA_OK(cudaGetLastError());
+    join_rows<float>(call, loss, log_sum, sums, parts, at_target, rows, p.targets, vocabulary, p.ignored);
 }
 
 void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad_A, const Array& grad_W, const Array& grad_loss, const Array& grad_log_sum, const Array& loss,
@@ -386,12 +389,17 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     const int64_t most = std::max<int64_t>(kMostValues / n / 256 * 256, 256), pieces = ceil_div(vocabulary, most);
     const int64_t width = std::min(ceil_div(ceil_div(vocabulary, pieces), 256) * 256, whole_packs(vocabulary));
     Scratch room_dx(call, static_cast<size_t>(n * width) * 2);
-    // slices of the piece: as many as there have to be for tiles for all
-    const bool wide = ceil_div(n, 2 * kTileRows) * ceil_div(columns, 256) * 2 >= sms;
-    const int64_t tiles = wide ? 1 : ceil_div(n, kTileRows) * ceil_div(columns, 128);
+    // Slices of the piece for the products with W: so many that the last round of pairs is nearly full, each of 1024 values of depth at least. What a slice more costs, sums that are written and read,
+    // counts as 2 % of a round.
     const int64_t steps = ceil_div(std::min(width, vocabulary), kBoxDepth);
-    const int64_t wanted = wide ? 1 : std::max<int64_t>(std::min(ceil_div(3 * int64_t(sms), 2 * tiles), width / 1024), 1);
-    const int64_t slices = ceil_div(steps, ceil_div(steps, wanted)); // (none without steps: the first piece writes the sums of all)
+    const int64_t tiles = ceil_div(n, 2 * kTileRows) * ceil_div(columns, 256), workers = sms / 2;
+    int64_t slices = 1;
+    double least = 1e30;
+    for (int64_t s = 1; s <= 16 && (s == 1 || steps / s >= 16); s++) {
+        const double rounds = static_cast<double>(ceil_div(tiles * s, workers)) / s + 0.02 * s;
+        if (rounds < least) least = rounds, slices = s;
+    }
+    slices = ceil_div(steps, ceil_div(steps, slices)); // (none without steps: the first piece writes the sums of all)
     const int64_t stride = (columns + 3) / 4 * 4;
     Scratch room_sums(call);
     if (need_A) room_sums.take(static_cast<size_t>(slices * n * stride) * sizeof(float));
@@ -414,15 +422,11 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
             if (need_A) {
                 const TileProblem sum_problem{dx, rows.offsets, 1, n, here, columns, slices};
                 const TileOperand by_rows[2] = {{w, W.stride[0], 1, 0}, {w, W.stride[0], 1, 0}};
-                auto launch = [&](auto tile, auto paired) {
-                    using Sums = SumStore<decltype(tile)::value>;
-                    typename Sums::Args to{};
-                    to.map = tensor_map(MOPS_B200_F32, sums, columns, n, slices, stride, n * stride, 32);
-                    to.out = sums, to.rows = n, to.stride = stride, to.columns = static_cast<int>(columns), to.add = v0 > 0;
-                    launch_tiles<BF16, true, decltype(tile)::value, decltype(paired)::value, Sums, DecodeSlices>(call, op, sum_problem, by_rows, to);
-                };
-                if (wide) launch(integral_constant<int, 256>(), std::true_type());
-                else launch(integral_constant<int, 128>(), std::false_type());
+                using Sums = SumStore<256>;
+                typename Sums::Args to{};
+                to.map = tensor_map(MOPS_B200_F32, sums, columns, n, slices, stride, n * stride, 32);
+                to.out = sums, to.rows = n, to.stride = stride, to.columns = static_cast<int>(columns), to.add = v0 > 0;
+                launch_tiles<BF16, true, 256, true, Sums, DecodeSlices>(call, op, sum_problem, by_rows, to);
             }
         });
         MOPS_CUDA_OK(cudaGetLastError());
@@ -433,7 +437,12 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
         for_sixteen(A.type, [&](auto type) {
             using T = std::conditional_t<decltype(type)::value, __nv_bfloat16, __half>;
             const bool by_four = columns % 4 == 0 && reinterpret_cast<uintptr_t>(grad_A.data) % 8 == 0;
-            scatter_rows<T><<<warps_for(call, n), kGatherThreads, 0, call.stream>>>(static_cast<T*>(grad_A.data), sums, slices, stride, rows, n, columns, by_four, factor);
+            unsigned across = 32;
+            while (across < kGatherThreads && across * 4 < columns) across *= 2;
+            const dim3 block(across, kGatherThreads / across);
+            const unsigned down = static_cast<unsigned>(std::min<int64_t>(ceil_div(n, block.y), int64_t(sms) * 32));
+            scatter_rows<T><<<down, block, 0, call.stream>>>(static_cast<T*>(grad_A.data), sums, static_cast<int>(slices), stride, rows, n, static_cast<int>(columns), by_four,
+                                                             factor);
         });
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("loss_gradient_mma<%s>, %d pieces, %d slices", A.type == MOPS_B200_BF16 ? "bf16" : "f16", static_cast<int>(pieces), static_cast<int>(slices));

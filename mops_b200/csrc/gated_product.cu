@@ -102,6 +102,29 @@ struct Widened {
 };
 
 // ---- f16 and bf16 on tensor cores
+// The halves of matrices (of `from_columns` columns each) where those of others (of `to_columns`) are, both by columns or both by depth; zeros where there are none. A row of `to` to kRowThreads threads.
+template <bool kByColumns>
+__global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
+copy_halves(uint16_t* __restrict__ to, int64_t to_group_stride, int64_t to_stride, int to_columns, const uint16_t* __restrict__ from, int64_t from_group_stride, int64_t from_stride,
+            int from_columns, int64_t groups, int to_depth, int from_depth) {
+    const int64_t outer = kByColumns ? to_depth : 2 * to_columns;
+    for (int64_t row = first_row(); row < groups * outer; row += row_step()) {
+        const int64_t g = row / outer;
+        const int o = static_cast<int>(row - g * outer);
+        uint16_t* q = to + g * to_group_stride + o * to_stride;
+        const uint16_t* p = from + g * from_group_stride;
+        if constexpr (kByColumns) { // depth o, both halves of its row
+            for (int c = threadIdx.x; c < 2 * to_columns; c += kRowThreads) {
+                const int half = c >= to_columns, j = half ? c - to_columns : c;
+                q[c] = j < from_columns && o < from_depth ? p[o * from_stride + half * from_columns + j] : 0;
+            }
+        } else {
+            const int half = o >= to_columns, j = half ? o - to_columns : o;
+            for (int d = threadIdx.x; d < to_depth; d += kRowThreads)
+                q[d] = j < from_columns && d < from_depth ? p[(half * from_columns + j) * from_stride + d] : 0;
+        }
+    }
+}
 // A and W as the copy engine can fetch them, or copies: rows of A whole packs apart, and of W both halves, with zeros behind the columns of either up to a multiple of 8. `padded`: gradients
 // are to be taken, too, whose products go along both halves at once.
 struct Boxed {
@@ -118,26 +141,24 @@ struct Boxed {
             const int64_t groups = p.groups, depth = p.depth, wide = (columns + 7) / 8 * 8, deep = (depth + 7) / 8 * 8;
             p.columns = wide;
             p.W = p.by_columns() ? contiguous(nullptr, A.type, groups, depth, 2 * wide) : contiguous(nullptr, A.type, groups, 2 * wide, deep);
-            const size_t bytes = static_cast<size_t>(values_of(p.W)) * 2;
-            room.take(bytes);
+            room.take(static_cast<size_t>(values_of(p.W)) * 2);
             p.W.data = room.as<void>();
-            if (W.stride[2] != 1) std::swap(p.W.shape[1], p.W.shape[2]), std::swap(p.W.stride[1], p.W.stride[2]), p.W.shape[1] = depth;
-            MOPS_CUDA_OK(cudaMemsetAsync(p.W.data, 0, bytes, call.stream));
-            copy_halves(p.W, wide, W, columns);
+            if (W.stride[2] != 1) std::swap(p.W.shape[1], p.W.shape[2]), std::swap(p.W.stride[1], p.W.stride[2]);
+            move_halves(p.W, wide, W, columns);
+            p.W.shape[1] = depth;
         } else {
             packing.add(p.W);
         }
         packing.run();
     }
-    // The halves of `from` (of `n` columns each) go where those of `to` (of `m`, n or more there or here) are; both are stored the same way round.
-    void copy_halves(const Array& to, int64_t m, const Array& from, int64_t n) {
+    // The halves of `from` (of `n` columns each) go where those of `to` (of `m`) are; both are stored the same way round.
+    void move_halves(const Array& to, int64_t m, const Array& from, int64_t n) {
         const bool by_columns = from.stride[2] == 1;
-        const int64_t columns = std::min(m, n), outer = by_columns ? from.shape[1] : columns, inner = by_columns ? columns : from.shape[1];
-        for (int half = 0; half < 2; half++) // (their values are only moved)
-            convert_rows<uint16_t, uint16_t><<<row_blocks(call, from.shape[0] * outer), row_threads(), 0, call.stream>>>(
-                static_cast<uint16_t*>(to.data) + half * m * to.stride[2], to.stride[0], by_columns ? to.stride[1] : to.stride[2],
-                static_cast<const uint16_t*>(from.data) + half * n * from.stride[2], from.shape[0], outer, inner, from.stride[0],
-                by_columns ? from.stride[1] : from.stride[2]);
+        const int64_t rows = to.shape[0] * (by_columns ? to.shape[1] : 2 * m);
+        auto kernel = by_columns ? copy_halves<true> : copy_halves<false>;
+        kernel<<<row_blocks(call, rows), row_threads(), 0, call.stream>>>(
+            static_cast<uint16_t*>(to.data), to.stride[0], by_columns ? to.stride[1] : to.stride[2], static_cast<int>(m), static_cast<const uint16_t*>(from.data),
+            from.stride[0], by_columns ? from.stride[1] : from.stride[2], static_cast<int>(n), to.shape[0], static_cast<int>(to.shape[1]), static_cast<int>(from.shape[1]));
         MOPS_CUDA_OK(cudaGetLastError());
     }
 };
@@ -173,7 +194,7 @@ void gradients_16(const Call& call, const Array& grad_A, const Array& grad_W, bo
         Array result = grad_W;
         if (turned)
             for (Array* a : {&to, &result}) std::swap(a->shape[1], a->shape[2]), std::swap(a->stride[1], a->stride[2]);
-        boxed.copy_halves(result, boxed.real_columns, to, p.columns);
+        boxed.move_halves(result, boxed.real_columns, to, p.columns);
     }
 }
 

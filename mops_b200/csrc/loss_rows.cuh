@@ -32,14 +32,16 @@ template <typename S> struct alignas(2 * sizeof(S)) PartSum {
     }
 };
 
-// The i-th row's loss and log_sum from the sums of its parts, in their order, and x at the target. A block to a row. Where rows have not been numbered (no order) they
-// are all there, and those without a target get their zeros here.
+// The i-th row's loss and log_sum from the sums of its parts, and x at the target. A warp to a row: its lanes find the largest first, and take one exponential for each part. Where rows have not
+// been numbered (no order) they are all there, and those without a target get their zeros here.
+constexpr int kJoinThreads = 128;
 template <typename S>
-static __global__ void __launch_bounds__(128)
-loss_join(S* __restrict__ loss, S* __restrict__ log_sum, const PartSum<S>* __restrict__ parts, int64_t n, const S* __restrict__ at_target,
+static __global__ void __launch_bounds__(kJoinThreads)
+loss_join(S* __restrict__ loss, S* __restrict__ log_sum, const PartSum<S>* __restrict__ parts, int64_t n, int64_t all_rows, const S* __restrict__ at_target,
           const LossRows rows, const int32_t* __restrict__ targets, int64_t vocabulary, int64_t ignored, Status st) {
-    __shared__ PartSum<S> of_warp[4];
-    const int64_t i = blockIdx.x;
+    const int lane = threadIdx.x & 31;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + threadIdx.x / 32;
+    if (i >= all_rows) return;
     int64_t r = i;
     if (rows.order != nullptr) {
         if (i >= rows.offsets[1]) return;
@@ -47,29 +49,48 @@ loss_join(S* __restrict__ loss, S* __restrict__ log_sum, const PartSum<S>* __res
     } else {
         const int64_t t = targets[i];
         if (t < 0 || t >= vocabulary || t == ignored) {
-            if (threadIdx.x == 0) {
+            if (lane == 0) {
                 loss[i] = log_sum[i] = S(0);
                 if (t != ignored) report_bad_index(st, 0);
             }
             return;
         }
     }
-    PartSum<S> all = PartSum<S>::none();
-    for (int64_t p = threadIdx.x; p < n; p += 128) all.join(parts[i * n + p]);
+    constexpr int kInFlight = 8;
+    const PartSum<S>* of_row = parts + i * n;
+    S top = -S(INFINITY);
+    for (int64_t p0 = lane; p0 < n; p0 += 32 * kInFlight) {
+        S v[kInFlight];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        PartSum<S> other;
-        other.top = __shfl_down_sync(kFullMask, all.top, d);
-        other.sum = __shfl_down_sync(kFullMask, all.sum, d);
-        all.join(other);
+        for (int k = 0; k < kInFlight; k++) v[k] = p0 + 32 * k < n ? of_row[p0 + 32 * k].top : -S(INFINITY);
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) top = fmax(top, v[k]);
     }
-    if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = all;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int w = 1; w < 4; w++) all.join(of_warp[w]);
-    const S value = PartSum<S>::from(all.top) + log(all.sum);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(kFullMask, top, d));
+    const S base = PartSum<S>::from(top);
+    S sum = 0;
+    for (int64_t p0 = lane; p0 < n; p0 += 32 * kInFlight) { // (from the L1, or near it)
+        PartSum<S> v[kInFlight];
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) v[k] = p0 + 32 * k < n ? of_row[p0 + 32 * k] : PartSum<S>::none();
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) sum += v[k].sum * v[k].weight(base);
+    }
+    sum = warp_sum(sum);
+    if (lane != 0) return;
+    const S value = base + log(sum);
     log_sum[r] = value;
     loss[r] = value - at_target[i];
+}
+template <typename S>
+void join_rows(const Call& call, const Array& loss, const Array& log_sum, const PartSum<S>* parts, int64_t n, const S* at_target, const LossRows& rows, const Array& targets,
+               int64_t vocabulary, int64_t ignored) {
+    const int64_t all = targets.shape[0];
+    loss_join<S><<<static_cast<unsigned>(ceil_div(all, kJoinThreads / 32)), kJoinThreads, 0, call.stream>>>(
+        static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), parts, n, all, at_target, rows, static_cast<const int32_t*>(targets.data), vocabulary, ignored,
+        call.status);
+    MOPS_CUDA_OK(cudaGetLastError());
 }
 
 inline LossRows take_rows(Scratch& room, int64_t rows) {
