@@ -7,8 +7,7 @@
 //
 // A piece of the vocabulary at a time: its logits are a product into scratch memory, of which sums are taken, or which become dx where they stand and are multiplied by the
 // piece's rows of W and, the other way, by A. The gradients compute the logits again. In f32 the logits of more than a few rows are worked on where they are summed (LossStore32, GradientStore32)
-// and never stored. Here: f32 and f64, and f16 and bf16, widened to f32, where there are few rows to differentiate; the rest of
-// them is in cross_entropy_mma.cu.
+// and never stored. Here: f32 and f64 (and f16 and bf16 without columns); f16 and bf16 are in cross_entropy_mma.cu.
 #include "block_ops.hpp"
 #include "convert.cuh"
 #include "grouped_mma.hpp"
@@ -110,7 +109,7 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
             *to.unit = largest[1] <= 2 * largest[0] ? largest[0] : largest[2];
         }
     }
-    if (threadIdx.x == 0) to.offsets[0] = 0, to.offsets[1] = before;
+    if (threadIdx.x == 0) to.offsets[0] = 0, to.offsets[1] = before, to.doubled[0] = 0, to.doubled[1] = 2 * before;
     if (bad) report_bad_index(st, 0);
 }
 
@@ -504,9 +503,6 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
 
 bool sixteen_bits(const Array& A) { return (A.type == MOPS_B200_F16 || A.type == MOPS_B200_BF16) && A.shape[1] > 0; }
 
-// Up to so many rows gradients are computed in f32 throughout: a row's gradient is for the most part that of its target, whose rounding to 16 bits would be an error of the row as a whole.
-constexpr int64_t kFewGradients = 256;
-
 } // namespace
 
 void linear_cross_entropy(Array loss, Array log_sum, Array A, Array W, Array targets, double scale, int64_t ignore_index) {
@@ -545,7 +541,7 @@ void linear_cross_entropy_vjp(Array grad_A, Array grad_W, Array grad_loss, Array
     if (A.shape[0] == 0) {
         if (grad_W.data != nullptr)
             MOPS_CUDA_OK(cudaMemsetAsync(grad_W.data, 0, static_cast<size_t>(values_of(grad_W) * type_bytes(grad_W.type)), call.stream));
-    } else if (sixteen_bits(A) && A.shape[0] > kFewGradients) {
+    } else if (sixteen_bits(A)) {
         loss_backward_mma(call, {A, W, targets, scale, ignore_index}, grad_A, grad_W, grad_loss, grad_log_sum, loss, log_sum, op);
     } else if (A.type == MOPS_B200_F64) {
         loss_backward<double>(call, grad_A, grad_W, grad_loss, grad_log_sum, log_sum, A, W, targets, scale, ignore_index, op);

@@ -6,6 +6,8 @@
 //
 // dx is rounded to 16 bits in units of the largest gradient of a loss (f16: of 2^-14 of it, so that probabilities down to 2^-28 are normal numbers), which
 // multiplies the results: so the gradient of a mean, which is the same for all rows, leaves -1 at the targets as it is. A row's value there is 1 - exp(-loss), not the difference of rounded numbers.
+// A row's gradient is for the most part that of its target, whose rounding is an error of the row as a whole; where there are too few rows for such errors to average out, dx is kept in two parts of
+// 16 bits (a row of what the first leaves under it, and rows of A twice): the products are bounded by memory there.
 #include "block_ops.hpp"
 #include "grouped_mma.hpp"
 #include "loss_rows.cuh"
@@ -94,25 +96,26 @@ struct alignas(16) RowFactors {
     int32_t target;
 };
 
-template <bool BF16, int kColumns> struct GradientStore {
+template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
     static constexpr bool kHalves = false;
     static constexpr int kStoreWarps = 8, kStaging = BoxOut::kBytes, kOwn = kColumns / 2;
     struct Args {
-        CUtensorMap map;
-        uint16_t* out;
+        CUtensorMap map, map_rest;
+        uint16_t *out, *rest;
         int64_t stride;
         int columns, first_column; // of the piece
         float scale2;
         const RowFactors* factors;
     };
     const Args& a;
-    BoxOut out;
+    BoxOut out, rest;
     uint32_t staging;
     int lane;
     int64_t row = 0;
     int here = 0, column = 0;
     RowFactors f{};
-    __device__ GradientStore(const Args& a, uint32_t staging, int lane) : a(a), out{a.map, a.out, a.stride, a.columns, false}, staging(staging), lane(lane) {}
+    __device__ GradientStore(const Args& a, uint32_t staging, int lane)
+        : a(a), out{a.map, a.out, a.stride, a.columns, false}, rest{a.map_rest, a.rest, a.stride, a.columns, false}, staging(staging), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) {
         row = r, here = h, column = piece.column;
         if (lane < here) {
@@ -124,7 +127,7 @@ template <bool BF16, int kColumns> struct GradientStore {
 #pragma unroll 1
         for (int c = part * kOwn; c < part * kOwn + kOwn; c += 64) {
             if (column + c >= a.columns) return;
-            uint4 v[8];
+            uint4 v[8], w[8];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t r[32];
@@ -140,12 +143,22 @@ template <bool BF16, int kColumns> struct GradientStore {
                     for (int j = 0; j < 32; j++)
                         if (j == at) x[j] = f.at_target;
                 }
+                auto packs = [&](uint4* to) {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    v[h * 4 + j] = make_uint4(pack_pair<BF16>(x[8 * j], x[8 * j + 1]), pack_pair<BF16>(x[8 * j + 2], x[8 * j + 3]),
-                                              pack_pair<BF16>(x[8 * j + 4], x[8 * j + 5]), pack_pair<BF16>(x[8 * j + 6], x[8 * j + 7]));
+                    for (int j = 0; j < 4; j++)
+                        to[h * 4 + j] = make_uint4(pack_pair<BF16>(x[8 * j], x[8 * j + 1]), pack_pair<BF16>(x[8 * j + 2], x[8 * j + 3]),
+                                                   pack_pair<BF16>(x[8 * j + 4], x[8 * j + 5]), pack_pair<BF16>(x[8 * j + 6], x[8 * j + 7]));
+                };
+                packs(v);
+                if constexpr (kTwoParts) {
+                    using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) x[j] -= widen(narrow<T>(x[j]));
+                    packs(w);
+                }
             }
             out.put(v, staging, row, here, column + c, lane);
+            if constexpr (kTwoParts) rest.put(w, staging, row, here, column + c, lane);
         }
     }
     __device__ __forceinline__ void clear() const {}
@@ -221,7 +234,7 @@ template <int kColumns> struct SumStore {
     }
 };
 
-// to[i,:] = from[order[i],:], a warp to a row; and what dx takes of the row, if that is asked for.
+// to[i,:] = from[order[i],:], or rows 2i and 2i + 1, a warp to a row; and what dx takes of the row, if that is asked for.
 struct FactorArgs {
     RowFactors* factors; // none: a forward pass
     float* factor;       // of the results
@@ -230,7 +243,8 @@ struct FactorArgs {
 };
 __global__ void __launch_bounds__(kGatherThreads)
 gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const __half* __restrict__ from, int64_t stride, bool aligned, const unsigned char* begin,
-            const unsigned char* end, const LossRows rows, int64_t columns, const FactorArgs f) {
+            const unsigned char* end, const LossRows rows, int64_t columns, bool twice,
+            const FactorArgs f) {
     const int64_t kept = rows.offsets[1];
     const int lane = threadIdx.x & 31;
     const float unit = f.factors != nullptr ? *rows.unit : 0.f;
@@ -238,13 +252,16 @@ gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const __half* __restri
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kGatherThreads / 32) + threadIdx.x / 32; i < kept; i += static_cast<int64_t>(gridDim.x) * (kGatherThreads / 32)) {
         const int64_t r = rows.order[i];
         const __half* p = from + r * stride;
-        uint4* q = reinterpret_cast<uint4*>(to + i * to_stride);
-        if (aligned) {
+        const int64_t packs = to_stride / 8;
+        uint4* q = reinterpret_cast<uint4*>(to) + (twice ? 2 * i : i) * packs;
+        if (twice) {
+            for (int64_t c = lane; c < packs; c += 32) q[c] = q[c + packs] = load_anywhere<__half>(p + c * 8, columns - c * 8, begin, end);
+        } else if (aligned) {
 #pragma unroll 4
-            for (int64_t c = lane; c < columns / 8; c += 32) q[c] = __ldg(reinterpret_cast<const uint4*>(p) + c);
+            for (int64_t c = lane; c < packs; c += 32) q[c] = __ldg(reinterpret_cast<const uint4*>(p) + c);
         } else {
 #pragma unroll 2
-            for (int64_t c = lane; c < to_stride / 8; c += 32) q[c] = load_anywhere<__half>(p + c * 8, columns - c * 8, begin, end);
+            for (int64_t c = lane; c < packs; c += 32) q[c] = load_anywhere<__half>(p + c * 8, columns - c * 8, begin, end);
         }
         if (f.factors != nullptr && lane == 0) {
             const float of_loss = f.grad_loss != nullptr ? f.grad_loss[r] : 0.f, of_sum = f.grad_log_sum != nullptr ? f.grad_log_sum[r] : 0.f;
@@ -255,26 +272,30 @@ gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const __half* __restri
     }
 }
 
-// grad_A[r,:] = factor times the sums of row place[r], zeros for rows that have no place. Four columns to a thread; the sums have room up to a multiple of 4.
+// grad_A[r,:] = factor times the sums of row place[r] (of both its rows, if `twice`), zeros for rows that have no place. Four columns to a thread; the sums have room up to a multiple of 4.
 template <typename T>
 __global__ void __launch_bounds__(kGatherThreads)
 scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int slices, int64_t stride, const LossRows rows, int64_t n, int columns, bool by_four,
-             const float* __restrict__ factor) {
+             bool twice, const float* __restrict__ factor) {
     const float f = *factor;
     const int quads = static_cast<int>(stride / 4), per = (quads + gridDim.y - 1) / gridDim.y;
     const int begin = blockIdx.y * per, end = min(begin + per, quads);
-    const int64_t slice = n * stride;
+    const int64_t copies = twice ? 2 : 1, slice = copies * n * stride;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; r < n; r += static_cast<int64_t>(gridDim.x) * blockDim.y) {
         const int64_t i = rows.place[r];
 #pragma unroll 2
         for (int q = begin + threadIdx.x; q < end; q += blockDim.x) {
             Pack<T, 4> out;
             if (i >= 0) {
-                const float* from = sums + i * stride + 4 * q;
-                float4 v = *reinterpret_cast<const float4*>(from);
-                for (int s = 1; s < slices; s++) {
-                    const float4 w = *reinterpret_cast<const float4*>(from + s * slice);
+                const float* from = sums + copies * i * stride + 4 * q;
+                float4 v = make_float4(0, 0, 0, 0);
+                for (int s = 0; s < slices; s++) {
+                    float4 w = *reinterpret_cast<const float4*>(from + s * slice);
                     v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                    if (twice) {
+                        w = *reinterpret_cast<const float4*>(from + s * slice + stride);
+                        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                    }
                 }
                 out.v[0] = narrow<T>(v.x * f), out.v[1] = narrow<T>(v.y * f), out.v[2] = narrow<T>(v.z * f), out.v[3] = narrow<T>(v.w * f);
             } else {
@@ -298,17 +319,17 @@ unsigned warps_for(const Call& call, int64_t rows) {
 
 int64_t whole_packs(int64_t n) { return (n + 7) / 8 * 8; }
 
-// The kept rows of A, one after the other, as the copy engine can fetch them.
-Array gathered(const Call& call, Scratch& room, const Array& A, const LossRows& rows, const FactorArgs& factors) {
-    const int64_t stride = whole_packs(A.shape[1]);
-    room.take(static_cast<size_t>(A.shape[0] * stride) * 2);
-    Array to = contiguous(room.as<void>(), A.type, A.shape[0], A.shape[1]);
+// The kept rows of A, one after the other (or each twice), as the copy engine can fetch them.
+Array gathered(const Call& call, Scratch& room, const Array& A, const LossRows& rows, bool twice, const FactorArgs& factors) {
+    const int64_t stride = whole_packs(A.shape[1]), copies = twice ? 2 : 1;
+    room.take(static_cast<size_t>(copies * A.shape[0] * stride) * 2);
+    Array to = contiguous(room.as<void>(), A.type, copies * A.shape[0], A.shape[1]);
     to.stride[0] = stride;
     const bool aligned = A.shape[1] % 8 == 0 && A.stride[0] % 8 == 0 && reinterpret_cast<uintptr_t>(A.data) % 16 == 0;
     const unsigned char* begin = static_cast<const unsigned char*>(A.data);
     gather_rows<<<warps_for(call, A.shape[0]), kGatherThreads, 0, call.stream>>>(static_cast<uint16_t*>(to.data), stride, static_cast<const __half*>(A.data), A.stride[0],
                                                                                   aligned, begin, begin + ((A.shape[0] - 1) * A.stride[0] + A.shape[1]) * 2, rows,
-                                                                                  A.shape[1], factors);
+                                                                                  A.shape[1], twice, factors);
     MOPS_CUDA_OK(cudaGetLastError());
     return to;
 }
@@ -317,6 +338,9 @@ template <typename F> void for_sixteen(int32_t type, F&& f) {
     if (type == MOPS_B200_BF16) f(std::true_type());
     else f(std::false_type());
 }
+
+// Up to so many rows dx is kept in two parts.
+constexpr int64_t kTwoPartsTo = 256;
 
 // Whether rows are numbered and gathered in front of a forward pass, which takes some 10 us: where all of them take 50 us or more on the tensor cores.
 bool worth_gathering(int64_t rows, int64_t vocabulary, int64_t columns) { return rows >= 512 && 2.0 * rows * vocabulary * columns >= 5e10; }
@@ -335,7 +359,7 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
     if (gather) {
         rows = take_rows(room_rows, n);
         prepare_rows<float>(call, rows, static_cast<float*>(loss.data), static_cast<float*>(log_sum.data), p.targets, vocabulary, p.ignored, nullptr, nullptr);
-        A = gathered(call, room_A, p.A, rows, {});
+        A = gathered(call, room_A, p.A, rows, false, {});
     } else {
         packing.add(A);
     }
@@ -377,22 +401,27 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     RowFactors* factors = room_factors.as<RowFactors>();
     float* factor = reinterpret_cast<float*>(factors + n);
     const float scale2 = static_cast<float>(p.scale * 1.4426950408889634);
-    const Array A = gathered(call, room_A, p.A, rows,
+    const bool twice = n <= kTwoPartsTo;
+    const int64_t copies = twice ? 2 : 1, all = copies * n; // rows of dx
+    const int32_t* all_rows = twice ? rows.doubled : rows.offsets;
+    const Array A = gathered(call, room_A, p.A, rows, twice,
                              {factors, factor, of_loss, of_sum, static_cast<const float*>(loss.data), static_cast<const float*>(log_sum.data), static_cast<float>(p.scale),
                               p.A.type == MOPS_B200_F16 ? 16384.f : 1.f});
+    Array first = A; // of the two rows of each
+    first.shape[0] = n, first.stride[0] = copies * A.stride[0];
     Packing packing(call);
     Array W = p.W;
     packing.add(W);
     packing.run();
     // pieces of the vocabulary, of about the same width
     constexpr int64_t kMostValues = int64_t(1) << 27; // of dx
-    const int64_t most = std::max<int64_t>(kMostValues / n / 256 * 256, 256), pieces = ceil_div(vocabulary, most);
+    const int64_t most = std::max<int64_t>(kMostValues / all / 256 * 256, 256), pieces = ceil_div(vocabulary, most);
     const int64_t width = std::min(ceil_div(ceil_div(vocabulary, pieces), 256) * 256, whole_packs(vocabulary));
-    Scratch room_dx(call, static_cast<size_t>(n * width) * 2);
+    Scratch room_dx(call, static_cast<size_t>(all * width) * 2);
     // Slices of the piece for the products with W: so many that the last round of pairs is nearly full, each of 1024 values of depth at least. What a slice more costs, sums that are written and read,
     // counts as 2 % of a round.
     const int64_t steps = ceil_div(std::min(width, vocabulary), kBoxDepth);
-    const int64_t tiles = ceil_div(n, 2 * kTileRows) * ceil_div(columns, 256), workers = sms / 2;
+    const int64_t tiles = ceil_div(all, 2 * kTileRows) * ceil_div(columns, 256), workers = sms / 2;
     int64_t slices = 1;
     double least = 1e30;
     for (int64_t s = 1; s <= 16 && (s == 1 || steps / s >= 16); s++) {
@@ -402,36 +431,43 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     slices = ceil_div(steps, ceil_div(steps, slices)); // (none without steps: the first piece writes the sums of all)
     const int64_t stride = (columns + 3) / 4 * 4;
     Scratch room_sums(call);
-    if (need_A) room_sums.take(static_cast<size_t>(slices * n * stride) * sizeof(float));
+    if (need_A) room_sums.take(static_cast<size_t>(slices * all * stride) * sizeof(float));
     float* sums = room_sums.as<float>();
     for (int64_t v0 = 0; v0 < vocabulary; v0 += width) {
         const int64_t here = std::min(width, vocabulary - v0);
         uint16_t* w = static_cast<uint16_t*>(W.data) + v0 * W.stride[0];
-        Array dx = contiguous(room_dx.as<void>(), A.type, n, here);
+        Array dx = contiguous(room_dx.as<void>(), A.type, all, here);
         dx.stride[0] = width;
         for_sixteen(A.type, [&](auto type) {
             constexpr bool BF16 = decltype(type)::value;
-            using E = GradientStore<BF16, 256>;
-            typename E::Args args{};
-            args.map = tensor_map(A.type, dx.data, here, n, 1, width, 0, 32);
-            args.out = static_cast<uint16_t*>(dx.data), args.stride = width, args.columns = static_cast<int>(here), args.first_column = static_cast<int>(v0);
-            args.scale2 = scale2, args.factors = factors;
-            const TileProblem problem{A, rows.offsets, 1, n, columns, here};
-            const TileOperand operands[2] = {{w, 1, W.stride[0], 0}, {w, 1, W.stride[0], 0}};
-            launch_tiles<BF16, false, 256, true, E, DecodeTable>(call, op, problem, operands, args);
+            auto launch = [&](auto parts) {
+                using E = GradientStore<BF16, 256, decltype(parts)::value>;
+                typename E::Args args{};
+                args.out = static_cast<uint16_t*>(dx.data), args.rest = args.out + width, args.stride = copies * width;
+                args.map = tensor_map(A.type, args.out, here, n, 1, args.stride, 0, 32);
+                if (twice) args.map_rest = tensor_map(A.type, args.rest, here, n, 1, args.stride, 0, 32);
+                args.columns = static_cast<int>(here), args.first_column = static_cast<int>(v0);
+                args.scale2 = scale2, args.factors = factors;
+                const TileProblem problem{first, rows.offsets, 1, n, columns, here};
+                const TileOperand operands[2] = {{w, 1, W.stride[0], 0}, {w, 1, W.stride[0], 0}};
+                if (n <= kTileRows) launch_tiles<BF16, false, 256, false, E, DecodeTable>(call, op, problem, operands, args);
+                else launch_tiles<BF16, false, 256, true, E, DecodeTable>(call, op, problem, operands, args);
+            };
+            if (twice) launch(std::true_type());
+            else launch(std::false_type());
             if (need_A) {
-                const TileProblem sum_problem{dx, rows.offsets, 1, n, here, columns, slices};
+                const TileProblem sum_problem{dx, all_rows, 1, all, here, columns, slices};
                 const TileOperand by_rows[2] = {{w, W.stride[0], 1, 0}, {w, W.stride[0], 1, 0}};
                 using Sums = SumStore<256>;
                 typename Sums::Args to{};
-                to.map = tensor_map(MOPS_B200_F32, sums, columns, n, slices, stride, n * stride, 32);
-                to.out = sums, to.rows = n, to.stride = stride, to.columns = static_cast<int>(columns), to.add = v0 > 0;
+                to.map = tensor_map(MOPS_B200_F32, sums, columns, all, slices, stride, all * stride, 32);
+                to.out = sums, to.rows = all, to.stride = stride, to.columns = static_cast<int>(columns), to.add = v0 > 0;
                 launch_tiles<BF16, true, 256, true, Sums, DecodeSlices>(call, op, sum_problem, by_rows, to);
             }
         });
         MOPS_CUDA_OK(cudaGetLastError());
         if (need_W)
-            multiply_outer(call, {contiguous(static_cast<uint16_t*>(grad_W.data) + v0 * columns, A.type, 1, here, columns), dx, A, rows.offsets, 1, factor}, op);
+            multiply_outer(call, {contiguous(static_cast<uint16_t*>(grad_W.data) + v0 * columns, A.type, 1, here, columns), dx, A, all_rows, 1, factor}, op);
     }
     if (need_A)
         for_sixteen(A.type, [&](auto type) {
@@ -442,7 +478,7 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
             const dim3 block(across, kGatherThreads / across);
             const unsigned down = static_cast<unsigned>(std::min<int64_t>(ceil_div(n, block.y), int64_t(sms) * 32));
             scatter_rows<T><<<down, block, 0, call.stream>>>(static_cast<T*>(grad_A.data), sums, static_cast<int>(slices), stride, rows, n, static_cast<int>(columns), by_four,
-                                                             factor);
+                                                             twice, factor);
         });
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("loss_gradient_mma<%s>, %d pieces, %d slices", A.type == MOPS_B200_BF16 ? "bf16" : "f16", static_cast<int>(pieces), static_cast<int>(slices));

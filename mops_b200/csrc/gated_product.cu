@@ -167,8 +167,9 @@ bool sixteen_bits(const Array& A, const Array& W) {
     return (A.type == MOPS_B200_F16 || A.type == MOPS_B200_BF16) && A.shape[0] > 0 && A.shape[1] > 0 && W.shape[0] > 0 && W.shape[2] > 0;
 }
 
-// Up to so many rows gradients are computed in f32 throughout: rounded to 16 bits, dU and dV of a few rows are few values, whose errors do not average out.
-constexpr int64_t kFewGradients = 64;
+// Up to so many values of dU and dV gradients are computed in f32 throughout: the errors of so few, rounded to 16 bits, do not average out. (On average they add to the error of results that are rounded
+// themselves as much as that is, 1.4 times in all.)
+constexpr int64_t kFewGradients = 2048;
 
 void gradients_16(const Call& call, const Array& grad_A, const Array& grad_W, bool turned, const Array& grad_output, const Array& A, const Array& W, const int32_t* offsets,
                   int32_t activation, const std::string& op) {
@@ -260,7 +261,7 @@ void grouped_gated_product_vjp(Array grad_A, Array grad_W, Array grad_output, Ar
     Call call = begin_call();
     const int32_t* starts = static_cast<const int32_t*>(offsets.data);
     const int64_t rows = A.shape[0], columns = W.shape[2];
-    if (sixteen_bits(A, W) && rows > kFewGradients) {
+    if (sixteen_bits(A, W) && rows * columns > kFewGradients) {
         gradients_16(call, grad_A, grad_W, turned, grad_output, A, W, starts, activation, op);
         end_call(call, op.c_str(), kIndexNames, 1);
         return;

@@ -145,7 +145,7 @@ void multiply_outer(const Call& call, const OuterProblem& p, const std::string& 
     const Array &out = p.out, &X = p.X, &Y = p.Y;
     const int32_t* offsets = p.offsets;
     const int64_t groups = p.groups, rows = X.shape[0], height = X.shape[1], columns = Y.shape[1];
-    if (groups == 0 || height == 0 || columns == 0 || multiply_outer_few(call, p, op) || multiply_outer_mma(call, p, op) ||
+    if (groups == 0 || height == 0 || columns == 0 || (p.factor == nullptr && multiply_outer_few(call, p, op)) || multiply_outer_mma(call, p, op) ||
         multiply_outer_split(call, p, op))
         return;
     fits_int32(static_cast<size_t>(groups), "the number of groups", op);

@@ -14,7 +14,7 @@ struct RowsProblem {
     int64_t groups, rows, depth, columns;
 };
 
-// out[g] = X[rows of g]^T Y[rows of g]; out is contiguous. factor: in device memory, of 16-bit results on tensor cores (more than two rows for each group) alone.
+// out[g] = X[rows of g]^T Y[rows of g]; out is contiguous. factor, if any: in device memory, for 16-bit results.
 struct OuterProblem {
     Array out, X, Y;
     const int32_t* offsets;

@@ -11,6 +11,7 @@ namespace mops_b200 {
 
 struct LossRows {
     int32_t* offsets; // 0, kept
+    int32_t* doubled; // 0, 2 kept
     int32_t* order;   // of the i-th kept row: its number
     int32_t* place;   // of a row: i, or -1
     int32_t* target;  // of the i-th kept row
@@ -94,9 +95,9 @@ void join_rows(const Call& call, const Array& loss, const Array& log_sum, const 
 }
 
 inline LossRows take_rows(Scratch& room, int64_t rows) {
-    room.take(static_cast<size_t>(3 * rows + 4) * sizeof(int32_t));
+    room.take(static_cast<size_t>(3 * rows + 8) * sizeof(int32_t));
     int32_t* p = room.as<int32_t>();
-    return {p, p + 4, p + 4 + rows, p + 4 + 2 * rows, reinterpret_cast<float*>(p + 2)};
+    return {p, p + 2, p + 8, p + 8 + rows, p + 8 + 2 * rows, reinterpret_cast<float*>(p + 4)};
 }
 
 // Numbers the rows that have a target (cross_entropy.cu). The others get zeros in loss and log_sum, if these are given; of gradients, if they are, the unit is found.
