@@ -10,6 +10,7 @@
 // and never stored. Here: f32 and f64 (and f16 and bf16 without columns); f16 and bf16 are in cross_entropy_mma.cu.
 #include "block_ops.hpp"
 #include "convert.cuh"
+#include "few_rows.cuh"
 #include "grouped_mma.hpp"
 #include "loss_rows.cuh"
 #include "pack.hpp"
@@ -22,7 +23,8 @@ constexpr int kPrepareThreads = 1024, kPrepareRows = 8;
 constexpr int64_t kPartColumns = 4096;             // of a part of a row's sums, at most
 constexpr int64_t kMostLogits = int64_t(64) << 20; // of a piece
 
-// Numbers the rows that have a target, by one block; the others get zeros, if loss is given.
+// Numbers the rows that have a target, by a block, or a cluster of blocks with a part of the rows each, which count theirs first; the others get zeros, if loss is given. (16 384 rows: one block 13.8 us,
+// 9 by eight; 48 285: 31 and 9.)
 template <typename S>
 __global__ void __launch_bounds__(kPrepareThreads)
 loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, const int32_t* __restrict__ targets, int64_t rows, int64_t vocabulary,
@@ -31,22 +33,42 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
     __shared__ int in_run[kRuns], in_front[kRuns + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool gradients = grad_loss != nullptr || grad_log_sum != nullptr;
-    int before = 0;
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int64_t part = (rows + blocks - 1) / blocks, begin = min(rank * part, rows), end = min(begin + part, rows);
+    int before = 0, all = 0;
+    __shared__ int own_count;
+    if (blocks > 1) {
+        if (threadIdx.x == 0) own_count = 0;
+        __syncthreads();
+        int own = 0;
+        for (int64_t r = begin + threadIdx.x; r < end; r += kPrepareThreads) {
+            const int64_t t = targets[r];
+            own += t >= 0 && t < vocabulary && t != ignored;
+        }
+        own = __reduce_add_sync(kFullMask, own);
+        if (lane == 0) atomicAdd(&own_count, own);
+        cluster.sync();
+        for (int b = 0; b < blocks; b++) {
+            const int n = *cluster.map_shared_rank(&own_count, b);
+            before += b < rank ? n : 0, all += n;
+        }
+    }
     float largest[3] = {}; // of the gradients of losses, of sums, of both together
     bool bad = false;
-    for (int64_t r0 = 0; r0 < rows; r0 += kPrepareThreads * kPrepareRows) {
+    for (int64_t r0 = begin; r0 < end; r0 += kPrepareThreads * kPrepareRows) {
         int32_t target[kPrepareRows];
         unsigned kept[kPrepareRows];
 #pragma unroll
         for (int k = 0; k < kPrepareRows; k++) {
             const int64_t r = r0 + k * kPrepareThreads + threadIdx.x;
-            target[k] = r < rows ? targets[r] : 0;
+            target[k] = r < end ? targets[r] : 0;
         }
 #pragma unroll
         for (int k = 0; k < kPrepareRows; k++) {
             const int64_t r = r0 + k * kPrepareThreads + threadIdx.x, t = target[k];
-            const bool in = r < rows && t >= 0 && t < vocabulary && t != ignored;
-            bad |= r < rows && !in && t != ignored;
+            const bool in = r < end && t >= 0 && t < vocabulary && t != ignored;
+            bad |= r < end && !in && t != ignored;
             kept[k] = __ballot_sync(kFullMask, in);
             if (lane == 0) in_run[k * (kPrepareThreads / 32) + warp] = __popc(kept[k]);
         }
@@ -71,7 +93,7 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
 #pragma unroll
         for (int k = 0; k < kPrepareRows; k++) {
             const int64_t r = r0 + k * kPrepareThreads + threadIdx.x;
-            if (r >= rows) continue;
+            if (r >= end) continue;
             const bool in = kept[k] >> lane & 1;
             const int i = before + in_front[k * (kPrepareThreads / 32) + warp] + __popc(kept[k] & ((1u << lane) - 1));
             to.place[r] = in ? i : -1;
@@ -93,8 +115,8 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
         before += in_front[kRuns];
         __syncthreads();
     }
+    __shared__ float most[3][kPrepareThreads / 32];
     if (gradients) {
-        __shared__ float most[3][kPrepareThreads / 32];
 #pragma unroll
         for (int q = 0; q < 3; q++) {
 #pragma unroll
@@ -102,14 +124,27 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
             if (lane == 0) most[q][warp] = largest[q];
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < kPrepareThreads / 32; w++)
-                for (int q = 0; q < 3; q++) largest[q] = fmaxf(largest[q], most[q][w]);
+        if (threadIdx.x < 3) {
+            float m = 0;
+            for (int w = 0; w < kPrepareThreads / 32; w++) m = fmaxf(m, most[threadIdx.x][w]);
+            most[threadIdx.x][0] = m;
+        }
+    }
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
+    if (threadIdx.x == 0 && rank == 0) {
+        const int kept = blocks > 1 ? all : before;
+        to.offsets[0] = 0, to.offsets[1] = kept, to.doubled[0] = 0, to.doubled[1] = 2 * kept;
+        if (gradients) {
+            for (int q = 0; q < 3; q++) {
+                largest[q] = 0;
+                for (int b = 0; b < blocks; b++) largest[q] = fmaxf(largest[q], *cluster.map_shared_rank(&most[q][0], b));
+            }
             // (small gradients of sums are left out: 16-bit units are those of the losses', so that -1 stays -1)
             *to.unit = largest[1] <= 2 * largest[0] ? largest[0] : largest[2];
         }
     }
-    if (threadIdx.x == 0) to.offsets[0] = 0, to.offsets[1] = before, to.doubled[0] = 0, to.doubled[1] = 2 * before;
+    if (blocks > 1) cluster.sync(); // (nobody leaves while others read what it found)
     if (bad) report_bad_index(st, 0);
 }
 
@@ -298,8 +333,10 @@ const char* const kIndexNames[] = {"targets"};
 template <typename S>
 void prepare_rows(const Call& call, const LossRows& to, S* loss, S* log_sum, const Array& targets, int64_t vocabulary, int64_t ignored, const S* grad_loss,
                   const S* grad_log_sum) {
-    loss_prepare<S><<<1, kPrepareThreads, 0, call.stream>>>(to, loss, log_sum, static_cast<const int32_t*>(targets.data), targets.shape[0], vocabulary, ignored, grad_loss,
-                                                            grad_log_sum, call.status);
+    const int64_t rows = targets.shape[0];
+    Clusters clusters(call, "linear_cross_entropy", 1, rows > kPrepareThreads * kPrepareRows / 2 ? 8 : 1, 1, kPrepareThreads, 0);
+    MOPS_CUDA_OK(cudaLaunchKernelEx(&clusters.config, loss_prepare<S>, to, loss, log_sum, static_cast<const int32_t*>(targets.data), rows, vocabulary, ignored, grad_loss,
+                                    grad_log_sum, call.status));
     MOPS_CUDA_OK(cudaGetLastError());
 }
 template void prepare_rows(const Call&, const LossRows&, float*, float*, const Array&, int64_t, int64_t, const float*, const float*);
@@ -343,14 +380,12 @@ template <typename S> struct Pieces {
     Array A, W, logits;
     int64_t width, part; // columns of a piece, and of a part of it
     bool fused;          // worked on where they are summed
+    bool numbered;       // rows without a target have been left out
     static constexpr int32_t kType = sizeof(S) == 8 ? MOPS_B200_F64 : MOPS_B200_F32;
 
-    Pieces(const Call& call, const std::string& op, const Array& a, const Array& w)
+    Pieces(const Call& call, const std::string& op, const Array& a, const Array& w, bool forward)
         : call(call), op(op), room_rows(call), room_A(call), room_W(call), room_logits(call), packing(call), W(w) {
         const int64_t n = a.shape[0], columns = a.shape[1];
-        rows = take_rows(room_rows, n);
-        room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
-        A = contiguous(room_A.as<void>(), kType, n, columns);
         if (w.type != kType) {
             room_W.take(static_cast<size_t>(values_of(w)) * sizeof(S) + 16);
             W = converted(call, w, room_W.as<S>(), kType);
@@ -359,19 +394,31 @@ template <typename S> struct Pieces {
         width = width >= kPartColumns ? width / kPartColumns * kPartColumns : width / 256 * 256;
         part = std::min(width, kPartColumns);
         width = std::min(width, W.shape[0]);
-        fused = kType == MOPS_B200_F32 && columns > 0 && !straight_rows(matrices(0, W.shape[0]), n, false);
+        // (15 rows of 30 029 x 96: 16.6 us, by the kernels for few rows and a pass over their logits 44; but those read W wherever its rows begin, which costs a copy here, and gradients take
+        // that copy in any case)
+        fused = kType == MOPS_B200_F32 && columns > 0 &&
+                (!forward || !straight_rows(matrices(0, W.shape[0]), n, false) || boxable(kType, W.data, columns, W.shape[0], 1, W.stride[0], 0));
+        numbered = !forward || !fused || a.type != kType || worth_gathering(kType, n, W.shape[0], columns);
+        if (numbered) {
+            rows = take_rows(room_rows, n);
+            room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
+            A = contiguous(room_A.as<void>(), kType, n, columns);
+        } else {
+            rows = LossRows{};
+            A = a;
+        }
     }
     void take_logits() { room_logits.take(static_cast<size_t>(A.shape[0] * (width + 3)) * sizeof(S) + 16); }
     TileProblem problem(int64_t columns) const { return {A, rows.offsets, 1, A.shape[0], A.shape[1], columns}; }
     void gather(const Array& a) {
         if (a.shape[1] == 0) return;
-        for_type(a.type, [&](auto zero) {
+        if (numbered) for_type(a.type, [&](auto zero) {
             using From = decltype(zero);
             loss_gather<S, From><<<row_blocks(call, a.shape[0]), row_threads(), 0, call.stream>>>(
                 static_cast<S*>(A.data), a.shape[1], static_cast<const From*>(a.data), a.stride[0], rows, a.shape[1]);
         });
         MOPS_CUDA_OK(cudaGetLastError());
-        if (kType == MOPS_B200_F32 && !straight_rows(matrices(0, W.shape[0]), A.shape[0], false)) {
+        if (fused) {
             packing.add(A);
             packing.add(W);
             packing.run();
@@ -400,17 +447,17 @@ template <typename S> struct Pieces {
 template <typename S>
 void loss_forward(const Call& call, const Array& loss, const Array& log_sum, const Array& A, const Array& W, const Array& targets, double scale,
                   int64_t ignored, const std::string& op) {
-    Pieces<S> pieces(call, op, A, W);
+    Pieces<S> pieces(call, op, A, W, true);
     const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.fused ? LossStore32::kOwn : pieces.part);
     const int32_t* t = static_cast<const int32_t*>(targets.data);
-    prepare_rows<S>(call, pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), targets, W.shape[0], ignored, nullptr, nullptr);
+    if (pieces.numbered) prepare_rows<S>(call, pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), targets, W.shape[0], ignored, nullptr, nullptr);
     pieces.gather(A);
     Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<S>) + static_cast<size_t>(n) * sizeof(S));
     PartSum<S>* sums = room.as<PartSum<S>>();
     S* at_target = reinterpret_cast<S*>(sums + n * parts);
     if constexpr (sizeof(S) == 4) {
         if (pieces.fused) {
-            const LossStore32::Args args{sums, parts, at_target, pieces.rows.target, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
+            const LossStore32::Args args{sums, parts, at_target, pieces.numbered ? pieces.rows.target : t, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
             const TileOperand w{pieces.W.data, 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
             launch_split<false, LossStore32, DecodeTable>(call, op, pieces.problem(W.shape[0]), operands, args);
             note_kernel("loss_rows_split");
@@ -427,7 +474,7 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
 template <typename S>
 void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, const Array& grad_loss, const Array& grad_log_sum, const Array& log_sum,
                    const Array& A, const Array& W, const Array& targets, double scale, int64_t ignored, const std::string& op) {
-    Pieces<S> pieces(call, op, A, W);
+    Pieces<S> pieces(call, op, A, W, false);
     const int64_t n = A.shape[0], columns = A.shape[1];
     const int32_t* t = static_cast<const int32_t*>(targets.data);
     prepare_rows<S>(call, pieces.rows, nullptr, nullptr, targets, W.shape[0], ignored, nullptr, nullptr);
@@ -435,9 +482,15 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     pieces.gather(A);
     const bool need_A = grad_A.data != nullptr, need_W = grad_W.data != nullptr, widened = A.type != pieces.kType;
     Scratch room_A(call), room_more(call), room_W(call);
-    const size_t bytes = static_cast<size_t>(n * columns) * sizeof(S);
+    const int64_t stride_A = pieces.fused ? (columns + 3) / 4 * 4 : columns; // of the sums for grad_A
+    int64_t slices = 1;
+    if (pieces.fused && need_A) {
+        const int64_t deep = ceil_div(pieces.width, split::kDepth), tiles = ceil_div(n, kTileRows) * ceil_div(columns, kSplitColumns);
+        slices = best_slices(tiles, sm_count(call.device), deep, 0.7, 16, static_cast<double>(n) * columns * 8);
+    }
+    const size_t bytes = static_cast<size_t>(slices * n * stride_A) * sizeof(S);
     if (need_A) room_A.take(bytes);
-    if (need_A && pieces.width < W.shape[0]) room_more.take(bytes);
+    if (need_A && !pieces.fused && pieces.width < W.shape[0]) room_more.take(bytes);
     if (need_W && widened) room_W.take(static_cast<size_t>(pieces.width * columns) * sizeof(S));
     auto multiply = [&](int64_t v0, int64_t v1, Array dx) {
         Array m = pieces.matrices(v0, v1), a = pieces.A;
@@ -451,7 +504,13 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
             if (outer_packed) packing.add(a);
             packing.run();
         }
-        if (need_A) {
+        if (need_A && pieces.fused) {
+            if constexpr (sizeof(S) == 4) {
+                TileProblem problem{dx, pieces.rows.offsets, 1, n, v1 - v0, columns, slices};
+                const TileOperand w{m.data, m.stride[1], 1, 0}, operands[2] = {w, w};
+                launch_split<true, SumStore32, DecodeSlices>(call, op, problem, operands, sum_args(room_A.template as<float>(), slices, n, stride_A, columns, v0 > 0));
+            }
+        } else if (need_A) {
             S* to = v0 == 0 ? room_A.as<S>() : room_more.as<S>();
             multiply_rows(call, {contiguous(to, pieces.kType, n, columns), dx, m, m.stride[1], 1, pieces.rows.offsets, 1, n, v1 - v0, columns}, op);
             if (v0 > 0) add_values<S><<<blocks_for(call, n * columns), 256, 0, call.stream>>>(room_A.as<S>(), to, n * columns);
@@ -492,11 +551,22 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
             multiply(v0, v1, pieces.logits);
         });
     }
-    if (need_A)
-        for_type(grad_A.type, [&](auto zero) {
-            using T = decltype(zero);
-            loss_scatter<T, S><<<row_blocks(call, n), row_threads(), 0, call.stream>>>(static_cast<T*>(grad_A.data), room_A.as<S>(), pieces.rows, n, columns);
-        });
+    if (need_A) {
+        if constexpr (sizeof(S) == 4) {
+            if (pieces.fused) {
+                for_type(grad_A.type, [&](auto zero) {
+                    using T = decltype(zero);
+                    if constexpr (!std::is_same<T, double>::value)
+                        scatter_sums(call, static_cast<T*>(grad_A.data), room_A.template as<float>(), slices, stride_A, pieces.rows, n, columns, false, nullptr);
+                });
+            }
+        }
+        if (!pieces.fused)
+            for_type(grad_A.type, [&](auto zero) {
+                using T = decltype(zero);
+                loss_scatter<T, S><<<row_blocks(call, n), row_threads(), 0, call.stream>>>(static_cast<T*>(grad_A.data), room_A.as<S>(), pieces.rows, n, columns);
+            });
+    }
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("loss_gradient<%s>", scalar_name<S>());
 }

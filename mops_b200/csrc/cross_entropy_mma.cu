@@ -8,6 +8,8 @@
 // multiplies the results: so the gradient of a mean, which is the same for all rows, leaves -1 at the targets as it is. A row's value there is 1 - exp(-loss), not the difference of rounded numbers.
 // A row's gradient is for the most part that of its target, whose rounding is an error of the row as a whole; where there are too few rows for such errors to average out, dx is kept in two parts of
 // 16 bits (a row of what the first leaves under it, and rows of A twice): the products are bounded by memory there.
+#include <numeric>
+
 #include "block_ops.hpp"
 #include "grouped_mma.hpp"
 #include "loss_rows.cuh"
@@ -169,13 +171,6 @@ template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
 
 // Sums in f32: of the first piece of the vocabulary they are written, those of others are added to what is there. Each slice of the depth has sums of its own, so that no two
 // blocks add to one place, and the order of the additions is that of the pieces.
-__device__ __forceinline__ void box_add(const CUtensorMap& map, int inner, int outer, int slice, uint32_t smem) {
-    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(&map), "r"(inner), "r"(outer),
-                 "r"(slice), "r"(smem)
-                 : "memory");
-    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
-}
-
 template <int kColumns> struct SumStore {
     static constexpr bool kHalves = false;
     static constexpr int kStoreWarps = 8, kStaging = 32 * kBoxRow, kOwn = kColumns / 2;
@@ -272,47 +267,6 @@ gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const __half* __restri
     }
 }
 
-// grad_A[r,:] = factor times the sums of row place[r] (of both its rows, if `twice`), zeros for rows that have no place. Four columns to a thread; the sums have room up to a multiple of 4.
-template <typename T>
-__global__ void __launch_bounds__(kGatherThreads)
-scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int slices, int64_t stride, const LossRows rows, int64_t n, int columns, bool by_four,
-             bool twice, const float* __restrict__ factor) {
-    const float f = *factor;
-    const int quads = static_cast<int>(stride / 4), per = (quads + gridDim.y - 1) / gridDim.y;
-    const int begin = blockIdx.y * per, end = min(begin + per, quads);
-    const int64_t copies = twice ? 2 : 1, slice = copies * n * stride;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; r < n; r += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-        const int64_t i = rows.place[r];
-#pragma unroll 2
-        for (int q = begin + threadIdx.x; q < end; q += blockDim.x) {
-            Pack<T, 4> out;
-            if (i >= 0) {
-                const float* from = sums + copies * i * stride + 4 * q;
-                float4 v = make_float4(0, 0, 0, 0);
-                for (int s = 0; s < slices; s++) {
-                    float4 w = *reinterpret_cast<const float4*>(from + s * slice);
-                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                    if (twice) {
-                        w = *reinterpret_cast<const float4*>(from + s * slice + stride);
-                        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                    }
-                }
-                out.v[0] = narrow<T>(v.x * f), out.v[1] = narrow<T>(v.y * f), out.v[2] = narrow<T>(v.z * f), out.v[3] = narrow<T>(v.w * f);
-            } else {
-                out.v[0] = out.v[1] = out.v[2] = out.v[3] = T(0.f);
-            }
-            T* p = to + r * columns + 4 * q;
-            if (by_four) {
-                *reinterpret_cast<Pack<T, 4>*>(p) = out;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (4 * q + k < columns) p[k] = out.v[k];
-            }
-        }
-    }
-}
-
 unsigned warps_for(const Call& call, int64_t rows) {
     return static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(rows, kGatherThreads / 32), 1), int64_t(sm_count(call.device)) * 16));
 }
@@ -342,9 +296,6 @@ template <typename F> void for_sixteen(int32_t type, F&& f) {
 // Up to so many rows dx is kept in two parts.
 constexpr int64_t kTwoPartsTo = 256;
 
-// Whether rows are numbered and gathered in front of a forward pass, which takes some 10 us: where all of them take 50 us or more on the tensor cores.
-bool worth_gathering(int64_t rows, int64_t vocabulary, int64_t columns) { return rows >= 512 && 2.0 * rows * vocabulary * columns >= 5e10; }
-
 } // namespace
 
 void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss, const Array& log_sum, const std::string& op) {
@@ -355,7 +306,7 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
     Array A = p.A, W = p.W;
     LossRows rows{};
     const int32_t* targets = static_cast<const int32_t*>(p.targets.data);
-    const bool gather = worth_gathering(n, vocabulary, p.A.shape[1]);
+    const bool gather = worth_gathering(A.type, n, vocabulary, p.A.shape[1]);
     if (gather) {
         rows = take_rows(room_rows, n);
         prepare_rows<float>(call, rows, static_cast<float*>(loss.data), static_cast<float*>(log_sum.data), p.targets, vocabulary, p.ignored, nullptr, nullptr);
@@ -365,7 +316,9 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
     }
     packing.add(W);
     packing.run();
-    const bool narrow_tiles = n <= kTileRows;
+    // (where rows are a quarter of a box at most, which is fetched for each tile, tiles of 128 columns leave no SM with twice the work of others: 8 rows of 50021 x 1024 26 us; with more, wider ones are
+    // faster: 66 rows of 88288 x 736 41 us in tiles of 128, 36 in tiles of 256)
+    const bool narrow_tiles = n <= kTileRows / 4;
     const int64_t own = narrow_tiles ? 64 : 128, parts = ceil_div(vocabulary, own);
     Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<float>) + static_cast<size_t>(n) * sizeof(float));
     PartSum<float>* sums = room.as<PartSum<float>>();
@@ -381,6 +334,7 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
             note_kernel_f("loss_rows_mma<%s,%d,%s>", type ? "bf16" : "f16", static_cast<int>(width), paired ? "pair" : "block");
         };
         if (narrow_tiles) launch(integral_constant<int, 128>(), std::false_type());
+        else if (n <= kTileRows) launch(integral_constant<int, 256>(), std::false_type());
         else launch(integral_constant<int, 256>(), std::true_type());
     });
     MOPS_CUDA_OK(cudaGetLastError());
@@ -413,22 +367,15 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     Array W = p.W;
     packing.add(W);
     packing.run();
-    // pieces of the vocabulary, of about the same width
-    constexpr int64_t kMostValues = int64_t(1) << 27; // of dx
-    const int64_t most = std::max<int64_t>(kMostValues / all / 256 * 256, 256), pieces = ceil_div(vocabulary, most);
-    const int64_t width = std::min(ceil_div(ceil_div(vocabulary, pieces), 256) * 256, whole_packs(vocabulary));
+    // Pieces of the vocabulary: as wide as there is room for dx, by steps whose tiles of grad_W are whole rounds of pairs (8192 rows of 100 003 x 1024: seven equal pieces, whose last rounds were a twelfth
+    // full, took 1666 us for grad_W, some 1300 in these).
+    constexpr int64_t kMostValues = int64_t(1) << 28; // of dx
+    const int64_t most = std::max<int64_t>(kMostValues / all / 256 * 256, 256), across = ceil_div(columns, 256), unit = sms / 2 / std::gcd<int64_t>(sms / 2, across) * 256;
+    const int64_t width = std::min(unit <= most ? most / unit * unit : most, whole_packs(vocabulary)), pieces = ceil_div(vocabulary, width);
     Scratch room_dx(call, static_cast<size_t>(all * width) * 2);
-    // Slices of the piece for the products with W: so many that the last round of pairs is nearly full, each of 1024 values of depth at least. What a slice more costs, sums that are written and read,
-    // counts as 2 % of a round.
+    // Slices of the piece for the products with W.
     const int64_t steps = ceil_div(std::min(width, vocabulary), kBoxDepth);
-    const int64_t tiles = ceil_div(all, 2 * kTileRows) * ceil_div(columns, 256), workers = sms / 2;
-    int64_t slices = 1;
-    double least = 1e30;
-    for (int64_t s = 1; s <= 16 && (s == 1 || steps / s >= 16); s++) {
-        const double rounds = static_cast<double>(ceil_div(tiles * s, workers)) / s + 0.02 * s;
-        if (rounds < least) least = rounds, slices = s;
-    }
-    slices = ceil_div(steps, ceil_div(steps, slices)); // (none without steps: the first piece writes the sums of all)
+    const int64_t slices = best_slices(ceil_div(all, 2 * kTileRows) * ceil_div(columns, 256), sms / 2, steps, 0.42, 16, static_cast<double>(all) * columns * 8);
     const int64_t stride = (columns + 3) / 4 * 4;
     Scratch room_sums(call);
     if (need_A) room_sums.take(static_cast<size_t>(slices * all * stride) * sizeof(float));
@@ -472,13 +419,7 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     if (need_A)
         for_sixteen(A.type, [&](auto type) {
             using T = std::conditional_t<decltype(type)::value, __nv_bfloat16, __half>;
-            const bool by_four = columns % 4 == 0 && reinterpret_cast<uintptr_t>(grad_A.data) % 8 == 0;
-            unsigned across = 32;
-            while (across < kGatherThreads && across * 4 < columns) across *= 2;
-            const dim3 block(across, kGatherThreads / across);
-            const unsigned down = static_cast<unsigned>(std::min<int64_t>(ceil_div(n, block.y), int64_t(sms) * 32));
-            scatter_rows<T><<<down, block, 0, call.stream>>>(static_cast<T*>(grad_A.data), sums, static_cast<int>(slices), stride, rows, n, static_cast<int>(columns), by_four,
-                                                             twice, factor);
+            scatter_sums(call, static_cast<T*>(grad_A.data), sums, slices, stride, rows, n, columns, twice, factor);
         });
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("loss_gradient_mma<%s>, %d pieces, %d slices", A.type == MOPS_B200_BF16 ? "bf16" : "f16", static_cast<int>(pieces), static_cast<int>(slices));

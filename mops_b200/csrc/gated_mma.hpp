@@ -2,7 +2,7 @@
 #ifndef MOPS_B200_GATED_MMA_HPP
 #define MOPS_B200_GATED_MMA_HPP
 
-#include "arrays.hpp"
+#include "grouped_mma.hpp"
 
 namespace mops_b200 {
 
@@ -24,6 +24,8 @@ void gated_rows_vjp_mma(const Call& call, const GatedProblem& p, void* to, const
 // The same of f32; `to` is rows x 2 columns, boxable or not.
 void gated_rows_split(const Call& call, const GatedProblem& p, const Array& output, const std::string& op);
 void gated_rows_vjp_split(const Call& call, const GatedProblem& p, const Array& to, const Array& grad, const std::string& op);
+// grad_A = duv W^T, where that is worth cutting the depth for (few tiles of a long depth); else false.
+bool multiply_rows_sliced(const Call& call, const RowsProblem& p, const std::string& op);
 
 } // namespace mops_b200
 

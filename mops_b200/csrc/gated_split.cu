@@ -128,4 +128,23 @@ void gated_rows_vjp_split(const Call& call, const GatedProblem& p, const Array& 
     });
 }
 
+bool multiply_rows_sliced(const Call& call, const RowsProblem& p, const std::string& op) {
+    const int64_t sms = sm_count(call.device), tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kSplitColumns);
+    const int64_t slices = best_slices(tiles, sms, ceil_div(p.depth, split::kDepth), 0.7, 16, static_cast<double>(p.rows) * p.columns * 8);
+    if (2 * tiles > sms || slices == 1) return false;
+    const int64_t stride = (p.columns + 3) / 4 * 4;
+    Scratch room(call, static_cast<size_t>(slices * p.rows * stride) * sizeof(float));
+    const TileProblem problem{p.X, p.offsets, p.groups, p.rows, p.depth, p.columns, slices};
+    const TileOperand m{p.M.data, p.depth_stride, p.column_stride, p.M.stride[0]}, operands[2] = {m, m};
+    const SumStore32::Args args = sum_args(room.as<float>(), slices, p.rows, stride, p.columns, false);
+    if (m.by_columns()) launch_split<true, SumStore32, DecodeRowSlices>(call, op, problem, operands, args);
+    else launch_split<false, SumStore32, DecodeRowSlices>(call, op, problem, operands, args);
+    const int64_t blocks = std::min<int64_t>(ceil_div(p.rows * stride / 4, 256), sms * 16);
+    add_slices<<<static_cast<unsigned>(blocks), 256, 0, call.stream>>>(static_cast<float*>(p.out.data), room.as<float>(), static_cast<int>(slices), p.rows, stride,
+                                                                        static_cast<int>(p.columns));
+    MOPS_CUDA_OK(cudaGetLastError());
+    note_kernel_f("split_rows, %d slices", static_cast<int>(slices));
+    return true;
+}
+
 } // namespace mops_b200

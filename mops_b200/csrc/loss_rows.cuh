@@ -105,6 +105,63 @@ template <typename S>
 void prepare_rows(const Call& call, const LossRows& to, S* loss, S* log_sum, const Array& targets, int64_t vocabulary, int64_t ignored, const S* grad_loss,
                   const S* grad_log_sum);
 
+// grad_A[r,:] = *factor (if it is given) times the sums of row place[r] (of both its rows, if `twice`), zeros for rows that have no place. Four columns to a thread; the sums have room up to a multiple of 4.
+constexpr int kScatterThreads = 256;
+template <typename T>
+static __global__ void __launch_bounds__(kScatterThreads)
+scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int slices, int64_t stride, const LossRows rows, int64_t n, int columns, bool by_four,
+             bool twice, const float* __restrict__ factor) {
+    const float f = factor != nullptr ? *factor : 1.f;
+    const int quads = static_cast<int>(stride / 4);
+    const int64_t copies = twice ? 2 : 1, slice = copies * n * stride;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; r < n; r += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        const int64_t i = rows.place[r];
+#pragma unroll 2
+        for (int q = threadIdx.x; q < quads; q += blockDim.x) {
+            Pack<T, 4> out;
+            if (i >= 0) {
+                const float* from = sums + copies * i * stride + 4 * q;
+                float4 v = make_float4(0, 0, 0, 0);
+                for (int s = 0; s < slices; s++) {
+                    float4 w = *reinterpret_cast<const float4*>(from + s * slice);
+                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                    if (twice) {
+                        w = *reinterpret_cast<const float4*>(from + s * slice + stride);
+                        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                    }
+                }
+                out.v[0] = narrow<T>(v.x * f), out.v[1] = narrow<T>(v.y * f), out.v[2] = narrow<T>(v.z * f), out.v[3] = narrow<T>(v.w * f);
+            } else {
+                out.v[0] = out.v[1] = out.v[2] = out.v[3] = T(0.f);
+            }
+            T* p = to + r * columns + 4 * q;
+            if (by_four) {
+                *reinterpret_cast<Pack<T, 4>*>(p) = out;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (4 * q + k < columns) p[k] = out.v[k];
+            }
+        }
+    }
+}
+template <typename T>
+void scatter_sums(const Call& call, T* grad_A, const float* sums, int64_t slices, int64_t stride, const LossRows& rows, int64_t n, int64_t columns, bool twice,
+                  const float* factor) {
+    const bool by_four = columns % 4 == 0 && reinterpret_cast<uintptr_t>(grad_A) % (4 * sizeof(T)) == 0;
+    unsigned across = 32;
+    while (across < kScatterThreads && across * 4 < columns) across *= 2;
+    const dim3 block(across, kScatterThreads / across);
+    const unsigned down = static_cast<unsigned>(std::min<int64_t>(ceil_div(n, block.y), int64_t(sm_count(call.device)) * 32));
+    scatter_rows<T><<<down, block, 0, call.stream>>>(grad_A, sums, static_cast<int>(slices), stride, rows, n, static_cast<int>(columns), by_four, twice, factor);
+    MOPS_CUDA_OK(cudaGetLastError());
+}
+
+// Whether rows are numbered and gathered in front of a forward pass, which takes some 10 us: where all of them take 50 us or more (f32 takes eight times as long as 16 bits).
+inline bool worth_gathering(int32_t type, int64_t rows, int64_t vocabulary, int64_t columns) {
+    return rows >= 512 && 2.0 * rows * vocabulary * columns >= (type == MOPS_B200_F32 ? 6e9 : 5e10);
+}
+
 // The vocabulary's loss on tensor cores, f16 and bf16 (cross_entropy_mma.cu).
 struct LossProblem {
     Array A, W, targets;

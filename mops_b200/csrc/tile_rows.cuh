@@ -132,6 +132,14 @@ struct BoxOut {
     }
 };
 
+// As box_out, but added (f32) to what is there.
+__device__ __forceinline__ void box_add(const CUtensorMap& map, int inner, int outer, int slice, uint32_t smem) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(&map), "r"(inner), "r"(outer),
+                 "r"(slice), "r"(smem)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+
 // Rows of 128 bytes that a warp has in its staging memory before its accumulator is there: a row for each lane, laid out as a box is.
 struct RowsIn {
     // from: the first row's first byte, all on multiples of 16 bytes. `here` rows; the others are left as they are.
@@ -316,6 +324,19 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
     __syncwarp();
     block.end(warp);
+}
+
+// How many slices the depth of a product (of `steps` stages, microseconds each; slices of `least` stages at least) is cut into, each with sums of its own: so many that the last round of `workers` is nearly
+// full, for what the sums (bytes, written and read again) take at some 4 TB/s.
+inline int64_t best_slices(int64_t tiles, int64_t workers, int64_t steps, double microseconds, int64_t least, double bytes) {
+    int64_t best = 1;
+    double shortest = 1e30;
+    for (int64_t s = 1; s <= 64 && (s == 1 || steps / s >= least); s++) {
+        const int64_t per = ceil_div(steps, s);
+        const double time = static_cast<double>(ceil_div(tiles * ceil_div(steps, per), workers)) * (per * microseconds + 1.0) + s * bytes / 4e6;
+        if (time < shortest) shortest = time, best = s;
+    }
+    return ceil_div(steps, ceil_div(steps, best)); // (none without steps: all have sums)
 }
 
 // What a launch takes from its problem; `columns`: of the result.
