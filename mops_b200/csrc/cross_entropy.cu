@@ -244,7 +244,7 @@ struct LossStore32 {
     __device__ LossStore32(const Args& a, uint32_t, int lane) : a(a), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
         row = r + lane, here = h, first = piece.column + half * kOwn;
-        target = lane < here ? a.target[row] : -1;
+        target = lane < here && piece.group >= 0 ? a.target[row] : -1;
     }
     __device__ __forceinline__ void store(float (&sum)[kOwn]) const {
         const int wide = min(a.columns - first, kOwn);
@@ -297,7 +297,7 @@ struct GradientStore32 {
     __device__ GradientStore32(const Args& a, uint32_t staging, int lane) : a(a), out{a.map, a.out, a.stride, a.columns, false}, staging(staging), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
         row = r, here = h, first = piece.column + half * kOwn;
-        if (lane < here) {
+        if (lane < here && piece.group >= 0) { // (behind the last numbered row there are no numbers)
             const int64_t of = a.rows.order[row + lane];
             target = a.rows.target[row + lane] - a.first_column;
             const float l = a.grad_loss != nullptr ? a.grad_loss[of] : 0.f, m = a.grad_log_sum != nullptr ? a.grad_log_sum[of] : 0.f;
@@ -459,7 +459,8 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
         if (pieces.fused) {
             const LossStore32::Args args{sums, parts, at_target, pieces.numbered ? pieces.rows.target : t, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
             const TileOperand w{pieces.W.data, 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
-            launch_split<false, LossStore32, DecodeTable>(call, op, pieces.problem(W.shape[0]), operands, args);
+            if (pieces.numbered) launch_split<false, LossStore32, DecodeRows>(call, op, pieces.problem(W.shape[0]), operands, args);
+            else launch_split<false, LossStore32, DecodeTable>(call, op, pieces.problem(W.shape[0]), operands, args);
             note_kernel("loss_rows_split");
         }
     }
@@ -508,7 +509,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
             if constexpr (sizeof(S) == 4) {
                 TileProblem problem{dx, pieces.rows.offsets, 1, n, v1 - v0, columns, slices};
                 const TileOperand w{m.data, m.stride[1], 1, 0}, operands[2] = {w, w};
-                launch_split<true, SumStore32, DecodeSlices>(call, op, problem, operands, sum_args(room_A.template as<float>(), slices, n, stride_A, columns, v0 > 0));
+                launch_split<true, SumStore32, DecodeRowSlices>(call, op, problem, operands, sum_args(room_A.template as<float>(), slices, n, stride_A, columns, v0 > 0));
             }
         } else if (need_A) {
             S* to = v0 == 0 ? room_A.as<S>() : room_more.as<S>();
@@ -539,7 +540,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
                                                  static_cast<int>(v1 - v0), static_cast<int>(v0), static_cast<float>(scale), static_cast<const float*>(grad_loss.data),
                                                  static_cast<const float*>(grad_log_sum.data), static_cast<const float*>(log_sum.data), pieces.rows};
                 const TileOperand w{static_cast<float*>(pieces.W.data) + v0 * pieces.W.stride[0], 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
-                launch_split<false, GradientStore32, DecodeTable>(call, op, pieces.problem(v1 - v0), operands, args);
+                launch_split<false, GradientStore32, DecodeRows>(call, op, pieces.problem(v1 - v0), operands, args);
                 multiply(v0, v1, dx);
                 MOPS_CUDA_OK(cudaGetLastError());
             }

@@ -47,7 +47,7 @@ template <int kColumns> struct LossStore {
     __device__ LossStore(const Args& a, uint32_t, int lane) : a(a), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) {
         row = r + lane, here = h, column = piece.column;
-        target = lane < here ? a.target[row] : -1;
+        target = lane < here && piece.group >= 0 ? a.target[row] : -1;
     }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
         const int first = column + part * kOwn, wide = min(a.columns - first, kOwn);
@@ -120,7 +120,7 @@ template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
         : a(a), out{a.map, a.out, a.stride, a.columns, false}, rest{a.map_rest, a.rest, a.stride, a.columns, false}, staging(staging), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) {
         row = r, here = h, column = piece.column;
-        if (lane < here) {
+        if (lane < here && piece.group >= 0) {
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(a.factors + row + lane));
             f = RowFactors{__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), static_cast<int32_t>(v.w) - a.first_column};
         }
@@ -330,7 +330,8 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
         auto launch = [&](auto width, auto paired) {
             using E = LossStore<decltype(width)::value>;
             const typename E::Args args{sums, parts, at_target, gather ? rows.target : targets, static_cast<int>(vocabulary), scale, scale2};
-            launch_tiles<decltype(type)::value, false, decltype(width)::value, decltype(paired)::value, E, DecodeTable>(call, op, problem, operands, args);
+            if (gather) launch_tiles<decltype(type)::value, false, decltype(width)::value, decltype(paired)::value, E, DecodeRows>(call, op, problem, operands, args);
+            else launch_tiles<decltype(type)::value, false, decltype(width)::value, decltype(paired)::value, E, DecodeTable>(call, op, problem, operands, args);
             note_kernel_f("loss_rows_mma<%s,%d,%s>", type ? "bf16" : "f16", static_cast<int>(width), paired ? "pair" : "block");
         };
         if (narrow_tiles) launch(integral_constant<int, 128>(), std::false_type());
@@ -397,8 +398,8 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
                 args.scale2 = scale2, args.factors = factors;
                 const TileProblem problem{first, rows.offsets, 1, n, columns, here};
                 const TileOperand operands[2] = {{w, 1, W.stride[0], 0}, {w, 1, W.stride[0], 0}};
-                if (n <= kTileRows) launch_tiles<BF16, false, 256, false, E, DecodeTable>(call, op, problem, operands, args);
-                else launch_tiles<BF16, false, 256, true, E, DecodeTable>(call, op, problem, operands, args);
+                if (n <= kTileRows) launch_tiles<BF16, false, 256, false, E, DecodeRows>(call, op, problem, operands, args);
+                else launch_tiles<BF16, false, 256, true, E, DecodeRows>(call, op, problem, operands, args);
             };
             if (twice) launch(std::true_type());
             else launch(std::false_type());
@@ -409,7 +410,7 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
                 typename Sums::Args to{};
                 to.map = tensor_map(MOPS_B200_F32, sums, columns, all, slices, stride, all * stride, 32);
                 to.out = sums, to.rows = all, to.stride = stride, to.columns = static_cast<int>(columns), to.add = v0 > 0;
-                launch_tiles<BF16, true, 256, true, Sums, DecodeSlices>(call, op, sum_problem, by_rows, to);
+                launch_tiles<BF16, true, 256, true, Sums, DecodeRowSlices>(call, op, sum_problem, by_rows, to);
             }
         });
         MOPS_CUDA_OK(cudaGetLastError());

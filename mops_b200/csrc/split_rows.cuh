@@ -23,23 +23,6 @@ struct SplitOperands {
     int64_t x_stride, group_stride, depth_stride, column_stride; // of m the last three
 };
 
-// Tiles of groups' rows, each with the depth cut into slices of `slice_steps` stages: a piece's first stage is in p.slot, its slice in p.row.
-template <int kRows, int kColumns> struct DecodeRowSlices {
-    DecodeRows<kRows, kColumns> rows;
-    int slices, slice_steps, all_steps;
-    __device__ DecodeRowSlices(const int32_t* offsets, int64_t groups, int64_t rows, int64_t columns, int steps, int slices, int lane)
-        : rows(offsets, groups, rows, columns, steps, lane), slices(slices), slice_steps((steps + slices - 1) / slices), all_steps(steps) {}
-    __device__ bool operator()(int64_t want, Piece& p) {
-        const int64_t tile = want / slices;
-        const int slice = static_cast<int>(want - tile * slices);
-        if (!rows(tile, p)) return false;
-        p.slot = min(slice * slice_steps, all_steps), p.row = slice;
-        if (p.group >= 0) p.steps = min(slice_steps, all_steps - static_cast<int>(p.slot));
-        return true;
-    }
-};
-template <template <int, int> class Decode> constexpr bool kRowSlices = std::is_same<Decode<1, 1>, DecodeRowSlices<1, 1>>::value;
-
 template <bool M_MN, typename E, template <int, int> class Decode>
 __global__ void __launch_bounds__(split::kThreads, 1)
 split_rows(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_m0, const __grid_constant__ CUtensorMap map_m1,
@@ -47,14 +30,14 @@ split_rows(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
            int depth, int columns, int slices, Status st) {
     extern __shared__ unsigned char raw[];
     using namespace split;
-    constexpr bool kSliced = kRowSlices<Decode> || std::is_same<Decode<1, 1>, DecodeSlices<1, 1>>::value;
+    constexpr bool kSliced = kRowSlices<Decode>;
     using W = Work<false, M_MN, kSplitColumns>;
     using L = typename W::L;
     constexpr int kTile = E::kHalves ? kSplitColumns / 2 : kSplitColumns; // columns of the result
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
-    if constexpr (!kOneGroup<Decode> || kRowSlices<Decode>)
+    if constexpr (!kOneGroup<Decode>)
         if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
 
     W work{block};
@@ -103,7 +86,7 @@ split_rows(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
         } else if (warp == kPieceWarp) {
             const int steps = (depth + kDepth - 1) / kDepth;
             if constexpr (kRowSlices<Decode>) hand_out(block, 0, lane, Decode<kTileRows, kTile>(offsets, groups, rows, columns, steps, slices, lane));
-            else hand_out(block, 0, lane, Decode<kTileRows, kTile>(offsets, kSliced ? slices : groups, rows, columns, steps, lane));
+            else hand_out(block, 0, lane, Decode<kTileRows, kTile>(offsets, groups, rows, columns, steps, lane));
         } else if (warp == kCopyWarp) {
             while (ok && supply.next(piece, lane)) {
                 if (lane == 0)
@@ -259,7 +242,7 @@ void launch_split(const Call& call, const std::string& op, const TileProblem& p,
     const CUtensorMap m0 = map_of(b[0]), m1 = E::kHalves ? map_of(b[1]) : m0;
     const SplitOperands from{static_cast<const float*>(p.A.data), {static_cast<const float*>(b[0].data), static_cast<const float*>(b[1].data)}, p.A.stride[0],
                              b[0].group_stride, b[0].depth_stride, b[0].column_stride};
-    const int64_t tiles = (kOneGroup<Decode> && !kRowSlices<Decode> ? ceil_div(p.rows, kTileRows) : most_row_tiles(p.rows, p.groups, kTileRows)) * ceil_div(p.columns, kTile) *
+    const int64_t tiles = (kOneGroup<Decode> ? ceil_div(p.rows, kTileRows) : most_row_tiles(p.rows, p.groups, kTileRows)) * ceil_div(p.columns, kTile) *
                           p.slices;
     auto kernel = split_rows<M_MN, E, Decode>;
     check_registers(reinterpret_cast<const void*>(kernel), op);
