@@ -318,7 +318,7 @@ MOPS_EXPORT int mops_b200_cuda_linear_cross_entropy_vjp(
  * arrays is, else f32. The squares are f32 products (f64 for f64), their sums f64 beyond a few hundred of them. */
 MOPS_EXPORT int mops_b200_cuda_gradient_norm(mops_b200_array_t norm, const mops_b200_array_t* gradients, int64_t n);
 /* outputs[i] = gradients[i] * max_norm / norm where norm > max_norm (>= 0), else gradients[i]; so they are where the norm is not finite. An output
- * has the type and size of its gradient, and may be that gradient (which is then written only where it changes); other than that no two of the arrays overlap. */
+ * has the type and size of its gradient, and may be that gradient (which is then written only where it changes); other than that no two of the arrays overlap, nor do they the norm. */
 MOPS_EXPORT int mops_b200_cuda_clip_gradient_norm(mops_b200_array_t norm, const mops_b200_array_t* outputs,
                                                   const mops_b200_array_t* gradients, int64_t n, double max_norm);
 

@@ -581,9 +581,19 @@ void linear_cross_entropy(Array loss, Array log_sum, Array A, Array W, Array tar
     check_loss(A, W, targets, loss, log_sum, scale, op);
     if (A.shape[0] == 0) return;
     Call call = begin_call();
-    if (sixteen_bits(A)) loss_forward_mma(call, {A, W, targets, scale, ignore_index}, loss, log_sum, op);
-    else if (A.type == MOPS_B200_F64) loss_forward<double>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
-    else loss_forward<float>(call, loss, log_sum, A, W, targets, scale, ignore_index, op);
+    // Rows some at a time: the sums of their parts, one for each 64 columns at the most, shall not take more than 2 GB.
+    const int64_t most = std::max<int64_t>((int64_t(1) << 31) / (ceil_div(W.shape[0], 64) * 16), 1024), n = A.shape[0];
+    for (int64_t r = 0; r < n; r += most) {
+        auto rows = [&](const Array& a) {
+            Array part = a;
+            part.data = static_cast<unsigned char*>(a.data) + r * a.stride[0] * type_bytes(a.type);
+            part.shape[0] = std::min(most, n - r);
+            return part;
+        };
+        if (sixteen_bits(A)) loss_forward_mma(call, {rows(A), W, rows(targets), scale, ignore_index}, rows(loss), rows(log_sum), op);
+        else if (A.type == MOPS_B200_F64) loss_forward<double>(call, rows(loss), rows(log_sum), rows(A), W, rows(targets), scale, ignore_index, op);
+        else loss_forward<float>(call, rows(loss), rows(log_sum), rows(A), W, rows(targets), scale, ignore_index, op);
+    }
     end_call(call, op.c_str(), kIndexNames, 1);
 }
 

@@ -207,19 +207,27 @@ Tensors check_tensors(Array& norm, const Array* outputs, const Array* gradients,
     }
     check_array(norm, "norm", 1, wide ? MOPS_B200_F64 : MOPS_B200_F32, op);
     if (norm.shape[0] != 1) throw std::runtime_error("norm must have one value in " + op);
-    // no two of them overlap, but an output and its gradient where they are the same
-    std::vector<std::pair<uintptr_t, uintptr_t>> places;
+    // no two of them overlap, but an output and its gradient where they are the same (and gradients of which only the norm is asked for)
+    using Place = std::pair<uintptr_t, uintptr_t>;
+    auto place = [](const void* p, int64_t bytes) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+        return Place{from, from + static_cast<uintptr_t>(bytes)};
+    };
+    const Place result = place(norm.data, type_bytes(norm.type));
+    std::vector<Place> places;
     places.reserve(2 * t.entries.size());
     for (const Entry& e : t.entries) {
-        const uintptr_t from = reinterpret_cast<uintptr_t>(e.from), to = reinterpret_cast<uintptr_t>(e.to), bytes = static_cast<uintptr_t>(e.values * type_bytes(e.type));
-        places.push_back({from, from + bytes});
-        if (outputs != nullptr && to != from) places.push_back({to, to + bytes});
+        const int64_t bytes = e.values * type_bytes(e.type);
+        places.push_back(place(e.from, bytes));
+        if (outputs != nullptr && e.to != e.from) places.push_back(place(e.to, bytes));
     }
+    bool apart = true;
+    for (const Place& p : places) apart = apart && (p.second <= result.first || result.second <= p.first);
     if (outputs != nullptr) {
         std::sort(places.begin(), places.end());
-        for (size_t i = 1; i < places.size(); i++)
-            if (places[i].first < places[i - 1].second) throw std::runtime_error("gradients and outputs overlap in " + op);
+        for (size_t i = 1; i < places.size(); i++) apart = apart && places[i - 1].second <= places[i].first;
     }
+    if (!apart) throw std::runtime_error("gradients and " + std::string(outputs != nullptr ? "outputs" : "norm") + " overlap in " + op);
     return t;
 }
 

@@ -190,18 +190,20 @@ def test_entry_points_refuse_wrong_arrays(name, arguments, message):
 
 
 @pytest.mark.parametrize("norm,outputs,gradients,max_norm,message", [
-    (_array((1,), "float64"), None, [_array((5,))], 1.0, "Expected norm to be of type float32"),
-    (_array((1,)), None, [_array((5,)), _array((5,), "float64")], 1.0, "Expected norm to be of type float64"),
-    (_array((2,)), None, [_array((5,))], 1.0, "norm must have one value"),
-    (_array((1,)), None, [_array((5,), "int32")], 1.0, "Wrong dtype for a gradient"),
-    (_array((1,)), None, [_array((5, 4), stride=(8, 1))], 1.0, "a gradient must be contiguous"),
-    (_array((1,)), [_array((4,), data=0x2000)], [_array((5,))], 1.0, "the sizes of its gradient along dimension 0 and an output"),
-    (_array((1,)), [_array((5,), "bfloat16", data=0x2000)], [_array((5,))], 1.0, "Expected an output to be of type float32"),
-    (_array((1,)), [_array((5,))], [_array((5,))], -1.0, "max_norm must not be negative"),
-    (_array((1,)), [_array((5,))], [_array((5,))], float("nan"), "max_norm must not be negative"),
-    (_array((1,)), [_array((5,))] * 2, [_array((5,))] * 2, 1.0, "gradients and outputs overlap"),
-    (_array((1,)), [_array((5,), data=0x1004)], [_array((5,))], 1.0, "gradients and outputs overlap"),
-    (_array((1,)), [_array((5,)), _array((5,), data=0x1010)], [_array((5,)), _array((5,), data=0x1010)], 1.0, "gradients and outputs overlap"),
+    (_array((1,), "float64", data=0x8000), None, [_array((5,))], 1.0, "Expected norm to be of type float32"),
+    (_array((1,), data=0x8000), None, [_array((5,)), _array((5,), "float64")], 1.0, "Expected norm to be of type float64"),
+    (_array((2,), data=0x8000), None, [_array((5,))], 1.0, "norm must have one value"),
+    (_array((1,), data=0x8000), None, [_array((5,), "int32")], 1.0, "Wrong dtype for a gradient"),
+    (_array((1,), data=0x8000), None, [_array((5, 4), stride=(8, 1))], 1.0, "a gradient must be contiguous"),
+    (_array((1,), data=0x8000), [_array((4,), data=0x2000)], [_array((5,))], 1.0, "the sizes of its gradient along dimension 0 and an output"),
+    (_array((1,), data=0x8000), [_array((5,), "bfloat16", data=0x2000)], [_array((5,))], 1.0, "Expected an output to be of type float32"),
+    (_array((1,), data=0x8000), [_array((5,))], [_array((5,))], -1.0, "max_norm must not be negative"),
+    (_array((1,), data=0x8000), [_array((5,))], [_array((5,))], float("nan"), "max_norm must not be negative"),
+    (_array((1,), data=0x8000), [_array((5,))] * 2, [_array((5,))] * 2, 1.0, "gradients and outputs overlap"),
+    (_array((1,), data=0x8000), [_array((5,), data=0x1004)], [_array((5,))], 1.0, "gradients and outputs overlap"),
+    (_array((1,), data=0x2010), [_array((5,), data=0x2000)], [_array((5,))], 1.0, "gradients and outputs overlap"),
+    (_array((1,), data=0x100c), None, [_array((5,))], 1.0, "gradients and norm overlap"),
+    (_array((1,), data=0x8000), [_array((5,)), _array((5,), data=0x1010)], [_array((5,)), _array((5,), data=0x1010)], 1.0, "gradients and outputs overlap"),
 ])
 def test_norm_refuses_wrong_arrays(norm, outputs, gradients, max_norm, message):
     from mops_b200 import _lib
@@ -337,6 +339,28 @@ def test_gated_rows_of_no_group_and_empty_sizes(dtype, N):
 
 
 @pytest.mark.gpu
+def test_operators_refuse_what_does_not_fit():
+    A, o = normal((70, 16), torch.bfloat16, 1), offsets_of([70])
+    with pytest.raises(RuntimeError, match="an even number in all, in cuda_grouped_gated_product"):
+        mt.grouped_gated_product(A, normal((1, 16, 7), torch.bfloat16, 2), o)
+    with pytest.raises(RuntimeError, match="the sizes of W along dimension 1 and A along dimension 1 must match"):
+        mt.grouped_gated_product(A, normal((1, 24, 8), torch.bfloat16, 2), o)
+    with pytest.raises(RuntimeError, match="and offsets along dimension 0 must match"):
+        mt.grouped_gated_product(A, normal((2, 16, 8), torch.bfloat16, 2), o)
+    T, t = normal((9, 16), torch.bfloat16, 3), some_targets(70, 9, 1.0)
+    with pytest.raises(RuntimeError, match="scale must be positive"):
+        mt.linear_cross_entropy(A, T, t, -1.0)
+    with pytest.raises(RuntimeError, match="W must have a row"):
+        mt.linear_cross_entropy(A, T[:0], t)
+    with pytest.raises(RuntimeError, match="the sizes of targets along dimension 0|and targets along dimension 0 must match"):
+        mt.linear_cross_entropy(A, T, t[:-1])
+    with pytest.raises(ValueError, match="All tensors must be on the same device"):
+        mt.linear_cross_entropy(A, T, t.cpu())
+    with pytest.raises(ValueError, match="All tensors must be on the same device"):
+        mt.clip_gradient_norm([A, T.cpu()], 1.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_gated_reports_wrong_offsets(dtype):
     for R in (20, 300):
@@ -445,7 +469,7 @@ def some_targets(R, V, kept, seed=5, ignored=-1):
 @pytest.mark.parametrize("R,V,C,kept", [
     (1, 1, 1, 1.0), (1, 2, 8, 1.0), (2, 5, 3, 1.0), (1, 5000, 64, 1.0), (3, 257, 40, 0.5), (8, 1000, 1030, 1.0), (31, 4097, 72, 0.8), (64, 63, 16, 1.0),
     (130, 300, 64, 0.9), (257, 1000, 129, 0.5), (300, 8200, 96, 0.95), (400, 129, 256, 0.7), (700, 5003, 203, 0.3), (1025, 2, 40, 0.9),
-    (2000, 77, 520, 1.0), (513, 12345, 8, 0.9), (2049, 3000, 64, 0.9), (4100, 511, 72, 0.4), (300, 70001, 24, 0.9), (3000, 50001, 16, 0.9), (300, 100, 1, 1.0), (5000, 600, 136, 0.02), (385, 3000, 700, 0.99)])
+    (2000, 77, 520, 1.0), (513, 12345, 8, 0.9), (2049, 3000, 64, 0.9), (4100, 511, 72, 0.4), (300, 70001, 24, 0.9), (3000, 50001, 16, 0.9), (70000, 40, 8, 0.6), (9000, 3, 24, 0.5), (300, 100, 1, 1.0), (5000, 600, 136, 0.02), (385, 3000, 700, 0.99)])
 def test_loss_matches_64_bits(dtype, R, V, C, kept):
     A, W = normal((R, C), dtype, 1, 2.0), normal((V, C), dtype, 2, C ** -0.5)
     check_loss(A, W, some_targets(R, V, kept), 1.25)
@@ -513,6 +537,19 @@ def test_loss_on_strided_and_shifted_tensors(dtype, R):
                           (A[:, ::2], W[:400, ::2], t[:R]), (A[:1, :128].expand(R, 128), W[:400, :128], t[:R]),
                           (A[:, :128].T.contiguous().T, W[:400, :128].T.contiguous().T, t[:R]), (A[:, :128], W[:1, :128].expand(400, 128), t[:R])):
         check_loss(a.detach(), w.detach(), targets)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_of_many_rows_is_that_of_each(dtype):
+    """So many rows that they are taken in turns: each has the loss that it has among a few."""
+    R, V, C = 70000, 150001, 8
+    A, W, t = normal((R, C), dtype, 1), normal((V, C), dtype, 2, 0.3), some_targets(R, V, 0.9)
+    loss, log_sum = mt.linear_cross_entropy(A, W, t)
+    for rows in (slice(0, 40), slice(56000, 57600), slice(R - 300, R)):
+        values, errors = loss_plain(A[rows], W, t[rows], 1.0, -1, *(torch.ones(R, device="cuda")[rows] for _ in range(2)))
+        within(loss[rows], values[0], errors[0], "loss")
+        within(log_sum[rows], values[1], errors[1], "log_sum")
 
 
 @pytest.mark.gpu
