@@ -53,6 +53,21 @@ template <typename To> Array converted(const Call& call, const Array& a, To* to,
     return r;
 }
 
+// Launches a kernel that begins with after_others(), where it waits for what is in front of it on the stream: its blocks are in place when that is done.
+template <typename... P, typename... A> void launch_early(const Call& call, void (*kernel)(P...), dim3 grid, dim3 block, const A&... arguments) {
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.stream = call.stream;
+    MOPS_CUDA_OK(cudaLaunchKernelEx(&config, kernel, P(arguments)...));
+}
+__device__ __forceinline__ void after_others() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 inline int64_t values_of(const Array& a) {
     int64_t n = 1;
     for (int d = 0; d < a.dimensions; d++) n *= a.shape[d];

@@ -285,11 +285,11 @@ template <typename F> void choose_tiles(const Call& call, const GatedProblem& p,
     auto by_width = [&](auto type, auto major, auto activation) {
         using std::integral_constant;
         const int64_t across = ceil_div(p.columns, 128);
-        // (see grouped_mma.cu: half a tile of each group is rows that are not there; a pair takes some 0.8 of the time of two blocks)
+        // (half a tile of each group is rows that are not there; a pair takes some 0.9 of the time of two blocks: 8192 rows of 16 groups, 2048 x 1280: six rounds of pairs 87 us, five of blocks 80)
         const int64_t of_blocks = ceil_div((2 * p.rows / kTileRows + p.groups) * across, 2 * sms);
         const int64_t of_pairs = ceil_div((p.rows / kTileRows + p.groups) * across, sms);
         if (p.columns > 64 && most_row_tiles(p.rows, p.groups, kTileRows) * across >= sms) {
-            if (4 * of_pairs <= 5 * of_blocks - 1) f(type, major, activation, integral_constant<int, 256>(), std::true_type());
+            if (10 * of_blocks >= 9 * of_pairs) f(type, major, activation, integral_constant<int, 256>(), std::true_type());
             else f(type, major, activation, integral_constant<int, 256>(), std::false_type());
         } else {
             f(type, major, activation, integral_constant<int, 128>(), std::false_type());

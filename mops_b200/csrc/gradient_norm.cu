@@ -147,6 +147,7 @@ __device__ __forceinline__ void write_norm(void* to, bool wide, double norm) {
 
 __global__ void __launch_bounds__(kThreads)
 join_norm(void* __restrict__ norm, bool wide, const double* __restrict__ sums, int n) {
+    after_others();
     const double value = join_sums(sums, n);
     if (threadIdx.x == 0) write_norm(norm, wide, value);
 }
@@ -154,6 +155,7 @@ join_norm(void* __restrict__ norm, bool wide, const double* __restrict__ sums, i
 template <int kMost>
 __global__ void __launch_bounds__(kThreads, kScaleBlocks)
 scale_values(void* norm, bool wide, const double* __restrict__ sums, int n, double max_norm, const __grid_constant__ Table<kMost> table) {
+    after_others();
     const double value = join_sums(sums, n);
     if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) write_norm(norm, wide, value);
     const double factor = isfinite(value) && value > max_norm ? max_norm / value : 1.0;
@@ -275,11 +277,11 @@ void norm_of(Array norm, const Array* outputs, const Array* gradients, int64_t n
     if (outputs != nullptr)
         for_tables(t, most, [&](const auto& table, auto most_tensors) {
             const int64_t blocks = std::min(table.chunks, most_scaling);
-            scale_values<decltype(most_tensors)::value><<<static_cast<unsigned>(blocks), kThreads, 0, call.stream>>>(
-                written ? nullptr : norm.data, wide, sums, static_cast<int>(parts), max_norm, table);
+            launch_early(call, scale_values<decltype(most_tensors)::value>, static_cast<unsigned>(blocks), kThreads, written ? nullptr : norm.data, wide, sums,
+                         static_cast<int>(parts), max_norm, table);
             written = true;
         });
-    if (!written) join_norm<<<1, kThreads, 0, call.stream>>>(norm.data, wide, sums, static_cast<int>(parts));
+    if (!written) launch_early(call, join_norm, 1, kThreads, norm.data, wide, sums, static_cast<int>(parts));
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("sum_squares, %d tensors", static_cast<int>(t.entries.size()));
     end_call(call, op.c_str(), nullptr, 0);

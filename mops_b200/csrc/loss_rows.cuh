@@ -40,6 +40,7 @@ template <typename S>
 static __global__ void __launch_bounds__(kJoinThreads)
 loss_join(S* __restrict__ loss, S* __restrict__ log_sum, const PartSum<S>* __restrict__ parts, int64_t n, int64_t all_rows, const S* __restrict__ at_target,
           const LossRows rows, const int32_t* __restrict__ targets, int64_t vocabulary, int64_t ignored, Status st) {
+    after_others();
     const int lane = threadIdx.x & 31;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + threadIdx.x / 32;
     if (i >= all_rows) return;
@@ -88,10 +89,8 @@ template <typename S>
 void join_rows(const Call& call, const Array& loss, const Array& log_sum, const PartSum<S>* parts, int64_t n, const S* at_target, const LossRows& rows, const Array& targets,
                int64_t vocabulary, int64_t ignored) {
     const int64_t all = targets.shape[0];
-    loss_join<S><<<static_cast<unsigned>(ceil_div(all, kJoinThreads / 32)), kJoinThreads, 0, call.stream>>>(
-        static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), parts, n, all, at_target, rows, static_cast<const int32_t*>(targets.data), vocabulary, ignored,
-        call.status);
-    MOPS_CUDA_OK(cudaGetLastError());
+    launch_early(call, loss_join<S>, static_cast<unsigned>(ceil_div(all, kJoinThreads / 32)), kJoinThreads, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), parts, n,
+                 all, at_target, rows, static_cast<const int32_t*>(targets.data), vocabulary, ignored, call.status);
 }
 
 inline LossRows take_rows(Scratch& room, int64_t rows) {
@@ -111,6 +110,7 @@ template <typename T>
 static __global__ void __launch_bounds__(kScatterThreads)
 scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int slices, int64_t stride, const LossRows rows, int64_t n, int columns, bool by_four,
              bool twice, const float* __restrict__ factor) {
+    after_others();
     const float f = factor != nullptr ? *factor : 1.f;
     const int quads = static_cast<int>(stride / 4);
     const int64_t copies = twice ? 2 : 1, slice = copies * n * stride;
@@ -153,8 +153,7 @@ void scatter_sums(const Call& call, T* grad_A, const float* sums, int64_t slices
     while (across < kScatterThreads && across * 4 < columns) across *= 2;
     const dim3 block(across, kScatterThreads / across);
     const unsigned down = static_cast<unsigned>(std::min<int64_t>(ceil_div(n, block.y), int64_t(sm_count(call.device)) * 32));
-    scatter_rows<T><<<down, block, 0, call.stream>>>(grad_A, sums, static_cast<int>(slices), stride, rows, n, static_cast<int>(columns), by_four, twice, factor);
-    MOPS_CUDA_OK(cudaGetLastError());
+    launch_early(call, scatter_rows<T>, down, block, grad_A, sums, static_cast<int>(slices), stride, rows, n, static_cast<int>(columns), by_four, twice, factor);
 }
 
 // Whether rows are numbered and gathered in front of a forward pass, which takes some 10 us: where all of them take 50 us or more (f32 takes eight times as long as 16 bits).
