@@ -14,7 +14,7 @@
 #include "grouped_mma.hpp"
 #include "loss_rows.cuh"
 #include "pack.hpp"
-#include "split_rows.cuh"
+#include "parts_rows.cuh"
 
 namespace mops_b200 {
 namespace {
@@ -226,9 +226,9 @@ loss_gradient(S* __restrict__ logits, int64_t columns, S scale, const S* __restr
 }
 
 // ---- f32, where the logits are summed: a lane has 64 of its row
-struct LossStore32 {
-    static constexpr bool kHalves = false;
-    static constexpr int kOwn = kSplitColumns / 2;
+template <int kOwn_> struct LossStoreOf {
+    static constexpr bool kHalves = false, kMend = true, kAllRows = false;
+    static constexpr int kOwn = kOwn_;
     struct Args {
         PartSum<float>* parts;
         int64_t n;
@@ -241,7 +241,7 @@ struct LossStore32 {
     int lane;
     int64_t row = 0;
     int here = 0, first = 0, target = -1;
-    __device__ LossStore32(const Args& a, uint32_t, int lane) : a(a), lane(lane) {}
+    __device__ LossStoreOf(const Args& a, uint32_t, int lane) : a(a), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
         row = r + lane, here = h, first = piece.column + half * kOwn;
         target = lane < here && piece.group >= 0 ? a.target[row] : -1;
@@ -275,6 +275,20 @@ struct LossStore32 {
     __device__ __forceinline__ void end() const {}
 };
 
+using LossStore32 = LossStoreOf<kSplitColumns / 2>;
+
+// What dx takes of a lane's row.
+struct RowGradient {
+    int target = -1; // in the piece
+    float base = 0, both = 0, of_loss = 0; // with the scale of the gradients
+    template <typename Args> __device__ __forceinline__ void load(const Args& a, int64_t i) {
+        const int64_t of = a.rows.order[i];
+        target = a.rows.target[i] - a.first_column;
+        const float l = a.grad_loss != nullptr ? a.grad_loss[of] : 0.f, m = a.grad_log_sum != nullptr ? a.grad_log_sum[of] : 0.f;
+        base = a.log_sum[of], both = (l + m) * a.scale, of_loss = l * a.scale;
+    }
+};
+
 struct GradientStore32 {
     static constexpr bool kHalves = false;
     static constexpr int kOwn = kSplitColumns / 2;
@@ -292,17 +306,12 @@ struct GradientStore32 {
     uint32_t staging;
     int lane;
     int64_t row = 0;
-    int here = 0, first = 0, target = -1;
-    float base = 0, both = 0, of_loss = 0; // with the scale of the gradients
+    int here = 0, first = 0;
+    RowGradient g;
     __device__ GradientStore32(const Args& a, uint32_t staging, int lane) : a(a), out{a.map, a.out, a.stride, a.columns, false}, staging(staging), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
         row = r, here = h, first = piece.column + half * kOwn;
-        if (lane < here && piece.group >= 0) { // (behind the last numbered row there are no numbers)
-            const int64_t of = a.rows.order[row + lane];
-            target = a.rows.target[row + lane] - a.first_column;
-            const float l = a.grad_loss != nullptr ? a.grad_loss[of] : 0.f, m = a.grad_log_sum != nullptr ? a.grad_log_sum[of] : 0.f;
-            base = a.log_sum[of], both = (l + m) * a.scale, of_loss = l * a.scale;
-        }
+        if (lane < here && piece.group >= 0) g.load(a, row + lane); // (behind the last numbered row there are no numbers)
     }
     __device__ __forceinline__ void store(const float (&sum)[kOwn]) const {
 #pragma unroll
@@ -310,14 +319,75 @@ struct GradientStore32 {
             if (first + c >= a.columns) return;
             float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = both * expf(fmaf(sum[c + j], a.scale, -base));
-            const int at = target - first - c;
+            for (int j = 0; j < 32; j++) v[j] = g.both * expf(fmaf(sum[c + j], a.scale, -g.base));
+            const int at = g.target - first - c;
             if (__any_sync(kFullMask, at >= 0 && at < 32)) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
-                    if (j == at) v[j] -= of_loss;
+                    if (j == at) v[j] -= g.of_loss;
             }
             out.put(v, staging, row, here, first + c, lane);
+        }
+    }
+    __device__ __forceinline__ void clear() const {}
+    __device__ __forceinline__ void end() const {
+        if (lane == 0) boxes_left<0>();
+    }
+};
+
+// dx in three parts, with zeros in the rows behind the last one up to the end of the tile: products over the rows take whole stages of 64.
+struct GradientParts {
+    static constexpr bool kHalves = false, kMend = true, kAllRows = true;
+    static constexpr int kOwn = kPartsOwn;
+    struct Args {
+        CUtensorMap map;
+        int columns, first_column; // of the piece
+        float scale;
+        const float *grad_loss, *grad_log_sum, *log_sum;
+        LossRows rows;
+    };
+    const Args& a;
+    uint32_t staging;
+    int lane;
+    int64_t row = 0;
+    int here = 0, first = 0;
+    RowGradient g;
+    __device__ GradientParts(const Args& a, uint32_t staging, int lane) : a(a), staging(staging), lane(lane) {}
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) {
+        row = r, here = h, first = piece.column + half * kOwn;
+        if (lane < here && piece.group >= 0) g.load(a, row + lane);
+    }
+    __device__ __forceinline__ void store(float (&sum)[kOwn]) const {
+#pragma unroll
+        for (int c = 0; c < kOwn; c += 64) {
+            if (first + c >= a.columns) return;
+            const int at = g.target - first - c;
+            const bool any = __any_sync(kFullMask, at >= 0 && at < 64);
+#pragma unroll
+            for (int j = 0; j < 64; j++) {
+                float v = g.both * expf(fmaf(sum[c + j], a.scale, -g.base));
+                if (any && j == at) v -= g.of_loss;
+                sum[c + j] = lane < here ? v : 0.f;
+            }
+#pragma unroll
+            for (int p = 0; p < kThreeParts; p++) {
+                if (lane == 0) boxes_left<0>();
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t x = __float_as_uint(sum[c + 8 * k + 2 * q]), y = __float_as_uint(sum[c + 8 * k + 2 * q + 1]);
+                        w[q] = split::cut_part(x, y);
+                        sum[c + 8 * k + 2 * q] = __uint_as_float(x), sum[c + 8 * k + 2 * q + 1] = __uint_as_float(y);
+                    }
+                    smem_store16(staging + lane * kBoxRow + ((k ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                }
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) box_out(a.map, first + c, static_cast<int>(row), p, staging);
+            }
         }
     }
     __device__ __forceinline__ void clear() const {}
@@ -370,6 +440,9 @@ unsigned blocks_for(const Call& call, int64_t n) {
     return static_cast<unsigned>(std::min<int64_t>(ceil_div(n, 256), int64_t(sm_count(call.device)) * 16));
 }
 
+// Whether operands are cut into parts beforehand.
+bool worth_cutting(int64_t rows, int64_t vocabulary, int64_t columns) { return rows >= 512 && vocabulary >= 512 && columns >= 64; }
+
 // What forward and backward share: the rows that count, gathered and as the products want them, W likewise, and the logits of a piece.
 template <typename S> struct Pieces {
     const Call& call;
@@ -381,10 +454,13 @@ template <typename S> struct Pieces {
     int64_t width, part; // columns of a piece, and of a part of it
     bool fused;          // worked on where they are summed
     bool numbered;       // rows without a target have been left out
+    bool in_parts;       // operands are cut beforehand
+    PartsArray parts_A{}, parts_W{};
+    Scratch room_parts_A, room_parts_W;
     static constexpr int32_t kType = sizeof(S) == 8 ? MOPS_B200_F64 : MOPS_B200_F32;
 
     Pieces(const Call& call, const std::string& op, const Array& a, const Array& w, bool forward)
-        : call(call), op(op), room_rows(call), room_A(call), room_W(call), room_logits(call), packing(call), W(w) {
+        : call(call), op(op), room_rows(call), room_A(call), room_W(call), room_logits(call), packing(call), W(w), room_parts_A(call), room_parts_W(call) {
         const int64_t n = a.shape[0], columns = a.shape[1];
         if (w.type != kType) {
             room_W.take(static_cast<size_t>(values_of(w)) * sizeof(S) + 16);
@@ -398,7 +474,8 @@ template <typename S> struct Pieces {
         // that copy in any case)
         fused = kType == MOPS_B200_F32 && columns > 0 &&
                 (!forward || !straight_rows(matrices(0, W.shape[0]), n, false) || boxable(kType, W.data, columns, W.shape[0], 1, W.stride[0], 0));
-        numbered = !forward || !fused || a.type != kType || worth_gathering(kType, n, W.shape[0], columns);
+        in_parts = fused && worth_cutting(n, W.shape[0], columns);
+        numbered = !forward || !fused || in_parts || a.type != kType || worth_gathering(kType, n, W.shape[0], columns);
         if (numbered) {
             rows = take_rows(room_rows, n);
             room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
@@ -418,11 +495,28 @@ template <typename S> struct Pieces {
                 static_cast<S*>(A.data), a.shape[1], static_cast<const From*>(a.data), a.stride[0], rows, a.shape[1]);
         });
         MOPS_CUDA_OK(cudaGetLastError());
-        if (fused) {
+        if (in_parts) {
+            if constexpr (sizeof(S) == 4) {
+                const int64_t outer = padded_rows(), wide = (W.shape[1] + 7) / 8 * 8;
+                room_parts_A.take(static_cast<size_t>(outer * wide) * 2 * kThreeParts);
+                room_parts_W.take(static_cast<size_t>(W.shape[0] * wide) * 2 * kThreeParts);
+                parts_A = cut(call, room_parts_A.as<void>(), static_cast<const float*>(A.data), A.stride[0], A.shape[0], outer, A.shape[1], nullptr, rows.offsets + 1);
+                parts_W = cut(call, room_parts_W.as<void>(), static_cast<const float*>(W.data), W.stride[0], W.shape[0], W.shape[0], W.shape[1], nullptr, nullptr);
+            }
+        } else if (fused) {
             packing.add(A);
             packing.add(W);
             packing.run();
         }
+    }
+    int64_t padded_rows() const { return ceil_div(A.shape[0], kPartsTile) * kPartsTile; }
+    SplitOperands operands(int64_t v0) const { // in f32
+        return {static_cast<const float*>(A.data), {static_cast<const float*>(W.data) + v0 * W.stride[0], nullptr}, A.stride[0], 0, 1, W.stride[0]};
+    }
+    PartsArray parts_of(int64_t v0, int64_t v1) const { // rows v0 .. v1 of W
+        PartsArray p = parts_W;
+        p.data = static_cast<uint16_t*>(p.data) + v0 * p.stride, p.outer = v1 - v0;
+        return p;
     }
     // The rows v0 .. v1 of W as the single group's matrix, C x (v1 - v0).
     Array matrices(int64_t v0, int64_t v1) const {
@@ -448,7 +542,7 @@ template <typename S>
 void loss_forward(const Call& call, const Array& loss, const Array& log_sum, const Array& A, const Array& W, const Array& targets, double scale,
                   int64_t ignored, const std::string& op) {
     Pieces<S> pieces(call, op, A, W, true);
-    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.fused ? LossStore32::kOwn : pieces.part);
+    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.in_parts ? kPartsOwn : pieces.fused ? LossStore32::kOwn : pieces.part);
     const int32_t* t = static_cast<const int32_t*>(targets.data);
     if (pieces.numbered) prepare_rows<S>(call, pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), targets, W.shape[0], ignored, nullptr, nullptr);
     pieces.gather(A);
@@ -456,7 +550,12 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
     PartSum<S>* sums = room.as<PartSum<S>>();
     S* at_target = reinterpret_cast<S*>(sums + n * parts);
     if constexpr (sizeof(S) == 4) {
-        if (pieces.fused) {
+        if (pieces.in_parts) {
+            using E = LossStoreOf<kPartsOwn>;
+            const E::Args args{sums, parts, at_target, pieces.rows.target, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
+            launch_parts<false, false, E, DecodeRows>(call, op, pieces.parts_A, pieces.parts_W, pieces.rows.offsets, n, W.shape[1], W.shape[0], 1, pieces.operands(0), args);
+            note_kernel("loss_rows_parts");
+        } else if (pieces.fused) {
             const LossStore32::Args args{sums, parts, at_target, pieces.numbered ? pieces.rows.target : t, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
             const TileOperand w{pieces.W.data, 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
             if (pieces.numbered) launch_split<false, LossStore32, DecodeRows>(call, op, pieces.problem(W.shape[0]), operands, args);
@@ -485,7 +584,10 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     Scratch room_A(call), room_more(call), room_W(call);
     const int64_t stride_A = pieces.fused ? (columns + 3) / 4 * 4 : columns; // of the sums for grad_A
     int64_t slices = 1;
-    if (pieces.fused && need_A) {
+    if (pieces.in_parts && need_A) {
+        slices = best_slices(ceil_div(n, kPartsTile) * ceil_div(columns, kPartsTile), sm_count(call.device) / 2, ceil_div(pieces.width, kBoxDepth), 2.5, 8,
+                             static_cast<double>(n) * columns * 8);
+    } else if (pieces.fused && need_A) {
         const int64_t deep = ceil_div(pieces.width, split::kDepth), tiles = ceil_div(n, kTileRows) * ceil_div(columns, kSplitColumns);
         slices = best_slices(tiles, sm_count(call.device), deep, 0.7, 16, static_cast<double>(n) * columns * 8);
     }
@@ -528,7 +630,36 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
         }
         packing.release();
     };
-    if (pieces.fused) {
+    if (pieces.in_parts) {
+        if constexpr (sizeof(S) == 4) {
+            const int64_t stride = (pieces.width + 7) / 8 * 8, outer = pieces.padded_rows();
+            Scratch room_dx(call, static_cast<size_t>(outer * stride) * 2 * kThreeParts), room_sums(call);
+            // the products with A: straight to where they belong, if that can be, and their depth need not be cut
+            const int64_t deep = ceil_div(n, kBoxDepth), tiles = ceil_div(pieces.width, kPartsTile) * ceil_div(columns, kPartsTile);
+            const int64_t cuts = best_slices(tiles, sm_count(call.device) / 2, deep, 2.5, 8, static_cast<double>(pieces.width) * columns * 8);
+            const bool straight = cuts == 1 && columns % 4 == 0 && reinterpret_cast<uintptr_t>(grad_W.data) % 16 == 0 && !widened;
+            if (need_W && !straight) room_sums.take(static_cast<size_t>(cuts * pieces.width * stride_A) * sizeof(float));
+            using Sums = SumStoreOf<kPartsOwn>;
+            for (int64_t v0 = 0; v0 < W.shape[0]; v0 += pieces.width) {
+                const int64_t v1 = std::min(v0 + pieces.width, W.shape[0]), here = v1 - v0;
+                const PartsArray dx{room_dx.as<void>(), here, outer, stride, outer * stride}, w = pieces.parts_of(v0, v1);
+                const GradientParts::Args args{dx.map(32), static_cast<int>(here), static_cast<int>(v0), static_cast<float>(scale), static_cast<const float*>(grad_loss.data),
+                                               static_cast<const float*>(grad_log_sum.data), static_cast<const float*>(log_sum.data), pieces.rows};
+                launch_parts<false, false, GradientParts, DecodeRows>(call, op, pieces.parts_A, w, pieces.rows.offsets, n, columns, here, 1, pieces.operands(v0), args);
+                if (need_A)
+                    launch_parts<false, true, Sums, DecodeRowSlices>(call, op, dx, w, pieces.rows.offsets, n, here, columns, slices, {},
+                                                                     sum_args<Sums>(room_A.template as<float>(), slices, n, stride_A, columns, v0 > 0));
+                if (need_W) {
+                    float* to = static_cast<float*>(grad_W.data) + v0 * columns;
+                    launch_parts<true, true, Sums, DecodeDepth>(call, op, dx, pieces.parts_A, pieces.rows.offsets, here, n, columns, cuts, {},
+                                                                sum_args<Sums>(straight ? to : room_sums.as<float>(), cuts, here, stride_A, columns, false));
+                    if (!straight) add_slices<<<blocks_for(call, here * stride_A / 4), 256, 0, call.stream>>>(to, room_sums.as<float>(), static_cast<int>(cuts), here, stride_A,
+                                                                                                         static_cast<int>(columns));
+                }
+                MOPS_CUDA_OK(cudaGetLastError());
+            }
+        }
+    } else if (pieces.fused) {
         if constexpr (sizeof(S) == 4) {
             pieces.take_logits();
             const int64_t stride = (pieces.width + 3) / 4 * 4;

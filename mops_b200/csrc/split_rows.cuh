@@ -143,9 +143,9 @@ struct BoxOut32 {
 };
 
 // Sums as they are, each slice of the depth in an array of its own; `add`: to what is there. Zeros for rows of no group.
-struct SumStore32 {
-    static constexpr bool kHalves = false;
-    static constexpr int kOwn = kSplitColumns / 2;
+template <int kOwn_> struct SumStoreOf {
+    static constexpr bool kHalves = false, kMend = false, kAllRows = false;
+    static constexpr int kOwn = kOwn_;
     struct Args {
         CUtensorMap map;
         float* out;
@@ -158,7 +158,7 @@ struct SumStore32 {
     int lane;
     int64_t row = 0;
     int here = 0, column = 0, slice = 0;
-    __device__ SumStore32(const Args& a, uint32_t staging, int lane) : a(a), staging(staging), lane(lane) {}
+    __device__ SumStoreOf(const Args& a, uint32_t staging, int lane) : a(a), staging(staging), lane(lane) {}
     __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int half) { row = r, here = h, column = piece.column + half * kOwn, slice = piece.row; }
     __device__ __forceinline__ void store(const float (&sum)[kOwn]) const {
 #pragma unroll
@@ -195,13 +195,14 @@ struct SumStore32 {
     }
     __device__ __forceinline__ void clear() const {
         for (int i = 0; i < here; i++)
-            for (int c = lane; c < kSplitColumns && column + c < a.columns; c += 32) a.out[(slice * a.rows + row + i) * a.stride + column + c] = 0.f;
+            for (int c = lane; c < 2 * kOwn && column + c < a.columns; c += 32) a.out[(slice * a.rows + row + i) * a.stride + column + c] = 0.f;
     }
     __device__ __forceinline__ void end() const {
         if (lane == 0) boxes_left<0>();
     }
 };
-inline SumStore32::Args sum_args(float* out, int64_t slices, int64_t rows, int64_t stride, int64_t columns, bool add) {
+using SumStore32 = SumStoreOf<kSplitColumns / 2>;
+template <typename E = SumStore32> typename E::Args sum_args(float* out, int64_t slices, int64_t rows, int64_t stride, int64_t columns, bool add) {
     return {tensor_map(MOPS_B200_F32, out, columns, rows, slices, stride, rows * stride, 32), out, rows, stride, static_cast<int>(columns), add};
 }
 
