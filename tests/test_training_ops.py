@@ -469,7 +469,8 @@ def some_targets(R, V, kept, seed=5, ignored=-1):
 @pytest.mark.parametrize("R,V,C,kept", [
     (1, 1, 1, 1.0), (1, 2, 8, 1.0), (2, 5, 3, 1.0), (1, 5000, 64, 1.0), (3, 257, 40, 0.5), (8, 1000, 1030, 1.0), (31, 4097, 72, 0.8), (64, 63, 16, 1.0),
     (130, 300, 64, 0.9), (257, 1000, 129, 0.5), (300, 8200, 96, 0.95), (400, 129, 256, 0.7), (700, 5003, 203, 0.3), (1025, 2, 40, 0.9),
-    (2000, 77, 520, 1.0), (513, 12345, 8, 0.9), (2049, 3000, 64, 0.9), (4100, 511, 72, 0.4), (300, 70001, 24, 0.9), (3000, 50001, 16, 0.9), (70000, 40, 8, 0.6), (9000, 3, 24, 0.5), (300, 100, 1, 1.0), (5000, 600, 136, 0.02), (385, 3000, 700, 0.99)])
+    (2000, 77, 520, 1.0), (513, 12345, 8, 0.9), (2049, 3000, 64, 0.9), (4100, 511, 72, 0.4), (300, 70001, 24, 0.9), (3000, 50001, 16, 0.9), (70000, 40, 8, 0.6), (9000, 3, 24, 0.5), (1100, 9001, 520, 0.8),
+    (4224, 8191, 130, 0.94), (770, 12000, 1030, 1.0), (300, 100, 1, 1.0), (5000, 600, 136, 0.02), (385, 3000, 700, 0.99)])
 def test_loss_matches_64_bits(dtype, R, V, C, kept):
     A, W = normal((R, C), dtype, 1, 2.0), normal((V, C), dtype, 2, C ** -0.5)
     check_loss(A, W, some_targets(R, V, kept), 1.25)
@@ -493,10 +494,9 @@ def test_loss_of_a_mean(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("R", [20, 400])
-def test_loss_rows_without_target(dtype, R):
+@pytest.mark.parametrize("R,V,C", [(20, 500, 72), (400, 500, 72), (1100, 9001, 520)])
+def test_loss_rows_without_target(dtype, R, V, C):
     """What stands in rows without a target does not matter; all rows may be without one."""
-    V, C = 500, 72
     A, W, targets = normal((R, C), dtype, 1), normal((V, C), dtype, 2, 0.1), some_targets(R, V, 0.5, ignored=499)
     A[targets == 499] = float("nan")
     got = check_loss(A, W, targets, ignored=499)
@@ -541,6 +541,14 @@ def test_loss_on_strided_and_shifted_tensors(dtype, R):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_of_many_logits_on_strided_tensors(dtype):
+    A, W, t = normal((900, 1300), dtype, 1), normal((9100, 1300), dtype, 2, 0.1), some_targets(900, 9000, 0.9)
+    for a, w in ((A[:, :516], W[:9000, 4:520]), (A[:, 3:523], W[100:9100, 5:525]), (A[:, ::2], W[:9000, ::2]), (A[:1, :512].expand(900, 512), W[:9000, :512])):
+        check_loss(a.detach(), w.detach(), t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_loss_of_many_rows_is_that_of_each(dtype):
     """So many rows that they are taken in turns: each has the loss that it has among a few."""
     R, V, C = 70000, 150001, 8
@@ -554,9 +562,8 @@ def test_loss_of_many_rows_is_that_of_each(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("R", [9, 300])
-def test_loss_of_large_and_infinite_logits(dtype, R):
-    V, C = 700, 16
+@pytest.mark.parametrize("R,V,C", [(9, 700, 16), (300, 700, 16), (600, 13001, 520)])
+def test_loss_of_large_and_infinite_logits(dtype, R, V, C):
     A, W = normal((R, C), dtype, 1, 100.0), normal((V, C), dtype, 2, 10.0)
     targets = some_targets(R, V, 1.0)
     check_loss(A, W, targets)  # most p are zero, some losses in the thousands
