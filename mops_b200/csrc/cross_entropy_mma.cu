@@ -30,7 +30,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // ------------------------------------------------------------------------------- forward
 template <int kColumns> struct LossStore {
-    static constexpr bool kHalves = false;
+    static constexpr bool kHalves = false, kAllRows = false;
     static constexpr int kStoreWarps = 8, kStaging = 0, kOwn = kColumns / 2;
     struct Args {
         PartSum<float>* parts; // row by row
@@ -99,7 +99,7 @@ struct alignas(16) RowFactors {
 };
 
 template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
-    static constexpr bool kHalves = false;
+    static constexpr bool kHalves = false, kAllRows = true; // (zeros behind the last row, up to the end of the tile: products over the rows take whole stages of 64)
     static constexpr int kStoreWarps = 8, kStaging = BoxOut::kBytes, kOwn = kColumns / 2;
     struct Args {
         CUtensorMap map, map_rest;
@@ -145,6 +145,10 @@ template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
                     for (int j = 0; j < 32; j++)
                         if (j == at) x[j] = f.at_target;
                 }
+                if (here < 32) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) x[j] = lane < here ? x[j] : 0.f;
+                }
                 auto packs = [&](uint4* to) {
 #pragma unroll
                     for (int j = 0; j < 4; j++)
@@ -159,8 +163,8 @@ template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
                     packs(w);
                 }
             }
-            out.put(v, staging, row, here, column + c, lane);
-            if constexpr (kTwoParts) rest.put(w, staging, row, here, column + c, lane);
+            out.put(v, staging, row, 32, column + c, lane); // (there is room up to the end of the tile)
+            if constexpr (kTwoParts) rest.put(w, staging, row, 32, column + c, lane);
         }
     }
     __device__ __forceinline__ void clear() const {}
@@ -172,7 +176,7 @@ template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
 // Sums in f32: of the first piece of the vocabulary they are written, those of others are added to what is there. Each slice of the depth has sums of its own, so that no two
 // blocks add to one place, and the order of the additions is that of the pieces.
 template <int kColumns> struct SumStore {
-    static constexpr bool kHalves = false;
+    static constexpr bool kHalves = false, kAllRows = false;
     static constexpr int kStoreWarps = 8, kStaging = 32 * kBoxRow, kOwn = kColumns / 2;
     struct Args {
         CUtensorMap map;
@@ -229,6 +233,55 @@ template <int kColumns> struct SumStore {
     }
 };
 
+// grad_W = factor dx^T A in 16 bits (DecodeDepth); zeros where there are no rows.
+template <bool BF16> struct ScaledStore {
+    static constexpr bool kHalves = false, kAllRows = false;
+    static constexpr int kStoreWarps = 8, kStaging = BoxOut::kBytes, kOwn = 128;
+    struct Args {
+        CUtensorMap map;
+        uint16_t* out;
+        int columns;
+        bool loose;
+        const float* factor;
+    };
+    BoxOut out;
+    uint32_t staging;
+    int lane;
+    float factor;
+    int64_t row = 0;
+    int here = 0, column = 0;
+    bool empty = false;
+    __device__ ScaledStore(const Args& a, uint32_t staging, int lane)
+        : out{a.map, a.out, a.columns, a.columns, a.loose}, staging(staging), lane(lane), factor(__ldg(a.factor)) {}
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) { row = r, here = h, column = piece.column, empty = piece.steps == 0; }
+    __device__ __forceinline__ void store(uint32_t accumulator, int part) {
+#pragma unroll 1
+        for (int c = part * kOwn; c < part * kOwn + kOwn; c += 64) {
+            if (column + c >= out.columns) return;
+            uint4 v[8];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t r[32];
+                tmem_load(accumulator + c + h * 32, r);
+                tmem_wait_load();
+                tmem_pin(r);
+                float x[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) x[j] = empty ? 0.f : __uint_as_float(r[j]) * factor;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    v[h * 4 + j] = make_uint4(pack_pair<BF16>(x[8 * j], x[8 * j + 1]), pack_pair<BF16>(x[8 * j + 2], x[8 * j + 3]),
+                                              pack_pair<BF16>(x[8 * j + 4], x[8 * j + 5]), pack_pair<BF16>(x[8 * j + 6], x[8 * j + 7]));
+            }
+            out.put(v, staging, row, here, column + c, lane);
+        }
+    }
+    __device__ __forceinline__ void clear() const {}
+    __device__ __forceinline__ void end() const {
+        if (lane == 0) boxes_left<0>();
+    }
+};
+
 // to[i,:] = from[order[i],:], or rows 2i and 2i + 1, a warp to a row; and what dx takes of the row, if that is asked for.
 struct FactorArgs {
     RowFactors* factors; // none: a forward pass
@@ -242,6 +295,11 @@ gather_rows(uint16_t* __restrict__ to, int64_t to_stride, const __half* __restri
             const FactorArgs f) {
     const int64_t kept = rows.offsets[1];
     const int lane = threadIdx.x & 31;
+    if (f.factors != nullptr) { // zeros behind the last row, up to a whole stage (there is room for them)
+        const int64_t packs = to_stride / 8, first = (twice ? 2 * kept : kept) * packs, last = ((twice ? 2 * kept : kept) + 63) / 64 * 64 * packs;
+        for (int64_t c = first + static_cast<int64_t>(blockIdx.x) * kGatherThreads + threadIdx.x; c < last; c += static_cast<int64_t>(gridDim.x) * kGatherThreads)
+            reinterpret_cast<uint4*>(to)[c] = make_uint4(0, 0, 0, 0);
+    }
     const float unit = f.factors != nullptr ? *rows.unit : 0.f;
     if (f.factors != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *f.factor = unit * f.scale / f.units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kGatherThreads / 32) + threadIdx.x / 32; i < kept; i += static_cast<int64_t>(gridDim.x) * (kGatherThreads / 32)) {
@@ -276,7 +334,7 @@ int64_t whole_packs(int64_t n) { return (n + 7) / 8 * 8; }
 // The kept rows of A, one after the other (or each twice), as the copy engine can fetch them.
 Array gathered(const Call& call, Scratch& room, const Array& A, const LossRows& rows, bool twice, const FactorArgs& factors) {
     const int64_t stride = whole_packs(A.shape[1]), copies = twice ? 2 : 1;
-    room.take(static_cast<size_t>(copies * A.shape[0] * stride) * 2);
+    room.take(static_cast<size_t>((copies * A.shape[0] + 63) / 64 * 64 * stride) * 2);
     Array to = contiguous(room.as<void>(), A.type, copies * A.shape[0], A.shape[1]);
     to.stride[0] = stride;
     const bool aligned = A.shape[1] % 8 == 0 && A.stride[0] % 8 == 0 && reinterpret_cast<uintptr_t>(A.data) % 16 == 0;
@@ -357,7 +415,7 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     float* factor = reinterpret_cast<float*>(factors + n);
     const float scale2 = static_cast<float>(p.scale * 1.4426950408889634);
     const bool twice = n <= kTwoPartsTo;
-    const int64_t copies = twice ? 2 : 1, all = copies * n; // rows of dx
+    const int64_t copies = twice ? 2 : 1, all = copies * n, whole = ceil_div(n, 2 * kTileRows) * 2 * kTileRows; // rows of dx, and rows up to the end of a tile
     const int32_t* all_rows = twice ? rows.doubled : rows.offsets;
     const Array A = gathered(call, room_A, p.A, rows, twice,
                              {factors, factor, of_loss, of_sum, static_cast<const float*>(loss.data), static_cast<const float*>(log_sum.data), static_cast<float>(p.scale),
@@ -373,7 +431,7 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     constexpr int64_t kMostValues = int64_t(1) << 28; // of dx
     const int64_t most = std::max<int64_t>(kMostValues / all / 256 * 256, 256), across = ceil_div(columns, 256), unit = sms / 2 / std::gcd<int64_t>(sms / 2, across) * 256;
     const int64_t width = std::min(unit <= most ? most / unit * unit : most, whole_packs(vocabulary)), pieces = ceil_div(vocabulary, width);
-    Scratch room_dx(call, static_cast<size_t>(all * width) * 2);
+    Scratch room_dx(call, static_cast<size_t>(copies * whole * width) * 2);
     // Slices of the piece for the products with W.
     const int64_t steps = ceil_div(std::min(width, vocabulary), kBoxDepth);
     const int64_t slices = best_slices(ceil_div(all, 2 * kTileRows) * ceil_div(columns, 256), sms / 2, steps, 0.42, 16, static_cast<double>(all) * columns * 8);
@@ -392,8 +450,8 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
                 using E = GradientStore<BF16, 256, decltype(parts)::value>;
                 typename E::Args args{};
                 args.out = static_cast<uint16_t*>(dx.data), args.rest = args.out + width, args.stride = copies * width;
-                args.map = tensor_map(A.type, args.out, here, n, 1, args.stride, 0, 32);
-                if (twice) args.map_rest = tensor_map(A.type, args.rest, here, n, 1, args.stride, 0, 32);
+                args.map = tensor_map(A.type, args.out, here, whole, 1, args.stride, 0, 32);
+                if (twice) args.map_rest = tensor_map(A.type, args.rest, here, whole, 1, args.stride, 0, 32);
                 args.columns = static_cast<int>(here), args.first_column = static_cast<int>(v0);
                 args.scale2 = scale2, args.factors = factors;
                 const TileProblem problem{first, rows.offsets, 1, n, columns, here};
@@ -414,7 +472,22 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
             }
         });
         MOPS_CUDA_OK(cudaGetLastError());
-        if (need_W)
+        uint16_t* const to_W = need_W ? static_cast<uint16_t*>(grad_W.data) + v0 * columns : nullptr;
+        // (whole tiles of the gradient, or rows cut into slices and joined. Where the tiles are more than half of the pairs, or rows few, the first: 16384 rows of 9000 x 512 118 us against 151, of
+        // 5000 x 512 108 and 114, of 2048 x 512 105 and 52; 1500 rows of 1000 x 256 16 and 18; 8192 rows of 26 112 x 1024 333 and 350)
+        if (need_W && (ceil_div(here, 2 * kTileRows) * across >= sms / 4 || all <= 2048)) {
+            for_sixteen(A.type, [&](auto type) {
+                using E = ScaledStore<decltype(type)::value>;
+                typename E::Args to{};
+                to.loose = columns % 8 != 0 || reinterpret_cast<uintptr_t>(to_W) % 16 != 0;
+                if (!to.loose) to.map = tensor_map(A.type, to_W, columns, here, 1, columns, 0, 32);
+                to.out = to_W, to.columns = static_cast<int>(columns), to.factor = factor;
+                // (the rows up to a whole stage are zeros)
+                const TileProblem outer{dx, all_rows, 1, here, (all + 63) / 64 * 64, columns};
+                const TileOperand a{A.data, A.stride[0], 1, 0}, operands[2] = {a, a};
+                launch_tiles<decltype(type)::value, true, 256, true, E, DecodeDepth>(call, op, outer, operands, to);
+            });
+        } else if (need_W)
             multiply_outer(call, {contiguous(static_cast<uint16_t*>(grad_W.data) + v0 * columns, A.type, 1, here, columns), dx, A, all_rows, 1, factor}, op);
     }
     if (need_A)

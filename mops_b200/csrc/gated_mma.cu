@@ -24,7 +24,7 @@ __device__ __forceinline__ void gate_values(const uint32_t (&u)[32], const uint3
 }
 
 template <bool BF16, int kActivation, int kColumns> struct GateStore {
-    static constexpr bool kHalves = true;
+    static constexpr bool kHalves = true, kAllRows = false;
     static constexpr int kStoreWarps = kColumns == 256 ? 8 : 4, kStaging = BoxOut::kBytes;
     struct Args {
         CUtensorMap map;
@@ -62,7 +62,7 @@ template <bool BF16, int kActivation, int kColumns> struct GateStore {
 };
 
 template <bool BF16, int kActivation, int kColumns> struct GateStoreVjp {
-    static constexpr bool kHalves = true;
+    static constexpr bool kHalves = true, kAllRows = false;
     static constexpr int kStoreWarps = kColumns == 256 ? 8 : 4, kStaging = BoxOut::kBytes;
     using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
     struct Args {

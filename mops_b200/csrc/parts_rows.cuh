@@ -1,6 +1,6 @@
 // Products of f32 on tensor cores whose operands have been cut into three bf16 parts beforehand (x = x0 + x1 + x2, by cutting bits off; grouped_split.cu says why six products of them and in what
 // order), as arrays of three slices. Cutting takes a pass over the operands, 10 bytes a value; in return nothing stands between the copies and the products, so that pairs of blocks can multiply: tiles of 256 x 256, of
-// whose stages of 64 values of depth each block takes 96 KB in and gives the tensor cores 192 KB in the 3072 clocks of their six products. As there, an accumulator takes a stage and is then added, rounded, to sums in
+// whose stages of 64 values of depth each block takes 96 KB in and gives the tensor cores 192 KB for six products. As there, an accumulator takes a stage and is then added, rounded, to sums in
 // registers. For a single group of rows, or the columns of outer products.
 //
 // E as in split_rows.cuh, with sums of 128 columns, of the tile's first half or its second. E::kAllRows: it stores also where the warp has no rows; E::kMend: sums that are NaN are computed again.
@@ -40,29 +40,6 @@ struct PartsLayout {
     };
     static_assert(sizeof(Rings) <= 512, "room for the rings");
 };
-
-// Tiles of height x columns whose depth is the rows that offsets[1] says, cut into slices: an outer product over the rows of a single group.
-template <int kRows, int kColumns> struct DecodeDepth {
-    int64_t row_tiles, column_tiles;
-    int slices, slice_steps, all_steps;
-    __device__ DecodeDepth(const int32_t* offsets, int64_t most_rows, int64_t height, int64_t columns, int, int slices, int)
-        : row_tiles((height + kRows - 1) / kRows), column_tiles((columns + kColumns - 1) / kColumns), slices(slices) {
-        all_steps = static_cast<int>((rows_between(0, __ldg(offsets + 1), most_rows).hi + kBoxDepth - 1) / kBoxDepth);
-        slice_steps = (all_steps + slices - 1) / slices;
-    }
-    __device__ bool operator()(int64_t want, Piece& p) const {
-        const int64_t tile = want / slices;
-        const int slice = static_cast<int>(want - tile * slices);
-        if (tile >= row_tiles * column_tiles) return false;
-        int64_t tile_row, tile_column;
-        banded(tile, row_tiles, column_tiles, tile_row, tile_column);
-        p.lo = tile_row * kRows, p.hi = INT32_MAX, p.group = 0;
-        p.slot = min(slice * slice_steps, all_steps), p.row = slice, p.column = static_cast<int>(tile_column) * kColumns;
-        p.steps = min(slice_steps, all_steps - static_cast<int>(p.slot));
-        return true;
-    }
-};
-template <template <int, int> class Decode> constexpr bool kOfDepth = std::is_same<Decode<1, 1>, DecodeDepth<1, 1>>::value;
 
 // As Work::mend (split_block.cuh): sums that are NaN are replaced by what the ordinary units make of the f32 operands. terms: of the warp's first row and column.
 template <int kOwn> __device__ __noinline__ void mend_parts(float* sum, const split::Terms& all, int lane) {

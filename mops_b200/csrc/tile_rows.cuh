@@ -5,7 +5,7 @@
 // by warps of which two (or one) take the 32 rows of a quadrant, while the next tile is under way in the other half of tensor memory. The second operand may come in two halves (E::kHalves), each with
 // a map of its own: kColumns / 2 columns of either stand in an accumulator, so that a lane finds both of its values in its own row. Of a pair the first block fetches one and the second the other.
 //
-// E has: kHalves, kStoreWarps (4 or 8), kStaging (bytes of shared memory of each of them), Args (among the kernel's arguments), and
+// E has: kHalves, kAllRows (whether it stores also where the warp has no rows), kStoreWarps (4 or 8), kStaging (bytes of shared memory of each of them), Args (among the kernel's arguments), and
 //   E(args, staging, lane)                            what a storing warp keeps
 //   begin(piece, row, here, part)                     before the accumulator is there: what can be loaded (of rows of no group nothing: piece.group < 0). The warp's first row, how many it
 //                                                     has, and its part of the columns
@@ -204,8 +204,32 @@ template <int kRows, int kColumns> struct DecodeRowSlices {
 template <template <int, int> class Decode> constexpr bool kRowSlices = std::is_same<Decode<1, 1>, DecodeRowSlices<1, 1>>::value;
 template <template <int, int> class Decode> constexpr bool kOneGroup = std::is_same<Decode<1, 1>, DecodeTable<1, 1>>::value;
 
+// Tiles of height x columns whose depth is the rows that offsets[1] says, cut into slices: an outer product over the rows of a single group.
+template <int kRows, int kColumns> struct DecodeDepth {
+    int64_t row_tiles, column_tiles;
+    int slices, slice_steps, all_steps;
+    __device__ DecodeDepth(const int32_t* offsets, int64_t most_rows, int64_t height, int64_t columns, int, int slices, int)
+        : row_tiles((height + kRows - 1) / kRows), column_tiles((columns + kColumns - 1) / kColumns), slices(slices) {
+        all_steps = static_cast<int>((rows_between(0, __ldg(offsets + 1), most_rows).hi + kBoxDepth - 1) / kBoxDepth);
+        slice_steps = (all_steps + slices - 1) / slices;
+    }
+    __device__ bool operator()(int64_t want, Piece& p) const {
+        const int64_t tile = want / slices;
+        const int slice = static_cast<int>(want - tile * slices);
+        if (tile >= row_tiles * column_tiles) return false;
+        int64_t tile_row, tile_column;
+        banded(tile, row_tiles, column_tiles, tile_row, tile_column);
+        p.lo = tile_row * kRows, p.hi = INT32_MAX, p.group = 0;
+        p.slot = min(slice * slice_steps, all_steps), p.row = slice, p.column = static_cast<int>(tile_column) * kColumns;
+        p.steps = min(slice_steps, all_steps - static_cast<int>(p.slot));
+        return true;
+    }
+};
+template <template <int, int> class Decode> constexpr bool kOfDepth = std::is_same<Decode<1, 1>, DecodeDepth<1, 1>>::value;
+
 // a_bytes: of a box of the first operand, which may have fewer than 128 rows where there are no more (what stands in the others does not matter). B_MN: the columns of the second operand are
-// neighbours in memory, else its depth is. map_b1: its second half.
+// neighbours in memory, else its depth is. map_b1: its second half. rows, depth: of an outer product (DecodeDepth) the height, and the most rows there may be; the rows of both operands are the depth then,
+// and those behind the last one, up to a whole stage, are zeros.
 template <bool BF16, bool B_MN, int kColumns, bool kPair, typename E, template <int, int> class Decode>
 __global__ void __launch_bounds__(TileLayout<kColumns, kPair, E>::kThreads, 1)
 tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1, int a_bytes,
@@ -213,16 +237,18 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     extern __shared__ unsigned char raw[];
     using L = TileLayout<kColumns, kPair, E>;
     using H = Hands<L>;
+    constexpr bool A_MN = kOfDepth<Decode>, kSliced = kRowSlices<Decode> || kOfDepth<Decode>;
     const int rank = kPair ? static_cast<int>(pair_rank()) : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Block<L> block(raw, st);
     block.begin(warp);
-    if constexpr (!kOneGroup<Decode>)
+    if constexpr (!kOneGroup<Decode> && !kOfDepth<Decode>)
         if (blockIdx.x == 0) check_offsets(offsets, groups, rows, st);
     auto stage_at = [&](const Turn<L::kStages>& stage) { return block.base + static_cast<uint32_t>(stage.at) * L::kStage; };
     if (warp == kTilePieceWarp) {
         const int steps = (depth + kBoxDepth - 1) / kBoxDepth;
-        if constexpr (kRowSlices<Decode>) hand_out(block, rank, lane, Decode<L::kRows, L::kTileColumns>(offsets, groups, rows, columns, steps, slices, lane));
+        if constexpr (kOfDepth<Decode>) hand_out(block, rank, lane, Decode<L::kRows, L::kTileColumns>(offsets, depth, rows, columns, steps, slices, lane));
+        else if constexpr (kSliced) hand_out(block, rank, lane, Decode<L::kRows, L::kTileColumns>(offsets, groups, rows, columns, steps, slices, lane));
         else hand_out(block, rank, lane, Decode<L::kRows, L::kTileColumns>(offsets, groups, rows, columns, steps, lane));
     } else if (warp == 0) {
         Supply<L> supply{block};
@@ -237,9 +263,15 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     if (!ok) break;
                     uint64_t* full = &block.rings->stages.full[stage.at];
                     const uint32_t a = stage_at(stage), b = a + L::kA;
-                    const int deep = (kRowSlices<Decode> ? static_cast<int>(piece.slot) + s : s) * kBoxDepth;
+                    const int deep = (kSliced ? static_cast<int>(piece.slot) + s : s) * kBoxDepth;
                     H::expect(full, static_cast<uint32_t>(a_bytes) + L::kB);
-                    H::fetch(a, map_a, deep, row, 0, full);
+                    if constexpr (A_MN) {
+                        const int first = static_cast<int>(piece.lo) + rank * kTileRows; // (a multiple of 64 whatever the number of rows is)
+                        H::fetch(a, map_a, first, deep, 0, full);
+                        H::fetch(a + kBoxBytes, map_a, first + 64, deep, 0, full);
+                    } else {
+                        H::fetch(a, map_a, deep, row, 0, full);
+                    }
                     if constexpr (!E::kHalves) {
                         const int column = piece.column + rank * L::kOwnColumns;
                         if constexpr (B_MN) {
@@ -283,7 +315,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (Piece piece; supply.next(piece, lane);) {
             bool ok = true;
             if (lane == 0 && piece.group >= 0 && rank == 0) {
-                constexpr uint32_t instruction = instruction_descriptor(BF16, false, B_MN, kColumns, L::kRows);
+                constexpr uint32_t instruction = instruction_descriptor(BF16, A_MN, B_MN, kColumns, L::kRows);
                 ok = block.wait_empty(block.rings->accumulators, tile);
                 tmem_fence_after_sync();
                 for (int s = 0; s < piece.steps && ok; s++) {
@@ -293,7 +325,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     const uint64_t a = operand_descriptor(stage_at(stage), kBoxBytes), b = operand_descriptor(stage_at(stage) + L::kA, kBoxBytes);
 #pragma unroll
                     for (int k = 0; k < kBoxDepth / 16; k++)
-                        H::multiply(block.accumulator(tile), a + k * kDepthStep<false>, b + k * kDepthStep<B_MN>, instruction, s + k > 0);
+                        H::multiply(block.accumulator(tile), a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, instruction, s + k > 0);
                     H::multiplied(&block.rings->stages.empty[stage.at]);
                     stage.next();
                 }
@@ -309,7 +341,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         E work(args, block.base + L::kStagingAt + (warp - kFirstStoreWarp) * E::kStaging, lane);
         for (Piece piece; supply.next(piece, lane);) {
             const int64_t row = piece.lo + rank * kTileRows + quadrant * 32;
-            const int here = static_cast<int>(min(max(piece.hi - row, int64_t(0)), int64_t(32)));
+            const int here = static_cast<int>(min(max(min(piece.hi, kOfDepth<Decode> ? rows : piece.hi) - row, int64_t(0)), int64_t(32)));
             work.begin(piece, row, here, part);
             if (piece.group < 0) {
                 if (part == 0) work.clear();
@@ -317,7 +349,7 @@ tile_rows(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
             if (!__all_sync(kFullMask, block.wait_full(block.rings->accumulators, tile))) break;
             tmem_fence_after_sync();
-            if (here > 0) work.store(tmem_quadrant(block.accumulator(tile), quadrant), part);
+            if (here > 0 || E::kAllRows) work.store(tmem_quadrant(block.accumulator(tile), quadrant), part);
             tmem_fence_before_sync();
             __syncwarp();
             if (lane == 0) H::arrive(&block.rings->accumulators.empty[tile.at]);
@@ -362,15 +394,16 @@ void launch_tiles(const Call& call, const std::string& op, const TileProblem& p,
     using L = TileLayout<kColumns, kPair, E>;
     constexpr int32_t type = BF16 ? MOPS_B200_BF16 : MOPS_B200_F16;
     int box = kTileRows;
-    if (!kPair)
+    if (!kPair && !kOfDepth<Decode>)
         while (box > 16 && p.rows <= box / 2) box /= 2;
-    const CUtensorMap a = tensor_map(type, p.A.data, p.depth, p.rows, 1, p.A.stride[0], 0, box);
+    constexpr bool kDeep = kOfDepth<Decode>;
+    const CUtensorMap a = kDeep ? tensor_map(type, p.A.data, p.rows, p.depth, 1, p.A.stride[0], 0, 64) : tensor_map(type, p.A.data, p.depth, p.rows, 1, p.A.stride[0], 0, box);
     auto map_of = [&](const TileOperand& o) {
         return B_MN ? tensor_map(type, o.data, p.columns, p.depth, p.groups, o.depth_stride, o.group_stride, 64)
                     : tensor_map(type, o.data, p.depth, p.columns, p.groups, o.column_stride, o.group_stride, E::kHalves ? kColumns / 2 : L::kOwnColumns);
     };
     const CUtensorMap b0 = map_of(b[0]), b1 = E::kHalves ? map_of(b[1]) : b0;
-    const int64_t tiles = (kOneGroup<Decode> ? ceil_div(p.rows, L::kRows) : most_row_tiles(p.rows, p.groups, L::kRows)) * ceil_div(p.columns, L::kTileColumns) * p.slices;
+    const int64_t tiles = (kOneGroup<Decode> || kDeep ? ceil_div(p.rows, L::kRows) : most_row_tiles(p.rows, p.groups, L::kRows)) * ceil_div(p.columns, L::kTileColumns) * p.slices;
     launch_blocks<L>(call, op, tile_rows<BF16, B_MN, kColumns, kPair, E, Decode>, tiles, a, b0, b1, box * kBoxRow, args, p.offsets, p.groups, p.rows,
                      static_cast<int>(p.depth), static_cast<int>(p.columns), static_cast<int>(p.slices), call.status);
 }
