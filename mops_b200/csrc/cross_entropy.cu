@@ -149,23 +149,23 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
 }
 
 // to[i,:] = from[order[i],:]
-template <typename To, typename From>
+template <typename S>
 __global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
-loss_gather(To* __restrict__ to, int64_t to_stride, const From* __restrict__ from, int64_t stride, const LossRows rows, int64_t columns) {
+loss_gather(S* __restrict__ to, const S* __restrict__ from, int64_t stride, const LossRows rows, int64_t columns) {
     const int64_t kept = rows.offsets[1];
     for (int64_t i = first_row(); i < kept; i += row_step()) {
         const int64_t r = rows.order[i];
-        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[i * to_stride + c] = convert<To>(from[r * stride + c]);
+        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[i * columns + c] = from[r * stride + c];
     }
 }
 
 // to[r,:] = from[place[r],:], zeros for rows that have no place
-template <typename To, typename From>
+template <typename S>
 __global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
-loss_scatter(To* __restrict__ to, const From* __restrict__ from, const LossRows rows, int64_t n, int64_t columns) {
+loss_scatter(S* __restrict__ to, const S* __restrict__ from, const LossRows rows, int64_t n, int64_t columns) {
     for (int64_t r = first_row(); r < n; r += row_step()) {
         const int64_t i = rows.place[r];
-        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[r * columns + c] = i >= 0 ? convert<To>(from[i * columns + c]) : To(0);
+        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[r * columns + c] = i >= 0 ? from[i * columns + c] : S(0);
     }
 }
 
@@ -448,7 +448,7 @@ bool worth_cutting(int64_t rows, int64_t vocabulary, int64_t columns) { return r
 template <typename S> struct Pieces {
     const Call& call;
     const std::string& op;
-    Scratch room_rows, room_A, room_W, room_logits;
+    Scratch room_rows, room_A, room_logits;
     Packing packing;
     LossRows rows;
     Array A, W, logits;
@@ -461,12 +461,9 @@ template <typename S> struct Pieces {
     static constexpr int32_t kType = sizeof(S) == 8 ? MOPS_B200_F64 : MOPS_B200_F32;
 
     Pieces(const Call& call, const std::string& op, const Array& a, const Array& w, bool forward)
-        : call(call), op(op), room_rows(call), room_A(call), room_W(call), room_logits(call), packing(call), W(w), room_parts_A(call), room_parts_W(call) {
+        : call(call), op(op), room_rows(call), room_A(call), room_logits(call), packing(call), W(w), room_parts_A(call), room_parts_W(call) {
         const int64_t n = a.shape[0], columns = a.shape[1];
-        if (w.type != kType) {
-            room_W.take(static_cast<size_t>(values_of(w)) * sizeof(S) + 16);
-            W = converted(call, w, room_W.as<S>(), kType);
-        }
+        W.type = kType; // (of another type there are no values)
         width = std::max<int64_t>(kMostLogits / n, 256);
         width = width >= kPartColumns ? width / kPartColumns * kPartColumns : width / 256 * 256;
         part = std::min(width, kPartColumns);
@@ -476,7 +473,7 @@ template <typename S> struct Pieces {
         fused = kType == MOPS_B200_F32 && columns > 0 &&
                 (!forward || !straight_rows(matrices(0, W.shape[0]), n, false) || boxable(kType, W.data, columns, W.shape[0], 1, W.stride[0], 0));
         in_parts = fused && worth_cutting(n, W.shape[0], columns);
-        numbered = !forward || !fused || in_parts || a.type != kType || worth_gathering(kType, n, W.shape[0], columns);
+        numbered = !forward || !fused || in_parts || worth_gathering(kType, n, W.shape[0], columns);
         if (numbered) {
             rows = take_rows(room_rows, n);
             room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
@@ -490,19 +487,17 @@ template <typename S> struct Pieces {
     TileProblem problem(int64_t columns) const { return {A, rows.offsets, 1, A.shape[0], A.shape[1], columns}; }
     void gather(const Array& a) {
         if (a.shape[1] == 0) return;
-        if (numbered) for_type(a.type, [&](auto zero) {
-            using From = decltype(zero);
-            loss_gather<S, From><<<row_blocks(call, a.shape[0]), row_threads(), 0, call.stream>>>(
-                static_cast<S*>(A.data), a.shape[1], static_cast<const From*>(a.data), a.stride[0], rows, a.shape[1]);
-        });
+        if (numbered)
+            loss_gather<S><<<row_blocks(call, a.shape[0]), row_threads(), 0, call.stream>>>(static_cast<S*>(A.data), static_cast<const S*>(a.data), a.stride[0], rows,
+                                                                                             a.shape[1]);
         MOPS_CUDA_OK(cudaGetLastError());
         if (in_parts) {
             if constexpr (sizeof(S) == 4) {
                 const int64_t outer = padded_rows(), wide = (W.shape[1] + 7) / 8 * 8;
                 room_parts_A.take(static_cast<size_t>(outer * wide) * 2 * kThreeParts);
                 room_parts_W.take(static_cast<size_t>(W.shape[0] * wide) * 2 * kThreeParts);
-                parts_A = cut(call, room_parts_A.as<void>(), static_cast<const float*>(A.data), A.stride[0], A.shape[0], outer, A.shape[1], nullptr, rows.offsets + 1);
-                parts_W = cut(call, room_parts_W.as<void>(), static_cast<const float*>(W.data), W.stride[0], W.shape[0], W.shape[0], W.shape[1], nullptr, nullptr);
+                parts_A = cut(call, room_parts_A.as<void>(), static_cast<const float*>(A.data), A.stride[0], A.shape[0], outer, A.shape[1], rows.offsets + 1);
+                parts_W = cut(call, room_parts_W.as<void>(), static_cast<const float*>(W.data), W.stride[0], W.shape[0], W.shape[0], W.shape[1], nullptr);
             }
         } else if (fused) {
             packing.add(A);
@@ -581,8 +576,8 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     prepare_rows<S>(call, pieces.rows, nullptr, nullptr, targets, W.shape[0], ignored, nullptr, nullptr);
     if (columns == 0) return;
     pieces.gather(A);
-    const bool need_A = grad_A.data != nullptr, need_W = grad_W.data != nullptr, widened = A.type != pieces.kType;
-    Scratch room_A(call), room_more(call), room_W(call);
+    const bool need_A = grad_A.data != nullptr, need_W = grad_W.data != nullptr;
+    Scratch room_A(call), room_more(call);
     const int64_t stride_A = pieces.fused ? (columns + 3) / 4 * 4 : columns; // of the sums for grad_A
     int64_t slices = 1;
     if (pieces.in_parts && need_A) {
@@ -595,7 +590,6 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     const size_t bytes = static_cast<size_t>(slices * n * stride_A) * sizeof(S);
     if (need_A) room_A.take(bytes);
     if (need_A && !pieces.fused && pieces.width < W.shape[0]) room_more.take(bytes);
-    if (need_W && widened) room_W.take(static_cast<size_t>(pieces.width * columns) * sizeof(S));
     auto multiply = [&](int64_t v0, int64_t v1, Array dx) {
         Array m = pieces.matrices(v0, v1), a = pieces.A;
         m.shape[1] = v1 - v0, m.shape[2] = columns; // (v1 - v0) x C
@@ -619,16 +613,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
             multiply_rows(call, {contiguous(to, pieces.kType, n, columns), dx, m, m.stride[1], 1, pieces.rows.offsets, 1, n, v1 - v0, columns}, op);
             if (v0 > 0) add_values<S><<<blocks_for(call, n * columns), 256, 0, call.stream>>>(room_A.as<S>(), to, n * columns);
         }
-        if (need_W) {
-            char* to = static_cast<char*>(grad_W.data) + v0 * columns * type_bytes(grad_W.type);
-            const Array part = contiguous(widened ? room_W.as<void>() : to, pieces.kType, 1, v1 - v0, columns);
-            multiply_outer(call, {part, dx, a, pieces.rows.offsets, 1}, op);
-            if (widened)
-                for_type(grad_W.type, [&](auto zero) {
-                    using T = decltype(zero);
-                    (void)converted(call, part, reinterpret_cast<T*>(to), grad_W.type);
-                });
-        }
+        if (need_W) multiply_outer(call, {contiguous(static_cast<S*>(grad_W.data) + v0 * columns, pieces.kType, 1, v1 - v0, columns), dx, a, pieces.rows.offsets, 1}, op);
         packing.release();
     };
     if (pieces.in_parts) {
@@ -638,7 +623,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
             // the products with A: straight to where they belong, if that can be, and their depth need not be cut
             const int64_t deep = ceil_div(n, kBoxDepth), tiles = ceil_div(pieces.width, kPartsTile) * ceil_div(columns, kPartsTile);
             const int64_t cuts = best_slices(tiles, sm_count(call.device) / 2, deep, 2.5, 8, static_cast<double>(pieces.width) * columns * 8);
-            const bool straight = cuts == 1 && columns % 4 == 0 && reinterpret_cast<uintptr_t>(grad_W.data) % 16 == 0 && !widened;
+            const bool straight = cuts == 1 && columns % 4 == 0 && reinterpret_cast<uintptr_t>(grad_W.data) % 16 == 0;
             if (need_W && !straight) room_sums.take(static_cast<size_t>(cuts * pieces.width * stride_A) * sizeof(float));
             using Sums = SumStoreOf<kPartsOwn>;
             for (int64_t v0 = 0; v0 < W.shape[0]; v0 += pieces.width) {
@@ -686,19 +671,9 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
     }
     if (need_A) {
         if constexpr (sizeof(S) == 4) {
-            if (pieces.fused) {
-                for_type(grad_A.type, [&](auto zero) {
-                    using T = decltype(zero);
-                    if constexpr (!std::is_same<T, double>::value)
-                        scatter_sums(call, static_cast<T*>(grad_A.data), room_A.template as<float>(), slices, stride_A, pieces.rows, n, columns, false, nullptr);
-                });
-            }
+            if (pieces.fused) scatter_sums(call, static_cast<float*>(grad_A.data), room_A.template as<float>(), slices, stride_A, pieces.rows, n, columns, false, nullptr);
         }
-        if (!pieces.fused)
-            for_type(grad_A.type, [&](auto zero) {
-                using T = decltype(zero);
-                loss_scatter<T, S><<<row_blocks(call, n), row_threads(), 0, call.stream>>>(static_cast<T*>(grad_A.data), room_A.as<S>(), pieces.rows, n, columns);
-            });
+        if (!pieces.fused) loss_scatter<S><<<row_blocks(call, n), row_threads(), 0, call.stream>>>(static_cast<S*>(grad_A.data), room_A.as<S>(), pieces.rows, n, columns);
     }
     MOPS_CUDA_OK(cudaGetLastError());
     note_kernel_f("loss_gradient<%s>", scalar_name<S>());

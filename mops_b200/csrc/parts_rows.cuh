@@ -233,13 +233,13 @@ __device__ __forceinline__ void cut_three(float x, float y, uint32_t (&w)[kThree
     for (int p = 0; p < kThreeParts; p++) w[p] = split::cut_part(u, v);
 }
 
-// Rows of f32 in parts, 8 columns (a pack of each part) to a thread; `order`: of the i-th row (kept of them, then 64 rows of zeros), or none.
+// Rows of f32 in parts, 8 columns (a pack of each part) to a thread: all of them, or *kept and 64 of zeros behind them.
 static __global__ void __launch_bounds__(256)
 cut_rows(uint4* __restrict__ to, int64_t slice_packs, int64_t packs, const float* __restrict__ from, int64_t stride, int64_t rows, int columns,
-         const int32_t* __restrict__ order, const int32_t* __restrict__ kept, bool aligned) {
+         const int32_t* __restrict__ kept, bool aligned) {
     const int64_t n = kept != nullptr ? min(int64_t(*kept) + 64, rows) : rows, real = kept != nullptr ? *kept : rows;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; i < n; i += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-        const float* p = from + (order != nullptr && i < real ? order[i] : i) * stride;
+        const float* p = from + i * stride;
         for (int64_t c = threadIdx.x; c < packs; c += blockDim.x) {
             alignas(16) float x[8];
             const int here = i < real ? columns - static_cast<int>(c) * 8 : 0;
@@ -259,14 +259,14 @@ cut_rows(uint4* __restrict__ to, int64_t slice_packs, int64_t packs, const float
     }
 }
 // room: 6 bytes for each of `outer` x whole packs
-inline PartsArray cut(const Call& call, void* room, const float* from, int64_t stride, int64_t rows, int64_t outer, int64_t columns, const int32_t* order, const int32_t* kept) {
+inline PartsArray cut(const Call& call, void* room, const float* from, int64_t stride, int64_t rows, int64_t outer, int64_t columns, const int32_t* kept) {
     const int64_t packs = (columns + 7) / 8;
     unsigned across = 4;
     while (across < 32 && across < packs) across *= 2;
     const dim3 block(across, 256 / across);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(outer, block.y), int64_t(sm_count(call.device)) * 16));
-    cut_rows<<<grid, block, 0, call.stream>>>(static_cast<uint4*>(room), outer * packs, packs, from, stride, kept != nullptr ? outer : rows, static_cast<int>(columns), order,
-                                              kept, stride % 4 == 0 && reinterpret_cast<uintptr_t>(from) % 16 == 0);
+    cut_rows<<<grid, block, 0, call.stream>>>(static_cast<uint4*>(room), outer * packs, packs, from, stride, kept != nullptr ? outer : rows, static_cast<int>(columns), kept,
+                                              stride % 4 == 0 && reinterpret_cast<uintptr_t>(from) % 16 == 0);
     MOPS_CUDA_OK(cudaGetLastError());
     return {room, columns, outer, packs * 8, outer * packs * 8};
 }

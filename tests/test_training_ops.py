@@ -13,6 +13,7 @@ output's (f16 2^-11, bf16 2^-8):
 """
 import ctypes
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -403,6 +404,33 @@ def test_gated_far_from_zero(dtype, activation):
     check_gated(A, W, offsets_of([R]), torch.ones(R, 8, dtype=dtype, device="cuda"), activation)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_on_broadcast_tensors(dtype):
+    """One matrix for all groups, one row for all rows, one gradient for all results: strides of zero."""
+    offsets, one = offsets_of([100, 0, 150, 50]), torch.ones((), device="cuda", dtype=dtype)
+    check_gated(normal((300, 64), dtype, 1), normal((1, 64, 96), dtype, 2, 0.125).expand(4, 64, 96), offsets, one.expand(300, 48))
+    check_gated(normal((1, 64), dtype, 1).expand(300, 64), normal((4, 64, 96), dtype, 2, 0.125), offsets, normal((300, 48), dtype, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [5, 3000])
+def test_gated_of_more_groups_than_a_grid_is_wide(dtype, R):
+    rows = torch.bincount(torch.randint(70000, (R,), generator=torch.Generator().manual_seed(1)), minlength=70000)
+    A, W, grad = normal((R, 8), dtype, 1), normal((70000, 8, 16), dtype, 2, 0.35), normal((R, 8), dtype, 3)
+    offsets = offsets_of(rows.tolist())
+    full = rows.nonzero()[:, 0]
+    A_, W_ = A.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    output = mt.grouped_gated_product(A_, W_, offsets)
+    grad_A, grad_W = torch.autograd.grad(output, [A_, W_], grad)
+    values, errors = gated_plain(A, W[full.cuda()], offsets_of(rows[full].tolist()), grad, "silu")
+    for g, w, e, what in zip((output.detach(), grad_A, grad_W[full.cuda()]), values, errors, ("output", "grad_A", "grad_W")):
+        within(g, w, e, what)
+    grad_W[full.cuda()] = 0
+    assert (grad_W == 0).all()
+
+
 # ================================================================== linear_cross_entropy
 def loss_plain(A, W, targets, scale, ignored, grad_loss, grad_log_sum):
     """Values and bounds of (loss, log_sum, grad_A, grad_W)."""
@@ -537,6 +565,20 @@ def test_loss_on_strided_and_shifted_tensors(dtype, R):
                           (A[:, ::2], W[:400, ::2], t[:R]), (A[:1, :128].expand(R, 128), W[:400, :128], t[:R]),
                           (A[:, :128].T.contiguous().T, W[:400, :128].T.contiguous().T, t[:R]), (A[:, :128], W[:1, :128].expand(400, 128), t[:R])):
         check_loss(a.detach(), w.detach(), targets)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [200, 3000])
+def test_loss_after_one_of_nan(dtype, R):
+    """What a call leaves in workspaces is not found again: rows behind the last one that counts are zeros there."""
+    A, W = normal((R, 264), dtype, 1), normal((6000, 264), dtype, 2, 0.125)
+    leaves = [torch.full_like(A, float("nan")).requires_grad_(True), W.clone().requires_grad_(True)]
+    loss = mt.linear_cross_entropy(*leaves, some_targets(R, 6000, 1.0))[0]
+    assert loss.isnan().all() and torch.autograd.grad(loss.sum(), leaves)[1].isnan().all()
+    check_loss(A, W, some_targets(R, 6000, 0.37))
+    check_loss(A.detach(), W.detach(), torch.arange(R, dtype=torch.int32, device="cuda") % 7, ignored=5)
+    check_loss(A.detach(), W.detach(), torch.full((R,), 5, dtype=torch.int32, device="cuda"), ignored=5)
 
 
 @pytest.mark.gpu
@@ -815,6 +857,53 @@ def test_a_step_on_other_streams_and_in_a_graph(R):
     for c in captured:
         assert all(torch.equal(x, y) for x, y in zip(c, fresh))
     assert not torch.equal(fresh[0], want[0])
+
+
+@pytest.mark.gpu
+def test_graphs_at_the_same_time():
+    """Two captured steps, replayed over and over on two streams, have workspaces of their own."""
+    def step(seed):
+        A, W, t = normal((2000, 128), torch.bfloat16, seed), normal((9000, 128), torch.bfloat16, seed + 1, 0.1), some_targets(2000, 9000, 0.7, seed)
+        M, offsets = normal((3, 128, 256), torch.bfloat16, seed + 2, 0.1), offsets_of([700, 600, 700])
+        return lambda: [*mt.linear_cross_entropy(A, W, t), mt.grouped_gated_product(A, M, offsets), *mt.clip_gradient_norm([A, W], 0.1)[1]]
+
+    steps = [step(11), step(23)]
+    want = [[x.clone() for x in f()] for f in steps]
+    graphs, got, streams = [], [], [torch.cuda.Stream() for _ in steps]
+    for f in steps:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(f())
+        graphs.append(graph)
+    for _ in range(20):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(g, w))
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads():
+    failures = []
+
+    def work(seed, dtype):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(3):
+                    check_loss(normal((600 + seed, 72), dtype, seed), normal((900, 72), dtype, 2 + seed, 0.125), some_targets(600 + seed, 900, 0.7, seed))
+                    check_gated(normal((500 + seed, 72), dtype, seed), normal((2, 72, 80), dtype, 2, 0.125), offsets_of([200, 300]), normal((500 + seed, 40), dtype, 9))
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i, DTYPES[i % len(DTYPES)])) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures[0]
 
 
 @pytest.mark.gpu
