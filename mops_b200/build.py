@@ -29,7 +29,7 @@ NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-ccbin", HOST_CXX, "-Xco
                      "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr"]
 
 KERNEL_SOURCES = ["runtime.cu", "hpe.cu", "hpe_tmem.cu", "sap.cu", "sap_tmem.cu", "opsa.cu", "opsa_gathered.cu",
-                  "embedding.cu", "grouped.cu", "grouped_mma.cu", "grouped_split.cu", "grouped_few.cu", "gated_product.cu", "gated_mma.cu", "gated_split.cu", "cross_entropy.cu", "cross_entropy_mma.cu", "gradient_norm.cu", "pack.cu", "tensor_map.cu", "residual_norm.cu", "sasaw.cu", "sasaw_rows.cu", "sort.cu", "capi.cu", "host_stubs.cpp"]
+                  "embedding.cu", "grouped.cu", "grouped_mma.cu", "grouped_split.cu", "grouped_few.cu", "gated_product.cu", "gated_mma.cu", "gated_split.cu", "cross_entropy.cu", "cross_entropy_mma.cu", "cross_entropy_few.cu", "gradient_norm.cu", "pack.cu", "tensor_map.cu", "residual_norm.cu", "sasaw.cu", "sasaw_rows.cu", "sort.cu", "capi.cu", "host_stubs.cpp"]
 
 
 def _newer(target, deps):

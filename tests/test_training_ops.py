@@ -569,6 +569,19 @@ def test_loss_on_strided_and_shifted_tensors(dtype, R):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V,C,stride", [
+    (1, 1, 8, 8), (1, 7, 8, 8), (3, 15, 24, 40), (8, 16, 32, 32), (9, 17, 37, 40), (16, 2400, 40, 40), (17, 2400, 40, 40), (8, 100, 1000, 1000), (7, 3001, 2064, 2064),
+    (16, 50021, 64, 64), (5, 40000, 255, 256)])
+def test_loss_of_few_rows(dtype, R, V, C, stride):
+    table = normal((V, stride), dtype, 2, C ** -0.5)
+    table[:, C:] = float("nan")
+    targets = torch.tensor([V - 1, 0, -1, V // 2], device="cuda", dtype=torch.int32)[torch.arange(R, device="cuda") % 4]
+    check_loss(normal((R, C), dtype, 1, 2.0), table[:, :C], targets, 1.5)
+    assert not mt.linear_cross_entropy(normal((R, C), dtype, 1), table[:, :C], targets)[0].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("R", [200, 3000])
 def test_loss_after_one_of_nan(dtype, R):
     """What a call leaves in workspaces is not found again: rows behind the last one that counts are zeros there."""
