@@ -1,4 +1,6 @@
 // grouped_gated_product on tensor cores, for f32: products in three bf16 parts (grouped_split.cu), whose sums of U and V are gated in registers.
+// 100 003 rows of 20 groups, 128 x 2 x 128, gelu: 66 us (102 MB of rows take 16, six products 24), dU and dV 87. With a depth of two or four stages a tile, operands that are cut into parts, sums that leave
+// tensor memory after each stage and what the stores do of them take turns on one SM.
 #include "activation.cuh"
 #include "gated_mma.hpp"
 #include "split_rows.cuh"
