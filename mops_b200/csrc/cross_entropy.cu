@@ -11,6 +11,7 @@
 #include "block_ops.hpp"
 #include "convert.cuh"
 #include "few_rows.cuh"
+#include "gated_mma.hpp"
 #include "grouped_mma.hpp"
 #include "loss_rows.cuh"
 #include "pack.hpp"
@@ -22,6 +23,7 @@ namespace {
 constexpr int kPrepareThreads = 1024, kPrepareRows = 8;
 constexpr int64_t kPartColumns = 4096;             // of a part of a row's sums, at most
 constexpr int64_t kMostLogits = int64_t(64) << 20; // of a piece
+constexpr int64_t kLeastSteps = 4;                 // stages of depth of a slice of f32 products
 
 // Numbers the rows that have a target, by a block, or a cluster of blocks with a part of the rows each, which count theirs first; the others get zeros, if loss is given. (16 384 rows: one block 13.8 us,
 // 9 by eight; 48 285: 31 and 9.)
@@ -456,6 +458,7 @@ template <typename S> struct Pieces {
     bool fused;          // worked on where they are summed
     bool numbered;       // rows without a target have been left out
     bool in_parts;       // operands are cut beforehand
+    bool sliced;         // or in slices of the depth, where tiles would leave SMs without work, to be worked on where they are stored
     PartsArray parts_A{}, parts_W{};
     Scratch room_parts_A, room_parts_W;
     static constexpr int32_t kType = sizeof(S) == 8 ? MOPS_B200_F64 : MOPS_B200_F32;
@@ -473,7 +476,10 @@ template <typename S> struct Pieces {
         fused = kType == MOPS_B200_F32 && columns > 0 &&
                 (!forward || !straight_rows(matrices(0, W.shape[0]), n, false) || boxable(kType, W.data, columns, W.shape[0], 1, W.stride[0], 0));
         in_parts = fused && worth_cutting(n, W.shape[0], columns);
-        numbered = !forward || !fused || in_parts || worth_gathering(kType, n, W.shape[0], columns);
+        // (674 rows of 60 x 3040, 6 tiles: 31 us for 86, with gradients 97 for 219; 200 of 1000 x 4096, 16 tiles, 53 and 159 for 115 and 290. But 60 of 4000 x 2048, 32 tiles, 76 and 197 for 63 and 179, and
+        // with less depth the host's part of three more launches is longer: 674 of 60 x 1024 43 for 37)
+        sliced = fused && !in_parts && columns >= 2048 && 8 * ceil_div(n, kTileRows) * ceil_div(W.shape[0], kSplitColumns) <= sm_count(call.device);
+        numbered = !forward || !fused || in_parts || sliced || worth_gathering(kType, n, W.shape[0], columns);
         if (numbered) {
             rows = take_rows(room_rows, n);
             room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
@@ -526,7 +532,8 @@ template <typename S> struct Pieces {
             const int64_t v1 = std::min(v0 + width, W.shape[0]);
             const Array m = matrices(v0, v1);
             logits = contiguous(room_logits.as<void>(), kType, A.shape[0], v1 - v0);
-            multiply_rows(call, {logits, A, m, m.stride[1], m.stride[2], rows.offsets, 1, A.shape[0], A.shape[1], v1 - v0}, op);
+            const RowsProblem problem{logits, A, m, m.stride[1], m.stride[2], rows.offsets, 1, A.shape[0], A.shape[1], v1 - v0};
+            if (!sliced || !multiply_rows_sliced(call, problem, kLeastSteps, op)) multiply_rows(call, problem, op);
             const dim3 grid(static_cast<unsigned>(A.shape[0]), static_cast<unsigned>(ceil_div(v1 - v0, part)));
             f(v0, v1, grid, static_cast<S*>(logits.data));
             MOPS_CUDA_OK(cudaGetLastError());
@@ -538,7 +545,7 @@ template <typename S>
 void loss_forward(const Call& call, const Array& loss, const Array& log_sum, const Array& A, const Array& W, const Array& targets, double scale,
                   int64_t ignored, const std::string& op) {
     Pieces<S> pieces(call, op, A, W, true);
-    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.in_parts ? kPartsOwn : pieces.fused ? LossStore32::kOwn : pieces.part);
+    const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.in_parts ? kPartsOwn : pieces.fused && !pieces.sliced ? LossStore32::kOwn : pieces.part);
     const int32_t* t = static_cast<const int32_t*>(targets.data);
     if (pieces.numbered) prepare_rows<S>(call, pieces.rows, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), targets, W.shape[0], ignored, nullptr, nullptr);
     pieces.gather(A);
@@ -551,7 +558,7 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
             const E::Args args{sums, parts, at_target, pieces.rows.target, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
             launch_parts<false, false, E, DecodeRows>(call, op, pieces.parts_A, pieces.parts_W, pieces.rows.offsets, n, W.shape[1], W.shape[0], 1, pieces.operands(0), args);
             note_kernel("loss_rows_parts");
-        } else if (pieces.fused) {
+        } else if (pieces.fused && !pieces.sliced) {
             const LossStore32::Args args{sums, parts, at_target, pieces.numbered ? pieces.rows.target : t, static_cast<int>(W.shape[0]), static_cast<float>(scale)};
             const TileOperand w{pieces.W.data, 1, pieces.W.stride[0], 0}, operands[2] = {w, w};
             if (pieces.numbered) launch_split<false, LossStore32, DecodeRows>(call, op, pieces.problem(W.shape[0]), operands, args);
@@ -559,7 +566,7 @@ void loss_forward(const Call& call, const Array& loss, const Array& log_sum, con
             note_kernel("loss_rows_split");
         }
     }
-    if (!pieces.fused) pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
+    if (!pieces.fused || pieces.sliced) pieces.for_each([&](int64_t v0, int64_t v1, dim3 grid, S* logits) {
         loss_sums<S><<<grid, 256, 0, call.stream>>>(sums, parts, v0 / pieces.part, at_target, logits, v1 - v0, static_cast<S>(scale), t, v0, pieces.part,
                                                      pieces.rows);
     });
@@ -596,7 +603,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
         std::swap(m.stride[1], m.stride[2]);
         Packing packing(call);
         if (pieces.kType == MOPS_B200_F32) {
-            const bool rows_packed = need_A && !straight_rows(m, n, true), outer_packed = need_W && !straight_outer(n, 1, v1 - v0, columns, pieces.kType);
+            const bool rows_packed = need_A && (pieces.fused || !straight_rows(m, n, true)), outer_packed = need_W && !straight_outer(n, 1, v1 - v0, columns, pieces.kType);
             if (rows_packed || outer_packed) packing.add(dx);
             if (rows_packed) packing.add(m);
             if (outer_packed) packing.add(a);
@@ -645,7 +652,7 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
                 MOPS_CUDA_OK(cudaGetLastError());
             }
         }
-    } else if (pieces.fused) {
+    } else if (pieces.fused && !pieces.sliced) {
         if constexpr (sizeof(S) == 4) {
             pieces.take_logits();
             const int64_t stride = (pieces.width + 3) / 4 * 4;

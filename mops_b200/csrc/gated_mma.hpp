@@ -25,7 +25,7 @@ void gated_rows_vjp_mma(const Call& call, const GatedProblem& p, void* to, const
 void gated_rows_split(const Call& call, const GatedProblem& p, const Array& output, const std::string& op);
 void gated_rows_vjp_split(const Call& call, const GatedProblem& p, const Array& to, const Array& grad, const std::string& op);
 // grad_A = duv W^T, where that is worth cutting the depth for (few tiles of a long depth); else false.
-bool multiply_rows_sliced(const Call& call, const RowsProblem& p, const std::string& op);
+bool multiply_rows_sliced(const Call& call, const RowsProblem& p, int64_t least, const std::string& op);
 
 } // namespace mops_b200
 

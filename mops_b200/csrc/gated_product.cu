@@ -320,7 +320,7 @@ void grouped_gated_product_vjp(Array grad_A, Array grad_W, Array grad_output, Ar
     if (need_A)
         result(grad_A, [&](const Array& to) {
             const RowsProblem problem{to, wide.uv, wide.W, wide.W.stride[2], wide.W.stride[1], starts, W.shape[0], rows, columns, A.shape[1]};
-            if (!wide.fused || !multiply_rows_sliced(call, problem, op)) multiply_rows(call, problem, op);
+            if (!wide.fused || !multiply_rows_sliced(call, problem, 16, op)) multiply_rows(call, problem, op);
         });
     if (need_W)
         result(grad_W, [&](const Array& to) {

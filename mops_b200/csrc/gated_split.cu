@@ -130,9 +130,9 @@ void gated_rows_vjp_split(const Call& call, const GatedProblem& p, const Array& 
     });
 }
 
-bool multiply_rows_sliced(const Call& call, const RowsProblem& p, const std::string& op) {
+bool multiply_rows_sliced(const Call& call, const RowsProblem& p, int64_t least, const std::string& op) {
     const int64_t sms = sm_count(call.device), tiles = most_row_tiles(p.rows, p.groups, kTileRows) * ceil_div(p.columns, kSplitColumns);
-    const int64_t slices = best_slices(tiles, sms, ceil_div(p.depth, split::kDepth), 0.7, 16, static_cast<double>(p.rows) * p.columns * 8);
+    const int64_t slices = best_slices(tiles, sms, ceil_div(p.depth, split::kDepth), 0.7, least, static_cast<double>(p.rows) * p.columns * 8);
     if (2 * tiles > sms || slices == 1) return false;
     const int64_t stride = (p.columns + 3) / 4 * 4;
     Scratch room(call, static_cast<size_t>(slices * p.rows * stride) * sizeof(float));

@@ -595,6 +595,21 @@ def test_loss_after_one_of_nan(dtype, R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V,C", [(130, 7, 2049), (674, 61, 2600), (40, 1999, 2300), (1, 3, 2500)])
+def test_loss_of_few_tiles_of_much_depth(dtype, R, V, C):
+    """Also where an operand is infinite, and rows and table begin anywhere."""
+    A, W = normal((R, C + 3), dtype, 1)[:, 1:C + 1], normal((V, C + 1), dtype, 2, C ** -0.5)[:, 1:]
+    targets = some_targets(R, V, 0.8)
+    check_loss(A, W, targets, 1.25)
+    A = A.detach().clone()
+    A[R // 2, C - 1] = float("inf")
+    targets[R // 2] = 0
+    loss, log_sum = mt.linear_cross_entropy(A, W.detach(), targets)
+    assert not log_sum[R // 2].isfinite() and log_sum.isfinite().sum() == R - 1
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_loss_of_many_logits_on_strided_tensors(dtype):
     A, W, t = normal((900, 1300), dtype, 1), normal((9100, 1300), dtype, 2, 0.1), some_targets(900, 9000, 0.9)
