@@ -888,6 +888,35 @@ def test_a_step_on_other_streams_and_in_a_graph(R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_step_with_autograd_in_a_graph(dtype):
+    """Forward, gradients through autograd and clipping, captured after an eager step of which nothing is left, and replayed on new values."""
+    leaves = [normal((1000, 64), dtype, 1), normal((3, 64, 192), dtype, 2, 0.125), normal((3, 96, 64), dtype, 3, 0.125)]
+    leaves = [t.requires_grad_(True) for t in leaves]
+    offsets, tokens, targets = offsets_of([100, 0, 500]), some_targets(600, 1000, 1.0), some_targets(600, 1000, 0.9, 6)
+
+    def step():
+        table, W1, W2 = leaves
+        out = mt.grouped_matrix_product(mt.grouped_gated_product(mt.embedding_lookup(table, tokens), W1, offsets), W2, offsets)
+        loss, log_sum = mt.linear_cross_entropy(out, table, targets)
+        gradients = torch.autograd.grad(loss.mean() + 1e-3 * log_sum.mean(), leaves)
+        norm, clipped = mt.clip_gradient_norm(gradients, 1e-3)
+        return [loss.detach(), norm, *clipped]
+
+    before = [t.clone() for t in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    with torch.no_grad():
+        leaves[0].mul_(1.25)
+    targets.copy_(some_targets(600, 1000, 0.8, 8))
+    graph.replay()
+    graph.replay()
+    for c, f, b in zip(captured, step(), before):
+        assert torch.equal(c, f) and not torch.equal(c, b)
+
+
+@pytest.mark.gpu
 def test_graphs_at_the_same_time():
     """Two captured steps, replayed over and over on two streams, have workspaces of their own."""
     def step(seed):
