@@ -153,11 +153,11 @@ loss_prepare(const LossRows to, S* __restrict__ loss, S* __restrict__ log_sum, c
 // to[i,:] = from[order[i],:]
 template <typename S>
 __global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
-loss_gather(S* __restrict__ to, const S* __restrict__ from, int64_t stride, const LossRows rows, int64_t columns) {
+loss_gather(S* __restrict__ to, int64_t to_stride, const S* __restrict__ from, int64_t stride, const LossRows rows, int64_t columns) {
     const int64_t kept = rows.offsets[1];
     for (int64_t i = first_row(); i < kept; i += row_step()) {
         const int64_t r = rows.order[i];
-        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[i * columns + c] = from[r * stride + c];
+        for (int64_t c = threadIdx.x; c < columns; c += kRowThreads) to[i * to_stride + c] = from[r * stride + c];
     }
 }
 
@@ -478,12 +478,15 @@ template <typename S> struct Pieces {
         in_parts = fused && worth_cutting(n, W.shape[0], columns);
         // (674 rows of 60 x 3040, 6 tiles: 31 us for 86, with gradients 97 for 219; 200 of 1000 x 4096, 16 tiles, 53 and 159 for 115 and 290. But 60 of 4000 x 2048, 32 tiles, 76 and 197 for 63 and 179, and
         // with less depth the host's part of three more launches is longer: 674 of 60 x 1024 43 for 37)
-        sliced = fused && !in_parts && columns >= 2048 && 8 * ceil_div(n, kTileRows) * ceil_div(W.shape[0], kSplitColumns) <= sm_count(call.device);
+        const int64_t tiles = ceil_div(n, kTileRows) * ceil_div(W.shape[0], kSplitColumns), sms = sm_count(call.device);
+        sliced = fused && !in_parts && columns >= 2048 && (8 * tiles <= sms || (4 * tiles <= sms && W.shape[0] <= kSplitColumns));
         numbered = !forward || !fused || in_parts || sliced || worth_gathering(kType, n, W.shape[0], columns);
         if (numbered) {
             rows = take_rows(room_rows, n);
-            room_A.take(static_cast<size_t>(n * columns) * sizeof(S) + 16);
+            const int64_t stride = fused ? (columns + 3) / 4 * 4 : columns; // (as the copy engine can fetch them)
+            room_A.take(static_cast<size_t>(n * stride) * sizeof(S) + 16);
             A = contiguous(room_A.as<void>(), kType, n, columns);
+            A.stride[0] = stride;
         } else {
             rows = LossRows{};
             A = a;
@@ -494,7 +497,7 @@ template <typename S> struct Pieces {
     void gather(const Array& a) {
         if (a.shape[1] == 0) return;
         if (numbered)
-            loss_gather<S><<<row_blocks(call, a.shape[0]), row_threads(), 0, call.stream>>>(static_cast<S*>(A.data), static_cast<const S*>(a.data), a.stride[0], rows,
+            loss_gather<S><<<row_blocks(call, a.shape[0]), row_threads(), 0, call.stream>>>(static_cast<S*>(A.data), A.stride[0], static_cast<const S*>(a.data), a.stride[0], rows,
                                                                                              a.shape[1]);
         MOPS_CUDA_OK(cudaGetLastError());
         if (in_parts) {

@@ -102,26 +102,38 @@ struct Widened {
 };
 
 // ---- f16 and bf16 on tensor cores
+// n values where there are m, zeros behind those, by kRowThreads threads: 16 bytes at a time, as the result lies.
+__device__ __forceinline__ void copy_run(uint16_t* q, int n, const uint16_t* p, int m, const unsigned char* begin, const unsigned char* end) {
+    const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(q) & 15)) & 15) / 2), packs = (n - head) / 8;
+    for (int i = threadIdx.x; i < head; i += kRowThreads) q[i] = i < m ? p[i] : 0;
+    for (int c = threadIdx.x; c < packs; c += kRowThreads) {
+        const int at = head + c * 8;
+        *reinterpret_cast<uint4*>(q + at) = at < m ? load_anywhere<__half>(reinterpret_cast<const __half*>(p + at), m - at, begin, end) : make_uint4(0, 0, 0, 0);
+    }
+    for (int i = head + packs * 8 + threadIdx.x; i < n; i += kRowThreads) q[i] = i < m ? p[i] : 0;
+}
 // The halves of matrices (of `from_columns` columns each) where those of others (of `to_columns`) are, both by columns or both by depth; zeros where there are none. A row of `to` to kRowThreads threads.
-template <bool kByColumns>
+// Of groups without rows: zeros (kZeros), or nothing, as nobody reads their matrices. (43 groups of 464 x 2 x 802, 128 MB read and written: 27 us, value by value 42; 62 groups of 594 x 2 x 1405,
+// three of which have rows: 11 and 120)
+template <bool kByColumns, bool kZeros>
 __global__ void __launch_bounds__(kRowThreads * kRowsAtATime)
 copy_halves(uint16_t* __restrict__ to, int64_t to_group_stride, int64_t to_stride, int to_columns, const uint16_t* __restrict__ from, int64_t from_group_stride, int64_t from_stride,
-            int from_columns, int64_t groups, int to_depth, int from_depth) {
+            int from_columns, int64_t groups, int to_depth, int from_depth, const unsigned char* end, const int32_t* __restrict__ offsets) {
+    const unsigned char* begin = reinterpret_cast<const unsigned char*>(from);
     const int64_t outer = kByColumns ? to_depth : 2 * to_columns;
     for (int64_t row = first_row(); row < groups * outer; row += row_step()) {
         const int64_t g = row / outer;
         const int o = static_cast<int>(row - g * outer);
         uint16_t* q = to + g * to_group_stride + o * to_stride;
         const uint16_t* p = from + g * from_group_stride;
+        const bool empty = __ldg(offsets + g + 1) <= __ldg(offsets + g);
+        if (empty && !kZeros) continue;
         if constexpr (kByColumns) { // depth o, both halves of its row
-            for (int c = threadIdx.x; c < 2 * to_columns; c += kRowThreads) {
-                const int half = c >= to_columns, j = half ? c - to_columns : c;
-                q[c] = j < from_columns && o < from_depth ? p[o * from_stride + half * from_columns + j] : 0;
-            }
+            for (int half = 0; half < 2; half++)
+                copy_run(q + half * to_columns, to_columns, p + o * from_stride + half * from_columns, o < from_depth && !empty ? from_columns : 0, begin, end);
         } else {
             const int half = o >= to_columns, j = half ? o - to_columns : o;
-            for (int d = threadIdx.x; d < to_depth; d += kRowThreads)
-                q[d] = j < from_columns && d < from_depth ? p[(half * from_columns + j) * from_stride + d] : 0;
+            copy_run(q, to_depth, p + (half * from_columns + j) * from_stride, j < from_columns && !empty ? from_depth : 0, begin, end);
         }
     }
 }
@@ -144,7 +156,7 @@ struct Boxed {
             room.take(static_cast<size_t>(values_of(p.W)) * 2);
             p.W.data = room.as<void>();
             if (W.stride[2] != 1) std::swap(p.W.shape[1], p.W.shape[2]), std::swap(p.W.stride[1], p.W.stride[2]);
-            move_halves(p.W, wide, W, columns);
+            move_halves<false>(p.W, wide, W, columns);
             p.W.shape[1] = depth;
         } else {
             packing.add(p.W);
@@ -152,13 +164,15 @@ struct Boxed {
         packing.run();
     }
     // The halves of `from` (of `n` columns each) go where those of `to` (of `m`) are; both are stored the same way round.
-    void move_halves(const Array& to, int64_t m, const Array& from, int64_t n) {
+    template <bool kZeros> void move_halves(const Array& to, int64_t m, const Array& from, int64_t n) {
         const bool by_columns = from.stride[2] == 1;
         const int64_t rows = to.shape[0] * (by_columns ? to.shape[1] : 2 * m);
-        auto kernel = by_columns ? copy_halves<true> : copy_halves<false>;
+        const int64_t outer = by_columns ? from.shape[1] : 2 * n, inner = by_columns ? 2 * n : from.shape[1], stride = by_columns ? from.stride[1] : from.stride[2];
+        const unsigned char* end = static_cast<const unsigned char*>(from.data) + ((from.shape[0] - 1) * from.stride[0] + (outer - 1) * stride + inner) * 2;
+        auto kernel = by_columns ? copy_halves<true, kZeros> : copy_halves<false, kZeros>;
         kernel<<<row_blocks(call, rows), row_threads(), 0, call.stream>>>(
             static_cast<uint16_t*>(to.data), to.stride[0], by_columns ? to.stride[1] : to.stride[2], static_cast<int>(m), static_cast<const uint16_t*>(from.data),
-            from.stride[0], by_columns ? from.stride[1] : from.stride[2], static_cast<int>(n), to.shape[0], static_cast<int>(to.shape[1]), static_cast<int>(from.shape[1]));
+            from.stride[0], stride, static_cast<int>(n), to.shape[0], static_cast<int>(to.shape[1]), static_cast<int>(from.shape[1]), end, p.offsets);
         MOPS_CUDA_OK(cudaGetLastError());
     }
 };
@@ -195,7 +209,7 @@ void gradients_16(const Call& call, const Array& grad_A, const Array& grad_W, bo
         Array result = grad_W;
         if (turned)
             for (Array* a : {&to, &result}) std::swap(a->shape[1], a->shape[2]), std::swap(a->stride[1], a->stride[2]);
-        boxed.move_halves(result, boxed.real_columns, to, p.columns);
+        boxed.move_halves<true>(result, boxed.real_columns, to, p.columns);
     }
 }
 

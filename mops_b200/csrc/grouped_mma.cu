@@ -383,7 +383,10 @@ grouped_outer_mma(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                         for (int c = 0; c < wide; c += 64)
                             store_columns<BF16, kScaled>(from + c, staging, sent, map_out, to, band, piece.group,
                                                          column + c, columns, loose ? here : 32, loose, lane, scaled);
-                    } else { // a group without rows
+                    } else if (!loose) { // a group without rows
+                        for (int i = 0; i < here; i++)
+                            for (int c = lane * 8; c < wide; c += 32 * 8) *reinterpret_cast<uint4*>(to + static_cast<int64_t>(i) * columns + column + c) = make_uint4(0, 0, 0, 0);
+                    } else {
                         for (int i = 0; i < here; i++)
                             for (int c = lane; c < wide; c += 32) to[static_cast<int64_t>(i) * columns + column + c] = 0;
                     }

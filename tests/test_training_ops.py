@@ -415,6 +415,17 @@ def test_gated_on_broadcast_tensors(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("other_way", [False, True])
+@pytest.mark.parametrize("K,N", [(33, 65), (64, 96), (137, 261)])
+def test_gated_matrices_of_empty_groups_are_not_read(dtype, other_way, K, N):
+    rows = [0, 70, 0, 0, 400, 1, 0]
+    W = normal((7, 2 * N, K) if other_way else (7, K, 2 * N), dtype, 2, K ** -0.5)
+    W[[i for i, n in enumerate(rows) if n == 0]] = float("nan")
+    check_gated(normal((471, K), dtype, 1), W.transpose(1, 2) if other_way else W, offsets_of(rows), normal((471, N), dtype, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("R", [5, 3000])
 def test_gated_of_more_groups_than_a_grid_is_wide(dtype, R):
     rows = torch.bincount(torch.randint(70000, (R,), generator=torch.Generator().manual_seed(1)), minlength=70000)
