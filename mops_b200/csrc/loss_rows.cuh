@@ -33,16 +33,17 @@ template <typename S> struct alignas(2 * sizeof(S)) PartSum {
     }
 };
 
-// The i-th row's loss and log_sum from the sums of its parts, and x at the target. A warp to a row: its lanes find the largest first, and take one exponential for each part. Where rows have not
+// The i-th row's loss and log_sum from the sums of its parts, and x at the target. kLanes to a row (a warp, or 4 where its parts are few: 53 996 rows of one 4.5 us for 18.6, 62 070 of five 5.3 for 16.9): they find the largest first, and take one exponential for each part. Where rows have not
 // been numbered (no order) they are all there, and those without a target get their zeros here.
-constexpr int kJoinThreads = 128;
-template <typename S>
+constexpr int kJoinThreads = 128, kInFlight = 8; // parts that a lane has under way
+template <typename S, int kLanes>
 static __global__ void __launch_bounds__(kJoinThreads)
 loss_join(S* __restrict__ loss, S* __restrict__ log_sum, const PartSum<S>* __restrict__ parts, int64_t n, int64_t all_rows, const S* __restrict__ at_target,
           const LossRows rows, const int32_t* __restrict__ targets, int64_t vocabulary, int64_t ignored, Status st) {
     after_others();
-    const int lane = threadIdx.x & 31;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + threadIdx.x / 32;
+    const int lane = threadIdx.x % kLanes;
+    const unsigned group = kLanes == 32 ? kFullMask : ((1u << kLanes) - 1) << (threadIdx.x & 31) / kLanes * kLanes;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
     if (i >= all_rows) return;
     int64_t r = i;
     if (rows.order != nullptr) {
@@ -58,28 +59,28 @@ loss_join(S* __restrict__ loss, S* __restrict__ log_sum, const PartSum<S>* __res
             return;
         }
     }
-    constexpr int kInFlight = 8;
     const PartSum<S>* of_row = parts + i * n;
     S top = -S(INFINITY);
-    for (int64_t p0 = lane; p0 < n; p0 += 32 * kInFlight) {
+    for (int64_t p0 = lane; p0 < n; p0 += kLanes * kInFlight) {
         S v[kInFlight];
 #pragma unroll
-        for (int k = 0; k < kInFlight; k++) v[k] = p0 + 32 * k < n ? of_row[p0 + 32 * k].top : -S(INFINITY);
+        for (int k = 0; k < kInFlight; k++) v[k] = p0 + kLanes * k < n ? of_row[p0 + kLanes * k].top : -S(INFINITY);
 #pragma unroll
         for (int k = 0; k < kInFlight; k++) top = fmax(top, v[k]);
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(kFullMask, top, d));
+    for (int d = kLanes / 2; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(group, top, d));
     const S base = PartSum<S>::from(top);
     S sum = 0;
-    for (int64_t p0 = lane; p0 < n; p0 += 32 * kInFlight) { // (from the L1, or near it)
+    for (int64_t p0 = lane; p0 < n; p0 += kLanes * kInFlight) { // (from the L1, or near it)
         PartSum<S> v[kInFlight];
 #pragma unroll
-        for (int k = 0; k < kInFlight; k++) v[k] = p0 + 32 * k < n ? of_row[p0 + 32 * k] : PartSum<S>::none();
+        for (int k = 0; k < kInFlight; k++) v[k] = p0 + kLanes * k < n ? of_row[p0 + kLanes * k] : PartSum<S>::none();
 #pragma unroll
         for (int k = 0; k < kInFlight; k++) sum += v[k].sum * v[k].weight(base);
     }
-    sum = warp_sum(sum);
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(group, sum, d);
     if (lane != 0) return;
     const S value = base + log(sum);
     log_sum[r] = value;
@@ -89,8 +90,13 @@ template <typename S>
 void join_rows(const Call& call, const Array& loss, const Array& log_sum, const PartSum<S>* parts, int64_t n, const S* at_target, const LossRows& rows, const Array& targets,
                int64_t vocabulary, int64_t ignored) {
     const int64_t all = targets.shape[0];
-    launch_early(call, loss_join<S>, static_cast<unsigned>(ceil_div(all, kJoinThreads / 32)), kJoinThreads, static_cast<S*>(loss.data), static_cast<S*>(log_sum.data), parts, n,
-                 all, at_target, rows, static_cast<const int32_t*>(targets.data), vocabulary, ignored, call.status);
+    auto launch = [&](auto lanes) {
+        constexpr int kLanes = decltype(lanes)::value;
+        launch_early(call, loss_join<S, kLanes>, static_cast<unsigned>(ceil_div(all, kJoinThreads / kLanes)), kJoinThreads, static_cast<S*>(loss.data),
+                     static_cast<S*>(log_sum.data), parts, n, all, at_target, rows, static_cast<const int32_t*>(targets.data), vocabulary, ignored, call.status);
+    };
+    if (n <= 4 * kInFlight) launch(std::integral_constant<int, 4>());
+    else launch(std::integral_constant<int, 32>());
 }
 
 inline LossRows take_rows(Scratch& room, int64_t rows) {
@@ -137,7 +143,7 @@ scatter_rows(T* __restrict__ to, const float* __restrict__ sums, int slices, int
             T* p = to + r * columns + 4 * q;
             if (by_four) {
                 *reinterpret_cast<Pack<T, 4>*>(p) = out;
-            } else {
+            } else { // (a column to a thread: 48 357 rows of 469 59 us for 44)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                     if (4 * q + k < columns) p[k] = out.v[k];
