@@ -547,6 +547,12 @@ template <typename S> struct Pieces {
 template <typename S>
 void loss_forward(const Call& call, const Array& loss, const Array& log_sum, const Array& A, const Array& W, const Array& targets, double scale,
                   int64_t ignored, const std::string& op) {
+    if constexpr (sizeof(S) == 4) {
+        if (A.type == MOPS_B200_F32 && few_loss_rows({A, W, targets, scale, ignored})) {
+            loss_forward_few(call, {A, W, targets, scale, ignored}, loss, log_sum);
+            return;
+        }
+    }
     Pieces<S> pieces(call, op, A, W, true);
     const int64_t n = A.shape[0], parts = ceil_div(W.shape[0], pieces.in_parts ? kPartsOwn : pieces.fused && !pieces.sliced ? LossStore32::kOwn : pieces.part);
     const int32_t* t = static_cast<const int32_t*>(targets.data);

@@ -1,4 +1,4 @@
-// linear_cross_entropy of a few rows in f16 and bf16: how likely the tokens in flight were.
+// linear_cross_entropy of a few rows in f16, bf16 and f32: how likely the tokens in flight were.
 //
 // The table is all that is moved, once. A warp takes 16 of its rows at a time, whose values go from memory straight to the operands of matrix instructions (16 of the table's rows by 8 of A's): a lane has 8
 // neighbours of each row, and as the order of a sum's terms is free, A is read from shared memory in the order that this gives. No row of the table passes through shared memory, none has to begin
@@ -13,7 +13,7 @@
 namespace mops_b200 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;
 constexpr int kUnitRows = 16, kFewDepth = 32; // of the table; of a step
 constexpr int kMostFewBytes = 200 * 1024;
@@ -169,6 +169,169 @@ loss_few(PartSum<float>* __restrict__ parts, float* __restrict__ at_target, cons
     }
 }
 
+// ---- f32, by the ordinary units: a warp takes 16 of the table's rows, eight lanes to four of them, kVector neighbours to a lane at a time. 8 rows of A with 50 021 x 1024
+// (205 MB, 31 us): 49 us, on tensor cores in three parts 94; 16 rows 87 and 94; 5 with 104 534 x 146 19 us, by a product into memory and a pass over it 72. Reading A from shared memory takes as long as the
+// products, which wait for memory in between: fetching a warp's next rows ahead to L2 costs more (54 us) than it gives.
+template <int kVector> struct FewVector {
+    float v[kVector];
+    __device__ __forceinline__ void load(const float* p) {
+        if constexpr (kVector == 4) {
+            const uint4 w = load_once(reinterpret_cast<const uint16_t*>(p));
+            v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
+        } else if constexpr (kVector == 2) {
+            const float2 w = __ldg(reinterpret_cast<const float2*>(p));
+            v[0] = w.x, v[1] = w.y;
+        } else {
+            v[0] = __ldg(p);
+        }
+    }
+    __device__ __forceinline__ void load_shared(const float* p) {
+        if constexpr (kVector == 4) {
+            const float4 w = *reinterpret_cast<const float4*>(p);
+            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+        } else if constexpr (kVector == 2) {
+            const float2 w = *reinterpret_cast<const float2*>(p);
+            v[0] = w.x, v[1] = w.y;
+        } else {
+            v[0] = *p;
+        }
+    }
+};
+struct FewOperand32 {
+    const float* data;
+    int64_t stride, rows;
+};
+
+// kTiles: of 8 rows of A. split: as in loss_few.
+template <int kTiles, int kVector>
+__global__ void __launch_bounds__(kFewThreads, 1)
+loss_few32(PartSum<float>* __restrict__ parts, float* __restrict__ at_target, const FewOperand32 A, const FewOperand32 W, int depth, const int32_t* __restrict__ targets, float scale,
+           int row_values, int split) {
+    constexpr int kRows = kTiles * 8, kStep = 8 * kVector, kMany = kVector == 4 ? (kTiles == 1 ? 4 : 2) : 4;
+    extern __shared__ __align__(16) float values_of_A[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 3, t = lane & 7;
+    const int chunks = (depth + kStep - 1) / kStep, own_chunks = (chunks + split - 1) / split, part = warp & (split - 1);
+    const int chunk0 = min(part * own_chunks, chunks), chunk1 = min(chunk0 + own_chunks, chunks);
+    const int64_t first = static_cast<int64_t>(warp / split) * gridDim.x + blockIdx.x;
+    for (int i = warp; i < kRows; i += kFewWarps)
+        for (int c = lane; c < row_values; c += 32) values_of_A[i * row_values + c] = i < A.rows && c < depth ? A.data[i * A.stride + c] : 0.f;
+    float* const of_parts = values_of_A + kRows * row_values; // (if there are parts)
+    int target[kTiles];
+    PartSum<float> all[kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; j++) target[j] = j * 8 + t < A.rows ? targets[j * 8 + t] : -1, all[j] = PartSum<float>::none();
+    __syncthreads();
+    const float* const own = values_of_A + t * kVector;
+
+    for (int64_t unit = first;; unit += static_cast<int64_t>(kFewWarps) * gridDim.x) {
+        const bool there = unit * kUnitRows < W.rows;
+        if (!there && split == 1) break;
+        const float* p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = W.data + min(unit * kUnitRows + g + 4 * k, W.rows - 1) * W.stride + t * kVector;
+        float sum[4][kRows] = {};
+        auto steps = [&](int c, auto many, bool whole) {
+            constexpr int kNow = decltype(many)::value;
+            FewVector<kVector> w[kNow][4];
+#pragma unroll
+            for (int q = 0; q < kNow; q++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int d = (c + q) * kStep;
+                    if (whole) {
+                        w[q][k].load(p[k] + d);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kVector; e++) w[q][k].v[e] = d + t * kVector + e < depth ? __ldg(p[k] + d + e) : 0.f;
+                    }
+                }
+#pragma unroll
+            for (int q = 0; q < kNow; q++)
+#pragma unroll
+                for (int i = 0; i < kRows; i++) {
+                    FewVector<kVector> a;
+                    a.load_shared(own + i * row_values + (c + q) * kStep);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int e = 0; e < kVector; e++) sum[k][i] = fmaf(w[q][k].v[e], a.v[e], sum[k][i]);
+                }
+        };
+        if (there) {
+            const int whole = min(chunk1, depth / kStep);
+            int c = chunk0;
+            for (; c + kMany <= whole; c += kMany) steps(c, std::integral_constant<int, kMany>(), true);
+            for (; c < chunk1; c++) steps(c, std::integral_constant<int, 1>(), c < whole);
+        }
+        // of each row of A the sums of eight lanes, to the lane of that number
+        float x[kTiles][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int j = 0; j < kTiles; j++) {
+                float four[4], two[2];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float low = sum[k][j * 8 + i], high = sum[k][j * 8 + i + 4];
+                    four[i] = (t & 4 ? high : low) + __shfl_xor_sync(kFullMask, t & 4 ? low : high, 4);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) two[i] = (t & 2 ? four[i + 2] : four[i]) + __shfl_xor_sync(kFullMask, t & 2 ? four[i] : four[i + 2], 2);
+                x[j][k] = (t & 1 ? two[1] : two[0]) + __shfl_xor_sync(kFullMask, t & 1 ? two[0] : two[1], 1);
+            }
+        if (split > 1) { // the only unit
+            float* const to = of_parts + warp * kTiles * 4 * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < kTiles; j++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) to[(j * 4 + k) * 32] = x[j][k];
+            __syncthreads();
+            if (!there || part > 0) break;
+#pragma unroll 1
+            for (int q = 1; q < split; q++)
+#pragma unroll
+                for (int j = 0; j < kTiles; j++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) x[j][k] += to[((q * kTiles + j) * 4 + k) * 32];
+        }
+#pragma unroll
+        for (int j = 0; j < kTiles; j++) {
+            PartSum<float> now{-INFINITY, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int64_t v = unit * kUnitRows + g + 4 * k;
+                if (v < W.rows && v == target[j]) at_target[j * 8 + t] = x[j][k] * scale;
+                x[j][k] = v < W.rows ? x[j][k] : -INFINITY;
+                now.top = fmaxf(now.top, x[j][k] * scale);
+            }
+            const float base = PartSum<float>::from(now.top);
+#pragma unroll
+            for (int k = 0; k < 4; k++) now.sum += expf(fmaf(x[j][k], scale, -base));
+            all[j].join(now);
+        }
+        if (split > 1) break;
+    }
+    __shared__ PartSum<float> of_warp[kFewWarps][kRows];
+#pragma unroll
+    for (int j = 0; j < kTiles; j++) {
+#pragma unroll
+        for (int d = 8; d < 32; d <<= 1) {
+            const PartSum<float> other{__shfl_xor_sync(kFullMask, all[j].top, d), __shfl_xor_sync(kFullMask, all[j].sum, d)};
+            all[j].join(other);
+        }
+        if (g == 0) of_warp[warp][j * 8 + t] = all[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < A.rows) {
+        PartSum<float> whole = of_warp[0][threadIdx.x];
+#pragma unroll 1
+        for (int w = 1; w < kFewWarps; w++) whole.join(of_warp[w][threadIdx.x]);
+        parts[static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x] = whole;
+    }
+}
+
+int few_row_values(int64_t depth) { return static_cast<int>(ceil_div(depth, 32) * 32); }
+
 FewOperand operand_of(const Array& a) {
     const unsigned char* begin = static_cast<const unsigned char*>(a.data);
     return {static_cast<const uint16_t*>(a.data), a.stride[0], a.shape[0], begin, begin + ((a.shape[0] - 1) * a.stride[0] + a.shape[1]) * 2};
@@ -185,18 +348,39 @@ int few_row_bytes(int64_t depth) {
 // (with more than 16 rows what is read from shared memory is the bound: 24 rows of 50 021 x 4096 138 us, 91 by the kernel of cross_entropy_mma.cu; 16 of them 90 and 90, 16 rows of 50 021 x 1024 23 and 26)
 bool few_loss_rows(const LossProblem& p) {
     const int64_t n = p.A.shape[0];
+    if (p.A.type == MOPS_B200_F32) return n <= 16 && p.A.shape[1] > 0 && p.A.shape[1] <= kMostFewBytes / 32 && ceil_div(n, 8) * 32 * few_row_values(p.A.shape[1]) <= kMostFewBytes;
     return n <= 16 && p.A.shape[1] <= kMostFewBytes / 16 && ceil_div(n, 8) * 8 * few_row_bytes(p.A.shape[1]) <= kMostFewBytes && p.W.stride[0] % 8 == 0 &&
            reinterpret_cast<uintptr_t>(p.W.data) % 16 == 0;
 }
 
-int64_t few_loss_parts(const Call& call, const LossProblem& p) { return std::min<int64_t>(ceil_div(p.W.shape[0], kUnitRows), sm_count(call.device)); }
-
-void loss_few_rows(const Call& call, const LossProblem& p, PartSum<float>* parts, float* at_target) {
-    const int bytes = few_row_bytes(p.A.shape[1]), tiles = static_cast<int>(ceil_div(p.A.shape[0], 8));
-    const unsigned blocks = static_cast<unsigned>(few_loss_parts(call, p));
-    const FewOperand A = operand_of(p.A), W = operand_of(p.W);
+static void launch_few(const Call& call, const LossProblem& p, unsigned blocks, PartSum<float>* parts, float* at_target) {
+    const int tiles = static_cast<int>(ceil_div(p.A.shape[0], 8));
     int split = 1; // (8 rows of 3000 x 4096: 14.0 us, 18.8 with a warp to a unit)
     while (split < kFewWarps && ceil_div(p.W.shape[0], kUnitRows) * 2 * split <= int64_t(blocks) * kFewWarps && p.A.shape[1] >= 2 * split * 4 * kFewDepth) split *= 2;
+    if (p.A.type == MOPS_B200_F32) {
+        const FewOperand32 A{static_cast<const float*>(p.A.data), p.A.stride[0], p.A.shape[0]}, W{static_cast<const float*>(p.W.data), p.W.stride[0], p.W.shape[0]};
+        const int values = few_row_values(p.A.shape[1]);
+        const size_t shared = (static_cast<size_t>(tiles * 8 * values) + (split > 1 ? static_cast<size_t>(tiles) * 4 * kFewThreads : 0)) * sizeof(float);
+        auto launch = [&](auto most, auto vector) {
+            auto kernel = loss_few32<decltype(most)::value, decltype(vector)::value>;
+            allow_dynamic_smem(reinterpret_cast<const void*>(kernel), call.device, shared);
+            kernel<<<blocks, kFewThreads, shared, call.stream>>>(parts, at_target, A, W, static_cast<int>(p.A.shape[1]), static_cast<const int32_t*>(p.targets.data),
+                                                                 static_cast<float>(p.scale), values, split);
+            note_kernel_f("loss_few<f32,%d,%d>", tiles, static_cast<int>(vector));
+        };
+        auto by_rows = [&](auto vector) {
+            if (tiles == 1) launch(std::integral_constant<int, 1>(), vector);
+            else launch(std::integral_constant<int, 2>(), vector);
+        };
+        const uintptr_t place = reinterpret_cast<uintptr_t>(W.data) | static_cast<uintptr_t>(W.stride * 4);
+        if (place % 16 == 0) by_rows(std::integral_constant<int, 4>());
+        else if (place % 8 == 0) by_rows(std::integral_constant<int, 2>());
+        else by_rows(std::integral_constant<int, 1>());
+        MOPS_CUDA_OK(cudaGetLastError());
+        return;
+    }
+    const int bytes = few_row_bytes(p.A.shape[1]);
+    const FewOperand A = operand_of(p.A), W = operand_of(p.W);
     auto launch = [&](auto type, auto most) {
         constexpr bool BF16 = decltype(type)::value;
         auto kernel = loss_few<BF16, decltype(most)::value>;
@@ -213,6 +397,15 @@ void loss_few_rows(const Call& call, const LossProblem& p, PartSum<float>* parts
     if (p.A.type == MOPS_B200_BF16) by_rows(std::true_type());
     else by_rows(std::false_type());
     MOPS_CUDA_OK(cudaGetLastError());
+}
+
+void loss_forward_few(const Call& call, const LossProblem& p, const Array& loss, const Array& log_sum) {
+    const int64_t n = p.A.shape[0], parts = std::min<int64_t>(ceil_div(p.W.shape[0], kUnitRows), sm_count(call.device)); // of a row: a block to each
+    Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<float>) + static_cast<size_t>(n) * sizeof(float));
+    PartSum<float>* sums = room.as<PartSum<float>>();
+    float* at_target = reinterpret_cast<float*>(sums + n * parts);
+    launch_few(call, p, static_cast<unsigned>(parts), sums, at_target);
+    join_rows<float>(call, loss, log_sum, sums, parts, at_target, LossRows{}, p.targets, p.W.shape[0], p.ignored);
 }
 
 } // namespace mops_b200

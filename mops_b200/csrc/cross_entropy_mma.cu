@@ -366,15 +366,7 @@ void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss,
     Packing packing(call);
     Array A = p.A, W = p.W;
     LossRows rows{};
-    if (few_loss_rows(p)) {
-        const int64_t parts = few_loss_parts(call, p);
-        Scratch room(call, static_cast<size_t>(n * parts) * sizeof(PartSum<float>) + static_cast<size_t>(n) * sizeof(float));
-        PartSum<float>* sums = room.as<PartSum<float>>();
-        float* at_target = reinterpret_cast<float*>(sums + n * parts);
-        loss_few_rows(call, p, sums, at_target);
-        join_rows<float>(call, loss, log_sum, sums, parts, at_target, rows, p.targets, vocabulary, p.ignored);
-        return;
-    }
+    if (few_loss_rows(p)) return loss_forward_few(call, p, loss, log_sum);
     const int32_t* targets = static_cast<const int32_t*>(p.targets.data);
     const bool gather = worth_gathering(A.type, n, vocabulary, p.A.shape[1]);
     if (gather) {

@@ -173,10 +173,9 @@ struct LossProblem {
     double scale;
     int64_t ignored;
 };
-// A few rows (cross_entropy_few.cu): whether they are, how many parts each has, and the sums of these (row by row) with x at the targets.
+// A few rows (cross_entropy_few.cu; not f64).
 bool few_loss_rows(const LossProblem& p);
-int64_t few_loss_parts(const Call& call, const LossProblem& p);
-void loss_few_rows(const Call& call, const LossProblem& p, PartSum<float>* parts, float* at_target);
+void loss_forward_few(const Call& call, const LossProblem& p, const Array& loss, const Array& log_sum);
 void loss_forward_mma(const Call& call, const LossProblem& p, const Array& loss, const Array& log_sum, const std::string& op);
 void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad_A, const Array& grad_W, const Array& grad_loss, const Array& grad_log_sum, const Array& loss,
                        const Array& log_sum, const std::string& op);
