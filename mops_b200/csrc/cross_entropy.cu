@@ -6,8 +6,8 @@
 //   grad_A = scale dx W, grad_W = scale dx^T A
 //
 // A piece of the vocabulary at a time: its logits are a product into scratch memory, of which sums are taken, or which become dx where they stand and are multiplied by the
-// piece's rows of W and, the other way, by A. The gradients compute the logits again. In f32 the logits of more than a few rows are worked on where they are summed (LossStore32, GradientStore32)
-// and never stored. Here: f32 and f64 (and f16 and bf16 without columns); f16 and bf16 are in cross_entropy_mma.cu.
+// piece's rows of W and, the other way, by A. The gradients compute the logits again. In f32 the logits are worked on where they are summed (LossStore32, GradientStore32) and
+// never stored, but for few tiles of much depth. Here: f32 and f64 (and f16 and bf16 without columns); f16 and bf16 are in cross_entropy_mma.cu, a few rows in cross_entropy_few.cu.
 #include "block_ops.hpp"
 #include "convert.cuh"
 #include "few_rows.cuh"
@@ -471,10 +471,7 @@ template <typename S> struct Pieces {
         width = width >= kPartColumns ? width / kPartColumns * kPartColumns : width / 256 * 256;
         part = std::min(width, kPartColumns);
         width = std::min(width, W.shape[0]);
-        // (15 rows of 30 029 x 96: 16.6 us, by the kernels for few rows and a pass over their logits 44; but those read W wherever its rows begin, which costs a copy here, and gradients take
-        // that copy in any case)
-        fused = kType == MOPS_B200_F32 && columns > 0 &&
-                (!forward || !straight_rows(matrices(0, W.shape[0]), n, false) || boxable(kType, W.data, columns, W.shape[0], 1, W.stride[0], 0));
+        fused = kType == MOPS_B200_F32 && columns > 0;
         in_parts = fused && worth_cutting(n, W.shape[0], columns);
         // (674 rows of 60 x 3040, 6 tiles: 31 us for 86, with gradients 97 for 219; 200 of 1000 x 4096, 16 tiles, 53 and 159 for 115 and 290. But 60 of 4000 x 2048, 32 tiles, 76 and 197 for 63 and 179, and
         // with less depth the host's part of three more launches is longer: 674 of 60 x 1024 43 for 37)
@@ -611,10 +608,10 @@ void loss_backward(const Call& call, const Array& grad_A, const Array& grad_W, c
         m.shape[1] = v1 - v0, m.shape[2] = columns; // (v1 - v0) x C
         std::swap(m.stride[1], m.stride[2]);
         Packing packing(call);
-        if (pieces.kType == MOPS_B200_F32) {
-            const bool rows_packed = need_A && (pieces.fused || !straight_rows(m, n, true)), outer_packed = need_W && !straight_outer(n, 1, v1 - v0, columns, pieces.kType);
-            if (rows_packed || outer_packed) packing.add(dx);
-            if (rows_packed) packing.add(m);
+        if (pieces.fused) {
+            const bool outer_packed = need_W && !straight_outer(n, 1, v1 - v0, columns, pieces.kType);
+            if (need_A || outer_packed) packing.add(dx);
+            if (need_A) packing.add(m);
             if (outer_packed) packing.add(a);
             packing.run();
         }

@@ -582,7 +582,7 @@ def test_loss_on_strided_and_shifted_tensors(dtype, R):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("R,V,C,stride", [
     (1, 1, 8, 8), (1, 7, 8, 8), (3, 15, 24, 40), (8, 16, 32, 32), (9, 17, 37, 40), (16, 2400, 40, 40), (17, 2400, 40, 40), (8, 100, 1000, 1000), (7, 3001, 2064, 2064),
-    (16, 50021, 64, 64), (5, 40000, 255, 256), (6, 900, 37, 37), (12, 5000, 146, 146), (16, 130, 2050, 2050), (16, 300, 3200, 3200)])
+    (16, 50021, 64, 64), (5, 40000, 255, 256), (6, 900, 37, 37), (12, 5000, 146, 146), (16, 130, 2050, 2050), (16, 300, 3200, 3200), (3, 200, 6500, 6501)])
 def test_loss_of_few_rows(dtype, R, V, C, stride):
     table = normal((V, stride), dtype, 2, C ** -0.5)
     table[:, C:] = float("nan")
