@@ -177,7 +177,8 @@ template <bool BF16, int kColumns, bool kTwoParts> struct GradientStore {
 };
 
 // Sums in f32: of the first piece of the vocabulary they are written, those of others are added to what is there. Each slice of the depth has sums of its own, so that no two
-// blocks add to one place, and the order of the additions is that of the pieces.
+// blocks add to one place, and the order of the additions is that of the pieces. The last piece may have fewer stages than there are slices: a slice without any has summed nothing, and its accumulator has what
+// another tile left there.
 template <int kColumns> struct SumStore {
     static constexpr bool kHalves = false, kAllRows = false;
     static constexpr int kStoreWarps = 8, kStaging = 32 * kBoxRow, kOwn = kColumns / 2;
@@ -193,9 +194,13 @@ template <int kColumns> struct SumStore {
     int lane;
     int64_t row = 0;
     int here = 0, column = 0, slice = 0;
+    bool empty = false;
     __device__ SumStore(const Args& a, uint32_t staging, int lane) : a(a), staging(staging), lane(lane) {}
-    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) { row = r, here = h, column = piece.column, slice = piece.row; }
+    __device__ __forceinline__ void begin(const Piece& piece, int64_t r, int h, int) {
+        row = r, here = h, column = piece.column, slice = piece.row, empty = piece.steps == 0;
+    }
     __device__ __forceinline__ void store(uint32_t accumulator, int part) {
+        if (empty && a.add) return;
 #pragma unroll 1
         for (int c = part * kOwn; c < part * kOwn + kOwn; c += 32) {
             if (column + c >= a.columns) return;
@@ -203,6 +208,10 @@ template <int kColumns> struct SumStore {
             tmem_load(accumulator + c, r);
             tmem_wait_load();
             tmem_pin(r);
+            if (empty) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) r[j] = 0;
+            }
             if (here == 32) {
                 if (lane == 0) boxes_left<0>();
                 __syncwarp();

@@ -9,7 +9,8 @@
 //   E(args, staging, lane)                            what a storing warp keeps
 //   begin(piece, row, here, part)                     before the accumulator is there: what can be loaded (of rows of no group nothing: piece.group < 0). The warp's first row, how many it
 //                                                     has, and its part of the columns
-//   store(accumulator, part)                          the warp's part of the columns (0 of 1, or of 2)
+//   store(accumulator, part)                          the warp's part of the columns (0 of 1, or of 2). A slice of the depth may have no stages (piece.steps == 0): then nothing has been summed, and the
+//                                                     accumulator has what stood there before
 //   clear()                                           rows of no group
 //   end()                                             before the block leaves
 #ifndef MOPS_B200_TILE_ROWS_CUH
@@ -186,7 +187,7 @@ template <int kRows, int kColumns> struct DecodeTable {
     }
 };
 
-// Tiles of groups' rows, each with the depth cut into slices of `slice_steps` stages: a piece's first stage is in p.slot, its slice in p.row.
+// Tiles of groups' rows, each with the depth cut into slices of `slice_steps` stages (the last ones may have fewer, or none): a piece's first stage is in p.slot, its slice in p.row.
 template <int kRows, int kColumns> struct DecodeRowSlices {
     DecodeRows<kRows, kColumns> rows;
     int slices, slice_steps, all_steps;
@@ -371,7 +372,7 @@ inline int64_t best_slices(int64_t tiles, int64_t workers, int64_t steps, double
         const double time = static_cast<double>(ceil_div(tiles * ceil_div(steps, per), workers)) * (per * microseconds + 1.0) + s * bytes / 4e6;
         if (time < shortest) shortest = time, best = s;
     }
-    return ceil_div(steps, ceil_div(steps, best)); // (none without steps: all have sums)
+    return ceil_div(steps, ceil_div(steps, best)); // (none without steps, of so many; where a product of fewer is cut into as many slices, the last ones may have none)
 }
 
 // What a launch takes from its problem; `columns`: of the result.
