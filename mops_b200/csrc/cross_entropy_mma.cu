@@ -428,7 +428,8 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     float* factor = reinterpret_cast<float*>(factors + n);
     const float scale2 = static_cast<float>(p.scale * 1.4426950408889634);
     const bool twice = n <= kTwoPartsTo;
-    const int64_t copies = twice ? 2 : 1, all = copies * n, whole = ceil_div(n, 2 * kTileRows) * 2 * kTileRows; // rows of dx, and rows up to the end of a tile
+    const int64_t copies = twice ? 2 : 1, all = copies * n; // rows of dx
+    const int64_t height = n <= kTileRows ? kTileRows : 2 * kTileRows, whole = ceil_div(n, height) * height; // of a tile, and rows up to the end of one
     const int32_t* all_rows = twice ? rows.doubled : rows.offsets;
     const Array A = gathered(call, room_A, p.A, rows, twice,
                              {factors, factor, of_loss, of_sum, static_cast<const float*>(loss.data), static_cast<const float*>(log_sum.data), static_cast<float>(p.scale),
@@ -441,8 +442,8 @@ void loss_backward_mma(const Call& call, const LossProblem& p, const Array& grad
     packing.run();
     // Pieces of the vocabulary: as wide as there is room for dx, by steps whose tiles of grad_W are whole rounds of pairs (8192 rows of 100 003 x 1024: seven equal pieces, whose last rounds were a twelfth
     // full, took 1666 us for grad_W, some 1300 in these).
-    constexpr int64_t kMostValues = int64_t(1) << 28; // of dx
-    const int64_t most = std::max<int64_t>(kMostValues / all / 256 * 256, 256), across = ceil_div(columns, 256), unit = sms / 2 / std::gcd<int64_t>(sms / 2, across) * 256;
+    constexpr int64_t kMostValues = int64_t(1) << 28; // of dx, with those behind the last row
+    const int64_t most = std::max<int64_t>(kMostValues / (copies * whole) / 256 * 256, 256), across = ceil_div(columns, 256), unit = sms / 2 / std::gcd<int64_t>(sms / 2, across) * 256;
     const int64_t width = std::min(unit <= most ? most / unit * unit : most, whole_packs(vocabulary)), pieces = ceil_div(vocabulary, width);
     Scratch room_dx(call, static_cast<size_t>(copies * whole * width) * 2);
     // Slices of the piece for the products with W.

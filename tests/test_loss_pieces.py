@@ -2,10 +2,14 @@
 depth of its products is cut as that of the others is. Against a plain implementation in 64 bits, some rows at a time; tolerances as in
 test_training_ops.py, with the sums over all rows counted as such.
 """
+import ctypes
+
 import pytest
 import torch
 
+import mops_b200
 import mops_b200.torch as mt
+from mops_b200 import _lib
 
 from test_training_ops import inner_round, normal, some_targets, unit, within
 
@@ -88,3 +92,26 @@ def test_gradients_whose_last_piece_has_fewer_stages_than_slices(dtype, R, V, C)
     (torch.float32, 2100, 40000, 128), (torch.float32, 2100, 28673, 130)])
 def test_gradients_of_several_pieces(dtype, R, V, C):
     check_pieces(dtype, R, V, C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("R,V,pieces", [(1, 2200000, 3), (128, 1100003, 2), (129, 1100003, 3), (256, 1100003, 3), (300, 1100003, 3)])
+def test_gradients_of_few_rows_of_a_very_large_table(dtype, R, V, pieces):
+    """dx has room up to the end of a tile, for two parts of up to 256 rows each: half a GB at the most, however few the rows are."""
+    A, W, targets = normal((R, 8), dtype, 1, 2.0), normal((V, 8), dtype, 2, 0.35), some_targets(R, V, 1.0)
+    targets[R // 2] = V - 1
+    loss, log_sum = mops_b200.linear_cross_entropy(A, W, targets)
+    grads = [normal((R,), torch.float32, 9 + i) for i in range(2)]
+    got_A, got_W = torch.empty_like(A), torch.empty_like(W)
+    arrays = [_lib.make_array(t.data_ptr(), str(t.dtype).split(".")[1], tuple(t.shape), t.stride())
+              for t in (got_A, got_W, *grads, loss, log_sum, A, W, targets)]
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    _lib.call("mops_b200_cuda_linear_cross_entropy_vjp", arrays + [ctypes.c_double(1.0), ctypes.c_int64(-1)])
+    torch.cuda.synchronize()
+    assert any(f", {pieces} pieces" in k for k in _lib.last_kernels()), _lib.last_kernels()
+    assert before - torch.cuda.mem_get_info()[0] < 640 << 20
+    values, errors = plain_in_blocks(A, W, targets, 1.0, *grads)
+    for g, w, e, what in zip((loss, log_sum, got_A, got_W), values, errors, ("loss", "log_sum", "grad_A", "grad_W")):
+        within(g, w, e, what)
