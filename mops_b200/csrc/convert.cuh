@@ -43,6 +43,7 @@ template <typename To> Array converted(const Call& call, const Array& a, To* to,
     const int64_t slices = a.dimensions == 3 ? a.shape[0] : 1;
     r.stride[inner] = 1, r.stride[outer] = a.shape[inner];
     if (a.dimensions == 3) r.stride[0] = a.shape[inner] * a.shape[outer];
+    if (inner != last && a.shape[inner] == 1) r.stride[inner] = a.shape[outer]; // (columns of one value are rows of the copy: one stride of 1 alone says which way round it is)
     if (slices * a.shape[outer] * a.shape[inner] > 0)
         for_type(a.type, [&](auto zero) {
             using From = decltype(zero);
