@@ -234,8 +234,8 @@ MOPS_EXPORT int mops_b200_cuda_sort_index(mops_tensor_1d_i32_t sorted,
  *
  * Arrays are views with a type and strides (counted in values), of f32, f64, f16 or bf16; all
  * floating-point arrays of a call have one type. Inputs may have rows that lie apart (any stride but
- * the last, which is 1); outputs are contiguous. Sums are held in 32 bits (f64: 64) and rounded
- * once. A gradient output with data == NULL is skipped. Same status convention, stream and completion rules as the
+ * the last, which is 1); outputs are contiguous. Sums are held in 32 bits (f64: 64) and results rounded
+ * once; what goes from one product into another in 16 bits is said where that is. A gradient output with data == NULL is skipped. Same status convention, stream and completion rules as the
  * mops_cuda_* entry points. */
 enum {
     MOPS_B200_F32 = 0,
@@ -291,7 +291,8 @@ MOPS_EXPORT int mops_b200_cuda_gated_residual_norm_vjp(
 /* The gated feed-forward layer of groups: W[g] holds the N columns of the gate, then those of the values (K x 2N), and
  * output[r,j] = f(A[r,:] W[g,:,j]) * (A[r,:] W[g,:,N+j]) for the rows offsets[g] <= r < offsets[g+1] of group g; zeros for
  * rows of no group. f is one of MOPS_B200_SILU (u sigmoid(u)) and MOPS_B200_GELU (u Phi(u), by the error function). Offsets and
- * the ways W and grad_W may be stored: as of the grouped product. */
+ * the ways W and grad_W may be stored: as of the grouped product. In f16 and bf16 the gradients of the two products, of which grad_A and grad_W
+ * are made, are rounded to that type (and infinite beyond its range), but for up to 2048 of them (rows x 2N). */
 enum { MOPS_B200_SILU = 0, MOPS_B200_GELU = 1 };
 MOPS_EXPORT int mops_b200_cuda_grouped_gated_product(mops_b200_array_t output, mops_b200_array_t A,
                                                      mops_b200_array_t W, mops_b200_array_t offsets,
@@ -308,7 +309,9 @@ MOPS_EXPORT int mops_b200_cuda_grouped_gated_product_vjp(mops_b200_array_t grad_
 MOPS_EXPORT int mops_b200_cuda_linear_cross_entropy(mops_b200_array_t loss, mops_b200_array_t log_sum,
                                                     mops_b200_array_t A, mops_b200_array_t W,
                                                     mops_b200_array_t targets, double scale, int64_t ignore_index);
-/* Gradients for those of loss and log_sum (an array of 0 dimensions: zeros); loss and log_sum are the forward call's. */
+/* Gradients for those of loss and log_sum (an array of 0 dimensions: zeros); loss and log_sum are the forward call's. In f16 and bf16 the
+ * gradients of the logits, of which both are made, are rounded to that type, in units of the largest gradient of a loss (those of up to 256 rows
+ * have two parts of 16 bits each). */
 MOPS_EXPORT int mops_b200_cuda_linear_cross_entropy_vjp(
     mops_b200_array_t grad_A, mops_b200_array_t grad_W, mops_b200_array_t grad_loss, mops_b200_array_t grad_log_sum,
     mops_b200_array_t loss, mops_b200_array_t log_sum, mops_b200_array_t A, mops_b200_array_t W,

@@ -4,8 +4,8 @@
 // the SM: f32 to the end, rounded once. The backward pass computes U and V again (a third more of its products; kept in 16 bits, their rounding would add to that of dU and dV), writes dU and dV side by
 // side and leaves the rest to the grouped products.
 //
-// Bound by the tensor cores, at the clock that the power limit leaves: 16 384 rows of 8 groups, 2048 x 2 x 2048 in bf16, 199 us (1.38 PFLOP/s), dU and dV 216; 8192 rows of 16 groups, 2048 x 2 x 1280,
-// 80 us (1.07), by blocks that fetch their operands for themselves, in five rounds of tiles that are 4.9 full. Few rows by memory: 16 of 12 groups, 2048 x 2 x 1024 (101 MB), 20 us.
+// Bound by the tensor cores: 16 384 rows of 8 groups, 2048 x 2 x 2048 in bf16, 207 us (1.33 PFLOP/s), dU and dV 220, at 1965 MHz, which the GPU holds for some milliseconds; in steps without a pause 245 and 256, at
+// the 1455 MHz that the power limit leaves. 8192 rows of 16 groups, 2048 x 2 x 1280, 82 us (1.05), by blocks that fetch their operands for themselves, in five rounds of tiles that are 4.9 full. Few rows by memory: 16 of 12 groups, 2048 x 2 x 1024 (101 MB), 20 us.
 #include "activation.cuh"
 #include "few_rows.cuh"
 #include "gated_mma.hpp"
